@@ -108,6 +108,47 @@ hipError_t dispatch(int dtype, int head_dim, bool causal, F&& f) {
 #undef FHOG_CASE
 }
 
+// Calls f.template operator()<T, D>() for the runtime (dtype, head_dim).
+template <typename F> hipError_t dispatch(int dtype, int head_dim, F&& f) {
+  return dispatch(dtype, head_dim, false, [&]<typename T, int D, bool C>() { return f.template operator()<T, D>(); });
+}
+
+// A window of keys and sinks, as the kernels take them: both cut to what the sizes can show.
+struct Window {
+  int window, sinks;
+  fhog::SinkGrid sink;
+};
+
+int check_window(const Shape& s, int window, int sinks, Window* w, const char* who) {
+  if (int st = check_shape(s, who)) return st;
+  if (s.causal == FHOG_CAUSAL_NONE)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: a window needs causal 1 (top-left) or 2 (bottom-right)", who);
+  if (window < 1) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: window must be >= 1, got %d", who, window);
+  if (sinks < 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sinks must be >= 0, got %d", who, sinks);
+  const int most = s.n_q > s.n_k ? s.n_q : s.n_k;
+  if (most > (1 << 30)) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  w->window = window < most ? window : most;  // positions are below `most`
+  w->sinks = sinks < s.n_k ? sinks : s.n_k;
+  const fhog::Mask m{true, s.n_q, s.n_k, s.coff()};
+  w->sink = fhog::SinkGrid{(w->sinks + 63) / 64, fhog::sink_chunks(m, w->window, w->sinks),
+                           fhog::sink_step(w->window, w->sinks)};
+  const long long groups = ((s.n_k + 63) / 64 + (long long)w->sink.blocks * w->sink.chunks) * s.batch * s.kv_heads;
+  if (groups >= (1ll << 31)) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  return FHOG_OK;
+}
+
+size_t sink_parts_bytes(const Shape& s, const Window& w) {
+  if (w.sink.chunks == 0) return 0;
+  return (size_t)(1 + w.sink.chunks) * s.batch * s.kv_heads * w.sinks * 2 * s.head_dim * sizeof(float);
+}
+
+// The workspace of a call that has sinks to join.
+int check_workspace(const char* who, const Window& w, const void* workspace) {
+  if (w.sink.chunks > 0 && !aligned(workspace, 16))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null or not 16-byte aligned", who);
+  return FHOG_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -302,6 +343,79 @@ int fhog_attention_bwdbwd_noalloc(fhog_stream_t stream, const void* q, const voi
   return bwdbwd_impl(who, 3, stream, q, k, v, o, dout, ddq, ddk, ddv, lse, dq2, dk2, dv2, ddo, ws,
                      ws + kScratchRows, ws + 2 * kScratchRows, batch, n_q, n_k, heads, kv_heads, head_dim, dtype,
                      causal, scale);
+}
+
+size_t fhog_window_workspace_bytes(int batch, int n_q, int n_k, int kv_heads, int head_dim, int causal, int window,
+                                   int sinks) {
+  const Shape s{batch, n_q, n_k, kv_heads, kv_heads, head_dim, FHOG_DTYPE_BF16, causal, 1.0f};
+  Window w;
+  if (check_window(s, window, sinks, &w, "fhog_window_workspace_bytes")) return 0;
+  return sink_parts_bytes(s, w);
+}
+
+int fhog_window_attention_fwd(fhog_stream_t stream, const void* q, const void* k, const void* v, void* o, float* lse,
+                              int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim, int dtype,
+                              int causal, int window, int sinks, float scale) {
+  static const char* who = "fhog_window_attention_fwd";
+  const Shape s{batch, n_q, n_k, heads, kv_heads, head_dim, dtype, causal, scale};
+  Window w;
+  if (int st = check_window(s, window, sinks, &w, who)) return st;
+  if (int st = check_ptrs(who, {{"q", q}, {"k", k}, {"v", v}, {"o", o}}, {{"lse", lse}})) return st;
+  auto run = [&]<typename T, int D>() {
+    fhog::FwdParams<T> p{(const T*)q, (const T*)k, (const T*)v, (T*)o,    lse,   batch,    n_q,
+                         n_k,         heads,       kv_heads,    s.coff(), scale, w.window, w.sinks};
+    return fhog::launch_fwd<T, D, fhog::kWindow>(p, (hipStream_t)stream);
+  };
+  return launch_status(dispatch(dtype, head_dim, run), who);
+}
+
+int fhog_window_attention_bwd(fhog_stream_t stream, const void* q, const void* k, const void* v, const void* o,
+                              const void* dout, const float* lse, void* dq, void* dk, void* dv, float* delta,
+                              void* workspace, int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim,
+                              int dtype, int causal, int window, int sinks, float scale) {
+  static const char* who = "fhog_window_attention_bwd";
+  const Shape s{batch, n_q, n_k, heads, kv_heads, head_dim, dtype, causal, scale};
+  Window w;
+  if (int st = check_window(s, window, sinks, &w, who)) return st;
+  if (int st = check_ptrs(who, {{"q", q}, {"k", k}, {"v", v}, {"o", o}, {"dout", dout}, {"dq", dq}, {"dk", dk},
+                                {"dv", dv}},
+                           {{"lse", lse}, {"delta", delta}}))
+    return st;
+  if (int st = check_workspace(who, w, workspace)) return st;
+  auto run = [&]<typename T, int D>() {
+    fhog::BwdParams<T> p{(const T*)q, (const T*)k, (const T*)v, (const T*)o, (const T*)dout, lse,
+                         (T*)dq, (T*)dk, (T*)dv, delta, batch, n_q, n_k, heads, kv_heads, s.coff(), scale,
+                         w.window, w.sinks, w.sink, (float*)workspace};
+    return fhog::launch_window_bwd<T, D>(p, (hipStream_t)stream);
+  };
+  return launch_status(dispatch(dtype, head_dim, run), who);
+}
+
+int fhog_window_attention_bwdbwd(fhog_stream_t stream, const void* q, const void* k, const void* v, const void* o,
+                                 const void* dout, const void* ddq, const void* ddk, const void* ddv,
+                                 const float* lse, void* dq2, void* dk2, void* dv2, void* ddo, float* delta,
+                                 float* ddelta, float* bstat, void* workspace, int batch, int n_q, int n_k, int heads,
+                                 int kv_heads, int head_dim, int dtype, int causal, int window, int sinks,
+                                 float scale) {
+  static const char* who = "fhog_window_attention_bwdbwd";
+  const Shape s{batch, n_q, n_k, heads, kv_heads, head_dim, dtype, causal, scale};
+  Window w;
+  if (int st = check_window(s, window, sinks, &w, who)) return st;
+  if (int st = check_ptrs(who, {{"q", q}, {"k", k}, {"v", v}, {"o", o}, {"dout", dout}, {"ddq", ddq}, {"ddk", ddk},
+                                {"ddv", ddv}, {"dq2", dq2}, {"dk2", dk2}, {"dv2", dv2}, {"ddo", ddo}},
+                           {{"lse", lse}, {"delta", delta}, {"ddelta", ddelta}, {"bstat", bstat}}))
+    return st;
+  if (int st = check_workspace(who, w, workspace)) return st;
+  auto run = [&]<typename T, int D>() {
+    fhog::BwdBwdParams<T> p{(const T*)q,   (const T*)k,   (const T*)v,   (const T*)o, (const T*)dout,
+                            (const T*)ddq, (const T*)ddk, (const T*)ddv, lse,         (T*)dq2,
+                            (T*)dk2,       (T*)dv2,       (T*)ddo,       delta,       ddelta,
+                            bstat,         batch,         n_q,           n_k,         heads,
+                            kv_heads,      s.coff(),      scale,         w.window,    w.sinks,
+                            w.sink,        (float*)workspace};
+    return fhog::launch_window_bwdbwd<T, D>(p, (hipStream_t)stream);
+  };
+  return launch_status(dispatch(dtype, head_dim, run), who);
 }
 
 }  // extern "C"

@@ -49,10 +49,11 @@ constexpr int kPairs = 2;  // four pairs (128 keys) per workgroup: 4-10 % slower
 constexpr int kWaves = 2 * kPairs;
 constexpr int kThreads = 64 * kWaves;
 
-template <typename T, int D, bool CAUSAL, int OCC>
+template <typename T, int D, int MASK, int OCC>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
@@ -81,8 +82,19 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
   const GridSlot gs = grid_slot(blockIdx.x, nbh, nkb, chunk);
   // causal: the longest key columns come first, up to rank `fold`; the ranks
   // from there on run backwards (fold_rank)
-  const int kb = folded(gs.rank, nkb, fold);
-  const int bh = gs.pair;
+  int bkb = folded(gs.rank, nkb, fold), bbh = gs.pair, bpart = 0;
+  if constexpr (MASK == kWindow) {
+    const int extra = (int)blockIdx.x - nkb * nbh;  // workgroups of sinks' further queries (SinkGrid)
+    if (extra >= 0) {
+      const int c = extra / nbh;
+      bbh = extra - c * nbh;
+      bpart = 1 + c / p.sink.blocks;
+      bkb = c % p.sink.blocks;
+    }
+  }
+  const int kb = bkb, bh = bbh;
+  [[maybe_unused]] const int part = bpart;
+  const QueryBounds<MASK> qs(p, kb, BKB, part, p.sink.step);
   const int b = bh / p.kv_heads, hk = bh % p.kv_heads;
   const int grp = p.heads / p.kv_heads;  // query heads per key/value head
   const long rs = (long)p.heads * D;      // query-side row stride
@@ -98,8 +110,8 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
 
   // Iteration i visits query tile qt_begin + i / grp of query head
   // hk * grp + i % grp: the heads of a group share each tile's causal bounds.
-  const int nqt = (p.nq + BQ - 1) / BQ;
-  const int qt_begin = CAUSAL ? max(0, kb * BKB - p.coff) / BQ : 0;
+  const int nqt = (qs.q_end + BQ - 1) / BQ;
+  const int qt_begin = qs.q_begin / BQ;
   const int total = nqt > qt_begin ? (nqt - qt_begin) * grp : 0;
 
   f32x16 acc[DT];  // A: dV, B: dK
@@ -187,7 +199,7 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
           advance(nxt);
         }
         const int q0 = (qt_begin + cur.qt) * BQ;
-        const bool active = k0 < p.nk && (!CAUSAL || q0 + BQ - 1 >= k0 - p.coff);
+        const bool active = k0 < p.nk && qs.active(q0, k0);
         const uint32_t slot = ((uint32_t)i % NST) * kStage;
         const uint32_t sa = lds0 + slot;  // Q at 0, dO at kTile
         float* xp = reinterpret_cast<float*>(s_p + pair * kExch) + 4 * lane;
@@ -208,9 +220,9 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
           if (role == 0) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) C[r] = exp2_fast(C[r] * c2);
-            if ((q0 + BQ > p.nq) || (CAUSAL && q0 < k0 + 31 - p.coff)) {
-              // visible iff query >= key - coff (causal) and query < nq
-              const int qlo = (CAUSAL ? kj - p.coff : 0) - q0, qhi = p.nq - q0;
+            if (qs.masked(q0, k0)) {
+              // visible iff query >= key - coff (causal) and query < nq, or the window's bounds
+              const int qlo = qs.lo(kj) - q0, qhi = qs.hi(kj) - q0;
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const int m = crow(r, g);
@@ -256,6 +268,21 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
     }
   }
 
+  if constexpr (MASK == kWindow) {
+    if (kvalid && kj < p.sinks && p.sink.chunks > 0) {
+      const long row = ((long)part * nbh + bh) * min(p.sinks, p.nk) + kj;
+      float* dst = p.sink_parts + (2 * row + wave_role) * D;
+      const float f = wave_role ? p.scale : 1.0f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * a + 4 * g) = f32x4{acc[dt][4 * a] * f, acc[dt][4 * a + 1] * f,
+                                                                           acc[dt][4 * a + 2] * f, acc[dt][4 * a + 3] * f};
+      return;
+    }
+    if (part > 0) return;  // keys of the block that are no sinks
+  }
   if (kvalid) {
     T* dst = (wave_role ? p.dk : p.dv) + kbase + (long)kj * rsk;
     const float f = wave_role ? scale : 1.0f;
@@ -272,31 +299,31 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
   }
 }
 
-template <typename T, int D, bool CAUSAL, int OCC>
+template <typename T, int D, int MASK, int OCC>
 hipError_t launch_occ(const BwdParams<T>& p, int nkb, int npairs, int cus, hipStream_t stream) {
-  hipLaunchKernelGGL((bwd_pair_kernel<T, D, CAUSAL, OCC>), dim3(nkb * npairs), dim3(kThreads), 0, stream, p,
-                     grid_chunk(npairs, nkb, OCC * cus), fold_rank(CAUSAL, nkb, npairs, cus));
+  hipLaunchKernelGGL((bwd_pair_kernel<T, D, MASK, OCC>), dim3(key_grid<MASK>(p, 32 * kPairs)), dim3(kThreads), 0, stream, p,
+                     grid_chunk(npairs, nkb, OCC * cus), fold_rank(MASK == 1, nkb, npairs, cus));
   return hipGetLastError();
 }
 
 }  // namespace
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwd_pair(const BwdParams<T>& p, hipStream_t stream) {
   const int nkb = (p.nk + 32 * kPairs - 1) / (32 * kPairs);
   const int npairs = p.batch * p.kv_heads;
   const int cus = resident_workgroups(1);
-  [[maybe_unused]] const int waves = bwd_pair_waves(mask_of(CAUSAL, p), npairs, D, (int)sizeof(T), cus);
+  [[maybe_unused]] const int waves = bwd_pair_waves(mask_of(MASK != 0, p), npairs, D, (int)sizeof(T), cus);
   if constexpr (sizeof(T) == 4 && D == 64) {
-    return launch_occ<T, D, CAUSAL, 3>(p, nkb, npairs, cus, stream);
+    return launch_occ<T, D, MASK, 3>(p, nkb, npairs, cus, stream);
   } else {
     if constexpr (sizeof(T) == 2 && D == 128) {
-      if (waves == 3) return launch_occ<T, D, CAUSAL, 3>(p, nkb, npairs, cus, stream);
+      if (waves == 3) return launch_occ<T, D, MASK, 3>(p, nkb, npairs, cus, stream);
     }
     if constexpr (sizeof(T) == 2 && D == 64) {
-      if (waves == 4) return launch_occ<T, D, CAUSAL, 4>(p, nkb, npairs, cus, stream);
+      if (waves == 4) return launch_occ<T, D, MASK, 4>(p, nkb, npairs, cus, stream);
     }
-    return launch_occ<T, D, CAUSAL, 2>(p, nkb, npairs, cus, stream);
+    return launch_occ<T, D, MASK, 2>(p, nkb, npairs, cus, stream);
   }
 }
 

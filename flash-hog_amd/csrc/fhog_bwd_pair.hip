@@ -15,6 +15,11 @@ FHOG_INST(_Float16, 128, true)
 FHOG_INST(_Float16, 128, false)
 FHOG_INST(float, 64, true)
 FHOG_INST(float, 64, false)
+FHOG_INST(__bf16, 64, kWindow)
+FHOG_INST(__bf16, 128, kWindow)
+FHOG_INST(_Float16, 64, kWindow)
+FHOG_INST(_Float16, 128, kWindow)
+FHOG_INST(float, 64, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

@@ -13,6 +13,9 @@ FHOG_INST(_Float16, 256, true)
 FHOG_INST(_Float16, 256, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
+FHOG_INST(__bf16, 256, kWindow)
+FHOG_INST(_Float16, 256, kWindow)
+FHOG_INST(float, 128, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

@@ -36,10 +36,11 @@ constexpr int kThreads = 64 * kWaves;
 // three or four (a bound of two: 430 -> 481 us for the first backward at B128 N512
 // H12 D64 causal).
 constexpr int kOcc = 2;
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kOcc, 8)))
 bwd_qpair_kernel(BwdParams<T> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;
   constexpr int DT = D / 64;  // 32-column blocks of dQ per wave
@@ -77,14 +78,11 @@ bwd_qpair_kernel(BwdParams<T> p, int chunk, int fold) {
   const int qi = q0 + n;
   const bool qvalid = qi < p.nq;
 
-  // Keys [0, kend) are visible to some query of the workgroup, [0, wend) to
-  // some query of this pair.
-  int kend = p.nk;
-  if (CAUSAL) kend = min(kend, qb * BQ + BQ + p.coff);
-  const int nkt = __builtin_amdgcn_readfirstlane(kend > 0 ? (kend + BK - 1) / BK : 0);
-  int wend = p.nk;
-  if (CAUSAL) wend = max(0, min(wend, q0 + 32 + p.coff));
-  const int wkt = q0 < p.nq ? (wend + BK - 1) / BK : 0;
+  // The tiles that hold keys visible to some query of the workgroup, and to some
+  // query of this pair.
+  const KeyTiles<MASK> tiles(p, qb * BQ, BQ);
+  const int nkt = tiles.count;
+  const KeyBounds<MASK> sees(p, q0, 32);
 
   SwzFrags<T, D> fr;
   fr.init(lane);
@@ -94,9 +92,10 @@ bwd_qpair_kernel(BwdParams<T> p, int chunk, int fold) {
   TileDma<T, D, kPer> dma;
   dma.init(row_bytes, BK, lane, kPer * pair);
   const uint32_t lds0 = lds_base_u32(s_kv);
-  auto issue = [&](int kt) {
+  auto issue = [&](int it) {
+    const int kt = tiles.tile(it);
     const int nvalid = p.nk - kt * BK;
-    const uint32_t dst = lds0 + tensor * kTile + (uint32_t)(((uint32_t)kt % NST) * kStage);
+    const uint32_t dst = lds0 + tensor * kTile + (uint32_t)(((uint32_t)it % NST) * kStage);
     const T* gsrc = src + (long)kt * BK * rsk;
     if (nvalid >= BK) {
       dma.issue(dst, gsrc);
@@ -142,14 +141,15 @@ bwd_qpair_kernel(BwdParams<T> p, int chunk, int fold) {
     for (int i = 0; i < NST - 1; ++i)
       if (i < nkt) issue(i);
 
-    // After its first barrier of iteration kt every wave is done with tile
-    // kt - 1, whose stage tile kt + 1 takes, and with the exchange buffer.
-    for (int kt = 0; kt < nkt; ++kt) {
-      wait_tile<NST, kPer>(kt, nkt);
+    // After its first barrier of iteration `it` every wave is done with tile
+    // it - 1, whose stage tile it + 1 takes, and with the exchange buffer.
+    for (int it = 0; it < nkt; ++it) {
+      wait_tile<NST, kPer>(it, nkt);
       __syncthreads();
-      if (kt + NST - 1 < nkt) issue(kt + NST - 1);
-      const bool active = kt < wkt;
-      const uint32_t sa = lds0 + (uint32_t)(((uint32_t)kt % NST) * kStage);  // K at 0, V at kTile
+      if (it + NST - 1 < nkt) issue(it + NST - 1);
+      const int kt = tiles.tile(it);
+      const bool active = sees.active(kt);
+      const uint32_t sa = lds0 + (uint32_t)(((uint32_t)it % NST) * kStage);  // K at 0, V at kTile
       float* xp = reinterpret_cast<float*>(s_x + pair * 2 * kExch) + 4 * lane;  // P, then u
       f32x16 C;
       if (active) {
@@ -162,11 +162,12 @@ bwd_qpair_kernel(BwdParams<T> p, int chunk, int fold) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) C[r] = exp2_fast(fmaf(C[r], c2, nL2));
           const int k0 = kt * BK;
-          if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff)) {
+          if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff) || sees.below(k0)) {
             const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - k0;  // last visible key, tile-relative
+            const int klow = qi + p.coff - p.window + 1 - k0;                       // first one of the window
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              if (crow(r, g) > klim) C[r] = 0.f;
+              if (crow(r, g) > klim || outside<MASK>(crow(r, g), klow, p.sinks - k0)) C[r] = 0.f;
           }
         } else if constexpr (!kU0) {
 #pragma unroll
@@ -218,13 +219,13 @@ bwd_qpair_kernel(BwdParams<T> p, int chunk, int fold) {
 
 }  // namespace
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwd_qpair(const BwdParams<T>& p, hipStream_t stream) {
   const int nqb = (p.nq + 32 * kPairs - 1) / (32 * kPairs);
   const int npairs = p.batch * p.heads;
   const int cus = resident_workgroups(1);
-  hipLaunchKernelGGL((bwd_qpair_kernel<T, D, CAUSAL>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
-                     grid_chunk(npairs, nqb, kOcc * cus), fold_rank(CAUSAL, nqb, npairs, cus));
+  hipLaunchKernelGGL((bwd_qpair_kernel<T, D, MASK>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
+                     grid_chunk(npairs, nqb, kOcc * cus), fold_rank(MASK == 1, nqb, npairs, cus));
   return hipGetLastError();
 }
 
@@ -245,6 +246,14 @@ FHOG_INST(float, 64, true)
 FHOG_INST(float, 64, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
+FHOG_INST(__bf16, 64, kWindow)
+FHOG_INST(__bf16, 128, kWindow)
+FHOG_INST(__bf16, 256, kWindow)
+FHOG_INST(_Float16, 64, kWindow)
+FHOG_INST(_Float16, 128, kWindow)
+FHOG_INST(_Float16, 256, kWindow)
+FHOG_INST(float, 64, kWindow)
+FHOG_INST(float, 128, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

@@ -80,10 +80,11 @@ struct Scores {
   f32x4 S[2], ddS[2], dP[2], dPa[2];
 };
 
-template <typename T, int D, bool CAUSAL, bool PRE>
+template <typename T, int D, int MASK, bool PRE>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1, D == 64 ? 2 : 1)))
 bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 32;       // 32-deep steps over the head dim (score products)
   constexpr int DB = D / 16;       // 16-wide output column blocks
@@ -120,15 +121,32 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   const int qi = q0 + n;
   const bool qvalid = qi < p.nq;
 
-  // Keys [0, kend) are visible to some query of the workgroup, [0, wend) to
-  // some query of this wave.
-  int kend = p.nk;
-  if (CAUSAL) kend = min(kend, qb * BQ + BQ + p.coff);
-  // (uniform; saying so keeps the compiler from treating the loop as divergent)
-  const int nkt = __builtin_amdgcn_readfirstlane(kend > 0 ? (kend + BK - 1) / BK : 0);
-  int wend = p.nk;
-  if (CAUSAL) wend = max(0, min(wend, q0 + kQ + p.coff));
-  const int wkt = q0 < p.nq ? (wend + BK - 1) / BK : 0;  // tiles with work for this wave
+  // The tiles that hold keys visible to some query of the workgroup, the whole ones
+  // (visible to every query of it and inside nk) first, and to some query of this wave.
+  const KeyTiles<MASK> tiles(p, qb * BQ, BQ);
+  const int nkt = tiles.count;
+  const KeyBounds<MASK> sees(p, q0, kQ);
+  int full = p.nk / BK;
+  if (CAUSAL) full = min(full, max(0, qb * BQ + p.coff + 1) / BK);
+  int lower = 0;  // window mode: tiles below the whole ones, which some query's window starts in
+  if constexpr (MASK == kWindow) {
+    const int begin = tiles.sink_tiles + tiles.jump, end = begin + nkt - tiles.sink_tiles;
+    const int whole = (max(0, qb * BQ + BQ + p.coff - p.window) + BK - 1) / BK;
+    lower = __builtin_amdgcn_readfirstlane(min(max(whole, begin), end) - begin);
+    full = max(0, min(full, end) - (begin + lower));
+  }
+  const int nfull = __builtin_amdgcn_readfirstlane(min(full, nkt));
+  // Iteration t's tile; in window mode the whole ones, those below them, those above and
+  // the sinks'.
+  auto tile = [&](int t) {
+    if constexpr (MASK == kWindow) {
+      const int in_window = nkt - tiles.sink_tiles, begin = tiles.sink_tiles + tiles.jump;
+      if (t < nfull) return begin + lower + t;
+      if (t < nfull + lower) return begin + t - nfull;
+      return t < in_window ? begin + t : t - in_window;
+    }
+    return t;
+  };
 
   SwzFrags16<T, D> fr;
   fr.init(lane);
@@ -141,11 +159,13 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   dma.init(row_bytes, BK, lane);
   const uint32_t lds_kv = lds_base_u32(s_kv);
   const uint32_t lds_wave = lds_kv + wave * kTile;
-  auto issue = [&](int kt) {
+  auto issue = [&](int t) {
+    const int kt = tile(t);
     const int nvalid = p.nk - kt * BK;
-    const uint32_t dst = lds_wave + (uint32_t)(((uint32_t)kt % NST) * kStage);
+    const uint32_t dst = lds_wave + (uint32_t)(((uint32_t)t % NST) * kStage);
+    if constexpr (MASK == kWindow) gnext = src + (long)kt * BK * rsk;
     const T* gsrc = gnext;
-    gnext += BK * rsk;
+    if constexpr (MASK != kWindow) gnext += BK * rsk;
     if (nvalid >= BK) {
       dma.issue(dst, gsrc);
     } else {
@@ -240,15 +260,15 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   // Element-wise step and output products of the key tile in slot sa whose
   // scores are sc. Element e of the permuted key order is C tile e / 4,
   // register e % 4 (tile-relative key 16 (e / 4) + 4 g + e % 4); keys past
-  // klim are masked when MASK.
-  auto finish = [&](uint32_t sa, const Scores& sc, int klim, auto mask_tag) {
-    constexpr bool MASK = decltype(mask_tag)::value;
+  // klim, and those below klow that are no sinks, are masked when EDGE.
+  auto finish = [&](uint32_t sa, const Scores& sc, int klim, int klow, int ksinks, auto mask_tag) {
+    constexpr bool EDGE = decltype(mask_tag)::value;
     f32x8 vP, vx, vu, vX;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int kb = e >> 2, i = e & 3;
       float P = exp2_fast(fmaf(sc.S[kb][i], c2, nL2));
-      if (MASK && 16 * kb + 4 * g + i > klim) P = 0.f;
+      if (EDGE && (16 * kb + 4 * g + i > klim || outside<MASK>(16 * kb + 4 * g + i, klow, ksinks))) P = 0.f;
       const float x = PRE ? P * sc.ddS[kb][i] : P * (sc.ddS[kb][i] * scale);  // P ddS
       const float u = sc.dP[kb][i];                 // dP - D
       dd_acc += x;
@@ -286,20 +306,16 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
     __syncthreads();
   };
 
-  // Full tiles [0, nfull): visible to every query of the workgroup and inside
-  // nk, so no mask. Pipelined: the scores of tile t + 1 are formed in the step
+  // Full tiles [0, nfull), no mask. Pipelined: the scores of tile t + 1 are formed in the step
   // that finishes tile t, so each wave has independent matrix work to issue
   // beside its element-wise work. Buffers alternate, the loop being unrolled
   // by two.
-  int full = p.nk / BK;
-  if (CAUSAL) full = min(full, max(0, qb * BQ + p.coff + 1) / BK);
-  const int nfull = __builtin_amdgcn_readfirstlane(min(full, nkt));
   auto step = [&](int t, Scores& cur, Scores& nxt, auto next_tag) {
     constexpr bool NEXT = decltype(next_tag)::value;
     advance(NEXT ? t + 1 : t);
     if (hi + 1 < nkt) issue(++hi);
     if constexpr (NEXT) scores(slot(t + 1), nxt);
-    finish(slot(t), cur, 0, std::false_type{});
+    finish(slot(t), cur, 0, 0, 0, std::false_type{});
   };
 
   int t = 0;
@@ -309,7 +325,7 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
       if (hi + 1 < nkt) issue(++hi);
       Scores A;
       scores(slot(t), A);
-      finish(slot(t), A, 0, std::false_type{});
+      finish(slot(t), A, 0, 0, 0, std::false_type{});
     }
   } else if (nfull > 0) {
     Scores A, B;
@@ -332,11 +348,13 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   for (; t < nkt; ++t) {
     advance(t);
     if (hi + 1 < nkt) issue(++hi);
-    if (t < wkt) {
+    const int kt = tile(t);
+    if (sees.active(kt)) {
       Scores sc;
       scores(slot(t), sc);
-      const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - t * BK;  // last visible key, tile-relative
-      finish(slot(t), sc, klim, std::true_type{});
+      const int k0 = kt * BK;
+      const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - k0;  // last visible key, tile-relative
+      finish(slot(t), sc, klim, qi + p.coff - p.window + 1 - k0, p.sinks - k0, std::true_type{});
     }
   }
 
@@ -345,7 +363,7 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   // (see above).
   const float dDo = group4_sum(ddr_acc);
   // A row that sees exactly one key (see above).
-  const bool one_key = (CAUSAL ? min(p.nk, qi + p.coff + 1) : p.nk) == 1;
+  const bool one_key = keys_seen<MASK>(p, qi) == 1;
   // c = D dD + B from the unrounded per-pair sums (see above).
   const float c = group4_sum(xs_acc) - dD * group4_sum(pu_acc);
   // ddO = acc_o - dD O, from this lane's four columns of each 16-column block
@@ -382,19 +400,19 @@ bwdbwd_q_fused_kernel(BwdBwdParams<T> p, int chunk, int fold) {
 
 }  // namespace
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwdbwd_stage1_fused(const BwdBwdParams<T>& p, hipStream_t stream) {
   const int nqb = (p.nq + kQ * kWaves - 1) / (kQ * kWaves);
   const int npairs = p.batch * p.heads;
   const int chunk = grid_chunk(npairs, nqb, resident_workgroups(D == 64 ? 2 : 1));
-  const int fold = fold_rank(CAUSAL && D == 64, nqb, npairs, resident_workgroups(1));
+  const int fold = fold_rank(MASK == 1 && D == 64, nqb, npairs, resident_workgroups(1));
   const dim3 grid(nqb * npairs);
   int e2;
   if (std::is_same_v<T, __bf16> && std::frexp(p.scale, &e2) == 0.5f)  // scale = 2^(e2 - 1)
-    hipLaunchKernelGGL((bwdbwd_q_fused_kernel<T, D, CAUSAL, std::is_same_v<T, __bf16>>), grid, dim3(kThreads), 0,
+    hipLaunchKernelGGL((bwdbwd_q_fused_kernel<T, D, MASK, std::is_same_v<T, __bf16>>), grid, dim3(kThreads), 0,
                        stream, p, chunk, fold);
   else
-    hipLaunchKernelGGL((bwdbwd_q_fused_kernel<T, D, CAUSAL, false>), grid, dim3(kThreads), 0, stream, p, chunk, fold);
+    hipLaunchKernelGGL((bwdbwd_q_fused_kernel<T, D, MASK, false>), grid, dim3(kThreads), 0, stream, p, chunk, fold);
   return hipGetLastError();
 }
 
@@ -408,6 +426,10 @@ FHOG_INST(__bf16, 256, true)
 FHOG_INST(__bf16, 256, false)
 FHOG_INST(_Float16, 256, true)
 FHOG_INST(_Float16, 256, false)
+FHOG_INST(__bf16, 64, kWindow)
+FHOG_INST(__bf16, 256, kWindow)
+FHOG_INST(_Float16, 64, kWindow)
+FHOG_INST(_Float16, 256, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

@@ -40,10 +40,11 @@ namespace {
 
 constexpr int kOcc = 2;  // waves per SIMD
 
-template <typename T, int D, bool CAUSAL, bool PRE, int PAIRS>
+template <typename T, int D, int MASK, bool PRE, int PAIRS>
 __global__ void __launch_bounds__(128 * PAIRS)
 __attribute__((amdgpu_waves_per_eu(kOcc, kOcc)))
 bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
@@ -84,12 +85,9 @@ bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   const int qi = q0 + n;
   const bool qvalid = qi < p.nq;
 
-  int kend = p.nk;
-  if (CAUSAL) kend = min(kend, qb * BQ + BQ + p.coff);
-  const int nkt = __builtin_amdgcn_readfirstlane(kend > 0 ? (kend + BK - 1) / BK : 0);
-  int wend = p.nk;
-  if (CAUSAL) wend = max(0, min(wend, q0 + 32 + p.coff));
-  const int wkt = q0 < p.nq ? (wend + BK - 1) / BK : 0;  // tiles with work for this pair
+  const KeyTiles<MASK> tiles(p, qb * BQ, BQ);
+  const int nkt = tiles.count;
+  const KeyBounds<MASK> sees(p, q0, 32);
 
   SwzFrags<T, D> fr;
   fr.init(lane);
@@ -98,9 +96,11 @@ bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   dma.init(row_bytes, BK, lane, kPart * wave);
   const uint32_t lds0 = lds_base_u32(s_kv);
   long gnext = kbase;
-  auto issue = [&](int kt) {
-    const uint32_t stage = lds0 + (uint32_t)(((uint32_t)kt % NST) * kStage);
+  auto issue = [&](int it) {
+    const int kt = tiles.tile(it);
+    const uint32_t stage = lds0 + (uint32_t)(((uint32_t)it % NST) * kStage);
     const int nvalid = p.nk - kt * BK;
+    if constexpr (MASK == kWindow) gnext = kbase + (long)kt * BK * rsk;
     if (nvalid >= BK) {
       dma.issue(stage, p.k + gnext);
       dma.issue(stage + kTile, p.v + gnext);
@@ -114,7 +114,7 @@ bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
       part.issue(stage + 2 * kTile, p.ddk + gnext);
       part.issue(stage + 3 * kTile, p.ddv + gnext);
     }
-    gnext += BK * rsk;
+    if constexpr (MASK != kWindow) gnext += BK * rsk;
   };
 
   const float scale = p.scale;
@@ -164,7 +164,8 @@ bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
       wait_vmem();
       __syncthreads();
       if (t + 1 < nkt) issue(t + 1);
-      const bool active = t < wkt;
+      const int kt = tiles.tile(t);
+      const bool active = sees.active(kt);
       const uint32_t sa = lds0 + (uint32_t)(((uint32_t)t % NST) * kStage);
       float* xp = reinterpret_cast<float*>(s_x + pair * 2 * kExch) + 4 * lane;  // P, then x
       f32x16 C0, C1;
@@ -182,12 +183,13 @@ bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) C0[r] = exp2_fast(fmaf(C0[r], c2, nL2));
-          const int k0 = t * BK;
-          if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff)) {
+          const int k0 = kt * BK;
+          if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff) || sees.below(k0)) {
             const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - k0;  // last visible key, tile-relative
+            const int klow = qi + p.coff - p.window + 1 - k0;                       // first one of the window
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              if (crow(r, g) > klim) C0[r] = 0.f;
+              if (crow(r, g) > klim || outside<MASK>(crow(r, g), klow, p.sinks - k0)) C0[r] = 0.f;
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
@@ -289,7 +291,7 @@ bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
     } else {
       const float dD = *xd;
       const float c = s0 - dD * s1;
-      const bool one_key = (CAUSAL ? min(p.nk, qi + p.coff + 1) : p.nk) == 1;
+      const bool one_key = keys_seen<MASK>(p, qi) == 1;
       if (qvalid) {
         if (g == 0) {
           p.delta[sbase + qi] = Di;
@@ -319,30 +321,34 @@ bwdbwd_fused_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
     sweep(std::integral_constant<int, 1>{});
 }
 
-template <typename T, int D, bool CAUSAL, int PAIRS>
+template <typename T, int D, int MASK, int PAIRS>
 hipError_t launch_pairs(const BwdBwdParams<T>& p, int cus, hipStream_t stream) {
   const int nqb = (p.nq + 32 * PAIRS - 1) / (32 * PAIRS);
   const int npairs = p.batch * p.heads;
-  const int fold = fold_rank(CAUSAL && PAIRS == 2, nqb, npairs, cus);
+  const int fold = fold_rank(MASK == 1 && PAIRS == 2, nqb, npairs, cus);
   const int chunk = grid_chunk(npairs, nqb, PAIRS == 2 ? 2 * cus : cus);
   const dim3 grid(nqb * npairs), block(128 * PAIRS);
   int e2;
   constexpr bool kPre = std::is_same_v<T, __bf16>;
   if (kPre && std::frexp(p.scale, &e2) == 0.5f)  // scale = 2^(e2 - 1)
-    hipLaunchKernelGGL((bwdbwd_fused_pair_kernel<T, D, CAUSAL, kPre, PAIRS>), grid, block, 0, stream, p, chunk, fold);
+    hipLaunchKernelGGL((bwdbwd_fused_pair_kernel<T, D, MASK, kPre, PAIRS>), grid, block, 0, stream, p, chunk, fold);
   else
-    hipLaunchKernelGGL((bwdbwd_fused_pair_kernel<T, D, CAUSAL, false, PAIRS>), grid, block, 0, stream, p, chunk, fold);
+    hipLaunchKernelGGL((bwdbwd_fused_pair_kernel<T, D, MASK, false, PAIRS>), grid, block, 0, stream, p, chunk, fold);
   return hipGetLastError();
 }
 
 }  // namespace
 
-template <typename T, bool CAUSAL>
+template <typename T, int MASK>
 hipError_t launch_bwdbwd_stage1_fused_pair(const BwdBwdParams<T>& p, hipStream_t stream) {
   const int cus = resident_workgroups(1);
-  if (stage1_pairs_rule(mask_of(CAUSAL, p), p.batch * p.heads, cus) == 2)
-    return launch_pairs<T, 128, CAUSAL, 2>(p, cus, stream);
-  return launch_pairs<T, 128, CAUSAL, 4>(p, cus, stream);
+  if constexpr (MASK == kWindow) {
+    return launch_pairs<T, 128, MASK, 2>(p, cus, stream);
+  } else {
+    if (stage1_pairs_rule(mask_of(MASK != 0, p), p.batch * p.heads, cus) == 2)
+      return launch_pairs<T, 128, MASK, 2>(p, cus, stream);
+    return launch_pairs<T, 128, MASK, 4>(p, cus, stream);
+  }
 }
 
 #define FHOG_INST(T, C) \
@@ -351,6 +357,8 @@ FHOG_INST(__bf16, true)
 FHOG_INST(__bf16, false)
 FHOG_INST(_Float16, true)
 FHOG_INST(_Float16, false)
+FHOG_INST(__bf16, kWindow)
+FHOG_INST(_Float16, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

@@ -54,10 +54,11 @@ template <typename T, int D> struct Occupancy {
   static constexpr int value = D * sizeof(T) >= 512 ? 1 : 2;
 };
 
-template <typename T, int D, bool CAUSAL, bool PRE>
+template <typename T, int D, int MASK, bool PRE>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(Occupancy<T, D>::value, Occupancy<T, D>::value)))
 bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
@@ -83,8 +84,19 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   const GridSlot gs = grid_slot(blockIdx.x, nbh, nkb, chunk);
   // causal: the longest key columns come first, up to rank `fold`; the ranks
   // from there on run backwards (fold_rank)
-  const int kb = folded(gs.rank, nkb, fold);
-  const int bh = gs.pair;
+  int bkb = folded(gs.rank, nkb, fold), bbh = gs.pair, bpart = 0;
+  if constexpr (MASK == kWindow) {
+    const int extra = (int)blockIdx.x - nkb * nbh;  // workgroups of sinks' further queries (SinkGrid)
+    if (extra >= 0) {
+      const int c = extra / nbh;
+      bbh = extra - c * nbh;
+      bpart = 1 + c / p.sink.blocks;
+      bkb = c % p.sink.blocks;
+    }
+  }
+  const int kb = bkb, bh = bbh;
+  [[maybe_unused]] const int part = bpart;
+  const QueryBounds<MASK> qs(p, kb, BKB, part, p.sink.step);
   const int b = bh / p.kv_heads, hk = bh % p.kv_heads;
   const int grp = p.heads / p.kv_heads;  // query heads per key/value head
   const long rs = (long)p.heads * D;      // query-side row stride
@@ -96,12 +108,13 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   const int k0 = kb * BKB + pair * 32;
   const int kj = k0 + n;
   const bool kvalid = kj < p.nk;
-  const int qfirst = first_contributing_query(p, kj, CAUSAL);
+  // (window mode drops the rows that see one key by their logsumexp, below)
+  const int qfirst = MASK == kWindow ? qs.lo(kj) : first_contributing_query(p, kj, CAUSAL);
 
   // Iteration i visits query tile qt_begin + i / grp of query head
   // hk * grp + i % grp (the group reduction of _pallas_gpu_kernel.py:333-370).
-  const int nqt = (p.nq + BQ - 1) / BQ;
-  const int qt_begin = CAUSAL ? max(0, kb * BKB - p.coff) / BQ : 0;
+  const int nqt = (qs.q_end + BQ - 1) / BQ;
+  const int qt_begin = qs.q_begin / BQ;
   const int total = __builtin_amdgcn_readfirstlane(nqt > qt_begin ? (nqt - qt_begin) * grp : 0);
 
   f32x16 acc[DT];  // A: dV2, B: dK2
@@ -152,10 +165,14 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
       gnext += c.gi + 1 == grp ? row_step : (long)D;
       c.next(grp);
     };
-    auto finish_stats = [&](int i) {
+    // Turns tile i's statistics, queries from q0 on, into the accumulators' constants. In
+    // window mode a query that sees one key gets L = +inf and so P = 0 (its pair's terms
+    // are exactly zero, first_contributing_query).
+    auto finish_stats = [&](int i, int q0) {
       if (g == 0) {
         float* st = reinterpret_cast<float*>(s_q + ((uint32_t)i % NST) * kStage + 3 * kTile);
-        const float L = st[n], Dq = st[BQ + n], dDq = st[2 * BQ + n], Bq = st[3 * BQ + n];
+        const float L = MASK == kWindow && keys_seen<MASK>(p, q0 + n) == 1 ? INFINITY : st[n];
+        const float Dq = st[BQ + n], dDq = st[2 * BQ + n], Bq = st[3 * BQ + n];
         st[n] = PRE ? -L : -L * inv_scale;
         st[BQ + n] = PRE ? -dDq : -dDq * inv_scale;
         st[2 * BQ + n] = -Dq;
@@ -164,6 +181,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
     };
 
     GroupCursor nxt;  // iteration of the next tile to issue
+    int issued_q0 = qt_begin * BQ;  // first query of the last tile issued
     issue(0, nxt);
     advance(nxt);
 
@@ -193,7 +211,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
       const float c2 = PRE ? kLog2e : scale * kLog2e;
       // Retire the key-side loads, and with them the first tile, before the loop.
       wait_vmem();
-      if (wave == kStatWave) finish_stats(0);
+      if (wave == kStatWave) finish_stats(0, issued_q0);
 
       // After its first barrier of iteration i every wave is done with tile
       // i - 1, whose stage tile i + 1 takes, and with the exchange buffer.
@@ -202,11 +220,12 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
         wait_vmem();
         __syncthreads();
         if (i + 1 < total) {
+          issued_q0 = (qt_begin + nxt.qt) * BQ;
           issue(i + 1, nxt);
           advance(nxt);
         }
         const int q0 = (qt_begin + cur.qt) * BQ;
-        const bool active = k0 < p.nk && (!CAUSAL || q0 + BQ - 1 >= k0 - p.coff);
+        const bool active = k0 < p.nk && qs.active(q0, k0);
         const uint32_t slot = ((uint32_t)i % NST) * kStage;
         const uint32_t sa = lds0 + slot;  // Q, dO, ddQ
         float* xp = reinterpret_cast<float*>(s_x + pair * 2 * kExch) + 4 * lane;  // P, then t
@@ -240,9 +259,9 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
               C0[r] = exp2_fast(C0[r] * c2);
               if (!PRE) C1[r] *= scale;
             }
-            if ((q0 + BQ > p.nq) || (CAUSAL && q0 < k0 + 31 - p.coff) || p.nk == 1) {
-              // a pair enters iff qfirst <= query < nq
-              const int qlo = qfirst - q0, qhi = p.nq - q0;
+            if (qs.masked(q0, k0) || p.nk == 1) {
+              // a pair enters iff qfirst <= query < nq (or the window's end)
+              const int qlo = qfirst - q0, qhi = qs.hi(kj) - q0;
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const int m = crow(r, g);
@@ -302,7 +321,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
         // The next tile's statistics, whose DMA went out with this iteration's issue.
         if (wave == kStatWave && i + 1 < total) {
           wait_vmem();
-          finish_stats(i + 1);
+          finish_stats(i + 1, issued_q0);
         }
       }
     };
@@ -312,6 +331,21 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
       sweep(std::integral_constant<int, 1>{});
   }
 
+  if constexpr (MASK == kWindow) {
+    if (kvalid && kj < p.sinks && p.sink.chunks > 0) {
+      const long row = ((long)part * nbh + bh) * min(p.sinks, p.nk) + kj;
+      float* dst = p.sink_parts + (2 * row + wave_role) * D;
+      const float f = wave_role ? p.scale : 1.0f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * a + 4 * g) = f32x4{acc[dt][4 * a] * f, acc[dt][4 * a + 1] * f,
+                                                                           acc[dt][4 * a + 2] * f, acc[dt][4 * a + 3] * f};
+      return;
+    }
+    if (part > 0) return;  // keys of the block that are no sinks
+  }
   if (kvalid) {
     T* dst = (wave_role ? p.dk2 : p.dv2) + kbase + (long)kj * rsk;
     const float f = wave_role ? p.scale : 1.0f;
@@ -330,20 +364,20 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
 
 }  // namespace
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwdbwd_stage2_pair(const BwdBwdParams<T>& p, hipStream_t stream) {
   const int nkb = (p.nk + 32 * kPairs - 1) / (32 * kPairs);
   const int npairs = p.batch * p.kv_heads;
   const int cus = resident_workgroups(1);
-  const int fold = fold_rank(CAUSAL && Occupancy<T, D>::value == 2, nkb, npairs, cus);
+  const int fold = fold_rank(MASK == 1 && Occupancy<T, D>::value == 2, nkb, npairs, cus);
   const int chunk = grid_chunk(npairs, nkb, Occupancy<T, D>::value * cus);
-  const dim3 grid(nkb * npairs);
+  const dim3 grid(key_grid<MASK>(p, 32 * kPairs));
   int e2;
   constexpr bool kPre = std::is_same_v<T, __bf16>;
   if (kPre && std::frexp(p.scale, &e2) == 0.5f)  // scale = 2^(e2 - 1)
-    hipLaunchKernelGGL((bwdbwd_pair_kernel<T, D, CAUSAL, kPre>), grid, dim3(kThreads), 0, stream, p, chunk, fold);
+    hipLaunchKernelGGL((bwdbwd_pair_kernel<T, D, MASK, kPre>), grid, dim3(kThreads), 0, stream, p, chunk, fold);
   else
-    hipLaunchKernelGGL((bwdbwd_pair_kernel<T, D, CAUSAL, false>), grid, dim3(kThreads), 0, stream, p, chunk, fold);
+    hipLaunchKernelGGL((bwdbwd_pair_kernel<T, D, MASK, false>), grid, dim3(kThreads), 0, stream, p, chunk, fold);
   return hipGetLastError();
 }
 
@@ -364,6 +398,14 @@ FHOG_INST(float, 64, true)
 FHOG_INST(float, 64, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
+FHOG_INST(__bf16, 64, kWindow)
+FHOG_INST(__bf16, 128, kWindow)
+FHOG_INST(__bf16, 256, kWindow)
+FHOG_INST(_Float16, 64, kWindow)
+FHOG_INST(_Float16, 128, kWindow)
+FHOG_INST(_Float16, 256, kWindow)
+FHOG_INST(float, 64, kWindow)
+FHOG_INST(float, 128, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

@@ -52,10 +52,11 @@ template <int D> struct Occupancy {
   static constexpr int value = D == 64 ? 2 : 1;
 };
 
-template <int D, bool CAUSAL>
+template <int D, int MASK>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(Occupancy<D>::value, Occupancy<D>::value)))
 bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef float T;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;       // 16-deep steps over the head dim
@@ -94,12 +95,9 @@ bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
   const int qi = q0 + n;
   const bool qvalid = qi < p.nq;
 
-  int kend = p.nk;
-  if (CAUSAL) kend = min(kend, qb * BQ + BQ + p.coff);
-  const int nkt = __builtin_amdgcn_readfirstlane(kend > 0 ? (kend + BK - 1) / BK : 0);  // tiles the workgroup streams
-  int wend = p.nk;
-  if (CAUSAL) wend = max(0, min(wend, q0 + 32 + p.coff));
-  const int wkt = q0 < p.nq ? (wend + BK - 1) / BK : 0;  // tiles with work for this pair
+  const KeyTiles<MASK> tiles(p, qb * BQ, BQ);  // tiles the workgroup streams
+  const int nkt = tiles.count;
+  const KeyBounds<MASK> sees(p, q0, 32);
 
   SwzFrags<T, D> fr;
   fr.init(lane);
@@ -112,7 +110,7 @@ bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
   const uint32_t lds0 = lds_base_u32(s_kv);
   const int total = 2 * nkt;
   auto issue = [&](int it) {
-    const int kt = it < nkt ? it : it - nkt;
+    const int kt = tiles.tile(it < nkt ? it : it - nkt);
     const int nvalid = p.nk - kt * BK;
     const uint32_t stage = lds0 + (uint32_t)(((uint32_t)it % NST) * kStage);
     const long off = kbase + (long)kt * BK * rsk;
@@ -186,11 +184,12 @@ bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) C0[r] = exp2_fast(fmaf(C0[r], c2, nL2));
       const int k0 = kt * BK;
-      if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff)) {
+      if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff) || sees.below(k0)) {
         const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - k0;  // last visible key, tile-relative
+        const int klow = qi + p.coff - p.window + 1 - k0;                       // first one of the window
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (crow(r, g) > klim) C0[r] = 0.f;
+          if (crow(r, g) > klim || outside<MASK>(crow(r, g), klow, p.sinks - k0)) C0[r] = 0.f;
       }
     };
 
@@ -202,10 +201,11 @@ bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
     for (int it = 0; it < nkt; ++it) {
       advance(it);
       const uint32_t sa = lds0 + (uint32_t)(((uint32_t)it % NST) * kStage);  // K, V, ddK, ddV
-      const bool active = it < wkt;
+      const int kt = tiles.tile(it);
+      const bool active = sees.active(kt);
       if (active) {
         if constexpr (role == 0) {
-          scores_a(sa, it);
+          scores_a(sa, kt);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             C1[r] = C1[r] * C0[r];
@@ -300,10 +300,11 @@ bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
     for (int it = nkt; it < total; ++it) {
       advance(it);
       const uint32_t sa = lds0 + (uint32_t)(((uint32_t)it % NST) * kStage);  // K, V, ddK, ddV
-      const bool active = it - nkt < wkt;
+      const int kt = tiles.tile(it - nkt);
+      const bool active = sees.active(kt);
       if (active) {
         if constexpr (role == 0) {
-          scores_a(sa, it - nkt);
+          scores_a(sa, kt);
 #pragma unroll
           for (int r = 0; r < 16; ++r) C1[r] = fmaf(C1[r], scale, ndD);  // ddS - dD
           put(0, C0);
@@ -357,7 +358,7 @@ bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
       T* dst = (role ? p.dq2 : p.ddo) + qbase + (long)qi * rs;
       // A row that sees exactly one key has a constant softmax: its dQ2 is
       // exactly 0, while the sums above cancel only to rounding of c.
-      const bool one_key = (CAUSAL ? min(p.nk, qi + p.coff + 1) : p.nk) == 1;
+      const bool one_key = keys_seen<MASK>(p, qi) == 1;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
@@ -381,14 +382,14 @@ bwdbwd_qpair_kernel(BwdBwdParams<float> p, int chunk, int fold) {
 
 }  // namespace
 
-template <int D, bool CAUSAL>
+template <int D, int MASK>
 hipError_t launch_bwdbwd_stage1_qpair(const BwdBwdParams<float>& p, hipStream_t stream) {
   const int nqb = (p.nq + 32 * kPairs - 1) / (32 * kPairs);
   const int npairs = p.batch * p.heads;
   const int cus = resident_workgroups(1);
-  hipLaunchKernelGGL((bwdbwd_qpair_kernel<D, CAUSAL>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
+  hipLaunchKernelGGL((bwdbwd_qpair_kernel<D, MASK>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
                      grid_chunk(npairs, nqb, Occupancy<D>::value * cus),
-                     fold_rank(CAUSAL && Occupancy<D>::value == 2, nqb, npairs, cus));
+                     fold_rank(MASK == 1 && Occupancy<D>::value == 2, nqb, npairs, cus));
   return hipGetLastError();
 }
 
@@ -397,6 +398,8 @@ FHOG_INST(64, true)
 FHOG_INST(64, false)
 FHOG_INST(128, true)
 FHOG_INST(128, false)
+FHOG_INST(64, kWindow)
+FHOG_INST(128, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

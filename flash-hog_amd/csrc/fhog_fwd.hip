@@ -39,10 +39,11 @@ template <typename T, int D> struct Stages {
   static constexpr int value = sizeof(T) == 4 && D == 64 ? 3 : 4;
 };
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(Occupancy<T, D>::value, Occupancy<T, D>::value)))
 fwd_kernel(FwdParams<T> p, int chunk) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
@@ -84,15 +85,11 @@ fwd_kernel(FwdParams<T> p, int chunk) {
     if (negate) qf[ks] = -qf[ks];
   }
 
-  // Keys [0, kend) are visible to some query of the workgroup, [0, wend) to
-  // some query of this wave.
-  int kend = p.nk;
-  if (CAUSAL) kend = min(kend, qb * BQ + BQ + p.coff);
-  // (uniform; saying so keeps the compiler from treating the loop as divergent)
-  const int nkt = __builtin_amdgcn_readfirstlane(kend > 0 ? (kend + BK - 1) / BK : 0);
-  int wend = p.nk;
-  if (CAUSAL) wend = max(0, min(wend, q0 + 32 + p.coff));
-  const int wkt = q0 < p.nq ? (wend + BK - 1) / BK : 0;
+  // The tiles that hold keys visible to some query of the workgroup, and to some
+  // query of this wave.
+  const KeyTiles<MASK> tiles(p, qb * BQ, BQ);
+  const int nkt = tiles.count;
+  const KeyBounds<MASK> sees(p, q0, 32);
 
   // (offsets of its own for every column: with shared ones D = 128 was 1-2 % slower)
   WaveFrags<T, D, sizeof(T) == 2 ? D : 64> fr;
@@ -104,9 +101,10 @@ fwd_kernel(FwdParams<T> p, int chunk) {
   dma.init(row_bytes, BK, lane, kPer * (wave & 1));
   const uint32_t lds_kv = lds_base_u32(s_kv);
   const uint32_t lds_tensor = lds_kv + tensor * kTile;
-  auto issue = [&](int kt) {
+  auto issue = [&](int it) {
+    const int kt = tiles.tile(it);
     const int nvalid = p.nk - kt * BK;
-    const uint32_t dst = lds_tensor + (uint32_t)(((uint32_t)kt % NST) * kStage);
+    const uint32_t dst = lds_tensor + (uint32_t)(((uint32_t)it % NST) * kStage);
     const T* gsrc = src + (long)kt * BK * rsk;
     if (nvalid >= BK) {
       dma.issue(dst, gsrc);
@@ -133,12 +131,13 @@ fwd_kernel(FwdParams<T> p, int chunk) {
   for (int i = 0; i < NST - 1; ++i)
     if (i < nkt) issue(i);
 
-  for (int kt = 0; kt < nkt; ++kt) {
-    wait_tile<NST, kPer>(kt, nkt);
+  for (int it = 0; it < nkt; ++it) {
+    wait_tile<NST, kPer>(it, nkt);
     __syncthreads();
-    if (kt + NST - 1 < nkt) issue(kt + NST - 1);
-    if (kt < wkt) {
-      const uint32_t sa = lds_kv + (uint32_t)(((uint32_t)kt % NST) * kStage);  // K at 0, V at kTile
+    if (it + NST - 1 < nkt) issue(it + NST - 1);
+    const int kt = tiles.tile(it);
+    if (sees.active(kt)) {
+      const uint32_t sa = lds_kv + (uint32_t)(((uint32_t)it % NST) * kStage);  // K at 0, V at kTile
       f32x16 S = zero16();
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -158,11 +157,12 @@ fwd_kernel(FwdParams<T> p, int chunk) {
       // (c2 > 0, and rounding is monotonic, so this equals the maximum of the
       // scaled values), and the scale enters the exponent's fma below.
       const int k0 = kt * BK;
-      if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff)) {
+      if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff) || sees.below(k0)) {
         const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - k0;  // last visible key, tile-relative
+        const int klow = qi + p.coff - p.window + 1 - k0;                       // first one of the window
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (crow(r, g) > klim) S[r] = -INFINITY;
+          if (crow(r, g) > klim || outside<MASK>(crow(r, g), klow, p.sinks - k0)) S[r] = -INFINITY;
       }
       // Lazy rescale: a row keeps its running maximum m (log2 units) while the
       // probabilities it gives stay small, and O, l carry the same stale factor,
@@ -237,18 +237,18 @@ inline bool fwd_pair_selected(Mask m, int npairs, int head_dim) {
   return fwd_pair_rule(m, npairs, head_dim, resident_workgroups(1));
 }
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_fwd(const FwdParams<T>& p, hipStream_t stream) {
   if constexpr (sizeof(T) == 2 && D == 256) {
-    return launch_fwd_pair<T, D, CAUSAL>(p, stream);
+    return launch_fwd_pair<T, D, MASK>(p, stream);
   } else {
     const int npairs = p.batch * p.heads;
     if constexpr (sizeof(T) == 4) {
-      if (fwd_pair_selected(mask_of(CAUSAL, p), npairs, D)) return launch_fwd_pair<T, D, CAUSAL>(p, stream);
+      if (fwd_pair_selected(mask_of(MASK != 0, p), npairs, D)) return launch_fwd_pair<T, D, MASK>(p, stream);
     }
     const int nqb = (p.nq + 32 * kWaves - 1) / (32 * kWaves);
     const int chunk = grid_chunk(npairs, nqb, resident_workgroups(Occupancy<T, D>::value));
-    hipLaunchKernelGGL((fwd_kernel<T, D, CAUSAL>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p, chunk);
+    hipLaunchKernelGGL((fwd_kernel<T, D, MASK>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p, chunk);
     return hipGetLastError();
   }
 }
@@ -270,6 +270,14 @@ FHOG_INST(float, 64, true)
 FHOG_INST(float, 64, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
+FHOG_INST(__bf16, 64, kWindow)
+FHOG_INST(__bf16, 128, kWindow)
+FHOG_INST(__bf16, 256, kWindow)
+FHOG_INST(_Float16, 64, kWindow)
+FHOG_INST(_Float16, 128, kWindow)
+FHOG_INST(_Float16, 256, kWindow)
+FHOG_INST(float, 64, kWindow)
+FHOG_INST(float, 128, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

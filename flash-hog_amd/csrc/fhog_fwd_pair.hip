@@ -33,10 +33,11 @@ constexpr int kThreads = 64 * kWaves;
 // allow more (a bound of two: 312 -> 329 us at B4 N2048 H16 causal).
 constexpr int kOcc = 2;
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kOcc, 8)))
 fwd_pair_kernel(FwdParams<T> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 32;  // 16-deep steps of half the head dim
   constexpr int DT = D / 64;  // 32-wide column blocks of half of O
@@ -74,14 +75,11 @@ fwd_pair_kernel(FwdParams<T> p, int chunk, int fold) {
   const int qi = q0 + n;
   const bool qvalid = qi < p.nq;
 
-  // Keys [0, kend) are visible to some query of the workgroup, [0, wend) to
-  // some query of this pair.
-  int kend = p.nk;
-  if (CAUSAL) kend = min(kend, qb * BQ + BQ + p.coff);
-  const int nkt = __builtin_amdgcn_readfirstlane(kend > 0 ? (kend + BK - 1) / BK : 0);
-  int wend = p.nk;
-  if (CAUSAL) wend = max(0, min(wend, q0 + 32 + p.coff));
-  const int wkt = q0 < p.nq ? (wend + BK - 1) / BK : 0;
+  // The tiles that hold keys visible to some query of the workgroup, and to some
+  // query of this pair.
+  const KeyTiles<MASK> tiles(p, qb * BQ, BQ);
+  const int nkt = tiles.count;
+  const KeyBounds<MASK> sees(p, q0, 32);
 
   SwzFrags<T, D> fr;
   fr.init(lane);
@@ -91,9 +89,10 @@ fwd_pair_kernel(FwdParams<T> p, int chunk, int fold) {
   TileDma<T, D, kPer> dma;
   dma.init(row_bytes, BK, lane, kPer * pair);
   const uint32_t lds0 = lds_base_u32(s_kv);
-  auto issue = [&](int kt) {
+  auto issue = [&](int it) {
+    const int kt = tiles.tile(it);
     const int nvalid = p.nk - kt * BK;
-    const uint32_t dst = lds0 + tensor * kTile + (uint32_t)(((uint32_t)kt % NST) * kStage);
+    const uint32_t dst = lds0 + tensor * kTile + (uint32_t)(((uint32_t)it % NST) * kStage);
     const T* gsrc = src + (long)kt * BK * rsk;
     if (nvalid >= BK) {
       dma.issue(dst, gsrc);
@@ -129,14 +128,15 @@ fwd_pair_kernel(FwdParams<T> p, int chunk, int fold) {
     wait_vmem();
     if (nkt > 0) issue(0);
 
-    // After its first barrier of iteration kt every wave is done with tile
-    // kt - 1, whose stage tile kt + 1 takes, and with the exchange buffer.
-    for (int kt = 0; kt < nkt; ++kt) {
+    // After its first barrier of iteration `it` every wave is done with tile
+    // it - 1, whose stage tile it + 1 takes, and with the exchange buffer.
+    for (int it = 0; it < nkt; ++it) {
       wait_vmem();
       __syncthreads();
-      if (kt + 1 < nkt) issue(kt + 1);
-      const bool active = kt < wkt;
-      const uint32_t sa = lds0 + (uint32_t)(((uint32_t)kt % NST) * kStage);  // K at 0, V at kTile
+      if (it + 1 < nkt) issue(it + 1);
+      const int kt = tiles.tile(it);
+      const bool active = sees.active(kt);
+      const uint32_t sa = lds0 + (uint32_t)(((uint32_t)it % NST) * kStage);  // K at 0, V at kTile
       f32x16 S;
       if (active) {
         S = zero16();
@@ -155,11 +155,12 @@ fwd_pair_kernel(FwdParams<T> p, int chunk, int fold) {
           for (int j = 0; j < 4; ++j) S[4 * a + j] += y[j];
         }
         const int k0 = kt * BK;
-        if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff)) {
+        if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff) || sees.below(k0)) {
           const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - k0;  // last visible key, tile-relative
+          const int klow = qi + p.coff - p.window + 1 - k0;                       // first one of the window
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (crow(r, g) > klim) S[r] = -INFINITY;
+            if (crow(r, g) > klim || outside<MASK>(crow(r, g), klow, p.sinks - k0)) S[r] = -INFINITY;
         }
         // The lazy rescale of fwd_kernel.
         f32x16 P;
@@ -222,13 +223,13 @@ fwd_pair_kernel(FwdParams<T> p, int chunk, int fold) {
 
 }  // namespace
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_fwd_pair(const FwdParams<T>& p, hipStream_t stream) {
   const int nqb = (p.nq + 32 * kPairs - 1) / (32 * kPairs);
   const int npairs = p.batch * p.heads;
   const int cus = resident_workgroups(1);
-  hipLaunchKernelGGL((fwd_pair_kernel<T, D, CAUSAL>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
-                     grid_chunk(npairs, nqb, kOcc * cus), fold_rank(CAUSAL, nqb, npairs, cus));
+  hipLaunchKernelGGL((fwd_pair_kernel<T, D, MASK>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
+                     grid_chunk(npairs, nqb, kOcc * cus), fold_rank(MASK == 1, nqb, npairs, cus));
   return hipGetLastError();
 }
 
@@ -241,6 +242,10 @@ FHOG_INST(float, 64, true)
 FHOG_INST(float, 64, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
+FHOG_INST(__bf16, 256, kWindow)
+FHOG_INST(_Float16, 256, kWindow)
+FHOG_INST(float, 64, kWindow)
+FHOG_INST(float, 128, kWindow)
 #undef FHOG_INST
 
 }  // namespace fhog

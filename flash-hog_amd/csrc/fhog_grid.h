@@ -395,4 +395,22 @@ inline bool q32_deal_rule(Mask m, int npairs, int cus) {
   return load.folded > (near_square(m, 4) ? 1.07 : 1.15) * load.dealt;
 }
 
+// Windowed attention, key-tiled kernels (64-key blocks): queries per chunk of those that see
+// a sink as a sink only, and how many chunks that makes. A chunk is as long as an ordinary
+// block's share, window + 64, so that no workgroup outlasts the others; at least 512 queries,
+// so that the parts that the chunks leave stay few where the window is short; and at least
+// twice the number of sinks, which keeps all parts together below (n_q / 2 + 2 sinks) rows of
+// dK and dV a head.
+inline int sink_step(int window, int sinks) {
+  long step = window + 64l;
+  if (step < 512) step = 512;
+  if (step < 2l * sinks) step = 2l * sinks;
+  return (int)((step < (1l << 30) ? step : 1l << 30) + 31) / 32 * 32;
+}
+inline int sink_chunks(Mask m, int window, int sinks) {
+  const long first = window - (long)m.coff, begin = first > 0 ? first / 32 * 32 : 0;  // the first that sees key 0 so
+  const int step = sink_step(window, sinks);
+  return sinks > 0 && first < m.nq ? (int)((m.nq - begin + step - 1) / step) : 0;
+}
+
 }  // namespace fhog

@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include "fhog_grid.h"
+#include "fhog_window.h"
 
 namespace fhog {
 
@@ -25,6 +26,7 @@ template <typename T> struct FwdParams {
   T* o; float* lse;
   int batch, nq, nk, heads, kv_heads, coff;
   float scale;
+  int window = 0, sinks = 0;  // MASK = kWindow only, as below
 };
 
 template <typename T> struct BwdParams {
@@ -34,6 +36,9 @@ template <typename T> struct BwdParams {
   float* delta;
   int batch, nq, nk, heads, kv_heads, coff;
   float scale;
+  int window = 0, sinks = 0;
+  SinkGrid sink = {};
+  float* sink_parts = nullptr;  // (part, batch, kv_head, sink, dV and dK, head_dim)
 };
 
 template <typename T> struct BwdBwdParams {
@@ -44,6 +49,9 @@ template <typename T> struct BwdBwdParams {
   float* delta; float* ddelta; float* bstat;
   int batch, nq, nk, heads, kv_heads, coff;
   float scale;
+  int window = 0, sinks = 0;
+  SinkGrid sink = {};
+  float* sink_parts = nullptr;
 };
 
 // First query row whose pair with key kj enters dK2 and dV2. A query that
@@ -59,23 +67,29 @@ __device__ inline int first_contributing_query(const BwdBwdParams<T>& p, int kj,
   return causal ? kj - p.coff + (kj == 0) : 0;
 }
 
+// Workgroups of a key-tiled launch with blocks of `rows` keys.
+template <int MASK, typename P> inline int key_grid(const P& p, int rows) {
+  const int npairs = p.batch * p.kv_heads;
+  return ((p.nk + rows - 1) / rows + (MASK == kWindow ? p.sink.blocks * p.sink.chunks : 0)) * npairs;
+}
+
 // What the launch rules look at.
 template <typename P> inline Mask mask_of(bool causal, const P& p) { return Mask{causal, p.nq, p.nk, p.coff}; }
 
-template <typename T, int D, bool CAUSAL> hipError_t launch_fwd(const FwdParams<T>& p, hipStream_t s);
+template <typename T, int D, int MASK> hipError_t launch_fwd(const FwdParams<T>& p, hipStream_t s);
 // The forward with two waves per 32 queries: 2-byte types at D = 256, and fp32 on
 // small grids; launch_fwd selects it.
-template <typename T, int D, bool CAUSAL> hipError_t launch_fwd_pair(const FwdParams<T>& p, hipStream_t s);
+template <typename T, int D, int MASK> hipError_t launch_fwd_pair(const FwdParams<T>& p, hipStream_t s);
 template <typename T, int D, bool CAUSAL> hipError_t launch_bwd(const BwdParams<T>& p, hipStream_t s);
 // stages: bit 0 = stage 1 (passes 1-3), bit 1 = stage 2 (pass 4).
 template <typename T, int D, bool CAUSAL>
 hipError_t launch_bwdbwd(const BwdBwdParams<T>& p, hipStream_t s, int stages = 3);
 // Stage 1 in one sweep, 16 queries per wave (2-byte types, D = 64 and 256);
 // launch_bwdbwd selects it.
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwdbwd_stage1_fused(const BwdBwdParams<T>& p, hipStream_t s);
 // Stage 1 in one sweep, two waves per 32 queries (2-byte types, D = 128).
-template <typename T, bool CAUSAL>
+template <typename T, int MASK>
 hipError_t launch_bwdbwd_stage1_fused_pair(const BwdBwdParams<T>& p, hipStream_t s);
 // Stage 1 with 32 queries per wave at one wave per SIMD (2-byte types, D = 64);
 // launch_bwdbwd selects it.
@@ -97,20 +111,25 @@ template <typename T, bool CAUSAL>
 hipError_t launch_bwd_q64(const BwdParams<T>& p, hipStream_t s);
 // dQ and D of the first backward with two waves per 32 queries (all types and
 // head dims; launch_bwd selects it but for 2-byte D = 64 and 128 on larger grids).
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwd_qpair(const BwdParams<T>& p, hipStream_t s);
 // dK and dV of the first backward with two waves per 32 keys (all types and
 // head dims; at 2-byte D = 64 launch_bwd selects it for small grids and short causal
 // problems, bwd_pair_rule).
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwd_pair(const BwdParams<T>& p, hipStream_t s);
 // Stage 1 for fp32 with two waves per 32 queries; launch_bwdbwd selects it for
 // small grids.
-template <int D, bool CAUSAL>
+template <int D, int MASK>
 hipError_t launch_bwdbwd_stage1_qpair(const BwdBwdParams<float>& p, hipStream_t s);
 // Stage 2 with two waves per 32 keys (all types and head dims; at 2-byte
 // D = 64 launch_bwdbwd selects it for small grids).
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 hipError_t launch_bwdbwd_stage2_pair(const BwdBwdParams<T>& p, hipStream_t s);
+
+// The first backward and the double backward with a window of keys and sinks; the
+// forward is launch_fwd<T, D, kWindow>.
+template <typename T, int D> hipError_t launch_window_bwd(const BwdParams<T>& p, hipStream_t s);
+template <typename T, int D> hipError_t launch_window_bwdbwd(const BwdBwdParams<T>& p, hipStream_t s);
 
 }  // namespace fhog

@@ -53,6 +53,10 @@ struct Api {
   decltype(&fhog_attention_bwdbwd) bwdbwd = nullptr;
   decltype(&fhog_last_error) last_error = nullptr;
   decltype(&fhog_status_string) status_string = nullptr;
+  decltype(&fhog_window_workspace_bytes) window_bytes = nullptr;
+  decltype(&fhog_window_attention_fwd) window_fwd = nullptr;
+  decltype(&fhog_window_attention_bwd) window_bwd = nullptr;
+  decltype(&fhog_window_attention_bwdbwd) window_bwdbwd = nullptr;
   py::object error_cls;
 };
 
@@ -70,6 +74,14 @@ void bind(std::uintptr_t fwd, std::uintptr_t bwd, std::uintptr_t bwdbwd, std::ui
   a.last_error = reinterpret_cast<decltype(a.last_error)>(last_error);
   a.status_string = reinterpret_cast<decltype(a.status_string)>(status_string);
   a.error_cls = std::move(error_cls);
+}
+
+void bind_window(std::uintptr_t bytes, std::uintptr_t fwd, std::uintptr_t bwd, std::uintptr_t bwdbwd) {
+  Api& a = api();
+  a.window_bytes = reinterpret_cast<decltype(a.window_bytes)>(bytes);
+  a.window_fwd = reinterpret_cast<decltype(a.window_fwd)>(fwd);
+  a.window_bwd = reinterpret_cast<decltype(a.window_bwd)>(bwd);
+  a.window_bwdbwd = reinterpret_cast<decltype(a.window_bwdbwd)>(bwdbwd);
 }
 
 std::string shape_str(const at::Tensor& t) {
@@ -189,8 +201,19 @@ void require_bound(const void* fn) {
   if (!fn) throw std::runtime_error("_fhog_torch.bind() has not been called");
 }
 
+// A window of keys and sinks (0, 0: none), and the workspace that a backward with one needs
+// (undefined where it needs none).
+struct Window {
+  int window = 0, sinks = 0;
+  at::Tensor workspace(const at::Tensor& q, const Dims& d, int causal) const {
+    const size_t size = api().window_bytes(d.B, d.Tq, d.Tk, d.Nk, d.H, causal, window, sinks);
+    return size ? at::empty({(int64_t)size}, q.options().dtype(at::kByte)) : at::Tensor();
+  }
+};
+void* data_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
 std::tuple<at::Tensor, at::Tensor> fwd_core(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
-                                            int causal, double scale) {
+                                            int causal, double scale, Window w) {
   require_bound((const void*)api().fwd);
   check_inputs({{"q", &q_}, {"k", &k_}, {"v", &v_}}, q_.scalar_type());
   const Dims d = dims(q_, k_);
@@ -199,16 +222,20 @@ std::tuple<at::Tensor, at::Tensor> fwd_core(const at::Tensor& q_, const at::Tens
   at::Tensor o = at::empty_like(q);
   at::Tensor lse = at::empty({(int64_t)d.B, (int64_t)d.N, (int64_t)d.Tq}, q.options().dtype(at::kFloat));
   c10::DeviceGuard guard(q.device());
-  const int status = api().fwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                               lse.data_ptr<float>(), d.B, d.Tq, d.Tk, d.N, d.Nk, d.H, dtype_code(q.scalar_type()),
-                               causal, (float)scale);
+  const int dt = dtype_code(q.scalar_type());
+  const int status =
+      w.window ? api().window_fwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                  lse.data_ptr<float>(), d.B, d.Tq, d.Tk, d.N, d.Nk, d.H, dt, causal, w.window,
+                                  w.sinks, (float)scale)
+               : api().fwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                           lse.data_ptr<float>(), d.B, d.Tq, d.Tk, d.N, d.Nk, d.H, dt, causal, (float)scale);
   check_status(status);
   return {o, lse};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bwd_core(
     const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& o_, const at::Tensor& dout_,
-    const at::Tensor& lse_, int causal, double scale) {
+    const at::Tensor& lse_, int causal, double scale, Window w) {
   require_bound((const void*)api().bwd);
   check_inputs({{"q", &q_}, {"k", &k_}, {"v", &v_}, {"o", &o_}, {"dout", &dout_}}, q_.scalar_type());
   check_inputs({{"q", &q_}, {"lse", &lse_}}, c10::nullopt);
@@ -222,10 +249,19 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bwd_core(
   at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
   at::Tensor delta = at::empty({(int64_t)d.B, (int64_t)d.N, (int64_t)d.Tq}, q.options().dtype(at::kFloat));
   c10::DeviceGuard guard(q.device());
-  const int status =
-      api().bwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(),
-                lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr<float>(), d.B,
-                d.Tq, d.Tk, d.N, d.Nk, d.H, dtype_code(q.scalar_type()), causal, (float)scale);
+  const int dt = dtype_code(q.scalar_type());
+  int status;
+  if (w.window) {
+    const at::Tensor ws = w.workspace(q, d, causal);
+    status = api().window_bwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                              dout.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                              delta.data_ptr<float>(), data_or_null(ws), d.B, d.Tq, d.Tk, d.N, d.Nk, d.H, dt, causal,
+                              w.window, w.sinks, (float)scale);
+  } else {
+    status = api().bwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(),
+                       lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr<float>(),
+                       d.B, d.Tq, d.Tk, d.N, d.Nk, d.H, dt, causal, (float)scale);
+  }
   check_status(status);
   return {dq, dk, dv, delta};
 }
@@ -234,7 +270,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bwd_core(
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> bwdbwd_core(
     const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& o_, const at::Tensor& dout_,
     const at::Tensor& ddq_, const at::Tensor& ddk_, const at::Tensor& ddv_, const at::Tensor& lse_, int causal,
-    double scale) {
+    double scale, Window w) {
   require_bound((const void*)api().bwdbwd);
   check_inputs({{"q", &q_}, {"k", &k_}, {"v", &v_}, {"o", &o_}, {"dout", &dout_}, {"ddq", &ddq_}, {"ddk", &ddk_},
                 {"ddv", &ddv_}},
@@ -255,11 +291,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> bwdbwd_co
   float* st = stats.data_ptr<float>();
   const int64_t n_stat = (int64_t)d.B * d.N * d.Tq;
   c10::DeviceGuard guard(q.device());
-  const int status = api().bwdbwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                                  dout.data_ptr(), ddq.data_ptr(), ddk.data_ptr(), ddv.data_ptr(),
-                                  lse.data_ptr<float>(), dq2.data_ptr(), dk2.data_ptr(), dv2.data_ptr(),
-                                  ddo.data_ptr(), st, st + n_stat, st + 2 * n_stat, d.B, d.Tq, d.Tk, d.N, d.Nk, d.H,
-                                  dtype_code(q.scalar_type()), causal, (float)scale);
+  const int dt = dtype_code(q.scalar_type());
+  int status;
+  if (w.window) {
+    const at::Tensor ws = w.workspace(q, d, causal);
+    status = api().window_bwdbwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                 dout.data_ptr(), ddq.data_ptr(), ddk.data_ptr(), ddv.data_ptr(),
+                                 lse.data_ptr<float>(), dq2.data_ptr(), dk2.data_ptr(), dv2.data_ptr(),
+                                 ddo.data_ptr(), st, st + n_stat, st + 2 * n_stat, data_or_null(ws), d.B, d.Tq, d.Tk,
+                                 d.N, d.Nk, d.H, dt, causal, w.window, w.sinks, (float)scale);
+  } else {
+    status = api().bwdbwd(current_stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                          dout.data_ptr(), ddq.data_ptr(), ddk.data_ptr(), ddv.data_ptr(), lse.data_ptr<float>(),
+                          dq2.data_ptr(), dk2.data_ptr(), dv2.data_ptr(), ddo.data_ptr(), st, st + n_stat,
+                          st + 2 * n_stat, d.B, d.Tq, d.Tk, d.N, d.Nk, d.H, dt, causal, (float)scale);
+  }
   check_status(status);
   return {dq2, dk2, dv2, ddo, stats};
 }
@@ -285,25 +331,35 @@ struct NoThirdOrder : public torch::autograd::Function<NoThirdOrder> {
   }
 };
 
+void save_mask(AutogradContext* ctx, int64_t causal, double scale, Window w) {
+  ctx->saved_data["causal"] = causal;
+  ctx->saved_data["scale"] = scale;
+  ctx->saved_data["window"] = (int64_t)w.window;
+  ctx->saved_data["sinks"] = (int64_t)w.sinks;
+}
+Window saved_window(AutogradContext* ctx) {
+  return {(int)ctx->saved_data["window"].toInt(), (int)ctx->saved_data["sinks"].toInt()};
+}
+
 // Primal (q, k, v, O, L, dO) -> (dQ, dK, dV), differentiable once in q, k, v
 // and dO: _DotProductAttentionBwd (the rule
 // dot_product_attention_bwd_rule_fwd_rule and its rule
 // dot_product_attention_bwd_rule_bwd_rule).
 struct AttentionBwdFn : public torch::autograd::Function<AttentionBwdFn> {
-  static variable_list forward(AutogradContext* ctx, int64_t causal, double scale, const at::Tensor& q,
-                               const at::Tensor& k, const at::Tensor& v, const at::Tensor& lse, const at::Tensor& o,
-                               const at::Tensor& g) {
-    auto [dq, dk, dv, delta] = bwd_core(q, k, v, o, g, lse, (int)causal, scale);
+  static variable_list forward(AutogradContext* ctx, int64_t causal, double scale, int64_t window, int64_t sinks,
+                               const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& lse,
+                               const at::Tensor& o, const at::Tensor& g) {
+    const Window w{(int)window, (int)sinks};
+    auto [dq, dk, dv, delta] = bwd_core(q, k, v, o, g, lse, (int)causal, scale, w);
     ctx->save_for_backward({q, k, v, o, lse, g});
-    ctx->saved_data["causal"] = causal;
-    ctx->saved_data["scale"] = scale;
+    save_mask(ctx, causal, scale, w);
     return {dq, dk, dv};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list r = ctx->get_saved_variables();  // q, k, v, O, L, dO
     auto [dq2, dk2, dv2, ddo, stats] =
         bwdbwd_core(r[0], r[1], r[2], r[3], r[5], grads[0], grads[1], grads[2], r[4],
-                    (int)ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble());
+                    (int)ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble(), saved_window(ctx));
     if (c10::GradMode::is_enabled() &&
         (grads[0].requires_grad() || grads[1].requires_grad() || grads[2].requires_grad())) {
       auto mark = [](const at::Tensor& t) { return t.detach().requires_grad_(true); };
@@ -311,7 +367,7 @@ struct AttentionBwdFn : public torch::autograd::Function<AttentionBwdFn> {
       dq2 = w[0], dk2 = w[1], dv2 = w[2], ddo = w[3];
     }
     // no cotangent for L and O (flash_hog/jax/_attention_impl.py:278-303)
-    return {at::Tensor(), at::Tensor(), dq2, dk2, dv2, at::Tensor(), at::Tensor(), ddo};
+    return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), dq2, dk2, dv2, at::Tensor(), at::Tensor(), ddo};
   }
 };
 
@@ -320,11 +376,11 @@ struct AttentionBwdFn : public torch::autograd::Function<AttentionBwdFn> {
 // dot_product_attention_bwd_rule, through AttentionBwdFn).
 struct AttentionFn : public torch::autograd::Function<AttentionFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                               int64_t causal, double scale) {
-    auto [o, lse] = fwd_core(q, k, v, (int)causal, scale);
+                               int64_t causal, double scale, int64_t window, int64_t sinks) {
+    const Window w{(int)window, (int)sinks};
+    auto [o, lse] = fwd_core(q, k, v, (int)causal, scale, w);
     ctx->save_for_backward({q, k, v, lse, o});
-    ctx->saved_data["causal"] = causal;
-    ctx->saved_data["scale"] = scale;
+    save_mask(ctx, causal, scale, w);
     ctx->mark_non_differentiable({lse});
     return {o, lse};
   }
@@ -333,10 +389,10 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
     // O enters the first backward as a constant: the double backward returns
     // no cotangent for it, and detaching it keeps this node out of a second
     // derivative's graph.
-    const variable_list d = AttentionBwdFn::apply(ctx->saved_data["causal"].toInt(),
-                                                  ctx->saved_data["scale"].toDouble(), r[0], r[1], r[2], r[3],
-                                                  r[4].detach(), grads[0]);
-    return {d[0], d[1], d[2], at::Tensor(), at::Tensor()};
+    const variable_list d = AttentionBwdFn::apply(
+        ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["window"].toInt(),
+        ctx->saved_data["sinks"].toInt(), r[0], r[1], r[2], r[3], r[4].detach(), grads[0]);
+    return {d[0], d[1], d[2], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
@@ -357,31 +413,32 @@ auto py_call(F&& f) {
 }
 
 std::tuple<at::Tensor, at::Tensor> attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                 int causal, double scale) {
+                                                 int causal, double scale, int window, int sinks) {
   require_bound((const void*)api().fwd);
-  return py_call([&] { return fwd_core(q, k, v, causal, scale); });
+  return py_call([&] { return fwd_core(q, k, v, causal, scale, {window, sinks}); });
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> attention_bwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& dout,
-    const at::Tensor& lse, int causal, double scale) {
+    const at::Tensor& lse, int causal, double scale, int window, int sinks) {
   require_bound((const void*)api().bwd);
-  return py_call([&] { return bwd_core(q, k, v, o, dout, lse, causal, scale); });
+  return py_call([&] { return bwd_core(q, k, v, o, dout, lse, causal, scale, {window, sinks}); });
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> attention_bwdbwd(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& dout,
     const at::Tensor& ddq, const at::Tensor& ddk, const at::Tensor& ddv, const at::Tensor& lse, int causal,
-    double scale) {
+    double scale, int window, int sinks) {
   require_bound((const void*)api().bwdbwd);
-  return py_call([&] { return bwdbwd_core(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale); });
+  return py_call([&] { return bwdbwd_core(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale, {window, sinks}); });
 }
 
 // O of attention(q, k, v) with the autograd nodes above (when q, k or v
 // require grad and grad mode is on).
-at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t causal, double scale) {
+at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t causal, double scale,
+                     int64_t window, int64_t sinks) {
   require_bound((const void*)api().bwdbwd);
-  return py_call([&] { return AttentionFn::apply(q, k, v, causal, scale)[0]; });
+  return py_call([&] { return AttentionFn::apply(q, k, v, causal, scale, window, sinks)[0]; });
 }
 
 }  // namespace
@@ -389,8 +446,14 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "Tensor-level calls of the Flash-HOG C ABI (see flash_hog/_hip.py)";
   m.def("bind", &bind, "bind(fwd, bwd, bwdbwd, last_error, status_string, error_cls): entry-point addresses");
-  m.def("attention_fwd", &attention_fwd);
-  m.def("attention_bwd", &attention_bwd);
-  m.def("attention_bwdbwd", &attention_bwdbwd);
-  m.def("attention", &attention, "attention(q, k, v, causal, scale) -> O, differentiable twice");
+  m.def("bind_window", &bind_window, "bind_window(workspace_bytes, fwd, bwd, bwdbwd): their addresses");
+  using py::arg;
+  m.def("attention_fwd", &attention_fwd, arg("q"), arg("k"), arg("v"), arg("causal"), arg("scale"), arg("window") = 0,
+        arg("sinks") = 0);
+  m.def("attention_bwd", &attention_bwd, arg("q"), arg("k"), arg("v"), arg("o"), arg("dout"), arg("lse"),
+        arg("causal"), arg("scale"), arg("window") = 0, arg("sinks") = 0);
+  m.def("attention_bwdbwd", &attention_bwdbwd, arg("q"), arg("k"), arg("v"), arg("o"), arg("dout"), arg("ddq"),
+        arg("ddk"), arg("ddv"), arg("lse"), arg("causal"), arg("scale"), arg("window") = 0, arg("sinks") = 0);
+  m.def("attention", &attention, "attention(q, k, v, causal, scale) -> O, differentiable twice", arg("q"), arg("k"),
+        arg("v"), arg("causal"), arg("scale"), arg("window") = 0, arg("sinks") = 0);
 }

@@ -54,6 +54,10 @@ SIGNATURES = {
     "fhog_attention_bwdbwd": (_i, [_p] * 17 + [_i] * 8 + [_f]),
     "fhog_attention_bwdbwd_stage": (_i, [_p, _i] + [_p] * 16 + [_i] * 8 + [_f]),
     "fhog_attention_bwdbwd_noalloc": (_i, [_p] * 14 + [_i] * 8 + [_f]),
+    "fhog_window_workspace_bytes": (ctypes.c_size_t, [_i] * 8),
+    "fhog_window_attention_fwd": (_i, [_p] * 6 + [_i] * 10 + [_f]),
+    "fhog_window_attention_bwd": (_i, [_p] * 12 + [_i] * 10 + [_f]),
+    "fhog_window_attention_bwdbwd": (_i, [_p] * 18 + [_i] * 10 + [_f]),
 }
 
 
@@ -107,6 +111,8 @@ def torch_ext():
         addr = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value
         mod.bind(addr(L.fhog_attention_fwd), addr(L.fhog_attention_bwd), addr(L.fhog_attention_bwdbwd),
                  addr(L.fhog_last_error), addr(L.fhog_status_string), FlashHogError)
+        mod.bind_window(addr(L.fhog_window_workspace_bytes), addr(L.fhog_window_attention_fwd),
+                        addr(L.fhog_window_attention_bwd), addr(L.fhog_window_attention_bwdbwd))
     except (ImportError, OSError, AttributeError) as exc:
         warnings.warn(f"Flash-HOG torch extension {TORCH_EXT_PATH} not loaded ({exc}); "
                       "using the Python wrappers", RuntimeWarning, stacklevel=2)
@@ -212,11 +218,29 @@ def attention_supported(batch: int, n_q: int, n_k: int, heads: int, kv_heads: in
     return status == 0, "" if status == 0 else lib().fhog_last_error().decode()
 
 
-def attention_fwd(q, k, v, causal, scale: float):
-    """O (B, T, N, H) in q's dtype and the natural-log logsumexp L (B, N, T) fp32."""
+def _window_args(window: int, sinks: int):
+    """window and sinks as the C ABI's ints; window 0 is none."""
+    window, sinks = int(window), int(sinks)
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError(f"window must be >= 1 (or 0: none) and sinks >= 0 (0 without a window), got {window}, {sinks}")
+    return min(window, (1 << 31) - 1), min(sinks, (1 << 31) - 1)
+
+
+def _window_workspace(q, dims, causal, window, sinks):
+    """Workspace of a windowed backward (fhog_window_workspace_bytes), or None where it needs none."""
+    B, Tq, Tk, _, Nk, Hd = dims
+    size = lib().fhog_window_workspace_bytes(B, Tq, Tk, Nk, Hd, causal_code(causal), window, sinks)
+    return torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
+
+
+def attention_fwd(q, k, v, causal, scale: float, window: int = 0, sinks: int = 0):
+    """O (B, T, N, H) in q's dtype and the natural-log logsumexp L (B, N, T) fp32.
+    window > 0 (here and below; causal masks only): the last `window` keys up to a
+    query's own position and the first `sinks` keys are visible to it."""
+    window, sinks = _window_args(window, sinks)
     ext = torch_ext()
     if ext is not None:
-        return ext.attention_fwd(q, k, v, causal_code(causal), float(scale))
+        return ext.attention_fwd(q, k, v, causal_code(causal), float(scale), window, sinks)
     _check_inputs([("q", q), ("k", k), ("v", v)], q.dtype)
     B, Tq, Tk, N, Nk, Hd = _dims(q, k)
     _expect("v", v, k.shape)
@@ -224,17 +248,21 @@ def attention_fwd(q, k, v, causal, scale: float):
     o = torch.empty_like(q)
     lse = torch.empty((B, N, Tq), device=q.device, dtype=torch.float32)
     with _on_device(q.device):
-        check(lib().fhog_attention_fwd(
-            _stream(q.device), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse),
-            B, Tq, Tk, N, Nk, Hd, DTYPE_CODES[q.dtype], causal_code(causal), float(scale)))
+        args = (_stream(q.device), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse),
+                B, Tq, Tk, N, Nk, Hd, DTYPE_CODES[q.dtype], causal_code(causal))
+        if window:
+            check(lib().fhog_window_attention_fwd(*args, window, sinks, float(scale)))
+        else:
+            check(lib().fhog_attention_fwd(*args, float(scale)))
     return o, lse
 
 
-def attention_bwd(q, k, v, o, dout, lse, causal, scale: float):
+def attention_bwd(q, k, v, o, dout, lse, causal, scale: float, window: int = 0, sinks: int = 0):
     """dQ, dK, dV of attention given its residual; also returns D (B, N, T) fp32."""
+    window, sinks = _window_args(window, sinks)
     ext = torch_ext()
     if ext is not None:
-        return ext.attention_bwd(q, k, v, o, dout, lse, causal_code(causal), float(scale))
+        return ext.attention_bwd(q, k, v, o, dout, lse, causal_code(causal), float(scale), window, sinks)
     _check_inputs([("q", q), ("k", k), ("v", v), ("o", o), ("dout", dout)], q.dtype)
     _check_inputs([("q", q), ("lse", lse)])
     B, Tq, Tk, N, Nk, Hd = _dims(q, k)
@@ -246,20 +274,25 @@ def attention_bwd(q, k, v, o, dout, lse, causal, scale: float):
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     delta = torch.empty((B, N, Tq), device=q.device, dtype=torch.float32)
     with _on_device(q.device):
-        check(lib().fhog_attention_bwd(
-            _stream(q.device), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout), _ptr(lse),
-            _ptr(dq), _ptr(dk), _ptr(dv), _ptr(delta),
-            B, Tq, Tk, N, Nk, Hd, DTYPE_CODES[q.dtype], causal_code(causal), float(scale)))
+        ptrs = (_stream(q.device), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout), _ptr(lse),
+                _ptr(dq), _ptr(dk), _ptr(dv), _ptr(delta))
+        sizes = (B, Tq, Tk, N, Nk, Hd, DTYPE_CODES[q.dtype], causal_code(causal))
+        if window:
+            ws = _window_workspace(q, (B, Tq, Tk, N, Nk, Hd), causal, window, sinks)
+            check(lib().fhog_window_attention_bwd(*ptrs, _ptr(ws), *sizes, window, sinks, float(scale)))
+        else:
+            check(lib().fhog_attention_bwd(*ptrs, *sizes, float(scale)))
     return dq, dk, dv, delta
 
 
 def attention_bwdbwd(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale: float,
-                     return_stats: bool = False):
+                     return_stats: bool = False, window: int = 0, sinks: int = 0):
     """dQ2, dK2, dV2, ddO of the double backward [and the row statistics D, dD, B]."""
+    window, sinks = _window_args(window, sinks)
     ext = torch_ext()
     if ext is not None:
         dq2, dk2, dv2, ddo, stats = ext.attention_bwdbwd(q, k, v, o, dout, ddq, ddk, ddv, lse, causal_code(causal),
-                                                         float(scale))
+                                                         float(scale), window, sinks)
         return (dq2, dk2, dv2, ddo, tuple(stats.unbind(0))) if return_stats else (dq2, dk2, dv2, ddo)
     _check_inputs([("q", q), ("k", k), ("v", v), ("o", o), ("dout", dout),
                    ("ddq", ddq), ("ddk", ddk), ("ddv", ddv)], q.dtype)
@@ -275,12 +308,16 @@ def attention_bwdbwd(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale: float,
     dq2, dk2, dv2, ddo = (torch.empty_like(x) for x in (q, k, v, dout))
     stats = torch.empty((3, B, N, Tq), device=q.device, dtype=torch.float32)
     with _on_device(q.device):
-        check(lib().fhog_attention_bwdbwd(
-            _stream(q.device), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout),
-            _ptr(ddq), _ptr(ddk), _ptr(ddv), _ptr(lse),
-            _ptr(dq2), _ptr(dk2), _ptr(dv2), _ptr(ddo),
-            _ptr(stats[0]), _ptr(stats[1]), _ptr(stats[2]),
-            B, Tq, Tk, N, Nk, Hd, DTYPE_CODES[q.dtype], causal_code(causal), float(scale)))
+        ptrs = (_stream(q.device), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(dout),
+                _ptr(ddq), _ptr(ddk), _ptr(ddv), _ptr(lse),
+                _ptr(dq2), _ptr(dk2), _ptr(dv2), _ptr(ddo),
+                _ptr(stats[0]), _ptr(stats[1]), _ptr(stats[2]))
+        sizes = (B, Tq, Tk, N, Nk, Hd, DTYPE_CODES[q.dtype], causal_code(causal))
+        if window:
+            ws = _window_workspace(q, (B, Tq, Tk, N, Nk, Hd), causal, window, sinks)
+            check(lib().fhog_window_attention_bwdbwd(*ptrs, _ptr(ws), *sizes, window, sinks, float(scale)))
+        else:
+            check(lib().fhog_attention_bwdbwd(*ptrs, *sizes, float(scale)))
     if return_stats:
         return dq2, dk2, dv2, ddo, (stats[0], stats[1], stats[2])
     return dq2, dk2, dv2, ddo

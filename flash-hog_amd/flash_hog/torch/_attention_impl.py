@@ -26,35 +26,45 @@ from flash_hog.torch import _hip_gpu
 _CONFIG = TuningConfig(tile_q=32, tile_k=32, max_concurrent_steps=4)
 
 
-def dot_product_attention_fwd(query, key, value, mask_type: MaskType, scale: float):
-    out, _ = _hip_gpu.flash_fwd(query, key, value, mask_type=mask_type, scale=scale)
+# window and sinks are additions to the reference's rules (dot_product_attention's, window 0
+# for none). The front-end passes them only where there is a window, so that a rule swapped
+# in with the reference's arguments serves every other call.
+
+def dot_product_attention_fwd(query, key, value, mask_type: MaskType, scale: float, window: int = 0, sinks: int = 0):
+    out, _ = _hip_gpu.flash_fwd(query, key, value, mask_type=mask_type, scale=scale, window=window, sinks=sinks)
     return out
 
 
-def dot_product_attention_fwd_rule(query, key, value, mask_type: MaskType, scale: float):
-    out, activation = _hip_gpu.flash_fwd(query, key, value, mask_type=mask_type, scale=scale)
+def dot_product_attention_fwd_rule(query, key, value, mask_type: MaskType, scale: float, window: int = 0,
+                                   sinks: int = 0):
+    out, activation = _hip_gpu.flash_fwd(query, key, value, mask_type=mask_type, scale=scale, window=window,
+                                         sinks=sinks)
     res = (query, key, value, activation, out)
     return out, res
 
 
-def dot_product_attention_bwd_rule(mask_type: MaskType, scale: float, res, g):
+def dot_product_attention_bwd_rule(mask_type: MaskType, scale: float, res, g, window: int = 0, sinks: int = 0):
     query, key, value, activation, out = res
-    return _hip_gpu.flash_bwd(query, key, value, out, g, activation, mask_type=mask_type, scale=scale)
+    return _hip_gpu.flash_bwd(query, key, value, out, g, activation, mask_type=mask_type, scale=scale, window=window,
+                              sinks=sinks)
 
 
-def dot_product_attention_bwd_rule_fwd_rule(mask_type: MaskType, scale: float, res, g):
+def dot_product_attention_bwd_rule_fwd_rule(mask_type: MaskType, scale: float, res, g, window: int = 0,
+                                            sinks: int = 0):
     query, key, value, activation, out = res
     dO = g
-    dQ, dK, dV = dot_product_attention_bwd_rule(mask_type=mask_type, scale=scale, res=res, g=dO)
+    more = {"window": window, "sinks": sinks} if window else {}
+    dQ, dK, dV = dot_product_attention_bwd_rule(mask_type=mask_type, scale=scale, res=res, g=dO, **more)
     residual = (query, key, value, out, activation, dO)
     return (dQ, dK, dV), residual
 
 
-def dot_product_attention_bwd_rule_bwd_rule(mask_type: MaskType, scale: float, res, g):
+def dot_product_attention_bwd_rule_bwd_rule(mask_type: MaskType, scale: float, res, g, window: int = 0,
+                                            sinks: int = 0):
     query, key, value, out, activation, dO = res
     ddQ, ddK, ddV = g
     dQ2, dK2, dV2, ddO = _hip_gpu.flash_bwdbwd(
         Q=query, K=key, V=value, O=out, dO=dO, ddQ=ddQ, ddK=ddK, ddV=ddV, L=activation,
-        mask_type=mask_type, scale=scale, config=_CONFIG)
+        mask_type=mask_type, scale=scale, config=_CONFIG, window=window, sinks=sinks)
     d_res = (dQ2, dK2, dV2, None, None)
     return d_res, ddO

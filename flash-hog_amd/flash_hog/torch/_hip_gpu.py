@@ -39,22 +39,23 @@ Tensor = torch.Tensor
 
 
 @torch.library.custom_op("flash_hog::attention_fwd", mutates_args=())
-def attention_fwd_op(q: Tensor, k: Tensor, v: Tensor, causal: int, scale: float) -> tuple[Tensor, Tensor]:
-    return _hip.attention_fwd(q, k, v, causal, scale)
+def attention_fwd_op(q: Tensor, k: Tensor, v: Tensor, causal: int, scale: float, window: int = 0,
+                     sinks: int = 0) -> tuple[Tensor, Tensor]:
+    return _hip.attention_fwd(q, k, v, causal, scale, window, sinks)
 
 
 @torch.library.custom_op("flash_hog::attention_bwd", mutates_args=())
 def attention_bwd_op(q: Tensor, k: Tensor, v: Tensor, o: Tensor, dout: Tensor, lse: Tensor, causal: int,
-                     scale: float) -> tuple[Tensor, Tensor, Tensor]:
-    dq, dk, dv, _ = _hip.attention_bwd(q, k, v, o, dout, lse, causal, scale)
+                     scale: float, window: int = 0, sinks: int = 0) -> tuple[Tensor, Tensor, Tensor]:
+    dq, dk, dv, _ = _hip.attention_bwd(q, k, v, o, dout, lse, causal, scale, window, sinks)
     return dq, dk, dv
 
 
 @torch.library.custom_op("flash_hog::attention_bwdbwd", mutates_args=())
 def attention_bwdbwd_op(q: Tensor, k: Tensor, v: Tensor, o: Tensor, dout: Tensor, ddq: Tensor, ddk: Tensor,
-                        ddv: Tensor, lse: Tensor, causal: int,
-                        scale: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-    return _hip.attention_bwdbwd(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale)
+                        ddv: Tensor, lse: Tensor, causal: int, scale: float, window: int = 0,
+                        sinks: int = 0) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    return _hip.attention_bwdbwd(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale, window=window, sinks=sinks)
 
 
 def _row_stats(q):
@@ -63,17 +64,17 @@ def _row_stats(q):
 
 
 @attention_fwd_op.register_fake
-def _(q, k, v, causal, scale):
+def _(q, k, v, causal, scale, window=0, sinks=0):
     return torch.empty_like(q), _row_stats(q)
 
 
 @attention_bwd_op.register_fake
-def _(q, k, v, o, dout, lse, causal, scale):
+def _(q, k, v, o, dout, lse, causal, scale, window=0, sinks=0):
     return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
 
 
 @attention_bwdbwd_op.register_fake
-def _(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale):
+def _(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale, window=0, sinks=0):
     return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), torch.empty_like(dout)
 
 
@@ -92,19 +93,20 @@ def _unfold(info, results):
 
 
 @attention_fwd_op.register_vmap
-def _(info, in_dims, q, k, v, causal, scale):
-    return _unfold(info, attention_fwd_op(*_fold(info, in_dims[:3], (q, k, v)), causal, scale))
+def _(info, in_dims, q, k, v, causal, scale, window=0, sinks=0):
+    return _unfold(info, attention_fwd_op(*_fold(info, in_dims[:3], (q, k, v)), causal, scale, window, sinks))
 
 
 @attention_bwd_op.register_vmap
-def _(info, in_dims, q, k, v, o, dout, lse, causal, scale):
-    return _unfold(info, attention_bwd_op(*_fold(info, in_dims[:6], (q, k, v, o, dout, lse)), causal, scale))
+def _(info, in_dims, q, k, v, o, dout, lse, causal, scale, window=0, sinks=0):
+    return _unfold(info, attention_bwd_op(*_fold(info, in_dims[:6], (q, k, v, o, dout, lse)), causal, scale, window,
+                                          sinks))
 
 
 @attention_bwdbwd_op.register_vmap
-def _(info, in_dims, q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale):
+def _(info, in_dims, q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale, window=0, sinks=0):
     args = _fold(info, in_dims[:9], (q, k, v, o, dout, ddq, ddk, ddv, lse))
-    return _unfold(info, attention_bwdbwd_op(*args, causal, scale))
+    return _unfold(info, attention_bwdbwd_op(*args, causal, scale, window, sinks))
 
 
 # ------------------------------------------------------------ kernel calls
@@ -136,8 +138,8 @@ class _FwdKernel(torch.autograd.Function):
     generate_vmap_rule = True
 
     @staticmethod
-    def forward(q, k, v, causal, scale):
-        return attention_fwd_op(q, k, v, causal, scale)
+    def forward(q, k, v, causal, scale, window, sinks):
+        return attention_fwd_op(q, k, v, causal, scale, window, sinks)
 
     setup_context = staticmethod(_mark_outputs)
     backward = _no_derivative("flash_hog_attention_fwd")
@@ -147,8 +149,8 @@ class _BwdKernel(torch.autograd.Function):
     generate_vmap_rule = True
 
     @staticmethod
-    def forward(q, k, v, o, dout, lse, causal, scale):
-        return attention_bwd_op(q, k, v, o, dout, lse, causal, scale)
+    def forward(q, k, v, o, dout, lse, causal, scale, window, sinks):
+        return attention_bwd_op(q, k, v, o, dout, lse, causal, scale, window, sinks)
 
     setup_context = staticmethod(_mark_outputs)
     backward = _no_derivative("flash_hog_attention_bwd")
@@ -158,8 +160,8 @@ class _BwdBwdKernel(torch.autograd.Function):
     generate_vmap_rule = True
 
     @staticmethod
-    def forward(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale):
-        return attention_bwdbwd_op(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale)
+    def forward(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale, window, sinks):
+        return attention_bwdbwd_op(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale, window, sinks)
 
     setup_context = staticmethod(_mark_outputs)
     backward = _no_derivative("flash_hog_attention_bwdbwd")
@@ -180,42 +182,49 @@ def _direct(*tensors) -> bool:
             and all(type(t) is torch.Tensor for t in tensors))
 
 
-def flash_fwd(query, key, value, *, mask_type: MaskType, scale: float | None):
-    """Returns (out, activation): out like query, activation = L (B, N, T) fp32."""
+def flash_fwd(query, key, value, *, mask_type: MaskType, scale: float | None, window: int = 0, sinks: int = 0):
+    """Returns (out, activation): out like query, activation = L (B, N, T) fp32.
+    window and sinks (here and below): those of dot_product_attention, window 0 for none."""
     if query.ndim == 3:
-        out, lse = flash_fwd(*_batchify(query, key, value), mask_type=mask_type, scale=scale)
+        out, lse = flash_fwd(*_batchify(query, key, value), mask_type=mask_type, scale=scale, window=window,
+                             sinks=sinks)
         return out[0], lse[0]
     if _direct(query, key, value):
-        return _hip.attention_fwd(query, key, value, causal_code(mask_type), _default_scale(query, scale))
-    return _FwdKernel.apply(query, key, value, causal_code(mask_type), _default_scale(query, scale))
+        return _hip.attention_fwd(query, key, value, causal_code(mask_type), _default_scale(query, scale), window,
+                                  sinks)
+    return _FwdKernel.apply(query, key, value, causal_code(mask_type), _default_scale(query, scale), window, sinks)
 
 
-def flash_bwd(query, key, value, out, dO, activation, *, mask_type: MaskType, scale: float | None):
+def flash_bwd(query, key, value, out, dO, activation, *, mask_type: MaskType, scale: float | None, window: int = 0,
+              sinks: int = 0):
     """Returns (dQ, dK, dV)."""
     if query.ndim == 3:
-        res = flash_bwd(*_batchify(query, key, value, out, dO, activation), mask_type=mask_type, scale=scale)
+        res = flash_bwd(*_batchify(query, key, value, out, dO, activation), mask_type=mask_type, scale=scale,
+                        window=window, sinks=sinks)
         return tuple(r[0] for r in res)
     if _direct(query, key, value, out, dO, activation):
         return _hip.attention_bwd(query, key, value, out, dO, activation, causal_code(mask_type),
-                                  _default_scale(query, scale))[:3]
+                                  _default_scale(query, scale), window, sinks)[:3]
     return _BwdKernel.apply(query, key, value, out, dO, activation, causal_code(mask_type),
-                            _default_scale(query, scale))
+                            _default_scale(query, scale), window, sinks)
 
 
 def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, *, mask_type: MaskType, scale: float | None,
-                 config: TuningConfig | None = None):
+                 config: TuningConfig | None = None, window: int = 0, sinks: int = 0):
     """Returns (dQ2, dK2, dV2, ddO) (flash_hog/jax/_pallas_gpu.py:51-114).
     config is the reference's tile configuration, accepted and type-checked
     for call compatibility; the HIP kernels' tiles are fixed (TuningConfig)."""
     if config is not None and not isinstance(config, TuningConfig):
         raise TypeError(f"config must be a flash_hog TuningConfig, got {type(config).__name__}")
     if Q.ndim == 3:
-        res = flash_bwdbwd(*_batchify(Q, K, V, O, dO, ddQ, ddK, ddV, L), mask_type=mask_type, scale=scale)
+        res = flash_bwdbwd(*_batchify(Q, K, V, O, dO, ddQ, ddK, ddV, L), mask_type=mask_type, scale=scale,
+                           window=window, sinks=sinks)
         return tuple(r[0] for r in res)
     if _direct(Q, K, V, O, dO, ddQ, ddK, ddV, L):
         return _hip.attention_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal_code(mask_type),
-                                     _default_scale(Q, scale))
-    return _BwdBwdKernel.apply(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal_code(mask_type), _default_scale(Q, scale))
+                                     _default_scale(Q, scale), window=window, sinks=sinks)
+    return _BwdBwdKernel.apply(Q, K, V, O, dO, ddQ, ddK, ddV, L, causal_code(mask_type), _default_scale(Q, scale),
+                               window, sinks)
 
 
 # ------------------------------------------------------------- capability

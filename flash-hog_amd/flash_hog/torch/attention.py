@@ -72,8 +72,17 @@ def kernel_head_dim(dtype, head_dim: int) -> int | None:
     return None
 
 
+def _effective_window(n_q: int, n_k: int, causal_alignment: str, window: int, sinks: int) -> tuple[int, int]:
+    """(window, sinks), or (0, 0) where they hide nothing that the causal mask shows: the
+    causal kernels then compute the same, and faster."""
+    last = n_q - 1 + (n_k - n_q if causal_alignment == "bottom_right" else 0)  # the last query's position
+    if last - window < sinks or sinks >= n_k:
+        return 0, 0
+    return window, sinks
+
+
 def dot_product_attention(query, key, value, is_causal: bool = False, scale: float | None = None, *,
-                          causal_alignment: str = "top_left"):
+                          causal_alignment: str = "top_left", window: int | None = None, sinks: int = 0):
     """Softmax attention over (B, T, N, H) or unbatched (T, N, H) tensors.
 
     Dimensions: T query length, S key/value length, N heads, H head dim
@@ -85,6 +94,12 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     causal diagonal: "top_left" (key s visible to query t iff s <= t, the
     reference kernel's mask) or "bottom_right" (s <= t + S - T, the mask of
     flash_hog/_jax_refs/jax_impl.py:104-109); they agree when T == S.
+
+    window and sinks (additions as well, with is_causal only) narrow the mask to a sliding
+    window: a query at position p (t, or t + S - T with "bottom_right") sees the `window`
+    keys p - window < s <= p, itself among them, and besides these the first `sinks` keys
+    (s < sinks, s <= p). Work grows with T * window, memory with T + S, in all three
+    derivatives. A query that sees no key gives zeros.
 
     Like the reference's kernel, any head dim H >= 1 works up to the largest
     one the kernels take (256 for bf16 and fp16, 128 for fp32); head dims the
@@ -98,13 +113,24 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     if padded is not None and padded != head_dim and key.shape[-1] == value.shape[-1] == head_dim:
         pad = lambda t: torch.nn.functional.pad(t, (0, padded - head_dim))
         out = dot_product_attention(pad(query), pad(key), pad(value), is_causal, scale,
-                                    causal_alignment=causal_alignment)
+                                    causal_alignment=causal_alignment, window=window, sinks=sinks)
         return out[..., :head_dim]
     dtype = query.dtype
     if not (dtype == key.dtype == value.dtype):
         raise ValueError(f"query, key and value must share a dtype, got {query.dtype}, {key.dtype}, {value.dtype}")
     if causal_alignment not in ("top_left", "bottom_right"):
         raise ValueError(f"causal_alignment must be 'top_left' or 'bottom_right', got {causal_alignment!r}")
+    if window is None:
+        if sinks != 0:
+            raise ValueError(f"sinks needs a window, got sinks={sinks}")
+        window = 0
+    else:
+        if not is_causal:
+            raise ValueError("window needs is_causal=True")
+        if window < 1 or sinks < 0:
+            raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
+        if query.ndim in (3, 4) and key.ndim == query.ndim:
+            window, sinks = _effective_window(query.shape[-3], key.shape[-3], causal_alignment, window, sinks)
     if not is_causal:
         mask_type = MaskType.NO_MASK
     elif causal_alignment == "top_left":
@@ -116,10 +142,11 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
         query, key, value = query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0)
     native = _native_path(query, key, value)
     if native is not None:
-        result = native.attention(query, key, value, causal_code(mask_type), float(scale))
+        result = native.attention(query, key, value, causal_code(mask_type), float(scale),
+                                  *_hip._window_args(window, sinks))
     else:
         fn = _DotProductAttention if torch._C._are_functorch_transforms_active() else _DotProductAttentionEager
-        result, _ = fn.apply(query, key, value, mask_type, float(scale))
+        result, _ = fn.apply(query, key, value, mask_type, float(scale), window, sinks)
     if unbatched:
         result = result.squeeze(0)
     return result
@@ -130,6 +157,11 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
 # with them; under vmap the kernels' own vmap rules fold the mapped axis into
 # the batch axis (flash_hog/torch/_hip_gpu.py).
 
+def _window_kwargs(window, sinks):
+    """The rules' arguments beyond the reference's, where there is a window."""
+    return {"window": window, "sinks": sinks} if window else {}
+
+
 class _DotProductAttention(torch.autograd.Function):
     """Primal: (q, k, v) -> (O, L); L = activation, the fwd rule's residual
     (attention.py:64-72), is returned so that it can be saved, and is not
@@ -138,20 +170,21 @@ class _DotProductAttention(torch.autograd.Function):
     generate_vmap_rule = True
 
     @staticmethod
-    def forward(query, key, value, mask_type, scale):
+    def forward(query, key, value, mask_type, scale, window, sinks):
         out, (_, _, _, activation, _) = attn_impl.dot_product_attention_fwd_rule(
-            query, key, value, mask_type=mask_type, scale=scale)
+            query, key, value, mask_type=mask_type, scale=scale, **_window_kwargs(window, sinks))
         return out, activation
 
     @staticmethod
     def setup_context(ctx, inputs, output):
-        query, key, value, mask_type, scale = inputs
+        query, key, value, mask_type, scale, window, sinks = inputs
         out, activation = output
         # the residual (q, k, v, L, O) of dot_product_attention_fwd_rule
         ctx.save_for_backward(query, key, value, activation, out)
         ctx.mark_non_differentiable(activation)
         ctx.mask_type = mask_type
         ctx.scale = scale
+        ctx.window, ctx.sinks = window, sinks
 
     @staticmethod
     def backward(ctx, g, _g_activation):
@@ -161,8 +194,8 @@ class _DotProductAttention(torch.autograd.Function):
         # graph of a second derivative, which would otherwise call it again with
         # a zero cotangent.
         fn = _DotProductAttentionBwd if torch._C._are_functorch_transforms_active() else _DotProductAttentionBwdEager
-        dq, dk, dv = fn.apply(ctx.mask_type, ctx.scale, q, k, v, activation, o.detach(), g)
-        return dq, dk, dv, None, None
+        dq, dk, dv = fn.apply(ctx.mask_type, ctx.scale, q, k, v, activation, o.detach(), g, ctx.window, ctx.sinks)
+        return dq, dk, dv, None, None, None, None
 
 
 class _DotProductAttentionBwd(torch.autograd.Function):
@@ -171,18 +204,20 @@ class _DotProductAttentionBwd(torch.autograd.Function):
     generate_vmap_rule = True
 
     @staticmethod
-    def forward(mask_type, scale, query, key, value, activation, out, g):
+    def forward(mask_type, scale, query, key, value, activation, out, g, window, sinks):
         (dq, dk, dv), _ = attn_impl.dot_product_attention_bwd_rule_fwd_rule(
-            mask_type=mask_type, scale=scale, res=(query, key, value, activation, out), g=g)
+            mask_type=mask_type, scale=scale, res=(query, key, value, activation, out), g=g,
+            **_window_kwargs(window, sinks))
         return dq, dk, dv
 
     @staticmethod
     def setup_context(ctx, inputs, output):
-        mask_type, scale, query, key, value, activation, out, g = inputs
+        mask_type, scale, query, key, value, activation, out, g, window, sinks = inputs
         # the residual (q, k, v, O, L, dO) of dot_product_attention_bwd_rule_fwd_rule
         ctx.save_for_backward(query, key, value, out, activation, g)
         ctx.mask_type = mask_type
         ctx.scale = scale
+        ctx.window, ctx.sinks = window, sinks
 
     @staticmethod
     @once_differentiable
@@ -191,8 +226,9 @@ class _DotProductAttentionBwd(torch.autograd.Function):
         # of this backward raise if differentiated again.
         res = ctx.saved_tensors
         (dq2, dk2, dv2, _, _), ddo = attn_impl.dot_product_attention_bwd_rule_bwd_rule(
-            mask_type=ctx.mask_type, scale=ctx.scale, res=res, g=(ddq, ddk, ddv))
-        return None, None, dq2, dk2, dv2, None, None, ddo
+            mask_type=ctx.mask_type, scale=ctx.scale, res=res, g=(ddq, ddk, ddv),
+            **_window_kwargs(ctx.window, ctx.sinks))
+        return None, None, dq2, dk2, dv2, None, None, ddo, None, None
 
 
 # The same two Functions in the ctx-first form. Function.apply binds a
@@ -203,9 +239,9 @@ class _DotProductAttentionBwd(torch.autograd.Function):
 
 class _DotProductAttentionEager(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, mask_type, scale):
-        output = _DotProductAttention.forward(query, key, value, mask_type, scale)
-        _DotProductAttention.setup_context(ctx, (query, key, value, mask_type, scale), output)
+    def forward(ctx, query, key, value, mask_type, scale, window, sinks):
+        output = _DotProductAttention.forward(query, key, value, mask_type, scale, window, sinks)
+        _DotProductAttention.setup_context(ctx, (query, key, value, mask_type, scale, window, sinks), output)
         return output
 
     backward = _DotProductAttention.backward
@@ -213,9 +249,10 @@ class _DotProductAttentionEager(torch.autograd.Function):
 
 class _DotProductAttentionBwdEager(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, mask_type, scale, query, key, value, activation, out, g):
-        output = _DotProductAttentionBwd.forward(mask_type, scale, query, key, value, activation, out, g)
-        _DotProductAttentionBwd.setup_context(ctx, (mask_type, scale, query, key, value, activation, out, g), output)
+    def forward(ctx, mask_type, scale, query, key, value, activation, out, g, window, sinks):
+        args = (mask_type, scale, query, key, value, activation, out, g, window, sinks)
+        output = _DotProductAttentionBwd.forward(*args)
+        _DotProductAttentionBwd.setup_context(ctx, args, output)
         return output
 
     backward = _DotProductAttentionBwd.backward

@@ -187,6 +187,45 @@ int fhog_attention_bwdbwd_noalloc(fhog_stream_t stream,
                                   int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim,
                                   int dtype, int causal, float scale);
 
+/*
+ * Attention over a window of keys with sinks: with p = i (causal 1, top-left) or
+ * p = i + n_k - n_q (causal 2, bottom-right; causal 0 is invalid), query i sees key j iff
+ * j <= p and (j > p - window or j < sinks), window >= 1, sinks >= 0. Everything else is as
+ * in the entry points of the same name without a window, the double backward included; a
+ * query that sees no key (also top-left, n_q > n_k, behind the last key's window) gets o = 0,
+ * lse = +inf and zero gradients. These have no counterpart in the reference.
+ * Work and memory grow with n_q * window and n_q + n_k.
+ *
+ * workspace (caller-owned, 16-byte aligned, fhog_window_workspace_bytes; may be null when
+ * that is 0, as without sinks): fp32 parts of the sinks' dk and dv rows, scratch between the
+ * kernels of one call. Calls that may overlap need one each.
+ */
+size_t fhog_window_workspace_bytes(int batch, int n_q, int n_k, int kv_heads, int head_dim, int causal, int window,
+                                   int sinks);
+
+int fhog_window_attention_fwd(fhog_stream_t stream,
+                              const void* q, const void* k, const void* v,
+                              void* o, float* lse,
+                              int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim,
+                              int dtype, int causal, int window, int sinks, float scale);
+
+int fhog_window_attention_bwd(fhog_stream_t stream,
+                              const void* q, const void* k, const void* v,
+                              const void* o, const void* dout, const float* lse,
+                              void* dq, void* dk, void* dv, float* delta, void* workspace,
+                              int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim,
+                              int dtype, int causal, int window, int sinks, float scale);
+
+int fhog_window_attention_bwdbwd(fhog_stream_t stream,
+                                 const void* q, const void* k, const void* v,
+                                 const void* o, const void* dout,
+                                 const void* ddq, const void* ddk, const void* ddv,
+                                 const float* lse,
+                                 void* dq2, void* dk2, void* dv2, void* ddo,
+                                 float* delta, float* ddelta, float* bstat, void* workspace,
+                                 int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim,
+                                 int dtype, int causal, int window, int sinks, float scale);
+
 #ifdef __cplusplus
 }
 #endif
