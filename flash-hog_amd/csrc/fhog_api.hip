@@ -13,6 +13,7 @@
 
 #include "flash_hog.h"
 #include "fhog_params.h"
+#include "fhog_paged.h"
 
 namespace {
 
@@ -147,6 +148,73 @@ int check_workspace(const char* who, const Window& w, const void* workspace) {
   if (w.sink.chunks > 0 && !aligned(workspace, 16))
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null or not 16-byte aligned", who);
   return FHOG_OK;
+}
+
+}  // namespace
+
+namespace {
+
+// What the three paged entry points share. `rows`: the packed rows (attention, write).
+struct Paged {
+  int batch, rows, heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype;
+};
+
+int check_paged(const Paged& s, const char* who) {
+  if (s.batch < 0 || s.rows < 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sizes must not be negative", who);
+  if (s.heads < 1 || s.kv_heads < 1 || s.num_pages < 1 || s.pages_per_seq < 1)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sizes must be >= 1 (heads=%d kv_heads=%d num_pages=%d pages_per_seq=%d)",
+                who, s.heads, s.kv_heads, s.num_pages, s.pages_per_seq);
+  if (s.heads % s.kv_heads != 0)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: heads (%d) must be a multiple of kv_heads (%d)", who, s.heads,
+                s.kv_heads);
+  if (s.page_size < 16 || (s.page_size & (s.page_size - 1)) != 0)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: page_size must be a power of two >= 16, got %d", who, s.page_size);
+  if (s.dtype != FHOG_DTYPE_F16 && s.dtype != FHOG_DTYPE_BF16)
+    return fail(FHOG_ERR_UNSUPPORTED, "%s: dtype must be bf16 or fp16, got %d", who, s.dtype);
+  if (s.cache_dtype != s.dtype && s.cache_dtype != FHOG_DTYPE_E4M3)
+    return fail(FHOG_ERR_UNSUPPORTED, "%s: the cache must be of dtype %d or e4m3, got %d", who, s.dtype, s.cache_dtype);
+  if (s.head_dim != 64 && s.head_dim != 128 && s.head_dim != 256)
+    return fail(FHOG_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256, got %d", who, s.head_dim);
+  // packed (token, head) rows and positions are ints, a launch's threads 32 bits
+  if ((long long)s.rows * s.heads >= (1ll << 30) || s.batch >= (1 << 24) ||
+      (long long)s.pages_per_seq * s.page_size > (1ll << 30))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  return FHOG_OK;
+}
+
+int check_cache(const char* who, const Paged& s, const void* k, const void* v, const void* ks, const void* vs,
+                const void* table, const void* lengths) {
+  if (int st = check_ptrs(who, {{"k_cache", k}, {"v_cache", v}}, {{"page_table", table}, {"lengths", lengths}}))
+    return st;
+  if (s.cache_dtype == FHOG_DTYPE_E4M3 && (ks == nullptr || vs == nullptr))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: an e4m3 cache needs k_scale and v_scale", who);
+  return FHOG_OK;
+}
+
+fhog::CacheShape cache_shape(const Paged& s, const int* table, const int* lengths, const int* offsets) {
+  return fhog::CacheShape{table, lengths, offsets, s.batch, s.rows, s.kv_heads, s.num_pages,
+                          __builtin_ctz((unsigned)s.page_size), s.pages_per_seq};
+}
+
+// Calls f.template operator()<T, C, D>() for the runtime (dtype, cache_dtype, head_dim).
+template <typename F> hipError_t dispatch_paged(const Paged& s, F&& f) {
+  auto dim = [&]<typename T, typename C>() {
+    if (s.head_dim == 64) return f.template operator()<T, C, 64>();
+    if (s.head_dim == 128) return f.template operator()<T, C, 128>();
+    return f.template operator()<T, C, 256>();
+  };
+  const bool quantised = s.cache_dtype == FHOG_DTYPE_E4M3;
+  if (s.dtype == FHOG_DTYPE_BF16)
+    return quantised ? dim.template operator()<__bf16, fhog::e4m3>() : dim.template operator()<__bf16, __bf16>();
+  return quantised ? dim.template operator()<_Float16, fhog::e4m3>() : dim.template operator()<_Float16, _Float16>();
+}
+
+int compute_units() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    return 0;
+  return cus;
 }
 
 }  // namespace
@@ -416,6 +484,103 @@ int fhog_window_attention_bwdbwd(fhog_stream_t stream, const void* q, const void
     return fhog::launch_window_bwdbwd<T, D>(p, (hipStream_t)stream);
   };
   return launch_status(dispatch(dtype, head_dim, run), who);
+}
+
+size_t fhog_paged_workspace_bytes(int batch, int total, int single, int heads, int kv_heads, int head_dim,
+                                  int page_size, int pages_per_seq, int window, int sinks) {
+  const Paged s{batch, total, heads, kv_heads, head_dim, 1, page_size, pages_per_seq, FHOG_DTYPE_BF16, FHOG_DTYPE_BF16};
+  if (check_paged(s, "fhog_paged_workspace_bytes") || window < 0 || sinks < 0 || batch < 1 || total < 1) return 0;
+  const fhog::PagedPlan plan = fhog::paged_plan(batch, total, single != 0, heads, kv_heads,
+                                                (long)page_size * pages_per_seq, window, sinks, compute_units());
+  return (size_t)plan.parts * (head_dim + 2) * sizeof(float);
+}
+
+int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                         const void* k_scale, const void* v_scale, const int* page_table, const int* lengths,
+                         const int* query_offsets, void* out, void* workspace, size_t workspace_bytes, int batch,
+                         int total, int heads, int kv_heads, int head_dim, int num_pages, int page_size,
+                         int pages_per_seq, int dtype, int cache_dtype, int window, int sinks, int clear_tail,
+                         float scale) {
+  static const char* who = "fhog_paged_attention";
+  const Paged s{batch, total, heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype};
+  if (int st = check_paged(s, who)) return st;
+  if (!(scale == scale) || scale - scale != 0.0f)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: scale must be finite", who);
+  if (scale == 0.0f) return fail(FHOG_ERR_UNSUPPORTED, "%s: scale must be nonzero", who);
+  if (window < 0 || sinks < 0 || (sinks > 0 && window == 0))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: window must be >= 1 (or 0: none) and sinks >= 0 (0 without a window)", who);
+  if (query_offsets == nullptr && total != batch)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: without query_offsets there is one row a sequence: %d rows, %d sequences",
+                who, total, batch);
+  if (total == 0) return ok();
+  if (batch == 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: rows without a sequence", who);
+  if (int st = check_ptrs(who, {{"q", q}, {"out", out}}, {})) return st;
+  if (int st = check_cache(who, s, k_cache, v_cache, k_scale, v_scale, page_table, lengths)) return st;
+  if (query_offsets != nullptr && !aligned(query_offsets, 4))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: query_offsets is not 4-byte aligned", who);
+  const int most = 1 << 30;  // (positions are below it)
+  if (window > most) window = most;
+  if (sinks > most) sinks = most;
+  const fhog::PagedPlan plan = fhog::paged_plan(batch, total, query_offsets == nullptr, heads, kv_heads,
+                                                (long)page_size * pages_per_seq, window, sinks, compute_units());
+  if ((long long)plan.slots * kv_heads >= (1ll << 31) || plan.splits > 65535)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  const size_t need = (size_t)plan.parts * (head_dim + 2) * sizeof(float);
+  if (need > 0 && (!aligned(workspace, 16) || workspace_bytes < need))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null, not 16-byte aligned or below its %zu bytes", who, need);
+  auto run = [&]<typename T, typename C, int D>() {
+    fhog::PagedParams<T, C> p{(const T*)q, (T*)out,
+                              {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
+                              cache_shape(s, page_table, lengths, query_offsets), (float*)workspace, heads, window,
+                              sinks, plan.slots, plan.splits, plan.split_tiles, clear_tail, scale};
+    return fhog::launch_paged_attention<T, C, D>(p, plan.chunk, (hipStream_t)stream);
+  };
+  return launch_status(dispatch_paged(s, run), who);
+}
+
+int fhog_paged_cache_write(fhog_stream_t stream, const void* k, const void* v, void* k_cache, void* v_cache,
+                           void* k_scale, void* v_scale, const int* page_table, const int* lengths,
+                           const int* query_offsets, int batch, int total, int kv_heads, int head_dim, int num_pages,
+                           int page_size, int pages_per_seq, int dtype, int cache_dtype) {
+  static const char* who = "fhog_paged_cache_write";
+  const Paged s{batch, total, kv_heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype};
+  if (int st = check_paged(s, who)) return st;
+  if (query_offsets == nullptr && total != batch)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: without query_offsets there is one row a sequence: %d rows, %d sequences",
+                who, total, batch);
+  if (total == 0 || batch == 0) return ok();
+  if (int st = check_ptrs(who, {{"k", k}, {"v", v}}, {})) return st;
+  if (int st = check_cache(who, s, k_cache, v_cache, k_scale, v_scale, page_table, lengths)) return st;
+  if (query_offsets != nullptr && !aligned(query_offsets, 4))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: query_offsets is not 4-byte aligned", who);
+  auto run = [&]<typename T, typename C, int D>() {
+    fhog::CacheWriteParams<T, C> p{(const T*)k, (const T*)v, (C*)k_cache, (C*)v_cache, (uint8_t*)k_scale,
+                                   (uint8_t*)v_scale, cache_shape(s, page_table, lengths, query_offsets)};
+    return fhog::launch_cache_write<T, C, D>(p, (hipStream_t)stream);
+  };
+  return launch_status(dispatch_paged(s, run), who);
+}
+
+int fhog_paged_cache_read(fhog_stream_t stream, const void* k_cache, const void* v_cache, const void* k_scale,
+                          const void* v_scale, const int* page_table, const int* lengths, void* k, void* v, int batch,
+                          int max_length, int kv_heads, int head_dim, int num_pages, int page_size,
+                          int pages_per_seq, int dtype, int cache_dtype) {
+  static const char* who = "fhog_paged_cache_read";
+  const Paged s{batch, 0, kv_heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype};
+  if (int st = check_paged(s, who)) return st;
+  if (max_length < 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sizes must not be negative", who);
+  if ((double)batch * max_length * kv_heads * head_dim >= 2048.0 * (1ll << 31))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  if (batch == 0 || max_length == 0) return ok();
+  if (int st = check_ptrs(who, {{"k", k}, {"v", v}}, {})) return st;
+  if (int st = check_cache(who, s, k_cache, v_cache, k_scale, v_scale, page_table, lengths)) return st;
+  auto run = [&]<typename T, typename C, int D>() {
+    fhog::CacheReadParams<T, C> p{
+        {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
+        (T*)k, (T*)v, cache_shape(s, page_table, lengths, nullptr), max_length};
+    return fhog::launch_cache_read<T, C, D>(p, (hipStream_t)stream);
+  };
+  return launch_status(dispatch_paged(s, run), who);
 }
 
 }  // extern "C"

@@ -413,4 +413,38 @@ inline int sink_chunks(Mask m, int window, int sinks) {
   return sinks > 0 && first < m.nq ? (int)((m.nq - begin + step - 1) / step) : 0;
 }
 
+// Paged attention: which kernel, how many tiles of rows ("slots") and how a sequence's keys are
+// split. `single`: one new token a sequence, no offsets.
+struct PagedPlan {
+  bool chunk;       // 128-row tiles (paged_chunk_kernel), else 16 (paged_token_kernel)
+  int rows, slots;
+  int splits, split_tiles;  // splits of split_tiles 32-key tiles; one split: no join
+  long parts;       // fp32 rows of head_dim + 2 in the workspace
+};
+inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv_heads, long capacity, int window,
+                            int sinks, int cus) {
+  if (cus <= 0) cus = 256;
+  PagedPlan p;
+  const int group = heads / kv_heads;
+  // More than 16 rows a sequence on average (tokens times heads of a group): the wide tile.
+  p.chunk = (long)total * group > 16l * batch;
+  p.rows = p.chunk ? 128 : 16;
+  p.slots = (int)(single ? (long)batch * ((group + p.rows - 1) / p.rows) : (long)total * group / p.rows + batch);
+  // The most tiles that a tile of rows reads: with a window its keys, those between the tile's
+  // first and last position and the sinks.
+  long keys = capacity;
+  if (window > 0) {
+    const long most = (long)window + p.rows / group + 1 + sinks;
+    if (most < keys) keys = most;
+  }
+  const long tiles = (keys + 31) / 32 + 2;
+  const long blocks = (long)p.slots * kv_heads, target = (p.chunk ? 2l : 4l) * cus;
+  long split_tiles = blocks >= target ? tiles : (tiles * blocks + target - 1) / target;
+  if (split_tiles < 8) split_tiles = 8;
+  p.splits = (int)((tiles + split_tiles - 1) / split_tiles);
+  p.split_tiles = (int)split_tiles;
+  p.parts = p.splits > 1 ? blocks * p.splits * p.rows : 0;
+  return p;
+}
+
 }  // namespace fhog

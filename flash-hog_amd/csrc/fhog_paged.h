@@ -1,0 +1,204 @@
+// The paged key/value cache: parameter blocks, launch rules and the device code that its
+// kernels share.
+//
+// A cache is (pages, kv_heads, page_size, head_dim): the rows of one head in a page are
+// contiguous, so a workgroup that serves one key/value head reads whole lines. Page sizes
+// are powers of two from 16 on, so that 16 keys from a multiple of 16 on never leave a page.
+// Token s of sequence b is row s % page_size of page table[b][s / page_size].
+//
+// The new tokens of all sequences are packed: sequence b's are rows offsets[b] to
+// offsets[b + 1], or row b alone without offsets, and its last `rows` positions: token i
+// of its n new ones is at position lengths[b] - n + i.
+//
+// Nothing on the device is trusted: a table entry outside [0, pages) or a length beyond the
+// table's capacity makes the output rows that depend on it NaN (attention, reading) or is
+// skipped (writing); offsets are cut to [0, total]. No access leaves its tensor.
+//
+// An e4m3 cache has an e8m0 scale for each key and value row, (pages, kv_heads, page_size):
+// the row's values are code * 2^(scale byte - 127).
+#pragma once
+
+#include "fhog_device.h"
+
+namespace fhog {
+
+struct e4m3 {  // one byte of an e4m3 cache
+  uint8_t byte;
+};
+
+struct CacheShape {
+  const int* table;    // (batch, pages_per_seq)
+  const int* lengths;  // (batch)
+  const int* offsets;  // (batch + 1), or null: one new token each
+  int batch, total;    // sequences, packed rows
+  int kv_heads, pages, page_shift, pages_per_seq;
+};
+
+template <typename C> struct CacheRows {
+  const C* k;
+  const C* v;
+  const uint8_t* k_scale;  // e4m3 only
+  const uint8_t* v_scale;
+};
+
+template <typename T, typename C> struct PagedParams {
+  const T* q;
+  T* out;
+  CacheRows<C> cache;
+  CacheShape at;
+  float* parts;  // fp32 outputs of the splits, (slot, kv_head, split, row of the tile, head_dim), and their m, l
+  int heads, window, sinks;  // window 0: none
+  int slots, splits, split_tiles;
+  int clear_tail;  // whether rows behind the last sequence are zeroed
+  float scale;
+};
+
+template <typename T, typename C> struct CacheWriteParams {
+  const T* k;
+  const T* v;
+  C* k_cache;
+  C* v_cache;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  CacheShape at;
+};
+
+template <typename T, typename C> struct CacheReadParams {
+  CacheRows<C> cache;
+  T* k;
+  T* v;
+  CacheShape at;
+  int max_length;
+};
+
+template <typename T, typename C, int D> hipError_t launch_paged_attention(const PagedParams<T, C>& p, bool chunk, hipStream_t s);
+template <typename T, typename C, int D> hipError_t launch_cache_write(const CacheWriteParams<T, C>& p, hipStream_t s);
+template <typename T, typename C, int D> hipError_t launch_cache_read(const CacheReadParams<T, C>& p, hipStream_t s);
+
+// ---------------------------------------------------------------------------
+// Packed rows and their sequences.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int packed_begin(const CacheShape& c, int b) {
+  return c.offsets ? min(max(c.offsets[b], 0), c.total) : b;
+}
+
+// The last sequence whose first slot is at or before `slot`, where a sequence's slots start
+// at offset * group / tile + index (PagedPlan); any answer in range if offsets do not rise.
+template <typename F> __device__ __forceinline__ int last_at_or_before(int count, int slot, F&& first_slot) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_slot(mid) <= slot)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of cached rows: fetched from their pages into registers, 16 bytes of cache a thread
+// and load, and stored to LDS as T, swizzled, where the matrix operands are read. e4m3 rows
+// are scaled in between; the scale is a power of two, so bf16 holds the product exactly and
+// fp16 wherever its range does.
+// ---------------------------------------------------------------------------
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Four e4m3 values (the bytes of x) times a power of two, as T.
+template <typename T> __device__ __forceinline__ V4<T> dequantise4(uint32_t x, float scale) {
+  u32x2 y;
+  if constexpr (std::is_same_v<T, __bf16>) {
+    y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, false));
+    y[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, true));
+  } else {
+    y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, false));
+    y[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, true));
+  }
+  return __builtin_bit_cast(V4<T>, y);
+}
+// The power of two that an e8m0 code stands for.
+__device__ __forceinline__ float scale_of(uint32_t code) { return __builtin_bit_cast(float, code << 23); }
+
+template <typename T, typename C, int D, int THREADS, int SWZ> struct PageTile {
+  static constexpr bool kQuantised = sizeof(C) == 1;
+  static constexpr int kPerLoad = 16 / (int)sizeof(C);  // elements
+  static constexpr int kChunks = D / kPerLoad;          // 16-byte pieces of a row
+  static constexpr int kTensor = 32 * kChunks;          // of a tile of one tensor
+  static constexpr int kLoads = 2 * kTensor / THREADS;  // a thread's, keys and values
+  static constexpr int kTileBytes = 32 * D * (int)sizeof(T);
+  static_assert(2 * kTensor % THREADS == 0, "tile must divide into whole loads");
+  u32x4 data[kLoads];
+  uint32_t code[kQuantised ? kLoads : 1];
+
+  // Rows [rlo, rhi] of the 32 keys from k0 (a multiple of 16) on; rows outside repeat the
+  // nearest of them, so that what no token has written is never read. page[h] is the
+  // page of keys k0 + 16 h and on.
+  __device__ __forceinline__ void fetch(const CacheRows<C>& cache, int hk, int kv_heads, int page_shift, int k0,
+                                        int rlo, int rhi, int page0, int page1, int thread) {
+    const int page_rows = 1 << page_shift;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * THREADS + thread;
+      const bool value = at >= kTensor;
+      const int row = min(max(at % kTensor / kChunks, rlo), rhi);
+      const long head = (long)(row < 16 ? page0 : page1) * kv_heads + hk;
+      const long line = (head << page_shift) + ((k0 + row) & (page_rows - 1));
+      const C* src = (value ? cache.v : cache.k) + line * D + at % kChunks * kPerLoad;
+      data[i] = *reinterpret_cast<const u32x4*>(src);
+      if constexpr (kQuantised) code[i] = (value ? cache.v_scale : cache.k_scale)[line];
+    }
+  }
+
+  // To LDS: the tile of keys at byte address lds, that of values behind it.
+  __device__ __forceinline__ void store(uint32_t lds, int thread) const {
+    typedef __attribute__((address_space(3))) char lds_char;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * THREADS + thread;
+      const int row = at % kTensor / kChunks, chunk = at % kChunks;
+      const uint32_t base = lds + (at >= kTensor ? kTileBytes : 0) + row * D * (int)sizeof(T);
+      auto put = [&](int c, u32x4 x) {
+        *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(
+            reinterpret_cast<lds_char*>((uintptr_t)(base + 16 * phys_chunk<SWZ>(row, c)))) = x;
+      };
+      if constexpr (kQuantised) {
+        const float scale = scale_of(code[i]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const V4<T> a = dequantise4<T>(data[i][2 * h], scale), b = dequantise4<T>(data[i][2 * h + 1], scale);
+          put(2 * chunk + h, __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)));
+        }
+      } else {
+        put(chunk, data[i]);
+      }
+    }
+  }
+};
+
+// The keys that a tile of rows of one sequence reads, as 32-key tiles: those that are visible
+// as sinks only, then those from its first row's window to its last row's position.
+struct PageSpan {
+  int sink_keys, sink_tiles;  // keys [0, sink_keys)
+  int lo, hi;                 // keys [lo, hi)
+  int start;                  // lo, down to a multiple of 16
+  int tiles;
+
+  __device__ __forceinline__ PageSpan(int first_pos, int last_pos, int length, int window, int sinks) {
+    hi = max(0, min(length, last_pos + 1));
+    lo = window ? min(max(0, first_pos - window + 1), hi) : 0;
+    sink_keys = window ? max(0, min(sinks, lo)) : 0;
+    sink_tiles = (sink_keys + 31) / 32;
+    start = lo & ~15;
+    tiles = sink_tiles + (hi - start + 31) / 32;
+    if (hi == 0) tiles = sink_tiles = 0;
+  }
+  // First key of tile t, and the first and last of its rows that are read.
+  __device__ __forceinline__ int key(int t) const { return t < sink_tiles ? 32 * t : start + 32 * (t - sink_tiles); }
+  __device__ __forceinline__ int first_row(int t) const { return t < sink_tiles ? 0 : max(0, lo - key(t)); }
+  __device__ __forceinline__ int last_row(int t) const {
+    return min(31, (t < sink_tiles ? sink_keys : hi) - 1 - key(t));
+  }
+};
+
+}  // namespace fhog

@@ -1,0 +1,487 @@
+// Attention of new tokens over a paged key/value cache (fhog_paged.h): O = softmax(scale q K^T) V
+// for the packed new tokens of several sequences, each against its own sequence's cached
+// keys up to its own position, optionally the last `window` of them and the first `sinks`.
+//
+// Query heads that share a key/value head are taken together: row r of a sequence's tile is
+// token r / group, head r % group, so a cached row is read once for the whole group.
+// Scores are formed transposed (keys x rows), so that a lane holds one row's scores, and
+// the output as O^T = V^T P^T, as in the dense forward; one sweep with the running maximum
+// and sum, rescaled only when a row's probabilities exceed 2^8.
+//
+// paged_token_kernel, for few rows a sequence: 16 rows a workgroup, whose waves take every
+// kWaves-th tile of 32 keys each on their own, through LDS of their own (no barrier in
+// the sweep), and join at the end.
+// paged_chunk_kernel, for many: 128 rows a workgroup, 32 a wave, all on the same tile.
+//
+// Where tiles of rows are few, a sequence's keys are dealt to several workgroups (splits of
+// split_tiles tiles), which leave unnormalised fp32 outputs with their maxima and sums;
+// paged_join_kernel joins them in order. The number of splits follows from sizes that the
+// host knows (no length is read back), so a call can be captured; workgroups of splits
+// beyond a sequence's end leave at once.
+#include "fhog_paged.h"
+
+namespace fhog {
+
+namespace {
+
+constexpr float kBound = 256.f;  // bound on an unnormalised probability
+
+// A workgroup's rows: `rows` of them from row0 of sequence b on.
+struct RowTile {
+  int b, row0, rows, group;
+  int begin;    // packed row of the sequence's first new token
+  int pos0;     // that token's position
+  int length;   // cut to the table's capacity
+  bool beyond;  // the length is beyond it
+
+  template <int ROWS, typename P> __device__ __forceinline__ static RowTile at(const P& p, int slot) {
+    const CacheShape& c = p.at;
+    RowTile t;
+    t.group = p.heads / c.kv_heads;
+    auto first_slot = [&](int b) { return (int)((long)packed_begin(c, b) * t.group / ROWS) + b; };
+    t.b = c.offsets ? last_at_or_before(c.batch, slot, first_slot) : slot / p_slots<ROWS>(t.group);
+    t.begin = packed_begin(c, t.b);
+    const int count = c.offsets ? max(0, packed_begin(c, t.b + 1) - t.begin) : 1;
+    const int tile = c.offsets ? slot - first_slot(t.b) : slot % p_slots<ROWS>(t.group);
+    // (long: a wrong slot's tile times ROWS)
+    const long left = (long)count * t.group - (long)tile * ROWS;
+    t.row0 = tile * ROWS;
+    t.rows = tile < 0 || left < 0 ? 0 : (int)(left < ROWS ? left : ROWS);
+    const long capacity = (long)c.pages_per_seq << c.page_shift;
+    const int length = max(0, c.lengths[t.b]);
+    t.beyond = length > capacity;
+    t.length = t.beyond ? (int)capacity : length;
+    t.pos0 = length - count;
+    return t;
+  }
+  // Tiles of a sequence of one token.
+  template <int ROWS> __device__ __forceinline__ static int p_slots(int group) { return (group + ROWS - 1) / ROWS; }
+
+  __device__ __forceinline__ int position(int r) const { return pos0 + (row0 + r) / group; }
+  // Element offset of row r's head in q and out.
+  __device__ __forceinline__ long offset(int r, int hk, int heads, int d) const {
+    const int i = (row0 + r) / group, h = (row0 + r) % group;
+    return ((long)(begin + i) * heads + hk * group + h) * d;
+  }
+};
+
+// Zeroes the packed rows behind the last sequence.
+template <int D, typename P> __device__ __forceinline__ void clear_tail(const P& p, int worker, int workers, int threads) {
+  if (!p.clear_tail || !p.at.offsets) return;
+  const long per_row = (long)p.heads * D / 8;
+  const long begin = (long)packed_begin(p.at, p.at.batch) * per_row, end = (long)p.at.total * per_row;
+  u32x4* out = reinterpret_cast<u32x4*>(p.out);
+  for (long i = begin + (long)worker * threads + threadIdx.x; i < end; i += (long)workers * threads) out[i] = u32x4{0, 0, 0, 0};
+}
+
+// The pages of a tile's two halves.
+struct Pages {
+  int page0, page1;
+  bool bad;
+  __device__ __forceinline__ void load(const CacheShape& c, int b, int k0, int rlo, int rhi) {
+    // (each half's page from the nearest row that is read)
+    const int* row = c.table + (long)b * c.pages_per_seq;
+    page0 = row[(k0 + min(rlo, 15)) >> c.page_shift];
+    page1 = rhi >= 16 ? row[(k0 + 16) >> c.page_shift] : page0;
+    bad = (unsigned)page0 >= (unsigned)c.pages || (unsigned)page1 >= (unsigned)c.pages;
+    if (bad) page0 = page1 = 0;
+  }
+};
+
+// Where split `split` of a tile of rows leaves its output (ROWS rows of D) and, behind all
+// outputs, its rows' maxima and sums.
+template <int ROWS, int D, typename P> struct Parts {
+  float* out;
+  float* ml;
+  __device__ __forceinline__ Parts(const P& p, int slot, int hk, int split) {
+    const long part = ((long)slot * p.at.kv_heads + hk) * p.splits + split;
+    const long count = (long)p.slots * p.at.kv_heads * p.splits;
+    out = p.parts + part * ROWS * D;
+    ml = p.parts + count * ROWS * D + part * ROWS * 2;
+  }
+};
+
+// ------------------------------------------------------------------ few rows
+
+template <typename T, typename C, int D> struct Token {
+  static constexpr int kRows = 16;
+  static constexpr int kWaves = D == 256 ? 2 : 4;  // LDS: a tile of keys and values a wave
+  static constexpr int kThreads = 64 * kWaves;
+};
+
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__((Token<T, C, D>::kThreads))
+paged_token_kernel(PagedParams<T, C> p) {
+  constexpr int kWaves = Token<T, C, D>::kWaves, ROWS = Token<T, C, D>::kRows;
+  constexpr int KS = D / 32, DB = D / 16;
+  typedef PageTile<T, C, D, 64, kSwzRows> Tile;
+  constexpr int kWaveLds = 2 * Tile::kTileBytes;
+  __shared__ __attribute__((aligned(1024))) char s_kv[kWaves * kWaveLds];
+  __shared__ float s_ml[kWaves][ROWS][2];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads, split = blockIdx.y;
+  clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, Token<T, C, D>::kThreads);
+  const RowTile rt = RowTile::template at<ROWS>(p, slot);
+  if (rt.rows <= 0) return;
+  const int first_pos = __builtin_amdgcn_readfirstlane(rt.position(0));
+  const int last_pos = __builtin_amdgcn_readfirstlane(rt.position(rt.rows - 1));
+  const PageSpan span(first_pos, last_pos, rt.length, p.window, p.sinks);
+  const int t0 = split * p.split_tiles, t1 = min(span.tiles, t0 + p.split_tiles);
+  if (split > 0 && t0 >= t1) return;
+
+  // This lane's row (n): its queries as the score products' B operand, and its position.
+  const int r = min(n, rt.rows - 1);
+  const int pos = rt.position(r);
+  const bool negate = p.scale < 0.f;  // applied as |scale| to -q (negation is exact)
+  V8<T> qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    qf[ks] = *reinterpret_cast<const V8<T>*>(p.q + rt.offset(r, hk, p.heads, D) + 32 * ks + 8 * g);
+    if (negate) qf[ks] = -qf[ks];
+  }
+  const float c2 = fabsf(p.scale) * kLog2e;
+
+  SwzFrags16<T, D> fr;
+  fr.init(lane);
+  const uint32_t lds = lds_base_u32(s_kv) + wave * kWaveLds;
+  float m = -1e30f, lpart = 0.f;
+  f32x4 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) acc[db] = zero4();
+  bool bad = rt.beyond;
+
+  Tile tile;
+  auto fetch = [&](int t) {
+    const int k0 = span.key(t), rlo = span.first_row(t), rhi = span.last_row(t);
+    Pages pg;
+    pg.load(p.at, rt.b, k0, rlo, rhi);
+    bad |= pg.bad;
+    tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, k0, rlo, rhi, pg.page0, pg.page1, lane);
+  };
+  int t = t0 + wave;
+  if (t < t1) fetch(t);
+  for (; t < t1; t += kWaves) {
+    __builtin_amdgcn_wave_barrier();  // (the wave's LDS operations run in order; only the compiler could move them)
+    tile.store(lds, lane);
+    __builtin_amdgcn_wave_barrier();
+    if (t + kWaves < t1) fetch(t + kWaves);
+    const int k0 = span.key(t), rlo = span.first_row(t), rhi = span.last_row(t);
+    f32x4 S[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      S[kb] = zero4();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) S[kb] = mma16<T>(fr.rowf(lds, 0, kb, ks), qf[ks], S[kb]);
+    }
+    if (rlo > 0 || rhi < 31 || k0 + 31 > first_pos || (p.window && k0 <= last_pos - p.window)) {
+      const int klim = min(rhi, pos - k0);
+      const int klow = p.window ? pos - p.window + 1 - k0 : 0, ksinks = p.sinks - k0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = 16 * (e >> 2) + 4 * g + (e & 3);
+        if (key > klim || key < rlo || (key < klow && key >= ksinks)) S[e >> 2][e & 3] = -INFINITY;
+      }
+    }
+    f32x8 P;
+    auto probabilities = [&] {
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        P[e] = exp2_fast(fmaf(S[e >> 2][e & 3], c2, -m));  // masked: exp2(-inf) = 0
+        sum += P[e];
+      }
+      return sum;
+    };
+    float psum = probabilities();
+    if (__any(!(psum <= kBound))) {
+      float top = S[0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, S[e >> 2][e & 3]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float mnew = fmaxf(m, top * c2);
+      const float alpha = exp2_fast(m - mnew);
+      lpart *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+      m = mnew;
+      psum = probabilities();
+    }
+    lpart += psum;
+    const V8<T> oP = cvt8<T>(P);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = mma16<T>(fr.trf(lds, Tile::kTileBytes, db), oP, acc[db]);
+  }
+
+  // The waves' outputs meet in LDS, in place of the tiles: (wave, column, row), so that the
+  // lanes of a column block write 16 rows side by side.
+  if (__any(bad)) lpart = NAN;
+  const float l = group4_sum(lpart);
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(s_kv);
+  static_assert(kWaves * ROWS * D * (int)sizeof(float) <= kWaves * kWaveLds, "the join reuses the tiles");
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) so[(wave * D + 16 * db + 4 * g + i) * ROWS + n] = acc[db][i];
+  if (g == 0) {
+    s_ml[wave][n][0] = m;
+    s_ml[wave][n][1] = l;
+  }
+  __syncthreads();
+  Parts<ROWS, D, PagedParams<T, C>> parts(p, slot, hk, split);
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += Token<T, C, D>::kThreads) {
+    const int row = i / (D / 4), col = 4 * (i % (D / 4));
+    if (row >= rt.rows) break;
+    float top = s_ml[0][row][0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_ml[w][row][0]);
+    float sum = 0.f;
+    f32x4 o = zero4();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = exp2_fast(s_ml[w][row][0] - top);
+      sum += f * s_ml[w][row][1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += f * so[(w * D + col + j) * ROWS + row];
+    }
+    if (p.splits > 1) {
+      *reinterpret_cast<f32x4*>(parts.out + row * D + col) = o;
+      if (col == 0) {
+        parts.ml[2 * row] = top;
+        parts.ml[2 * row + 1] = sum;
+      }
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: 0
+      *reinterpret_cast<V4<T>*>(p.out + rt.offset(row, hk, p.heads, D) + col) = cvt4<T>(o * inv);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ many rows
+
+constexpr int kChunkRows = 128;
+
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+paged_chunk_kernel(PagedParams<T, C> p) {
+  constexpr int ROWS = kChunkRows;
+  constexpr int KS = D / 16, DT = D / 32;
+  typedef PageTile<T, C, D, 256, kSwzPairs> Tile;
+  constexpr int kStage = 2 * Tile::kTileBytes;
+  __shared__ __attribute__((aligned(1024))) char s_kv[2 * kStage];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, g = lane >> 5;
+  const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads, split = blockIdx.y;
+  clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 256);
+  const RowTile rt = RowTile::template at<ROWS>(p, slot);
+  if (rt.rows <= 0) return;
+  const int first_pos = __builtin_amdgcn_readfirstlane(rt.position(0));
+  const int last_pos = __builtin_amdgcn_readfirstlane(rt.position(rt.rows - 1));
+  const PageSpan span(first_pos, last_pos, rt.length, p.window, p.sinks);
+  const int t0 = split * p.split_tiles;
+  const int t1 = __builtin_amdgcn_readfirstlane(min(span.tiles, t0 + p.split_tiles));
+  if (split > 0 && t0 >= t1) return;
+
+  // This wave's rows, from 32 * wave on, and this lane's.
+  const bool any = 32 * wave < rt.rows;
+  const int wfirst = __builtin_amdgcn_readfirstlane(rt.position(min(32 * wave, rt.rows - 1)));
+  const int wlast = __builtin_amdgcn_readfirstlane(rt.position(min(32 * wave + 31, rt.rows - 1)));
+  const int r = min(32 * wave + n, rt.rows - 1);
+  const bool valid = 32 * wave + n < rt.rows;
+  const int pos = rt.position(r);
+  const bool negate = p.scale < 0.f;
+  V8<T> qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    qf[ks] = *reinterpret_cast<const V8<T>*>(p.q + rt.offset(r, hk, p.heads, D) + 16 * ks + 8 * g);
+    if (negate) qf[ks] = -qf[ks];
+  }
+  const float c2 = fabsf(p.scale) * kLog2e;
+
+  SwzFrags<T, D> fr;
+  fr.init(lane);
+  const uint32_t lds = lds_base_u32(s_kv);
+  float m = -1e30f, lpart = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
+  bool bad = rt.beyond;
+
+  Tile tile;
+  auto fetch = [&](int t) {
+    const int k0 = span.key(t), rlo = span.first_row(t), rhi = span.last_row(t);
+    Pages pg;
+    pg.load(p.at, rt.b, k0, rlo, rhi);
+    bad |= pg.bad;
+    tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, k0, rlo, rhi, pg.page0, pg.page1, threadIdx.x);
+  };
+  // Tile t is stored to stage t % 2 in iteration t - 1, whose barrier at its end shows it; the
+  // stage's last readers passed the barrier of iteration t - 2.
+  if (t0 < t1) {
+    fetch(t0);
+    tile.store(lds + (t0 & 1) * kStage, threadIdx.x);
+    if (t0 + 1 < t1) fetch(t0 + 1);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    if (t + 1 < t1) {
+      tile.store(lds + ((t + 1) & 1) * kStage, threadIdx.x);
+      if (t + 2 < t1) fetch(t + 2);
+    }
+    const int k0 = span.key(t);
+    // a wave's own positions: nothing before its window's start or behind its last row
+    const bool active = any && k0 <= wlast &&
+                        (t < span.sink_tiles || !p.window || k0 + 31 > wfirst - p.window || k0 < p.sinks);
+    if (active) {
+      const uint32_t sa = lds + (t & 1) * kStage;
+      f32x16 S = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) S = mma<T>(fr.rowf(sa, 0, ks), qf[ks], S);
+      const int rlo = span.first_row(t), rhi = span.last_row(t);
+      if (rlo > 0 || rhi < 31 || k0 + 31 > wfirst || (p.window && k0 <= wlast - p.window)) {
+        const int klim = min(rhi, pos - k0);
+        const int klow = p.window ? pos - p.window + 1 - k0 : 0, ksinks = p.sinks - k0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = crow(i, g);
+          if (key > klim || key < rlo || (key < klow && key >= ksinks)) S[i] = -INFINITY;
+        }
+      }
+      f32x16 P;
+      auto probabilities = [&] {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          P[i] = exp2_fast(fmaf(S[i], c2, -m));  // masked: exp2(-inf) = 0
+          sum += P[i];
+        }
+        return sum;
+      };
+      float psum = probabilities();
+      if (__any(!(psum <= kBound))) {
+        float top = S[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
+        const float mnew = fmaxf(m, xgroup_max(top * c2));
+        const float alpha = exp2_fast(m - mnew);
+        lpart *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+        m = mnew;
+        psum = probabilities();
+      }
+      lpart += psum;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const V8<T> oP = cvt8<T>(s ? hi8(P) : lo8(P));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = mma<T>(fr.trf(sa, Tile::kTileBytes, dt, s), oP, acc[dt]);
+      }
+    }
+    __syncthreads();
+  }
+
+  if (bad) lpart = NAN;
+  const float l = xgroup_sum(lpart);
+  if (!valid) return;
+  const int row = 32 * wave + n;
+  if (p.splits > 1) {
+    Parts<ROWS, D, PagedParams<T, C>> parts(p, slot, hk, split);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        *reinterpret_cast<f32x4*>(parts.out + row * D + 32 * dt + 8 * a + 4 * g) =
+            f32x4{acc[dt][4 * a], acc[dt][4 * a + 1], acc[dt][4 * a + 2], acc[dt][4 * a + 3]};
+    if (g == 0) {
+      parts.ml[2 * row] = m;
+      parts.ml[2 * row + 1] = l;
+    }
+  } else {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: 0
+    T* o = p.out + rt.offset(row, hk, p.heads, D);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        f32x4 x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = acc[dt][4 * a + j] * inv;
+        *reinterpret_cast<V4<T>*>(o + 32 * dt + 8 * a + 4 * g) = cvt4<T>(x);
+      }
+  }
+}
+
+// ------------------------------------------------------------------ the splits' join
+
+// One workgroup a tile of rows and key/value head; the splits in order, four columns a thread.
+template <typename T, typename C, int D, int ROWS>
+__global__ void __launch_bounds__(256)
+paged_join_kernel(PagedParams<T, C> p) {
+  const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads;
+  const RowTile rt = RowTile::template at<ROWS>(p, slot);
+  if (rt.rows <= 0) return;
+  const PageSpan span(rt.position(0), rt.position(rt.rows - 1), rt.length, p.window, p.sinks);
+  const int splits = max(1, min(p.splits, (span.tiles + p.split_tiles - 1) / p.split_tiles));
+  for (int i = threadIdx.x; i < rt.rows * (D / 4); i += 256) {
+    const int row = i / (D / 4), col = 4 * (i % (D / 4));
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, Parts<ROWS, D, PagedParams<T, C>>(p, slot, hk, s).ml[2 * row]);
+    f32x4 o = zero4();
+    for (int s = 0; s < splits; ++s) {
+      const Parts<ROWS, D, PagedParams<T, C>> part(p, slot, hk, s);
+      const float f = exp2_fast(part.ml[2 * row] - top);
+      sum += f * part.ml[2 * row + 1];
+      o += f * *reinterpret_cast<const f32x4*>(part.out + row * D + col);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<V4<T>*>(p.out + rt.offset(row, hk, p.heads, D) + col) = cvt4<T>(o * inv);
+  }
+}
+
+template <typename T, typename C, int D, int ROWS>
+hipError_t join(const PagedParams<T, C>& p, hipStream_t stream) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  hipLaunchKernelGGL((paged_join_kernel<T, C, D, ROWS>), dim3(p.slots * p.at.kv_heads), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+template <typename T, typename C, int D>
+hipError_t launch_paged_attention(const PagedParams<T, C>& p, bool chunk, hipStream_t stream) {
+  const dim3 grid(p.slots * p.at.kv_heads, p.splits);
+  if (chunk) {
+    hipLaunchKernelGGL((paged_chunk_kernel<T, C, D>), grid, dim3(256), 0, stream, p);
+    return join<T, C, D, kChunkRows>(p, stream);
+  }
+  typedef Token<T, C, D> K;
+  hipLaunchKernelGGL((paged_token_kernel<T, C, D>), grid, dim3(K::kThreads), 0, stream, p);
+  return join<T, C, D, K::kRows>(p, stream);
+}
+
+#define FHOG_INST(T, C, D) \
+  template hipError_t launch_paged_attention<T, C, D>(const PagedParams<T, C>&, bool, hipStream_t);
+FHOG_INST(__bf16, __bf16, 64)
+FHOG_INST(__bf16, __bf16, 128)
+FHOG_INST(__bf16, __bf16, 256)
+FHOG_INST(__bf16, e4m3, 64)
+FHOG_INST(__bf16, e4m3, 128)
+FHOG_INST(__bf16, e4m3, 256)
+FHOG_INST(_Float16, _Float16, 64)
+FHOG_INST(_Float16, _Float16, 128)
+FHOG_INST(_Float16, _Float16, 256)
+FHOG_INST(_Float16, e4m3, 64)
+FHOG_INST(_Float16, e4m3, 128)
+FHOG_INST(_Float16, e4m3, 256)
+#undef FHOG_INST
+
+}  // namespace fhog

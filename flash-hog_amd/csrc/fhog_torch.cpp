@@ -57,6 +57,10 @@ struct Api {
   decltype(&fhog_window_attention_fwd) window_fwd = nullptr;
   decltype(&fhog_window_attention_bwd) window_bwd = nullptr;
   decltype(&fhog_window_attention_bwdbwd) window_bwdbwd = nullptr;
+  decltype(&fhog_paged_workspace_bytes) paged_bytes = nullptr;
+  decltype(&fhog_paged_attention) paged_attention = nullptr;
+  decltype(&fhog_paged_cache_write) cache_write = nullptr;
+  decltype(&fhog_paged_cache_read) cache_read = nullptr;
   py::object error_cls;
 };
 
@@ -82,6 +86,14 @@ void bind_window(std::uintptr_t bytes, std::uintptr_t fwd, std::uintptr_t bwd, s
   a.window_fwd = reinterpret_cast<decltype(a.window_fwd)>(fwd);
   a.window_bwd = reinterpret_cast<decltype(a.window_bwd)>(bwd);
   a.window_bwdbwd = reinterpret_cast<decltype(a.window_bwdbwd)>(bwdbwd);
+}
+
+void bind_paged(std::uintptr_t bytes, std::uintptr_t attention, std::uintptr_t write, std::uintptr_t read) {
+  Api& a = api();
+  a.paged_bytes = reinterpret_cast<decltype(a.paged_bytes)>(bytes);
+  a.paged_attention = reinterpret_cast<decltype(a.paged_attention)>(attention);
+  a.cache_write = reinterpret_cast<decltype(a.cache_write)>(write);
+  a.cache_read = reinterpret_cast<decltype(a.cache_read)>(read);
 }
 
 std::string shape_str(const at::Tensor& t) {
@@ -310,6 +322,147 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> bwdbwd_co
   return {dq2, dk2, dv2, ddo, stats};
 }
 
+// -------------------------------------------------------------- paged cache
+
+typedef c10::optional<at::Tensor> MaybeTensor;
+
+const at::Tensor* get(const MaybeTensor& t) { return t && t->defined() ? &*t : nullptr; }
+const void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// A paged cache and what finds tokens in it, checked (_hip.py _check_cache).
+struct Cache {
+  const at::Tensor *k, *v, *k_scale = nullptr, *v_scale = nullptr;
+  at::Tensor table, lengths, offsets;  // contiguous; offsets undefined if there are none
+  int pages, kv_heads, page, head_dim, batch, width, dtype;
+
+  Cache(const char* first_name, const at::Tensor& first, const at::Tensor& k_, const at::Tensor& v_,
+        const at::Tensor& table_, const at::Tensor& lengths_, const MaybeTensor& offsets_, const MaybeTensor& ks,
+        const MaybeTensor& vs, at::ScalarType dt)
+      : k(&k_), v(&v_) {
+    const bool quantised = k_.scalar_type() == at::kFloat8_e4m3fn;
+    const at::Tensor *kst = get(ks), *vst = get(vs), *off = get(offsets_);
+    check_inputs({{first_name, &first}, {"key_cache", &k_}, {"value_cache", &v_}, {"page_table", &table_},
+                  {"lengths", &lengths_}},
+                 c10::nullopt);
+    if (quantised) {
+      if (!kst || !vst) value_error("an e4m3 cache needs key_scale and value_scale");
+      check_inputs({{first_name, &first}, {"key_scale", kst}, {"value_scale", vst}}, c10::nullopt);
+    } else if (kst || vst) {
+      value_error("key_scale and value_scale are for an e4m3 cache, not " + dtype_str(k_.scalar_type()));
+    }
+    if (off) check_inputs({{first_name, &first}, {"query_offsets", off}}, c10::nullopt);
+    if (k_.dim() != 4) value_error("expected a (pages, kv_heads, page_size, head_dim) cache, got " + shape_str(k_));
+    expect("value_cache", v_, k_.sizes(), k_.scalar_type());
+    if (k_.scalar_type() != dt && !quantised)
+      value_error("the cache must be of " + dtype_str(dt) + " or torch.float8_e4m3fn, got " +
+                  dtype_str(k_.scalar_type()));
+    if (!k_.is_contiguous()) value_error("key_cache must be contiguous");
+    if (!v_.is_contiguous()) value_error("value_cache must be contiguous");
+    if (quantised) {
+      k_scale = kst;
+      v_scale = vst;
+      for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"key_scale", kst}, {"value_scale", vst}}) {
+        expect(name, *t, k_.sizes().slice(0, 3));
+        if ((t->scalar_type() != at::kFloat8_e8m0fnu && t->scalar_type() != at::kByte) || !t->is_contiguous())
+          value_error(std::string(name) + " must be a contiguous tensor of torch.float8_e8m0fnu or torch.uint8");
+      }
+    }
+    if (table_.dim() != 2) value_error("expected a (batch, pages) page_table, got " + shape_str(table_));
+    expect("lengths", lengths_, {table_.size(0)});
+    if (off) expect("query_offsets", *off, {table_.size(0) + 1});
+    for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"page_table", &table_},
+                                  {"lengths", &lengths_}, {"query_offsets", off}})
+      if (t && t->scalar_type() != at::kInt)
+        value_error(std::string(name) + " has dtype " + dtype_str(t->scalar_type()) + ", expected torch.int32");
+    for (int64_t s : k_.sizes())
+      if (s > INT32_MAX) value_error("key_cache" + shape_str(k_) + " has a dimension beyond the C ABI's int range");
+    for (int64_t s : table_.sizes())
+      if (s > INT32_MAX) value_error("page_table" + shape_str(table_) + " has a dimension beyond the C ABI's int range");
+    table = contig(table_);
+    lengths = contig(lengths_);
+    if (off) offsets = contig(*off);
+    pages = (int)k_.size(0), kv_heads = (int)k_.size(1), page = (int)k_.size(2), head_dim = (int)k_.size(3);
+    batch = (int)table_.size(0), width = (int)table_.size(1);
+    dtype = quantised ? FHOG_DTYPE_E4M3 : dtype_code(dt);
+  }
+  const int* table_ptr() const { return table.data_ptr<int>(); }
+  const int* lengths_ptr() const { return lengths.data_ptr<int>(); }
+  const int* offsets_ptr() const { return offsets.defined() ? offsets.data_ptr<int>() : nullptr; }
+};
+
+int rows_of(const char* name, const at::Tensor& t) {
+  if (t.dim() != 3) value_error(std::string("expected a (T, N, H) ") + name + ", got " + shape_str(t));
+  for (int64_t s : t.sizes())
+    if (s > INT32_MAX) value_error(name + shape_str(t) + " has a dimension beyond the C ABI's int range");
+  return (int)t.size(0);
+}
+
+at::Tensor paged_attention_core(const at::Tensor& q_, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& offsets,
+                                const MaybeTensor& k_scale, const MaybeTensor& v_scale, int window, int sinks,
+                                double scale, const MaybeTensor& out_) {
+  const int total = rows_of("query", q_);
+  const Cache c("query", q_, k_cache, v_cache, table, lengths, offsets, k_scale, v_scale, q_.scalar_type());
+  if (q_.size(2) != c.head_dim)
+    value_error("query" + shape_str(q_) + " and key_cache" + shape_str(k_cache) + " disagree on head_dim");
+  const int dt = dtype_code(q_.scalar_type());
+  const at::Tensor* given = get(out_);
+  if (given) {
+    check_inputs({{"query", &q_}, {"out", given}}, q_.scalar_type());
+    expect("out", *given, q_.sizes());
+    if (!given->is_contiguous()) value_error("out must be contiguous");
+  }
+  at::Tensor out = given ? *given : at::empty(q_.sizes(), q_.options());
+  const at::Tensor q = contig(q_);
+  const int heads = (int)q.size(1);
+  c10::DeviceGuard guard(q.device());
+  const size_t size = api().paged_bytes(c.batch, total, !c.offsets.defined(), heads, c.kv_heads, c.head_dim, c.page,
+                                        c.width, window, sinks);
+  const at::Tensor ws = size ? at::empty({(int64_t)size}, q.options().dtype(at::kByte)) : at::Tensor();
+  check_status(api().paged_attention(current_stream(q), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                     ptr(c.k_scale), ptr(c.v_scale), c.table_ptr(), c.lengths_ptr(), c.offsets_ptr(),
+                                     out.data_ptr(), data_or_null(ws), size, c.batch, total, heads, c.kv_heads,
+                                     c.head_dim, c.pages, c.page, c.width, dt, c.dtype, window, sinks, given == nullptr,
+                                     (float)scale));
+  return out;
+}
+
+void cache_write_core(const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                      const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& offsets,
+                      const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  const int total = rows_of("key", k_);
+  const Cache c("key", k_, k_cache, v_cache, table, lengths, offsets, k_scale, v_scale, k_.scalar_type());
+  check_inputs({{"key", &k_}, {"value", &v_}}, k_.scalar_type());
+  expect("value", v_, k_.sizes());
+  if (k_.size(1) != c.kv_heads || k_.size(2) != c.head_dim)
+    value_error("key" + shape_str(k_) + " and key_cache" + shape_str(k_cache) + " disagree on heads or head_dim");
+  const int dt = dtype_code(k_.scalar_type());
+  const at::Tensor k = contig(k_), v = contig(v_);
+  c10::DeviceGuard guard(k.device());
+  check_status(api().cache_write(current_stream(k), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
+                                 v_cache.data_ptr(), const_cast<void*>(ptr(c.k_scale)),
+                                 const_cast<void*>(ptr(c.v_scale)), c.table_ptr(), c.lengths_ptr(), c.offsets_ptr(),
+                                 c.batch, total, c.kv_heads, c.head_dim, c.pages, c.page, c.width, dt, c.dtype));
+}
+
+std::tuple<at::Tensor, at::Tensor> cache_read_core(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                   const at::Tensor& table, const at::Tensor& lengths,
+                                                   int64_t max_length, at::ScalarType dtype,
+                                                   const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  const Cache c("key_cache", k_cache, k_cache, v_cache, table, lengths, c10::nullopt, k_scale, v_scale, dtype);
+  if (max_length < 0) value_error("max_length must be >= 0, got " + std::to_string(max_length));
+  if (max_length > INT32_MAX) value_error("max_length is beyond the C ABI's int range");
+  const int dt = dtype_code(dtype);
+  const auto options = k_cache.options().dtype(dtype);
+  at::Tensor k = at::empty({(int64_t)c.batch, max_length, (int64_t)c.kv_heads, (int64_t)c.head_dim}, options);
+  at::Tensor v = at::empty(k.sizes(), options);
+  c10::DeviceGuard guard(k.device());
+  check_status(api().cache_read(current_stream(k), k_cache.data_ptr(), v_cache.data_ptr(), ptr(c.k_scale),
+                                ptr(c.v_scale), c.table_ptr(), c.lengths_ptr(), k.data_ptr(), v.data_ptr(), c.batch,
+                                (int)max_length, c.kv_heads, c.head_dim, c.pages, c.page, c.width, dt, c.dtype));
+  return {k, v};
+}
+
 // ------------------------------------------------------------------ autograd
 
 using torch::autograd::AutogradContext;
@@ -433,6 +586,32 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> attention
   return py_call([&] { return bwdbwd_core(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale, {window, sinks}); });
 }
 
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& offsets,
+                           const MaybeTensor& k_scale, const MaybeTensor& v_scale, int window, int sinks, double scale,
+                           const MaybeTensor& out) {
+  require_bound((const void*)api().paged_attention);
+  return py_call([&] {
+    return paged_attention_core(q, k_cache, v_cache, table, lengths, offsets, k_scale, v_scale, window, sinks, scale,
+                                out);
+  });
+}
+
+void paged_cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                       const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& offsets,
+                       const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  require_bound((const void*)api().cache_write);
+  py_call([&] { cache_write_core(k, v, k_cache, v_cache, table, lengths, offsets, k_scale, v_scale); });
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_cache_read(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                    const at::Tensor& table, const at::Tensor& lengths,
+                                                    int64_t max_length, at::ScalarType dtype,
+                                                    const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  require_bound((const void*)api().cache_read);
+  return py_call([&] { return cache_read_core(k_cache, v_cache, table, lengths, max_length, dtype, k_scale, v_scale); });
+}
+
 // O of attention(q, k, v) with the autograd nodes above (when q, k or v
 // require grad and grad mode is on).
 at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t causal, double scale,
@@ -447,6 +626,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "Tensor-level calls of the Flash-HOG C ABI (see flash_hog/_hip.py)";
   m.def("bind", &bind, "bind(fwd, bwd, bwdbwd, last_error, status_string, error_cls): entry-point addresses");
   m.def("bind_window", &bind_window, "bind_window(workspace_bytes, fwd, bwd, bwdbwd): their addresses");
+  m.def("bind_paged", &bind_paged, "bind_paged(workspace_bytes, attention, write, read): their addresses");
+  m.def("paged_attention", &paged_attention);
+  m.def("paged_cache_write", &paged_cache_write);
+  m.def("paged_cache_read", &paged_cache_read);
   using py::arg;
   m.def("attention_fwd", &attention_fwd, arg("q"), arg("k"), arg("v"), arg("causal"), arg("scale"), arg("window") = 0,
         arg("sinks") = 0);

@@ -9,5 +9,7 @@ through the C ABI in include/flash_hog.h.
 from flash_hog._types import MaskType, TuningConfig
 from flash_hog.torch._hip_gpu import supported
 from flash_hog.torch.attention import dot_product_attention
+from flash_hog.torch.paged import paged_attention, paged_cache_read, paged_cache_write
 
-__all__ = ["MaskType", "TuningConfig", "dot_product_attention", "supported"]
+__all__ = ["MaskType", "TuningConfig", "dot_product_attention", "paged_attention", "paged_cache_read",
+           "paged_cache_write", "supported"]

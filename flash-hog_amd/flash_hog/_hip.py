@@ -58,6 +58,10 @@ SIGNATURES = {
     "fhog_window_attention_fwd": (_i, [_p] * 6 + [_i] * 10 + [_f]),
     "fhog_window_attention_bwd": (_i, [_p] * 12 + [_i] * 10 + [_f]),
     "fhog_window_attention_bwdbwd": (_i, [_p] * 18 + [_i] * 10 + [_f]),
+    "fhog_paged_workspace_bytes": (ctypes.c_size_t, [_i] * 10),
+    "fhog_paged_attention": (_i, [_p] * 11 + [ctypes.c_size_t] + [_i] * 13 + [_f]),
+    "fhog_paged_cache_write": (_i, [_p] * 10 + [_i] * 9),
+    "fhog_paged_cache_read": (_i, [_p] * 9 + [_i] * 9),
 }
 
 
@@ -113,6 +117,8 @@ def torch_ext():
                  addr(L.fhog_last_error), addr(L.fhog_status_string), FlashHogError)
         mod.bind_window(addr(L.fhog_window_workspace_bytes), addr(L.fhog_window_attention_fwd),
                         addr(L.fhog_window_attention_bwd), addr(L.fhog_window_attention_bwdbwd))
+        mod.bind_paged(addr(L.fhog_paged_workspace_bytes), addr(L.fhog_paged_attention),
+                       addr(L.fhog_paged_cache_write), addr(L.fhog_paged_cache_read))
     except (ImportError, OSError, AttributeError) as exc:
         warnings.warn(f"Flash-HOG torch extension {TORCH_EXT_PATH} not loaded ({exc}); "
                       "using the Python wrappers", RuntimeWarning, stacklevel=2)
@@ -353,3 +359,136 @@ def attention_bwdbwd_noalloc(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale
             _ptr(dq2), _ptr(dk2), _ptr(dv2), _ptr(ddo),
             B, Tq, Tk, N, Nk, Hd, DTYPE_CODES[q.dtype], causal_code(causal), float(scale)))
     return dq2, dk2, dv2, ddo
+
+
+# ------------------------------------------------------------- paged cache
+
+CACHE_DTYPE_CODES = {torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3}
+_SCALE_DTYPES = (torch.float8_e8m0fnu, torch.uint8)
+
+
+def _check_cache(first, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, dtype):
+    """Checks a paged cache and what finds tokens in it; `first` is the (name, tensor) whose
+    device all share. Returns (num_pages, kv_heads, page_size, head_dim, batch, pages_per_seq)
+    and the index tensors, contiguous."""
+    named = [first, ("key_cache", k_cache), ("value_cache", v_cache), ("page_table", page_table),
+             ("lengths", lengths)]
+    quantised = k_cache.dtype == torch.float8_e4m3fn
+    if quantised:
+        if k_scale is None or v_scale is None:
+            raise ValueError("an e4m3 cache needs key_scale and value_scale")
+        named += [("key_scale", k_scale), ("value_scale", v_scale)]
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError(f"key_scale and value_scale are for an e4m3 cache, not {k_cache.dtype}")
+    if query_offsets is not None:
+        named.append(("query_offsets", query_offsets))
+    _check_inputs(named)
+    if k_cache.ndim != 4:
+        raise ValueError(f"expected a (pages, kv_heads, page_size, head_dim) cache, got {tuple(k_cache.shape)}")
+    _expect("value_cache", v_cache, k_cache.shape, k_cache.dtype)
+    if k_cache.dtype not in (dtype, torch.float8_e4m3fn):
+        raise ValueError(f"the cache must be of {dtype} or torch.float8_e4m3fn, got {k_cache.dtype}")
+    for name, t in (("key_cache", k_cache), ("value_cache", v_cache)):
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if quantised:
+        for name, t in (("key_scale", k_scale), ("value_scale", v_scale)):
+            _expect(name, t, k_cache.shape[:3])
+            if t.dtype not in _SCALE_DTYPES or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous tensor of torch.float8_e8m0fnu or torch.uint8")
+    if page_table.ndim != 2:
+        raise ValueError(f"expected a (batch, pages) page_table, got {tuple(page_table.shape)}")
+    batch = page_table.shape[0]
+    _expect("lengths", lengths, (batch,))
+    index = [("page_table", page_table), ("lengths", lengths)]
+    if query_offsets is not None:
+        _expect("query_offsets", query_offsets, (batch + 1,))
+        index.append(("query_offsets", query_offsets))
+    for name, t in index:
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} has dtype {t.dtype}, expected torch.int32")
+    page_table, lengths = _contig(page_table, lengths)
+    if query_offsets is not None:
+        query_offsets = query_offsets.contiguous()
+    return (*k_cache.shape, batch, page_table.shape[1]), page_table, lengths, query_offsets
+
+
+def paged_attention(q, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, window: int,
+                    sinks: int, scale: float, out=None):
+    """out (T, N, H) of the packed new tokens q over a paged cache (fhog_paged_attention); window 0: none."""
+    window, sinks = _window_args(window, sinks)
+    ext = torch_ext()
+    if ext is not None:
+        return ext.paged_attention(q, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, window,
+                                   sinks, float(scale), out)
+    if q.ndim != 3:
+        raise ValueError(f"expected a (T, N, H) query, got {tuple(q.shape)}")
+    (pages, Nk, page, Hd, B, width), page_table, lengths, query_offsets = _check_cache(
+        ("query", q), k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, q.dtype)
+    T, N, Hq = q.shape
+    if Hq != Hd:
+        raise ValueError(f"query{tuple(q.shape)} and key_cache{tuple(k_cache.shape)} disagree on head_dim")
+    if q.dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {q.dtype}")
+    clear = out is None
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _check_inputs([("query", q), ("out", out)], q.dtype)
+        _expect("out", out, q.shape)
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+    q = q.contiguous()
+    with _on_device(q.device):
+        size = lib().fhog_paged_workspace_bytes(B, T, int(query_offsets is None), N, Nk, Hd, page, width, window, sinks)
+        ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
+        check(lib().fhog_paged_attention(
+            _stream(q.device), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(page_table),
+            _ptr(lengths), _ptr(query_offsets), _ptr(out), _ptr(ws), size, B, T, N, Nk, Hd, pages, page, width,
+            DTYPE_CODES[q.dtype], CACHE_DTYPE_CODES[k_cache.dtype], window, sinks, int(clear), float(scale)))
+    return out
+
+
+def paged_cache_write(k, v, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale) -> None:
+    """The packed new tokens' keys and values (T, N, H) into their pages (fhog_paged_cache_write)."""
+    ext = torch_ext()
+    if ext is not None:
+        ext.paged_cache_write(k, v, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale)
+        return
+    if k.ndim != 3:
+        raise ValueError(f"expected a (T, N, H) key, got {tuple(k.shape)}")
+    (pages, Nk, page, Hd, B, width), page_table, lengths, query_offsets = _check_cache(
+        ("key", k), k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, k.dtype)
+    _check_inputs([("key", k), ("value", v)], k.dtype)
+    _expect("value", v, k.shape)
+    if tuple(k.shape[1:]) != (Nk, Hd):
+        raise ValueError(f"key{tuple(k.shape)} and key_cache{tuple(k_cache.shape)} disagree on heads or head_dim")
+    if k.dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {k.dtype}")
+    k, v = _contig(k, v)
+    with _on_device(k.device):
+        check(lib().fhog_paged_cache_write(
+            _stream(k.device), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+            _ptr(page_table), _ptr(lengths), _ptr(query_offsets), B, k.shape[0], Nk, Hd, pages, page, width,
+            DTYPE_CODES[k.dtype], CACHE_DTYPE_CODES[k_cache.dtype]))
+
+
+def paged_cache_read(k_cache, v_cache, page_table, lengths, max_length: int, dtype, k_scale, v_scale):
+    """The sequences' keys and values (B, max_length, N, H) in dtype, zeros behind their lengths
+    (fhog_paged_cache_read)."""
+    ext = torch_ext()
+    if ext is not None:
+        return ext.paged_cache_read(k_cache, v_cache, page_table, lengths, max_length, dtype, k_scale, v_scale)
+    (pages, Nk, page, Hd, B, width), page_table, lengths, _ = _check_cache(
+        ("key_cache", k_cache), k_cache, v_cache, page_table, lengths, None, k_scale, v_scale, dtype)
+    if max_length < 0:
+        raise ValueError(f"max_length must be >= 0, got {max_length}")
+    if dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {dtype}")
+    k, v = (torch.empty((B, max_length, Nk, Hd), device=k_cache.device, dtype=dtype) for _ in range(2))
+    with _on_device(k_cache.device):
+        check(lib().fhog_paged_cache_read(
+            _stream(k_cache.device), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(page_table),
+            _ptr(lengths), _ptr(k), _ptr(v), B, max_length, Nk, Hd, pages, page, width, DTYPE_CODES[dtype],
+            CACHE_DTYPE_CODES[k_cache.dtype]))
+    return k, v

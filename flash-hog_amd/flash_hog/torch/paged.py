@@ -1,0 +1,142 @@
+"""Attention over a paged key/value cache: serving what dot_product_attention trains.
+
+  paged_cache_write   the keys and values of new tokens into their sequences' pages,
+                      quantised to e4m3 on the way where the cache holds that
+  paged_attention     the new tokens' attention over the cached keys of their sequences:
+                      one token each (decoding) or chunks of unequal length (prompts), with the
+                      window and sinks of dot_product_attention
+  paged_cache_read    cached sequences back as dense tensors, as dot_product_attention takes them
+
+No counterpart in the reference, which trains only. All three enqueue their kernels on the
+current stream of the tensors' device, read no length back to the host, and can be captured in
+a HIP graph; workspaces come from torch's allocator, a new one for each call.
+
+A cache is two contiguous tensors (pages, kv_heads, page_size, head_dim), of the queries' dtype
+(bfloat16 or float16) or float8_e4m3fn; the page size is a power of two from 16 on, the head dim
+64, 128 or 256. An e4m3 cache has key_scale and value_scale, (pages, kv_heads, page_size) of
+float8_e8m0fnu (or its bytes, uint8): a row of the cache stands for its e4m3 values times its
+scale, a power of two.
+
+page_table (batch, pages per sequence) int32: token s of sequence b is row s % page_size of page
+page_table[b, s // page_size]. lengths (batch,) int32: the tokens that a sequence holds, its new
+ones included. query_offsets (batch + 1,) int32: the new tokens of all sequences are packed,
+sequence b's are rows query_offsets[b] to query_offsets[b + 1] and take its last positions, in
+order; None: each sequence has one.
+
+The index tensors are read on the device only, so mistakes in them cannot raise: an attended
+page outside the cache, or a length beyond its table, makes the rows that depend on it NaN
+(paged_cache_write leaves such a token out), and no access leaves its tensor. Entries and cache
+slots that no visible token needs may hold anything, NaN included. Among the keys of one 32-key
+tile, though, a NaN or infinity in a value that one token sees also reaches the rows beside it.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from flash_hog import _hip
+from flash_hog.torch._hip_gpu import _default_scale
+
+Tensor = torch.Tensor
+
+
+def _refuse_gradients(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no derivative: call it under torch.no_grad() (training attends through "
+                           "flash_hog.dot_product_attention)")
+
+
+@torch.library.custom_op("flash_hog::paged_attention", mutates_args=())
+def paged_attention_op(query: Tensor, key_cache: Tensor, value_cache: Tensor, page_table: Tensor, lengths: Tensor,
+                       query_offsets: Tensor | None, key_scale: Tensor | None, value_scale: Tensor | None, window: int,
+                       sinks: int, scale: float) -> Tensor:
+    return _hip.paged_attention(query, key_cache, value_cache, page_table, lengths, query_offsets, key_scale,
+                                value_scale, window, sinks, scale)
+
+
+@paged_attention_op.register_fake
+def _(query, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale, window, sinks, scale):
+    return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("flash_hog::paged_cache_write",
+                         mutates_args=("key_cache", "value_cache", "key_scale", "value_scale"))
+def paged_cache_write_op(key: Tensor, value: Tensor, key_cache: Tensor, value_cache: Tensor, page_table: Tensor,
+                         lengths: Tensor, query_offsets: Tensor | None, key_scale: Tensor | None,
+                         value_scale: Tensor | None) -> None:
+    _hip.paged_cache_write(key, value, key_cache, value_cache, page_table, lengths, query_offsets, key_scale,
+                           value_scale)
+
+
+@torch.library.custom_op("flash_hog::paged_cache_read", mutates_args=())
+def paged_cache_read_op(key_cache: Tensor, value_cache: Tensor, page_table: Tensor, lengths: Tensor, max_length: int,
+                        dtype: torch.dtype, key_scale: Tensor | None,
+                        value_scale: Tensor | None) -> tuple[Tensor, Tensor]:
+    return _hip.paged_cache_read(key_cache, value_cache, page_table, lengths, max_length, dtype, key_scale, value_scale)
+
+
+@paged_cache_read_op.register_fake
+def _(key_cache, value_cache, page_table, lengths, max_length, dtype, key_scale, value_scale):
+    shape = (page_table.shape[0], max_length, key_cache.shape[1], key_cache.shape[3])
+    return key_cache.new_empty(shape, dtype=dtype), key_cache.new_empty(shape, dtype=dtype)
+
+
+def paged_attention(query, key_cache, value_cache, page_table, lengths, query_offsets=None, *, key_scale=None,
+                    value_scale=None, window: int | None = None, sinks: int = 0, scale: float | None = None, out=None):
+    """Attention of the packed new tokens query (T, N, H) over the cached keys and values of
+    their sequences; returns (T, N, H). The new tokens' own keys are read from the cache too:
+    paged_cache_write goes first.
+
+    A token at position p of its sequence sees its keys s <= p; with a window those with
+    s > p - window, and the first `sinks` ones besides. One that sees none (a sequence of length
+    zero) gives zeros. Query heads share key/value heads as in dot_product_attention; scale
+    defaults to H ** -0.5.
+
+    out: a contiguous tensor for the result; its rows behind the last sequence
+    (query_offsets[batch] and on, a padded batch) are left as they were. Without it they are zero.
+    """
+    _refuse_gradients("paged_attention", query, key_cache, value_cache)
+    if window is None:
+        if sinks != 0:
+            raise ValueError(f"sinks needs a window, got sinks={sinks}")
+        window = 0
+    elif window < 1 or sinks < 0:
+        raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
+    scale = _default_scale(query, scale)
+    args = (query, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale, window, sinks,
+            scale)
+    if torch.compiler.is_compiling():
+        if out is None:
+            return paged_attention_op(*args)
+        raise ValueError("out is not supported under torch.compile")
+    return _hip.paged_attention(*args, out=out)
+
+
+def paged_cache_write(key, value, key_cache, value_cache, page_table, lengths, query_offsets=None, *, key_scale=None,
+                      value_scale=None) -> None:
+    """Writes key and value (T, N_kv, H) of the packed new tokens to their places in the cache, in
+    place. An e4m3 cache gets each row quantised: its scale is the smallest power of two (at least
+    2 ** -126) with which the row's largest finite magnitude stays within 448, its values round
+    to nearest even, and infinities become NaN. Rows behind the last sequence and tokens at
+    positions below zero (a sequence of length zero) are not written. No two tokens may name the
+    same place: pages that sequences share are read-only."""
+    _refuse_gradients("paged_cache_write", key, value, key_cache, value_cache)
+    call = paged_cache_write_op if torch.compiler.is_compiling() else _hip.paged_cache_write
+    call(key, value, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale)
+
+
+def paged_cache_read(key_cache, value_cache, page_table, lengths, *, max_length: int | None = None, dtype=None,
+                     key_scale=None, value_scale=None):
+    """The first max_length tokens (default: what the table can hold) of the sequences as dense
+    keys and values (batch, max_length, N_kv, H), zeros behind a sequence's length. dtype is the
+    cache's, or for an e4m3 cache bfloat16 (default) or float16, to which its values are rounded."""
+    _refuse_gradients("paged_cache_read", key_cache, value_cache)
+    if dtype is None:
+        dtype = torch.bfloat16 if key_cache.dtype == torch.float8_e4m3fn else key_cache.dtype
+    if max_length is None:
+        if page_table.ndim != 2 or key_cache.ndim != 4:
+            raise ValueError("expected a (batch, pages) page_table and a (pages, kv_heads, page_size, head_dim) cache, "
+                             f"got {tuple(page_table.shape)} and {tuple(key_cache.shape)}")
+        max_length = page_table.shape[1] * key_cache.shape[2]
+    call = paged_cache_read_op if torch.compiler.is_compiling() else _hip.paged_cache_read
+    return call(key_cache, value_cache, page_table, lengths, max_length, dtype, key_scale, value_scale)

@@ -52,7 +52,8 @@ enum fhog_status {
   FHOG_ERR_LAUNCH = 3            /* the HIP runtime rejected a kernel launch */
 };
 
-enum fhog_dtype { FHOG_DTYPE_F32 = 0, FHOG_DTYPE_F16 = 1, FHOG_DTYPE_BF16 = 2 };
+/* E4M3: paged caches only. */
+enum fhog_dtype { FHOG_DTYPE_F32 = 0, FHOG_DTYPE_F16 = 1, FHOG_DTYPE_BF16 = 2, FHOG_DTYPE_E4M3 = 3 };
 
 /* Values of the `causal` argument. */
 enum fhog_causal { FHOG_CAUSAL_NONE = 0, FHOG_CAUSAL_TOP_LEFT = 1, FHOG_CAUSAL_BOTTOM_RIGHT = 2 };
@@ -225,6 +226,63 @@ int fhog_window_attention_bwdbwd(fhog_stream_t stream,
                                  float* delta, float* ddelta, float* bstat, void* workspace,
                                  int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim,
                                  int dtype, int causal, int window, int sinks, float scale);
+
+/*
+ * The paged key/value cache (no counterpart in the reference): serving the attention that the
+ * entry points above train.
+ *
+ * k_cache, v_cache: (num_pages, kv_heads, page_size, head_dim) contiguous, of the calls' dtype
+ * (bf16 or fp16) or FHOG_DTYPE_E4M3; page_size a power of two >= 16, head_dim 64, 128 or 256.
+ * k_scale, v_scale: (num_pages, kv_heads, page_size) e8m0 bytes of an e4m3 cache (a row's values
+ * are code * 2^(byte - 127)), ignored otherwise.
+ * page_table: (batch, pages_per_seq) int32; token s of sequence b is row s % page_size of page
+ * page_table[b][s / page_size]. lengths: (batch) int32, the tokens that each sequence holds,
+ * the new ones included.
+ * query_offsets: (batch + 1) int32, rising: the new tokens of sequence b are the packed rows
+ * query_offsets[b] to query_offsets[b + 1], its last positions in order. Null: one new token a
+ * sequence (total == batch).
+ * table, lengths and offsets are device memory and read by the kernels only: no entry point
+ * waits for the device. Entries that no visible token needs may hold anything. A needed entry
+ * outside [0, num_pages), or a length beyond pages_per_seq * page_size, gives NaN rows
+ * (attention, read) or leaves the token unwritten (write); offsets are cut to [0, total].
+ */
+
+/* Bytes of workspace of fhog_paged_attention on the current device; single: query_offsets is
+ * null. Calls that may overlap need one each. */
+size_t fhog_paged_workspace_bytes(int batch, int total, int single, int heads, int kv_heads, int head_dim,
+                                  int page_size, int pages_per_seq, int window, int sinks);
+
+/*
+ * out (total, heads, head_dim): attention of the new tokens q (same shape) over the cached
+ * keys of their sequences, their own among them (written before). Token i of n new ones is at
+ * position p = length - n + i and sees the keys j <= p, with window > 0 those with j > p - window
+ * or j < sinks only. A token that sees no key gets 0. Rows behind the last sequence
+ * (query_offsets[batch] to total) are zeroed if clear_tail, else left as they were.
+ */
+int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                         const void* k_scale, const void* v_scale, const int* page_table, const int* lengths,
+                         const int* query_offsets, void* out, void* workspace, size_t workspace_bytes, int batch,
+                         int total, int heads, int kv_heads, int head_dim, int num_pages, int page_size,
+                         int pages_per_seq, int dtype, int cache_dtype, int window, int sinks, int clear_tail,
+                         float scale);
+
+/*
+ * Writes the keys and values of the new tokens, (total, kv_heads, head_dim), to their places.
+ * e4m3: a row's scale is the smallest power of two (at least 2^-126) with which its largest
+ * finite magnitude stays within 448; values round to nearest even, infinities become NaN.
+ * Every token's place must be its own; a place that two tokens name holds either's bytes.
+ */
+int fhog_paged_cache_write(fhog_stream_t stream, const void* k, const void* v, void* k_cache, void* v_cache,
+                           void* k_scale, void* v_scale, const int* page_table, const int* lengths,
+                           const int* query_offsets, int batch, int total, int kv_heads, int head_dim, int num_pages,
+                           int page_size, int pages_per_seq, int dtype, int cache_dtype);
+
+/* Tokens [0, min(length, max_length)) of each sequence, as k and v (batch, max_length, kv_heads,
+ * head_dim); zeros behind a sequence's length. */
+int fhog_paged_cache_read(fhog_stream_t stream, const void* k_cache, const void* v_cache, const void* k_scale,
+                          const void* v_scale, const int* page_table, const int* lengths, void* k, void* v, int batch,
+                          int max_length, int kv_heads, int head_dim, int num_pages, int page_size,
+                          int pages_per_seq, int dtype, int cache_dtype);
 
 #ifdef __cplusplus
 }
