@@ -35,10 +35,11 @@ constexpr int kStages = 4;  // 3 stages: 2.6 % slower at B4 N2048 H16
 // D = 64 and 128; at D = 128 the dQ kernel takes 228 VGPRs).
 constexpr int kOcc = 2;
 
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kOcc, kOcc)))
 bwd_q_kernel(BwdParams<T> p, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
@@ -90,13 +91,9 @@ bwd_q_kernel(BwdParams<T> p, int chunk, int fold) {
   const float Di = xgroup_sum(dpart);
   const float nL2 = qvalid ? -p.lse[sbase + qi] * kLog2e : 0.f;
 
-  int kend = p.nk;
-  if (CAUSAL) kend = min(kend, qb * BQ + BQ + p.coff);
-  // (uniform; saying so keeps the compiler from treating the loop as divergent)
-  const int nkt = __builtin_amdgcn_readfirstlane(kend > 0 ? (kend + BK - 1) / BK : 0);
-  int wend = p.nk;
-  if (CAUSAL) wend = max(0, min(wend, q0 + 32 + p.coff));
-  const int wkt = q0 < p.nq ? (wend + BK - 1) / BK : 0;
+  const KeyTiles<MASK> tiles(p, qb * BQ, BQ);
+  const int nkt = tiles.count;
+  const KeyBounds<MASK> sees(p, q0, 32);
 
   const float scale = p.scale;
   const float c2 = scale * kLog2e;
@@ -124,9 +121,10 @@ bwd_q_kernel(BwdParams<T> p, int chunk, int fold) {
   dma.init(row_bytes, BK, lane, kPer * (wave & 1));
   const uint32_t lds_kv = lds_base_u32(s_kv);
   const uint32_t lds_tensor = lds_kv + tensor * kTile;
-  auto issue = [&](int kt) {
+  auto issue = [&](int it) {
+    const int kt = tiles.tile(it);
     const int nvalid = p.nk - kt * BK;
-    const uint32_t dst = lds_tensor + (uint32_t)(((uint32_t)kt % NST) * kStage);
+    const uint32_t dst = lds_tensor + (uint32_t)(((uint32_t)it % NST) * kStage);
     const T* gsrc = src + (long)kt * BK * rsk;
     if (nvalid >= BK) {
       dma.issue(dst, gsrc);
@@ -143,12 +141,13 @@ bwd_q_kernel(BwdParams<T> p, int chunk, int fold) {
   for (int i = 0; i < NST - 1; ++i)
     if (i < nkt) issue(i);
 
-  for (int kt = 0; kt < nkt; ++kt) {
-    wait_tile<NST, kPer>(kt, nkt);
+  for (int it = 0; it < nkt; ++it) {
+    wait_tile<NST, kPer>(it, nkt);
     __syncthreads();
-    if (kt + NST - 1 < nkt) issue(kt + NST - 1);
-    if (kt < wkt) {
-      const uint32_t sa = lds_kv + (uint32_t)(((uint32_t)kt % NST) * kStage);  // K at 0, V at kTile
+    if (it + NST - 1 < nkt) issue(it + NST - 1);
+    const int kt = tiles.tile(it);
+    if (sees.active(kt)) {
+      const uint32_t sa = lds_kv + (uint32_t)(((uint32_t)it % NST) * kStage);  // K at 0, V at kTile
       f32x16 S = zero16(), u = u0;  // u: dP - D at D = 64, dP otherwise
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -159,11 +158,12 @@ bwd_q_kernel(BwdParams<T> p, int chunk, int fold) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) P[r] = exp2_fast(fmaf(S[r], c2, nL2));
       const int k0 = kt * BK;
-      if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff)) {
+      if ((k0 + BK > p.nk) || (CAUSAL && k0 + BK - 1 > q0 + p.coff) || sees.below(k0)) {
         const int klim = min(p.nk - 1, CAUSAL ? qi + p.coff : p.nk - 1) - k0;  // last visible key, tile-relative
+        const int klow = qi + p.coff - p.window + 1 - k0;                       // first one of the window
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (crow(r, g) > klim) P[r] = 0.f;
+          if (crow(r, g) > klim || outside<MASK>(crow(r, g), klow, p.sinks - k0)) P[r] = 0.f;
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -200,7 +200,7 @@ bwd_q_kernel(BwdParams<T> p, int chunk, int fold) {
 //
 // It serves 2-byte types at D = 64; every other type and head dim, and small
 // grids at D = 64, run bwd_pair_kernel (fhog_bwd_pair.h).
-template <typename T, int D, bool CAUSAL>
+template <typename T, int D, int MASK>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kOcc, kOcc)))
 bwd_k_kernel(BwdParams<T> p, int chunk) {
@@ -226,8 +226,11 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
   const int nbh = p.batch * p.kv_heads;
   const int nkb = (p.nk + 32 * kWaves - 1) / (32 * kWaves);
   const GridSlot gs = grid_slot(blockIdx.x, nbh, nkb, chunk);
-  const int kb = gs.rank;  // causal: the longest key columns come first
-  const int bh = gs.pair;
+  int bkb = gs.rank, bbh = gs.pair, bpart = 0;  // causal: the longest key columns come first
+  if constexpr (MASK == kWindow) sink_workgroup(p.sink, (int)blockIdx.x - nkb * nbh, nbh, bkb, bbh, bpart);
+  const int kb = bkb, bh = bbh;
+  [[maybe_unused]] const int part = bpart;
+  const QueryBounds<MASK> qs(p, kb, BKB, part, p.sink.step);
   const int b = bh / p.kv_heads, hk = bh % p.kv_heads;
   const int grp = p.heads / p.kv_heads;  // query heads per key/value head
   const long rs = (long)p.heads * D;      // query-side row stride
@@ -243,8 +246,8 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
 
   // Iteration i visits query tile qt_begin + i / grp of query head
   // hk * grp + i % grp: the heads of a group share each tile's causal bounds.
-  const int nqt = (p.nq + BQ - 1) / BQ;
-  const int qt_begin = CAUSAL ? max(0, kb * BKB - p.coff) / BQ : 0;
+  const int nqt = (qs.q_end + BQ - 1) / BQ;
+  const int qt_begin = qs.q_begin / BQ;
   const int total = nqt > qt_begin ? (nqt - qt_begin) * grp : 0;
 
   f32x16 acc_dk[DT], acc_dv[DT];
@@ -339,7 +342,7 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
         advance(nxt);
       }
       const int q0 = (qt_begin + cur.qt) * BQ;
-      const bool active = k0 < p.nk && (!CAUSAL || q0 + BQ - 1 >= k0 - p.coff);
+      const bool active = k0 < p.nk && qs.active(q0, k0);
       if (active) {
         const char* st = s_q + ((uint32_t)i % NST) * kStage;
         const uint32_t sa = lds0 + (uint32_t)(((uint32_t)i % NST) * kStage);  // Q at 0, dO at kTile
@@ -366,9 +369,9 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
         f32x16 P;
 #pragma unroll
         for (int r = 0; r < 16; ++r) P[r] = exp2_fast(S[r] * c2);
-        if ((q0 + BQ > p.nq) || (CAUSAL && q0 < k0 + 31 - p.coff)) {
-          // visible iff query >= key - coff (causal) and query < nq
-          const int qlo = (CAUSAL ? kj - p.coff : 0) - q0, qhi = p.nq - q0;
+        if (qs.masked(q0, k0)) {
+          // visible iff query >= key - coff (causal) and query < nq, or the window's bounds
+          const int qlo = qs.lo(kj) - q0, qhi = qs.hi(kj) - q0;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int m = crow(r, g);
@@ -392,6 +395,27 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
     }
   }
 
+  if constexpr (MASK == kWindow) {
+    if (kvalid && kj < p.sinks && p.sink.chunks > 0) {  // a sink's part, in fp32 (SinkGrid)
+      const long row = ((long)part * nbh + bh) * min(p.sinks, p.nk) + kj;
+      float* dst = p.sink_parts + 2 * row * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          f32x4 x, y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] = acc_dk[dt][4 * a + j] * p.scale;
+            y[j] = acc_dv[dt][4 * a + j];
+          }
+          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * a + 4 * g) = y;
+          *reinterpret_cast<f32x4*>(dst + D + 32 * dt + 8 * a + 4 * g) = x;
+        }
+      return;
+    }
+    if (part > 0) return;  // keys of the block that are no sinks
+  }
   if (kvalid) {
     T* dk = p.dk + kbase + (long)kj * rsk;
     T* dv = p.dv + kbase + (long)kj * rsk;
@@ -472,6 +496,39 @@ hipError_t launch_bwd_dkdv(const BwdParams<T>& p, hipStream_t stream) {
   return launch_bwd_pair<T, D, CAUSAL>(p, stream);
 }
 
+// dQ, then dK and dV, with a window (kernels and environment variables as above; the rules
+// are those of fhog_grid.h for windows).
+template <typename T, int D> hipError_t launch_window_dq(const BwdParams<T>& p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2 && D <= 128) {
+    const int npairs = p.batch * p.heads;
+    const char* v = std::getenv("FLASH_HOG_BWDQ");
+    const bool pair = v != nullptr && std::strcmp(v, "pair") == 0;
+    const bool compiled = v != nullptr && std::strcmp(v, "compiled") == 0;
+    if (compiled || (!pair && !window_qpair_rule(p.nq, npairs, resident_workgroups(1)))) {
+      const int nqb = (p.nq + 32 * kWaves - 1) / (32 * kWaves);
+      hipLaunchKernelGGL((bwd_q_kernel<T, D, kWindow>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
+                         grid_chunk(npairs, nqb, resident_workgroups(kOcc)), nqb);
+      return hipGetLastError();
+    }
+  }
+  return launch_bwd_qpair<T, D, kWindow>(p, stream);
+}
+template <typename T, int D> hipError_t launch_window_dkdv(const BwdParams<T>& p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2 && D == 64) {
+    const int npairs = p.batch * p.kv_heads;
+    const char* v = std::getenv("FLASH_HOG_BWD");
+    const bool pair = v != nullptr && std::strcmp(v, "pair") == 0;
+    const bool compiled = v != nullptr && std::strcmp(v, "compiled") == 0;
+    if (compiled || (!pair && !window_pair_rule(p.nk, npairs, resident_workgroups(1)))) {
+      const int nkb = (p.nk + 32 * kWaves - 1) / (32 * kWaves);
+      hipLaunchKernelGGL((bwd_k_kernel<T, D, kWindow>), dim3(key_grid<kWindow>(p, 32 * kWaves)), dim3(kThreads), 0,
+                         stream, p, grid_chunk(npairs, nkb, resident_workgroups(kOcc)));
+      return hipGetLastError();
+    }
+  }
+  return launch_bwd_pair<T, D, kWindow>(p, stream);
+}
+
 template <typename T, int D, bool CAUSAL>
 hipError_t launch_bwd(const BwdParams<T>& p, hipStream_t stream) {
   const hipError_t e = launch_bwd_dq<T, D, CAUSAL>(p, stream);
@@ -495,6 +552,18 @@ FHOG_INST(float, 64, true)
 FHOG_INST(float, 64, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
+#undef FHOG_INST
+#define FHOG_INST(T, D)                                                        \
+  template hipError_t launch_window_dq<T, D>(const BwdParams<T>&, hipStream_t); \
+  template hipError_t launch_window_dkdv<T, D>(const BwdParams<T>&, hipStream_t);
+FHOG_INST(__bf16, 64)
+FHOG_INST(__bf16, 128)
+FHOG_INST(__bf16, 256)
+FHOG_INST(_Float16, 64)
+FHOG_INST(_Float16, 128)
+FHOG_INST(_Float16, 256)
+FHOG_INST(float, 64)
+FHOG_INST(float, 128)
 #undef FHOG_INST
 
 }  // namespace fhog

@@ -83,15 +83,7 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
   // causal: the longest key columns come first, up to rank `fold`; the ranks
   // from there on run backwards (fold_rank)
   int bkb = folded(gs.rank, nkb, fold), bbh = gs.pair, bpart = 0;
-  if constexpr (MASK == kWindow) {
-    const int extra = (int)blockIdx.x - nkb * nbh;  // workgroups of sinks' further queries (SinkGrid)
-    if (extra >= 0) {
-      const int c = extra / nbh;
-      bbh = extra - c * nbh;
-      bpart = 1 + c / p.sink.blocks;
-      bkb = c % p.sink.blocks;
-    }
-  }
+  if constexpr (MASK == kWindow) sink_workgroup(p.sink, (int)blockIdx.x - nkb * nbh, nbh, bkb, bbh, bpart);
   const int kb = bkb, bh = bbh;
   [[maybe_unused]] const int part = bpart;
   const QueryBounds<MASK> qs(p, kb, BKB, part, p.sink.step);
@@ -121,6 +113,10 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
   if (total > 0) {
     const float c2 = scale * kLog2e;
     const float inv_scale = 1.0f / scale;
+    // fp32 with a window: L enters behind the score's sum, not as its start, -L / scale, whose
+    // size (60 at head dim 64) every partial sum would be rounded at: dK and dV of B1 N1000 H8
+    // D64 1.2e-6 -> 5e-7 from their 64-bit values.
+    constexpr bool kAddL = MASK == kWindow && sizeof(T) == 4;
 
     // Wave w streams part w % kPairs of tensor w / kPairs (0 = Q, 1 = dO); the
     // last wave also the tile's L and D, which it rewrites in LDS, once they
@@ -168,7 +164,7 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
     auto finish_stats = [&](int i) {
       if (wave == kStatWave && g == 0) {
         float* st = reinterpret_cast<float*>(s_q + ((uint32_t)i % NST) * kStage + 2 * kTile);
-        st[n] = -st[n] * inv_scale;
+        st[n] = kAddL ? -st[n] * kLog2e : -st[n] * inv_scale;
         st[kSR + n] = -st[kSR + n];
       }
     };
@@ -212,14 +208,15 @@ bwd_pair_kernel(BwdParams<T> p, int chunk, int fold) {
           for (int a = 0; a < 4; ++a) {
             const f32x4 v = *reinterpret_cast<const f32x4*>(sc + 8 * a + 4 * g);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) C[4 * a + j] = v[j];
+            for (int j = 0; j < 4; ++j) C[4 * a + j] = kAddL && role == 0 ? 0.f : v[j];
           }
           const uint32_t srow = sa + role * kTile;
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) C = mma<T>(fr.rowf(srow, 0, ks), res[ks], C);
           if (role == 0) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) C[r] = exp2_fast(C[r] * c2);
+            for (int r = 0; r < 16; ++r)
+              C[r] = exp2_fast(kAddL ? fmaf(C[r], c2, sc[crow(r, g)]) : C[r] * c2);
             if (qs.masked(q0, k0)) {
               // visible iff query >= key - coff (causal) and query < nq, or the window's bounds
               const int qlo = qs.lo(kj) - q0, qhi = qs.hi(kj) - q0;

@@ -340,10 +340,11 @@ bwdbwd_q_kernel(BwdBwdParams<T> p, int chunk) {
 // only vector-memory waits are the explicit ones. It serves 2-byte types at
 // D = 64; other types and head dims run bwdbwd_pair_kernel.
 // ----------------------------------------------------------------------------
-template <typename T, int D, bool CAUSAL, bool PRE>
+template <typename T, int D, int MASK, bool PRE>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(Occupancy<T, D>::value, Occupancy<T, D>::value)))
 bwdbwd_k_kernel(BwdBwdParams<T> p, int pairs, int chunk, int fold) {
+  constexpr bool CAUSAL = MASK != 0;
   typedef SwzTile<T, D> G;
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
@@ -364,8 +365,11 @@ bwdbwd_k_kernel(BwdBwdParams<T> p, int pairs, int chunk, int fold) {
   // rank `fold`; the ranks from there on run backwards, fold_rank), and with
   // pairs > 0 also a second one (block_pair).
   const GridSlot slot = grid_slot(blockIdx.x, nbh, pairs ? (nkb + 1) / 2 : nkb, chunk);
-  const int bh = slot.pair;
-  const BlockPair bp = block_pair(folded(slot.rank, nkb, fold), nkb, pairs);
+  int bbh = slot.pair, bpart = 0;
+  BlockPair bp = block_pair(folded(slot.rank, nkb, fold), nkb, pairs);
+  if constexpr (MASK == kWindow) sink_workgroup(p.sink, (int)blockIdx.x - nkb * nbh, nbh, bp.first, bbh, bpart);
+  const int bh = bbh;
+  [[maybe_unused]] const int part = bpart;
   for (int blk = 0; blk < bp.count; ++blk) {
     const int kb = blk == 0 ? bp.first : bp.second;
     if (blk > 0) __syncthreads();  // every wave is done with the previous block's ring
@@ -380,13 +384,15 @@ bwdbwd_k_kernel(BwdBwdParams<T> p, int pairs, int chunk, int fold) {
     const int k0 = kb * BKB + wave * 32;
     const int kj = k0 + n;
     const bool kvalid = kj < p.nk;
-    const int qfirst = first_contributing_query(p, kj, CAUSAL);
+    const QueryBounds<MASK> qs(p, kb, BKB, part, p.sink.step);
+    // (window mode drops the rows that see one key by their logsumexp, below)
+    const int qfirst = MASK == kWindow ? qs.lo(kj) : first_contributing_query(p, kj, CAUSAL);
 
     // Iteration i visits query tile qt_begin + i / grp of query head
     // hk * grp + i % grp (the group reduction of
     // flash_hog/jax/_pallas_gpu_kernel.py:333-370, in one ring).
-    const int nqt = (p.nq + BQ - 1) / BQ;
-    const int qt_begin = CAUSAL ? max(0, kb * BKB - p.coff) / BQ : 0;
+    const int nqt = (qs.q_end + BQ - 1) / BQ;
+    const int qt_begin = qs.q_begin / BQ;
 
     f32x16 acc_dk2[DT], acc_dv2[DT];
   #pragma unroll
@@ -435,10 +441,12 @@ bwdbwd_k_kernel(BwdBwdParams<T> p, int pairs, int chunk, int fold) {
         }
       };
       const float inv_scale = 1.0f / scale;
+      // (a query that sees one key: bwdbwd_pair_kernel)
       auto finish_stats = [&](int i) {
         if (g == 0) {
           float* st = reinterpret_cast<float*>(s_q + (i % NST) * kStage + 3 * kTile);
-          const float L = st[n], Dq = st[BQ + n], dDq = st[2 * BQ + n], Bq = st[3 * BQ + n];
+          const float L = MASK == kWindow && keys_seen<MASK>(p, (qt_begin + i / grp) * BQ + n) == 1 ? INFINITY : st[n];
+          const float Dq = st[BQ + n], dDq = st[2 * BQ + n], Bq = st[3 * BQ + n];
           st[n] = PRE ? -L : -L * inv_scale;
           st[BQ + n] = PRE ? -dDq : -dDq * inv_scale;
           st[2 * BQ + n] = -Dq;
@@ -539,7 +547,7 @@ bwdbwd_k_kernel(BwdBwdParams<T> p, int pairs, int chunk, int fold) {
           finish_stats(i + 1);
         }
         const int q0 = (qt_begin + cur.qt) * BQ;
-        const bool active = k0 < p.nk && (!CAUSAL || q0 + BQ - 1 >= k0 - p.coff);
+        const bool active = k0 < p.nk && qs.active(q0, k0);
         if (active) {
           const char* st = s_q + (i % NST) * kStage;
           const uint32_t sa = lds_q + (uint32_t)((i % NST) * kStage);  // tiles: Q, dO, ddQ
@@ -578,10 +586,10 @@ bwdbwd_k_kernel(BwdBwdParams<T> p, int pairs, int chunk, int fold) {
           f32x16 P;
   #pragma unroll
           for (int r = 0; r < 16; ++r) P[r] = exp2_fast(S[r] * c2);
-          const bool need_mask = (q0 + BQ > p.nq) || (CAUSAL && q0 < k0 + 31 - p.coff) || p.nk == 1;
+          const bool need_mask = qs.masked(q0, k0) || p.nk == 1;
           if (need_mask) {
-            // a pair enters iff qfirst <= query < nq
-            const int qlo = qfirst - q0, qhi = p.nq - q0;
+            // a pair enters iff qfirst <= query < nq (or the window's end)
+            const int qlo = qfirst - q0, qhi = qs.hi(kj) - q0;
   #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int m = crow(r, g);
@@ -614,6 +622,27 @@ bwdbwd_k_kernel(BwdBwdParams<T> p, int pairs, int chunk, int fold) {
       }
     }
 
+    if constexpr (MASK == kWindow) {
+      if (kvalid && kj < p.sinks && p.sink.chunks > 0) {  // a sink's part, in fp32 (SinkGrid)
+        const long row = ((long)part * nbh + bh) * min(p.sinks, p.nk) + kj;
+        float* dst = p.sink_parts + 2 * row * D;
+  #pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+  #pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            f32x4 x, y;
+  #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[j] = acc_dk2[dt][4 * a + j] * p.scale;
+              y[j] = acc_dv2[dt][4 * a + j];
+            }
+            *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * a + 4 * g) = y;
+            *reinterpret_cast<f32x4*>(dst + D + 32 * dt + 8 * a + 4 * g) = x;
+          }
+        return;
+      }
+      if (part > 0) return;  // keys of the block that are no sinks
+    }
     if (kvalid) {
       const float scale = p.scale;
       T* dk2 = p.dk2 + kbase + (long)kj * rsk;
@@ -662,6 +691,27 @@ inline bool stage2_pair_selected(const char* v, Mask m, int npairs) {
   if (named(v, "pair")) return true;
   if (named(v, "compiled")) return false;
   return stage2_pair_rule(m, npairs, resident_workgroups(1));
+}
+
+// Stage 2 with a window (kernels and environment variable as below).
+template <typename T, int D> hipError_t launch_window_stage2(const BwdBwdParams<T>& p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2 && D == 64) {
+    const char* v = std::getenv("FLASH_HOG_STAGE2");
+    const int npairs = p.batch * p.kv_heads;
+    if (named(v, "compiled") || (!named(v, "pair") && !window_stage2_pair_rule(p.nk, npairs, resident_workgroups(1)))) {
+      const int nkb = (p.nk + 32 * kWaves - 1) / (32 * kWaves);
+      const int chunk = grid_chunk(npairs, nkb, resident_workgroups(Occupancy<T, D>::value));
+      const dim3 grid(key_grid<kWindow>(p, 32 * kWaves));
+      int e2;
+      if (std::is_same_v<T, __bf16> && std::frexp(p.scale, &e2) == 0.5f)  // scale = 2^(e2 - 1)
+        hipLaunchKernelGGL((bwdbwd_k_kernel<T, D, kWindow, std::is_same_v<T, __bf16>>), grid, dim3(kThreads), 0, stream,
+                           p, 0, chunk, nkb);
+      else
+        hipLaunchKernelGGL((bwdbwd_k_kernel<T, D, kWindow, false>), grid, dim3(kThreads), 0, stream, p, 0, chunk, nkb);
+      return hipGetLastError();
+    }
+  }
+  return launch_bwdbwd_stage2_pair<T, D, kWindow>(p, stream);
 }
 
 template <typename T, int D, bool CAUSAL>
@@ -734,6 +784,16 @@ FHOG_INST(float, 64, true)
 FHOG_INST(float, 64, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
+#undef FHOG_INST
+#define FHOG_INST(T, D) template hipError_t launch_window_stage2<T, D>(const BwdBwdParams<T>&, hipStream_t);
+FHOG_INST(__bf16, 64)
+FHOG_INST(__bf16, 128)
+FHOG_INST(__bf16, 256)
+FHOG_INST(_Float16, 64)
+FHOG_INST(_Float16, 128)
+FHOG_INST(_Float16, 256)
+FHOG_INST(float, 64)
+FHOG_INST(float, 128)
 #undef FHOG_INST
 
 }  // namespace fhog

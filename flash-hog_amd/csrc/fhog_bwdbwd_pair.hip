@@ -85,15 +85,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   // causal: the longest key columns come first, up to rank `fold`; the ranks
   // from there on run backwards (fold_rank)
   int bkb = folded(gs.rank, nkb, fold), bbh = gs.pair, bpart = 0;
-  if constexpr (MASK == kWindow) {
-    const int extra = (int)blockIdx.x - nkb * nbh;  // workgroups of sinks' further queries (SinkGrid)
-    if (extra >= 0) {
-      const int c = extra / nbh;
-      bbh = extra - c * nbh;
-      bpart = 1 + c / p.sink.blocks;
-      bkb = c % p.sink.blocks;
-    }
-  }
+  if constexpr (MASK == kWindow) sink_workgroup(p.sink, (int)blockIdx.x - nkb * nbh, nbh, bkb, bbh, bpart);
   const int kb = bkb, bh = bbh;
   [[maybe_unused]] const int part = bpart;
   const QueryBounds<MASK> qs(p, kb, BKB, part, p.sink.step);
@@ -124,6 +116,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
   if (total > 0) {
     const float scale = p.scale;
     const float inv_scale = 1.0f / scale;
+    constexpr bool kAddL = MASK == kWindow && sizeof(T) == 4;  // bwd_pair_kernel
     SwzFrags<T, D> fr;
     fr.init(lane);
     // Wave w streams quarter w of each of the three tiles, the last wave also
@@ -173,7 +166,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
         float* st = reinterpret_cast<float*>(s_q + ((uint32_t)i % NST) * kStage + 3 * kTile);
         const float L = MASK == kWindow && keys_seen<MASK>(p, q0 + n) == 1 ? INFINITY : st[n];
         const float Dq = st[BQ + n], dDq = st[2 * BQ + n], Bq = st[3 * BQ + n];
-        st[n] = PRE ? -L : -L * inv_scale;
+        st[n] = PRE ? -L : kAddL ? -L * kLog2e : -L * inv_scale;
         st[BQ + n] = PRE ? -dDq : -dDq * inv_scale;
         st[2 * BQ + n] = -Dq;
         st[3 * BQ + n] = -fmaf(Dq, dDq, Bq);
@@ -241,7 +234,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
             const f32x4 v1 = *reinterpret_cast<const f32x4*>(sc + BQ + 8 * a + 4 * g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              C0[4 * a + j] = v0[j];
+              C0[4 * a + j] = kAddL && role == 0 ? 0.f : v0[j];
               C1[4 * a + j] = v1[j];
             }
           }
@@ -256,7 +249,7 @@ bwdbwd_pair_kernel(BwdBwdParams<T> p, int chunk, int fold) {
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              C0[r] = exp2_fast(C0[r] * c2);
+              C0[r] = exp2_fast(kAddL ? fmaf(C0[r], c2, sc[crow(r, g)]) : C0[r] * c2);
               if (!PRE) C1[r] *= scale;
             }
             if (qs.masked(q0, k0) || p.nk == 1) {

@@ -413,6 +413,10 @@ inline int sink_chunks(Mask m, int window, int sinks) {
   return sinks > 0 && first < m.nq ? (int)((m.nq - begin + step - 1) / step) : 0;
 }
 
+inline bool window_qpair_rule(int nq, int npairs, int cus) { return (long)((nq + 63) / 64) * npairs <= cus; }
+inline bool window_pair_rule(int nk, int npairs, int cus) { return (long)((nk + 63) / 64) * npairs <= 2l * cus; }
+inline bool window_stage2_pair_rule(int nk, int npairs, int cus) { return (long)((nk + 63) / 64) * npairs <= 2l * cus; }
+
 // Paged attention: which kernel, how many tiles of rows ("slots") and how a sequence's keys are
 // split. `single`: one new token a sequence, no offsets.
 struct PagedPlan {

@@ -129,6 +129,9 @@ hipError_t launch_bwdbwd_stage2_pair(const BwdBwdParams<T>& p, hipStream_t s);
 
 // The first backward and the double backward with a window of keys and sinks; the
 // forward is launch_fwd<T, D, kWindow>.
+template <typename T, int D> hipError_t launch_window_dq(const BwdParams<T>& p, hipStream_t s);
+template <typename T, int D> hipError_t launch_window_dkdv(const BwdParams<T>& p, hipStream_t s);
+template <typename T, int D> hipError_t launch_window_stage2(const BwdBwdParams<T>& p, hipStream_t s);
 template <typename T, int D> hipError_t launch_window_bwd(const BwdParams<T>& p, hipStream_t s);
 template <typename T, int D> hipError_t launch_window_bwdbwd(const BwdBwdParams<T>& p, hipStream_t s);
 

@@ -97,6 +97,16 @@ struct SinkGrid {
   int step;    // queries of a chunk, a multiple of 32
 };
 
+// The block, (batch, head) pair and part of workgroup `extra` of those behind the ordinary ones
+// (extra < 0: an ordinary one, which has them already).
+__device__ __forceinline__ void sink_workgroup(const SinkGrid& sink, int extra, int pairs, int& kb, int& pair, int& part) {
+  if (extra < 0) return;
+  const int c = extra / pairs;
+  pair = extra - c * pairs;
+  part = 1 + c / sink.blocks;
+  kb = c % sink.blocks;
+}
+
 // One workgroup's share of that grid: key block kb and queries [q_begin, q_end), of which
 // key j takes [lo(j), hi(j)).
 template <int MASK> struct QueryBounds {

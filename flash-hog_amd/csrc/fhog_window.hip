@@ -47,8 +47,8 @@ hipError_t join(const P& p, T* dk, T* dv, hipStream_t stream) {
 }  // namespace
 
 template <typename T, int D> hipError_t launch_window_bwd(const BwdParams<T>& p, hipStream_t stream) {
-  hipError_t e = launch_bwd_qpair<T, D, kWindow>(p, stream);
-  if (e == hipSuccess) e = launch_bwd_pair<T, D, kWindow>(p, stream);
+  hipError_t e = launch_window_dq<T, D>(p, stream);
+  if (e == hipSuccess) e = launch_window_dkdv<T, D>(p, stream);
   return e == hipSuccess ? join<T, D>(p, p.dk, p.dv, stream) : e;
 }
 
@@ -60,7 +60,7 @@ template <typename T, int D> hipError_t launch_window_bwdbwd(const BwdBwdParams<
     e = launch_bwdbwd_stage1_fused_pair<T, kWindow>(p, stream);
   else
     e = launch_bwdbwd_stage1_fused<T, D, kWindow>(p, stream);
-  if (e == hipSuccess) e = launch_bwdbwd_stage2_pair<T, D, kWindow>(p, stream);
+  if (e == hipSuccess) e = launch_window_stage2<T, D>(p, stream);
   return e == hipSuccess ? join<T, D>(p, p.dk2, p.dv2, stream) : e;
 }
 

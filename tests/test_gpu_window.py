@@ -131,3 +131,12 @@ def test_kernels(case, cuda_device):
 @pytest.mark.parametrize("case", [CASES[4], CASES[12], CASES[16], CASES[20], CASES[23]], ids=case_id)
 def test_other_scales(case, scale, cuda_device):
     run_case(case, cuda_device, scale=scale, seed=11)
+
+
+@pytest.mark.parametrize("variant", ["compiled", "pair"])
+@pytest.mark.parametrize("case", [c for c in CASES if c[6] != FP32 and c[5] <= 128][1::2], ids=case_id)
+def test_kernel_variants(case, variant, cuda_device, monkeypatch):
+    """The kernels with one wave and with two per 32 rows, whichever the sizes would choose."""
+    for name in ("FLASH_HOG_BWD", "FLASH_HOG_BWDQ", "FLASH_HOG_STAGE2"):
+        monkeypatch.setenv(name, variant)
+    run_case(case, cuda_device, seed=17)
