@@ -491,7 +491,7 @@ size_t fhog_paged_workspace_bytes(int batch, int total, int single, int heads, i
   const Paged s{batch, total, heads, kv_heads, head_dim, 1, page_size, pages_per_seq, FHOG_DTYPE_BF16, FHOG_DTYPE_BF16};
   if (check_paged(s, "fhog_paged_workspace_bytes") || window < 0 || sinks < 0 || batch < 1 || total < 1) return 0;
   const fhog::PagedPlan plan = fhog::paged_plan(batch, total, single != 0, heads, kv_heads,
-                                                (long)page_size * pages_per_seq, window, sinks, compute_units());
+                                                head_dim, (long)page_size * pages_per_seq, window, sinks, compute_units());
   return (size_t)plan.parts * (head_dim + 2) * sizeof(float);
 }
 
@@ -522,7 +522,7 @@ int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cach
   if (window > most) window = most;
   if (sinks > most) sinks = most;
   const fhog::PagedPlan plan = fhog::paged_plan(batch, total, query_offsets == nullptr, heads, kv_heads,
-                                                (long)page_size * pages_per_seq, window, sinks, compute_units());
+                                                head_dim, (long)page_size * pages_per_seq, window, sinks, compute_units());
   if ((long long)plan.slots * kv_heads >= (1ll << 31) || plan.splits > 65535)
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
   const size_t need = (size_t)plan.parts * (head_dim + 2) * sizeof(float);
@@ -533,7 +533,7 @@ int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cach
                               {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
                               cache_shape(s, page_table, lengths, query_offsets), (float*)workspace, heads, window,
                               sinks, plan.slots, plan.splits, plan.split_tiles, clear_tail, scale};
-    return fhog::launch_paged_attention<T, C, D>(p, plan.chunk, (hipStream_t)stream);
+    return fhog::launch_paged_attention<T, C, D>(p, plan.rows, (hipStream_t)stream);
   };
   return launch_status(dispatch_paged(s, run), who);
 }

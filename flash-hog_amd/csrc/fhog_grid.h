@@ -420,20 +420,32 @@ inline bool window_stage2_pair_rule(int nk, int npairs, int cus) { return (long)
 // Paged attention: which kernel, how many tiles of rows ("slots") and how a sequence's keys are
 // split. `single`: one new token a sequence, no offsets.
 struct PagedPlan {
-  bool chunk;       // 128-row tiles (paged_chunk_kernel), else 16 (paged_token_kernel)
-  int rows, slots;
+  int rows, slots;  // of a tile: 16 (paged_token_kernel), 64 or 128 (paged_chunk_kernel)
+  int waves;        // of a workgroup of paged_token_kernel
   int splits, split_tiles;  // splits of split_tiles 32-key tiles; one split: no join
   long parts;       // fp32 rows of head_dim + 2 in the workspace
 };
-inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv_heads, long capacity, int window,
-                            int sinks, int cus) {
+constexpr int kJoinWeights = 2048;  // the most rows of a tile times splits
+#ifndef FHOG_TT
+#define FHOG_TT 8l
+#endif
+#ifndef FHOG_CR
+#define FHOG_CR 2l
+#endif
+#ifndef FHOG_CT
+#define FHOG_CT 2l
+#endif
+inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv_heads, int head_dim, long capacity,
+                            int window, int sinks, int cus) {
   if (cus <= 0) cus = 256;
   PagedPlan p;
   const int group = heads / kv_heads;
-  // More than 16 rows a sequence on average (tokens times heads of a group): the wide tile.
-  p.chunk = (long)total * group > 16l * batch;
-  p.rows = p.chunk ? 128 : 16;
-  p.slots = (int)(single ? (long)batch * ((group + p.rows - 1) / p.rows) : (long)total * group / p.rows + batch);
+  auto slots = [&](int rows) {
+    return single ? (long)batch * ((group + rows - 1) / rows) : (long)total * group / rows + batch;
+  };
+  // More than 16 rows a sequence on average (tokens times heads of a group): the wide tiles.
+  p.rows = (long)total * group <= 16l * batch ? 16 : slots(128) * kv_heads >= FHOG_CR * cus ? 128 : 64;
+  p.slots = (int)slots(p.rows);
   // The most tiles that a tile of rows reads: with a window its keys, those between the tile's
   // first and last position and the sinks.
   long keys = capacity;
@@ -442,11 +454,22 @@ inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv
     if (most < keys) keys = most;
   }
   const long tiles = (keys + 31) / 32 + 2;
-  const long blocks = (long)p.slots * kv_heads, target = (p.chunk ? 2l : 4l) * cus;
-  long split_tiles = blocks >= target ? tiles : (tiles * blocks + target - 1) / target;
-  if (split_tiles < 8) split_tiles = 8;
-  p.splits = (int)((tiles + split_tiles - 1) / split_tiles);
-  p.split_tiles = (int)split_tiles;
+  const long blocks = (long)p.slots * kv_heads;
+  p.waves = head_dim == 64 ? 8 : head_dim == 128 ? 4 : 2;
+  long target, least;
+  if (p.rows > 16) {
+    target = FHOG_CT * cus;
+    least = 8;
+  } else {
+    target = FHOG_TT * cus;
+    least = 2 * blocks < cus ? (head_dim == 64 ? 32 : 8) : (blocks < 2l * cus ? 8l : 32l) * p.waves;
+  }
+  long splits = blocks >= target ? 1 : (target + blocks - 1) / blocks;
+  if (splits > tiles / least) splits = tiles / least;
+  if (splits > kJoinWeights / p.rows) splits = kJoinWeights / p.rows;
+  if (splits < 1) splits = 1;
+  p.split_tiles = (int)((tiles + splits - 1) / splits);
+  p.splits = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
   p.parts = p.splits > 1 ? blocks * p.splits * p.rows : 0;
   return p;
 }

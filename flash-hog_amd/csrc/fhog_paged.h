@@ -71,7 +71,7 @@ template <typename T, typename C> struct CacheReadParams {
   int max_length;
 };
 
-template <typename T, typename C, int D> hipError_t launch_paged_attention(const PagedParams<T, C>& p, bool chunk, hipStream_t s);
+template <typename T, typename C, int D> hipError_t launch_paged_attention(const PagedParams<T, C>& p, int rows, hipStream_t s);
 template <typename T, typename C, int D> hipError_t launch_cache_write(const CacheWriteParams<T, C>& p, hipStream_t s);
 template <typename T, typename C, int D> hipError_t launch_cache_read(const CacheReadParams<T, C>& p, hipStream_t s);
 
@@ -120,14 +120,15 @@ template <typename T> __device__ __forceinline__ V4<T> dequantise4(uint32_t x, f
 // The power of two that an e8m0 code stands for.
 __device__ __forceinline__ float scale_of(uint32_t code) { return __builtin_bit_cast(float, code << 23); }
 
-template <typename T, typename C, int D, int THREADS, int SWZ> struct PageTile {
+// TENSORS: 2 for keys and values, 1 for values alone.
+template <typename T, typename C, int D, int THREADS, int SWZ, int TENSORS = 2> struct PageTile {
   static constexpr bool kQuantised = sizeof(C) == 1;
   static constexpr int kPerLoad = 16 / (int)sizeof(C);  // elements
   static constexpr int kChunks = D / kPerLoad;          // 16-byte pieces of a row
   static constexpr int kTensor = 32 * kChunks;          // of a tile of one tensor
-  static constexpr int kLoads = 2 * kTensor / THREADS;  // a thread's, keys and values
+  static constexpr int kLoads = TENSORS * kTensor / THREADS;  // a thread's
   static constexpr int kTileBytes = 32 * D * (int)sizeof(T);
-  static_assert(2 * kTensor % THREADS == 0, "tile must divide into whole loads");
+  static_assert(TENSORS * kTensor % THREADS == 0, "tile must divide into whole loads");
   u32x4 data[kLoads];
   uint32_t code[kQuantised ? kLoads : 1];
 
@@ -140,7 +141,7 @@ template <typename T, typename C, int D, int THREADS, int SWZ> struct PageTile {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int at = i * THREADS + thread;
-      const bool value = at >= kTensor;
+      const bool value = TENSORS == 1 || at >= kTensor;
       const int row = min(max(at % kTensor / kChunks, rlo), rhi);
       const long head = (long)(row < 16 ? page0 : page1) * kv_heads + hk;
       const long line = (head << page_shift) + ((k0 + row) & (page_rows - 1));
@@ -150,14 +151,14 @@ template <typename T, typename C, int D, int THREADS, int SWZ> struct PageTile {
     }
   }
 
-  // To LDS: the tile of keys at byte address lds, that of values behind it.
+  // To LDS: the tile of keys at byte address lds, that of values behind it (or there).
   __device__ __forceinline__ void store(uint32_t lds, int thread) const {
     typedef __attribute__((address_space(3))) char lds_char;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int at = i * THREADS + thread;
       const int row = at % kTensor / kChunks, chunk = at % kChunks;
-      const uint32_t base = lds + (at >= kTensor ? kTileBytes : 0) + row * D * (int)sizeof(T);
+      const uint32_t base = lds + (TENSORS == 2 && at >= kTensor ? kTileBytes : 0) + row * D * (int)sizeof(T);
       auto put = [&](int c, u32x4 x) {
         *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(
             reinterpret_cast<lds_char*>((uintptr_t)(base + 16 * phys_chunk<SWZ>(row, c)))) = x;
@@ -172,6 +173,47 @@ template <typename T, typename C, int D, int THREADS, int SWZ> struct PageTile {
       } else {
         put(chunk, data[i]);
       }
+    }
+  }
+};
+
+// A tile's keys as one wave's operands of the 16x16x32 score products, straight from their pages:
+// lane (n, g) holds pieces of keys n and 16 + n. A piece is 16 bytes of cache: 8 elements, columns
+// 32 c + 8 g on, one product's; or 16 of e4m3, columns 64 c + 16 g on, two products' (the
+// contraction may take the columns in any order that the queries share).
+template <typename T, typename C, int D> struct KeyPieces {
+  static constexpr bool kQuantised = sizeof(C) == 1;
+  static constexpr int kPieces = D / (kQuantised ? 64 : 32);
+  u32x4 data[2][kPieces];
+  uint32_t code[kQuantised ? 2 : 1];
+
+  // Column of the queries that product ks takes, for lane group g.
+  __device__ __forceinline__ static int column(int ks, int g) {
+    return kQuantised ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
+  }
+  __device__ __forceinline__ void fetch(const CacheRows<C>& cache, int hk, int kv_heads, int page_shift, int k0,
+                                        int rlo, int rhi, int page0, int page1, int n, int g) {
+    const int page_rows = 1 << page_shift;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int row = min(max(16 * kb + n, rlo), rhi);  // (PageTile::fetch)
+      const long head = (long)(row < 16 ? page0 : page1) * kv_heads + hk;
+      const long line = (head << page_shift) + ((k0 + row) & (page_rows - 1));
+      const C* src = cache.k + line * D + g * (kQuantised ? 16 : 8);
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c)
+        data[kb][c] = *reinterpret_cast<const u32x4*>(src + c * (kQuantised ? 64 : 32));
+      if constexpr (kQuantised) code[kb] = cache.k_scale[line];
+    }
+  }
+  __device__ __forceinline__ V8<T> operand(int kb, int ks) const {
+    if constexpr (kQuantised) {
+      const u32x4 x = data[kb][ks >> 1];
+      const float scale = scale_of(code[kb]);
+      const V4<T> a = dequantise4<T>(x[2 * (ks & 1)], scale), b = dequantise4<T>(x[2 * (ks & 1) + 1], scale);
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return __builtin_bit_cast(V8<T>, data[kb][ks]);
     }
   }
 };

@@ -11,7 +11,8 @@
 // paged_token_kernel, for few rows a sequence: 16 rows a workgroup, whose waves take every
 // kWaves-th tile of 32 keys each on their own, through LDS of their own (no barrier in
 // the sweep), and join at the end.
-// paged_chunk_kernel, for many: 128 rows a workgroup, 32 a wave, all on the same tile.
+// paged_chunk_kernel, for many: 32 rows a wave, 128 rows a workgroup, all its waves on the same
+// tile, or 64 rows and two tiles at a time.
 //
 // Where tiles of rows are few, a sequence's keys are dealt to several workgroups (splits of
 // split_tiles tiles), which leave unnormalised fp32 outputs with their maxima and sums;
@@ -74,19 +75,31 @@ template <int D, typename P> __device__ __forceinline__ void clear_tail(const P&
   for (long i = begin + (long)worker * threads + threadIdx.x; i < end; i += (long)workers * threads) out[i] = u32x4{0, 0, 0, 0};
 }
 
-// The pages of a tile's two halves.
+// The pages of a tile's two halves, loaded a step before the tile's rows are.
 struct Pages {
-  int page0, page1;
-  bool bad;
-  __device__ __forceinline__ void load(const CacheShape& c, int b, int k0, int rlo, int rhi) {
-    // (each half's page from the nearest row that is read)
-    const int* row = c.table + (long)b * c.pages_per_seq;
-    page0 = row[(k0 + min(rlo, 15)) >> c.page_shift];
-    page1 = rhi >= 16 ? row[(k0 + 16) >> c.page_shift] : page0;
-    bad = (unsigned)page0 >= (unsigned)c.pages || (unsigned)page1 >= (unsigned)c.pages;
+  int page0 = 0, page1 = 0;
+  // `zero` is 0 in a vector register: the same address in every lane, but a vector load,
+  // which is waited for in order. A scalar one would be waited for with the step's first LDS
+  // read.
+  __device__ __forceinline__ void load(const CacheShape& c, const PageSpan& span, int b, int t, int zero) {
+    const int k0 = span.key(t), rhi = span.last_row(t);
+    // (each half's page from a row that is read)
+    const int* row = c.table + (long)b * c.pages_per_seq + zero;
+    page0 = row[(k0 + span.first_row(t)) >> c.page_shift];
+    page1 = row[(k0 + min(rhi, 16)) >> c.page_shift];
+  }
+  // Replaces pages that are none by page 0; whether there were any.
+  __device__ __forceinline__ bool check(const CacheShape& c) {
+    const bool bad = (unsigned)page0 >= (unsigned)c.pages || (unsigned)page1 >= (unsigned)c.pages;
     if (bad) page0 = page1 = 0;
+    return bad;
   }
 };
+__device__ __forceinline__ int vector_zero() {
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  return zero;
+}
 
 // Where split `split` of a tile of rows leaves its output (ROWS rows of D) and, behind all
 // outputs, its rows' maxima and sums.
@@ -103,19 +116,20 @@ template <int ROWS, int D, typename P> struct Parts {
 
 // ------------------------------------------------------------------ few rows
 
-template <typename T, typename C, int D> struct Token {
-  static constexpr int kRows = 16;
-  static constexpr int kWaves = D == 256 ? 2 : 4;  // LDS: a tile of keys and values a wave
-  static constexpr int kThreads = 64 * kWaves;
-};
+constexpr int kTokenRows = 16;
 
-template <typename T, typename C, int D>
-__global__ void __launch_bounds__((Token<T, C, D>::kThreads))
+template <typename T, typename C, int D, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves)
 paged_token_kernel(PagedParams<T, C> p) {
-  constexpr int kWaves = Token<T, C, D>::kWaves, ROWS = Token<T, C, D>::kRows;
+  constexpr int ROWS = kTokenRows;
   constexpr int KS = D / 32, DB = D / 16;
-  typedef PageTile<T, C, D, 64, kSwzRows> Tile;
-  constexpr int kWaveLds = 2 * Tile::kTileBytes;
+  // e4m3 keys go straight into operands (128.0 -> 125.3 us for 16 sequences of up to 32768 keys,
+  // 32 heads over 8, D = 128); 2-byte ones, whose operand loads take half lines, through LDS
+  // (215 us against 221).
+  typedef KeyPieces<T, C, D> Keys;
+  constexpr bool kDirect = Keys::kQuantised;
+  typedef PageTile<T, C, D, 64, kSwzRows, kDirect ? 1 : 2> Tile;
+  constexpr int kWaveLds = (kDirect ? 1 : 2) * Tile::kTileBytes;
   __shared__ __attribute__((aligned(1024))) char s_kv[kWaves * kWaveLds];
   __shared__ float s_ml[kWaves][ROWS][2];
 
@@ -123,7 +137,7 @@ paged_token_kernel(PagedParams<T, C> p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads, split = blockIdx.y;
-  clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, Token<T, C, D>::kThreads);
+  clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 64 * kWaves);
   const RowTile rt = RowTile::template at<ROWS>(p, slot);
   if (rt.rows <= 0) return;
   const int first_pos = __builtin_amdgcn_readfirstlane(rt.position(0));
@@ -139,7 +153,8 @@ paged_token_kernel(PagedParams<T, C> p) {
   V8<T> qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    qf[ks] = *reinterpret_cast<const V8<T>*>(p.q + rt.offset(r, hk, p.heads, D) + 32 * ks + 8 * g);
+    qf[ks] = *reinterpret_cast<const V8<T>*>(p.q + rt.offset(r, hk, p.heads, D) +
+                                             (kDirect ? Keys::column(ks, g) : 32 * ks + 8 * g));
     if (negate) qf[ks] = -qf[ks];
   }
   const float c2 = fabsf(p.scale) * kLog2e;
@@ -153,29 +168,42 @@ paged_token_kernel(PagedParams<T, C> p) {
   for (int db = 0; db < DB; ++db) acc[db] = zero4();
   bool bad = rt.beyond;
 
+  Keys keys;
   Tile tile;
+  Pages pages;
+  const int zero = vector_zero();
+  // Fetches tile t, whose pages are there, and loads those of this wave's next one.
   auto fetch = [&](int t) {
+    bad |= pages.check(p.at);
     const int k0 = span.key(t), rlo = span.first_row(t), rhi = span.last_row(t);
-    Pages pg;
-    pg.load(p.at, rt.b, k0, rlo, rhi);
-    bad |= pg.bad;
-    tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, k0, rlo, rhi, pg.page0, pg.page1, lane);
+    if constexpr (kDirect)
+      keys.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, k0, rlo, rhi, pages.page0, pages.page1, n, g);
+    tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, k0, rlo, rhi, pages.page0, pages.page1, lane);
+    if (t + kWaves < t1) pages.load(p.at, span, rt.b, t + kWaves, zero);
   };
   int t = t0 + wave;
-  if (t < t1) fetch(t);
+  if (t < t1) {
+    pages.load(p.at, span, rt.b, t, zero);
+    fetch(t);
+  }
   for (; t < t1; t += kWaves) {
+    const int k0 = span.key(t), rlo = span.first_row(t), rhi = span.last_row(t);
+    f32x4 S[2];
+    auto scores = [&](auto&& keys_of) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        S[kb] = zero4();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) S[kb] = mma16<T>(keys_of(kb, ks), qf[ks], S[kb]);
+      }
+    };
+    // (before the next tile takes the registers)
+    if constexpr (kDirect) scores([&](int kb, int ks) { return keys.operand(kb, ks); });
     __builtin_amdgcn_wave_barrier();  // (the wave's LDS operations run in order; only the compiler could move them)
     tile.store(lds, lane);
     __builtin_amdgcn_wave_barrier();
     if (t + kWaves < t1) fetch(t + kWaves);
-    const int k0 = span.key(t), rlo = span.first_row(t), rhi = span.last_row(t);
-    f32x4 S[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      S[kb] = zero4();
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) S[kb] = mma16<T>(fr.rowf(lds, 0, kb, ks), qf[ks], S[kb]);
-    }
+    if constexpr (!kDirect) scores([&](int kb, int ks) { return fr.rowf(lds, 0, kb, ks); });
     if (rlo > 0 || rhi < 31 || k0 + 31 > first_pos || (p.window && k0 <= last_pos - p.window)) {
       const int klim = min(rhi, pos - k0);
       const int klow = p.window ? pos - p.window + 1 - k0 : 0, ksinks = p.sinks - k0;
@@ -213,7 +241,7 @@ paged_token_kernel(PagedParams<T, C> p) {
     lpart += psum;
     const V8<T> oP = cvt8<T>(P);
 #pragma unroll
-    for (int db = 0; db < DB; ++db) acc[db] = mma16<T>(fr.trf(lds, Tile::kTileBytes, db), oP, acc[db]);
+    for (int db = 0; db < DB; ++db) acc[db] = mma16<T>(fr.trf(lds, kDirect ? 0 : Tile::kTileBytes, db), oP, acc[db]);
   }
 
   // The waves' outputs meet in LDS, in place of the tiles: (wave, column, row), so that the
@@ -233,7 +261,7 @@ paged_token_kernel(PagedParams<T, C> p) {
   }
   __syncthreads();
   Parts<ROWS, D, PagedParams<T, C>> parts(p, slot, hk, split);
-  for (int i = threadIdx.x; i < ROWS * (D / 4); i += Token<T, C, D>::kThreads) {
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += 64 * kWaves) {
     const int row = i / (D / 4), col = 4 * (i % (D / 4));
     if (row >= rt.rows) break;
     float top = s_ml[0][row][0];
@@ -263,20 +291,25 @@ paged_token_kernel(PagedParams<T, C> p) {
 
 // ------------------------------------------------------------------ many rows
 
-constexpr int kChunkRows = 128;
-
-template <typename T, typename C, int D>
+// Waves that share a tile of keys, 32 rows each: RW of four; the 4 / RW groups of them take
+// every (4 / RW)-th tile and join at the end.
+// (128 rows at D = 128: three waves per SIMD, 168 registers and 8 of them spilled outside the
+// loop, 158 -> 142 us for 8 sequences with 17 to 512 new tokens of 32 heads over 8, window 2048.)
+template <typename T, typename C, int D, int RW>
 __global__ void __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+__attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 64 || RW == 4 ? 3 : 2)))
 paged_chunk_kernel(PagedParams<T, C> p) {
-  constexpr int ROWS = kChunkRows;
+  constexpr int ROWS = 32 * RW, KW = 4 / RW;
   constexpr int KS = D / 16, DT = D / 32;
-  typedef PageTile<T, C, D, 256, kSwzPairs> Tile;
+  typedef PageTile<T, C, D, 64 * RW, kSwzPairs> Tile;
   constexpr int kStage = 2 * Tile::kTileBytes;
-  __shared__ __attribute__((aligned(1024))) char s_kv[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) char s_kv[KW * 2 * kStage];
+  __shared__ float s_ml[KW][ROWS][2];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % RW, kw = wave / RW;
+  const int thread = threadIdx.x % (64 * RW);  // of its group
   const int n = lane & 31, g = lane >> 5;
   const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads, split = blockIdx.y;
   clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 256);
@@ -289,12 +322,12 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   const int t1 = __builtin_amdgcn_readfirstlane(min(span.tiles, t0 + p.split_tiles));
   if (split > 0 && t0 >= t1) return;
 
-  // This wave's rows, from 32 * wave on, and this lane's.
-  const bool any = 32 * wave < rt.rows;
-  const int wfirst = __builtin_amdgcn_readfirstlane(rt.position(min(32 * wave, rt.rows - 1)));
-  const int wlast = __builtin_amdgcn_readfirstlane(rt.position(min(32 * wave + 31, rt.rows - 1)));
-  const int r = min(32 * wave + n, rt.rows - 1);
-  const bool valid = 32 * wave + n < rt.rows;
+  // This wave's rows, from 32 * rw on, and this lane's.
+  const bool any = 32 * rw < rt.rows;
+  const int wfirst = __builtin_amdgcn_readfirstlane(rt.position(min(32 * rw, rt.rows - 1)));
+  const int wlast = __builtin_amdgcn_readfirstlane(rt.position(min(32 * rw + 31, rt.rows - 1)));
+  const int row = 32 * rw + n;
+  const int r = min(row, rt.rows - 1);
   const int pos = rt.position(r);
   const bool negate = p.scale < 0.f;
   V8<T> qf[KS];
@@ -307,7 +340,7 @@ paged_chunk_kernel(PagedParams<T, C> p) {
 
   SwzFrags<T, D> fr;
   fr.init(lane);
-  const uint32_t lds = lds_base_u32(s_kv);
+  const uint32_t lds = lds_base_u32(s_kv) + kw * 2 * kStage;
   float m = -1e30f, lpart = 0.f;
   f32x16 acc[DT];
 #pragma unroll
@@ -315,32 +348,39 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   bool bad = rt.beyond;
 
   Tile tile;
+  Pages pages;
+  const int zero = vector_zero();
+  // Fetches tile t, whose pages are there, and loads those of this group's next one.
   auto fetch = [&](int t) {
-    const int k0 = span.key(t), rlo = span.first_row(t), rhi = span.last_row(t);
-    Pages pg;
-    pg.load(p.at, rt.b, k0, rlo, rhi);
-    bad |= pg.bad;
-    tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, k0, rlo, rhi, pg.page0, pg.page1, threadIdx.x);
+    bad |= pages.check(p.at);
+    tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, span.key(t), span.first_row(t), span.last_row(t),
+               pages.page0, pages.page1, thread);
+    if (t + KW < t1) pages.load(p.at, span, rt.b, t + KW, zero);
   };
-  // Tile t is stored to stage t % 2 in iteration t - 1, whose barrier at its end shows it; the
-  // stage's last readers passed the barrier of iteration t - 2.
-  if (t0 < t1) {
-    fetch(t0);
-    tile.store(lds + (t0 & 1) * kStage, threadIdx.x);
-    if (t0 + 1 < t1) fetch(t0 + 1);
+  // In step i a group works on tile t0 + kw + KW i, if there is one. It was stored to stage
+  // i % 2 in step i - 1, whose barrier at its end shows it; the stage's last readers passed the
+  // barrier of step i - 2.
+  const int steps = (t1 - t0 + KW - 1) / KW;
+  const int mine = t0 + kw;
+  if (mine < t1) {
+    pages.load(p.at, span, rt.b, mine, zero);
+    fetch(mine);
+    tile.store(lds, thread);
+    if (mine + KW < t1) fetch(mine + KW);
   }
   __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    if (t + 1 < t1) {
-      tile.store(lds + ((t + 1) & 1) * kStage, threadIdx.x);
-      if (t + 2 < t1) fetch(t + 2);
+  for (int i = 0; i < steps; ++i) {
+    const int t = mine + KW * i;
+    if (t + KW < t1) {
+      tile.store(lds + ((i + 1) & 1) * kStage, thread);
+      if (t + 2 * KW < t1) fetch(t + 2 * KW);
     }
     const int k0 = span.key(t);
     // a wave's own positions: nothing before its window's start or behind its last row
-    const bool active = any && k0 <= wlast &&
+    const bool active = any && t < t1 && k0 <= wlast &&
                         (t < span.sink_tiles || !p.window || k0 + 31 > wfirst - p.window || k0 < p.sinks);
     if (active) {
-      const uint32_t sa = lds + (t & 1) * kStage;
+      const uint32_t sa = lds + (i & 1) * kStage;
       f32x16 S = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) S = mma<T>(fr.rowf(sa, 0, ks), qf[ks], S);
@@ -349,18 +389,18 @@ paged_chunk_kernel(PagedParams<T, C> p) {
         const int klim = min(rhi, pos - k0);
         const int klow = p.window ? pos - p.window + 1 - k0 : 0, ksinks = p.sinks - k0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = crow(i, g);
-          if (key > klim || key < rlo || (key < klow && key >= ksinks)) S[i] = -INFINITY;
+        for (int j = 0; j < 16; ++j) {
+          const int key = crow(j, g);
+          if (key > klim || key < rlo || (key < klow && key >= ksinks)) S[j] = -INFINITY;
         }
       }
       f32x16 P;
       auto probabilities = [&] {
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          P[i] = exp2_fast(fmaf(S[i], c2, -m));  // masked: exp2(-inf) = 0
-          sum += P[i];
+        for (int j = 0; j < 16; ++j) {
+          P[j] = exp2_fast(fmaf(S[j], c2, -m));  // masked: exp2(-inf) = 0
+          sum += P[j];
         }
         return sum;
       };
@@ -368,7 +408,7 @@ paged_chunk_kernel(PagedParams<T, C> p) {
       if (__any(!(psum <= kBound))) {
         float top = S[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, S[i]);
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, S[j]);
         const float mnew = fmaxf(m, xgroup_max(top * c2));
         const float alpha = exp2_fast(m - mnew);
         lpart *= alpha;
@@ -389,9 +429,43 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   }
 
   if (bad) lpart = NAN;
-  const float l = xgroup_sum(lpart);
-  if (!valid) return;
-  const int row = 32 * wave + n;
+  float l = xgroup_sum(lpart);
+  if constexpr (KW > 1) {
+    // The other groups hand their sums to the first, in LDS in place of the tiles.
+    static_assert((KW - 1) * RW * DT * 4096 <= KW * 2 * kStage, "the join reuses the tiles");
+    float* box = reinterpret_cast<float*>(s_kv) + 4 * lane;
+    auto place = [&](int k, int dt, int a) { return box + 256 * (((k - 1) * RW + rw) * DT * 4 + 4 * dt + a); };
+    if (kw > 0) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *reinterpret_cast<f32x4*>(place(kw, dt, a)) =
+              f32x4{acc[dt][4 * a], acc[dt][4 * a + 1], acc[dt][4 * a + 2], acc[dt][4 * a + 3]};
+      if (g == 0) {
+        s_ml[kw][row][0] = m;
+        s_ml[kw][row][1] = l;
+      }
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int k = 1; k < KW; ++k) {
+      const float mk = s_ml[k][row][0], top = fmaxf(m, mk);
+      const float f = exp2_fast(m - top), fk = exp2_fast(mk - top);
+      l = l * f + s_ml[k][row][1] * fk;
+      m = top;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(place(k, dt, a));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[dt][4 * a + j] = acc[dt][4 * a + j] * f + y[j] * fk;
+        }
+    }
+  }
+  if (row >= rt.rows) return;
   if (p.splits > 1) {
     Parts<ROWS, D, PagedParams<T, C>> parts(p, slot, hk, split);
 #pragma unroll
@@ -421,28 +495,54 @@ paged_chunk_kernel(PagedParams<T, C> p) {
 
 // ------------------------------------------------------------------ the splits' join
 
-// One workgroup a tile of rows and key/value head; the splits in order, four columns a thread.
+// One workgroup a tile of rows and key/value head. Its rows' weights 2^(m - top) / sum come
+// first, in LDS; then each thread sums four columns of a row over the splits, or, where the
+// tile has fewer of those than there are threads, over every `ways`-th split, and the ways
+// meet in LDS. Always in the same order. (A thread that walked all splits of a short tile by
+// itself: 45 us behind 128 splits of one sequence of 32768 keys, 4 heads.)
 template <typename T, typename C, int D, int ROWS>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(PagedParams<T, C> p) {
+  __shared__ float s_w[kJoinWeights];
+  __shared__ f32x4 s_o[256];
   const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads;
   const RowTile rt = RowTile::template at<ROWS>(p, slot);
   if (rt.rows <= 0) return;
   const PageSpan span(rt.position(0), rt.position(rt.rows - 1), rt.length, p.window, p.sinks);
   const int splits = max(1, min(p.splits, (span.tiles + p.split_tiles - 1) / p.split_tiles));
-  for (int i = threadIdx.x; i < rt.rows * (D / 4); i += 256) {
-    const int row = i / (D / 4), col = 4 * (i % (D / 4));
+  const Parts<ROWS, D, PagedParams<T, C>> parts(p, slot, hk, 0);  // (a tile's splits are neighbours)
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int row = wave; row < rt.rows; row += 4) {
     float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, Parts<ROWS, D, PagedParams<T, C>>(p, slot, hk, s).ml[2 * row]);
+    for (int i = lane; i < splits; i += 64) top = fmaxf(top, parts.ml[2 * (i * ROWS + row)]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    for (int i = lane; i < splits; i += 64) sum += exp2_fast(parts.ml[2 * (i * ROWS + row)] - top) * parts.ml[2 * (i * ROWS + row) + 1];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: 0
+    for (int i = lane; i < splits; i += 64) s_w[row * splits + i] = exp2_fast(parts.ml[2 * (i * ROWS + row)] - top) * inv;
+  }
+  __syncthreads();
+  const int units = rt.rows * (D / 4);
+  int ways = 1;
+  while (2 * ways * units <= 256 && 2 * ways <= splits) ways *= 2;
+  for (int u0 = 0; u0 < units; u0 += 256 / ways) {
+    const int way = (int)threadIdx.x / (256 / ways), u = u0 + (int)threadIdx.x % (256 / ways);
+    const int row = u / (D / 4), col = 4 * (u % (D / 4));
     f32x4 o = zero4();
-    for (int s = 0; s < splits; ++s) {
-      const Parts<ROWS, D, PagedParams<T, C>> part(p, slot, hk, s);
-      const float f = exp2_fast(part.ml[2 * row] - top);
-      sum += f * part.ml[2 * row + 1];
-      o += f * *reinterpret_cast<const f32x4*>(part.out + row * D + col);
+    if (u < units) {
+#pragma unroll 4
+      for (int i = way; i < splits; i += ways)
+        o += s_w[row * splits + i] * *reinterpret_cast<const f32x4*>(parts.out + (long)(i * ROWS + row) * D + col);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<V4<T>*>(p.out + rt.offset(row, hk, p.heads, D) + col) = cvt4<T>(o * inv);
+    if (ways > 1) {  // (then this is the only round: units fit 256 / ways threads)
+      s_o[threadIdx.x] = o;
+      __syncthreads();
+      for (int w = 1; w < ways && way == 0; ++w) o += s_o[w * (256 / ways) + threadIdx.x];
+    }
+    if (way == 0 && u < units)
+      *reinterpret_cast<V4<T>*>(p.out + rt.offset(row, hk, p.heads, D) + col) = cvt4<T>(o);
   }
 }
 
@@ -457,19 +557,23 @@ hipError_t join(const PagedParams<T, C>& p, hipStream_t stream) {
 }  // namespace
 
 template <typename T, typename C, int D>
-hipError_t launch_paged_attention(const PagedParams<T, C>& p, bool chunk, hipStream_t stream) {
+hipError_t launch_paged_attention(const PagedParams<T, C>& p, int rows, hipStream_t stream) {
   const dim3 grid(p.slots * p.at.kv_heads, p.splits);
-  if (chunk) {
-    hipLaunchKernelGGL((paged_chunk_kernel<T, C, D>), grid, dim3(256), 0, stream, p);
-    return join<T, C, D, kChunkRows>(p, stream);
+  if (rows == 128) {
+    hipLaunchKernelGGL((paged_chunk_kernel<T, C, D, 4>), grid, dim3(256), 0, stream, p);
+    return join<T, C, D, 128>(p, stream);
   }
-  typedef Token<T, C, D> K;
-  hipLaunchKernelGGL((paged_token_kernel<T, C, D>), grid, dim3(K::kThreads), 0, stream, p);
-  return join<T, C, D, K::kRows>(p, stream);
+  if (rows == 64) {
+    hipLaunchKernelGGL((paged_chunk_kernel<T, C, D, 2>), grid, dim3(256), 0, stream, p);
+    return join<T, C, D, 64>(p, stream);
+  }
+  constexpr int kWaves = D == 64 ? 8 : D == 128 ? 4 : 2;
+  hipLaunchKernelGGL((paged_token_kernel<T, C, D, kWaves>), grid, dim3(64 * kWaves), 0, stream, p);
+  return join<T, C, D, kTokenRows>(p, stream);
 }
 
 #define FHOG_INST(T, C, D) \
-  template hipError_t launch_paged_attention<T, C, D>(const PagedParams<T, C>&, bool, hipStream_t);
+  template hipError_t launch_paged_attention<T, C, D>(const PagedParams<T, C>&, int, hipStream_t);
 FHOG_INST(__bf16, __bf16, 64)
 FHOG_INST(__bf16, __bf16, 128)
 FHOG_INST(__bf16, __bf16, 256)
