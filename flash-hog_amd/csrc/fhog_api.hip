@@ -131,8 +131,10 @@ int check_window(const Shape& s, int window, int sinks, Window* w, const char* w
   w->window = window < most ? window : most;  // positions are below `most`
   w->sinks = sinks < s.n_k ? sinks : s.n_k;
   const fhog::Mask m{true, s.n_q, s.n_k, s.coff()};
-  w->sink = fhog::SinkGrid{(w->sinks + 63) / 64, fhog::sink_chunks(m, w->window, w->sinks),
-                           fhog::sink_step(w->window, w->sinks)};
+  const int row_bytes = s.head_dim * (s.dtype == FHOG_DTYPE_F32 ? 4 : 2);
+  const fhog::SinkChunks c = fhog::sink_chunks(m, w->window, w->sinks, row_bytes, (long)s.batch * s.heads,
+                                               (long)s.batch * s.kv_heads);
+  w->sink = fhog::SinkGrid{(w->sinks + 31) / 32, c.count, c.step, c.apart};
   const long long groups = ((s.n_k + 63) / 64 + (long long)w->sink.blocks * w->sink.chunks) * s.batch * s.kv_heads;
   if (groups >= (1ll << 31)) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
   return FHOG_OK;
@@ -413,9 +415,9 @@ int fhog_attention_bwdbwd_noalloc(fhog_stream_t stream, const void* q, const voi
                      causal, scale);
 }
 
-size_t fhog_window_workspace_bytes(int batch, int n_q, int n_k, int kv_heads, int head_dim, int causal, int window,
-                                   int sinks) {
-  const Shape s{batch, n_q, n_k, kv_heads, kv_heads, head_dim, FHOG_DTYPE_BF16, causal, 1.0f};
+size_t fhog_window_workspace_bytes(int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim, int dtype,
+                                   int causal, int window, int sinks) {
+  const Shape s{batch, n_q, n_k, heads, kv_heads, head_dim, dtype, causal, 1.0f};
   Window w;
   if (check_window(s, window, sinks, &w, "fhog_window_workspace_bytes")) return 0;
   return sink_parts_bytes(s, w);

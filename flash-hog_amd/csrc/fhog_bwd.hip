@@ -200,7 +200,7 @@ bwd_q_kernel(BwdParams<T> p, int chunk, int fold) {
 //
 // It serves 2-byte types at D = 64; every other type and head dim, and small
 // grids at D = 64, run bwd_pair_kernel (fhog_bwd_pair.h).
-template <typename T, int D, int MASK>
+template <typename T, int D, bool CAUSAL>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kOcc, kOcc)))
 bwd_k_kernel(BwdParams<T> p, int chunk) {
@@ -226,11 +226,8 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
   const int nbh = p.batch * p.kv_heads;
   const int nkb = (p.nk + 32 * kWaves - 1) / (32 * kWaves);
   const GridSlot gs = grid_slot(blockIdx.x, nbh, nkb, chunk);
-  int bkb = gs.rank, bbh = gs.pair, bpart = 0;  // causal: the longest key columns come first
-  if constexpr (MASK == kWindow) sink_workgroup(p.sink, (int)blockIdx.x - nkb * nbh, nbh, bkb, bbh, bpart);
-  const int kb = bkb, bh = bbh;
-  [[maybe_unused]] const int part = bpart;
-  const QueryBounds<MASK> qs(p, kb, BKB, part, p.sink.step);
+  const int kb = gs.rank;  // causal: the longest key columns come first
+  const int bh = gs.pair;
   const int b = bh / p.kv_heads, hk = bh % p.kv_heads;
   const int grp = p.heads / p.kv_heads;  // query heads per key/value head
   const long rs = (long)p.heads * D;      // query-side row stride
@@ -246,8 +243,8 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
 
   // Iteration i visits query tile qt_begin + i / grp of query head
   // hk * grp + i % grp: the heads of a group share each tile's causal bounds.
-  const int nqt = (qs.q_end + BQ - 1) / BQ;
-  const int qt_begin = qs.q_begin / BQ;
+  const int nqt = (p.nq + BQ - 1) / BQ;
+  const int qt_begin = CAUSAL ? max(0, kb * BKB - p.coff) / BQ : 0;
   const int total = nqt > qt_begin ? (nqt - qt_begin) * grp : 0;
 
   f32x16 acc_dk[DT], acc_dv[DT];
@@ -342,7 +339,7 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
         advance(nxt);
       }
       const int q0 = (qt_begin + cur.qt) * BQ;
-      const bool active = k0 < p.nk && qs.active(q0, k0);
+      const bool active = k0 < p.nk && (!CAUSAL || q0 + BQ - 1 >= k0 - p.coff);
       if (active) {
         const char* st = s_q + ((uint32_t)i % NST) * kStage;
         const uint32_t sa = lds0 + (uint32_t)(((uint32_t)i % NST) * kStage);  // Q at 0, dO at kTile
@@ -369,9 +366,9 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
         f32x16 P;
 #pragma unroll
         for (int r = 0; r < 16; ++r) P[r] = exp2_fast(S[r] * c2);
-        if (qs.masked(q0, k0)) {
-          // visible iff query >= key - coff (causal) and query < nq, or the window's bounds
-          const int qlo = qs.lo(kj) - q0, qhi = qs.hi(kj) - q0;
+        if ((q0 + BQ > p.nq) || (CAUSAL && q0 < k0 + 31 - p.coff)) {
+          // visible iff query >= key - coff (causal) and query < nq
+          const int qlo = (CAUSAL ? kj - p.coff : 0) - q0, qhi = p.nq - q0;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int m = crow(r, g);
@@ -395,27 +392,6 @@ bwd_k_kernel(BwdParams<T> p, int chunk) {
     }
   }
 
-  if constexpr (MASK == kWindow) {
-    if (kvalid && kj < p.sinks && p.sink.chunks > 0) {  // a sink's part, in fp32 (SinkGrid)
-      const long row = ((long)part * nbh + bh) * min(p.sinks, p.nk) + kj;
-      float* dst = p.sink_parts + 2 * row * D;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          f32x4 x, y;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = acc_dk[dt][4 * a + j] * p.scale;
-            y[j] = acc_dv[dt][4 * a + j];
-          }
-          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * a + 4 * g) = y;
-          *reinterpret_cast<f32x4*>(dst + D + 32 * dt + 8 * a + 4 * g) = x;
-        }
-      return;
-    }
-    if (part > 0) return;  // keys of the block that are no sinks
-  }
   if (kvalid) {
     T* dk = p.dk + kbase + (long)kj * rsk;
     T* dv = p.dv + kbase + (long)kj * rsk;
@@ -496,15 +472,18 @@ hipError_t launch_bwd_dkdv(const BwdParams<T>& p, hipStream_t stream) {
   return launch_bwd_pair<T, D, CAUSAL>(p, stream);
 }
 
-// dQ, then dK and dV, with a window (kernels and environment variables as above; the rules
-// are those of fhog_grid.h for windows).
+// dQ with a window: FLASH_HOG_BWDQ = few (rows of up to 256 bytes), compiled or pair, or the
+// rules of fhog_grid.h.
 template <typename T, int D> hipError_t launch_window_dq(const BwdParams<T>& p, hipStream_t stream) {
+  const char* v = std::getenv("FLASH_HOG_BWDQ");
+  const int npairs = p.batch * p.heads;
+  if constexpr (kFewServes<T, D>) {
+    if (window_few_selected(v, p.nq, npairs, D * (int)sizeof(T))) return launch_few_dq<T, D>(p, stream);
+  }
   if constexpr (sizeof(T) == 2 && D <= 128) {
-    const int npairs = p.batch * p.heads;
-    const char* v = std::getenv("FLASH_HOG_BWDQ");
     const bool pair = v != nullptr && std::strcmp(v, "pair") == 0;
     const bool compiled = v != nullptr && std::strcmp(v, "compiled") == 0;
-    if (compiled || (!pair && !window_qpair_rule(p.nq, npairs, resident_workgroups(1)))) {
+    if (compiled || (!pair && !window_qpair_rule(p.nq, p.window, npairs, D, resident_workgroups(1)))) {
       const int nqb = (p.nq + 32 * kWaves - 1) / (32 * kWaves);
       hipLaunchKernelGGL((bwd_q_kernel<T, D, kWindow>), dim3(nqb * npairs), dim3(kThreads), 0, stream, p,
                          grid_chunk(npairs, nqb, resident_workgroups(kOcc)), nqb);
@@ -512,21 +491,6 @@ template <typename T, int D> hipError_t launch_window_dq(const BwdParams<T>& p, 
     }
   }
   return launch_bwd_qpair<T, D, kWindow>(p, stream);
-}
-template <typename T, int D> hipError_t launch_window_dkdv(const BwdParams<T>& p, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2 && D == 64) {
-    const int npairs = p.batch * p.kv_heads;
-    const char* v = std::getenv("FLASH_HOG_BWD");
-    const bool pair = v != nullptr && std::strcmp(v, "pair") == 0;
-    const bool compiled = v != nullptr && std::strcmp(v, "compiled") == 0;
-    if (compiled || (!pair && !window_pair_rule(p.nk, npairs, resident_workgroups(1)))) {
-      const int nkb = (p.nk + 32 * kWaves - 1) / (32 * kWaves);
-      hipLaunchKernelGGL((bwd_k_kernel<T, D, kWindow>), dim3(key_grid<kWindow>(p, 32 * kWaves)), dim3(kThreads), 0,
-                         stream, p, grid_chunk(npairs, nkb, resident_workgroups(kOcc)));
-      return hipGetLastError();
-    }
-  }
-  return launch_bwd_pair<T, D, kWindow>(p, stream);
 }
 
 template <typename T, int D, bool CAUSAL>
@@ -553,9 +517,7 @@ FHOG_INST(float, 64, false)
 FHOG_INST(float, 128, true)
 FHOG_INST(float, 128, false)
 #undef FHOG_INST
-#define FHOG_INST(T, D)                                                        \
-  template hipError_t launch_window_dq<T, D>(const BwdParams<T>&, hipStream_t); \
-  template hipError_t launch_window_dkdv<T, D>(const BwdParams<T>&, hipStream_t);
+#define FHOG_INST(T, D) template hipError_t launch_window_dq<T, D>(const BwdParams<T>&, hipStream_t);
 FHOG_INST(__bf16, 64)
 FHOG_INST(__bf16, 128)
 FHOG_INST(__bf16, 256)

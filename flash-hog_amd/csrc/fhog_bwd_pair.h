@@ -310,7 +310,9 @@ hipError_t launch_bwd_pair(const BwdParams<T>& p, hipStream_t stream) {
   const int nkb = (p.nk + 32 * kPairs - 1) / (32 * kPairs);
   const int npairs = p.batch * p.kv_heads;
   const int cus = resident_workgroups(1);
-  [[maybe_unused]] const int waves = bwd_pair_waves(mask_of(MASK != 0, p), npairs, D, (int)sizeof(T), cus);
+  // (a window's blocks are as even as a rectangle's that the diagonal hardly touches)
+  const Mask rule = MASK == kWindow ? Mask{false, p.nq, p.nk, 0} : mask_of(MASK != 0, p);
+  [[maybe_unused]] const int waves = bwd_pair_waves(rule, npairs, D, (int)sizeof(T), cus);
   if constexpr (sizeof(T) == 4 && D == 64) {
     return launch_occ<T, D, MASK, 3>(p, nkb, npairs, cus, stream);
   } else {

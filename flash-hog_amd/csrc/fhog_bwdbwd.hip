@@ -694,7 +694,17 @@ inline bool stage2_pair_selected(const char* v, Mask m, int npairs) {
 }
 
 // Stage 2 with a window (kernels and environment variable as below).
-template <typename T, int D> hipError_t launch_window_stage2(const BwdBwdParams<T>& p, hipStream_t stream) {
+template <typename T, int D> hipError_t launch_window_stage2(const BwdBwdParams<T>& p_, hipStream_t stream) {
+  BwdBwdParams<T> p = p_;
+  if constexpr (kFewServes<T, D>) {
+    if (p.sink.apart && p.sink.chunks > 0) {
+      const hipError_t e = launch_few_stage2<T, D>(p, true, stream);
+      if (e != hipSuccess) return e;
+    }
+    p = own_launch(p);
+    if (window_few_selected(std::getenv("FLASH_HOG_STAGE2"), p.nk, p.batch * p.kv_heads, D * (int)sizeof(T), true))
+      return launch_few_stage2<T, D>(p, false, stream);
+  }
   if constexpr (sizeof(T) == 2 && D == 64) {
     const char* v = std::getenv("FLASH_HOG_STAGE2");
     const int npairs = p.batch * p.kv_heads;

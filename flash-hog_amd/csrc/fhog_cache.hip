@@ -48,15 +48,28 @@ template <typename T> __device__ __forceinline__ u32x2 quantise8(V8<T> x, int la
   return y;
 }
 
-template <typename T, typename C, int D>
+// A workgroup takes HEADS heads of kRows packed rows: it reads whole lines at a stride, and what it
+// writes, neighbouring rows of a head's page and their scales, is contiguous. The rows are
+// loaded before their places are looked up, four dependent loads that four heads share where
+// there are many rows. Four prompts of up to 8192 tokens, 16 heads, D = 64, e4m3: 47.8 us
+// with neighbouring threads on one row's heads, 43.8 with a head a workgroup, 40.8 with four.
+template <typename T, typename C, int D, int HEADS>
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(CacheWriteParams<T, C> p) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 8, kRows = kThreads / kLanes;
   const CacheShape& c = p.at;
-  const long i = (long)blockIdx.x * kThreads + threadIdx.x;  // (packed row, kv_head, eight columns)
-  const int col = 8 * (int)(i % kLanes), hk = (int)(i / kLanes % c.kv_heads);
-  const long token = i / kLanes / c.kv_heads;
-  // (all lanes of a row take the same way, so the shuffles below find each other)
+  const int groups = (c.kv_heads + HEADS - 1) / HEADS;
+  const int col = 8 * (int)(threadIdx.x % kLanes), hk0 = (int)(blockIdx.x % groups) * HEADS;
+  const long token = (long)(blockIdx.x / groups) * kRows + threadIdx.x / kLanes;
+  // (all lanes of a row take the same way, so quantise8's shuffles find each other)
   if (token >= c.total) return;
+  const int heads = min(HEADS, c.kv_heads - hk0);
+  V8<T> k[HEADS], v[HEADS];
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    const long from = (token * c.kv_heads + hk0 + min(h, heads - 1)) * D + col;
+    k[h] = *reinterpret_cast<const V8<T>*>(p.k + from);
+    v[h] = *reinterpret_cast<const V8<T>*>(p.v + from);
+  }
   const int t = (int)token;
   const int b = c.offsets ? last_at_or_before(c.batch, t, [&](int s) { return packed_begin(c, s); }) : t;
   const int begin = packed_begin(c, b), end = c.offsets ? packed_begin(c, b + 1) : b + 1;
@@ -65,22 +78,24 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(CacheWriteParams<
   if (pos < 0 || (pos >> c.page_shift) >= c.pages_per_seq) return;
   const int page = c.table[(long)b * c.pages_per_seq + (pos >> c.page_shift)];
   if ((unsigned)page >= (unsigned)c.pages) return;
-  const long line = (((long)page * c.kv_heads + hk) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
-  const long from = (token * c.kv_heads + hk) * D + col, to = line * D + col;
-  const V8<T> k = *reinterpret_cast<const V8<T>*>(p.k + from);
-  const V8<T> v = *reinterpret_cast<const V8<T>*>(p.v + from);
-  if constexpr (sizeof(C) == 1) {
-    uint32_t kc, vc;
-    const u32x2 kq = quantise8<T>(k, kLanes, kc), vq = quantise8<T>(v, kLanes, vc);
-    *reinterpret_cast<u32x2*>(p.k_cache + to) = kq;
-    *reinterpret_cast<u32x2*>(p.v_cache + to) = vq;
-    if (col == 0) {
-      p.k_scale[line] = (uint8_t)kc;
-      p.v_scale[line] = (uint8_t)vc;
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    if (h >= heads) break;
+    const long line = (((long)page * c.kv_heads + hk0 + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+    const long to = line * D + col;
+    if constexpr (sizeof(C) == 1) {
+      uint32_t kc, vc;
+      const u32x2 kq = quantise8<T>(k[h], kLanes, kc), vq = quantise8<T>(v[h], kLanes, vc);
+      *reinterpret_cast<u32x2*>(p.k_cache + to) = kq;
+      *reinterpret_cast<u32x2*>(p.v_cache + to) = vq;
+      if (col == 0) {
+        p.k_scale[line] = (uint8_t)kc;
+        p.v_scale[line] = (uint8_t)vc;
+      }
+    } else {
+      *reinterpret_cast<V8<T>*>(p.k_cache + to) = k[h];
+      *reinterpret_cast<V8<T>*>(p.v_cache + to) = v[h];
     }
-  } else {
-    *reinterpret_cast<V8<T>*>(p.k_cache + to) = k;
-    *reinterpret_cast<V8<T>*>(p.v_cache + to) = v;
   }
 }
 
@@ -124,9 +139,14 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheReadParams<T,
 
 template <typename T, typename C, int D>
 hipError_t launch_cache_write(const CacheWriteParams<T, C>& p, hipStream_t stream) {
-  const long threads = (long)p.at.total * p.at.kv_heads * (D / 8);
-  hipLaunchKernelGGL((cache_write_kernel<T, C, D>), dim3((unsigned)((threads + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, stream, p);
+  constexpr int kRows = kThreads / (D / 8);
+  const long blocks = ((long)p.at.total + kRows - 1) / kRows;
+  const int groups = (p.at.kv_heads + 3) / 4;
+  if (blocks * groups >= 1024)
+    hipLaunchKernelGGL((cache_write_kernel<T, C, D, 4>), dim3((unsigned)(blocks * groups)), dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((cache_write_kernel<T, C, D, 1>), dim3((unsigned)(blocks * p.at.kv_heads)), dim3(kThreads), 0,
+                       stream, p);
   return hipGetLastError();
 }
 

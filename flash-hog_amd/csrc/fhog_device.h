@@ -564,16 +564,6 @@ __device__ __forceinline__ BlockPair block_pair(int rank, int nb, int pairs) {
   return BlockPair{rank, second, (pairs && second != rank) ? 2 : 1};
 }
 
-// Workgroups of 4 waves resident on the current device at once, at `waves`
-// waves per SIMD (0 if the device cannot be queried).
-inline int resident_workgroups(int waves) {
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-    return 0;
-  return cus * waves;
-}
-
 // Block of a rank, the ranks from `fold` (fold_rank) on running backwards.
 __device__ __forceinline__ int folded(int rank, int nb, int fold) { return rank < fold ? rank : nb - 1 - (rank - fold); }
 

@@ -395,26 +395,57 @@ inline bool q32_deal_rule(Mask m, int npairs, int cus) {
   return load.folded > (near_square(m, 4) ? 1.07 : 1.15) * load.dealt;
 }
 
-// Windowed attention, key-tiled kernels (64-key blocks): queries per chunk of those that see
-// a sink as a sink only, and how many chunks that makes. A chunk is as long as an ordinary
-// block's share, window + 64, so that no workgroup outlasts the others; at least 512 queries,
-// so that the parts that the chunks leave stay few where the window is short; and at least
-// twice the number of sinks, which keeps all parts together below (n_q / 2 + 2 sinks) rows of
-// dK and dV a head.
-inline int sink_step(int window, int sinks) {
-  long step = window + 64l;
-  if (step < 512) step = 512;
-  if (step < 2l * sinks) step = 2l * sinks;
-  return (int)((step < (1l << 30) ? step : 1l << 30) + 31) / 32 * 32;
-}
-inline int sink_chunks(Mask m, int window, int sinks) {
+// Windowed attention, key-tiled kernels: the queries that see a sink as a sink only, in `count`
+// chunks of `step`. In the launch of the ordinary blocks a chunk is as long as a block's share,
+// window + 64, so that no workgroup outlasts the others, and at least 512 queries, so that its
+// parts stay few where the window is short. Its workgroup holds 64 or 128 keys of which
+// few are sinks, though, so that in long calls they go `apart`, in a launch of
+// fhog_window_few.hip: about one chunk a CU, of 128 queries (a tile a wave) or more. A call is
+// long if its ordinary blocks stream over 200 tiles a CU (256 of them: the workspace's size
+// depends on it, so not on the device). dK/dV and stage 2 together, us, H12 D64 bf16 unless named,
+// one launch / apart: B1 N2048 window 512 (27 tiles) 57 / 68, B2 81 / 101, B32 N500 window 100 (60)
+// 167 / 170, H16 D128 N8192 window 512 (144) 331 / 356, B4 N2048 H16 (144) 184 / 178, B8 N2048 H16 over 4
+// key heads fp16 (288) 346 / 312, N16384 window 1024 (408) 451 / 435, B2 N4001 H32 over 8 key heads D128
+// fp16 (535) 1002 / 966. Always at least twice the number of sinks, which keeps all parts
+// together below (n_q / 2 + 2 sinks) rows of dK and dV a head.
+struct SinkChunks {
+  bool apart;
+  int step, count;
+};
+inline SinkChunks sink_chunks(Mask m, int window, int sinks, int row_bytes, long heads, long npairs) {
   const long first = window - (long)m.coff, begin = first > 0 ? first / 32 * 32 : 0;  // the first that sees key 0 so
-  const int step = sink_step(window, sinks);
-  return sinks > 0 && first < m.nq ? (int)((m.nq - begin + step - 1) / step) : 0;
+  const long queries = m.nq - begin, share = window + 64l;
+  const bool apart = row_bytes <= 256 && (m.nk + 63l) / 64 * heads * (share / 32) > 200l * 256;
+  long step = apart ? 128 : share > 512 ? share : 512;
+  if (apart && step * 256 < queries * npairs) step = (queries * npairs + 255) / 256;
+  if (step < 2l * sinks) step = 2l * sinks;
+  step = (step + 31) / 32 * 32;
+  return SinkChunks{apart, (int)step, sinks > 0 && first < m.nq ? (int)((queries + step - 1) / step) : 0};
 }
 
-inline bool window_qpair_rule(int nq, int npairs, int cus) { return (long)((nq + 63) / 64) * npairs <= cus; }
-inline bool window_pair_rule(int nk, int npairs, int cus) { return (long)((nk + 63) / 64) * npairs <= 2l * cus; }
+// The kernels of fhog_window_few.hip (one 32-row block a workgroup, its window's tiles dealt to
+// four waves) take a call of at most as many blocks as are resident at once: two a CU where
+// rows have 128 bytes, one where they have 256 and in stage 2. us, few / others, causal H12
+// D64 bf16 window 128 to 512 unless named; forward: B1 N300 (120 blocks) 9.4 / 12.6, N1000 (384)
+// 13.2 / 16.0, N2048 (768) 25.5 / 21.3, N1000 H16 D128 (512) 22.3 / 19.6, N1000 H8 fp32 (256) 17.9 /
+// 23.4; dQ: 7.4 / 11.3, 11.2 / 15.0, 23.5 / 22.7, 21.7 / 19.2, 18.5 / 29.3; dK/dV: 6.5 / 8.1, 10.6 /
+// 11.8, 24.6 / 21.4, over 4 key heads at D128 (128) 20.8 / 43.4, 21.6 / 28.7; stage 2: 9.1 / 11.3,
+// 21.8 / 16.0, 45.9 / 32.6, 39.9 / 65.8, 38.1 / 60.6.
+inline bool window_few_rule(int rows, int npairs, int row_bytes, bool stage2, int cus) {
+  return (long)((rows + 31) / 32) * npairs <= (row_bytes <= 128 && !stage2 ? 2l : 1l) * cus;
+}
+// Beyond, for 2-byte types: dQ at D = 64 and 128 in bwd_q_kernel (128-query blocks) or, on grids of
+// at most one workgroup per CU or where those cover so much more than 64-query ones, in
+// bwd_qpair_kernel; stage 2 at D = 64 in bwdbwd_k_kernel, up to two pair workgroups per CU in
+// bwdbwd_pair_kernel. All others, and dK/dV, have pair kernels only. us, one wave / pair, H12 D64 bf16
+// unless named; dQ: N16384 window 1024 130 / 151, B4 N2048 H16 window 512 55.5 / 55.6, N4096 window 256
+// 25.2 / 23.3, B32 N500 window 100 54.7 / 47.7, D128: B2 N4001 H32 fp16 window 1024 232 / 283, N8192
+// H16 window 512 97 / 107; stage 2: N2048 window 512 (384 pair workgroups) 36.1 / 32.4, B2 (768) 50.8 / 53.0,
+// B32 N500 76 / 82, N16384 247 / 318; dK/dV: N2048 23.7 / 21.1, B2 31.7 / 32.4, B32 N500 51.5 / 42.3, N16384 155 /
+// 152.
+inline bool window_qpair_rule(int nq, int window, int npairs, int head_dim, int cus) {
+  return (long)((nq + 63) / 64) * npairs <= cus || window <= (head_dim == 64 ? 256 : 128);
+}
 inline bool window_stage2_pair_rule(int nk, int npairs, int cus) { return (long)((nk + 63) / 64) * npairs <= 2l * cus; }
 
 // Paged attention: which kernel, how many tiles of rows ("slots") and how a sequence's keys are

@@ -16,10 +16,23 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdlib>
+#include <cstring>
+
 #include "fhog_grid.h"
 #include "fhog_window.h"
 
 namespace fhog {
+
+// Workgroups of 4 waves resident on the current device at once, at `waves`
+// waves per SIMD (0 if the device cannot be queried).
+inline int resident_workgroups(int waves) {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    return 0;
+  return cus * waves;
+}
 
 template <typename T> struct FwdParams {
   const T* q; const T* k; const T* v;
@@ -67,10 +80,22 @@ __device__ inline int first_contributing_query(const BwdBwdParams<T>& p, int kj,
   return causal ? kj - p.coff + (kj == 0) : 0;
 }
 
+// Whether a windowed kernel of fhog_window_few.hip takes a call: FLASH_HOG_FWD, _BWDQ, _BWD or
+// _STAGE2 = few, or window_few_rule unless the variable names another kernel.
+inline bool window_few_selected(const char* v, int rows, int npairs, int row_bytes, bool stage2 = false) {
+  if (v != nullptr && *v != 0) return std::strcmp(v, "few") == 0;
+  return window_few_rule(rows, npairs, row_bytes, stage2, resident_workgroups(1));
+}
+
 // Workgroups of a key-tiled launch with blocks of `rows` keys.
 template <int MASK, typename P> inline int key_grid(const P& p, int rows) {
   const int npairs = p.batch * p.kv_heads;
   return ((p.nk + rows - 1) / rows + (MASK == kWindow ? p.sink.blocks * p.sink.chunks : 0)) * npairs;
+}
+// p without the workgroups of the sinks' chunks, if they go apart.
+template <typename P> inline P own_launch(P p) {
+  if (p.sink.apart) p.sink.blocks = 0;
+  return p;
 }
 
 // What the launch rules look at.
@@ -129,8 +154,14 @@ hipError_t launch_bwdbwd_stage2_pair(const BwdBwdParams<T>& p, hipStream_t s);
 
 // The first backward and the double backward with a window of keys and sinks; the
 // forward is launch_fwd<T, D, kWindow>.
+// The same with one block of 32 rows a workgroup (fhog_window_few.hip; rows of 256 bytes at most);
+// only_sinks: of the key-tiled ones just the sinks' chunks.
+template <typename T, int D> constexpr bool kFewServes = D * sizeof(T) <= 256;
+template <typename T, int D> hipError_t launch_few_fwd(const FwdParams<T>& p, hipStream_t s);
+template <typename T, int D> hipError_t launch_few_dq(const BwdParams<T>& p, hipStream_t s);
+template <typename T, int D> hipError_t launch_few_dkdv(const BwdParams<T>& p, bool only_sinks, hipStream_t s);
+template <typename T, int D> hipError_t launch_few_stage2(const BwdBwdParams<T>& p, bool only_sinks, hipStream_t s);
 template <typename T, int D> hipError_t launch_window_dq(const BwdParams<T>& p, hipStream_t s);
-template <typename T, int D> hipError_t launch_window_dkdv(const BwdParams<T>& p, hipStream_t s);
 template <typename T, int D> hipError_t launch_window_stage2(const BwdBwdParams<T>& p, hipStream_t s);
 template <typename T, int D> hipError_t launch_window_bwd(const BwdParams<T>& p, hipStream_t s);
 template <typename T, int D> hipError_t launch_window_bwdbwd(const BwdBwdParams<T>& p, hipStream_t s);

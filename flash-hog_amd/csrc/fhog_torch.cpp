@@ -218,7 +218,8 @@ void require_bound(const void* fn) {
 struct Window {
   int window = 0, sinks = 0;
   at::Tensor workspace(const at::Tensor& q, const Dims& d, int causal) const {
-    const size_t size = api().window_bytes(d.B, d.Tq, d.Tk, d.Nk, d.H, causal, window, sinks);
+    const size_t size = api().window_bytes(d.B, d.Tq, d.Tk, d.N, d.Nk, d.H, dtype_code(q.scalar_type()), causal, window,
+                                           sinks);
     return size ? at::empty({(int64_t)size}, q.options().dtype(at::kByte)) : at::Tensor();
   }
 };

@@ -92,9 +92,10 @@ template <int MASK, typename P> __device__ __forceinline__ int keys_seen(const P
 // comes in parts, which go to p.sink_parts in fp32, part 0 from its own block and part
 // 1 + c from chunk c, and sink_join adds them in that order.
 struct SinkGrid {
-  int blocks;  // key blocks that hold sinks
+  int blocks;  // key blocks that hold sinks (32-key ones: enough of any kernel's)
   int chunks;  // chunks of queries
   int step;    // queries of a chunk, a multiple of 32
+  bool apart;  // whether the chunks have a launch of their own (sink_chunks)
 };
 
 // The block, (batch, head) pair and part of workgroup `extra` of those behind the ordinary ones

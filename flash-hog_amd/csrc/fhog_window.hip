@@ -27,6 +27,7 @@ sink_join_kernel(const float* parts, T* dk, T* dv, int pairs, int kv_heads, int 
   const long row = i / kCols;
   const int col = 4 * (int)(i % kCols);
   f32x4 sum = zero4();
+#pragma unroll 8
   for (int c = 0; c < count; ++c) sum += *reinterpret_cast<const f32x4*>(parts + (c * rows + row) * D + col);
   const int key = (int)(row / 2 % sinks), bh = (int)(row / 2 / sinks);
   const int b = bh / kv_heads, hk = bh % kv_heads;
@@ -45,6 +46,19 @@ hipError_t join(const P& p, T* dk, T* dv, hipStream_t stream) {
 }
 
 }  // namespace
+
+// dK and dV: FLASH_HOG_BWD = few (rows of up to 256 bytes) or pair, or the rules of fhog_grid.h.
+template <typename T, int D> hipError_t launch_window_dkdv(const BwdParams<T>& p, hipStream_t stream) {
+  if constexpr (kFewServes<T, D>) {
+    if (p.sink.apart && p.sink.chunks > 0) {
+      const hipError_t e = launch_few_dkdv<T, D>(p, true, stream);
+      if (e != hipSuccess) return e;
+    }
+    if (window_few_selected(std::getenv("FLASH_HOG_BWD"), p.nk, p.batch * p.kv_heads, D * (int)sizeof(T)))
+      return launch_few_dkdv<T, D>(own_launch(p), false, stream);
+  }
+  return launch_bwd_pair<T, D, kWindow>(own_launch(p), stream);
+}
 
 template <typename T, int D> hipError_t launch_window_bwd(const BwdParams<T>& p, hipStream_t stream) {
   hipError_t e = launch_window_dq<T, D>(p, stream);

@@ -54,7 +54,7 @@ SIGNATURES = {
     "fhog_attention_bwdbwd": (_i, [_p] * 17 + [_i] * 8 + [_f]),
     "fhog_attention_bwdbwd_stage": (_i, [_p, _i] + [_p] * 16 + [_i] * 8 + [_f]),
     "fhog_attention_bwdbwd_noalloc": (_i, [_p] * 14 + [_i] * 8 + [_f]),
-    "fhog_window_workspace_bytes": (ctypes.c_size_t, [_i] * 8),
+    "fhog_window_workspace_bytes": (ctypes.c_size_t, [_i] * 10),
     "fhog_window_attention_fwd": (_i, [_p] * 6 + [_i] * 10 + [_f]),
     "fhog_window_attention_bwd": (_i, [_p] * 12 + [_i] * 10 + [_f]),
     "fhog_window_attention_bwdbwd": (_i, [_p] * 18 + [_i] * 10 + [_f]),
@@ -234,8 +234,7 @@ def _window_args(window: int, sinks: int):
 
 def _window_workspace(q, dims, causal, window, sinks):
     """Workspace of a windowed backward (fhog_window_workspace_bytes), or None where it needs none."""
-    B, Tq, Tk, _, Nk, Hd = dims
-    size = lib().fhog_window_workspace_bytes(B, Tq, Tk, Nk, Hd, causal_code(causal), window, sinks)
+    size = lib().fhog_window_workspace_bytes(*dims, DTYPE_CODES[q.dtype], causal_code(causal), window, sinks)
     return torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
 
 

@@ -201,8 +201,8 @@ int fhog_attention_bwdbwd_noalloc(fhog_stream_t stream,
  * that is 0, as without sinks): fp32 parts of the sinks' dk and dv rows, scratch between the
  * kernels of one call. Calls that may overlap need one each.
  */
-size_t fhog_window_workspace_bytes(int batch, int n_q, int n_k, int kv_heads, int head_dim, int causal, int window,
-                                   int sinks);
+size_t fhog_window_workspace_bytes(int batch, int n_q, int n_k, int heads, int kv_heads, int head_dim, int dtype,
+                                   int causal, int window, int sinks);
 
 int fhog_window_attention_fwd(fhog_stream_t stream,
                               const void* q, const void* k, const void* v,

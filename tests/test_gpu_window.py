@@ -137,6 +137,15 @@ def test_other_scales(case, scale, cuda_device):
 @pytest.mark.parametrize("case", [c for c in CASES if c[6] != FP32 and c[5] <= 128][1::2], ids=case_id)
 def test_kernel_variants(case, variant, cuda_device, monkeypatch):
     """The kernels with one wave and with two per 32 rows, whichever the sizes would choose."""
-    for name in ("FLASH_HOG_BWD", "FLASH_HOG_BWDQ", "FLASH_HOG_STAGE2"):
+    for name in ("FLASH_HOG_FWD", "FLASH_HOG_BWD", "FLASH_HOG_BWDQ", "FLASH_HOG_STAGE2"):
         monkeypatch.setenv(name, variant)
     run_case(case, cuda_device, seed=17)
+
+
+@pytest.mark.parametrize("variant", ["few", "other"])
+@pytest.mark.parametrize("case", [c for c in CASES if c[5] * (4 if c[6] == FP32 else 2) <= 256], ids=case_id)
+def test_few_rows_kernels(case, variant, cuda_device, monkeypatch):
+    """The kernels with one 32-row block a workgroup, and the others (any other name), at every case."""
+    for name in ("FLASH_HOG_FWD", "FLASH_HOG_BWD", "FLASH_HOG_BWDQ", "FLASH_HOG_STAGE2"):
+        monkeypatch.setenv(name, variant)
+    run_case(case, cuda_device, seed=23)
