@@ -166,6 +166,18 @@ template <int SWZ = kSwzPairs> __device__ __forceinline__ int phys_chunk(int r, 
   return (c & ~7) | ((c & 7) ^ swz<SWZ>(r));
 }
 
+// Rows of 256 bytes and more start in the same bank, so that a key of eight values leaves sixteen
+// rows two to a place. kSwzWide permutes the chunks within aligned groups of sixteen: sixteen
+// successive rows have different keys (row reads), the keys of four rows differ in their upper
+// two bits and those of eight rows in their upper three (the 64 and 32 bytes of a row that the
+// transposed reads of the 32x32x16 and 16x16x32 operands take). It repeats every 16 rows, and
+// wide_key(r + 8) = wide_key(r) ^ 1.
+constexpr int kSwzWide = 2;
+__device__ __forceinline__ int wide_key(int r) { return ((r & 3) << 2) | ((r >> 1) & 2) | ((r >> 3) & 1); }
+template <> __device__ __forceinline__ int phys_chunk<kSwzWide>(int r, int c) {
+  return (c & ~15) | ((c & 15) ^ wide_key(r));
+}
+
 template <typename T, int D> struct SwzTile {
   static constexpr int kRows = 32;
   static constexpr int kRowBytes = D * (int)sizeof(T);
@@ -438,6 +450,34 @@ template <typename T, int D> struct PointerFrags {
     return (const T*)((const lds_cchar*)(uintptr_t)stage + off);
   }
 };
+// SwzFrags for 2-byte tiles swizzled by kSwzWide. The key is an exclusive or with the chunk, so
+// that one offset a lane serves all columns of 256 bytes: a step's columns are flipped into it.
+// stage + off has to be a multiple of 256, which every ring stage and tile offset here is.
+template <typename T, int D> struct WideFrags {
+  static_assert(sizeof(T) == 2 && D >= 128, "256-byte rows or wider");
+  uint32_t row, tr;
+  __device__ __forceinline__ void init(int lane) {
+    const int n = lane & 31, g = lane >> 5;
+    row = 2u * (uint32_t)(n * D + 8 * (g ^ wide_key(n)));
+    const int i = lane & 15, r = 4 * g + (i >> 2);
+    tr = 2u * (uint32_t)(r * D + 8 * ((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ wide_key(r)) + 4 * (i & 1));
+  }
+  __device__ __forceinline__ V8<T> rowf(uint32_t stage, int off, int ks) const {
+    const uint32_t a = (stage + row) ^ (uint32_t)(32 * (ks & 7));
+    const lds_cchar* p = reinterpret_cast<const lds_cchar*>((uintptr_t)a) + off + 256 * (ks >> 3);
+    return *reinterpret_cast<const __attribute__((address_space(3))) V8<T>*>(p);
+  }
+  __device__ __forceinline__ V8<T> trf(uint32_t stage, int off, int dt, int s) const {
+    const uint32_t a0 = (stage + tr) ^ (uint32_t)(64 * (dt & 3));
+    const int o = off + 256 * (dt >> 2) + s * 32 * D;
+    const lds_cchar* a = reinterpret_cast<const lds_cchar*>((uintptr_t)a0) + o;
+    const lds_cchar* b = reinterpret_cast<const lds_cchar*>((uintptr_t)(a0 ^ 16u)) + o + 16 * D;  // 8 rows on
+    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(a));
+    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(b));
+    return __builtin_shufflevector(__builtin_bit_cast(V4<T>, x), __builtin_bit_cast(V4<T>, y), 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
 // The operands of the kernels with one wave per 32 queries.
 template <typename T, int D, int COLS = 64>
 using WaveFrags = std::conditional_t<sizeof(T) == 4 && D == 64, PointerFrags<T, D>, SwzFrags<T, D, COLS>>;
@@ -522,6 +562,29 @@ template <typename T, int D> struct SwzFrags16 {
   }
 };
 
+// SwzFrags16 for tiles swizzled by kSwzWide (WideFrags).
+template <typename T, int D> struct WideFrags16 {
+  static_assert(sizeof(T) == 2 && D >= 128, "256-byte rows or wider");
+  uint32_t row, tr;
+  __device__ __forceinline__ void init(int lane) {
+    const int n = lane & 15, g = lane >> 4;
+    row = 2u * (uint32_t)(n * D + 8 * (g ^ wide_key(n)));
+    const int r = 4 * g + (n >> 2);
+    tr = 2u * (uint32_t)(r * D + 8 * (((n & 3) >> 1) ^ wide_key(r)) + 4 * (n & 1));
+  }
+  __device__ __forceinline__ V8<T> rowf(uint32_t stage, int off, int kb, int ks) const {
+    const uint32_t a = (stage + row) ^ (uint32_t)(64 * (ks & 3));
+    const lds_cchar* p = reinterpret_cast<const lds_cchar*>((uintptr_t)a) + off + 256 * (ks >> 2) + kb * 16 * D * 2;
+    return *reinterpret_cast<const __attribute__((address_space(3))) V8<T>*>(p);
+  }
+  __device__ __forceinline__ V8<T> trf(uint32_t stage, int off, int db) const {
+    const uint32_t a0 = (stage + tr) ^ (uint32_t)(32 * (db & 7));
+    const lds_cchar* a = reinterpret_cast<const lds_cchar*>((uintptr_t)a0) + off + 256 * (db >> 3);
+    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(a));
+    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(a + 16 * D * 2));
+    return __builtin_shufflevector(__builtin_bit_cast(V4<T>, x), __builtin_bit_cast(V4<T>, y), 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
 
 // Grid order of the sequence-tiled kernels. A workgroup takes one (batch,
 // head) pair and one block along the sequence, its `rank` (for causal grids

@@ -128,7 +128,7 @@ paged_token_kernel(PagedParams<T, C> p) {
   // (215 us against 221).
   typedef KeyPieces<T, C, D> Keys;
   constexpr bool kDirect = Keys::kQuantised;
-  typedef PageTile<T, C, D, 64, kSwzRows, kDirect ? 1 : 2> Tile;
+  typedef PageTile<T, C, D, 64, D == 64 ? kSwzRows : kSwzWide, kDirect ? 1 : 2> Tile;
   constexpr int kWaveLds = (kDirect ? 1 : 2) * Tile::kTileBytes;
   __shared__ __attribute__((aligned(1024))) char s_kv[kWaves * kWaveLds];
   __shared__ float s_ml[kWaves][ROWS][2];
@@ -159,7 +159,7 @@ paged_token_kernel(PagedParams<T, C> p) {
   }
   const float c2 = fabsf(p.scale) * kLog2e;
 
-  SwzFrags16<T, D> fr;
+  std::conditional_t<D == 64, SwzFrags16<T, D>, WideFrags16<T, D>> fr;
   fr.init(lane);
   const uint32_t lds = lds_base_u32(s_kv) + wave * kWaveLds;
   float m = -1e30f, lpart = 0.f;
@@ -301,7 +301,7 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 64 || RW == 4 ? 3 : 2)))
 paged_chunk_kernel(PagedParams<T, C> p) {
   constexpr int ROWS = 32 * RW, KW = 4 / RW;
   constexpr int KS = D / 16, DT = D / 32;
-  typedef PageTile<T, C, D, 64 * RW, kSwzPairs> Tile;
+  typedef PageTile<T, C, D, 64 * RW, D == 64 ? kSwzPairs : kSwzWide> Tile;
   constexpr int kStage = 2 * Tile::kTileBytes;
   __shared__ __attribute__((aligned(1024))) char s_kv[KW * 2 * kStage];
   __shared__ float s_ml[KW][ROWS][2];
@@ -311,7 +311,8 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   const int rw = wave % RW, kw = wave / RW;
   const int thread = threadIdx.x % (64 * RW);  // of its group
   const int n = lane & 31, g = lane >> 5;
-  const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads, split = blockIdx.y;
+  // (backwards: a sequence's last rows, which see most, first)
+  const int hk = blockIdx.x % p.at.kv_heads, slot = p.slots - 1 - (int)blockIdx.x / p.at.kv_heads, split = blockIdx.y;
   clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 256);
   const RowTile rt = RowTile::template at<ROWS>(p, slot);
   if (rt.rows <= 0) return;
@@ -338,7 +339,7 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   }
   const float c2 = fabsf(p.scale) * kLog2e;
 
-  SwzFrags<T, D> fr;
+  std::conditional_t<D == 64, SwzFrags<T, D>, WideFrags<T, D>> fr;
   fr.init(lane);
   const uint32_t lds = lds_base_u32(s_kv) + kw * 2 * kStage;
   float m = -1e30f, lpart = 0.f;
