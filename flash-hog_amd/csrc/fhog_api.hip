@@ -135,7 +135,7 @@ int check_window(const Shape& s, int window, int sinks, Window* w, const char* w
   const fhog::SinkChunks c = fhog::sink_chunks(m, w->window, w->sinks, row_bytes, (long)s.batch * s.heads,
                                                (long)s.batch * s.kv_heads);
   w->sink = fhog::SinkGrid{(w->sinks + 31) / 32, c.count, c.step, c.apart};
-  const long long groups = ((s.n_k + 63) / 64 + (long long)w->sink.blocks * w->sink.chunks) * s.batch * s.kv_heads;
+  const long long groups = ((s.n_k + 31) / 32 + (long long)w->sink.blocks * w->sink.chunks) * s.batch * s.kv_heads;
   if (groups >= (1ll << 31)) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
   return FHOG_OK;
 }
@@ -161,6 +161,8 @@ struct Paged {
   int batch, rows, heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype;
 };
 
+constexpr double kMostElements = 32.0 * (1ll << 30);  // of a packed tensor; eight a thread
+
 int check_paged(const Paged& s, const char* who) {
   if (s.batch < 0 || s.rows < 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sizes must not be negative", who);
   if (s.heads < 1 || s.kv_heads < 1 || s.num_pages < 1 || s.pages_per_seq < 1)
@@ -178,7 +180,8 @@ int check_paged(const Paged& s, const char* who) {
   if (s.head_dim != 64 && s.head_dim != 128 && s.head_dim != 256)
     return fail(FHOG_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256, got %d", who, s.head_dim);
   // packed (token, head) rows and positions are ints, a launch's threads 32 bits
-  if ((long long)s.rows * s.heads >= (1ll << 30) || s.batch >= (1 << 24) ||
+  if ((long long)s.rows * s.heads >= (1ll << 30) || (double)s.rows * s.heads * s.head_dim >= kMostElements ||
+      s.batch >= (1 << 24) ||
       (long long)s.pages_per_seq * s.page_size > (1ll << 30))
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
   return FHOG_OK;
@@ -501,7 +504,7 @@ int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cach
                          const void* k_scale, const void* v_scale, const int* page_table, const int* lengths,
                          const int* query_offsets, void* out, void* workspace, size_t workspace_bytes, int batch,
                          int total, int heads, int kv_heads, int head_dim, int num_pages, int page_size,
-                         int pages_per_seq, int dtype, int cache_dtype, int window, int sinks, int clear_tail,
+                         int pages_per_seq, int dtype, int cache_dtype, int window, int sinks, int clear_rest,
                          float scale) {
   static const char* who = "fhog_paged_attention";
   const Paged s{batch, total, heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype};
@@ -525,7 +528,7 @@ int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cach
   if (sinks > most) sinks = most;
   const fhog::PagedPlan plan = fhog::paged_plan(batch, total, query_offsets == nullptr, heads, kv_heads,
                                                 head_dim, (long)page_size * pages_per_seq, window, sinks, compute_units());
-  if ((long long)plan.slots * kv_heads >= (1ll << 31) || plan.splits > 65535)
+  if ((long long)plan.slots * kv_heads >= (1ll << 23) || plan.splits > 65535)
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
   const size_t need = (size_t)plan.parts * (head_dim + 2) * sizeof(float);
   if (need > 0 && (!aligned(workspace, 16) || workspace_bytes < need))
@@ -534,7 +537,7 @@ int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cach
     fhog::PagedParams<T, C> p{(const T*)q, (T*)out,
                               {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
                               cache_shape(s, page_table, lengths, query_offsets), (float*)workspace, heads, window,
-                              sinks, plan.slots, plan.splits, plan.split_tiles, clear_tail, scale};
+                              sinks, plan.slots, plan.splits, plan.split_tiles, clear_rest, scale};
     return fhog::launch_paged_attention<T, C, D>(p, plan.rows, (hipStream_t)stream);
   };
   return launch_status(dispatch_paged(s, run), who);
@@ -571,7 +574,7 @@ int fhog_paged_cache_read(fhog_stream_t stream, const void* k_cache, const void*
   const Paged s{batch, 0, kv_heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype};
   if (int st = check_paged(s, who)) return st;
   if (max_length < 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sizes must not be negative", who);
-  if ((double)batch * max_length * kv_heads * head_dim >= 2048.0 * (1ll << 31))
+  if ((double)batch * max_length * kv_heads * head_dim >= kMostElements)
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
   if (batch == 0 || max_length == 0) return ok();
   if (int st = check_ptrs(who, {{"k", k}, {"v", v}}, {})) return st;

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(CacheWriteParams<
   const int b = c.offsets ? last_at_or_before(c.batch, t, [&](int s) { return packed_begin(c, s); }) : t;
   const int begin = packed_begin(c, b), end = c.offsets ? packed_begin(c, b + 1) : b + 1;
   if (t < begin || t >= end) return;  // behind the last sequence
-  const int pos = c.lengths[b] - (end - t);
+  const int pos = max(c.lengths[b], 0) - (end - t);
   if (pos < 0 || (pos >> c.page_shift) >= c.pages_per_seq) return;
   const int page = c.table[(long)b * c.pages_per_seq + (pos >> c.page_shift)];
   if ((unsigned)page >= (unsigned)c.pages) return;

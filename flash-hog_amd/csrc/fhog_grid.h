@@ -419,6 +419,7 @@ inline SinkChunks sink_chunks(Mask m, int window, int sinks, int row_bytes, long
   long step = apart ? 128 : share > 512 ? share : 512;
   if (apart && step * 256 < queries * npairs) step = (queries * npairs + 255) / 256;
   if (step < 2l * sinks) step = 2l * sinks;
+  if (step > queries) step = queries;
   step = (step + 31) / 32 * 32;
   return SinkChunks{apart, (int)step, sinks > 0 && first < m.nq ? (int)((queries + step - 1) / step) : 0};
 }
@@ -457,15 +458,15 @@ struct PagedPlan {
   long parts;       // fp32 rows of head_dim + 2 in the workspace
 };
 constexpr int kJoinWeights = 2048;  // the most rows of a tile times splits
-#ifndef FHOG_TT
-#define FHOG_TT 8l
-#endif
-#ifndef FHOG_CR
-#define FHOG_CR 2l
-#endif
-#ifndef FHOG_CT
-#define FHOG_CT 2l
-#endif
+// us, H32/8 D128, with the chosen number and those on both sides of it:
+//  - wide tiles of 128 rows from two a CU on, of 64 below (64 everywhere / two): B8 x 512 tokens
+//    window 2048 159.7 / 136.8, N8192 e4m3 780 / 620; (one / two) B32 x 64 tokens of H16/4 D64 103 / 68;
+//  - their splits fill the CUs with as many workgroups as live there together, two, at D = 256 one
+//    (1 / 2 / 4 a CU): 512 tokens after 7680 152 / 127 / 130, 64 after 32704 e4m3 143 / 97 / 112, D256
+//    B2 x 1024 after 7168 H8 348 / 386 / 411;
+//  - splits of single tokens fill them with eight (4 / 8 / 16): B16 over 32768 keys e4m3 136 / 126 / 143,
+//    bf16 229 / 215 / 221, B64 over 4096 e4m3 67.4 / 67.6 / 67.4.
+constexpr long kWideTiles = 2, kTokenWorkgroups = 8;
 inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv_heads, int head_dim, long capacity,
                             int window, int sinks, int cus) {
   if (cus <= 0) cus = 256;
@@ -475,7 +476,7 @@ inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv
     return single ? (long)batch * ((group + rows - 1) / rows) : (long)total * group / rows + batch;
   };
   // More than 16 rows a sequence on average (tokens times heads of a group): the wide tiles.
-  p.rows = (long)total * group <= 16l * batch ? 16 : slots(128) * kv_heads >= FHOG_CR * cus ? 128 : 64;
+  p.rows = (long)total * group <= 16l * batch ? 16 : slots(128) * kv_heads >= kWideTiles * cus ? 128 : 64;
   p.slots = (int)slots(p.rows);
   // The most tiles that a tile of rows reads: with a window its keys, those between the tile's
   // first and last position and the sinks.
@@ -489,10 +490,10 @@ inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv
   p.waves = head_dim == 64 ? 8 : head_dim == 128 ? 4 : 2;
   long target, least;
   if (p.rows > 16) {
-    target = FHOG_CT * cus;
+    target = (head_dim == 256 ? 1l : 2l) * cus;
     least = 8;
   } else {
-    target = FHOG_TT * cus;
+    target = kTokenWorkgroups * cus;
     least = 2 * blocks < cus ? (head_dim == 64 ? 32 : 8) : (blocks < 2l * cus ? 8l : 32l) * p.waves;
   }
   long splits = blocks >= target ? 1 : (target + blocks - 1) / blocks;

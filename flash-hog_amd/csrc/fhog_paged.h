@@ -11,7 +11,7 @@
 // of its n new ones is at position lengths[b] - n + i.
 //
 // Nothing on the device is trusted: a table entry outside [0, pages) or a length beyond the
-// table's capacity makes the output rows that depend on it NaN (attention, reading) or is
+// table's capacity gives NaN in rows of its sequence (attention, reading) or is
 // skipped (writing); offsets are cut to [0, total]. No access leaves its tensor.
 //
 // An e4m3 cache has an e8m0 scale for each key and value row, (pages, kv_heads, page_size):
@@ -49,7 +49,7 @@ template <typename T, typename C> struct PagedParams {
   float* parts;  // fp32 outputs of the splits, (slot, kv_head, split, row of the tile, head_dim), and their m, l
   int heads, window, sinks;  // window 0: none
   int slots, splits, split_tiles;
-  int clear_tail;  // whether rows behind the last sequence are zeroed
+  int clear_rest;  // whether rows of no sequence are zeroed
   float scale;
 };
 

@@ -66,13 +66,16 @@ struct RowTile {
   }
 };
 
-// Zeroes the packed rows behind the last sequence.
-template <int D, typename P> __device__ __forceinline__ void clear_tail(const P& p, int worker, int workers, int threads) {
-  if (!p.clear_tail || !p.at.offsets) return;
+// Zeroes the packed rows behind the last sequence, and those before the first.
+template <int D, typename P> __device__ __forceinline__ void clear_rest(const P& p, int worker, int workers, int threads) {
+  if (!p.clear_rest || !p.at.offsets) return;
   const long per_row = (long)p.heads * D / 8;
-  const long begin = (long)packed_begin(p.at, p.at.batch) * per_row, end = (long)p.at.total * per_row;
+  const long first = (long)packed_begin(p.at, 0) * per_row;
+  const long last = (long)packed_begin(p.at, p.at.batch) * per_row, end = (long)p.at.total * per_row;
+  const long i0 = (long)worker * threads + threadIdx.x, step = (long)workers * threads;
   u32x4* out = reinterpret_cast<u32x4*>(p.out);
-  for (long i = begin + (long)worker * threads + threadIdx.x; i < end; i += (long)workers * threads) out[i] = u32x4{0, 0, 0, 0};
+  for (long i = i0; i < first; i += step) out[i] = u32x4{0, 0, 0, 0};
+  for (long i = last + i0; i < end; i += step) out[i] = u32x4{0, 0, 0, 0};
 }
 
 // The pages of a tile's two halves, loaded a step before the tile's rows are.
@@ -137,7 +140,7 @@ paged_token_kernel(PagedParams<T, C> p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % p.at.kv_heads, slot = blockIdx.x / p.at.kv_heads, split = blockIdx.y;
-  clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 64 * kWaves);
+  clear_rest<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 64 * kWaves);
   const RowTile rt = RowTile::template at<ROWS>(p, slot);
   if (rt.rows <= 0) return;
   const int first_pos = __builtin_amdgcn_readfirstlane(rt.position(0));
@@ -313,7 +316,7 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   const int n = lane & 31, g = lane >> 5;
   // (backwards: a sequence's last rows, which see most, first)
   const int hk = blockIdx.x % p.at.kv_heads, slot = p.slots - 1 - (int)blockIdx.x / p.at.kv_heads, split = blockIdx.y;
-  clear_tail<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 256);
+  clear_rest<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 256);
   const RowTile rt = RowTile::template at<ROWS>(p, slot);
   if (rt.rows <= 0) return;
   const int first_pos = __builtin_amdgcn_readfirstlane(rt.position(0));

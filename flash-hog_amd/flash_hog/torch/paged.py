@@ -24,8 +24,9 @@ sequence b's are rows query_offsets[b] to query_offsets[b + 1] and take its last
 order; None: each sequence has one.
 
 The index tensors are read on the device only, so mistakes in them cannot raise: an attended
-page outside the cache, or a length beyond its table, makes the rows that depend on it NaN
-(paged_cache_write leaves such a token out), and no access leaves its tensor. Entries and cache
+page outside the cache, or a length beyond its table, gives NaN in rows of its sequence, those
+that depend on it at least (paged_cache_write leaves such a token out), and no access leaves its
+tensor. Entries and cache
 slots that no visible token needs may hold anything, NaN included. Among the keys of one 32-key
 tile, though, a NaN or infinity in a value that one token sees also reaches the rows beside it.
 """
@@ -92,8 +93,8 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_of
     zero) gives zeros. Query heads share key/value heads as in dot_product_attention; scale
     defaults to H ** -0.5.
 
-    out: a contiguous tensor for the result; its rows behind the last sequence
-    (query_offsets[batch] and on, a padded batch) are left as they were. Without it they are zero.
+    out: a contiguous tensor for the result; its rows of no sequence (from query_offsets[batch]
+    on, a padded batch) are left as they were. Without it they are zero.
     """
     _refuse_gradients("paged_attention", query, key_cache, value_cache)
     if window is None:
@@ -117,7 +118,7 @@ def paged_cache_write(key, value, key_cache, value_cache, page_table, lengths, q
     """Writes key and value (T, N_kv, H) of the packed new tokens to their places in the cache, in
     place. An e4m3 cache gets each row quantised: its scale is the smallest power of two (at least
     2 ** -126) with which the row's largest finite magnitude stays within 448, its values round
-    to nearest even, and infinities become NaN. Rows behind the last sequence and tokens at
+    to nearest even, and infinities become NaN. Rows of no sequence and tokens at
     positions below zero (a sequence of length zero) are not written. No two tokens may name the
     same place: pages that sequences share are read-only."""
     _refuse_gradients("paged_cache_write", key, value, key_cache, value_cache)

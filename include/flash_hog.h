@@ -256,14 +256,14 @@ size_t fhog_paged_workspace_bytes(int batch, int total, int single, int heads, i
  * out (total, heads, head_dim): attention of the new tokens q (same shape) over the cached
  * keys of their sequences, their own among them (written before). Token i of n new ones is at
  * position p = length - n + i and sees the keys j <= p, with window > 0 those with j > p - window
- * or j < sinks only. A token that sees no key gets 0. Rows behind the last sequence
- * (query_offsets[batch] to total) are zeroed if clear_tail, else left as they were.
+ * or j < sinks only. A token that sees no key gets 0. Rows of no sequence (before
+ * query_offsets[0], from query_offsets[batch] on) are zeroed if clear_rest, else left as they were.
  */
 int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cache, const void* v_cache,
                          const void* k_scale, const void* v_scale, const int* page_table, const int* lengths,
                          const int* query_offsets, void* out, void* workspace, size_t workspace_bytes, int batch,
                          int total, int heads, int kv_heads, int head_dim, int num_pages, int page_size,
-                         int pages_per_seq, int dtype, int cache_dtype, int window, int sinks, int clear_tail,
+                         int pages_per_seq, int dtype, int cache_dtype, int window, int sinks, int clear_rest,
                          float scale);
 
 /*
