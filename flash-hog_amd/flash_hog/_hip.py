@@ -362,7 +362,7 @@ def attention_bwdbwd_noalloc(q, k, v, o, dout, ddq, ddk, ddv, lse, causal, scale
 
 # ------------------------------------------------------------- paged cache
 
-CACHE_DTYPE_CODES = {torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3}
+CACHE_DTYPE_CODES = {**DTYPE_CODES, torch.float8_e4m3fn: 3}  # (the library refuses an fp32 one)
 _SCALE_DTYPES = (torch.float8_e8m0fnu, torch.uint8)
 
 

@@ -51,8 +51,8 @@ def test_every_value_is_quantised(dtype, cuda_device):
 
 @pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
 def test_every_scale_is_read(dtype, cuda_device):
-    """All e8m0 scales that stand for a normal number (1 to 254) with all 256 codes, to the
-    nearest value of dtype; products beyond its normal range are as close as its smallest one."""
+    """All 256 e8m0 scales (255: NaN) with all 256 codes, to the nearest value of dtype; products
+    below its normal range are as close as its smallest normal number."""
     import flash_hog
 
     print("[case] every scale", dtype, flush=True)
@@ -64,8 +64,9 @@ def test_every_scale_is_read(dtype, cuda_device):
         pages, pages, torch.arange(64, dtype=torch.int32, device=cuda_device)[None],
         torch.tensor([1024], dtype=torch.int32, device=cuda_device), dtype=dtype, key_scale=scale, value_scale=scale)
     assert same(k, v)
-    got = k.view(256, 4, 64)[1:255].cpu()
-    exact = codes[1:255].view(E4M3).double() * ref.powers(scales[1:255])[..., None]
+    assert torch.isnan(k.view(256, 4, 64)[255]).all()
+    got = k.view(256, 4, 64)[:255].cpu()
+    exact = codes[:255].view(E4M3).double() * ref.powers(scales[:255])[..., None]
     want = exact.to(dtype)  # (double to fp16 and bf16 rounds once)
     info = torch.finfo(dtype)
     normal = ~(exact.abs() < info.tiny) & ~torch.isnan(exact)
