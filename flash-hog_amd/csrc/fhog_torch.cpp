@@ -485,35 +485,44 @@ struct NoThirdOrder : public torch::autograd::Function<NoThirdOrder> {
   }
 };
 
-void save_mask(AutogradContext* ctx, int64_t causal, double scale, Window w) {
-  ctx->saved_data["causal"] = causal;
-  ctx->saved_data["scale"] = scale;
-  ctx->saved_data["window"] = (int64_t)w.window;
-  ctx->saved_data["sinks"] = (int64_t)w.sinks;
-}
-Window saved_window(AutogradContext* ctx) {
-  return {(int)ctx->saved_data["window"].toInt(), (int)ctx->saved_data["sinks"].toInt()};
-}
+// A call's mask and scale, as one argument of the Functions.
+struct Mask {
+  int causal;
+  double scale;
+  Window w;
+  void save(AutogradContext* ctx) const {
+    ctx->saved_data["causal"] = (int64_t)causal;
+    ctx->saved_data["scale"] = scale;
+    if (w.window == 0) return;  // (an entry costs every call)
+    ctx->saved_data["window"] = (int64_t)w.window;
+    ctx->saved_data["sinks"] = (int64_t)w.sinks;
+  }
+  static Mask saved(AutogradContext* ctx) {
+    Mask m{(int)ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble(), {}};
+    const auto window = ctx->saved_data.find("window");
+    if (window != ctx->saved_data.end())
+      m.w = {(int)window->second.toInt(), (int)ctx->saved_data["sinks"].toInt()};
+    return m;
+  }
+};
 
 // Primal (q, k, v, O, L, dO) -> (dQ, dK, dV), differentiable once in q, k, v
 // and dO: _DotProductAttentionBwd (the rule
 // dot_product_attention_bwd_rule_fwd_rule and its rule
 // dot_product_attention_bwd_rule_bwd_rule).
 struct AttentionBwdFn : public torch::autograd::Function<AttentionBwdFn> {
-  static variable_list forward(AutogradContext* ctx, int64_t causal, double scale, int64_t window, int64_t sinks,
-                               const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& lse,
-                               const at::Tensor& o, const at::Tensor& g) {
-    const Window w{(int)window, (int)sinks};
-    auto [dq, dk, dv, delta] = bwd_core(q, k, v, o, g, lse, (int)causal, scale, w);
+  static variable_list forward(AutogradContext* ctx, const Mask& mask, const at::Tensor& q, const at::Tensor& k,
+                               const at::Tensor& v, const at::Tensor& lse, const at::Tensor& o, const at::Tensor& g) {
+    auto [dq, dk, dv, delta] = bwd_core(q, k, v, o, g, lse, mask.causal, mask.scale, mask.w);
     ctx->save_for_backward({q, k, v, o, lse, g});
-    save_mask(ctx, causal, scale, w);
+    mask.save(ctx);
     return {dq, dk, dv};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list r = ctx->get_saved_variables();  // q, k, v, O, L, dO
-    auto [dq2, dk2, dv2, ddo, stats] =
-        bwdbwd_core(r[0], r[1], r[2], r[3], r[5], grads[0], grads[1], grads[2], r[4],
-                    (int)ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble(), saved_window(ctx));
+    const Mask mask = Mask::saved(ctx);
+    auto [dq2, dk2, dv2, ddo, stats] = bwdbwd_core(r[0], r[1], r[2], r[3], r[5], grads[0], grads[1], grads[2], r[4],
+                                                   mask.causal, mask.scale, mask.w);
     if (c10::GradMode::is_enabled() &&
         (grads[0].requires_grad() || grads[1].requires_grad() || grads[2].requires_grad())) {
       auto mark = [](const at::Tensor& t) { return t.detach().requires_grad_(true); };
@@ -521,7 +530,7 @@ struct AttentionBwdFn : public torch::autograd::Function<AttentionBwdFn> {
       dq2 = w[0], dk2 = w[1], dv2 = w[2], ddo = w[3];
     }
     // no cotangent for L and O (flash_hog/jax/_attention_impl.py:278-303)
-    return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), dq2, dk2, dv2, at::Tensor(), at::Tensor(), ddo};
+    return {at::Tensor(), dq2, dk2, dv2, at::Tensor(), at::Tensor(), ddo};
   }
 };
 
@@ -530,11 +539,10 @@ struct AttentionBwdFn : public torch::autograd::Function<AttentionBwdFn> {
 // dot_product_attention_bwd_rule, through AttentionBwdFn).
 struct AttentionFn : public torch::autograd::Function<AttentionFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                               int64_t causal, double scale, int64_t window, int64_t sinks) {
-    const Window w{(int)window, (int)sinks};
-    auto [o, lse] = fwd_core(q, k, v, (int)causal, scale, w);
+                               const Mask& mask) {
+    auto [o, lse] = fwd_core(q, k, v, mask.causal, mask.scale, mask.w);
     ctx->save_for_backward({q, k, v, lse, o});
-    save_mask(ctx, causal, scale, w);
+    mask.save(ctx);
     ctx->mark_non_differentiable({lse});
     return {o, lse};
   }
@@ -543,10 +551,8 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
     // O enters the first backward as a constant: the double backward returns
     // no cotangent for it, and detaching it keeps this node out of a second
     // derivative's graph.
-    const variable_list d = AttentionBwdFn::apply(
-        ctx->saved_data["causal"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["window"].toInt(),
-        ctx->saved_data["sinks"].toInt(), r[0], r[1], r[2], r[3], r[4].detach(), grads[0]);
-    return {d[0], d[1], d[2], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const variable_list d = AttentionBwdFn::apply(Mask::saved(ctx), r[0], r[1], r[2], r[3], r[4].detach(), grads[0]);
+    return {d[0], d[1], d[2], at::Tensor()};
   }
 };
 
@@ -618,7 +624,7 @@ std::tuple<at::Tensor, at::Tensor> paged_cache_read(const at::Tensor& k_cache, c
 at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t causal, double scale,
                      int64_t window, int64_t sinks) {
   require_bound((const void*)api().bwdbwd);
-  return py_call([&] { return AttentionFn::apply(q, k, v, causal, scale, window, sinks)[0]; });
+  return py_call([&] { return AttentionFn::apply(q, k, v, Mask{(int)causal, scale, {(int)window, (int)sinks}})[0]; });
 }
 
 }  // namespace

@@ -142,8 +142,8 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
         query, key, value = query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0)
     native = _native_path(query, key, value)
     if native is not None:
-        result = native.attention(query, key, value, causal_code(mask_type), float(scale),
-                                  *_hip._window_args(window, sinks))
+        narrowed = _hip._window_args(window, sinks) if window else ()
+        result = native.attention(query, key, value, causal_code(mask_type), float(scale), *narrowed)
     else:
         fn = _DotProductAttention if torch._C._are_functorch_transforms_active() else _DotProductAttentionEager
         result, _ = fn.apply(query, key, value, mask_type, float(scale), window, sinks)
