@@ -478,7 +478,8 @@ template <typename T, int D> hipError_t launch_window_dq(const BwdParams<T>& p, 
   const char* v = std::getenv("FLASH_HOG_BWDQ");
   const int npairs = p.batch * p.heads;
   if constexpr (kFewServes<T, D>) {
-    if (window_few_selected(v, p.nq, npairs, D * (int)sizeof(T))) return launch_few_dq<T, D>(p, stream);
+    if (window_few_selected(v, FewKernel::kDq, (p.nq + 31l) / 32 * npairs, D, (int)sizeof(T)))
+      return launch_few_dq<T, D>(p, stream);
   }
   if constexpr (sizeof(T) == 2 && D <= 128) {
     const bool pair = v != nullptr && std::strcmp(v, "pair") == 0;

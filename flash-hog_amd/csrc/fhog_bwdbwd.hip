@@ -702,7 +702,8 @@ template <typename T, int D> hipError_t launch_window_stage2(const BwdBwdParams<
       if (e != hipSuccess) return e;
     }
     p = own_launch(p);
-    if (window_few_selected(std::getenv("FLASH_HOG_STAGE2"), p.nk, p.batch * p.kv_heads, D * (int)sizeof(T), true))
+    if (window_few_selected(std::getenv("FLASH_HOG_STAGE2"), FewKernel::kStage2, key_grid<kWindow>(p, 32), D,
+                            (int)sizeof(T)))
       return launch_few_stage2<T, D>(p, false, stream);
   }
   if constexpr (sizeof(T) == 2 && D == 64) {

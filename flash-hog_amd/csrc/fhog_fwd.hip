@@ -240,7 +240,8 @@ inline bool fwd_pair_selected(Mask m, int npairs, int head_dim) {
 template <typename T, int D, int MASK>
 hipError_t launch_fwd(const FwdParams<T>& p, hipStream_t stream) {
   if constexpr (MASK == kWindow && kFewServes<T, D>) {
-    if (window_few_selected(std::getenv("FLASH_HOG_FWD"), p.nq, p.batch * p.heads, D * (int)sizeof(T)))
+    if (window_few_selected(std::getenv("FLASH_HOG_FWD"), FewKernel::kForward,
+                            (p.nq + 31l) / 32 * p.batch * p.heads, D, (int)sizeof(T)))
       return launch_few_fwd<T, D>(p, stream);
   }
   if constexpr (sizeof(T) == 2 && D == 256) {

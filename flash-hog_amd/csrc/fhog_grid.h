@@ -425,15 +425,23 @@ inline SinkChunks sink_chunks(Mask m, int window, int sinks, int row_bytes, long
 }
 
 // The kernels of fhog_window_few.hip (one 32-row block a workgroup, its window's tiles dealt to
-// four waves) take a call of at most as many blocks as are resident at once: two a CU where
-// rows have 128 bytes, one where they have 256 and in stage 2. us, few / others, causal H12
-// D64 bf16 window 128 to 512 unless named; forward: B1 N300 (120 blocks) 9.4 / 12.6, N1000 (384)
-// 13.2 / 16.0, N2048 (768) 25.5 / 21.3, N1000 H16 D128 (512) 22.3 / 19.6, N1000 H8 fp32 (256) 17.9 /
-// 23.4; dQ: 7.4 / 11.3, 11.2 / 15.0, 23.5 / 22.7, 21.7 / 19.2, 18.5 / 29.3; dK/dV: 6.5 / 8.1, 10.6 /
-// 11.8, 24.6 / 21.4, over 4 key heads at D128 (128) 20.8 / 43.4, 21.6 / 28.7; stage 2: 9.1 / 11.3,
-// 21.8 / 16.0, 45.9 / 32.6, 39.9 / 65.8, 38.1 / 60.6.
-inline bool window_few_rule(int rows, int npairs, int row_bytes, bool stage2, int cus) {
-  return (long)((rows + 31) / 32) * npairs <= (row_bytes <= 128 && !stage2 ? 2l : 1l) * cus;
+// four waves) take a call of at most two blocks a CU, those of the sinks' chunks among them, where
+// two workgroups live on one; of one block where one does: dK/dV of 256-byte rows in 2-byte types,
+// and stage 2. dQ of such rows keeps to one as well, fp32 dK/dV, whose other kernel is the
+// slowest, goes to three. us, few / others, causal H12 D64 bf16 window 128 to 512 unless named;
+// forward: B1 N300 (120 blocks) 9.4 / 12.6, N1000 (384) 13.2 / 16.0, N2048 (768) 25.5 / 21.3, N1000 H16
+// D128 (512) 14.8 / 20.5, N2000 (1008) 35.6 / 27.1, N1000 H8 fp32 (256) 15.0 / 24.2, N2048 (512) 31.0 /
+// 37.8; dQ: 7.4 / 11.3, 11.2 / 15.0, 23.5 / 22.7, 19.8 / 18.8, 42.6 / 34.2, 18.6 / 30.4, 43.4 / 48.1;
+// dK/dV: 6.5 / 8.1, 10.6 / 11.8, 24.6 / 21.4, D128 H16 over 4 key heads (128) 20.8 / 43.4, H8 (272) 24.4 /
+// 20.7, fp32 36.9 / 43.7, N2048 (536) 74.6 / 83.4, N4096 (1080) 117.7 / 118.1; stage 2: 9.1 / 11.3,
+// 21.8 / 16.0, 45.9 / 32.6, D128 over 4 39.9 / 65.8, N1000 H8 fp32 38.1 / 60.6.
+enum class FewKernel { kForward, kDq, kDkdv, kStage2 };
+inline bool window_few_rule(FewKernel kernel, long blocks, int head_dim, int bytes, int cus) {
+  const bool wide = bytes == 2 && head_dim > 64;
+  long per_cu = 2;
+  if (kernel == FewKernel::kStage2 || (wide && kernel != FewKernel::kForward)) per_cu = 1;
+  if (kernel == FewKernel::kDkdv && bytes == 4) per_cu = 3;
+  return blocks <= per_cu * cus;
 }
 // Beyond, for 2-byte types: dQ at D = 64 and 128 in bwd_q_kernel (128-query blocks) or, on grids of
 // at most one workgroup per CU or where those cover so much more than 64-query ones, in

@@ -82,9 +82,9 @@ __device__ inline int first_contributing_query(const BwdBwdParams<T>& p, int kj,
 
 // Whether a windowed kernel of fhog_window_few.hip takes a call: FLASH_HOG_FWD, _BWDQ, _BWD or
 // _STAGE2 = few, or window_few_rule unless the variable names another kernel.
-inline bool window_few_selected(const char* v, int rows, int npairs, int row_bytes, bool stage2 = false) {
+inline bool window_few_selected(const char* v, FewKernel kernel, long blocks, int head_dim, int bytes) {
   if (v != nullptr && *v != 0) return std::strcmp(v, "few") == 0;
-  return window_few_rule(rows, npairs, row_bytes, stage2, resident_workgroups(1));
+  return window_few_rule(kernel, blocks, head_dim, bytes, resident_workgroups(1));
 }
 
 // Workgroups of a key-tiled launch with blocks of `rows` keys.

@@ -54,10 +54,14 @@ template <typename T, int D> hipError_t launch_window_dkdv(const BwdParams<T>& p
       const hipError_t e = launch_few_dkdv<T, D>(p, true, stream);
       if (e != hipSuccess) return e;
     }
-    if (window_few_selected(std::getenv("FLASH_HOG_BWD"), p.nk, p.batch * p.kv_heads, D * (int)sizeof(T)))
-      return launch_few_dkdv<T, D>(own_launch(p), false, stream);
   }
-  return launch_bwd_pair<T, D, kWindow>(own_launch(p), stream);
+  const BwdParams<T> own = own_launch(p);
+  if constexpr (kFewServes<T, D>) {
+    if (window_few_selected(std::getenv("FLASH_HOG_BWD"), FewKernel::kDkdv, key_grid<kWindow>(own, 32), D,
+                            (int)sizeof(T)))
+      return launch_few_dkdv<T, D>(own, false, stream);
+  }
+  return launch_bwd_pair<T, D, kWindow>(own, stream);
 }
 
 template <typename T, int D> hipError_t launch_window_bwd(const BwdParams<T>& p, hipStream_t stream) {

@@ -8,8 +8,12 @@
 // sinks: the queries that see one behind their window (SinkGrid) meet 32 keys or fewer, so
 // that in a key-tiled workgroup all waves but one would idle.
 //
-// 256-byte rows at most (2-byte types at D = 64 and 128, fp32 at 64): two stages of a ring for each
-// of four waves then fill 128 KiB of LDS, one stage of stage 2's three tensors 96 KiB.
+// 256-byte rows at most (2-byte types at D = 64 and 128, fp32 at 64). A wave's ring has two stages
+// where they leave room for two workgroups on a CU, and where registers allow one anyway; else one
+// stage and two workgroups, which hide each other's loads: causal N1000 window 256, H8 fp32 (256
+// blocks) dK/dV 43.4 -> 36.9 us, H16 D128 bf16 (512) forward 26.6 -> 14.8, dQ 24.4 -> 19.8. (Eight
+// waves a workgroup at fp32: 44.2; the blocks are bound by the CU's matrix rate, 256 operations a
+// cycle.)
 #include "fhog_device.h"
 #include "fhog_params.h"
 
@@ -19,15 +23,18 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
+template <typename T, int D> constexpr bool kNarrow = D * sizeof(T) <= 128;  // rows of 128 bytes
+
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // A wave's ring of tiles of TENSORS tensors with the same rows, and of STATS rows of 32 fp32
 // statistics behind them (256 bytes each). Tile i of the wave is in stage i % kStages.
-template <typename T, int D, int TENSORS, int STATS> struct WaveRing {
+template <typename T, int D, int TENSORS, int STATS, int STAGES>
+struct WaveRing {
   typedef SwzTile<T, D> G;
   static constexpr int kTile = G::kElems * (int)sizeof(T);
   static constexpr int kStage = TENSORS * kTile + STATS * 256;
-  static constexpr int kStages = kWaves * 2 * kStage <= 160 * 1024 ? 2 : 1;
+  static constexpr int kStages = STAGES;
   static constexpr int kBytes = kStages * kStage;
   static constexpr int kOps = TENSORS * G::kLoads + STATS;  // vector-memory operations of a tile
   uint32_t lds, row_bytes;
@@ -99,10 +106,10 @@ template <int DT> struct Box {
 // ------------------------------------------------------------------ forward
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1)))
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 few_fwd_kernel(FwdParams<T> p) {
   constexpr int KS = D / 16, DT = D / 32;
-  typedef WaveRing<T, D, 2, 0> Ring;
+  typedef WaveRing<T, D, 2, 0, kNarrow<T, D> ? 2 : 1> Ring;
   constexpr int kLds = kWaves * (Ring::kBytes > DT * 4096 ? Ring::kBytes : DT * 4096);
   __shared__ __attribute__((aligned(1024))) char s_kv[kLds];
   __shared__ float s_ml[kWaves][32][2];
@@ -221,10 +228,10 @@ few_fwd_kernel(FwdParams<T> p) {
 // ------------------------------------------------------------------ dQ and D
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1)))
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 few_dq_kernel(BwdParams<T> p) {
   constexpr int KS = D / 16, DT = D / 32;
-  typedef WaveRing<T, D, 2, 0> Ring;
+  typedef WaveRing<T, D, 2, 0, kNarrow<T, D> ? 2 : 1> Ring;
   constexpr int kLds = kWaves * (Ring::kBytes > DT * 4096 ? Ring::kBytes : DT * 4096);
   __shared__ __attribute__((aligned(1024))) char s_kv[kLds];
 
@@ -362,10 +369,10 @@ __device__ __forceinline__ void few_store(const P& p, const FewBlock& fb, const 
 }
 
 template <typename T, int D, bool ONLY_SINKS>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1)))
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : 1)))
 few_dkdv_kernel(BwdParams<T> p) {
   constexpr int KS = D / 16, DT = D / 32;
-  typedef WaveRing<T, D, 2, 2> Ring;
+  typedef WaveRing<T, D, 2, 2, sizeof(T) == 2 ? 2 : 1> Ring;
   constexpr int kBox = kWaves * DT * 4096;
   constexpr int kLds = kWaves * Ring::kBytes > 2 * kBox ? kWaves * Ring::kBytes : 2 * kBox;
   __shared__ __attribute__((aligned(1024))) char s_q[kLds];
@@ -473,7 +480,7 @@ template <typename T, int D, bool ONLY_SINKS>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1)))
 few_stage2_kernel(BwdBwdParams<T> p) {
   constexpr int KS = D / 16, DT = D / 32;
-  typedef WaveRing<T, D, 3, 4> Ring;
+  typedef WaveRing<T, D, 3, 4, kNarrow<T, D> ? 2 : 1> Ring;
   constexpr int kBox = kWaves * DT * 4096;
   constexpr int kLds = kWaves * Ring::kBytes > 2 * kBox ? kWaves * Ring::kBytes : 2 * kBox;
   __shared__ __attribute__((aligned(1024))) char s_q[kLds];
