@@ -177,6 +177,54 @@ template <typename T, typename C, int D, int THREADS, int SWZ, int TENSORS = 2> 
   }
 };
 
+// PageTile's rows straight to LDS, for 2-byte caches: each load a wave's LDS DMA from one half of the
+// tile, whose rows lie in one page, so that the address is the half's first row, uniform, and a
+// lane's offset from it, the same for every whole tile.
+template <typename T, int D, int THREADS, int SWZ> struct PageDma {
+  static constexpr int kRowBytes = D * (int)sizeof(T);
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kWaveRows = 64 / kChunks;               // of a load
+  static constexpr int kEach = 32 * kChunks / THREADS;         // a wave's loads of one tensor
+  static constexpr int kLoads = 2 * kEach;
+  static constexpr int kTileBytes = 32 * kRowBytes;
+  static_assert(32 * kChunks % THREADS == 0 && 16 % kWaveRows == 0, "tile must divide into whole loads of a half");
+  int wave, lane;
+  uint32_t voff[kEach];
+
+  __device__ __forceinline__ int first_row(int i) const { return i * (THREADS / kChunks) + wave * kWaveRows; }
+  __device__ __forceinline__ uint32_t chunk(int i) const {
+    return 16u * (uint32_t)phys_chunk<SWZ>(first_row(i) + lane / kChunks, lane % kChunks);
+  }
+  // wave (uniform) and lane within the THREADS threads that fill a tile.
+  __device__ __forceinline__ PageDma(int wave_, int lane_) : wave(wave_), lane(lane_) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      voff[i] = (uint32_t)((first_row(i) & 15) + lane / kChunks) * kRowBytes + chunk(i);
+  }
+  // PageTile::fetch; pages uniform and in the cache.
+  __device__ __forceinline__ void issue(uint32_t lds, const CacheRows<T>& cache, int hk, int kv_heads, int page_shift,
+                                        int k0, int rlo, int rhi, int page0, int page1) const {
+    const int page_rows = 1 << page_shift;
+    const int first1 = min(rhi, 16);  // of the second half's rows, those that are read
+    const long line0 = (((long)page0 * kv_heads + hk) << page_shift) + ((k0 + rlo) & (page_rows - 1));
+    const long line1 = (((long)page1 * kv_heads + hk) << page_shift) + ((k0 + first1) & (page_rows - 1));
+    const bool whole = rlo == 0 && rhi == 31;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const bool second = first_row(i) >= 16;
+      const long line = second ? line1 : line0;
+      uint32_t at = voff[i];
+      if (!whole) {
+        const int row = min(max(first_row(i) + lane / kChunks, rlo), rhi) - (second ? first1 : rlo);
+        at = (uint32_t)row * kRowBytes + chunk(i);
+      }
+      const uint32_t dst = lds + 1024u * (uint32_t)(i * (THREADS / 64) + wave);
+      dma16s(cache.k + line * D, at, dst);
+      dma16s(cache.v + line * D, at, dst + kTileBytes);
+    }
+  }
+};
+
 // A tile's keys as one wave's operands of the 16x16x32 score products, straight from their pages:
 // lane (n, g) holds pieces of keys n and 16 + n. A piece is 16 bytes of cache: 8 elements, columns
 // 32 c + 8 g on, one product's; or 16 of e4m3, columns 64 c + 16 g on, two products' (the

@@ -296,7 +296,7 @@ paged_token_kernel(PagedParams<T, C> p) {
 
 // Waves that share a tile of keys, 32 rows each: RW of four; the 4 / RW groups of them take
 // every (4 / RW)-th tile and join at the end.
-// (128 rows at D = 128: three waves per SIMD, 168 registers and 8 of them spilled outside the
+// (128 rows at D = 128: three waves per SIMD, 168 registers and one of them spilled outside the
 // loop, 158 -> 142 us for 8 sequences with 17 to 512 new tokens of 32 heads over 8, window 2048.)
 template <typename T, typename C, int D, int RW>
 __global__ void __launch_bounds__(256)
@@ -304,9 +304,12 @@ __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 64 || RW == 4 ? 3 : 2)))
 paged_chunk_kernel(PagedParams<T, C> p) {
   constexpr int ROWS = 32 * RW, KW = 4 / RW;
   constexpr int KS = D / 16, DT = D / 32;
-  typedef PageTile<T, C, D, 64 * RW, D == 64 ? kSwzPairs : kSwzWide> Tile;
+  constexpr int kSwz = D == 64 ? kSwzPairs : kSwzWide;
+  typedef PageTile<T, C, D, 64 * RW, kSwz> Tile;
+  constexpr bool kDma = sizeof(C) == sizeof(T);
   constexpr int kStage = 2 * Tile::kTileBytes;
-  __shared__ __attribute__((aligned(1024))) char s_kv[KW * 2 * kStage];
+  constexpr int kStages = kDma && KW * 3 * kStage <= (D == 256 ? 160 : 53) * 1024 ? 3 : 2;
+  __shared__ __attribute__((aligned(1024))) char s_kv[KW * kStages * kStage];
   __shared__ float s_ml[KW][ROWS][2];
 
   const int lane = threadIdx.x & 63;
@@ -344,47 +347,20 @@ paged_chunk_kernel(PagedParams<T, C> p) {
 
   std::conditional_t<D == 64, SwzFrags<T, D>, WideFrags<T, D>> fr;
   fr.init(lane);
-  const uint32_t lds = lds_base_u32(s_kv) + kw * 2 * kStage;
+  const uint32_t lds = lds_base_u32(s_kv) + kw * kStages * kStage;
   float m = -1e30f, lpart = 0.f;
   f32x16 acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
   bool bad = rt.beyond;
 
-  Tile tile;
-  Pages pages;
-  const int zero = vector_zero();
-  // Fetches tile t, whose pages are there, and loads those of this group's next one.
-  auto fetch = [&](int t) {
-    bad |= pages.check(p.at);
-    tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, span.key(t), span.first_row(t), span.last_row(t),
-               pages.page0, pages.page1, thread);
-    if (t + KW < t1) pages.load(p.at, span, rt.b, t + KW, zero);
-  };
-  // In step i a group works on tile t0 + kw + KW i, if there is one. It was stored to stage
-  // i % 2 in step i - 1, whose barrier at its end shows it; the stage's last readers passed the
-  // barrier of step i - 2.
-  const int steps = (t1 - t0 + KW - 1) / KW;
-  const int mine = t0 + kw;
-  if (mine < t1) {
-    pages.load(p.at, span, rt.b, mine, zero);
-    fetch(mine);
-    tile.store(lds, thread);
-    if (mine + KW < t1) fetch(mine + KW);
-  }
-  __syncthreads();
-  for (int i = 0; i < steps; ++i) {
-    const int t = mine + KW * i;
-    if (t + KW < t1) {
-      tile.store(lds + ((i + 1) & 1) * kStage, thread);
-      if (t + 2 * KW < t1) fetch(t + 2 * KW);
-    }
+  // Tile t, staged at sa, for this wave's rows.
+  auto attend = [&](int t, uint32_t sa) {
     const int k0 = span.key(t);
     // a wave's own positions: nothing before its window's start or behind its last row
-    const bool active = any && t < t1 && k0 <= wlast &&
+    const bool active = any && k0 <= wlast &&
                         (t < span.sink_tiles || !p.window || k0 + 31 > wfirst - p.window || k0 < p.sinks);
     if (active) {
-      const uint32_t sa = lds + (i & 1) * kStage;
       f32x16 S = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) S = mma<T>(fr.rowf(sa, 0, ks), qf[ks], S);
@@ -429,14 +405,84 @@ paged_chunk_kernel(PagedParams<T, C> p) {
         for (int dt = 0; dt < DT; ++dt) acc[dt] = mma<T>(fr.trf(sa, Tile::kTileBytes, dt, s), oP, acc[dt]);
       }
     }
+  };
+
+  const int steps = (t1 - t0 + KW - 1) / KW;
+  const int mine = t0 + kw;
+  if constexpr (kDma) {
+    // A ring of kStages tiles, filled by LDS DMAs. The tiles' pages come through LDS too, those
+    // of kIds steps at a time: a load from global memory in the loop would wait for the DMAs.
+    constexpr int kIds = 128;
+    __shared__ int s_ids[KW][kIds][2];
+    const PageDma<T, D, 64 * RW, kSwz> dma(rw, lane);
+    for (int s0 = 0; s0 < steps; s0 += kIds) {
+      const int first = mine + KW * s0, rounds = min(kIds, steps - s0);
+      const int count = min(rounds, (t1 - first + KW - 1) / KW);  // this group's tiles (may be below zero)
+      if (s0 > 0) __syncthreads();
+      for (int i = thread; i < count; i += 64 * RW) {
+        Pages pages;
+        pages.load(p.at, span, rt.b, first + KW * i, 0);
+        s_ids[kw][i][0] = (unsigned)pages.page0 < (unsigned)p.at.pages ? pages.page0 : -1;
+        s_ids[kw][i][1] = (unsigned)pages.page1 < (unsigned)p.at.pages ? pages.page1 : -1;
+      }
+      wait_vmem();
+      __syncthreads();
+      auto issue = [&](int i) {
+        const int page0 = __builtin_amdgcn_readfirstlane(s_ids[kw][i][0]);
+        const int page1 = __builtin_amdgcn_readfirstlane(s_ids[kw][i][1]);
+        bad |= page0 < 0 || page1 < 0;
+        const int t = first + KW * i;
+        dma.issue(lds + (uint32_t)(i % kStages) * kStage, p.cache, hk, p.at.kv_heads, p.at.page_shift, span.key(t),
+                  span.first_row(t), span.last_row(t), max(page0, 0), max(page1, 0));
+      };
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i)
+        if (i < count) issue(i);
+      for (int i = 0; i < rounds; ++i) {
+        wait_tile<kStages, dma.kLoads>(i, count);
+        __syncthreads();
+        if (i + kStages - 1 < count) issue(i + kStages - 1);
+        if (i < count) attend(first + KW * i, lds + (uint32_t)(i % kStages) * kStage);
+      }
+    }
     __syncthreads();
+  } else {
+    Tile tile;
+    Pages pages;
+    const int zero = vector_zero();
+    // Fetches tile t, whose pages are there, and loads those of this group's next one.
+    auto fetch = [&](int t) {
+      bad |= pages.check(p.at);
+      tile.fetch(p.cache, hk, p.at.kv_heads, p.at.page_shift, span.key(t), span.first_row(t), span.last_row(t),
+                 pages.page0, pages.page1, thread);
+      if (t + KW < t1) pages.load(p.at, span, rt.b, t + KW, zero);
+    };
+    // In step i a group works on tile t0 + kw + KW i, if there is one. It was stored to stage
+    // i % 2 in step i - 1, whose barrier at its end shows it; the stage's last readers passed the
+    // barrier of step i - 2.
+    if (mine < t1) {
+      pages.load(p.at, span, rt.b, mine, zero);
+      fetch(mine);
+      tile.store(lds, thread);
+      if (mine + KW < t1) fetch(mine + KW);
+    }
+    __syncthreads();
+    for (int i = 0; i < steps; ++i) {
+      const int t = mine + KW * i;
+      if (t + KW < t1) {
+        tile.store(lds + ((i + 1) & 1) * kStage, thread);
+        if (t + 2 * KW < t1) fetch(t + 2 * KW);
+      }
+      if (t < t1) attend(t, lds + (i & 1) * kStage);
+      __syncthreads();
+    }
   }
 
   if (bad) lpart = NAN;
   float l = xgroup_sum(lpart);
   if constexpr (KW > 1) {
     // The other groups hand their sums to the first, in LDS in place of the tiles.
-    static_assert((KW - 1) * RW * DT * 4096 <= KW * 2 * kStage, "the join reuses the tiles");
+    static_assert((KW - 1) * RW * DT * 4096 <= KW * kStages * kStage, "the join reuses the tiles");
     float* box = reinterpret_cast<float*>(s_kv) + 4 * lane;
     auto place = [&](int k, int dt, int a) { return box + 256 * (((k - 1) * RW + rw) * DT * 4 + 4 * dt + a); };
     if (kw > 0) {
