@@ -29,6 +29,8 @@ those of the Python Functions, bit for bit.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -127,6 +129,7 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     else:
         if not is_causal:
             raise ValueError("window needs is_causal=True")
+        window, sinks = operator.index(window), operator.index(sinks)
         if window < 1 or sinks < 0:
             raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
         if query.ndim in (3, 4) and key.ndim == query.ndim:

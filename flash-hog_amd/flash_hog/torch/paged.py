@@ -33,6 +33,8 @@ tile, though, a NaN or infinity in a value that one token sees also reaches the 
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from flash_hog import _hip
@@ -101,8 +103,10 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_of
         if sinks != 0:
             raise ValueError(f"sinks needs a window, got sinks={sinks}")
         window = 0
-    elif window < 1 or sinks < 0:
-        raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
+    else:
+        window, sinks = operator.index(window), operator.index(sinks)
+        if window < 1 or sinks < 0:
+            raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
     scale = _default_scale(query, scale)
     args = (query, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale, window, sinks,
             scale)

@@ -319,3 +319,31 @@ def test_refused_calls_on_the_device(cuda_device, monkeypatch):
             with pytest.raises((ValueError, TypeError, _hip.FlashHogError), match=needle):
                 call()
                 pytest.fail(f"call {i} was accepted")
+
+
+@pytest.mark.parametrize("D,dtype,new,kv_heads", [(64, BF16, 260, 192), (64, FP16, 64, 256), (128, FP16, 260, 192),
+                                                   (128, BF16, 64, 256), (256, BF16, 260, 192)])
+def test_long_chunks(D, dtype, new, kv_heads, cuda_device):
+    """Chunks that sweep thousands of keys in one go (heads enough that no split is made), in tiles
+    of 128 rows and of 64; then with a page far back that is none."""
+    import flash_hog
+
+    length, page = 9000, 32
+    print("[case] long chunk", D, dtype, new, kv_heads, flush=True)
+    gen = torch.Generator(device=cuda_device).manual_seed(D + new)
+    pages = -(-length // page)
+    cache = [torch.randn((pages, kv_heads, page, D), generator=gen, device=cuda_device, dtype=dtype) for _ in "kv"]
+    table = torch.randperm(pages, generator=gen, device=cuda_device).to(torch.int32)[None]
+    q = torch.randn((new, kv_heads, D), generator=gen, device=cuda_device, dtype=dtype)
+    kwargs = dict(lengths=torch.tensor([length], dtype=torch.int32, device=cuda_device),
+                  query_offsets=torch.tensor([0, new], dtype=torch.int32, device=cuda_device))
+    out = flash_hog.paged_attention(q, *cache, table, **kwargs)
+    hidden = torch.ones((new, length), dtype=torch.bool, device=cuda_device).triu(length - new + 1)
+    for head in (0, kv_heads // 2 + 1, kv_heads - 1):
+        k, v = (c[table[0].long(), head].flatten(0, 1)[:length].double() for c in cache)
+        scores = (q[:, head].double() @ k.T * D ** -0.5).masked_fill(hidden, float("-inf"))
+        check(out[:, head], (torch.softmax(scores, -1) @ v).cpu(), str(head))
+    table[0, pages - 3] = -1  # most tiles lie before it; tokens at positions from its first key on see it
+    out = flash_hog.paged_attention(q, *cache, table, **kwargs)
+    first = max(0, page * (pages - 3) - (length - new))
+    assert bool(torch.isnan(out[first:]).all())

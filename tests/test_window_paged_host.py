@@ -196,6 +196,9 @@ def test_window_arguments_are_checked():
             flash_hog.dot_product_attention(q, q, q, is_causal=True, window=window, sinks=sinks)
     with pytest.raises(ValueError, match="sinks needs a window"):
         flash_hog.dot_product_attention(q, q, q, is_causal=True, sinks=1)
+    for window, sinks in ((4.0, 0), (4, 1.5), ("4", 0)):
+        with pytest.raises(TypeError):
+            flash_hog.dot_product_attention(q, q, q, is_causal=True, window=window, sinks=sinks)
     for args in ((-1, 0), (0, 1), (3, -1)):
         with pytest.raises(ValueError, match="window"):
             _hip._window_args(*args)
@@ -276,6 +279,8 @@ def test_paged_window_arguments_are_checked():
             flash_hog.paged_attention(q, **_cache(), window=window, sinks=sinks)
     with pytest.raises(ValueError, match="sinks needs a window"):
         flash_hog.paged_attention(q, **_cache(), sinks=2)
+    with pytest.raises(TypeError):
+        flash_hog.paged_attention(q, **_cache(), window=2.5)
     with pytest.raises(ValueError, match="page_table"):
         flash_hog.paged_cache_read(**_cache(page_table=torch.zeros(3, dtype=torch.int32)))
 
