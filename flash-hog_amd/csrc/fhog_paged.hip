@@ -567,11 +567,12 @@ paged_join_kernel(PagedParams<T, C> p) {
     for (int i = lane; i < splits; i += 64) top = fmaxf(top, parts.ml[2 * (i * ROWS + row)]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    for (int i = lane; i < splits; i += 64) sum += exp2_fast(parts.ml[2 * (i * ROWS + row)] - top) * parts.ml[2 * (i * ROWS + row) + 1];
+    auto weight = [&](int i) { return exp2_fast(parts.ml[2 * (i * ROWS + row)] - top); };
+    for (int i = lane; i < splits; i += 64) sum += weight(i) * parts.ml[2 * (i * ROWS + row) + 1];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing: 0
-    for (int i = lane; i < splits; i += 64) s_w[row * splits + i] = exp2_fast(parts.ml[2 * (i * ROWS + row)] - top) * inv;
+    for (int i = lane; i < splits; i += 64) s_w[row * splits + i] = weight(i) * inv;
   }
   __syncthreads();
   const int units = rt.rows * (D / 4);

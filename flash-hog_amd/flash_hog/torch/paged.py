@@ -44,9 +44,11 @@ Tensor = torch.Tensor
 
 
 def _refuse_gradients(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no derivative: call it under torch.no_grad() (training attends through "
-                           "flash_hog.dot_product_attention)")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{name} has no derivative: call it under torch.no_grad() (training attends through "
+                                   "flash_hog.dot_product_attention)")
 
 
 @torch.library.custom_op("flash_hog::paged_attention", mutates_args=())
@@ -122,7 +124,8 @@ def paged_cache_write(key, value, key_cache, value_cache, page_table, lengths, q
     """Writes key and value (T, N_kv, H) of the packed new tokens to their places in the cache, in
     place. An e4m3 cache gets each row quantised: its scale is the smallest power of two (at least
     2 ** -126) with which the row's largest finite magnitude stays within 448, its values round
-    to nearest even, and infinities become NaN. Rows of no sequence and tokens at
+    to nearest even, and infinities become NaN; a value within 1/32 of the type's largest may
+    round beyond it, and then reads as infinite. Rows of no sequence and tokens at
     positions below zero (a sequence of length zero) are not written. No two tokens may name the
     same place: pages that sequences share are read-only."""
     _refuse_gradients("paged_cache_write", key, value, key_cache, value_cache)
