@@ -366,12 +366,22 @@ paged_chunk_kernel(PagedParams<T, C> p) {
       for (int ks = 0; ks < KS; ++ks) S = mma<T>(fr.rowf(sa, 0, ks), qf[ks], S);
       const int rlo = span.first_row(t), rhi = span.last_row(t);
       if (rlo > 0 || rhi < 31 || k0 + 31 > wfirst || (p.window && k0 <= wlast - p.window)) {
+        asm volatile("");  // (a branch: the compiler would take the masks' instructions into every tile)
         const int klim = min(rhi, pos - k0);
-        const int klow = p.window ? pos - p.window + 1 - k0 : 0, ksinks = p.sinks - k0;
+        const int wlow = p.window && t >= span.sink_tiles ? pos - p.window + 1 - k0 : 0, klow = max(rlo, wlow);
+        if (t >= span.sink_tiles && p.sinks - k0 > rlo) {  // sinks among the window's keys
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int key = crow(j, g);
-          if (key > klim || key < rlo || (key < klow && key >= ksinks)) S[j] = -INFINITY;
+          for (int j = 0; j < 16; ++j) {
+            const int key = crow(j, g);
+            if (key > klim || key < rlo || (key < klow && key >= p.sinks - k0)) S[j] = -INFINITY;
+          }
+        } else {
+          // klow <= key <= klim as one comparison; no key if there is none between
+          const int from = crow(0, g) - (klow <= klim ? klow : 64);
+          const unsigned most = (unsigned)max(klim - klow, 0);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if ((unsigned)(from + crow(j, 0)) > most) S[j] = -INFINITY;
         }
       }
       f32x16 P;
