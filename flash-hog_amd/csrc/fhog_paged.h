@@ -201,26 +201,40 @@ template <typename T, int D, int THREADS, int SWZ> struct PageDma {
     for (int i = 0; i < kEach; ++i)
       voff[i] = (uint32_t)((first_row(i) & 15) + lane / kChunks) * kRowBytes + chunk(i);
   }
-  // PageTile::fetch; pages uniform and in the cache.
-  __device__ __forceinline__ void issue(uint32_t lds, const CacheRows<T>& cache, int hk, int kv_heads, int page_shift,
-                                        int k0, int rlo, int rhi, int page0, int page1) const {
-    const int page_rows = 1 << page_shift;
-    const int first1 = min(rhi, 16);  // of the second half's rows, those that are read
-    const long line0 = (((long)page0 * kv_heads + hk) << page_shift) + ((k0 + rlo) & (page_rows - 1));
-    const long line1 = (((long)page1 * kv_heads + hk) << page_shift) + ((k0 + first1) & (page_rows - 1));
-    const bool whole = rlo == 0 && rhi == 31;
+  // Where a tile's halves begin: the byte offset of the first row of each that is read. In their
+  // lowest bits, which rows leave free: whether a page is none (the first's), and whether rows
+  // of the tile are not read (the second's).
+  struct Place {
+    long half[2];
+  };
+  __device__ __forceinline__ static Place place(const CacheShape& c, int hk, int k0, int rlo, int rhi, int page0,
+                                                int page1) {
+    const bool none = (unsigned)page0 >= (unsigned)c.pages || (unsigned)page1 >= (unsigned)c.pages;
+    if (none) page0 = page1 = 0;
+    const int in_page = (1 << c.page_shift) - 1;
+    auto row = [&](int page, int r) {
+      return ((((long)page * c.kv_heads + hk) << c.page_shift) + ((k0 + r) & in_page)) * kRowBytes;
+    };
+    return {{row(page0, rlo) + none, row(page1, min(rhi, 16)) + (rlo > 0 || rhi < 31)}};
+  }
+  // Rows [rlo, rhi] of a tile, the nearest of them for the others (PageTile::fetch).
+  __device__ __forceinline__ void issue(uint32_t lds, const CacheRows<T>& cache, const Place& at, int rlo,
+                                        int rhi) const {
+    const char* const k = reinterpret_cast<const char*>(cache.k);
+    const char* const v = reinterpret_cast<const char*>(cache.v);
+    const bool whole = (at.half[1] & 1) == 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const bool second = first_row(i) >= 16;
-      const long line = second ? line1 : line0;
-      uint32_t at = voff[i];
+      const long from = (second ? at.half[1] : at.half[0]) & ~1l;
+      uint32_t offset = voff[i];
       if (!whole) {
-        const int row = min(max(first_row(i) + lane / kChunks, rlo), rhi) - (second ? first1 : rlo);
-        at = (uint32_t)row * kRowBytes + chunk(i);
+        const int row = min(max(first_row(i) + lane / kChunks, rlo), rhi) - (second ? min(rhi, 16) : rlo);
+        offset = (uint32_t)row * kRowBytes + chunk(i);
       }
       const uint32_t dst = lds + 1024u * (uint32_t)(i * (THREADS / 64) + wave);
-      dma16s(cache.k + line * D, at, dst);
-      dma16s(cache.v + line * D, at, dst + kTileBytes);
+      dma16s(k + from, offset, dst);
+      dma16s(v + from, offset, dst + kTileBytes);
     }
   }
 };

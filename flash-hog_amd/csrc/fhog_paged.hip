@@ -420,38 +420,45 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   const int steps = (t1 - t0 + KW - 1) / KW;
   const int mine = t0 + kw;
   if constexpr (kDma) {
-    // A ring of kStages tiles, filled by LDS DMAs. The tiles' pages come through LDS too, those
-    // of kIds steps at a time: a load from global memory in the loop would wait for the DMAs.
-    constexpr int kIds = 128;
-    __shared__ int s_ids[KW][kIds][2];
-    const PageDma<T, D, 64 * RW, kSwz> dma(rw, lane);
-    for (int s0 = 0; s0 < steps; s0 += kIds) {
-      const int first = mine + KW * s0, rounds = min(kIds, steps - s0);
+    // A ring of kStages tiles, filled by LDS DMAs. Where the tiles begin comes through LDS too, for
+    // kAhead steps at a time: a load from global memory in the loop would wait for the DMAs.
+    constexpr int kAhead = 128 / KW;
+    typedef PageDma<T, D, 64 * RW, kSwz> Dma;
+    __shared__ typename Dma::Place s_at[KW][kAhead];
+    const Dma dma(rw, lane);
+    for (int s0 = 0; s0 < steps; s0 += kAhead) {
+      const int first = mine + KW * s0, rounds = min(kAhead, steps - s0);
       const int count = min(rounds, (t1 - first + KW - 1) / KW);  // this group's tiles (may be below zero)
       if (s0 > 0) __syncthreads();
       for (int i = thread; i < count; i += 64 * RW) {
+        const int t = first + KW * i;
         Pages pages;
-        pages.load(p.at, span, rt.b, first + KW * i, 0);
-        s_ids[kw][i][0] = (unsigned)pages.page0 < (unsigned)p.at.pages ? pages.page0 : -1;
-        s_ids[kw][i][1] = (unsigned)pages.page1 < (unsigned)p.at.pages ? pages.page1 : -1;
+        pages.load(p.at, span, rt.b, t, 0);
+        s_at[kw][i] = Dma::place(p.at, hk, span.key(t), span.first_row(t), span.last_row(t), pages.page0, pages.page1);
       }
       wait_vmem();
       __syncthreads();
-      auto issue = [&](int i) {
-        const int page0 = __builtin_amdgcn_readfirstlane(s_ids[kw][i][0]);
-        const int page1 = __builtin_amdgcn_readfirstlane(s_ids[kw][i][1]);
-        bad |= page0 < 0 || page1 < 0;
+      auto issue = [&](int i, const typename Dma::Place& place) {
+        typename Dma::Place at;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)place.half[h]);
+          const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(place.half[h] >> 32));
+          at.half[h] = (long)((unsigned long)hi << 32 | lo);
+        }
+        bad |= (at.half[0] & 1) != 0;
         const int t = first + KW * i;
-        dma.issue(lds + (uint32_t)(i % kStages) * kStage, p.cache, hk, p.at.kv_heads, p.at.page_shift, span.key(t),
-                  span.first_row(t), span.last_row(t), max(page0, 0), max(page1, 0));
+        dma.issue(lds + (uint32_t)(i % kStages) * kStage, p.cache, at, span.first_row(t), span.last_row(t));
       };
 #pragma unroll
       for (int i = 0; i < kStages - 1; ++i)
-        if (i < count) issue(i);
+        if (i < count) issue(i, s_at[kw][i]);
+      typename Dma::Place next = s_at[kw][min(kStages - 1, kAhead - 1)];  // (a step ahead of its use)
       for (int i = 0; i < rounds; ++i) {
-        wait_tile<kStages, dma.kLoads>(i, count);
+        wait_tile<kStages, Dma::kLoads>(i, count);
         __syncthreads();
-        if (i + kStages - 1 < count) issue(i + kStages - 1);
+        if (i + kStages - 1 < count) issue(i + kStages - 1, next);
+        next = s_at[kw][min(i + kStages, kAhead - 1)];
         if (i < count) attend(first + KW * i, lds + (uint32_t)(i % kStages) * kStage);
       }
     }
