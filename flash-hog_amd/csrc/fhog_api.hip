@@ -537,7 +537,7 @@ int fhog_paged_attention(fhog_stream_t stream, const void* q, const void* k_cach
     fhog::PagedParams<T, C> p{(const T*)q, (T*)out,
                               {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
                               cache_shape(s, page_table, lengths, query_offsets), (float*)workspace, heads, window,
-                              sinks, plan.slots, plan.splits, plan.split_tiles, clear_rest, scale};
+                              sinks, plan.slots, plan.splits, plan.split_tiles, plan.longest_first, clear_rest, scale};
     return fhog::launch_paged_attention<T, C, D>(p, plan.rows, (hipStream_t)stream);
   };
   return launch_status(dispatch_paged(s, run), who);

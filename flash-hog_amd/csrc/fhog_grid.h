@@ -464,6 +464,7 @@ struct PagedPlan {
   int waves;        // of a workgroup of paged_token_kernel
   int splits, split_tiles;  // splits of split_tiles 32-key tiles; one split: no join
   long parts;       // fp32 rows of head_dim + 2 in the workspace
+  bool longest_first;  // whether paged_chunk_kernel sorts its tiles by their keys
 };
 constexpr int kJoinWeights = 2048;  // the most rows of a tile times splits
 // us, H32/8 D128, with the chosen number and those on both sides of it:
@@ -511,6 +512,12 @@ inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv
   p.split_tiles = (int)((tiles + splits - 1) / splits);
   p.splits = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
   p.parts = p.splits > 1 ? blocks * p.splits * p.rows : 0;
+  // Sorting evens out the last round, but takes a workgroup about 1 us and mixes the sequences whose
+  // tiles would share L2: up to eight tiles a CU. us, sorted / by sequence, prompts of the lengths named:
+  // B4 N2048 H16 D128 (1088 tiles of rows) 93.5 / 103.8, B8 500 to 4000 H12 D64 (1788) 124 / 141, B4 1000 to
+  // 4000 H8/4 D256 (644) 256 / 311, B16 x 512 new H32/8 D128 (1664) 101.1 / 100.8; B32 100 to 1000 H16 D64
+  // (2710) 74 / 79, B40 N500 H16 D128 (3140) 118 / 108, B16 200 to 2000 H32/8 (4528) 273 / 267.
+  p.longest_first = p.rows > 16 && p.splits == 1 && window == 0 && batch > 1 && batch <= 64 && blocks <= 8l * cus;
   return p;
 }
 

@@ -49,6 +49,7 @@ template <typename T, typename C> struct PagedParams {
   float* parts;  // fp32 outputs of the splits, (slot, kv_head, split, row of the tile, head_dim), and their m, l
   int heads, window, sinks;  // window 0: none
   int slots, splits, split_tiles;
+  int longest_first;  // PagedPlan
   int clear_rest;  // whether rows of no sequence are zeroed
   float scale;
 };
@@ -94,6 +95,63 @@ template <typename F> __device__ __forceinline__ int last_at_or_before(int count
       hi = mid - 1;
   }
   return lo;
+}
+
+// A wave's sum over its lanes, in every lane.
+__device__ __forceinline__ int wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Sequence and tile (of ROWS rows) that come at place `order` when all tiles are sorted by the keys
+// that their last rows see, most first, then by sequence: at most 64 sequences, one a lane. False
+// behind the last tile.
+template <int ROWS>
+__device__ __forceinline__ bool longest_first(const CacheShape& c, int group, int order, int lane, int& seq, int& tile) {
+  const bool mine = lane < c.batch;
+  const int begin = mine ? packed_begin(c, lane) : 0;
+  const int count = mine ? max(0, packed_begin(c, lane + 1) - begin) : 0;
+  const int before = mine ? min(max(0, c.lengths[lane]), 1 << 30) - count : 0;  // keys before the new ones
+  const long rows = (long)count * group;
+  const int tiles = (int)((rows + ROWS - 1) / ROWS);
+  // How many of this lane's tiles see at least `keys` keys: those from the tile of the first row that does.
+  auto at_least = [&](int keys) {
+    const long row = max(0l, ((long)keys - 1 - before) * group);
+    return row < rows ? tiles - (int)(row / ROWS) : 0;
+  };
+  if (order >= wave_sum(tiles)) return false;
+  int lo = count > 0 ? before : 0x7fffffff, hi = count > 0 ? before + count : -0x7fffffff;
+  for (int d = 1; d < 64; d <<= 1) {
+    lo = min(lo, __shfl_xor(lo, d, 64));
+    hi = max(hi, __shfl_xor(hi, d, 64));
+  }
+  // The most keys that more than `order` tiles see: all see lo, none more than hi.
+  hi = __builtin_amdgcn_readfirstlane(hi) + 1;
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (wave_sum(at_least(mid)) > order)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  // Among the tiles that see exactly lo, in order of their lanes.
+  const int more = at_least(lo + 1), equal = at_least(lo) - more;
+  int through = equal;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int x = __shfl_up(through, d, 64);
+    if (lane >= d) through += x;
+  }
+  const int place = order - wave_sum(more) - (through - equal);
+  const unsigned long here = __ballot(place >= 0 && place < equal);
+  seq = __builtin_amdgcn_readfirstlane(here ? __builtin_ctzl(here) : 0);
+  tile = __builtin_amdgcn_readlane(tiles - 1 - more - place, seq);
+  return here != 0;
 }
 
 // ---------------------------------------------------------------------------

@@ -12,7 +12,10 @@
 // kWaves-th tile of 32 keys each on their own, through LDS of their own (no barrier in
 // the sweep), and join at the end.
 // paged_chunk_kernel, for many: 32 rows a wave, 128 rows a workgroup, all its waves on the same
-// tile, or 64 rows and two tiles at a time.
+// tile, or 64 rows and two tiles at a time. Tiles that see most keys go first: a sequence's last, or
+// on grids of a few rounds those of all sequences, sorted by each workgroup for itself. 2-byte rows
+// go to LDS by DMA (8 sequences of 17 to 512 new tokens, 32 heads over 8, D = 128, window 2048:
+// 138.5 us through registers, 119 so).
 //
 // Where tiles of rows are few, a sequence's keys are dealt to several workgroups (splits of
 // split_tiles tiles), which leave unnormalised fp32 outputs with their maxima and sums;
@@ -37,13 +40,19 @@ struct RowTile {
 
   template <int ROWS, typename P> __device__ __forceinline__ static RowTile at(const P& p, int slot) {
     const CacheShape& c = p.at;
+    const int group = p.heads / c.kv_heads;
+    auto first_slot = [&](int b) { return (int)((long)packed_begin(c, b) * group / ROWS) + b; };
+    const int b = c.offsets ? last_at_or_before(c.batch, slot, first_slot) : slot / p_slots<ROWS>(group);
+    return of<ROWS>(p, b, c.offsets ? slot - first_slot(b) : slot % p_slots<ROWS>(group));
+  }
+  // Tile `tile` of sequence b.
+  template <int ROWS, typename P> __device__ __forceinline__ static RowTile of(const P& p, int b, int tile) {
+    const CacheShape& c = p.at;
     RowTile t;
     t.group = p.heads / c.kv_heads;
-    auto first_slot = [&](int b) { return (int)((long)packed_begin(c, b) * t.group / ROWS) + b; };
-    t.b = c.offsets ? last_at_or_before(c.batch, slot, first_slot) : slot / p_slots<ROWS>(t.group);
+    t.b = b;
     t.begin = packed_begin(c, t.b);
     const int count = c.offsets ? max(0, packed_begin(c, t.b + 1) - t.begin) : 1;
-    const int tile = c.offsets ? slot - first_slot(t.b) : slot % p_slots<ROWS>(t.group);
     // (long: a wrong slot's tile times ROWS)
     const long left = (long)count * t.group - (long)tile * ROWS;
     t.row0 = tile * ROWS;
@@ -296,8 +305,8 @@ paged_token_kernel(PagedParams<T, C> p) {
 
 // Waves that share a tile of keys, 32 rows each: RW of four; the 4 / RW groups of them take
 // every (4 / RW)-th tile and join at the end.
-// (128 rows at D = 128: three waves per SIMD, 168 registers and one of them spilled outside the
-// loop, 158 -> 142 us for 8 sequences with 17 to 512 new tokens of 32 heads over 8, window 2048.)
+// (128 rows at D = 128: three waves per SIMD, 168 registers and a few of them spilled outside the
+// loop, 156 -> 120 us for those 8 sequences.)
 template <typename T, typename C, int D, int RW>
 __global__ void __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 64 || RW == 4 ? 3 : 2)))
@@ -317,10 +326,17 @@ paged_chunk_kernel(PagedParams<T, C> p) {
   const int rw = wave % RW, kw = wave / RW;
   const int thread = threadIdx.x % (64 * RW);  // of its group
   const int n = lane & 31, g = lane >> 5;
-  // (backwards: a sequence's last rows, which see most, first)
+  // (backwards: a sequence's last rows first)
   const int hk = blockIdx.x % p.at.kv_heads, slot = p.slots - 1 - (int)blockIdx.x / p.at.kv_heads, split = blockIdx.y;
   clear_rest<D>(p, blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y, 256);
-  const RowTile rt = RowTile::template at<ROWS>(p, slot);
+  RowTile rt;
+  if (p.longest_first) {
+    int seq, tile;
+    if (!longest_first<ROWS>(p.at, p.heads / p.at.kv_heads, p.slots - 1 - slot, lane, seq, tile)) return;
+    rt = RowTile::template of<ROWS>(p, seq, tile);
+  } else {
+    rt = RowTile::template at<ROWS>(p, slot);
+  }
   if (rt.rows <= 0) return;
   const int first_pos = __builtin_amdgcn_readfirstlane(rt.position(0));
   const int last_pos = __builtin_amdgcn_readfirstlane(rt.position(rt.rows - 1));

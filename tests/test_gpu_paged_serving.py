@@ -347,3 +347,23 @@ def test_long_chunks(D, dtype, new, kv_heads, cuda_device):
     out = flash_hog.paged_attention(q, *cache, table, **kwargs)
     first = max(0, page * (pages - 3) - (length - new))
     assert bool(torch.isnan(out[first:]).all())
+
+
+@pytest.mark.parametrize("batch", [2, 63, 64, 65])
+@pytest.mark.parametrize("quantised", [False, True], ids=["plain", "e4m3"])
+def test_sorted_tiles(batch, quantised, cuda_device):
+    """Chunks whose tiles are taken longest first (up to 64 sequences) and by sequence (65): empty
+    ones among them, equal lengths, fewer keys than new tokens, several tiles with the same keys."""
+    import flash_hog
+
+    print("[case] sorted", batch, quantised, flush=True)
+    new = [(0, 1, 150, 40, 40, 3)[i % 6] + (i % 7 == 3) for i in range(batch)]
+    lengths = [max(n - 2, 0) if i % 5 == 4 else n + 30 * (i % 3) for i, n in enumerate(new)]
+    lengths[-1], new[-1] = 200, 170
+    for heads, kv_heads, head_dim in ((2, 2, 64), (200, 1, 64), (6, 2, 128)):
+        if heads == 200 and batch > 2:
+            continue
+        case = (heads, kv_heads, head_dim, BF16, quantised, 16, lengths, new, 0, 0)
+        cache, counts, q, kwargs = make(case, cuda_device, seed=batch)
+        out = flash_hog.paged_attention(q.to(cuda_device), **kwargs)
+        check(out, ref.attention(q, cache, counts, 0, 0, q.shape[-1] ** -0.5), str(batch))

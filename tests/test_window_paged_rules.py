@@ -23,7 +23,7 @@ void chunks(int nq, int nk, int coff, int window, int sinks, int row_bytes, int 
 void plan(int batch, int total, int single, int heads, int kv_heads, int d, long capacity, int window, int sinks, int cus,
           long* out) {
   const fhog::PagedPlan p = fhog::paged_plan(batch, total, single, heads, kv_heads, d, capacity, window, sinks, cus);
-  out[0] = p.rows, out[1] = p.slots, out[2] = p.splits, out[3] = p.split_tiles, out[4] = p.parts;
+  out[0] = p.rows, out[1] = p.slots, out[2] = p.splits, out[3] = p.split_tiles, out[4] = p.parts, out[5] = p.longest_first;
 }
 }
 """
@@ -50,9 +50,9 @@ def sink_chunks(lib, *args):
 
 
 def plan(lib, *args):
-    out = (ctypes.c_long * 5)()
+    out = (ctypes.c_long * 6)()
     lib.plan(*args, out)
-    return dict(zip(("rows", "slots", "splits", "split_tiles", "parts"), out))
+    return dict(zip(("rows", "slots", "splits", "split_tiles", "parts", "longest_first"), out))
 
 
 def test_sink_chunks_cover_the_queries(rules):
@@ -109,6 +109,8 @@ def test_tiles_cover_rows_and_splits_cover_keys(rules, cus):
         p = plan(rules, batch, total, single, group * kv, kv, rng.choice([64, 128, 256]), capacity, window, sinks, cus)
         rows = p["rows"]
         assert p["splits"] >= 1 and p["splits"] * rows <= 2048 and p["split_tiles"] >= 1
+        if p["longest_first"]:  # one lane a sequence, no splits, nothing that cuts keys off
+            assert rows > 16 and 1 < batch <= 64 and p["splits"] == 1 and window == 0
         assert p["parts"] == (p["slots"] * kv * p["splits"] * rows if p["splits"] > 1 else 0)
         begin, seen = 0, 0
         for b, count in enumerate(counts):
