@@ -391,6 +391,12 @@ struct Cache {
   const int* offsets_ptr() const { return offsets.defined() ? offsets.data_ptr<int>() : nullptr; }
 };
 
+// Tells autograd that a tensor was written to: a graph that saved it before then raises in its
+// backward. (Inference tensors, which no graph can save, have no version.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int rows_of(const char* name, const at::Tensor& t) {
   if (t.dim() != 3) value_error(std::string("expected a (T, N, H) ") + name + ", got " + shape_str(t));
   for (int64_t s : t.sizes())
@@ -425,6 +431,7 @@ at::Tensor paged_attention_core(const at::Tensor& q_, const at::Tensor& k_cache,
                                      out.data_ptr(), data_or_null(ws), size, c.batch, total, heads, c.kv_heads,
                                      c.head_dim, c.pages, c.page, c.width, dt, c.dtype, window, sinks, given == nullptr,
                                      (float)scale));
+  if (given) written(out);
   return out;
 }
 
@@ -444,6 +451,8 @@ void cache_write_core(const at::Tensor& k_, const at::Tensor& v_, const at::Tens
                                  v_cache.data_ptr(), const_cast<void*>(ptr(c.k_scale)),
                                  const_cast<void*>(ptr(c.v_scale)), c.table_ptr(), c.lengths_ptr(), c.offsets_ptr(),
                                  c.batch, total, c.kv_heads, c.head_dim, c.pages, c.page, c.width, dt, c.dtype));
+  for (const at::Tensor* t : {&k_cache, &v_cache, c.k_scale, c.v_scale})
+    if (t) written(*t);
 }
 
 std::tuple<at::Tensor, at::Tensor> cache_read_core(const at::Tensor& k_cache, const at::Tensor& v_cache,

@@ -412,6 +412,12 @@ def _check_cache(first, k_cache, v_cache, page_table, lengths, query_offsets, k_
     return (*k_cache.shape, batch, page_table.shape[1]), page_table, lengths, query_offsets
 
 
+def _written(*tensors):
+    """Tells autograd that tensors were written to: a graph that saved one before then raises in its
+    backward. (Inference tensors, which no graph can save, have no version.)"""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])
+
+
 def paged_attention(q, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, window: int,
                     sinks: int, scale: float, out=None):
     """out (T, N, H) of the packed new tokens q over a paged cache (fhog_paged_attention); window 0: none."""
@@ -445,6 +451,8 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, query_offsets, k_s
             _stream(q.device), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(page_table),
             _ptr(lengths), _ptr(query_offsets), _ptr(out), _ptr(ws), size, B, T, N, Nk, Hd, pages, page, width,
             DTYPE_CODES[q.dtype], CACHE_DTYPE_CODES[k_cache.dtype], window, sinks, int(clear), float(scale)))
+    if not clear:
+        _written(out)
     return out
 
 
@@ -470,6 +478,7 @@ def paged_cache_write(k, v, k_cache, v_cache, page_table, lengths, query_offsets
             _stream(k.device), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
             _ptr(page_table), _ptr(lengths), _ptr(query_offsets), B, k.shape[0], Nk, Hd, pages, page, width,
             DTYPE_CODES[k.dtype], CACHE_DTYPE_CODES[k_cache.dtype]))
+    _written(k_cache, v_cache, k_scale, v_scale)
 
 
 def paged_cache_read(k_cache, v_cache, page_table, lengths, max_length: int, dtype, k_scale, v_scale):
