@@ -44,6 +44,7 @@ Tensor = torch.Tensor
 
 
 def _refuse_gradients(name, *tensors):
+    tensors = [t for t in tensors if t is not None]
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
@@ -100,7 +101,7 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_of
     out: a contiguous tensor for the result; its rows of no sequence (from query_offsets[batch]
     on, a padded batch) are left as they were. Without it they are zero.
     """
-    _refuse_gradients("paged_attention", query, key_cache, value_cache)
+    _refuse_gradients("paged_attention", query, key_cache, value_cache, key_scale, value_scale, out)
     if window is None:
         if sinks != 0:
             raise ValueError(f"sinks needs a window, got sinks={sinks}")
@@ -128,7 +129,7 @@ def paged_cache_write(key, value, key_cache, value_cache, page_table, lengths, q
     round beyond it, and then reads as infinite. Rows of no sequence and tokens at
     positions below zero (a sequence of length zero) are not written. No two tokens may name the
     same place: pages that sequences share are read-only."""
-    _refuse_gradients("paged_cache_write", key, value, key_cache, value_cache)
+    _refuse_gradients("paged_cache_write", key, value, key_cache, value_cache, key_scale, value_scale)
     call = paged_cache_write_op if torch.compiler.is_compiling() else _hip.paged_cache_write
     call(key, value, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale)
 
@@ -138,7 +139,7 @@ def paged_cache_read(key_cache, value_cache, page_table, lengths, *, max_length:
     """The first max_length tokens (default: what the table can hold) of the sequences as dense
     keys and values (batch, max_length, N_kv, H), zeros behind a sequence's length. dtype is the
     cache's, or for an e4m3 cache bfloat16 (default) or float16, to which its values are rounded."""
-    _refuse_gradients("paged_cache_read", key_cache, value_cache)
+    _refuse_gradients("paged_cache_read", key_cache, value_cache, key_scale, value_scale)
     if dtype is None:
         dtype = torch.bfloat16 if key_cache.dtype == torch.float8_e4m3fn else key_cache.dtype
     if max_length is None:
