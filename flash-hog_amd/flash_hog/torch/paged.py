@@ -36,6 +36,7 @@ from __future__ import annotations
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from flash_hog import _hip
 from flash_hog.torch._hip_gpu import _default_scale
@@ -50,6 +51,11 @@ def _refuse_gradients(name, *tensors):
             if t.requires_grad:
                 raise RuntimeError(f"{name} has no derivative: call it under torch.no_grad() (training attends through "
                                    "flash_hog.dot_product_attention)")
+    # A forward-mode dual tensor does not require a gradient, in grad mode or out of it.
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no derivative, in forward mode either: call it on tensors without a tangent")
 
 
 @torch.library.custom_op("flash_hog::paged_attention", mutates_args=())
