@@ -44,18 +44,35 @@ from flash_hog.torch._hip_gpu import _default_scale
 Tensor = torch.Tensor
 
 
-def _refuse_gradients(name, *tensors):
-    tensors = [t for t in tensors if t is not None]
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise RuntimeError(f"{name} has no derivative: call it under torch.no_grad() (training attends through "
-                                   "flash_hog.dot_product_attention)")
+_PLAIN = Tensor.__torch_dispatch__
+
+
+def _checked(name, index, *tensors) -> bool:
+    """Refuses tensors that carry a derivative or that vmap maps over. Returns whether the call goes
+    through its operator, because it is traced or because some tensor has no memory of its own to
+    point at (fake tensors, the wrappers of torch.func transforms); plain ones go straight to the C ABI.
+    index: the tensors that find tokens, which carry no derivative."""
+    through = torch.compiler.is_compiling()
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            continue
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{name} has no derivative: call it under torch.no_grad() (training attends through "
+                               "flash_hog.dot_product_attention)")
+        if type(t) is not Tensor and getattr(type(t), "__torch_dispatch__", _PLAIN) is not _PLAIN:
+            through = True
     # A forward-mode dual tensor does not require a gradient, in grad mode or out of it.
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
-        for t in tensors:
-            if forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{name} has no derivative, in forward mode either: call it on tensors without a tangent")
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError(f"{name} has no derivative, in forward mode either: call it on tensors without a tangent")
+    if torch._C._are_functorch_transforms_active():
+        ours = [t for t in (*tensors, *index) if isinstance(t, Tensor)]
+        if any(map(torch._C._functorch.is_batchedtensor, ours)):
+            raise RuntimeError(f"{name} has no batching rule, so torch.func.vmap cannot map it: its sequences are a batch "
+                               "already")
+        through = through or any(map(torch._C._functorch.is_functorch_wrapped_tensor, ours))
+    return through
 
 
 @torch.library.custom_op("flash_hog::paged_attention", mutates_args=())
@@ -107,7 +124,8 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_of
     out: a contiguous tensor for the result; its rows of no sequence (from query_offsets[batch]
     on, a padded batch) are left as they were. Without it they are zero.
     """
-    _refuse_gradients("paged_attention", query, key_cache, value_cache, key_scale, value_scale, out)
+    through = _checked("paged_attention", (page_table, lengths, query_offsets), query, key_cache, value_cache, key_scale,
+                       value_scale, out)
     if window is None:
         if sinks != 0:
             raise ValueError(f"sinks needs a window, got sinks={sinks}")
@@ -119,10 +137,10 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_of
     scale = _default_scale(query, scale)
     args = (query, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale, window, sinks,
             scale)
-    if torch.compiler.is_compiling():
+    if through:
         if out is None:
             return paged_attention_op(*args)
-        raise ValueError("out is not supported under torch.compile")
+        raise ValueError("out is not supported under torch.compile, transforms or fake tensors")
     return _hip.paged_attention(*args, out=out)
 
 
@@ -135,8 +153,9 @@ def paged_cache_write(key, value, key_cache, value_cache, page_table, lengths, q
     round beyond it, and then reads as infinite. Rows of no sequence and tokens at
     positions below zero (a sequence of length zero) are not written. No two tokens may name the
     same place: pages that sequences share are read-only."""
-    _refuse_gradients("paged_cache_write", key, value, key_cache, value_cache, key_scale, value_scale)
-    call = paged_cache_write_op if torch.compiler.is_compiling() else _hip.paged_cache_write
+    through = _checked("paged_cache_write", (page_table, lengths, query_offsets), key, value, key_cache, value_cache,
+                       key_scale, value_scale)
+    call = paged_cache_write_op if through else _hip.paged_cache_write
     call(key, value, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale)
 
 
@@ -145,7 +164,7 @@ def paged_cache_read(key_cache, value_cache, page_table, lengths, *, max_length:
     """The first max_length tokens (default: what the table can hold) of the sequences as dense
     keys and values (batch, max_length, N_kv, H), zeros behind a sequence's length. dtype is the
     cache's, or for an e4m3 cache bfloat16 (default) or float16, to which its values are rounded."""
-    _refuse_gradients("paged_cache_read", key_cache, value_cache, key_scale, value_scale)
+    through = _checked("paged_cache_read", (page_table, lengths), key_cache, value_cache, key_scale, value_scale)
     if dtype is None:
         dtype = torch.bfloat16 if key_cache.dtype == torch.float8_e4m3fn else key_cache.dtype
     if max_length is None:
@@ -153,5 +172,5 @@ def paged_cache_read(key_cache, value_cache, page_table, lengths, *, max_length:
             raise ValueError("expected a (batch, pages) page_table and a (pages, kv_heads, page_size, head_dim) cache, "
                              f"got {tuple(page_table.shape)} and {tuple(key_cache.shape)}")
         max_length = page_table.shape[1] * key_cache.shape[2]
-    call = paged_cache_read_op if torch.compiler.is_compiling() else _hip.paged_cache_read
+    call = paged_cache_read_op if through else _hip.paged_cache_read
     return call(key_cache, value_cache, page_table, lengths, max_length, dtype, key_scale, value_scale)

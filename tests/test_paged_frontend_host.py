@@ -1,10 +1,11 @@
-"""The paged cache's operators under autograd, without a GPU: forward-mode derivatives, and tensors that
-are written to or scale what is read while they require a gradient."""
+"""The paged cache's operators under torch's transforms, without a GPU: forward-mode derivatives,
+vmap, fake tensors, and tensors that are written to while they require a gradient."""
 
 from __future__ import annotations
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
 import flash_hog
@@ -69,3 +70,44 @@ def test_written_tensors_that_require_a_gradient_are_refused():
                 call()
         with torch.no_grad(), pytest.raises(ValueError, match="must be on a GPU device"):
             flash_hog.paged_attention(q, **changed)
+
+
+def test_vmap_is_refused():
+    x, q, k = cache(), rows(4), rows(2)
+    two = lambda t: torch.stack([t, t])
+    for call in (lambda: torch.func.vmap(lambda t: flash_hog.paged_attention(t, **x))(two(q)),
+                 lambda: torch.func.vmap(lambda t: flash_hog.paged_attention(q, **{**x, "lengths": t}))(two(x["lengths"])),
+                 lambda: torch.func.vmap(lambda t: flash_hog.paged_cache_write(t, t, **x))(two(k)),
+                 lambda: torch.func.vmap(lambda t: flash_hog.paged_cache_read(**{**x, "key_cache": t}))(two(x["key_cache"]))):
+        with pytest.raises(RuntimeError, match="vmap"):
+            call()
+
+
+@pytest.mark.parametrize("kind", [BF16, E4M3], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("device", ["cuda", "cpu"])
+def test_fake_tensors(device, kind):
+    """Shapes and types of all three outside of torch.compile, as dot_product_attention gives them."""
+    with FakeTensorMode():
+        x, q, k = cache(kind, device), rows(4, device), rows(2, device)
+        out = flash_hog.paged_attention(q, **x, window=9, sinks=1)
+        assert out.shape == q.shape and out.dtype == BF16 and out.device == q.device
+        assert flash_hog.paged_cache_write(k, k, **x) is None
+        for t in flash_hog.paged_cache_read(**x, dtype=BF16):
+            assert t.shape == (3, 32, 2, 64) and t.dtype == BF16
+        with pytest.raises(ValueError, match="out is not supported"):
+            flash_hog.paged_attention(q, **x, out=torch.empty_like(q))
+
+
+def test_tensors_made_under_a_transform():
+    """A tensor that torch.func.grad wraps without differentiating it reaches the operators."""
+    x, k = cache(device="meta"), rows(2, "meta")
+
+    def loss(w):
+        q = torch.zeros(3, 4, 64, dtype=BF16, device="meta")
+        flash_hog.paged_cache_write(k * 1, k, **x)
+        out = flash_hog.paged_attention(q, **x)
+        assert out.shape == q.shape
+        return (w * out.detach().float()).sum()
+
+    w = torch.zeros(3, 4, 64, device="meta")
+    assert torch.func.grad(loss)(w).shape == w.shape
