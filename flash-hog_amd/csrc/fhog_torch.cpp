@@ -397,6 +397,14 @@ void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Refuses an out whose memory a contiguous tensor that the kernels read shares; `same`: but for all
+// of it, row by row.
+void check_apart(const at::Tensor& out, const char* name, const at::Tensor& t, bool same) {
+  const char *a = (const char*)out.data_ptr(), *b = (const char*)t.data_ptr();
+  if (a < b + t.nbytes() && b < a + out.nbytes() && !(same && a == b))
+    value_error(std::string("out overlaps ") + name);
+}
+
 int rows_of(const char* name, const at::Tensor& t) {
   if (t.dim() != 3) value_error(std::string("expected a (T, N, H) ") + name + ", got " + shape_str(t));
   for (int64_t s : t.sizes())
@@ -421,6 +429,11 @@ at::Tensor paged_attention_core(const at::Tensor& q_, const at::Tensor& k_cache,
   }
   at::Tensor out = given ? *given : at::empty(q_.sizes(), q_.options());
   const at::Tensor q = contig(q_);
+  if (given) {
+    check_apart(out, "query", q, true);
+    check_apart(out, "key_cache", k_cache, false);
+    check_apart(out, "value_cache", v_cache, false);
+  }
   const int heads = (int)q.size(1);
   c10::DeviceGuard guard(q.device());
   const size_t size = api().paged_bytes(c.batch, total, !c.offsets.defined(), heads, c.kv_heads, c.head_dim, c.page,

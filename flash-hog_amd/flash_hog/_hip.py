@@ -412,6 +412,14 @@ def _check_cache(first, k_cache, v_cache, page_table, lengths, query_offsets, k_
     return (*k_cache.shape, batch, page_table.shape[1]), page_table, lengths, query_offsets
 
 
+def _check_apart(out, name, t, same=False):
+    """Refuses an out whose memory a contiguous tensor that the kernels read shares; same: but for all
+    of it, row by row."""
+    a, b = out.data_ptr(), t.data_ptr()
+    if a < b + t.nbytes and b < a + out.nbytes and not (same and a == b):
+        raise ValueError(f"out overlaps {name}")
+
+
 def _written(*tensors):
     """Tells autograd that tensors were written to: a graph that saved one before then raises in its
     backward. (Inference tensors, which no graph can save, have no version.)"""
@@ -444,6 +452,10 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, query_offsets, k_s
         if not out.is_contiguous():
             raise ValueError("out must be contiguous")
     q = q.contiguous()
+    if not clear:
+        _check_apart(out, "query", q, same=True)
+        _check_apart(out, "key_cache", k_cache)
+        _check_apart(out, "value_cache", v_cache)
     with _on_device(q.device):
         size = lib().fhog_paged_workspace_bytes(B, T, int(query_offsets is None), N, Nk, Hd, page, width, window, sinks)
         ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None

@@ -122,7 +122,8 @@ def paged_attention(query, key_cache, value_cache, page_table, lengths, query_of
     defaults to H ** -0.5.
 
     out: a contiguous tensor for the result; its rows of no sequence (from query_offsets[batch]
-    on, a padded batch) are left as they were. Without it they are zero.
+    on, a padded batch) are left as they were. Without it they are zero. It may be query itself, and
+    overlaps neither query otherwise nor the caches.
     """
     through = _checked("paged_attention", (page_table, lengths, query_offsets), query, key_cache, value_cache, key_scale,
                        value_scale, out)
