@@ -467,12 +467,13 @@ struct PagedPlan {
   bool longest_first;  // whether paged_chunk_kernel sorts its tiles by their keys
 };
 constexpr int kJoinWeights = 2048;  // the most rows of a tile times splits
-// us, H32/8 D128, with the chosen number and those on both sides of it:
-//  - wide tiles of 128 rows from two a CU on, of 64 below (64 everywhere / two): B8 x 512 tokens
-//    window 2048 159.7 / 136.8, N8192 e4m3 780 / 620; (one / two) B32 x 64 tokens of H16/4 D64 103 / 68;
+// us, H32/8 D128 bf16 unless named, with the chosen number and those on both sides of it:
+//  - wide tiles of 128 rows from two a CU on, of 64 below (64 everywhere / two): B8 x 17 to 512 tokens
+//    window 2048 142 / 118, N8192 e4m3 760 / 616; (one / two) B32 x 64 tokens after up to 4032 of H16/4 D64
+//    96 / 65, 4096 of 16384 tokens H12 D64 e4m3 312 / 301;
 //  - their splits fill the CUs with as many workgroups as live there together, two, at D = 256 one
-//    (1 / 2 / 4 a CU): 512 tokens after 7680 152 / 127 / 130, 64 after 32704 e4m3 143 / 97 / 112, D256
-//    B2 x 1024 after 7168 H8 348 / 386 / 411;
+//    (1 / 2 / 4 a CU): 512 tokens after 7680 140 / 115 / 118, 64 after 32704 e4m3 141 / 97 / 111, D256
+//    B2 x 1024 after 7168 H8 275 / 313 / 335; but B32 x 64 of H16/4 D64 57 / 65 / 69;
 //  - splits of single tokens fill them with eight (4 / 8 / 16): B16 over 32768 keys e4m3 136 / 126 / 143,
 //    bf16 229 / 215 / 221, B64 over 4096 e4m3 67.4 / 67.6 / 67.4.
 constexpr long kWideTiles = 2, kTokenWorkgroups = 8;
@@ -484,7 +485,10 @@ inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv
   auto slots = [&](int rows) {
     return single ? (long)batch * ((group + rows - 1) / rows) : (long)total * group / rows + batch;
   };
-  // More than 16 rows a sequence on average (tokens times heads of a group): the wide tiles.
+  // More than 16 rows a sequence on average (tokens times heads of a group): the wide tiles, for
+  // all sequences of the call. A single token of a long sequence beside a prompt thus has one
+  // workgroup a key/value head for all its keys: a prompt of 2048 69 us, a token of 32768 38, both in one
+  // call 888.
   p.rows = (long)total * group <= 16l * batch ? 16 : slots(128) * kv_heads >= kWideTiles * cus ? 128 : 64;
   p.slots = (int)slots(p.rows);
   // The most tiles that a tile of rows reads: with a window its keys, those between the tile's
@@ -494,6 +498,9 @@ inline PagedPlan paged_plan(int batch, int total, bool single, int heads, int kv
     const long most = (long)window + p.rows / group + 1 + sinks;
     if (most < keys) keys = most;
   }
+  // (capacity, not the lengths, which the host does not know: a table wider than its sequences
+  // need gives longer and fewer splits. H32/8 D128, tables 1 / 4 / 32 times as wide: one token of 4096
+  // 13.5 / 13.6 / 19.9, 16 of 32768 366 / 363 / 382, 64 tokens of 8192 52 / 68 / 157, 512 114 / 159 / 158.)
   const long tiles = (keys + 31) / 32 + 2;
   const long blocks = (long)p.slots * kv_heads;
   p.waves = head_dim == 64 ? 8 : head_dim == 128 ? 4 : 2;

@@ -8,6 +8,10 @@
 // sinks: the queries that see one behind their window (SinkGrid) meet 32 keys or fewer, so
 // that in a key-tiled workgroup all waves but one would idle.
 //
+// Sums and statistics are fp32; probabilities and score gradients enter the products over keys or
+// queries in T, one rounding of half a step a term, as in the other kernels (the matrix instructions take both
+// operands in it): for 2-byte types outputs are 1.2 to 1.5 times as far from 64 bits as with fp32 ones.
+//
 // 256-byte rows at most (2-byte types at D = 64 and 128, fp32 at 64). A wave's ring has two stages
 // where they leave room for two workgroups on a CU, and where registers allow one anyway; else one
 // stage and two workgroups, which hide each other's loads: causal N1000 window 256, H8 fp32 (256

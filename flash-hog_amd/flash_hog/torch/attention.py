@@ -101,7 +101,9 @@ def dot_product_attention(query, key, value, is_causal: bool = False, scale: flo
     window: a query at position p (t, or t + S - T with "bottom_right") sees the `window`
     keys p - window < s <= p, itself among them, and besides these the first `sinks` keys
     (s < sinks, s <= p). Work grows with T * window, memory with T + S, in all three
-    derivatives. A query that sees no key gives zeros.
+    derivatives. A query that sees no key gives zeros. Keys come in tiles of 32: a NaN or an infinity in
+    a value (in the derivatives: or in a key) reaches every query whose window or sinks share its tile,
+    seen or not.
 
     Like the reference's kernel, any head dim H >= 1 works up to the largest
     one the kernels take (256 for bf16 and fp16, 128 for fp32); head dims the

@@ -29,6 +29,15 @@ that depend on it at least (paged_cache_write leaves such a token out), and no a
 tensor. Entries and cache
 slots that no visible token needs may hold anything, NaN included. Among the keys of one 32-key
 tile, though, a NaN or infinity in a value that one token sees also reaches the rows beside it.
+
+The functions have no derivative: tensors that require a gradient (in grad mode) or carry a tangent are
+refused, and so are ones that torch.func.vmap maps over. What they write to gets a new autograd version.
+
+For speed: how a sequence's keys are split over workgroups follows from the table's width, since no
+length is read back, and how rows are tiled from the average number of new tokens. So give short chunks
+a table not much wider than they need (64 tokens of 8192 take three times as long with one 32 times as wide;
+single tokens hardly lose), and give prompts and single tokens on long contexts a call each (a prompt
+of 2048 and a token of 32768, 32 heads over 8 of 128: 69 and 38 us, in one call 888).
 """
 
 from __future__ import annotations
