@@ -162,7 +162,8 @@ def paged_cache_write(key, value, key_cache, value_cache, page_table, lengths, q
     to nearest even, and infinities become NaN; a value within 1/32 of the type's largest may
     round beyond it, and then reads as infinite. Rows of no sequence and tokens at
     positions below zero (a sequence of length zero) are not written. No two tokens may name the
-    same place: pages that sequences share are read-only."""
+    same place: pages that sequences share are read-only. key and value may lie in the cache too, but not
+    where this call writes."""
     through = _checked("paged_cache_write", (page_table, lengths, query_offsets), key, value, key_cache, value_cache,
                        key_scale, value_scale)
     call = paged_cache_write_op if through else _hip.paged_cache_write
