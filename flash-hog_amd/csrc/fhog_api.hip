@@ -14,6 +14,7 @@
 #include "flash_hog.h"
 #include "fhog_params.h"
 #include "fhog_paged.h"
+#include "fhog_rotary.h"
 
 namespace {
 
@@ -586,6 +587,196 @@ int fhog_paged_cache_read(fhog_stream_t stream, const void* k_cache, const void*
     return fhog::launch_cache_read<T, C, D>(p, (hipStream_t)stream);
   };
   return launch_status(dispatch_paged(s, run), who);
+}
+
+}  // extern "C"
+
+namespace {
+
+int check_rotary(const char* who, const fhog_rotary* s) {
+  if (s == nullptr) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: shape is null", who);
+  if (s->batch < 0 || s->tokens < 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sizes must not be negative", who);
+  if (s->heads < 1 || s->kv_heads < 1)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: sizes must be >= 1 (heads=%d kv_heads=%d)", who, s->heads, s->kv_heads);
+  if (s->dtype != FHOG_DTYPE_F32 && s->dtype != FHOG_DTYPE_F16 && s->dtype != FHOG_DTYPE_BF16)
+    return fail(FHOG_ERR_UNSUPPORTED, "%s: dtype must be bf16, fp16 or fp32, got %d", who, s->dtype);
+  if (s->weight_dtype != s->dtype && s->weight_dtype != FHOG_DTYPE_F32)
+    return fail(FHOG_ERR_UNSUPPORTED, "%s: weights must be of dtype %d or fp32, got %d", who, s->dtype, s->weight_dtype);
+  if (s->head_dim < 1 || s->head_dim > 256)
+    return fail(FHOG_ERR_UNSUPPORTED, "%s: head_dim must be 1 to 256, got %d", who, s->head_dim);
+  if (s->rotated < 0 || s->rotated > s->head_dim || s->rotated % 2 != 0)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: rotated must be even, 0 to head_dim, got %d", who, s->rotated);
+  if (s->norm && !(s->eps >= 0.0f && s->eps - s->eps == 0.0f))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: eps must be finite and >= 0", who);
+  if (s->rotated > 0 && !aligned(s->frequencies, 4))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: frequencies is null or not 4-byte aligned", who);
+  if (s->positions != nullptr) {
+    if (s->lengths != nullptr) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: positions and lengths exclude each other", who);
+    if ((s->position_bytes != 4 && s->position_bytes != 8) || !aligned(s->positions, s->position_bytes))
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: positions must be aligned elements of 4 or 8 bytes", who);
+    if (s->position_rows != 1 && s->position_rows != s->batch)
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: positions must have 1 or batch rows, got %d", who, s->position_rows);
+  }
+  if (s->lengths != nullptr) {
+    if (!aligned(s->lengths, 4) || (s->query_offsets != nullptr && !aligned(s->query_offsets, 4)))
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: lengths and query_offsets must be 4-byte aligned", who);
+    if (s->batch != 1) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: packed tokens have batch 1, got %d", who, s->batch);
+    if (s->tokens > 0 && s->sequences < 1)
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: rows without a sequence", who);
+    if (s->query_offsets == nullptr && s->sequences != s->tokens)
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: without query_offsets there is one row a sequence: %d rows, %d sequences",
+                  who, s->tokens, s->sequences);
+  } else if (s->query_offsets != nullptr) {
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: query_offsets needs lengths", who);
+  }
+  const double tokens = (double)s->batch * s->tokens;
+  if (tokens >= (1ll << 40) || tokens * (s->heads > s->kv_heads ? s->heads : s->kv_heads) * s->head_dim >= kMostElements ||
+      s->heads >= (1 << 24) || s->kv_heads >= (1 << 24))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  return FHOG_OK;
+}
+
+fhog::RotaryShape rotary_shape(const fhog_rotary& s) {
+  return fhog::RotaryShape{s.batch, s.tokens, {s.heads, s.kv_heads}, s.head_dim, s.rotated, s.interleaved != 0,
+                           s.norm != 0, s.weight_dtype == FHOG_DTYPE_F32 && s.dtype != FHOG_DTYPE_F32, s.eps,
+                           s.frequencies, s.positions, s.position_bytes, s.position_rows, s.lengths, s.query_offsets,
+                           s.sequences};
+}
+void rotary_strides(const fhog_rotary& s, fhog::RowStrides out[2]) {
+  out[0] = {(long)s.q_stride[0], (long)s.q_stride[1], (long)s.q_stride[2]};
+  out[1] = {(long)s.k_stride[0], (long)s.k_stride[1], (long)s.k_stride[2]};
+}
+// Whether rows can be read in 16-byte pieces of which each holds whole pairs: `rows` are the tensors, of which
+// the first `strided` have q's and k's strides.
+bool rotary_wide(const fhog_rotary& s, bool strided, std::initializer_list<const void*> rows) {
+  const long long each = s.dtype == FHOG_DTYPE_F32 ? 4 : 8;
+  if (s.head_dim % 16 != 0 || s.rotated % 16 != 0) return false;
+  for (const void* p : rows)
+    if (p != nullptr && !aligned(p, 16)) return false;
+  for (int i = 0; strided && i < 3; ++i)
+    if (s.q_stride[i] % each != 0 || s.k_stride[i] % each != 0) return false;
+  return true;
+}
+template <typename F> hipError_t dispatch_rows(int dtype, F&& f) {
+  if (dtype == FHOG_DTYPE_BF16) return f.template operator()<__bf16>();
+  if (dtype == FHOG_DTYPE_F16) return f.template operator()<_Float16>();
+  return f.template operator()<float>();
+}
+int check_rows(const char* who, const fhog_rotary& s, std::initializer_list<std::pair<const char*, const void*>> rows) {
+  const uintptr_t item = s.dtype == FHOG_DTYPE_F32 ? 4 : 2;
+  for (const auto& p : rows)
+    if (!aligned(p.second, item))
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: %s is null or not aligned to its elements", who, p.first);
+  return FHOG_OK;
+}
+// The weights, and what stands or falls with them.
+int check_weights(const char* who, const fhog_rotary& s, const void* q_weight, const void* k_weight,
+                  std::initializer_list<std::pair<const void*, const void*>> more) {
+  const uintptr_t item = s.weight_dtype == FHOG_DTYPE_F32 ? 4 : 2;
+  auto good = [&](const void* p) { return p == nullptr || aligned(p, item); };
+  if (!s.norm && (q_weight != nullptr || k_weight != nullptr))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: weights need norms", who);
+  if (!good(q_weight) || !good(k_weight))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: a weight is not aligned to its elements", who);
+  for (const auto& p : more) {
+    if ((p.first != nullptr) != (q_weight != nullptr) || (p.second != nullptr) != (k_weight != nullptr))
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: a weight's derivative is null where the weight is not, or the reverse", who);
+    if (!good(p.first) || !good(p.second))
+      return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: a weight's derivative is not aligned to its elements", who);
+  }
+  return FHOG_OK;
+}
+// Clears the weights' gradients of a call without rows.
+int clear_weights(const char* who, const fhog_rotary& s, void* const out[2], hipStream_t stream) {
+  return launch_status(dispatch_rows(s.dtype, [&]<typename T>() {
+    return fhog::sum_rotary_weights<T>(nullptr, out, rotary_shape(s), 0, stream);
+  }), who);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fhog_qk_norm_rotary_workspace_bytes(const fhog_rotary* shape) {
+  if (check_rotary("fhog_qk_norm_rotary_workspace_bytes", shape) || !shape->norm) return 0;
+  const long tokens = (long)shape->batch * shape->tokens;
+  return (size_t)2 * fhog::rotary_grid(tokens, compute_units()).groups * shape->head_dim * sizeof(float);
+}
+
+int fhog_qk_norm_rotary_fwd(fhog_stream_t stream, const fhog_rotary* shape, const void* q, const void* k,
+                            const void* q_weight, const void* k_weight, void* q_out, void* k_out) {
+  static const char* who = "fhog_qk_norm_rotary_fwd";
+  if (int st = check_rotary(who, shape)) return st;
+  const fhog_rotary& s = *shape;
+  if (int st = check_weights(who, s, q_weight, k_weight, {})) return st;
+  const long tokens = (long)s.batch * s.tokens;
+  if (tokens == 0) return ok();
+  if (int st = check_rows(who, s, {{"q", q}, {"k", k}, {"q_out", q_out}, {"k_out", k_out}})) return st;
+  auto run = [&]<typename T>() {
+    fhog::RotaryFwdParams<T> p{{(const T*)q, (const T*)k}, {q_weight, k_weight}, {(T*)q_out, (T*)k_out}, {}, rotary_shape(s)};
+    rotary_strides(s, p.stride);
+    return fhog::launch_rotary_fwd<T>(p, fhog::rotary_grid(tokens, compute_units()),
+                                      rotary_wide(s, true, {q, k, q_out, k_out}), (hipStream_t)stream);
+  };
+  return launch_status(dispatch_rows(s.dtype, run), who);
+}
+
+int fhog_qk_norm_rotary_bwd(fhog_stream_t stream, const fhog_rotary* shape, const void* q, const void* k,
+                            const void* q_weight, const void* k_weight, const void* dq_out, const void* dk_out,
+                            void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace) {
+  static const char* who = "fhog_qk_norm_rotary_bwd";
+  if (int st = check_rotary(who, shape)) return st;
+  const fhog_rotary& s = *shape;
+  if (int st = check_weights(who, s, q_weight, k_weight, {{dq_weight, dk_weight}})) return st;
+  const long tokens = (long)s.batch * s.tokens;
+  void* const dw[2] = {dq_weight, dk_weight};
+  if (tokens == 0) return clear_weights(who, s, dw, (hipStream_t)stream);
+  if (int st = check_rows(who, s, {{"dq_out", dq_out}, {"dk_out", dk_out}, {"dq", dq}, {"dk", dk}})) return st;
+  if (s.norm)
+    if (int st = check_rows(who, s, {{"q", q}, {"k", k}})) return st;
+  const bool parts = dq_weight != nullptr || dk_weight != nullptr;
+  if (parts && !aligned(workspace, 4))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null or not 4-byte aligned", who);
+  auto run = [&]<typename T>() {
+    fhog::RotaryBwdParams<T> p{{(const T*)q, (const T*)k}, {q_weight, k_weight}, {(const T*)dq_out, (const T*)dk_out},
+                               {(T*)dq, (T*)dk}, parts ? (float*)workspace : nullptr, {dq_weight, dk_weight}, {},
+                               rotary_shape(s)};
+    rotary_strides(s, p.stride);
+    const bool wide = rotary_wide(s, s.norm, {s.norm ? q : nullptr, s.norm ? k : nullptr, dq_out, dk_out, dq, dk});
+    return fhog::launch_rotary_bwd<T>(p, fhog::rotary_grid(tokens, compute_units()), wide, (hipStream_t)stream);
+  };
+  return launch_status(dispatch_rows(s.dtype, run), who);
+}
+
+int fhog_qk_norm_rotary_bwdbwd(fhog_stream_t stream, const fhog_rotary* shape, const void* q, const void* k,
+                               const void* q_weight, const void* k_weight, const void* dq_out, const void* dk_out,
+                               const void* ddq, const void* ddk, const void* ddq_weight, const void* ddk_weight,
+                               void* dq2, void* dk2, void* dq_weight2, void* dk_weight2, void* ddq_out, void* ddk_out,
+                               void* workspace) {
+  static const char* who = "fhog_qk_norm_rotary_bwdbwd";
+  if (int st = check_rotary(who, shape)) return st;
+  const fhog_rotary& s = *shape;
+  if (!s.norm) return fail(FHOG_ERR_UNSUPPORTED, "%s: without norms the backward is linear", who);
+  if (int st = check_weights(who, s, q_weight, k_weight, {{ddq_weight, ddk_weight}, {dq_weight2, dk_weight2}})) return st;
+  const long tokens = (long)s.batch * s.tokens;
+  void* const dw[2] = {dq_weight2, dk_weight2};
+  if (tokens == 0) return clear_weights(who, s, dw, (hipStream_t)stream);
+  if (int st = check_rows(who, s, {{"q", q}, {"k", k}, {"dq_out", dq_out}, {"dk_out", dk_out}, {"ddq", ddq}, {"ddk", ddk},
+                                   {"dq2", dq2}, {"dk2", dk2}, {"ddq_out", ddq_out}, {"ddk_out", ddk_out}}))
+    return st;
+  const bool parts = dq_weight2 != nullptr || dk_weight2 != nullptr;
+  if (parts && !aligned(workspace, 4))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null or not 4-byte aligned", who);
+  auto run = [&]<typename T>() {
+    fhog::RotaryBwdBwdParams<T> p{{(const T*)q, (const T*)k}, {q_weight, k_weight},
+                                  {(const T*)dq_out, (const T*)dk_out}, {(const T*)ddq, (const T*)ddk},
+                                  {ddq_weight, ddk_weight}, {(T*)dq2, (T*)dk2}, {(T*)ddq_out, (T*)ddk_out},
+                                  parts ? (float*)workspace : nullptr, {dq_weight2, dk_weight2}, {}, rotary_shape(s)};
+    rotary_strides(s, p.stride);
+    const bool wide = rotary_wide(s, true, {q, k, dq_out, dk_out, ddq, ddk, dq2, dk2, ddq_out, ddk_out});
+    return fhog::launch_rotary_bwdbwd<T>(p, fhog::rotary_grid(tokens, compute_units()), wide, (hipStream_t)stream);
+  };
+  return launch_status(dispatch_rows(s.dtype, run), who);
 }
 
 }  // extern "C"

@@ -1,0 +1,440 @@
+// Norms of queries and keys for each head, with the position rotation in the same pass, and their
+// first and second derivatives (fhog_rotary.h).
+//
+// A row x of H values, r = (mean x^2 + eps)^-1/2, n = r x, y = R(n w), where R turns the pairs of the
+// first columns by angles p f_i. With g = R^T dy and the row means C = <g w, n> / H:
+//   dx = r (g w - C n),   dw = sum over rows g n;
+// and with cotangents u of dx and z of dw, U = <u, n> / H, A = <u, g w> / H, Z = <z g, n> / H:
+//   ddy = R(r w (u - U n) + z n)
+//   dx2 = r^2 (n (3 C U - A) - U g w - C u) + r (z g - Z n)
+//   dw2 = sum over rows r g (u - U n).
+// Without norms r = 1 and n = x, and only the rotation remains.
+//
+// All of it is fp32 from the loaded values on, rounded once where a row is stored. Angles are formed
+// in 64 bits, reduced to a part of a turn there, and only then taken to fp32: at position 10^5 fp32
+// would leave 4 10^-3 of an angle. They belong to a token, not to a head: a workgroup forms those of
+// its tokens once, in LDS.
+//
+// L neighbouring lanes hold a row, eight pairs a lane: both partners of a rotation are in one lane, in
+// two 16-byte loads (of 2-byte types) where the row allows them. Every row is read once and written
+// once. The weights' gradients are summed in registers over a workgroup's rows, then over its threads,
+// then by a small kernel over the workgroups, always in the same order.
+#include "fhog_paged.h"
+#include "fhog_rotary.h"
+
+namespace fhog {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMostTile = 16;
+
+// Eight pairs of a row.
+struct Pairs {
+  float a[8], b[8];
+};
+
+// Where lane c of a row finds its pairs 8 c .. 8 c + 7. Columns behind the rotated ones are paired with
+// their neighbours and turned by nothing.
+template <bool WIDE> struct Columns {
+  int head_dim, half, pair0;
+  bool apart;  // partners are half the rotated columns apart
+  __device__ __forceinline__ Columns(const RotaryShape& s, int c)
+      : head_dim(s.head_dim), half(s.rotated / 2), pair0(8 * c), apart(!s.interleaved && 8 * c < s.rotated / 2) {}
+  // WIDE: head_dim and rotated are multiples of 16, rows of 16 bytes.
+  __device__ __forceinline__ bool any() const { return 2 * pair0 < head_dim; }
+  __device__ __forceinline__ int column(int i, int side, bool interleaved) const {
+    const int p = pair0 + i;
+    return p < half && !interleaved ? p + side * half : 2 * p + side;
+  }
+  template <typename T> __device__ __forceinline__ Pairs load(const T* row, bool interleaved) const {
+    Pairs x;
+    if constexpr (WIDE) {
+      V8<T> lo = zero8<T>(), hi = zero8<T>();
+      if (any()) {
+        lo = *reinterpret_cast<const V8<T>*>(row + (apart ? pair0 : 2 * pair0));
+        hi = *reinterpret_cast<const V8<T>*>(row + (apart ? pair0 + half : 2 * pair0 + 8));
+      }
+      if (apart) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.a[i] = (float)lo[i], x.b[i] = (float)hi[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x.a[i] = (float)lo[2 * i], x.b[i] = (float)lo[2 * i + 1];
+          x.a[4 + i] = (float)hi[2 * i], x.b[4 + i] = (float)hi[2 * i + 1];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int ca = column(i, 0, interleaved), cb = column(i, 1, interleaved);
+        x.a[i] = ca < head_dim ? (float)row[ca] : 0.f;
+        x.b[i] = cb < head_dim ? (float)row[cb] : 0.f;
+      }
+    }
+    return x;
+  }
+  template <typename T> __device__ __forceinline__ void store(T* row, const Pairs& x, bool interleaved) const {
+    if constexpr (WIDE) {
+      if (!any()) return;
+      f32x8 lo, hi;
+      if (apart) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lo[i] = x.a[i], hi[i] = x.b[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[2 * i] = x.a[i], lo[2 * i + 1] = x.b[i];
+          hi[2 * i] = x.a[4 + i], hi[2 * i + 1] = x.b[4 + i];
+        }
+      }
+      *reinterpret_cast<V8<T>*>(row + (apart ? pair0 : 2 * pair0)) = cvt8<T>(lo);
+      *reinterpret_cast<V8<T>*>(row + (apart ? pair0 + half : 2 * pair0 + 8)) = cvt8<T>(hi);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int ca = column(i, 0, interleaved), cb = column(i, 1, interleaved);
+        if (ca < head_dim) row[ca] = (T)x.a[i];
+        if (cb < head_dim) row[cb] = (T)x.b[i];
+      }
+    }
+  }
+};
+
+// A weight, or a cotangent of one: in T or, beside 2-byte rows, in fp32.
+template <typename T, bool WIDE>
+__device__ __forceinline__ Pairs load_weight(const Columns<WIDE>& at, const void* w, const RotaryShape& s, float none) {
+  Pairs x;
+  if (w == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.a[i] = x.b[i] = none;
+    return x;
+  }
+  const Columns<false> one(s, at.pair0 / 8);  // (its own alignment is not known)
+  return s.wide_weights ? one.load((const float*)w, s.interleaved) : one.load((const T*)w, s.interleaved);
+}
+
+// Sum over the L lanes of a row, in all of them.
+template <int L> __device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+  for (int d = 1; d < L; d <<= 1) x += __shfl_xor(x, d, 64);
+  return x;
+}
+
+__device__ __forceinline__ float dot(const Pairs& x, const Pairs& y) {
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = fmaf(x.a[i], y.a[i], fmaf(x.b[i], y.b[i], sum));
+  return sum;
+}
+
+// cos and sin of a token's angles for eight pairs of a row, and the rotations.
+struct Turn {
+  alignas(16) float c[8];
+  alignas(16) float s[8];
+  __device__ __forceinline__ Pairs there(const Pairs& x) const {
+    Pairs y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y.a[i] = x.a[i] * c[i] - x.b[i] * s[i];
+      y.b[i] = x.b[i] * c[i] + x.a[i] * s[i];
+    }
+    return y;
+  }
+  __device__ __forceinline__ Pairs back(const Pairs& y) const {
+    Pairs x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x.a[i] = y.a[i] * c[i] + y.b[i] * s[i];
+      x.b[i] = y.b[i] * c[i] - y.a[i] * s[i];
+    }
+    return x;
+  }
+};
+
+__device__ __forceinline__ double position(const RotaryShape& s, long token) {
+  if (s.positions != nullptr) {
+    const long at = s.position_rows > 1 ? token : token % s.tokens;
+    return s.position_bytes == 8 ? (double)((const long*)s.positions)[at] : (double)((const int*)s.positions)[at];
+  }
+  if (s.lengths == nullptr) return (double)(token % s.tokens);
+  const int t = (int)token;
+  if (s.offsets == nullptr) return (double)s.lengths[t] - 1.0;
+  const CacheShape c{nullptr, s.lengths, s.offsets, s.sequences, s.tokens, 0, 0, 0, 0};
+  const int b = last_at_or_before(s.sequences, t, [&](int i) { return packed_begin(c, i); });
+  const int begin = packed_begin(c, b), end = packed_begin(c, b + 1);
+  return t < begin || t >= end ? 0.0 : (double)s.lengths[b] - (double)(end - t);
+}
+
+// The workgroup's angles: those of tokens [first, first + count), kPairs a token.
+template <int L> struct Angles {
+  static constexpr int kPairs = 8 * L;
+  alignas(16) float c[kMostTile][kPairs];
+  alignas(16) float s[kMostTile][kPairs];
+  __device__ __forceinline__ void form(const RotaryShape& shape, long first, int count) {
+    for (int i = threadIdx.x; i < count * kPairs; i += kThreads) {
+      const int token = i / kPairs, pair = i % kPairs;
+      float cos = 1.f, sin = 0.f;
+      if (2 * pair < shape.rotated) {
+        const double turns = position(shape, first + token) * (double)shape.frequencies[pair] * 0.15915494309189535;
+        sincospif((float)(2.0 * (turns - rint(turns))), &sin, &cos);
+      }
+      c[token][pair] = cos;
+      s[token][pair] = sin;
+    }
+  }
+  __device__ __forceinline__ Turn of(int token, int lane) const {
+    Turn t;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      *reinterpret_cast<f32x4*>(t.c + i) = *reinterpret_cast<const f32x4*>(&c[token][8 * lane + i]);
+      *reinterpret_cast<f32x4*>(t.s + i) = *reinterpret_cast<const f32x4*>(&s[token][8 * lane + i]);
+    }
+    return t;
+  }
+};
+
+// Calls f(token of the tile, offset of the row in x, offset in contiguous tensors, Turn) for every row
+// that this thread's lane group has, of the workgroup's tiles.
+template <int L, typename F>
+__device__ __forceinline__ void for_rows(const RotaryShape& s, const RowStrides& stride, int which, int tile,
+                                         Angles<L>& angles, F&& f) {
+  constexpr int kRows = kThreads / L;
+  const int heads = s.heads[which], lane = threadIdx.x % L, group = threadIdx.x / L;
+  const long tokens = (long)s.batch * s.tokens;
+  for (long t0 = (long)blockIdx.x * tile; t0 < tokens; t0 += (long)gridDim.x * tile) {
+    const int count = (int)(tokens - t0 < tile ? tokens - t0 : tile);
+    __syncthreads();  // (the tile before is read)
+    angles.form(s, t0, count);
+    __syncthreads();
+    // (every lane of a group takes the same way, so the sums' shuffles find each other)
+    for (int r = group; r < count * heads; r += kRows) {
+      const int t = r / heads, h = r % heads;
+      const long token = t0 + t, b = token / s.tokens;
+      f(b * stride.batch + (token - b * s.tokens) * stride.token + h * stride.head,
+        (token * heads + h) * (long)s.head_dim, angles.of(t, lane));
+    }
+  }
+}
+
+// A workgroup's part of a weight's gradient: the sums of its threads that hold the same columns.
+template <int L, bool WIDE>
+__device__ __forceinline__ void leave_parts(const Columns<WIDE>& at, const RotaryShape& s, const Pairs& sum, float* part,
+                                            float* box) {
+  // Lanes with the same columns within a wave, then the waves, through LDS.
+  Pairs x = sum;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    for (int d = L; d < 64; d <<= 1) {
+      x.a[i] += __shfl_xor(x.a[i], d, 64);
+      x.b[i] += __shfl_xor(x.b[i], d, 64);
+    }
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __syncthreads();
+  if (lane < L)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      box[(wave * L + lane) * 16 + i] = x.a[i];
+      box[(wave * L + lane) * 16 + 8 + i] = x.b[i];
+    }
+  __syncthreads();
+  if (threadIdx.x < L)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float y = 0.f;
+      for (int w = 0; w < kThreads / 64; ++w) y += box[(w * L + threadIdx.x) * 16 + i];
+      const int col = at.column(i & 7, i >> 3, s.interleaved);
+      if (col < s.head_dim) part[col] = y;
+    }
+}
+
+template <typename T, int L, bool WIDE>
+__global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(RotaryFwdParams<T> p, int tile) {
+  __shared__ Angles<L> angles;
+  const int which = blockIdx.y;
+  const Columns<WIDE> at(p.s, threadIdx.x % L);
+  const Pairs w = load_weight<T>(at, p.weight[which], p.s, 1.f);
+  const float inv = 1.f / (float)p.s.head_dim;
+  const T* const rows = p.x[which];
+  T* const out = p.y[which];
+  for_rows<L>(p.s, p.stride[which], which, tile, angles, [&](long from, long to, const Turn& turn) {
+    Pairs x = at.load(rows + from, p.s.interleaved);
+    if (p.s.norm) {
+      const float r = rsqrtf(row_sum<L>(dot(x, x)) * inv + p.s.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x.a[i] *= r * w.a[i];
+        x.b[i] *= r * w.b[i];
+      }
+    }
+    at.store(out + to, turn.there(x), p.s.interleaved);
+  });
+}
+
+template <typename T, int L, bool WIDE>
+__global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(RotaryBwdParams<T> p, int tile) {
+  __shared__ Angles<L> angles;
+  __shared__ float box[kThreads / 64 * L * 16];
+  const int which = blockIdx.y;
+  const Columns<WIDE> at(p.s, threadIdx.x % L);
+  const Pairs w = load_weight<T>(at, p.weight[which], p.s, 1.f);
+  const float inv = 1.f / (float)p.s.head_dim;
+  const T* const rows = p.x[which];
+  const T* const dy = p.dy[which];
+  T* const dx = p.dx[which];
+  Pairs sum{};
+  for_rows<L>(p.s, p.stride[which], which, tile, angles, [&](long from, long to, const Turn& turn) {
+    Pairs g = turn.back(at.load(dy + to, p.s.interleaved));
+    if (p.s.norm) {
+      Pairs n = at.load(rows + from, p.s.interleaved);
+      const float r = rsqrtf(row_sum<L>(dot(n, n)) * inv + p.s.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        n.a[i] *= r;
+        n.b[i] *= r;
+        sum.a[i] = fmaf(g.a[i], n.a[i], sum.a[i]);
+        sum.b[i] = fmaf(g.b[i], n.b[i], sum.b[i]);
+        g.a[i] *= w.a[i];
+        g.b[i] *= w.b[i];
+      }
+      const float C = row_sum<L>(dot(g, n)) * inv;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        g.a[i] = r * (g.a[i] - C * n.a[i]);
+        g.b[i] = r * (g.b[i] - C * n.b[i]);
+      }
+    }
+    at.store(dx + to, g, p.s.interleaved);
+  });
+  if (p.parts != nullptr && p.weight[which] != nullptr)
+    leave_parts<L>(at, p.s, sum, p.parts + ((long)which * gridDim.x + blockIdx.x) * p.s.head_dim, box);
+}
+
+template <typename T, int L, bool WIDE>
+__global__ void __launch_bounds__(kThreads) rotary_bwdbwd_kernel(RotaryBwdBwdParams<T> p, int tile) {
+  __shared__ Angles<L> angles;
+  __shared__ float box[kThreads / 64 * L * 16];
+  const int which = blockIdx.y;
+  const Columns<WIDE> at(p.s, threadIdx.x % L);
+  const Pairs w = load_weight<T>(at, p.weight[which], p.s, 1.f);
+  const Pairs z = load_weight<T>(at, p.z[which], p.s, 0.f);
+  const float inv = 1.f / (float)p.s.head_dim;
+  const T* const rows = p.x[which];
+  const T* const dy = p.dy[which];
+  const T* const cot = p.u[which];
+  Pairs sum{};
+  for_rows<L>(p.s, p.stride[which], which, tile, angles, [&](long from, long to, const Turn& turn) {
+    Pairs n = at.load(rows + from, p.s.interleaved);
+    const Pairs g = turn.back(at.load(dy + to, p.s.interleaved));
+    const Pairs u = at.load(cot + to, p.s.interleaved);
+    const float r = rsqrtf(row_sum<L>(dot(n, n)) * inv + p.s.eps);
+    Pairs gw, zg;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      n.a[i] *= r, n.b[i] *= r;
+      gw.a[i] = g.a[i] * w.a[i], gw.b[i] = g.b[i] * w.b[i];
+      zg.a[i] = g.a[i] * z.a[i], zg.b[i] = g.b[i] * z.b[i];
+    }
+    const float C = row_sum<L>(dot(gw, n)) * inv, U = row_sum<L>(dot(u, n)) * inv;
+    const float A = row_sum<L>(dot(u, gw)) * inv, Z = row_sum<L>(dot(zg, n)) * inv;
+    const float r2 = r * r, nn = r2 * (3.f * C * U - A) - r * Z;
+    Pairs dd, d2;
+    auto one = [&](float n1, float g1, float gw1, float zg1, float u1, float w1, float z1, float& dd1, float& d21,
+                   float& sum1) {
+      const float rest = u1 - U * n1;
+      dd1 = r * w1 * rest + z1 * n1;
+      d21 = nn * n1 - r2 * (U * gw1 + C * u1) + r * zg1;
+      sum1 = fmaf(r * g1, rest, sum1);
+    };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      one(n.a[i], g.a[i], gw.a[i], zg.a[i], u.a[i], w.a[i], z.a[i], dd.a[i], d2.a[i], sum.a[i]);
+      one(n.b[i], g.b[i], gw.b[i], zg.b[i], u.b[i], w.b[i], z.b[i], dd.b[i], d2.b[i], sum.b[i]);
+    }
+    at.store(p.ddy[which] + to, turn.there(dd), p.s.interleaved);
+    at.store(p.dx2[which] + to, d2, p.s.interleaved);
+  });
+  if (p.parts != nullptr && p.weight[which] != nullptr)
+    leave_parts<L>(at, p.s, sum, p.parts + ((long)which * gridDim.x + blockIdx.x) * p.s.head_dim, box);
+}
+
+// The workgroups' parts of both weights' gradients to one: a workgroup eight columns, whose
+// threads take every 32nd part and meet in LDS.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rotary_weights_kernel(const float* parts, void* out_q, void* out_k, int groups,
+                                                                  int head_dim, int wide_weights) {
+  __shared__ float box[kThreads];
+  void* const out = blockIdx.y ? out_k : out_q;
+  if (out == nullptr) return;
+  const int col = 8 * (int)blockIdx.x + (int)threadIdx.x % 8, way = threadIdx.x / 8;
+  float sum = 0.f;
+  if (col < head_dim)
+    for (int i = way; i < groups; i += kThreads / 8) sum += parts[((long)blockIdx.y * groups + i) * head_dim + col];
+  box[threadIdx.x] = sum;
+  __syncthreads();
+  if (way > 0 || col >= head_dim) return;
+  for (int w = 1; w < kThreads / 8; ++w) sum += box[8 * w + threadIdx.x];
+  if (wide_weights)
+    ((float*)out)[col] = sum;
+  else
+    ((T*)out)[col] = (T)sum;
+}
+
+// f.template operator()<L, WIDE>() with the lanes that a row takes.
+template <typename F> void with_lanes(int head_dim, bool wide, F&& f) {
+  auto lanes = [&]<int L>() { wide ? f.template operator()<L, true>() : f.template operator()<L, false>(); };
+  if (head_dim <= 64)
+    lanes.template operator()<4>();
+  else if (head_dim <= 128)
+    lanes.template operator()<8>();
+  else
+    lanes.template operator()<16>();
+}
+
+}  // namespace
+
+template <typename T>
+hipError_t sum_rotary_weights(const float* parts, void* const out[2], const RotaryShape& s, int groups, hipStream_t stream) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || (out[0] == nullptr && out[1] == nullptr)) return e;
+  hipLaunchKernelGGL((rotary_weights_kernel<T>), dim3((s.head_dim + 7) / 8, 2), dim3(kThreads), 0, stream, parts, out[0],
+                     out[1], groups, s.head_dim, s.wide_weights);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_rotary_fwd(const RotaryFwdParams<T>& p, const RotaryGrid& g, bool wide, hipStream_t stream) {
+  with_lanes(p.s.head_dim, wide, [&]<int L, bool WIDE>() {
+    hipLaunchKernelGGL((rotary_fwd_kernel<T, L, WIDE>), dim3(g.groups, 2), dim3(kThreads), 0, stream, p, g.tile);
+  });
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_rotary_bwd(const RotaryBwdParams<T>& p, const RotaryGrid& g, bool wide, hipStream_t stream) {
+  with_lanes(p.s.head_dim, wide, [&]<int L, bool WIDE>() {
+    hipLaunchKernelGGL((rotary_bwd_kernel<T, L, WIDE>), dim3(g.groups, 2), dim3(kThreads), 0, stream, p, g.tile);
+  });
+  return sum_rotary_weights<T>(p.parts, p.dweight, p.s, g.groups, stream);
+}
+
+template <typename T>
+hipError_t launch_rotary_bwdbwd(const RotaryBwdBwdParams<T>& p, const RotaryGrid& g, bool wide, hipStream_t stream) {
+  with_lanes(p.s.head_dim, wide, [&]<int L, bool WIDE>() {
+    hipLaunchKernelGGL((rotary_bwdbwd_kernel<T, L, WIDE>), dim3(g.groups, 2), dim3(kThreads), 0, stream, p, g.tile);
+  });
+  return sum_rotary_weights<T>(p.parts, p.dweight2, p.s, g.groups, stream);
+}
+
+#define FHOG_INST(T)                                                                                         \
+  template hipError_t sum_rotary_weights<T>(const float*, void* const*, const RotaryShape&, int, hipStream_t); \
+  template hipError_t launch_rotary_fwd<T>(const RotaryFwdParams<T>&, const RotaryGrid&, bool, hipStream_t);  \
+  template hipError_t launch_rotary_bwd<T>(const RotaryBwdParams<T>&, const RotaryGrid&, bool, hipStream_t);  \
+  template hipError_t launch_rotary_bwdbwd<T>(const RotaryBwdBwdParams<T>&, const RotaryGrid&, bool, hipStream_t);
+FHOG_INST(__bf16)
+FHOG_INST(_Float16)
+FHOG_INST(float)
+#undef FHOG_INST
+
+}  // namespace fhog

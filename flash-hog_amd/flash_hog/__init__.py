@@ -10,6 +10,7 @@ from flash_hog._types import MaskType, TuningConfig
 from flash_hog.torch._hip_gpu import supported
 from flash_hog.torch.attention import dot_product_attention
 from flash_hog.torch.paged import paged_attention, paged_cache_read, paged_cache_write
+from flash_hog.torch.rotary import qk_norm_rotary
 
 __all__ = ["MaskType", "TuningConfig", "dot_product_attention", "paged_attention", "paged_cache_read",
-           "paged_cache_write", "supported"]
+           "paged_cache_write", "qk_norm_rotary", "supported"]

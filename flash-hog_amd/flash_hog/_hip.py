@@ -62,7 +62,21 @@ SIGNATURES = {
     "fhog_paged_attention": (_i, [_p] * 11 + [ctypes.c_size_t] + [_i] * 13 + [_f]),
     "fhog_paged_cache_write": (_i, [_p] * 10 + [_i] * 9),
     "fhog_paged_cache_read": (_i, [_p] * 9 + [_i] * 9),
+    "fhog_qk_norm_rotary_workspace_bytes": (ctypes.c_size_t, [_p]),
+    "fhog_qk_norm_rotary_fwd": (_i, [_p] * 8),
+    "fhog_qk_norm_rotary_bwd": (_i, [_p] * 13),
+    "fhog_qk_norm_rotary_bwdbwd": (_i, [_p] * 19),
 }
+
+
+class Rotary(ctypes.Structure):
+    """fhog_rotary."""
+
+    _fields_ = ([(n, _i) for n in ("batch", "tokens", "heads", "kv_heads", "head_dim", "rotated", "dtype",
+                                   "weight_dtype", "interleaved", "norm")]
+                + [("eps", _f)] + [(n, _i) for n in ("position_bytes", "position_rows", "sequences")]
+                + [(n, ctypes.c_longlong * 3) for n in ("q_stride", "k_stride")]
+                + [(n, _p) for n in ("frequencies", "positions", "lengths", "query_offsets")])
 
 
 class FlashHogError(RuntimeError):
@@ -512,3 +526,142 @@ def paged_cache_read(k_cache, v_cache, page_table, lengths, max_length: int, dty
             _ptr(lengths), _ptr(k), _ptr(v), B, max_length, Nk, Hd, pages, page, width, DTYPE_CODES[dtype],
             CACHE_DTYPE_CODES[k_cache.dtype]))
     return k, v
+
+
+# ------------------------------------------------- norms with rotation
+
+def _rows(t):
+    """t with its rows (last axis) contiguous; elements between rows may be any."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _RotaryCall:
+    """The checked arguments that the three calls share: q (B, T, N, H) and k (B, T, Nk, H) (any strides
+    between rows), weights (H,) or None, frequencies (R / 2,) fp32 or None, positions (T,) or (B, T) or
+    lengths (sequences,) [and query_offsets (sequences + 1,)] with B = 1 or neither, eps None: no norms.
+    like: tensors of q's and k's shapes that stand for them where the rows themselves are not read."""
+
+    def __init__(self, q, k, wq, wk, frequencies, positions, lengths, query_offsets, interleaved, eps, strided=True):
+        named = [("query", q), ("key", k)]
+        index = [(n, t) for n, t in (("positions", positions), ("lengths", lengths), ("query_offsets", query_offsets))
+                 if t is not None]
+        weights = [(n, t) for n, t in (("query_weight", wq), ("key_weight", wk)) if t is not None]
+        freq = [] if frequencies is None else [("frequencies", frequencies)]
+        _check_inputs(named + weights + freq + index)
+        _check_inputs(named, q.dtype)
+        if q.dtype not in DTYPE_CODES:
+            raise ValueError(f"unsupported dtype {q.dtype}")
+        if q.ndim != 4 or k.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+            raise ValueError("expected query (B, T, N, H) and key (B, T, N_kv, H) of the same tokens and head_dim, got "
+                             f"{tuple(q.shape)} and {tuple(k.shape)}")
+        B, T, N, Hd = q.shape
+        if eps is None and weights:
+            raise ValueError("weights need norms (eps is None)")
+        weight_dtype = weights[0][1].dtype if weights else q.dtype
+        for name, t in weights:
+            _expect(name, t, (Hd,), weight_dtype)
+        if weight_dtype not in (q.dtype, torch.float32):
+            raise ValueError(f"weights must be of {q.dtype} or torch.float32, got {weight_dtype}")
+        if frequencies is not None:
+            if frequencies.ndim != 1 or 2 * frequencies.shape[0] > Hd or frequencies.dtype != torch.float32:
+                raise ValueError(f"frequencies must be torch.float32 (R / 2,) with R <= head_dim, got "
+                                 f"{tuple(frequencies.shape)} of {frequencies.dtype} for head_dim {Hd}")
+        if positions is not None:
+            if lengths is not None:
+                raise ValueError("positions and lengths exclude each other")
+            if positions.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f"positions has dtype {positions.dtype}, expected torch.int32 or torch.int64")
+            if tuple(positions.shape) not in ((T,), (B, T)):
+                raise ValueError(f"positions has shape {tuple(positions.shape)}, expected {(T,)} or {(B, T)}")
+        if query_offsets is not None and lengths is None:
+            raise ValueError("query_offsets needs lengths")
+        if lengths is not None:
+            if lengths.ndim != 1:
+                raise ValueError(f"expected (batch,) lengths, got {tuple(lengths.shape)}")
+            if B != 1:
+                raise ValueError(f"lengths go with packed tokens (T, N, H), got a batch of {B}")
+            if query_offsets is None:
+                _expect("lengths", lengths, (T,))
+            else:
+                _expect("query_offsets", query_offsets, (lengths.shape[0] + 1,))
+            for name, t in index:
+                if t.dtype != torch.int32:
+                    raise ValueError(f"{name} has dtype {t.dtype}, expected torch.int32")
+        self.q, self.k = (_rows(q), _rows(k)) if strided else (q, k)
+        contiguous = lambda t: None if t is None else t.contiguous()
+        self.wq, self.wk = contiguous(wq), contiguous(wk)
+        self.held = tuple(map(contiguous, (frequencies, positions, lengths, query_offsets)))
+        frequencies, positions, lengths, query_offsets = self.held
+        self.device, self.weight_dtype = q.device, weight_dtype
+        self.shape = Rotary(
+            B, T, N, k.shape[2], Hd, 0 if frequencies is None else 2 * frequencies.shape[0], DTYPE_CODES[q.dtype],
+            DTYPE_CODES[weight_dtype], int(bool(interleaved)), int(eps is not None), 0.0 if eps is None else float(eps),
+            0 if positions is None else positions.element_size(),
+            0 if positions is None else 1 if positions.ndim == 1 else B, 0 if lengths is None else lengths.shape[0],
+            (ctypes.c_longlong * 3)(*self.q.stride()[:3]), (ctypes.c_longlong * 3)(*self.k.stride()[:3]),
+            *map(_ptr, self.held))
+
+    def contiguous(self, q_name, q, k_name, k):
+        """Tensors of q's and k's shapes, checked."""
+        _check_inputs([("query", self.q), (q_name, q), (k_name, k)], self.q.dtype)
+        _expect(q_name, q, self.q.shape)
+        _expect(k_name, k, self.k.shape)
+        return _contig(q, k)
+
+    def rows(self):
+        return tuple(torch.empty(t.shape, device=self.device, dtype=t.dtype) for t in (self.q, self.k))
+
+    def weights(self):
+        return tuple(None if w is None else torch.empty_like(w) for w in (self.wq, self.wk))
+
+    def workspace(self):
+        if self.wq is None and self.wk is None:
+            return None
+        size = lib().fhog_qk_norm_rotary_workspace_bytes(ctypes.byref(self.shape))
+        return torch.empty(size, device=self.device, dtype=torch.uint8) if size else None
+
+
+def qk_norm_rotary_fwd(q, k, wq, wk, frequencies, positions, lengths, query_offsets, interleaved, eps):
+    """(q_out, k_out), contiguous (fhog_qk_norm_rotary_fwd; the arguments: _RotaryCall)."""
+    c = _RotaryCall(q, k, wq, wk, frequencies, positions, lengths, query_offsets, interleaved, eps)
+    out = c.rows()
+    with _on_device(c.device):
+        check(lib().fhog_qk_norm_rotary_fwd(_stream(c.device), ctypes.byref(c.shape), _ptr(c.q), _ptr(c.k), _ptr(c.wq),
+                                            _ptr(c.wk), *map(_ptr, out)))
+    return out
+
+
+def qk_norm_rotary_bwd(q, k, wq, wk, gq, gk, frequencies, positions, lengths, query_offsets, interleaved, eps):
+    """(dq, dk, dwq, dwk) from the cotangents gq, gk of the forward's results; None where a weight is.
+    Without norms q and k are only looked at for their shapes."""
+    c = _RotaryCall(q, k, wq, wk, frequencies, positions, lengths, query_offsets, interleaved, eps, eps is not None)
+    gq, gk = c.contiguous("query's cotangent", gq, "key's cotangent", gk)
+    d, dw = c.rows(), c.weights()
+    with _on_device(c.device):
+        ws = c.workspace()
+        x = (None, None) if eps is None else (_ptr(c.q), _ptr(c.k))
+        check(lib().fhog_qk_norm_rotary_bwd(_stream(c.device), ctypes.byref(c.shape), *x, _ptr(c.wq), _ptr(c.wk),
+                                            _ptr(gq), _ptr(gk), *map(_ptr, d), *map(_ptr, dw), _ptr(ws)))
+    return (*d, *dw)
+
+
+def qk_norm_rotary_bwdbwd(q, k, wq, wk, gq, gk, uq, uk, zq, zk, frequencies, positions, lengths, query_offsets,
+                          interleaved, eps):
+    """Cotangents (dq2, dk2, dwq2, dwk2, dgq, dgk) of the backward's inputs from those (uq, uk, zq, zk) of its
+    results; norms only."""
+    c = _RotaryCall(q, k, wq, wk, frequencies, positions, lengths, query_offsets, interleaved, eps)
+    gq, gk = c.contiguous("query's cotangent", gq, "key's cotangent", gk)
+    uq, uk = c.contiguous("cotangent of query's gradient", uq, "cotangent of key's gradient", uk)
+    z = []
+    for w, t in ((c.wq, zq), (c.wk, zk)):
+        if w is not None:
+            _check_inputs([("query", c.q), ("cotangent of a weight's gradient", t)])
+            _expect("cotangent of a weight's gradient", t, w.shape, w.dtype)
+        z.append(None if w is None else t.contiguous())
+    d2, dg, dw2 = c.rows(), c.rows(), c.weights()
+    with _on_device(c.device):
+        ws = c.workspace()
+        check(lib().fhog_qk_norm_rotary_bwdbwd(
+            _stream(c.device), ctypes.byref(c.shape), _ptr(c.q), _ptr(c.k), _ptr(c.wq), _ptr(c.wk), _ptr(gq), _ptr(gk),
+            _ptr(uq), _ptr(uk), *map(_ptr, z), *map(_ptr, d2), *map(_ptr, dw2), *map(_ptr, dg), _ptr(ws)))
+    return (*d2, *dw2, *dg)

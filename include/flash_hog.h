@@ -284,6 +284,59 @@ int fhog_paged_cache_read(fhog_stream_t stream, const void* k_cache, const void*
                           int max_length, int kv_heads, int head_dim, int num_pages, int page_size,
                           int pages_per_seq, int dtype, int cache_dtype);
 
+/*
+ * Norms of queries and keys for each head with the position rotation, and their derivatives (no
+ * counterpart in the reference): what stands before the attention of either kind.
+ *
+ * A row x of head_dim values of q (batch, tokens, heads, head_dim) or k (.., kv_heads, ..) becomes
+ * R(w x (mean x^2 + eps)^-1/2), where R turns pairs of its first `rotated` columns (even; 0: none) by the
+ * angles position * frequencies[i], formed in 64 bits: columns i and i + rotated / 2, or 2 i and 2 i + 1
+ * if interleaved. norm 0: R(x). Any head_dim from 1 to 256, bf16, fp16 or fp32; sums are fp32.
+ */
+typedef struct fhog_rotary {
+  int batch, tokens, heads, kv_heads, head_dim, rotated;
+  int dtype;        /* of the rows */
+  int weight_dtype; /* of the weights and their gradients: dtype or FHOG_DTYPE_F32 */
+  int interleaved, norm;
+  float eps;
+  int position_bytes;       /* 4 or 8: an element of `positions`; otherwise ignored */
+  int position_rows;        /* of `positions`: 1 (tokens) or batch (batch, tokens) */
+  int sequences;            /* of `lengths` */
+  long long q_stride[3];    /* elements between batches, tokens and heads of q, whose rows are contiguous */
+  long long k_stride[3];
+  const float* frequencies; /* (rotated / 2), null if rotated is 0 */
+  const void* positions;    /* whole numbers, or null */
+  /* A paged cache's (see there), with batch 1 and positions null: the tokens are packed and take the last
+   * positions of their sequences; rows of no sequence are at position 0. Both null, and positions
+   * too: a token's place in its batch. */
+  const int* lengths;
+  const int* query_offsets;
+} fhog_rotary;
+
+/* Bytes of workspace of the two backwards on the current device (0 without weights or norms). Calls
+ * that may overlap need one each. */
+size_t fhog_qk_norm_rotary_workspace_bytes(const fhog_rotary* shape);
+
+/* q_out, k_out (contiguous, as all tensors but q and k) from q, k and the weights (head_dim) of their
+ * norms; a null weight is ones. shape and the arrays in it are read before the call returns. */
+int fhog_qk_norm_rotary_fwd(fhog_stream_t stream, const fhog_rotary* shape, const void* q, const void* k,
+                            const void* q_weight, const void* k_weight, void* q_out, void* k_out);
+
+/* dq, dk and the weights' gradients (null where the weight is) from the cotangents of q_out and k_out.
+ * Without norms q and k are not read and may be null. */
+int fhog_qk_norm_rotary_bwd(fhog_stream_t stream, const fhog_rotary* shape, const void* q, const void* k,
+                            const void* q_weight, const void* k_weight, const void* dq_out, const void* dk_out,
+                            void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace);
+
+/* With cotangents (ddq, ddk, ddq_weight, ddk_weight) of the backward's results: cotangents of its
+ * inputs q, k, the weights, dq_out and dk_out. Norms only (without them the backward is
+ * linear, and its derivative the forward). */
+int fhog_qk_norm_rotary_bwdbwd(fhog_stream_t stream, const fhog_rotary* shape, const void* q, const void* k,
+                               const void* q_weight, const void* k_weight, const void* dq_out, const void* dk_out,
+                               const void* ddq, const void* ddk, const void* ddq_weight, const void* ddk_weight,
+                               void* dq2, void* dk2, void* dq_weight2, void* dk_weight2, void* ddq_out, void* ddk_out,
+                               void* workspace);
+
 #ifdef __cplusplus
 }
 #endif
