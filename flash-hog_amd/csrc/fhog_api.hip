@@ -14,6 +14,7 @@
 #include "flash_hog.h"
 #include "fhog_params.h"
 #include "fhog_paged.h"
+#include "fhog_pages.h"
 #include "fhog_rotary.h"
 
 namespace {
@@ -777,6 +778,103 @@ int fhog_qk_norm_rotary_bwdbwd(fhog_stream_t stream, const fhog_rotary* shape, c
     return fhog::launch_rotary_bwdbwd<T>(p, fhog::rotary_grid(tokens, compute_units()), wide, (hipStream_t)stream);
   };
   return launch_status(dispatch_rows(s.dtype, run), who);
+}
+
+}  // extern "C"
+
+namespace {
+
+// What the allocator's two entry points share.
+int check_pages(const char* who, int batch, int kv_heads, int head_dim, int num_pages, int page_size, int pages_per_seq,
+                int cache_dtype) {
+  const int dtype = cache_dtype == FHOG_DTYPE_E4M3 ? (int)FHOG_DTYPE_BF16 : cache_dtype;
+  if (int st = check_paged({batch, 0, kv_heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype,
+                            cache_dtype}, who))
+    return st;
+  if ((long long)batch * pages_per_seq >= (1ll << 31) || kv_heads > 65535)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  return FHOG_OK;
+}
+
+int check_pages_workspace(const char* who, const void* workspace, size_t bytes, int batch, int num_pages,
+                          int pages_per_seq) {
+  const size_t need = fhog_paged_pages_workspace_bytes(batch, num_pages, pages_per_seq);
+  if (!aligned(workspace, 4) || bytes < need)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null, not 4-byte aligned or below its %zu bytes", who, need);
+  return FHOG_OK;
+}
+
+fhog::PageBytes page_bytes(const void* k, const void* v, const void* ks, const void* vs, const void* means, int head_dim,
+                           int page_size, int cache_dtype) {
+  const bool quantised = cache_dtype == FHOG_DTYPE_E4M3;
+  const int row = head_dim * (quantised ? 1 : 2);
+  return fhog::PageBytes{{(char*)k, (char*)v, quantised ? (char*)ks : nullptr, quantised ? (char*)vs : nullptr,
+                          (char*)means},
+                         {row * page_size, row * page_size, page_size, page_size, head_dim * 4}, {row, row, 1, 1, 0}};
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fhog_paged_pages_workspace_bytes(int batch, int num_pages, int pages_per_seq) {
+  if (batch < 0 || num_pages < 1 || pages_per_seq < 1) return 0;
+  return (size_t)fhog::pages_workspace_ints(batch, pages_per_seq, num_pages) * sizeof(int);
+}
+
+int fhog_paged_cache_extend(fhog_stream_t stream, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                            int* page_table, int* lengths, const int* parents, const int* new_tokens, int new_each,
+                            int* free_pages, void* workspace, size_t workspace_bytes, int batch, int kv_heads,
+                            int head_dim, int num_pages, int page_size, int pages_per_seq, int cache_dtype) {
+  static const char* who = "fhog_paged_cache_extend";
+  if (int st = check_pages(who, batch, kv_heads, head_dim, num_pages, page_size, pages_per_seq, cache_dtype)) return st;
+  if (batch == 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: no rows", who);
+  if (new_tokens == nullptr && new_each < 0)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: new_each must be >= 0, got %d", who, new_each);
+  const Paged s{batch, 0, kv_heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, FHOG_DTYPE_BF16, cache_dtype};
+  if (int st = check_cache(who, s, k_cache, v_cache, k_scale, v_scale, page_table, lengths)) return st;
+  if (int st = check_ptrs(who, {}, {{"free_pages", free_pages}})) return st;
+  if ((parents != nullptr && !aligned(parents, 4)) || (new_tokens != nullptr && !aligned(new_tokens, 4)))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: parents and new_tokens must be 4-byte aligned", who);
+  if (int st = check_pages_workspace(who, workspace, workspace_bytes, batch, num_pages, pages_per_seq)) return st;
+  fhog::PagesParams p{page_table, lengths, parents, new_tokens, new_each, batch, pages_per_seq, num_pages,
+                      __builtin_ctz((unsigned)page_size), kv_heads, 0};
+  fhog::pages_workspace(p, (int*)workspace);
+  return launch_status(fhog::launch_pages_extend(
+      p, page_bytes(k_cache, v_cache, k_scale, v_scale, nullptr, head_dim, page_size, cache_dtype), free_pages,
+      (hipStream_t)stream), who);
+}
+
+int fhog_paged_cache_compact(fhog_stream_t stream, const void* k_cache, const void* v_cache, const void* k_scale,
+                             const void* v_scale, const float* key_means, const int* page_table, const int* lengths,
+                             void* k_out, void* v_out, void* k_scale_out, void* v_scale_out, float* means_out,
+                             int* table_out, void* workspace, size_t workspace_bytes, int batch, int kv_heads,
+                             int head_dim, int num_pages, int page_size, int pages_per_seq, int out_pages,
+                             int cache_dtype) {
+  static const char* who = "fhog_paged_cache_compact";
+  if (int st = check_pages(who, batch, kv_heads, head_dim, num_pages, page_size, pages_per_seq, cache_dtype)) return st;
+  if (out_pages < 1) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: out_pages must be >= 1, got %d", who, out_pages);
+  const Paged s{batch, 0, kv_heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, FHOG_DTYPE_BF16, cache_dtype};
+  if (int st = check_ptrs(who, {{"k_cache", k_cache}, {"v_cache", v_cache}, {"k_out", k_out}, {"v_out", v_out}}, {}))
+    return st;
+  if (batch > 0)
+    if (int st = check_ptrs(who, {}, {{"page_table", page_table}, {"lengths", lengths}, {"table_out", table_out}})) return st;
+  if (cache_dtype == FHOG_DTYPE_E4M3)
+    if (int st = check_ptrs(who, {{"k_scale", k_scale}, {"v_scale", v_scale}, {"k_scale_out", k_scale_out},
+                                  {"v_scale_out", v_scale_out}}, {}))
+      return st;
+  if ((key_means != nullptr) != (means_out != nullptr))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: key_means and means_out go together", who);
+  if (key_means != nullptr)
+    if (int st = check_ptrs(who, {{"key_means", key_means}, {"means_out", means_out}}, {})) return st;
+  if (int st = check_pages_workspace(who, workspace, workspace_bytes, batch, num_pages, pages_per_seq)) return st;
+  fhog::PagesParams p{const_cast<int*>(page_table), const_cast<int*>(lengths), nullptr, nullptr, 0, batch, pages_per_seq,
+                      num_pages, __builtin_ctz((unsigned)page_size), kv_heads, 1};
+  fhog::pages_workspace(p, (int*)workspace);
+  return launch_status(fhog::launch_pages_compact(
+      p, page_bytes(k_cache, v_cache, k_scale, v_scale, key_means, head_dim, page_size, cache_dtype),
+      page_bytes(k_out, v_out, k_scale_out, v_scale_out, means_out, head_dim, page_size, cache_dtype), out_pages,
+      table_out, (hipStream_t)stream), who);
 }
 
 }  // extern "C"

@@ -1,0 +1,66 @@
+// The paged cache's allocator: parameter blocks and the split of its work (fhog_pages.hip).
+#pragma once
+
+#include "fhog_paged.h"
+
+namespace fhog {
+
+// A cache as bytes: page p of tensor i is rows [p * kv_heads, (p + 1) * kv_heads) of `row` bytes.
+struct PageBytes {
+  char* at[5];    // keys, values, their scales, key means; null: none
+  int row[5];     // bytes of one head in a page
+  int token[5];   // bytes of one token of one head (0: not by token)
+};
+
+struct PagesParams {
+  int* table;  // (batch, width)
+  int* lengths;
+  const int* parents;     // null: each row its own
+  const int* new_tokens;  // null: new_each
+  int new_each;
+  int batch, width, pages, page_shift, kv_heads;
+  int list_used;  // whether the used pages are listed instead of the free ones
+  // workspace
+  int* state;      // (pages) PageState, where LDS is too small
+  int* listed;     // (pages) the free (used) pages, lowest first
+  int* place;      // (pages) a used page's place in that list (list_used)
+  int* entries;    // (batch, width) the rows' entries before they grow (with parents)
+  int* held;       // (batch) lengths before
+  int* begin;      // (batch) first column that gets a new page
+  int* first;      // (batch) how many new pages the rows before get
+  int* source;     // (batch) page to copy to the first new one, or -1
+  int* chunks;     // listed pages before each chunk of kPageChunk
+  int* totals;     // [0] pages listed, [1] pages asked for
+};
+
+constexpr int kPageChunk = 4096;
+// Up to this many pages and entries one workgroup does the bookkeeping, with the pages' states in LDS: six
+// launches become two. (128 rows of 34 entries, 556 pages.)
+constexpr int kFewPages = 32768, kFewEntries = 1 << 17, kFewRows = 1 << 14;
+inline bool few_pages(int batch, int width, int pages) {
+  return pages <= kFewPages && (long)batch * width <= kFewEntries && batch <= kFewRows;
+}
+inline long pages_workspace_ints(int batch, int width, int pages) {
+  return 3l * pages + (long)batch * width + 4l * batch + pages / kPageChunk + 2 + 2;
+}
+inline void pages_workspace(PagesParams& p, int* ws) {
+  p.totals = ws;
+  p.listed = p.totals + 2;
+  p.state = p.listed + p.pages;
+  p.place = p.state + p.pages;
+  p.held = p.place + p.pages;
+  p.begin = p.held + p.batch;
+  p.first = p.begin + p.batch;
+  p.source = p.first + p.batch;
+  p.chunks = p.source + p.batch;
+  p.entries = p.chunks + p.pages / kPageChunk + 2;
+}
+
+// Extends the rows and copies the shared pages' held rows; *free_pages = free pages left, less those that
+// were lacking.
+hipError_t launch_pages_extend(const PagesParams& p, const PageBytes& cache, int* free_pages, hipStream_t s);
+// The used pages to the front of `out`, of out_pages pages, zeros behind; the table for it to table_out.
+hipError_t launch_pages_compact(const PagesParams& p, const PageBytes& cache, const PageBytes& out, int out_pages,
+                                int* table_out, hipStream_t s);
+
+}  // namespace fhog

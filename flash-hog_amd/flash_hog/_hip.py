@@ -62,6 +62,9 @@ SIGNATURES = {
     "fhog_paged_attention": (_i, [_p] * 11 + [ctypes.c_size_t] + [_i] * 13 + [_f]),
     "fhog_paged_cache_write": (_i, [_p] * 10 + [_i] * 9),
     "fhog_paged_cache_read": (_i, [_p] * 9 + [_i] * 9),
+    "fhog_paged_pages_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
+    "fhog_paged_cache_extend": (_i, [_p] * 9 + [_i, _p, _p, ctypes.c_size_t] + [_i] * 7),
+    "fhog_paged_cache_compact": (_i, [_p] * 15 + [ctypes.c_size_t] + [_i] * 8),
     "fhog_qk_norm_rotary_workspace_bytes": (ctypes.c_size_t, [_p]),
     "fhog_qk_norm_rotary_fwd": (_i, [_p] * 8),
     "fhog_qk_norm_rotary_bwd": (_i, [_p] * 13),
@@ -526,6 +529,73 @@ def paged_cache_read(k_cache, v_cache, page_table, lengths, max_length: int, dty
             _ptr(lengths), _ptr(k), _ptr(v), B, max_length, Nk, Hd, pages, page, width, DTYPE_CODES[dtype],
             CACHE_DTYPE_CODES[k_cache.dtype]))
     return k, v
+
+
+def _overlap(a, b) -> bool:
+    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
+
+
+def paged_cache_extend(k_cache, v_cache, page_table, lengths, new_tokens, new_each: int, parents, k_scale, v_scale):
+    """Rows of page_table and lengths go on from their parents and grow by new_tokens (None: new_each) tokens,
+    in place (fhog_paged_cache_extend); returns the free pages left, an int32 tensor of no axes."""
+    (pages, Nk, page, Hd, B, width), _, _, _ = _check_cache(
+        ("key_cache", k_cache), k_cache, v_cache, page_table, lengths, None, k_scale, v_scale, k_cache.dtype)
+    if k_cache.dtype not in CACHE_DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {k_cache.dtype}")
+    for name, t in (("page_table", page_table), ("lengths", lengths)):
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    for name, t in (("parents", parents), ("new_tokens", new_tokens)):
+        if t is None:
+            continue
+        _check_inputs([("key_cache", k_cache), (name, t)])
+        _expect(name, t, (B,), torch.int32)
+        if _overlap(t, page_table) or _overlap(t, lengths):
+            raise ValueError(f"{name} overlaps page_table or lengths")
+    if B == 0:
+        raise ValueError("expected at least one row of page_table")
+    parents, new_tokens = (None if t is None else t.contiguous() for t in (parents, new_tokens))
+    free = torch.empty((), device=k_cache.device, dtype=torch.int32)
+    with _on_device(k_cache.device):
+        size = lib().fhog_paged_pages_workspace_bytes(B, pages, width)
+        ws = torch.empty(size, device=k_cache.device, dtype=torch.uint8)
+        check(lib().fhog_paged_cache_extend(
+            _stream(k_cache.device), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(page_table),
+            _ptr(lengths), _ptr(parents), _ptr(new_tokens), new_each, _ptr(free), _ptr(ws), size, B, Nk, Hd, pages, page,
+            width, CACHE_DTYPE_CODES[k_cache.dtype]))
+    _written(k_cache, v_cache, k_scale, v_scale, page_table, lengths)
+    return free
+
+
+def paged_cache_compact(k_cache, v_cache, page_table, lengths, num_pages: int, k_scale, v_scale, key_means):
+    """(k_cache, v_cache, k_scale, v_scale, key_means, page_table): the used pages as the first of new caches
+    of num_pages pages (fhog_paged_cache_compact); None for what is not given."""
+    (pages, Nk, page, Hd, B, width), page_table, lengths, _ = _check_cache(
+        ("key_cache", k_cache), k_cache, v_cache, page_table, lengths, None, k_scale, v_scale, k_cache.dtype)
+    if k_cache.dtype not in CACHE_DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {k_cache.dtype}")
+    if key_means is not None:
+        _check_key_means(key_means, ("key_cache", k_cache), (pages, Nk, Hd))
+    if num_pages < 1 or num_pages > (1 << 31) - 1:
+        raise ValueError(f"num_pages must be >= 1 and below 2 ** 31, got {num_pages}")
+    inputs = (k_cache, v_cache, k_scale, v_scale, key_means)
+    outs = tuple(None if t is None else torch.empty((num_pages, *t.shape[1:]), device=t.device, dtype=t.dtype)
+                 for t in inputs)
+    table = torch.empty_like(page_table)
+    with _on_device(k_cache.device):
+        size = lib().fhog_paged_pages_workspace_bytes(B, pages, width)
+        ws = torch.empty(size, device=k_cache.device, dtype=torch.uint8)
+        check(lib().fhog_paged_cache_compact(
+            _stream(k_cache.device), *map(_ptr, inputs), _ptr(page_table), _ptr(lengths), *map(_ptr, outs), _ptr(table),
+            _ptr(ws), size, B, Nk, Hd, pages, page, width, num_pages, CACHE_DTYPE_CODES[k_cache.dtype]))
+    return (*outs, table)
+
+
+def _check_key_means(means, first, shape):
+    _check_inputs([first, ("key_means", means)])
+    _expect("key_means", means, shape, torch.float32)
+    if not means.is_contiguous():
+        raise ValueError("key_means must be contiguous")
 
 
 # ------------------------------------------------- norms with rotation

@@ -6,8 +6,11 @@
                       one token each (decoding) or chunks of unequal length (prompts), with the
                       window and sinks of dot_product_attention
   paged_cache_read    cached sequences back as dense tensors, as dot_product_attention takes them
+  paged_cache_extend  the cache's allocator: sequences fork, end and grow, pages are handed out and copied
+                      where rows that share one part ways
+  paged_cache_compact the used pages to the front of a cache of another size
 
-No counterpart in the reference, which trains only. All three enqueue their kernels on the
+No counterpart in the reference, which trains only. All enqueue their kernels on the
 current stream of the tensors' device, read no length back to the host, and can be captured in
 a HIP graph; workspaces come from torch's allocator, a new one for each call.
 
@@ -82,6 +85,35 @@ def _checked(name, index, *tensors) -> bool:
                                "already")
         through = through or any(map(torch._C._functorch.is_functorch_wrapped_tensor, ours))
     return through
+
+
+@torch.library.custom_op("flash_hog::paged_cache_extend",
+                         mutates_args=("key_cache", "value_cache", "page_table", "lengths", "key_scale", "value_scale"))
+def paged_cache_extend_op(key_cache: Tensor, value_cache: Tensor, page_table: Tensor, lengths: Tensor,
+                          new_tokens: Tensor | None, new_each: int, parents: Tensor | None, key_scale: Tensor | None,
+                          value_scale: Tensor | None) -> Tensor:
+    return _hip.paged_cache_extend(key_cache, value_cache, page_table, lengths, new_tokens, new_each, parents, key_scale,
+                                   value_scale)
+
+
+@paged_cache_extend_op.register_fake
+def _(key_cache, value_cache, page_table, lengths, new_tokens, new_each, parents, key_scale, value_scale):
+    return lengths.new_empty((), dtype=torch.int32)
+
+
+@torch.library.custom_op("flash_hog::paged_cache_compact", mutates_args=())
+def paged_cache_compact_op(key_cache: Tensor, value_cache: Tensor, page_table: Tensor, lengths: Tensor, num_pages: int,
+                           key_scale: Tensor | None, value_scale: Tensor | None,
+                           key_means: Tensor | None) -> list[Tensor]:
+    got = _hip.paged_cache_compact(key_cache, value_cache, page_table, lengths, num_pages, key_scale, value_scale,
+                                   key_means)
+    return [t for t in got if t is not None]
+
+
+@paged_cache_compact_op.register_fake
+def _(key_cache, value_cache, page_table, lengths, num_pages, key_scale, value_scale, key_means):
+    pools = [t for t in (key_cache, value_cache, key_scale, value_scale, key_means) if t is not None]
+    return [t.new_empty((num_pages, *t.shape[1:])) for t in pools] + [torch.empty_like(page_table)]
 
 
 @torch.library.custom_op("flash_hog::paged_attention", mutates_args=())
@@ -185,3 +217,53 @@ def paged_cache_read(key_cache, value_cache, page_table, lengths, *, max_length:
         max_length = page_table.shape[1] * key_cache.shape[2]
     call = paged_cache_read_op if through else _hip.paged_cache_read
     return call(key_cache, value_cache, page_table, lengths, max_length, dtype, key_scale, value_scale)
+
+
+def paged_cache_extend(key_cache, value_cache, page_table, lengths, new_tokens, parents=None, *, key_scale=None,
+                       value_scale=None):
+    """The cache's allocator: in place, every row of page_table and lengths becomes that of its parent and
+    then has room for its new tokens, which paged_cache_write fills next.
+
+    The table and the lengths are the allocator's only state: a page is used if a row has it among its first
+    ceil(length / page_size) entries, and free otherwise. So a sequence ends by its length becoming 0, tokens are
+    taken back by a smaller length, and a prefix that is kept for later is a row of its own.
+
+    new_tokens: how many each row grows by, an int or (batch,) int32 (below 0 counts as 0). parents (batch,)
+    int32: row b goes on from row parents[b] as it was before the call (a fork if several name the
+    same, an empty row for an index outside the batch); None: each from itself.
+
+    A row that grows within its last page must have that page for itself. If other rows use it, one that all others
+    grow in too goes on with the row of lowest index; else, and for the others, the tokens held in it are copied to
+    a new page. New pages are the free ones, lowest first, to the rows in order. Entries behind a row's last page
+    become -1, and so do those that no page was left for (their tokens are not written, and attention
+    to them gives NaN).
+
+    Returns the number of free pages left, less those that were lacking, as an int32 tensor of no axes."""
+    index = (page_table, lengths, parents) + ((new_tokens,) if isinstance(new_tokens, Tensor) else ())
+    through = _checked("paged_cache_extend", index, key_cache, value_cache, key_scale, value_scale)
+    if isinstance(new_tokens, Tensor):
+        new, each = new_tokens, 0
+    else:
+        new, each = None, operator.index(new_tokens)
+        if each < 0 or each >= 1 << 31:
+            raise ValueError(f"new_tokens must be >= 0 and below 2 ** 31, got {each}")
+    call = paged_cache_extend_op if through else _hip.paged_cache_extend
+    return call(key_cache, value_cache, page_table, lengths, new, each, parents, key_scale, value_scale)
+
+
+def paged_cache_compact(key_cache, value_cache, page_table, lengths, *, num_pages: int | None = None, key_scale=None,
+                        value_scale=None, key_means=None):
+    """The used pages (paged_cache_extend), in their order, as the first pages of a new cache of num_pages pages
+    (default: as many as now; zero bytes behind the used ones), for a pool that is to grow or to shrink.
+    Returns (key_cache, value_cache, key_scale, value_scale, key_means, page_table), None for what was not
+    given; entries of the table that name no page, and used ones beyond num_pages, are -1. Pages that rows
+    share stay shared."""
+    through = _checked("paged_cache_compact", (page_table, lengths), key_cache, value_cache, key_scale, value_scale,
+                       key_means)
+    num_pages = key_cache.shape[0] if num_pages is None else operator.index(num_pages)
+    args = (key_cache, value_cache, page_table, lengths, num_pages, key_scale, value_scale, key_means)
+    if not through:
+        return _hip.paged_cache_compact(*args)
+    got = iter(paged_cache_compact_op(*args))
+    return (*(None if t is None else next(got) for t in (key_cache, value_cache, key_scale, value_scale, key_means)),
+            next(got))

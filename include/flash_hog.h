@@ -285,6 +285,38 @@ int fhog_paged_cache_read(fhog_stream_t stream, const void* k_cache, const void*
                           int pages_per_seq, int dtype, int cache_dtype);
 
 /*
+ * The cache's allocator. The page table and the lengths are its only state: a page is used if a row of the
+ * table has it among its first ceil(length / page_size) entries (those in [0, num_pages)), else free.
+ *
+ * extend: in place and in one step for all rows, row b becomes row parents[b] (null: each its own; an
+ * index outside [0, batch): an empty row) and then grows by max(0, new_tokens[b]) tokens (null:
+ * new_each). If its last page is not full and it grows, that page becomes its own: it keeps it if all other
+ * users are rows of higher index that grow in it as well, else the rows held in it are copied (keys,
+ * values, scales) to a new page. New pages are the free ones (by the rows' state after parents), lowest
+ * first, to the rows in order, each row's columns in order. Entries behind a row's last page become -1, and so do
+ * those that no page was left for; *free_pages (device memory) = the free pages that are left, less
+ * those that were lacking. A length may grow beyond its table, and past 2^31 - 1 it stays there.
+ * parents, new_tokens (batch) int32. k_scale, v_scale: of an e4m3 cache.
+ */
+size_t fhog_paged_pages_workspace_bytes(int batch, int num_pages, int pages_per_seq);
+
+int fhog_paged_cache_extend(fhog_stream_t stream, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                            int* page_table, int* lengths, const int* parents, const int* new_tokens, int new_each,
+                            int* free_pages, void* workspace, size_t workspace_bytes, int batch, int kv_heads,
+                            int head_dim, int num_pages, int page_size, int pages_per_seq, int cache_dtype);
+
+/* The used pages, in their order, as the first pages of another cache of out_pages pages (zero bytes behind them),
+ * and the table (batch, pages_per_seq) for it: -1 where there is no page, and for used ones that out_pages
+ * has no room for. key_means, means_out: fhog_paged_key_means' of both, or null. All tensors 16-byte
+ * aligned, the outputs apart from the inputs. */
+int fhog_paged_cache_compact(fhog_stream_t stream, const void* k_cache, const void* v_cache, const void* k_scale,
+                             const void* v_scale, const float* key_means, const int* page_table, const int* lengths,
+                             void* k_out, void* v_out, void* k_scale_out, void* v_scale_out, float* means_out,
+                             int* table_out, void* workspace, size_t workspace_bytes, int batch, int kv_heads,
+                             int head_dim, int num_pages, int page_size, int pages_per_seq, int out_pages,
+                             int cache_dtype);
+
+/*
  * Norms of queries and keys for each head with the position rotation, and their derivatives (no
  * counterpart in the reference): what stands before the attention of either kind.
  *
