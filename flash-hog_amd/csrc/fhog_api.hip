@@ -15,6 +15,7 @@
 #include "fhog_params.h"
 #include "fhog_paged.h"
 #include "fhog_pages.h"
+#include "fhog_blocks.h"
 #include "fhog_rotary.h"
 
 namespace {
@@ -875,6 +876,148 @@ int fhog_paged_cache_compact(fhog_stream_t stream, const void* k_cache, const vo
       p, page_bytes(k_cache, v_cache, k_scale, v_scale, key_means, head_dim, page_size, cache_dtype),
       page_bytes(k_out, v_out, k_scale_out, v_scale_out, means_out, head_dim, page_size, cache_dtype), out_pages,
       table_out, (hipStream_t)stream), who);
+}
+
+}  // extern "C"
+
+namespace {
+
+// What tokens over chosen blocks share: the cache's sizes, and the offsets.
+int check_tokens(const char* who, const Paged& s, const int* query_offsets) {
+  if (query_offsets == nullptr && s.rows != s.batch)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: without query_offsets there is one row a sequence: %d rows, %d sequences",
+                who, s.rows, s.batch);
+  if (query_offsets != nullptr && !aligned(query_offsets, 4))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: query_offsets is not 4-byte aligned", who);
+  return FHOG_OK;
+}
+int check_blocks(const char* who, const Paged& s, int blocks) {
+  if (blocks < 1) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: blocks must be >= 1, got %d", who, blocks);
+  // (a split's blocks are listed in LDS, and a join's splits)
+  if (blocks > 32768 || (long long)blocks * s.page_size > (1ll << 30))
+    return fail(FHOG_ERR_UNSUPPORTED, "%s: blocks must be <= 32768 and hold at most 2^30 keys, got %d", who, blocks);
+  return FHOG_OK;
+}
+template <typename F> hipError_t dispatch_dim(int head_dim, F&& f) {
+  if (head_dim == 64) return f.template operator()<64>();
+  if (head_dim == 128) return f.template operator()<128>();
+  return f.template operator()<256>();
+}
+
+}  // namespace
+
+extern "C" {
+
+int fhog_paged_key_means(fhog_stream_t stream, const void* k_cache, const void* k_scale, float* key_means,
+                         const int* page_table, const int* lengths, const int* query_offsets, int batch, int kv_heads,
+                         int head_dim, int num_pages, int page_size, int pages_per_seq, int cache_dtype) {
+  static const char* who = "fhog_paged_key_means";
+  const int dtype = cache_dtype == FHOG_DTYPE_E4M3 ? (int)FHOG_DTYPE_BF16 : cache_dtype;
+  const Paged s{batch, 0, kv_heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype};
+  if (int st = check_paged(s, who)) return st;
+  if (query_offsets != nullptr && !aligned(query_offsets, 4))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: query_offsets is not 4-byte aligned", who);
+  if (batch == 0) return ok();
+  if (int st = check_cache(who, s, k_cache, k_cache, k_scale, k_scale, page_table, lengths)) return st;
+  if (int st = check_ptrs(who, {}, {{"key_means", key_means}})) return st;
+  // How many pages the tokens fill only the device knows; single tokens fill one each at most.
+  const long long most = (long long)batch * (query_offsets != nullptr ? pages_per_seq : 1) * kv_heads;
+  const long long fill = 8ll * (compute_units() > 0 ? compute_units() : 256);
+  const int workgroups = (int)(most < fill ? most : fill);
+  fhog::CacheShape at = cache_shape(s, page_table, lengths, query_offsets);
+  at.total = 0x7fffffff;
+  auto run = [&]<typename C>() {
+    return dispatch_dim(head_dim, [&]<int D>() {
+      return fhog::launch_key_means<C, D>({(const C*)k_cache, (const uint8_t*)k_scale, key_means, at}, workgroups,
+                                          (hipStream_t)stream);
+    });
+  };
+  return launch_status(cache_dtype == FHOG_DTYPE_E4M3  ? run.template operator()<fhog::e4m3>()
+                       : cache_dtype == FHOG_DTYPE_F16 ? run.template operator()<_Float16>()
+                                                       : run.template operator()<__bf16>(),
+                       who);
+}
+
+size_t fhog_paged_block_select_workspace_bytes(int total, int kv_heads, int pages_per_seq) {
+  if (total < 1 || kv_heads < 1 || pages_per_seq < 1) return 0;
+  return (size_t)fhog::select_slab(total, kv_heads, pages_per_seq) * kv_heads * pages_per_seq * sizeof(double);
+}
+
+int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* key_means, const int* page_table,
+                            const int* lengths, const int* query_offsets, int* chosen, void* workspace,
+                            size_t workspace_bytes, int batch, int total, int heads, int kv_heads, int head_dim,
+                            int num_pages, int page_size, int pages_per_seq, int dtype, int blocks, int first, int last) {
+  static const char* who = "fhog_paged_block_select";
+  const Paged s{batch, total, heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, dtype};
+  if (int st = check_paged(s, who)) return st;
+  if (int st = check_tokens(who, s, query_offsets)) return st;
+  if (int st = check_blocks(who, s, blocks)) return st;
+  if (first < 0 || last < 1 || (long long)first + last > blocks)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: needs first >= 0, last >= 1 and first + last <= blocks, got %d, %d and %d",
+                who, first, last, blocks);
+  if (total == 0) return ok();
+  if (batch == 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: rows without a sequence", who);
+  if (pages_per_seq > (1 << 21) || kv_heads > (1 << 16) || (double)total * kv_heads * blocks >= kMostElements)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  if (int st = check_ptrs(who, {{"q", q}, {"key_means", key_means}},
+                          {{"page_table", page_table}, {"lengths", lengths}, {"chosen", chosen}}))
+    return st;
+  const size_t need = fhog_paged_block_select_workspace_bytes(total, kv_heads, pages_per_seq);
+  if (!aligned(workspace, 8) || workspace_bytes < need)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null, not 8-byte aligned or below its %zu bytes", who, need);
+  auto run = [&]<typename T>() {
+    return dispatch_dim(head_dim, [&]<int D>() {
+      fhog::BlockSelectParams<T> p{(const T*)q, key_means, chosen, cache_shape(s, page_table, lengths, query_offsets),
+                                   (double*)workspace, heads, blocks, first, last, 0,
+                                   fhog::select_slab(total, kv_heads, pages_per_seq)};
+      return fhog::launch_block_select<T, D>(p, (hipStream_t)stream);
+    });
+  };
+  return launch_status(dtype == FHOG_DTYPE_BF16 ? run.template operator()<__bf16>() : run.template operator()<_Float16>(),
+                       who);
+}
+
+size_t fhog_paged_block_workspace_bytes(int total, int heads, int kv_heads, int head_dim, int page_size, int blocks) {
+  static const char* who = "fhog_paged_block_workspace_bytes";
+  const Paged s{1, total, heads, kv_heads, head_dim, 1, page_size, 1, FHOG_DTYPE_BF16, FHOG_DTYPE_BF16};
+  if (check_paged(s, who) || check_blocks(who, s, blocks) || total < 1) return 0;
+  const fhog::BlockPlan plan = fhog::block_plan(total, heads, kv_heads, head_dim, page_size, blocks, compute_units());
+  return (size_t)plan.parts * (head_dim + 2) * sizeof(float);
+}
+
+int fhog_paged_block_attention(fhog_stream_t stream, const void* q, const int* chosen, const void* k_cache,
+                               const void* v_cache, const void* k_scale, const void* v_scale, const int* page_table,
+                               const int* lengths, const int* query_offsets, void* out, void* workspace,
+                               size_t workspace_bytes, int batch, int total, int heads, int kv_heads, int head_dim,
+                               int num_pages, int page_size, int pages_per_seq, int dtype, int cache_dtype, int blocks,
+                               int clear_rest, float scale) {
+  static const char* who = "fhog_paged_block_attention";
+  const Paged s{batch, total, heads, kv_heads, head_dim, num_pages, page_size, pages_per_seq, dtype, cache_dtype};
+  if (int st = check_paged(s, who)) return st;
+  if (!(scale == scale) || scale - scale != 0.0f)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: scale must be finite", who);
+  if (scale == 0.0f) return fail(FHOG_ERR_UNSUPPORTED, "%s: scale must be nonzero", who);
+  if (int st = check_tokens(who, s, query_offsets)) return st;
+  if (int st = check_blocks(who, s, blocks)) return st;
+  if (total == 0) return ok();
+  if (batch == 0) return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: rows without a sequence", who);
+  if (int st = check_ptrs(who, {{"q", q}, {"out", out}}, {{"chosen", chosen}})) return st;
+  if (int st = check_cache(who, s, k_cache, v_cache, k_scale, v_scale, page_table, lengths)) return st;
+  const long long tiles = (long long)total * ((heads / kv_heads + 15) / 16);
+  if (tiles * kv_heads >= (1ll << 23) || (double)total * kv_heads * blocks >= kMostElements)
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
+  const fhog::BlockPlan plan = fhog::block_plan(total, heads, kv_heads, head_dim, page_size, blocks, compute_units());
+  const size_t need = (size_t)plan.parts * (head_dim + 2) * sizeof(float);
+  if (need > 0 && (!aligned(workspace, 16) || workspace_bytes < need))
+    return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null, not 16-byte aligned or below its %zu bytes", who, need);
+  auto run = [&]<typename T, typename C, int D>() {
+    fhog::BlockParams<T, C> p{(const T*)q, (T*)out,
+                              {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
+                              cache_shape(s, page_table, lengths, query_offsets), chosen, (float*)workspace, heads, blocks,
+                              plan.slots, plan.splits, plan.split_tiles, clear_rest, scale};
+    return fhog::launch_block_attention<T, C, D>(p, (hipStream_t)stream);
+  };
+  return launch_status(dispatch_paged(s, run), who);
 }
 
 }  // extern "C"

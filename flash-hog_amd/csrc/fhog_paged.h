@@ -108,6 +108,36 @@ __device__ __forceinline__ int wave_sum(int x) {
   return __builtin_amdgcn_readlane(x, 63);
 }
 
+// A lane's sum over the lanes before it, and in `total` the wave's.
+__device__ __forceinline__ int wave_scan(int x, int& total) {
+  const int lane = threadIdx.x & 63;
+  int through = x;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(through, d, 64);
+    if (lane >= d) through += y;
+  }
+  total = __shfl(through, 63, 64);
+  return through - x;
+}
+
+// The same over the threads of a workgroup of THREADS; box: an int a wave, in LDS.
+template <int THREADS> __device__ __forceinline__ int group_scan(int x, int& total, int* box) {
+  const int wave = threadIdx.x >> 6;
+  int sum;
+  const int before = wave_scan(x, sum);
+  __syncthreads();  // (the box's last use)
+  if ((threadIdx.x & 63) == 0) box[wave] = sum;
+  __syncthreads();
+  int more = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < wave) more += box[w];
+    total += box[w];
+  }
+  return before + more;
+}
+
 // Sequence and tile (of ROWS rows) that come at place `order` when all tiles are sorted by the keys
 // that their last rows see, most first, then by sequence: at most 64 sequences, one a lane. False
 // behind the last tile.
@@ -178,6 +208,16 @@ template <typename T> __device__ __forceinline__ V4<T> dequantise4(uint32_t x, f
 // The power of two that an e8m0 code stands for.
 __device__ __forceinline__ float scale_of(uint32_t code) { return __builtin_bit_cast(float, code << 23); }
 
+// Where a tile's two halves of 16 keys lie: the line (row of a head of a page) of each half's first key, and
+// the last of its rows that is read (the others repeat it, so that what no token has written is never read).
+struct HalfRows {
+  long line[2];
+  int last[2];
+  __device__ __forceinline__ long of(int row) const {
+    return (row < 16 ? line[0] : line[1]) + min(row & 15, row < 16 ? last[0] : last[1]);
+  }
+};
+
 // TENSORS: 2 for keys and values, 1 for values alone.
 template <typename T, typename C, int D, int THREADS, int SWZ, int TENSORS = 2> struct PageTile {
   static constexpr bool kQuantised = sizeof(C) == 1;
@@ -203,6 +243,18 @@ template <typename T, typename C, int D, int THREADS, int SWZ, int TENSORS = 2> 
       const int row = min(max(at % kTensor / kChunks, rlo), rhi);
       const long head = (long)(row < 16 ? page0 : page1) * kv_heads + hk;
       const long line = (head << page_shift) + ((k0 + row) & (page_rows - 1));
+      const C* src = (value ? cache.v : cache.k) + line * D + at % kChunks * kPerLoad;
+      data[i] = *reinterpret_cast<const u32x4*>(src);
+      if constexpr (kQuantised) code[i] = (value ? cache.v_scale : cache.k_scale)[line];
+    }
+  }
+
+  __device__ __forceinline__ void fetch(const CacheRows<C>& cache, const HalfRows& rows, int thread) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * THREADS + thread;
+      const bool value = TENSORS == 1 || at >= kTensor;
+      const long line = rows.of(at % kTensor / kChunks);
       const C* src = (value ? cache.v : cache.k) + line * D + at % kChunks * kPerLoad;
       data[i] = *reinterpret_cast<const u32x4*>(src);
       if constexpr (kQuantised) code[i] = (value ? cache.v_scale : cache.k_scale)[line];
@@ -319,6 +371,17 @@ template <typename T, typename C, int D> struct KeyPieces {
       const int row = min(max(16 * kb + n, rlo), rhi);  // (PageTile::fetch)
       const long head = (long)(row < 16 ? page0 : page1) * kv_heads + hk;
       const long line = (head << page_shift) + ((k0 + row) & (page_rows - 1));
+      const C* src = cache.k + line * D + g * (kQuantised ? 16 : 8);
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c)
+        data[kb][c] = *reinterpret_cast<const u32x4*>(src + c * (kQuantised ? 64 : 32));
+      if constexpr (kQuantised) code[kb] = cache.k_scale[line];
+    }
+  }
+  __device__ __forceinline__ void fetch(const CacheRows<C>& cache, const HalfRows& rows, int n, int g) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const long line = rows.of(16 * kb + n);
       const C* src = cache.k + line * D + g * (kQuantised ? 16 : 8);
 #pragma unroll
       for (int c = 0; c < kPieces; ++c)

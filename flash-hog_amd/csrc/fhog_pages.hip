@@ -65,36 +65,6 @@ __device__ __forceinline__ int ask(const PagesParams& p, const int* state, int b
   return max(0, row.end(p) - begin);
 }
 
-// A wave's running sum over its lanes, and the total.
-__device__ __forceinline__ int wave_scan(int x, int& total) {
-  const int lane = threadIdx.x & 63;
-  int through = x;
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(through, d, 64);
-    if (lane >= d) through += y;
-  }
-  total = __shfl(through, 63, 64);
-  return through - x;
-}
-
-// The sum of x over the threads before this one, of a workgroup of THREADS; the total in `total`.
-template <int THREADS> __device__ __forceinline__ int group_scan(int x, int& total, int* box) {
-  const int wave = threadIdx.x >> 6;
-  int sum;
-  const int before = wave_scan(x, sum);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) box[wave] = sum;
-  __syncthreads();
-  int more = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w < wave) more += box[w];
-    total += box[w];
-  }
-  return before + more;
-}
-
 __device__ __forceinline__ bool is_listed(const PagesParams& p, int state) { return (state == kFree) != (p.list_used != 0); }
 
 // Lists pages [from, to), `first` of which come before; by one wave.

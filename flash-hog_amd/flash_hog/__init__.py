@@ -9,9 +9,10 @@ through the C ABI in include/flash_hog.h.
 from flash_hog._types import MaskType, TuningConfig
 from flash_hog.torch._hip_gpu import supported
 from flash_hog.torch.attention import dot_product_attention
-from flash_hog.torch.paged import (paged_attention, paged_cache_compact, paged_cache_extend, paged_cache_read,
-                                   paged_cache_write)
+from flash_hog.torch.paged import (paged_attention, paged_block_attention, paged_block_select, paged_cache_compact,
+                                   paged_cache_extend, paged_cache_read, paged_cache_write, paged_key_means)
 from flash_hog.torch.rotary import qk_norm_rotary
 
-__all__ = ["MaskType", "TuningConfig", "dot_product_attention", "paged_attention", "paged_cache_compact",
-           "paged_cache_extend", "paged_cache_read", "paged_cache_write", "qk_norm_rotary", "supported"]
+__all__ = ["MaskType", "TuningConfig", "dot_product_attention", "paged_attention", "paged_block_attention",
+           "paged_block_select", "paged_cache_compact", "paged_cache_extend", "paged_cache_read", "paged_cache_write",
+           "paged_key_means", "qk_norm_rotary", "supported"]

@@ -65,6 +65,11 @@ SIGNATURES = {
     "fhog_paged_pages_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
     "fhog_paged_cache_extend": (_i, [_p] * 9 + [_i, _p, _p, ctypes.c_size_t] + [_i] * 7),
     "fhog_paged_cache_compact": (_i, [_p] * 15 + [ctypes.c_size_t] + [_i] * 8),
+    "fhog_paged_key_means": (_i, [_p] * 7 + [_i] * 7),
+    "fhog_paged_block_select_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
+    "fhog_paged_block_select": (_i, [_p] * 8 + [ctypes.c_size_t] + [_i] * 12),
+    "fhog_paged_block_workspace_bytes": (ctypes.c_size_t, [_i] * 6),
+    "fhog_paged_block_attention": (_i, [_p] * 12 + [ctypes.c_size_t] + [_i] * 12 + [_f]),
     "fhog_qk_norm_rotary_workspace_bytes": (ctypes.c_size_t, [_p]),
     "fhog_qk_norm_rotary_fwd": (_i, [_p] * 8),
     "fhog_qk_norm_rotary_bwd": (_i, [_p] * 13),
@@ -596,6 +601,108 @@ def _check_key_means(means, first, shape):
     _expect("key_means", means, shape, torch.float32)
     if not means.is_contiguous():
         raise ValueError("key_means must be contiguous")
+
+
+def _check_index(first, page_table, lengths, query_offsets):
+    """_check_cache's checks of what finds tokens; the contiguous tensors."""
+    named = [("page_table", page_table), ("lengths", lengths)]
+    if query_offsets is not None:
+        named.append(("query_offsets", query_offsets))
+    _check_inputs([first, *named])
+    if page_table.ndim != 2:
+        raise ValueError(f"expected a (batch, pages) page_table, got {tuple(page_table.shape)}")
+    _expect("lengths", lengths, (page_table.shape[0],))
+    if query_offsets is not None:
+        _expect("query_offsets", query_offsets, (page_table.shape[0] + 1,))
+    for name, t in named:
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name} has dtype {t.dtype}, expected torch.int32")
+    return tuple(None if t is None else t.contiguous() for t in (page_table, lengths, query_offsets))
+
+
+def paged_key_means(k_cache, key_means, page_table, lengths, query_offsets, k_scale) -> None:
+    """The means of the pages that the new tokens fill, into key_means (fhog_paged_key_means)."""
+    (pages, Nk, page, Hd, B, width), page_table, lengths, query_offsets = _check_cache(
+        ("key_cache", k_cache), k_cache, k_cache, page_table, lengths, query_offsets, k_scale, k_scale, k_cache.dtype)
+    if k_cache.dtype not in CACHE_DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {k_cache.dtype}")
+    _check_key_means(key_means, ("key_cache", k_cache), (pages, Nk, Hd))
+    if _overlap(key_means, k_cache):
+        raise ValueError("key_means overlaps key_cache")
+    with _on_device(k_cache.device):
+        check(lib().fhog_paged_key_means(
+            _stream(k_cache.device), _ptr(k_cache), _ptr(k_scale), _ptr(key_means), _ptr(page_table), _ptr(lengths),
+            _ptr(query_offsets), B, Nk, Hd, pages, page, width, CACHE_DTYPE_CODES[k_cache.dtype]))
+    _written(key_means)
+
+
+def paged_block_select(q, key_means, page_table, lengths, query_offsets, page_size: int, blocks: int, first: int,
+                       last: int):
+    """(T, N_kv, blocks) int32, the columns that each new token attends to (fhog_paged_block_select)."""
+    if q.ndim != 3:
+        raise ValueError(f"expected a (T, N, H) query, got {tuple(q.shape)}")
+    if key_means.ndim != 3 or key_means.shape[2] != q.shape[2]:
+        raise ValueError(f"expected (pages, kv_heads, head_dim) key_means for query{tuple(q.shape)}, got {tuple(key_means.shape)}")
+    _check_key_means(key_means, ("query", q), key_means.shape)
+    page_table, lengths, query_offsets = _check_index(("query", q), page_table, lengths, query_offsets)
+    if q.dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {q.dtype}")
+    T, N, Hd = q.shape
+    pages, Nk, _ = key_means.shape
+    B, width = page_table.shape
+    q = q.contiguous()
+    if not 1 <= blocks <= 32768:
+        raise ValueError(f"blocks must be 1 to 32768, got {blocks}")
+    chosen = torch.empty((T, Nk, blocks), device=q.device, dtype=torch.int32)
+    with _on_device(q.device):
+        size = lib().fhog_paged_block_select_workspace_bytes(T, Nk, width)
+        ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
+        check(lib().fhog_paged_block_select(
+            _stream(q.device), _ptr(q), _ptr(key_means), _ptr(page_table), _ptr(lengths), _ptr(query_offsets), _ptr(chosen),
+            _ptr(ws), size, B, T, N, Nk, Hd, pages, page_size, width, DTYPE_CODES[q.dtype], blocks, first, last))
+    return chosen
+
+
+def paged_block_attention(q, chosen, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, scale: float,
+                          out=None):
+    """out (T, N, H) of the packed new tokens q over the chosen (T, N_kv, blocks) columns of a paged cache
+    (fhog_paged_block_attention)."""
+    if q.ndim != 3:
+        raise ValueError(f"expected a (T, N, H) query, got {tuple(q.shape)}")
+    (pages, Nk, page, Hd, B, width), page_table, lengths, query_offsets = _check_cache(
+        ("query", q), k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale, q.dtype)
+    T, N, Hq = q.shape
+    if Hq != Hd:
+        raise ValueError(f"query{tuple(q.shape)} and key_cache{tuple(k_cache.shape)} disagree on head_dim")
+    if q.dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {q.dtype}")
+    _check_inputs([("query", q), ("blocks", chosen)])
+    if chosen.ndim != 3 or tuple(chosen.shape[:2]) != (T, Nk) or chosen.dtype != torch.int32:
+        raise ValueError(f"blocks must be torch.int32 {(T, Nk, 'blocks')}, got {tuple(chosen.shape)} of {chosen.dtype}")
+    clear = out is None
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _check_inputs([("query", q), ("out", out)], q.dtype)
+        _expect("out", out, q.shape)
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+    q, chosen = _contig(q, chosen)
+    if not clear:
+        _check_apart(out, "query", q)
+        _check_apart(out, "blocks", chosen)
+        _check_apart(out, "key_cache", k_cache)
+        _check_apart(out, "value_cache", v_cache)
+    with _on_device(q.device):
+        size = lib().fhog_paged_block_workspace_bytes(T, N, Nk, Hd, page, chosen.shape[2])
+        ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
+        check(lib().fhog_paged_block_attention(
+            _stream(q.device), _ptr(q), _ptr(chosen), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+            _ptr(page_table), _ptr(lengths), _ptr(query_offsets), _ptr(out), _ptr(ws), size, B, T, N, Nk, Hd, pages, page,
+            width, DTYPE_CODES[q.dtype], CACHE_DTYPE_CODES[k_cache.dtype], chosen.shape[2], int(clear), float(scale)))
+    if not clear:
+        _written(out)
+    return out
 
 
 # ------------------------------------------------- norms with rotation

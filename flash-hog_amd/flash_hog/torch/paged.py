@@ -10,6 +10,10 @@
                       where rows that share one part ways
   paged_cache_compact the used pages to the front of a cache of another size
 
+  paged_key_means, paged_block_select, paged_block_attention
+                      attention over a few pages of a long sequence: the mean key of each full page, the pages
+                      whose mean suits a token's queries best, and the token's attention over these
+
 No counterpart in the reference, which trains only. All enqueue their kernels on the
 current stream of the tensors' device, read no length back to the host, and can be captured in
 a HIP graph; workspaces come from torch's allocator, a new one for each call.
@@ -151,6 +155,36 @@ def _(key_cache, value_cache, page_table, lengths, max_length, dtype, key_scale,
     return key_cache.new_empty(shape, dtype=dtype), key_cache.new_empty(shape, dtype=dtype)
 
 
+@torch.library.custom_op("flash_hog::paged_key_means", mutates_args=("key_means",))
+def paged_key_means_op(key_cache: Tensor, key_means: Tensor, page_table: Tensor, lengths: Tensor,
+                       query_offsets: Tensor | None, key_scale: Tensor | None) -> None:
+    _hip.paged_key_means(key_cache, key_means, page_table, lengths, query_offsets, key_scale)
+
+
+@torch.library.custom_op("flash_hog::paged_block_select", mutates_args=())
+def paged_block_select_op(query: Tensor, key_means: Tensor, page_table: Tensor, lengths: Tensor,
+                          query_offsets: Tensor | None, page_size: int, blocks: int, first: int, last: int) -> Tensor:
+    return _hip.paged_block_select(query, key_means, page_table, lengths, query_offsets, page_size, blocks, first, last)
+
+
+@paged_block_select_op.register_fake
+def _(query, key_means, page_table, lengths, query_offsets, page_size, blocks, first, last):
+    return query.new_empty((query.shape[0], key_means.shape[1], blocks), dtype=torch.int32)
+
+
+@torch.library.custom_op("flash_hog::paged_block_attention", mutates_args=())
+def paged_block_attention_op(query: Tensor, blocks: Tensor, key_cache: Tensor, value_cache: Tensor, page_table: Tensor,
+                             lengths: Tensor, query_offsets: Tensor | None, key_scale: Tensor | None,
+                             value_scale: Tensor | None, scale: float) -> Tensor:
+    return _hip.paged_block_attention(query, blocks, key_cache, value_cache, page_table, lengths, query_offsets, key_scale,
+                                      value_scale, scale)
+
+
+@paged_block_attention_op.register_fake
+def _(query, blocks, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale, scale):
+    return torch.empty_like(query, memory_format=torch.contiguous_format)
+
+
 def paged_attention(query, key_cache, value_cache, page_table, lengths, query_offsets=None, *, key_scale=None,
                     value_scale=None, window: int | None = None, sinks: int = 0, scale: float | None = None, out=None):
     """Attention of the packed new tokens query (T, N, H) over the cached keys and values of
@@ -267,3 +301,45 @@ def paged_cache_compact(key_cache, value_cache, page_table, lengths, *, num_page
     got = iter(paged_cache_compact_op(*args))
     return (*(None if t is None else next(got) for t in (key_cache, value_cache, key_scale, value_scale, key_means)),
             next(got))
+
+
+def paged_key_means(key_cache, key_means, page_table, lengths, query_offsets=None, *, key_scale=None) -> None:
+    """The mean keys of full pages, key_means (pages, kv_heads, head_dim) float32, in place: those of the
+    pages that the new tokens fill (paged_cache_write goes first), so that a call after each write keeps all
+    of them up to date; the others stay. query_offsets as in paged_cache_write (only how many new tokens
+    each sequence has matters). Sums are in 64 bits and rounded once, so a mean is the same however its
+    tokens came."""
+    through = _checked("paged_key_means", (page_table, lengths, query_offsets), key_cache, key_means, key_scale)
+    call = paged_key_means_op if through else _hip.paged_key_means
+    call(key_cache, key_means, page_table, lengths, query_offsets, key_scale)
+
+
+def paged_block_select(query, key_means, page_table, lengths, query_offsets=None, *, page_size: int, blocks: int,
+                       first: int = 1, last: int = 1):
+    """The pages that each new token attends to, (T, N_kv, blocks) int32: columns of page_table, rising, -1 where there
+    are fewer. A token at position p has the pages of columns 0 to p // page_size. It takes the first `first` of
+    them and the last `last` (at least its own), and of those between the ones whose mean key has the
+    largest product with the sum of the queries of a head's group, `blocks` in all. Products are formed in 64
+    bits; ties go to the lowest column, and NaN (or a page outside the cache) is below every number.
+    query (T, N, H) as in paged_attention, key_means as paged_key_means keeps them."""
+    through = _checked("paged_block_select", (page_table, lengths, query_offsets), query, key_means)
+    page_size, blocks, first, last = map(operator.index, (page_size, blocks, first, last))
+    args = (query, key_means, page_table, lengths, query_offsets, page_size, blocks, first, last)
+    return paged_block_select_op(*args) if through else _hip.paged_block_select(*args)
+
+
+def paged_block_attention(query, blocks, key_cache, value_cache, page_table, lengths, query_offsets=None, *,
+                          key_scale=None, value_scale=None, scale: float | None = None, out=None):
+    """paged_attention (without a window) in which a new token sees, through each key/value head, only the
+    keys of the pages in columns blocks[token, head], up to its own position; blocks (T, N_kv, n) int32 as
+    paged_block_select gives them. Columns outside the table or behind the token show nothing, one named
+    twice counts twice, and a token that sees no key gives zeros. out: as in paged_attention, but apart from query."""
+    through = _checked("paged_block_attention", (blocks, page_table, lengths, query_offsets), query, key_cache, value_cache,
+                       key_scale, value_scale, out)
+    scale = _default_scale(query, scale)
+    args = (query, blocks, key_cache, value_cache, page_table, lengths, query_offsets, key_scale, value_scale, scale)
+    if through:
+        if out is None:
+            return paged_block_attention_op(*args)
+        raise ValueError("out is not supported under torch.compile, transforms or fake tensors")
+    return _hip.paged_block_attention(*args, out=out)

@@ -317,6 +317,44 @@ int fhog_paged_cache_compact(fhog_stream_t stream, const void* k_cache, const vo
                              int cache_dtype);
 
 /*
+ * Attention over chosen blocks. A block is a page, named by its column of the page table.
+ *
+ * key_means (num_pages, kv_heads, head_dim) fp32: the means of the full pages' keys (summed in 64 bits, rounded
+ * once; e4m3 keys are code * scale). This call writes those of the pages that the new tokens fill, the
+ * last query_offsets[b + 1] - query_offsets[b] (null: one) of each sequence, and leaves the others.
+ */
+int fhog_paged_key_means(fhog_stream_t stream, const void* k_cache, const void* k_scale, float* key_means,
+                         const int* page_table, const int* lengths, const int* query_offsets, int batch, int kv_heads,
+                         int head_dim, int num_pages, int page_size, int pages_per_seq, int cache_dtype);
+
+/*
+ * chosen (total, kv_heads, blocks) int32: for each new token, at position p, and key/value head the columns to attend
+ * to, rising, -1 behind them. Of columns 0 to p / page_size: the first `first` (>= 0), the last `last` (>= 1, so that
+ * a page that is not full yet is never chosen by its mean), and of the others those whose mean has the largest
+ * product with the sum of the queries q (total, heads, head_dim) of the head's group, formed in 64 bits, ties to
+ * the lowest column, NaN (also: a page outside the cache) last; `blocks` (>= first + last) in all, or all there
+ * are. Tokens of no sequence, before position 0 or beyond the table: -1 throughout.
+ */
+size_t fhog_paged_block_select_workspace_bytes(int total, int kv_heads, int pages_per_seq);
+int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* key_means, const int* page_table,
+                            const int* lengths, const int* query_offsets, int* chosen, void* workspace,
+                            size_t workspace_bytes, int batch, int total, int heads, int kv_heads, int head_dim,
+                            int num_pages, int page_size, int pages_per_seq, int dtype, int blocks, int first, int last);
+
+/*
+ * fhog_paged_attention (without a window) in which a token sees, through each key/value head, only the keys
+ * of the pages in columns chosen[token][head], up to its own position. Columns outside [0, pages_per_seq) and
+ * ones behind the token show nothing; one that is named twice counts twice.
+ */
+size_t fhog_paged_block_workspace_bytes(int total, int heads, int kv_heads, int head_dim, int page_size, int blocks);
+int fhog_paged_block_attention(fhog_stream_t stream, const void* q, const int* chosen, const void* k_cache,
+                               const void* v_cache, const void* k_scale, const void* v_scale, const int* page_table,
+                               const int* lengths, const int* query_offsets, void* out, void* workspace,
+                               size_t workspace_bytes, int batch, int total, int heads, int kv_heads, int head_dim,
+                               int num_pages, int page_size, int pages_per_seq, int dtype, int cache_dtype, int blocks,
+                               int clear_rest, float scale);
+
+/*
  * Norms of queries and keys for each head with the position rotation, and their derivatives (no
  * counterpart in the reference): what stands before the attention of either kind.
  *
