@@ -977,10 +977,13 @@ int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* ke
                        who);
 }
 
-size_t fhog_paged_block_workspace_bytes(int total, int heads, int kv_heads, int head_dim, int page_size, int blocks) {
+size_t fhog_paged_block_workspace_bytes(int batch, int total, int single, int heads, int kv_heads, int head_dim,
+                                        int page_size, int pages_per_seq, int blocks) {
   static const char* who = "fhog_paged_block_workspace_bytes";
-  const Paged s{1, total, heads, kv_heads, head_dim, 1, page_size, 1, FHOG_DTYPE_BF16, FHOG_DTYPE_BF16};
-  if (check_paged(s, who) || check_blocks(who, s, blocks) || total < 1) return 0;
+  const Paged s{batch, total, heads, kv_heads, head_dim, 1, page_size, pages_per_seq, FHOG_DTYPE_BF16, FHOG_DTYPE_BF16};
+  if (check_paged(s, who) || check_blocks(who, s, blocks) || batch < 1 || total < 1) return 0;
+  if (fhog::block_chunk_rule(batch, total, heads, kv_heads, pages_per_seq, blocks, single != 0))
+    return fhog::block_chunk_plan(batch, total, heads, kv_heads, head_dim, pages_per_seq, blocks).bytes;
   const fhog::BlockPlan plan = fhog::block_plan(total, heads, kv_heads, head_dim, page_size, blocks, compute_units());
   return (size_t)plan.parts * (head_dim + 2) * sizeof(float);
 }
@@ -1006,10 +1009,23 @@ int fhog_paged_block_attention(fhog_stream_t stream, const void* q, const int* c
   const long long tiles = (long long)total * ((heads / kv_heads + 15) / 16);
   if (tiles * kv_heads >= (1ll << 23) || (double)total * kv_heads * blocks >= kMostElements)
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
-  const fhog::BlockPlan plan = fhog::block_plan(total, heads, kv_heads, head_dim, page_size, blocks, compute_units());
-  const size_t need = (size_t)plan.parts * (head_dim + 2) * sizeof(float);
+  const size_t need = fhog_paged_block_workspace_bytes(batch, total, query_offsets == nullptr, heads, kv_heads, head_dim,
+                                                       page_size, pages_per_seq, blocks);
   if (need > 0 && (!aligned(workspace, 16) || workspace_bytes < need))
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null, not 16-byte aligned or below its %zu bytes", who, need);
+  if (fhog::block_chunk_rule(batch, total, heads, kv_heads, pages_per_seq, blocks, query_offsets == nullptr)) {
+    const fhog::BlockChunkPlan plan = fhog::block_chunk_plan(batch, total, heads, kv_heads, head_dim, pages_per_seq, blocks);
+    auto run = [&]<typename T, typename C, int D>() {
+      fhog::BlockChunkParams<T, C> p{(const T*)q, (T*)out,
+                                     {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
+                                     cache_shape(s, page_table, lengths, query_offsets), chosen, heads, blocks, clear_rest,
+                                     scale, (int)plan.lists};
+      fhog::block_chunk_workspace(p, plan, D, workspace);
+      return fhog::launch_block_chunk<T, C, D>(p, plan.slab, (hipStream_t)stream);
+    };
+    return launch_status(dispatch_paged(s, run), who);
+  }
+  const fhog::BlockPlan plan = fhog::block_plan(total, heads, kv_heads, head_dim, page_size, blocks, compute_units());
   auto run = [&]<typename T, typename C, int D>() {
     fhog::BlockParams<T, C> p{(const T*)q, (T*)out,
                               {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},

@@ -71,6 +71,90 @@ inline BlockPlan block_plan(int total, int heads, int kv_heads, int head_dim, in
   return p;
 }
 
+// Attention of many tokens, a block at a time (fhog_blocks_chunk.hip).
+constexpr int kTileRows = 128;       // rows of a tile
+constexpr int kMostColumns = 8192;   // of the page table (the masks of 64 tokens are in LDS)
+constexpr int kSumBlocks = 256;      // blocks of a list (a join's weights are)
+constexpr int kMostLists = 32768;    // sequences times heads times columns
+// A tile of a list (the tokens that chose one column of a sequence, for one head): its rows from row0 of its first
+// entry's token on.
+struct BlockItem {
+  int first, row0, rows;  // entries from first on
+  int page, hk;
+  int key0;               // the column's first position
+  int shift;              // positions above the tokens' indexes in the slab
+  int pad;
+};
+struct BlockEntryAt {
+  int token, slot;  // of the slab; where its list has the column, first of all
+};
+struct PackedTokenAt {
+  int pos;  // -1: of no sequence
+};
+template <typename T, typename C> struct BlockChunkParams {
+  const T* q;
+  T* out;
+  CacheRows<C> cache;
+  CacheShape at;
+  const int* chosen;
+  int heads, blocks, clear_rest;
+  float scale;
+  int lists;           // batch * kv_heads * pages_per_seq
+  int token0, tokens;  // the slab
+  int groups;          // of 64 of its tokens
+  // workspace
+  unsigned long* masks;     // (kv_heads, groups, pages_per_seq) which of a group's tokens chose each column
+  unsigned long* falling;   // (kv_heads, groups) whose lists do not rise
+  int* before;              // (kv_heads, groups, pages_per_seq) entries of a list before the group
+  int* base;                // (lists) its first entry
+  BlockEntryAt* entries;
+  BlockItem* items;
+  int* totals;              // items, entries
+  float* parts;      // (tokens, kv_heads, blocks, group, head_dim)
+  float* parts_ml;   // and their maxima and sums
+};
+// Tokens are taken in slabs whose outputs stay within this.
+constexpr long kPartBytes = 256l << 20;
+struct BlockChunkPlan {
+  int slab;
+  long lists, masks, groups, entries, items, parts;  // elements
+  size_t bytes;
+};
+inline BlockChunkPlan block_chunk_plan(int batch, int total, int heads, int kv_heads, int head_dim, int pages_per_seq, int blocks) {
+  BlockChunkPlan p;
+  const long token = (long)heads * blocks * (head_dim + 2) * 4;
+  const long fit = kPartBytes / token / 64 * 64;
+  p.slab = (int)(fit < 64 ? 64 : fit < total ? fit : total);
+  p.lists = (long)batch * kv_heads * pages_per_seq;
+  p.groups = (long)kv_heads * ((p.slab + 63) / 64);
+  p.masks = p.groups * pages_per_seq;
+  p.entries = (long)p.slab * blocks * kv_heads;
+  p.items = (long)p.slab * blocks * heads / kTileRows + p.lists;
+  p.parts = (long)p.slab * heads * blocks;
+  p.bytes = (size_t)(p.parts * (head_dim + 2) * 4 + p.items * sizeof(BlockItem) + p.entries * sizeof(BlockEntryAt) +
+                     (p.masks + p.groups) * 8 + (p.masks + p.lists + 2) * 4);
+  return p;
+}
+// Lays the workspace (16-byte aligned) out, larger elements first.
+template <typename T, typename C> void block_chunk_workspace(BlockChunkParams<T, C>& p, const BlockChunkPlan& plan, int head_dim, void* ws) {
+  p.items = (BlockItem*)ws;
+  p.parts = (float*)(p.items + plan.items);
+  p.parts_ml = p.parts + plan.parts * head_dim;
+  p.entries = (BlockEntryAt*)(p.parts_ml + plan.parts * 2);
+  p.masks = (unsigned long*)(p.entries + plan.entries);
+  p.falling = p.masks + plan.masks;
+  p.before = (int*)(p.falling + plan.groups);
+  p.base = p.before + plan.masks;
+  p.totals = p.base + plan.lists;
+}
+// Whether a call goes a block at a time.
+inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int pages_per_seq, int blocks, bool single) {
+  return !single && pages_per_seq <= kMostColumns && blocks <= kSumBlocks &&
+         (long)batch * kv_heads * pages_per_seq <= kMostLists;
+}
+
+template <typename T, typename C, int D>
+hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p, int slab, hipStream_t s);
 template <typename C, int D> hipError_t launch_key_means(const KeyMeansParams<C>& p, int workgroups, hipStream_t s);
 template <typename T, int D> hipError_t launch_block_select(const BlockSelectParams<T>& p, hipStream_t s);
 template <typename T, typename C, int D> hipError_t launch_block_attention(const BlockParams<T, C>& p, hipStream_t s);

@@ -68,7 +68,7 @@ SIGNATURES = {
     "fhog_paged_key_means": (_i, [_p] * 7 + [_i] * 7),
     "fhog_paged_block_select_workspace_bytes": (ctypes.c_size_t, [_i] * 3),
     "fhog_paged_block_select": (_i, [_p] * 8 + [ctypes.c_size_t] + [_i] * 12),
-    "fhog_paged_block_workspace_bytes": (ctypes.c_size_t, [_i] * 6),
+    "fhog_paged_block_workspace_bytes": (ctypes.c_size_t, [_i] * 9),
     "fhog_paged_block_attention": (_i, [_p] * 12 + [ctypes.c_size_t] + [_i] * 12 + [_f]),
     "fhog_qk_norm_rotary_workspace_bytes": (ctypes.c_size_t, [_p]),
     "fhog_qk_norm_rotary_fwd": (_i, [_p] * 8),
@@ -694,7 +694,8 @@ def paged_block_attention(q, chosen, k_cache, v_cache, page_table, lengths, quer
         _check_apart(out, "key_cache", k_cache)
         _check_apart(out, "value_cache", v_cache)
     with _on_device(q.device):
-        size = lib().fhog_paged_block_workspace_bytes(T, N, Nk, Hd, page, chosen.shape[2])
+        size = lib().fhog_paged_block_workspace_bytes(B, T, int(query_offsets is None), N, Nk, Hd, page, width,
+                                                      chosen.shape[2])
         ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
         check(lib().fhog_paged_block_attention(
             _stream(q.device), _ptr(q), _ptr(chosen), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),

@@ -346,7 +346,8 @@ int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* ke
  * of the pages in columns chosen[token][head], up to its own position. Columns outside [0, pages_per_seq) and
  * ones behind the token show nothing; one that is named twice counts twice.
  */
-size_t fhog_paged_block_workspace_bytes(int total, int heads, int kv_heads, int head_dim, int page_size, int blocks);
+size_t fhog_paged_block_workspace_bytes(int batch, int total, int single, int heads, int kv_heads, int head_dim,
+                                        int page_size, int pages_per_seq, int blocks);
 int fhog_paged_block_attention(fhog_stream_t stream, const void* q, const int* chosen, const void* k_cache,
                                const void* v_cache, const void* k_scale, const void* v_scale, const int* page_table,
                                const int* lengths, const int* query_offsets, void* out, void* workspace,

@@ -85,9 +85,9 @@ def test_workspace_bytes(lib):
     assert lib.fhog_paged_block_select_workspace_bytes(1 << 20, 8, 1024) == 1 << 28
     assert lib.fhog_paged_block_select_workspace_bytes(5, 64, 1 << 21) == 64 * 8 << 21
     assert lib.fhog_paged_block_select_workspace_bytes(0, 4, 100) == 0
-    assert lib.fhog_paged_block_workspace_bytes(1, 4, 2, 64, 16, 1) == 0
-    assert lib.fhog_paged_block_workspace_bytes(1, 4, 2, 64, 15, 1) == 0
-    few, many = (lib.fhog_paged_block_workspace_bytes(t, 32, 8, 128, 64, 64) for t in (1, 4096))
+    assert lib.fhog_paged_block_workspace_bytes(1, 1, 1, 4, 2, 64, 16, 5, 1) == 0
+    assert lib.fhog_paged_block_workspace_bytes(1, 1, 1, 4, 2, 64, 15, 5, 1) == 0
+    few, many = (lib.fhog_paged_block_workspace_bytes(t, t, 1, 32, 8, 128, 64, 500, 64) for t in (1, 4096))
     assert few > 0 and many == 0
 
 
