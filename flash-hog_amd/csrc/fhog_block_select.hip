@@ -7,9 +7,9 @@
 // position p of pages 0 to p / page_size takes the first `first` and the last `last` of them, and of those
 // between the ones with the largest scores, ties to the lowest index; NaN is below every number.
 //
-// The scores go through memory; then the k-th largest is found digit by digit (eight bits of the
-// scores' bits in an order that compares as they do), with a histogram in LDS, and the choice is
-// written in the order of the columns.
+// Scores are kept as their bits in an order that compares as they do. Where sequences have many new tokens, 16 of
+// them share the means' reads, as matrix products of 64 bits, whose scores stay in LDS; a wave then chooses for a
+// token. Else, and where a table is wider than LDS, scores go through memory.
 #include "fhog_blocks.h"
 
 namespace fhog {
@@ -79,13 +79,14 @@ struct TokenBlocks {
   int b, own;         // own: the token's own column, -1 if it sees nothing
   int lo, hi;         // columns [lo, hi) are chosen from by score
   int room;           // how many of them
-  template <typename P> __device__ __forceinline__ TokenBlocks(const P& p, int t) {
+  // most: as if its own column were the table's last at most (no token before it then chooses from more).
+  template <typename P> __device__ __forceinline__ TokenBlocks(const P& p, int t, bool most = false) {
     const CacheShape& c = p.at;
     b = c.offsets ? last_at_or_before(c.batch, t, [&](int s) { return packed_begin(c, s); }) : t;
     const int begin = packed_begin(c, b), end = c.offsets ? packed_begin(c, b + 1) : b + 1;
     const int pos = max(0, c.lengths[b]) - (end - t);
     own = t < begin || t >= end || pos < 0 ? -1 : pos >> c.page_shift;
-    if (own >= c.pages_per_seq) own = -1;  // a length beyond the table
+    if (own >= c.pages_per_seq) own = most ? c.pages_per_seq - 1 : -1;  // a length beyond the table
     lo = min(p.first, own + 1);
     hi = max(lo, own + 1 - p.last);
     room = max(0, p.blocks - lo - (own + 1 - hi));
@@ -100,7 +101,93 @@ __device__ __forceinline__ unsigned long sortable(double x) {
   return (unsigned long)bits ^ (bits < 0 ? ~0ul : 1ul << 63);
 }
 
-// The scores of kColumns columns of a token and key/value head; sixteen lanes a column.
+// The columns that are not chosen by score, and what is behind the last one, of a token's list; by `threads`
+// threads.
+__device__ __forceinline__ void write_forced(const TokenBlocks& tb, int* out, int blocks, int thread, int threads) {
+  const int count = min(blocks, tb.own + 1);
+  const bool by_score = tb.by_score();
+  for (int i = thread; i < blocks; i += threads)
+    if (!by_score || i < tb.lo || i >= tb.lo + tb.room)
+      // (the last ones end with the token's own)
+      out[i] = i >= count ? -1 : i < tb.lo || !by_score ? i : tb.own + 1 - (count - i);
+}
+
+// The largest value of 32 bits that `want` keys reach, bit by bit from bit `top` of `prefix` on, where count_from
+// says how many reach a value; or, sooner, one that exactly `want` reach (exact).
+template <typename F> __device__ __forceinline__ uint32_t reached_by(int want, uint32_t prefix, int top, bool& exact, F&& count_from) {
+  exact = false;
+  for (int bit = top; bit >= 0 && !exact; --bit) {
+    const uint32_t next = prefix | 1u << bit;
+    const int count = count_from(next);
+    if (count >= want) {
+      prefix = next;
+      exact = count == want;
+    }
+  }
+  return prefix;
+}
+
+// The `room` largest of a wave's n > room keys, KJ a lane: key j of lane l is column lo + 64 j + l. Writes their
+// columns, rising, to out. The scores' upper 32 bits first: most of the time those tell the last one taken
+// from the first one left, after as many bits from the highest in which keys differ on as that takes.
+template <int KJ, typename F> __device__ __forceinline__ void choose_in_wave(int n, int lo, int room, int* out, F&& key_of) {
+  const int lane = threadIdx.x & 63;
+  uint32_t hi[KJ], low[KJ];  // (0 where there is no key, which no value that is asked for counts)
+  uint32_t any = 0, all = ~0u;
+#pragma unroll
+  for (int j = 0; j < KJ; ++j) {  // (not in a branch a key: it would wait for each in turn)
+    const unsigned long key = key_of(min(64 * j + lane, n - 1));
+    const bool there = 64 * j + lane < n;
+    hi[j] = there ? (uint32_t)(key >> 32) : 0;
+    low[j] = there ? (uint32_t)key : 0;
+    any |= hi[j];
+    all &= there ? hi[j] : ~0u;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    any |= (uint32_t)__shfl_xor((int)any, d, 64);
+    all &= (uint32_t)__shfl_xor((int)all, d, 64);
+  }
+  any = __builtin_amdgcn_readfirstlane(any), all = __builtin_amdgcn_readfirstlane(all);
+  auto count = [&](auto&& which) {
+    int sum = 0;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j)
+      if (64 * j < n) sum += __popcll(__ballot(64 * j + lane < n && which(j)));
+    return sum;
+  };
+  const int top = any == all ? -1 : 31 - __builtin_clz(any ^ all);
+  const uint32_t same = top < 0 ? ~0u : top == 31 ? 0u : ~((2u << top) - 1);  // bits above that all keys share
+  bool exact;
+  const uint32_t h = reached_by(room, all & same, top, exact, [&](uint32_t x) { return count([&](int j) { return hi[j] >= x; }); });
+  uint32_t l = 0;
+  int left = 0;  // keys equal to (h, l) that are taken, if not all
+  if (!exact) {
+    const int above = count([&](int j) { return hi[j] > h; });
+    l = reached_by(room - above, 0, 31, exact, [&](uint32_t x) { return count([&](int j) { return hi[j] == h && low[j] >= x; }); });
+    if (!exact) left = room - above - count([&](int j) { return hi[j] == h && low[j] > l; });
+  }
+  const unsigned long below = (1ul << lane) - 1;
+  int at = 0;
+#pragma unroll
+  for (int j = 0; j < KJ; ++j) {
+    if (64 * j >= n) continue;
+    const bool there = 64 * j + lane < n, equal = there && hi[j] == h && low[j] == l;
+    bool take = there && (hi[j] > h || (hi[j] == h && low[j] >= l));
+    if (!exact) {
+      const unsigned long equals = __ballot(equal);
+      take = take && (!equal || (int)__popcll(equals & below) < left);
+      left = max(0, left - (int)__popcll(equals));
+    }
+    const unsigned long takes = __ballot(take);
+    if (take) out[at + __popcll(takes & below)] = lo + 64 * j + lane;
+    at += __popcll(takes);
+  }
+}
+
+// ------------------------------------------------------------------ scores
+
+// A token's scores of kColumns columns for a key/value head; sixteen lanes a column.
 constexpr int kColumns = 64;
 template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_score_kernel(BlockSelectParams<T> p) {
   constexpr int E = D / 16;
@@ -121,13 +208,14 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_s
       for (int e = 0; e < 4; ++e) q[j + e] += (double)(float)x[e];
     }
   }
-  double* const scores = p.scores + (long)blockIdx.x * c.pages_per_seq;
+  unsigned long* const scores = p.scores + (long)blockIdx.x * c.pages_per_seq;
   for (int col = c0 + way; col < min(c0 + kColumns, tb.hi); col += kThreads / 16) {
     if (col < tb.lo) continue;
     const int page = c.table[(long)tb.b * c.pages_per_seq + col];
-    double sum = 0.;
+    double sum = NAN;
     if ((unsigned)page < (unsigned)c.pages) {
       const float* m = p.means + ((long)page * c.kv_heads + hk) * D + lane * 4;
+      sum = 0.;
 #pragma unroll
       for (int j = 0; j < E; j += 4) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(m + 16 * j);
@@ -136,34 +224,139 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_s
       }
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    } else {
-      sum = NAN;
     }
-    if (lane == 0) scores[col] = sum;
+    if (lane == 0) scores[col] = sortable(sum);
   }
 }
 
+// Tiles of 16 tokens of a sequence, for many of them: a sequence's tiles start at offset / 16 + index.
+struct TokenTile {
+  int b, t0, count;
+  template <typename P> __device__ __forceinline__ TokenTile(const P& p, int slot) {
+    const CacheShape& c = p.at;
+    auto first_slot = [&](int s) { return packed_begin(c, s) / 16 + s; };
+    b = last_at_or_before(c.batch, slot, first_slot);
+    const int begin = packed_begin(c, b), end = packed_begin(c, b + 1);
+    const long at = begin + 16l * (slot - first_slot(b));  // (a wrong slot's too)
+    t0 = (int)at;
+    count = at < begin || at >= end ? 0 : (int)(end - at < 16 ? end - at : 16);
+  }
+};
+
+// Scores of a tile's tokens against columns [c0, c1) by matrix products of 64 bits, 16 columns a wave at a time:
+// put(row, column, key). Lane (n, g) holds columns g D / 4 on of q's row n and of a page's mean, of which the
+// products take one each in turn; it gets rows g + 4 i of column n.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+template <typename T, int D, typename F>
+__device__ __forceinline__ void score_tile(const BlockSelectParams<T>& p, const TokenTile& tile, int hk, int c0, int c1, F&& put) {
+  constexpr int K = D / 4;
+  const CacheShape& c = p.at;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, group = p.heads / c.kv_heads;
+  double q[K] = {};
+  const T* row = p.q + ((long)(tile.t0 + min(n, tile.count - 1)) * p.heads + hk * group) * D + g * K;
+  for (int h = 0; h < group; ++h, row += D)
+#pragma unroll
+    for (int k = 0; k < K; k += 8) {
+      const V8<T> x = *reinterpret_cast<const V8<T>*>(row + k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[k + e] += (double)(float)x[e];
+    }
+  const int* const table = c.table + (long)tile.b * c.pages_per_seq;
+  for (int col0 = c0 + 16 * (int)(threadIdx.x >> 6); col0 < c1; col0 += 16 * (kThreads / 64)) {
+    const int col = min(col0 + n, c1 - 1), page = table[col];
+    const bool bad = (unsigned)page >= (unsigned)c.pages;
+    const float* m = p.means + ((long)(bad ? 0 : page) * c.kv_heads + hk) * D + g * K;
+    f64x4 sum = {0., 0., 0., 0.};
+#pragma unroll
+    for (int k = 0; k < K; k += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(m + k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f64_16x16x4f64(q[k + e], (double)x[e], sum, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col0 + n < c1) put(g + 4 * i, col, bad ? 0ul : sortable(sum[i]));
+  }
+}
+
+// Scores and choice of a tile's tokens in one, with the scores in LDS, of up to COLUMNS columns chosen from.
+template <typename T, int D, int COLUMNS> __global__ void __launch_bounds__(kThreads) block_select_tile_kernel(BlockSelectParams<T> p) {
+  __shared__ unsigned long s_key[16][COLUMNS + 2];  // (rows apart, so that a column's keys are in different banks)
+  const CacheShape& c = p.at;
+  const int hk = blockIdx.x % c.kv_heads;
+  const TokenTile tile(p, blockIdx.x / c.kv_heads);
+  if (tile.count <= 0) return;
+  const TokenBlocks last(p, tile.t0 + tile.count - 1, true);
+  const int lo = min(p.first, c.pages_per_seq);
+  if (last.by_score()) score_tile<T, D>(p, tile, hk, lo, last.hi, [&](int row, int col, unsigned long key) { s_key[row][col - lo] = key; });
+  __syncthreads();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int r = wave; r < tile.count; r += kThreads / 64) {
+    const TokenBlocks tb(p, tile.t0 + r);
+    int* const out = p.chosen + ((long)(tile.t0 + r) * c.kv_heads + hk) * p.blocks;
+    write_forced(tb, out, p.blocks, threadIdx.x & 63, 64);
+    if (tb.by_score() && tb.room > 0)
+      choose_in_wave<COLUMNS / 64>(tb.hi - tb.lo, tb.lo, tb.room, out + tb.lo, [&](int i) { return s_key[r][i]; });
+  }
+}
+
+// Empty lists, before the tiles write theirs: those of packed rows that no sequence has stay so.
+template <typename T> __global__ void __launch_bounds__(kThreads) block_none_kernel(BlockSelectParams<T> p) {
+  const long i = (long)blockIdx.x * kThreads + threadIdx.x;
+  if (i < (long)p.at.total * p.at.kv_heads * p.blocks) p.chosen[i] = -1;
+}
+
+// Scores of a tile's tokens, in the slab, into memory, for wider tables: kWide columns a workgroup.
+constexpr int kWide = 1024;
+template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_score_tile_kernel(BlockSelectParams<T> p) {
+  const CacheShape& c = p.at;
+  const int hk = blockIdx.x % c.kv_heads;
+  const TokenTile tile(p, blockIdx.x / c.kv_heads);
+  if (tile.count <= 0 || tile.t0 >= p.token0 + p.tokens || tile.t0 + tile.count <= p.token0) return;
+  const TokenBlocks last(p, tile.t0 + tile.count - 1, true);
+  if (!last.by_score()) return;
+  const int c0 = max(last.lo, (int)blockIdx.y * kWide), c1 = min(last.hi, ((int)blockIdx.y + 1) * kWide);
+  if (c0 >= c1) return;
+  score_tile<T, D>(p, tile, hk, c0, c1, [&](int row, int col, unsigned long key) {
+    const int t = tile.t0 + row - p.token0;
+    if (row < tile.count && t >= 0 && t < p.tokens) p.scores[((long)t * c.kv_heads + hk) * c.pages_per_seq + col] = key;
+  });
+}
+
+// ------------------------------------------------------------------ choice from scores in memory
+
+// A wave a token and key/value head, which chooses from up to COLUMNS columns.
+template <typename T, int COLUMNS> __global__ void __launch_bounds__(kThreads) block_choose_wave_kernel(BlockSelectParams<T> p) {
+  const CacheShape& c = p.at;
+  const long i = (long)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (i >= (long)p.tokens * c.kv_heads) return;
+  const int hk = (int)(i % c.kv_heads), t = p.token0 + (int)(i / c.kv_heads);
+  const TokenBlocks tb(p, t);
+  int* const out = p.chosen + ((long)t * c.kv_heads + hk) * p.blocks;
+  write_forced(tb, out, p.blocks, threadIdx.x & 63, 64);
+  if (!tb.by_score() || tb.room == 0) return;
+  const unsigned long* const scores = p.scores + i * c.pages_per_seq + tb.lo;
+  choose_in_wave<COLUMNS / 64>(tb.hi - tb.lo, tb.lo, tb.room, out + tb.lo, [&](int j) { return scores[j]; });
+}
+
+// A workgroup a token and key/value head, of any number of columns: eight bits of the keys at a time, with a
+// histogram.
 template <typename T> __global__ void __launch_bounds__(kThreads) block_choose_kernel(BlockSelectParams<T> p) {
   __shared__ int hist[256], box[4], found[3];
   const CacheShape& c = p.at;
   const int hk = blockIdx.x % c.kv_heads, t = p.token0 + blockIdx.x / c.kv_heads;
   const TokenBlocks tb(p, t);
   int* const out = p.chosen + ((long)t * c.kv_heads + hk) * p.blocks;
-  const int count = min(p.blocks, tb.own + 1);
-  for (int i = threadIdx.x; i < p.blocks; i += kThreads)
-    if (!tb.by_score() || i < tb.lo || i >= tb.lo + tb.room) {
-      const int behind = count - i;  // (the last ones end with the token's own)
-      out[i] = i >= count ? -1 : i < tb.lo || !tb.by_score() ? i : tb.own + 1 - behind;
-    }
+  write_forced(tb, out, p.blocks, threadIdx.x, kThreads);
   if (!tb.by_score() || tb.room == 0) return;
-  const double* const scores = p.scores + (long)blockIdx.x * c.pages_per_seq;
+  const unsigned long* const scores = p.scores + (long)blockIdx.x * c.pages_per_seq;
   unsigned long prefix = 0, mask = 0;
   int left = tb.room;
   for (int shift = 56; shift >= 0; shift -= 8) {
     hist[threadIdx.x] = 0;
     __syncthreads();
     for (int col = tb.lo + (int)threadIdx.x; col < tb.hi; col += kThreads) {
-      const unsigned long key = sortable(scores[col]);
+      const unsigned long key = scores[col];
       if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
     }
     __syncthreads();
@@ -187,7 +380,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) block_choose_k
   int at = tb.lo;
   for (int col0 = tb.lo; col0 < tb.hi; col0 += kThreads) {
     const int col = col0 + (int)threadIdx.x;
-    const unsigned long key = col < tb.hi ? sortable(scores[col]) & mask : 0;
+    const unsigned long key = col < tb.hi ? scores[col] & mask : 0;
     const bool equal = col < tb.hi && key == prefix, above = col < tb.hi && key > prefix;
     int equals, takes;
     const int rank = group_scan<kThreads>(equal, equals, box);
@@ -206,15 +399,35 @@ template <typename C, int D> hipError_t launch_key_means(const KeyMeansParams<C>
   return hipGetLastError();
 }
 
-template <typename T, int D> hipError_t launch_block_select(const BlockSelectParams<T>& p_, hipStream_t stream) {
+template <typename T, int D> hipError_t launch_block_select(const BlockSelectParams<T>& p_, SelectPlan plan, hipStream_t stream) {
   BlockSelectParams<T> p = p_;
-  const int slab = p.tokens;
-  const unsigned columns = (p.at.pages_per_seq + kColumns - 1) / kColumns;
-  for (p.token0 = 0; p.token0 < p.at.total; p.token0 += slab) {
-    p.tokens = p.at.total - p.token0 < slab ? p.at.total - p.token0 : slab;
+  const int width = p.at.pages_per_seq, most = width - p.first - p.last;  // columns chosen from
+  if (plan.tiles && most <= kFusedColumns) {
+    const dim3 grid((unsigned)((long)plan.slots * p.at.kv_heads));
+    const long elements = (long)p.at.total * p.at.kv_heads * p.blocks;
+    hipLaunchKernelGGL((block_none_kernel<T>), dim3((unsigned)((elements + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, p);
+    if (most <= 256)
+      hipLaunchKernelGGL((block_select_tile_kernel<T, D, 256>), grid, dim3(kThreads), 0, stream, p);
+    else if (most <= 512)
+      hipLaunchKernelGGL((block_select_tile_kernel<T, D, 512>), grid, dim3(kThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((block_select_tile_kernel<T, D, kFusedColumns>), grid, dim3(kThreads), 0, stream, p);
+    return hipGetLastError();
+  }
+  for (p.token0 = 0; p.token0 < p.at.total; p.token0 += plan.slab) {
+    p.tokens = p.at.total - p.token0 < plan.slab ? p.at.total - p.token0 : plan.slab;
     const unsigned rows = (unsigned)p.tokens * p.at.kv_heads;
-    hipLaunchKernelGGL((block_score_kernel<T, D>), dim3(rows, columns), dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((block_choose_kernel<T>), dim3(rows), dim3(kThreads), 0, stream, p);
+    if (plan.tiles)
+      hipLaunchKernelGGL((block_score_tile_kernel<T, D>), dim3((unsigned)((long)plan.slots * p.at.kv_heads), (width + kWide - 1) / kWide),
+                         dim3(kThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((block_score_kernel<T, D>), dim3(rows, (width + kColumns - 1) / kColumns), dim3(kThreads), 0, stream, p);
+    if (most <= 256)
+      hipLaunchKernelGGL((block_choose_wave_kernel<T, 256>), dim3((rows + 3) / 4), dim3(kThreads), 0, stream, p);
+    else if (most <= 1024)
+      hipLaunchKernelGGL((block_choose_wave_kernel<T, 1024>), dim3((rows + 3) / 4), dim3(kThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((block_choose_kernel<T>), dim3(rows), dim3(kThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -225,8 +438,8 @@ template <typename T, int D> hipError_t launch_block_select(const BlockSelectPar
   template hipError_t launch_key_means<__bf16, D>(const KeyMeansParams<__bf16>&, int, hipStream_t);     \
   template hipError_t launch_key_means<_Float16, D>(const KeyMeansParams<_Float16>&, int, hipStream_t); \
   template hipError_t launch_key_means<e4m3, D>(const KeyMeansParams<e4m3>&, int, hipStream_t);         \
-  template hipError_t launch_block_select<__bf16, D>(const BlockSelectParams<__bf16>&, hipStream_t);    \
-  template hipError_t launch_block_select<_Float16, D>(const BlockSelectParams<_Float16>&, hipStream_t);
+  template hipError_t launch_block_select<__bf16, D>(const BlockSelectParams<__bf16>&, SelectPlan, hipStream_t); \
+  template hipError_t launch_block_select<_Float16, D>(const BlockSelectParams<_Float16>&, SelectPlan, hipStream_t);
 FHOG_INST(64)
 FHOG_INST(128)
 FHOG_INST(256)

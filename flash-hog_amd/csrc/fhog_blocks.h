@@ -18,7 +18,7 @@ template <typename T> struct BlockSelectParams {
   const float* means;
   int* chosen;  // (total, kv_heads, blocks)
   CacheShape at;
-  double* scores;  // workspace: (tokens of a slab, kv_heads, pages_per_seq)
+  unsigned long* scores;  // workspace: (tokens of a slab, kv_heads, pages_per_seq), as sortable bits
   int heads, blocks, first, last;
   int token0, tokens;  // the slab
 };
@@ -36,13 +36,23 @@ template <typename T, typename C> struct BlockParams {
   float scale;
 };
 
-// A token's scores, of all columns and key/value heads, are 8 bytes each; tokens are taken in slabs that keep
-// them within this.
+// How choices are made: by tiles of 16 tokens of a sequence (slots of them), or token by token; and how many
+// tokens' scores are in memory at a time (none where they stay in LDS).
+struct SelectPlan {
+  bool tiles;
+  int slots, slab;
+};
 constexpr long kScoreBytes = 256l << 20;
-inline int select_slab(int total, int kv_heads, int pages_per_seq) {
+constexpr int kFusedColumns = 1024;
+inline SelectPlan select_plan(int batch, int total, bool single, int kv_heads, int pages_per_seq, int first, int last) {
+  SelectPlan p;
+  p.tiles = !single && total >= 8l * batch;
+  p.slots = total / 16 + batch;
   long fit = kScoreBytes / (8l * kv_heads * pages_per_seq);
   if (fit > (1l << 22) / kv_heads) fit = (1l << 22) / kv_heads;  // (a launch's threads are 32 bits)
-  return (int)(fit < 1 ? 1 : fit < total ? fit : total);
+  p.slab = (int)(fit < 1 ? 1 : fit < total ? fit : total);
+  if (p.tiles && (long)pages_per_seq - first - last <= kFusedColumns) p.slab = 0;
+  return p;
 }
 
 // Attention of tokens over chosen blocks: tiles of 16 rows, and how the blocks are split.
@@ -156,7 +166,7 @@ inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int 
 template <typename T, typename C, int D>
 hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p, int slab, hipStream_t s);
 template <typename C, int D> hipError_t launch_key_means(const KeyMeansParams<C>& p, int workgroups, hipStream_t s);
-template <typename T, int D> hipError_t launch_block_select(const BlockSelectParams<T>& p, hipStream_t s);
+template <typename T, int D> hipError_t launch_block_select(const BlockSelectParams<T>& p, SelectPlan plan, hipStream_t s);
 template <typename T, typename C, int D> hipError_t launch_block_attention(const BlockParams<T, C>& p, hipStream_t s);
 
 }  // namespace fhog

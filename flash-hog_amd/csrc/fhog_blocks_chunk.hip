@@ -164,7 +164,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
 // 128 rows of tokens that chose one column, 32 a wave; row r of a list is its token r / group, head r % group.
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(kThreads)
-__attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2)))
+__attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 128 ? 3 : 4)))
 block_tile_kernel(BlockChunkParams<T, C> p) {
   constexpr int KS = D / 16, DT = D / 32;
   constexpr int kSwz = D == 64 ? kSwzPairs : kSwzWide;

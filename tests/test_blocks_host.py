@@ -80,11 +80,15 @@ def test_nothing_to_do(lib):
 
 
 def test_workspace_bytes(lib):
-    """Scores of the tokens of a slab: all of them, or as many as 256 MiB hold; at least one."""
-    assert lib.fhog_paged_block_select_workspace_bytes(10, 4, 100) == 10 * 4 * 100 * 8
-    assert lib.fhog_paged_block_select_workspace_bytes(1 << 20, 8, 1024) == 1 << 28
-    assert lib.fhog_paged_block_select_workspace_bytes(5, 64, 1 << 21) == 64 * 8 << 21
-    assert lib.fhog_paged_block_select_workspace_bytes(0, 4, 100) == 0
+    """Scores of the tokens of a slab: all of them, or as many as 256 MiB hold; at least one. None where
+    tiles of tokens keep them in LDS."""
+    scores = lambda *sizes: lib.fhog_paged_block_select_workspace_bytes(*sizes, 1, 1)
+    assert scores(10, 10, 1, 4, 100) == 10 * 4 * 100 * 8
+    assert scores(1, 7, 0, 4, 100) == 7 * 4 * 100 * 8
+    assert scores(1, 8, 0, 4, 1026) == 0 and scores(1, 8, 0, 4, 1027) == 8 * 4 * 1027 * 8
+    assert scores(1, 1 << 20, 0, 8, 2048) == 1 << 28
+    assert scores(5, 5, 1, 64, 1 << 21) == 64 * 8 << 21
+    assert scores(0, 0, 1, 4, 100) == 0
     assert lib.fhog_paged_block_workspace_bytes(1, 1, 1, 4, 2, 64, 16, 5, 1) == 0
     assert lib.fhog_paged_block_workspace_bytes(1, 1, 1, 4, 2, 64, 15, 5, 1) == 0
     few, many = (lib.fhog_paged_block_workspace_bytes(t, t, 1, 32, 8, 128, 64, 500, 64) for t in (1, 4096))

@@ -156,14 +156,50 @@ def test_many_blocks(blocks, page, length, cuda_device):
         check(out, flash_hog.paged_attention(q.to(cuda_device), moved["key_cache"], moved["value_cache"], **where).cpu())
 
 
-def choose(means, q, page, blocks, length, device, first=0, last=1, table=None):
+def choose(means, q, page, blocks, length, device, first=0, last=1, table=None, tiles=False):
+    """The lists of one token; tiles: as the last of sixteen."""
     import flash_hog
 
     pages = means.shape[0]
     table = torch.arange(pages, dtype=torch.int32)[None] if table is None else table
+    if tiles:
+        offsets = torch.tensor([0, 16], dtype=torch.int32, device=device)
+        return flash_hog.paged_block_select(q.expand(16, -1, -1).to(device), means.to(device), table.to(device),
+                                            torch.tensor([length], dtype=torch.int32, device=device), offsets,
+                                            page_size=page, blocks=blocks, first=first, last=last).cpu()[15]
     return flash_hog.paged_block_select(q.to(device), means.to(device), table.to(device),
                                         torch.tensor([length], dtype=torch.int32, device=device), page_size=page,
                                         blocks=blocks, first=first, last=last).cpu()[0]
+
+
+@pytest.mark.parametrize("width", [None, 300, 514, 1027, 1028, 3000])
+@pytest.mark.parametrize("new", [[1, 40, 16, 5], [130, 1, 0, 33], [2, 9, 1, 3]], ids=str)
+def test_select_tiles_and_tokens(new, width, cuda_device):
+    """Sequences with many and with few new tokens, and tables as wide as the rules tell apart: tiles of 16 tokens
+    that end anywhere, scores in LDS and in memory."""
+    import flash_hog
+
+    lengths = [3000, 700, 16, 2049]
+    case = (4, 2, 64, BF16, False, 16, lengths, new, 20, 2, 1)
+    print("[case] tiles", case_id(case), width, flush=True)
+    cache, counts, q, moved, where = make(case, cuda_device, width=width)
+    means = all_means(cache)
+    got = flash_hog.paged_block_select(q.to(cuda_device), means.to(cuda_device), **where, page_size=16, blocks=20, first=2)
+    assert torch.equal(got.cpu(), ref.select(q, means, cache.table, lengths, counts, 16, 20, 2, 1))
+
+
+def test_select_beyond_the_table(cuda_device):
+    """Tokens beyond the table have no list; those before them in the same tile have theirs."""
+    import flash_hog
+
+    gen = torch.Generator().manual_seed(0)
+    means, q = torch.randn((20, 1, 64), generator=gen), torch.randn((40, 1, 64), generator=gen).to(BF16)
+    table = torch.arange(20, dtype=torch.int32)[None]
+    for length in (321, 330, 340, 2 ** 31 - 1):
+        got = flash_hog.paged_block_select(
+            q.to(cuda_device), means.to(cuda_device), table.to(cuda_device), torch.tensor([length], dtype=torch.int32, device=cuda_device),
+            torch.tensor([0, 40], dtype=torch.int32, device=cuda_device), page_size=16, blocks=5)
+        assert torch.equal(got.cpu(), ref.select(q, means, table, [length], [40], 16, 5, 1, 1)), length
 
 
 @pytest.mark.parametrize("pages", [40, 300, 3000])
@@ -191,9 +227,10 @@ def test_ties_and_special_scores(pages, cuda_device):
         if kind == "special":
             table[0, 5], table[0, 6] = -1, pages
         for blocks in (1, 2, 5, 17, pages // 2, pages - 2):
-            got = choose(m, q, 16, blocks, length, cuda_device, table=table)
             want = ref.select(q, m, table, [length], [1], 16, blocks, 0, 1)[0]
-            assert torch.equal(got, want), (kind, blocks)
+            for tiles in (False, True):
+                got = choose(m, q, 16, blocks, length, cuda_device, table=table, tiles=tiles)
+                assert torch.equal(got, want), (kind, blocks, tiles)
 
 
 def test_close_scores(cuda_device):
@@ -205,9 +242,9 @@ def test_close_scores(cuda_device):
     means = torch.full((pages, 1, 64), 64.0)
     means[:, 0, 17] = 1 + order * 2.0 ** -23
     q = torch.ones((1, 1, 64), dtype=BF16)
-    got = choose(means, q, 16, 21, 16 * pages, cuda_device)
     want = torch.tensor(sorted([*order[:-1].argsort(descending=True)[:20].tolist(), pages - 1]), dtype=torch.int32)
-    assert torch.equal(got[0], want)
+    for tiles in (False, True):
+        assert torch.equal(choose(means, q, 16, 21, 16 * pages, cuda_device, tiles=tiles)[0], want)
 
 
 def test_rows_of_no_sequence(cuda_device):
@@ -421,9 +458,9 @@ def test_refusals(cuda_device):
             (lambda: select(q, means.transpose(0, 1).contiguous().transpose(0, 1)), ValueError, "contiguous"),
             (lambda: select(blocks=0), ValueError, "blocks must be 1 to 32768"),
             (lambda: select(blocks=32769), ValueError, "blocks must be 1 to 32768"),
-            (lambda: select(first=4), RuntimeError, r"first \+ last <= blocks"),
-            (lambda: select(last=0), RuntimeError, "last >= 1"),
-            (lambda: select(first=-1), RuntimeError, "first >= 0"),
+            (lambda: select(first=4), ValueError, r"first \+ last <= blocks"),
+            (lambda: select(last=0), ValueError, "last >= 1"),
+            (lambda: select(first=-1), ValueError, "first >= 0"),
             (lambda: select(page_size=24), RuntimeError, "power of two"),
             (lambda: attend(q, chosen.long()), ValueError, "blocks must be torch.int32"),
             (lambda: attend(q, chosen[1:]), ValueError, "blocks must be torch.int32"),
