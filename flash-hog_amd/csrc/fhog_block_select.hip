@@ -74,24 +74,31 @@ template <typename C, int D> __global__ void __launch_bounds__(kThreads) key_mea
   }
 }
 
-// A token's sequence and the columns it may choose from.
+// The columns that a token may choose from.
 struct TokenBlocks {
-  int b, own;         // own: the token's own column, -1 if it sees nothing
-  int lo, hi;         // columns [lo, hi) are chosen from by score
-  int room;           // how many of them
-  // most: as if its own column were the table's last at most (no token before it then chooses from more).
-  template <typename P> __device__ __forceinline__ TokenBlocks(const P& p, int t, bool most = false) {
-    const CacheShape& c = p.at;
-    b = c.offsets ? last_at_or_before(c.batch, t, [&](int s) { return packed_begin(c, s); }) : t;
-    const int begin = packed_begin(c, b), end = c.offsets ? packed_begin(c, b + 1) : b + 1;
-    const int pos = max(0, c.lengths[b]) - (end - t);
-    own = t < begin || t >= end || pos < 0 ? -1 : pos >> c.page_shift;
-    if (own >= c.pages_per_seq) own = most ? c.pages_per_seq - 1 : -1;  // a length beyond the table
+  int own;     // its own column, -1 if it sees nothing
+  int lo, hi;  // columns [lo, hi) are chosen from by score
+  int room;    // how many of them
+  // Of a position; most: as if its own column were the table's last at most (no token before it then chooses from more).
+  template <typename P> __device__ __forceinline__ TokenBlocks(const P& p, long pos, bool most = false) {
+    const long at = pos < 0 ? -1 : pos >> p.at.page_shift;
+    own = at < p.at.pages_per_seq ? (int)at : most ? p.at.pages_per_seq - 1 : -1;  // (a length beyond the table)
     lo = min(p.first, own + 1);
     hi = max(lo, own + 1 - p.last);
     room = max(0, p.blocks - lo - (own + 1 - hi));
   }
   __device__ __forceinline__ bool by_score() const { return hi - lo > room; }
+};
+
+// A packed token's sequence and position, below 0 if it is of none.
+struct TokenAt {
+  int b;
+  long pos;
+  __device__ __forceinline__ TokenAt(const CacheShape& c, int t) {
+    b = c.offsets ? last_at_or_before(c.batch, t, [&](int s) { return packed_begin(c, s); }) : t;
+    const int begin = packed_begin(c, b), end = c.offsets ? packed_begin(c, b + 1) : b + 1;
+    pos = t < begin || t >= end ? -1 : (long)max(0, c.lengths[b]) - (end - t);
+  }
 };
 
 // A score's bits in an order that compares as scores do, NaN lowest.
@@ -127,15 +134,86 @@ template <typename F> __device__ __forceinline__ uint32_t reached_by(int want, u
   return prefix;
 }
 
+// The score that sortable() made a key of.
+__device__ __forceinline__ double score_of(unsigned long key) {
+  return __builtin_bit_cast(double, key >> 63 ? key ^ 1ul << 63 : ~key);
+}
+
+// The least and the largest of a wave's lanes, in every lane.
+template <typename F> __device__ __forceinline__ float wave_reduce(float x, F&& f) {
+  auto step = [&](auto moved) { x = f(x, __builtin_bit_cast(float, moved(__builtin_bit_cast(int, x)))); };
+  // (lanes that get nothing keep their own)
+  step([](int i) { return __builtin_amdgcn_update_dpp(i, i, 0x111, 0xf, 0xf, false); });  // row_shr:1
+  step([](int i) { return __builtin_amdgcn_update_dpp(i, i, 0x112, 0xf, 0xf, false); });
+  step([](int i) { return __builtin_amdgcn_update_dpp(i, i, 0x114, 0xf, 0xf, false); });
+  step([](int i) { return __builtin_amdgcn_update_dpp(i, i, 0x118, 0xf, 0xf, false); });
+  step([](int i) { return __builtin_amdgcn_update_dpp(i, i, 0x142, 0xa, 0xf, false); });  // row_bcast:15
+  step([](int i) { return __builtin_amdgcn_update_dpp(i, i, 0x143, 0xc, 0xf, false); });  // row_bcast:31
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
 // The `room` largest of a wave's n > room keys, KJ a lane: key j of lane l is column lo + 64 j + l. Writes their
-// columns, rising, to out. The scores' upper 32 bits first: most of the time those tell the last one taken
-// from the first one left, after as many bits from the highest in which keys differ on as that takes.
+// columns, rising, to out.
+// Scores rounded to fp32 keep their order, so a value that exactly `room` of them reach tells the choice; halving
+// the range of the scores finds one as soon as it falls between the last one taken and the first one left: seven
+// or eight steps for 250 scores, where the bits of the keys, which spend the first dozen on sign and exponent,
+// take sixteen to twenty. Equal fp32 scores there, or ones that are not finite, leave it to the keys themselves.
 template <int KJ, typename F> __device__ __forceinline__ void choose_in_wave(int n, int lo, int room, int* out, F&& key_of) {
   const int lane = threadIdx.x & 63;
-  uint32_t hi[KJ], low[KJ];  // (0 where there is no key, which no value that is asked for counts)
-  uint32_t any = 0, all = ~0u;
+  const unsigned long below = (1ul << lane) - 1;
+  int at = 0;
+  auto put = [&](int j, bool take) {
+    const unsigned long takes = __ballot(take);
+    if (take) out[at + __popcll(takes & below)] = lo + 64 * j + lane;
+    at += __popcll(takes);
+  };
+  auto count = [&](auto&& which) {
+    int sum = 0;
+    if constexpr (KJ <= 4) {
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) sum += __popcll(__ballot(which(j)));
+      return sum;
+    } else {  // (a lane's own first: a ballot takes as long as four comparisons)
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) sum += which(j) ? 1 : 0;
+      return wave_sum(sum);
+    }
+  };
+  float f[KJ], least = INFINITY, most = -INFINITY;
+  bool good = true;
 #pragma unroll
   for (int j = 0; j < KJ; ++j) {  // (not in a branch a key: it would wait for each in turn)
+    const float x = (float)score_of(key_of(min(64 * j + lane, n - 1)));
+    good = good && fabsf(x) < INFINITY;
+    least = fminf(least, x), most = fmaxf(most, x);
+    f[j] = 64 * j + lane < n ? x : -INFINITY;
+  }
+  if (__all(good)) {
+    least = wave_reduce(least, [](float a, float b) { return fminf(a, b); });
+    most = wave_reduce(most, [](float a, float b) { return fmaxf(a, b); });
+    // (all reach `least`; what is reached by too few is above)
+    float above = most, middle = 0.5f * least + 0.5f * most;
+    while (middle > least && middle <= above) {
+      const int reach = count([&](int j) { return f[j] >= middle; });
+      if (reach == room) {
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+          if (64 * j < n) put(j, f[j] >= middle);
+        return;
+      }
+      if (reach > room)
+        least = middle;
+      else
+        above = middle;
+      const float next = 0.5f * least + 0.5f * above;
+      if (next == middle) break;
+      middle = next;
+    }
+  }
+  uint32_t hi[KJ], low[KJ];  // (0 where there is no key)
+  uint32_t any = 0, all = ~0u;
+#pragma unroll
+  for (int j = 0; j < KJ; ++j) {
     const unsigned long key = key_of(min(64 * j + lane, n - 1));
     const bool there = 64 * j + lane < n;
     hi[j] = there ? (uint32_t)(key >> 32) : 0;
@@ -149,39 +227,29 @@ template <int KJ, typename F> __device__ __forceinline__ void choose_in_wave(int
     all &= (uint32_t)__shfl_xor((int)all, d, 64);
   }
   any = __builtin_amdgcn_readfirstlane(any), all = __builtin_amdgcn_readfirstlane(all);
-  auto count = [&](auto&& which) {
-    int sum = 0;
-#pragma unroll
-    for (int j = 0; j < KJ; ++j)
-      if (64 * j < n) sum += __popcll(__ballot(64 * j + lane < n && which(j)));
-    return sum;
-  };
+  auto there = [&](int j) { return 64 * j + lane < n; };
   const int top = any == all ? -1 : 31 - __builtin_clz(any ^ all);
   const uint32_t same = top < 0 ? ~0u : top == 31 ? 0u : ~((2u << top) - 1);  // bits above that all keys share
   bool exact;
-  const uint32_t h = reached_by(room, all & same, top, exact, [&](uint32_t x) { return count([&](int j) { return hi[j] >= x; }); });
+  const uint32_t h = reached_by(room, all & same, top, exact, [&](uint32_t x) { return count([&](int j) { return there(j) && hi[j] >= x; }); });
   uint32_t l = 0;
   int left = 0;  // keys equal to (h, l) that are taken, if not all
   if (!exact) {
-    const int above = count([&](int j) { return hi[j] > h; });
-    l = reached_by(room - above, 0, 31, exact, [&](uint32_t x) { return count([&](int j) { return hi[j] == h && low[j] >= x; }); });
-    if (!exact) left = room - above - count([&](int j) { return hi[j] == h && low[j] > l; });
+    const int more = count([&](int j) { return there(j) && hi[j] > h; });
+    l = reached_by(room - more, 0, 31, exact, [&](uint32_t x) { return count([&](int j) { return there(j) && hi[j] == h && low[j] >= x; }); });
+    if (!exact) left = room - more - count([&](int j) { return there(j) && hi[j] == h && low[j] > l; });
   }
-  const unsigned long below = (1ul << lane) - 1;
-  int at = 0;
 #pragma unroll
   for (int j = 0; j < KJ; ++j) {
     if (64 * j >= n) continue;
-    const bool there = 64 * j + lane < n, equal = there && hi[j] == h && low[j] == l;
-    bool take = there && (hi[j] > h || (hi[j] == h && low[j] >= l));
+    const bool equal = there(j) && hi[j] == h && low[j] == l;
+    bool take = there(j) && (hi[j] > h || (hi[j] == h && low[j] >= l));
     if (!exact) {
       const unsigned long equals = __ballot(equal);
       take = take && (!equal || (int)__popcll(equals & below) < left);
       left = max(0, left - (int)__popcll(equals));
     }
-    const unsigned long takes = __ballot(take);
-    if (take) out[at + __popcll(takes & below)] = lo + 64 * j + lane;
-    at += __popcll(takes);
+    put(j, take);
   }
 }
 
@@ -193,7 +261,8 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_s
   constexpr int E = D / 16;
   const CacheShape& c = p.at;
   const int hk = blockIdx.x % c.kv_heads, t = p.token0 + blockIdx.x / c.kv_heads;
-  const TokenBlocks tb(p, t);
+  const TokenAt token(c, t);
+  const TokenBlocks tb(p, token.pos);
   if (!tb.by_score()) return;
   const int c0 = blockIdx.y * kColumns;
   if (c0 >= tb.hi || c0 + kColumns <= tb.lo) return;
@@ -209,29 +278,38 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_s
     }
   }
   unsigned long* const scores = p.scores + (long)blockIdx.x * c.pages_per_seq;
-  for (int col = c0 + way; col < min(c0 + kColumns, tb.hi); col += kThreads / 16) {
-    if (col < tb.lo) continue;
-    const int page = c.table[(long)tb.b * c.pages_per_seq + col];
-    double sum = NAN;
-    if ((unsigned)page < (unsigned)c.pages) {
-      const float* m = p.means + ((long)page * c.kv_heads + hk) * D + lane * 4;
-      sum = 0.;
+  // Its columns' pages first, then their means, then the sums.
+  constexpr int kEach = kColumns * 16 / kThreads;
+  const int* const table = c.table + (long)token.b * c.pages_per_seq;
+  int page[kEach];
+  f32x4 m[kEach][E / 4];
 #pragma unroll
-      for (int j = 0; j < E; j += 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(m + 16 * j);
+  for (int i = 0; i < kEach; ++i) page[i] = table[min(c0 + way + 16 * i, tb.hi - 1)];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum = fma(q[j + e], (double)x[e], sum);
-      }
+  for (int i = 0; i < kEach; ++i) {
+    const bool bad = (unsigned)page[i] >= (unsigned)c.pages;
+    const float* from = p.means + ((long)(bad ? 0 : page[i]) * c.kv_heads + hk) * D + lane * 4;
 #pragma unroll
-      for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    }
-    if (lane == 0) scores[col] = sortable(sum);
+    for (int j = 0; j < E / 4; ++j) m[i][j] = *reinterpret_cast<const f32x4*>(from + 64 * j);
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    double sum = 0.;
+#pragma unroll
+    for (int j = 0; j < E / 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = fma(q[4 * j + e], (double)m[i][j][e], sum);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    const int col = c0 + way + 16 * i;
+    if (lane == 0 && col >= tb.lo && col < tb.hi) scores[col] = (unsigned)page[i] < (unsigned)c.pages ? sortable(sum) : 0;
   }
 }
 
 // Tiles of 16 tokens of a sequence, for many of them: a sequence's tiles start at offset / 16 + index.
 struct TokenTile {
   int b, t0, count;
+  long pos;  // of the first one
   template <typename P> __device__ __forceinline__ TokenTile(const P& p, int slot) {
     const CacheShape& c = p.at;
     auto first_slot = [&](int s) { return packed_begin(c, s) / 16 + s; };
@@ -240,6 +318,7 @@ struct TokenTile {
     const long at = begin + 16l * (slot - first_slot(b));  // (a wrong slot's too)
     t0 = (int)at;
     count = at < begin || at >= end ? 0 : (int)(end - at < 16 ? end - at : 16);
+    pos = (long)max(0, c.lengths[b]) - (end - at);
   }
 };
 
@@ -261,21 +340,34 @@ __device__ __forceinline__ void score_tile(const BlockSelectParams<T>& p, const 
 #pragma unroll
       for (int e = 0; e < 8; ++e) q[k + e] += (double)(float)x[e];
     }
+  // A step's means are loaded a step ahead, their pages another one.
+  constexpr int kStep = 16 * (kThreads / 64);
   const int* const table = c.table + (long)tile.b * c.pages_per_seq;
-  for (int col0 = c0 + 16 * (int)(threadIdx.x >> 6); col0 < c1; col0 += 16 * (kThreads / 64)) {
-    const int col = min(col0 + n, c1 - 1), page = table[col];
-    const bool bad = (unsigned)page >= (unsigned)c.pages;
-    const float* m = p.means + ((long)(bad ? 0 : page) * c.kv_heads + hk) * D + g * K;
+  auto page_of = [&](int col0) { return table[min(col0 + n, c1 - 1)]; };
+  f32x4 m[K / 4];
+  auto load = [&](int page) {
+    const float* from = p.means + ((long)((unsigned)page < (unsigned)c.pages ? page : 0) * c.kv_heads + hk) * D + g * K;
+#pragma unroll
+    for (int k = 0; k < K / 4; ++k) m[k] = *reinterpret_cast<const f32x4*>(from + 4 * k);
+  };
+  int col0 = c0 + 16 * (int)(threadIdx.x >> 6);
+  if (col0 >= c1) return;
+  int page = page_of(col0), ahead = page_of(col0 + kStep);
+  load(page);
+  for (; col0 < c1; col0 += kStep) {
     f64x4 sum = {0., 0., 0., 0.};
+    f32x4 x[K / 4];
 #pragma unroll
-    for (int k = 0; k < K; k += 4) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(m + k);
+    for (int k = 0; k < K / 4; ++k) x[k] = m[k];
+    const bool bad = (unsigned)page >= (unsigned)c.pages;
+    page = ahead;
+    ahead = page_of(col0 + 2 * kStep);
+    if (col0 + kStep < c1) load(page);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f64_16x16x4f64(q[k + e], (double)x[e], sum, 0, 0, 0);
-    }
+    for (int k = 0; k < K; ++k) sum = __builtin_amdgcn_mfma_f64_16x16x4f64(q[k], (double)x[k / 4][k % 4], sum, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (col0 + n < c1) put(g + 4 * i, col, bad ? 0ul : sortable(sum[i]));
+      if (col0 + n < c1) put(g + 4 * i, col0 + n, bad ? 0ul : sortable(sum[i]));
   }
 }
 
@@ -283,27 +375,27 @@ __device__ __forceinline__ void score_tile(const BlockSelectParams<T>& p, const 
 template <typename T, int D, int COLUMNS> __global__ void __launch_bounds__(kThreads) block_select_tile_kernel(BlockSelectParams<T> p) {
   __shared__ unsigned long s_key[16][COLUMNS + 2];  // (rows apart, so that a column's keys are in different banks)
   const CacheShape& c = p.at;
-  const int hk = blockIdx.x % c.kv_heads;
-  const TokenTile tile(p, blockIdx.x / c.kv_heads);
+  const int hk = blockIdx.x % c.kv_heads, slot = blockIdx.x / c.kv_heads;
+  const TokenTile tile(p, slot);
+  // The lists of packed rows that no sequence has: a slot looks after sixteen rows (there are slots enough).
+  const int first = packed_begin(c, 0), behind = packed_begin(c, c.batch);
+  for (int i = threadIdx.x; i < 16 * p.blocks; i += kThreads) {
+    const long t = 16l * slot + i / p.blocks;
+    if (t < c.total && (t < first || t >= behind)) p.chosen[(t * c.kv_heads + hk) * p.blocks + i % p.blocks] = -1;
+  }
   if (tile.count <= 0) return;
-  const TokenBlocks last(p, tile.t0 + tile.count - 1, true);
+  const TokenBlocks last(p, tile.pos + tile.count - 1, true);
   const int lo = min(p.first, c.pages_per_seq);
   if (last.by_score()) score_tile<T, D>(p, tile, hk, lo, last.hi, [&](int row, int col, unsigned long key) { s_key[row][col - lo] = key; });
   __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int r = wave; r < tile.count; r += kThreads / 64) {
-    const TokenBlocks tb(p, tile.t0 + r);
+    const TokenBlocks tb(p, tile.pos + r);
     int* const out = p.chosen + ((long)(tile.t0 + r) * c.kv_heads + hk) * p.blocks;
     write_forced(tb, out, p.blocks, threadIdx.x & 63, 64);
     if (tb.by_score() && tb.room > 0)
       choose_in_wave<COLUMNS / 64>(tb.hi - tb.lo, tb.lo, tb.room, out + tb.lo, [&](int i) { return s_key[r][i]; });
   }
-}
-
-// Empty lists, before the tiles write theirs: those of packed rows that no sequence has stay so.
-template <typename T> __global__ void __launch_bounds__(kThreads) block_none_kernel(BlockSelectParams<T> p) {
-  const long i = (long)blockIdx.x * kThreads + threadIdx.x;
-  if (i < (long)p.at.total * p.at.kv_heads * p.blocks) p.chosen[i] = -1;
 }
 
 // Scores of a tile's tokens, in the slab, into memory, for wider tables: kWide columns a workgroup.
@@ -313,7 +405,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_s
   const int hk = blockIdx.x % c.kv_heads;
   const TokenTile tile(p, blockIdx.x / c.kv_heads);
   if (tile.count <= 0 || tile.t0 >= p.token0 + p.tokens || tile.t0 + tile.count <= p.token0) return;
-  const TokenBlocks last(p, tile.t0 + tile.count - 1, true);
+  const TokenBlocks last(p, tile.pos + tile.count - 1, true);
   if (!last.by_score()) return;
   const int c0 = max(last.lo, (int)blockIdx.y * kWide), c1 = min(last.hi, ((int)blockIdx.y + 1) * kWide);
   if (c0 >= c1) return;
@@ -331,7 +423,7 @@ template <typename T, int COLUMNS> __global__ void __launch_bounds__(kThreads) b
   const long i = (long)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= (long)p.tokens * c.kv_heads) return;
   const int hk = (int)(i % c.kv_heads), t = p.token0 + (int)(i / c.kv_heads);
-  const TokenBlocks tb(p, t);
+  const TokenBlocks tb(p, TokenAt(c, t).pos);
   int* const out = p.chosen + ((long)t * c.kv_heads + hk) * p.blocks;
   write_forced(tb, out, p.blocks, threadIdx.x & 63, 64);
   if (!tb.by_score() || tb.room == 0) return;
@@ -345,7 +437,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) block_choose_k
   __shared__ int hist[256], box[4], found[3];
   const CacheShape& c = p.at;
   const int hk = blockIdx.x % c.kv_heads, t = p.token0 + blockIdx.x / c.kv_heads;
-  const TokenBlocks tb(p, t);
+  const TokenBlocks tb(p, TokenAt(c, t).pos);
   int* const out = p.chosen + ((long)t * c.kv_heads + hk) * p.blocks;
   write_forced(tb, out, p.blocks, threadIdx.x, kThreads);
   if (!tb.by_score() || tb.room == 0) return;
@@ -404,8 +496,6 @@ template <typename T, int D> hipError_t launch_block_select(const BlockSelectPar
   const int width = p.at.pages_per_seq, most = width - p.first - p.last;  // columns chosen from
   if (plan.tiles && most <= kFusedColumns) {
     const dim3 grid((unsigned)((long)plan.slots * p.at.kv_heads));
-    const long elements = (long)p.at.total * p.at.kv_heads * p.blocks;
-    hipLaunchKernelGGL((block_none_kernel<T>), dim3((unsigned)((elements + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, p);
     if (most <= 256)
       hipLaunchKernelGGL((block_select_tile_kernel<T, D, 256>), grid, dim3(kThreads), 0, stream, p);
     else if (most <= 512)

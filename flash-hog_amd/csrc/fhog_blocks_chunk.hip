@@ -84,30 +84,41 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   if (threadIdx.x == 0) p.falling[(long)hk * p.groups + group] = s_falling;
 }
 
-// A thread a list: its entries and tiles get places behind others', a wave at a time (in any order: each tile's
-// outputs have places of their own).
-template <typename T, typename C> __global__ void __launch_bounds__(64) block_items_kernel(BlockChunkParams<T, C> p) {
+// Four threads a list, each a quarter of the groups, and then the first: the list's entries and tiles get places
+// behind others', a wave at a time (in any order: each tile's outputs have places of their own).
+template <typename T, typename C> __global__ void __launch_bounds__(kThreads) block_items_kernel(BlockChunkParams<T, C> p) {
+  __shared__ int s_count[4][64];
   const CacheShape& c = p.at;
-  const int i = blockIdx.x * 64 + threadIdx.x, width = c.pages_per_seq, group = p.heads / c.kv_heads;
-  int count = 0, col = 0, hk = 0, b = 0;
+  const int way = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 64 + lane, width = c.pages_per_seq, group = p.heads / c.kv_heads;
+  int count = 0, col = 0, hk = 0, b = 0, begin = 0, end = 0, g0 = 0, g1 = 0;
+  long at = 0;
   if (i < p.lists) {
     col = i % width, hk = i / width % c.kv_heads, b = i / width / c.kv_heads;
-    int begin, end;
     slab_range(p, b, begin, end);
-    const long at = (long)hk * p.groups * width + col;
-    const int g0 = begin / 64, g1 = (end + 63) / 64;
-#pragma unroll 8
-    for (int g = g0; g < g1; ++g) {
-      const unsigned long bits = p.masks[at + (long)g * width] & group_bits(g, begin, end);
-      // (a group that begins with an earlier sequence's tokens is that one's: this one's count there is 0)
-      if (g > g0) p.before[at + (long)g * width] = count;
-      count += __popcll(bits);
-    }
+    at = (long)hk * p.groups * width + col;
+    const int first = begin / 64, last = max(first, (end + 63) / 64), each = (last - first + 3) / 4;
+    g0 = min(last, first + way * each), g1 = min(last, g0 + each);
   }
+#pragma unroll 8
+  for (int g = g0; g < g1; ++g) count += __popcll(p.masks[at + (long)g * width] & group_bits(g, begin, end));
+  s_count[way][lane] = count;
+  __syncthreads();
+  int earlier = 0;
+  for (int w = 0; w < way; ++w) earlier += s_count[w][lane];
+  // (a group that begins with an earlier sequence's tokens is that one's: this one's count there is 0)
+#pragma unroll 8
+  for (int g = g0; g < g1; ++g) {
+    if (g > begin / 64) p.before[at + (long)g * width] = earlier;
+    earlier += __popcll(p.masks[at + (long)g * width] & group_bits(g, begin, end));
+  }
+  if (way > 0) return;
+  count = s_count[0][lane] + s_count[1][lane] + s_count[2][lane] + s_count[3][lane];
   const int tiles = (int)(((long)count * group + kTileRows - 1) / kTileRows);
   int sums[2], first[2];
   const int before[2] = {wave_scan(tiles, sums[0]), wave_scan(count, sums[1])};
-  if (threadIdx.x < 2) first[0] = atomicAdd(&p.totals[threadIdx.x], sums[threadIdx.x]);
+  first[0] = 0;
+  if (lane < 2) first[0] = atomicAdd(&p.totals[lane], lane ? sums[1] : sums[0]);
   first[1] = __shfl(first[0], 1, 64);
   first[0] = __shfl(first[0], 0, 64);
   if (count == 0) return;
@@ -398,7 +409,7 @@ hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p_, int slab, hipStr
     p.groups = (p.tokens + 63) / 64;
     const long most = (long)p.tokens * p.blocks * p.heads / kTileRows + p.lists;
     hipLaunchKernelGGL((block_masks_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((block_items_kernel<T, C>), dim3((p.lists + 63) / 64), dim3(64), 0, stream, p);
+    hipLaunchKernelGGL((block_items_kernel<T, C>), dim3((p.lists + 63) / 64), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_entries_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_tile_kernel<T, C, D>), dim3((unsigned)most), dim3(kThreads), 0, stream, p);
     constexpr long R = kThreads / (D / 4);
