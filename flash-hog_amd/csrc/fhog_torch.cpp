@@ -37,6 +37,7 @@
 
 #include <cstdint>
 #include <sstream>
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -61,6 +62,18 @@ struct Api {
   decltype(&fhog_paged_attention) paged_attention = nullptr;
   decltype(&fhog_paged_cache_write) cache_write = nullptr;
   decltype(&fhog_paged_cache_read) cache_read = nullptr;
+  decltype(&fhog_paged_pages_workspace_bytes) pages_bytes = nullptr;
+  decltype(&fhog_paged_cache_extend) cache_extend = nullptr;
+  decltype(&fhog_paged_cache_compact) cache_compact = nullptr;
+  decltype(&fhog_paged_key_means) key_means = nullptr;
+  decltype(&fhog_paged_block_select_workspace_bytes) select_bytes = nullptr;
+  decltype(&fhog_paged_block_select) block_select = nullptr;
+  decltype(&fhog_paged_block_workspace_bytes) block_bytes = nullptr;
+  decltype(&fhog_paged_block_attention) block_attention = nullptr;
+  decltype(&fhog_qk_norm_rotary_workspace_bytes) rotary_bytes = nullptr;
+  decltype(&fhog_qk_norm_rotary_fwd) rotary_fwd = nullptr;
+  decltype(&fhog_qk_norm_rotary_bwd) rotary_bwd = nullptr;
+  decltype(&fhog_qk_norm_rotary_bwdbwd) rotary_bwdbwd = nullptr;
   py::object error_cls;
 };
 
@@ -94,6 +107,31 @@ void bind_paged(std::uintptr_t bytes, std::uintptr_t attention, std::uintptr_t w
   a.paged_attention = reinterpret_cast<decltype(a.paged_attention)>(attention);
   a.cache_write = reinterpret_cast<decltype(a.cache_write)>(write);
   a.cache_read = reinterpret_cast<decltype(a.cache_read)>(read);
+}
+
+void bind_pages(std::uintptr_t bytes, std::uintptr_t extend, std::uintptr_t compact) {
+  Api& a = api();
+  a.pages_bytes = reinterpret_cast<decltype(a.pages_bytes)>(bytes);
+  a.cache_extend = reinterpret_cast<decltype(a.cache_extend)>(extend);
+  a.cache_compact = reinterpret_cast<decltype(a.cache_compact)>(compact);
+}
+
+void bind_blocks(std::uintptr_t means, std::uintptr_t select_bytes, std::uintptr_t select, std::uintptr_t bytes,
+                 std::uintptr_t attention) {
+  Api& a = api();
+  a.key_means = reinterpret_cast<decltype(a.key_means)>(means);
+  a.select_bytes = reinterpret_cast<decltype(a.select_bytes)>(select_bytes);
+  a.block_select = reinterpret_cast<decltype(a.block_select)>(select);
+  a.block_bytes = reinterpret_cast<decltype(a.block_bytes)>(bytes);
+  a.block_attention = reinterpret_cast<decltype(a.block_attention)>(attention);
+}
+
+void bind_rotary(std::uintptr_t bytes, std::uintptr_t fwd, std::uintptr_t bwd, std::uintptr_t bwdbwd) {
+  Api& a = api();
+  a.rotary_bytes = reinterpret_cast<decltype(a.rotary_bytes)>(bytes);
+  a.rotary_fwd = reinterpret_cast<decltype(a.rotary_fwd)>(fwd);
+  a.rotary_bwd = reinterpret_cast<decltype(a.rotary_bwd)>(bwd);
+  a.rotary_bwdbwd = reinterpret_cast<decltype(a.rotary_bwdbwd)>(bwdbwd);
 }
 
 std::string shape_str(const at::Tensor& t) {
@@ -486,6 +524,328 @@ std::tuple<at::Tensor, at::Tensor> cache_read_core(const at::Tensor& k_cache, co
   return {k, v};
 }
 
+// ------------------------------------------------- the cache's allocator, chosen blocks
+
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  const char *a = (const char*)x.data_ptr(), *b = (const char*)y.data_ptr();
+  return a < b + y.nbytes() && b < a + x.nbytes();
+}
+
+at::Tensor bytes_on(const at::Tensor& like, size_t size) {
+  return size ? at::empty({(int64_t)size}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+at::Tensor cache_extend_core(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table,
+                             const at::Tensor& lengths, const MaybeTensor& new_tokens, int new_each,
+                             const MaybeTensor& parents, const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  const Cache c("key_cache", k_cache, k_cache, v_cache, table, lengths, c10::nullopt, k_scale, v_scale,
+                k_cache.scalar_type());
+  for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"page_table", &table}, {"lengths", &lengths}})
+    if (!t->is_contiguous()) value_error(std::string(name) + " must be contiguous");
+  at::Tensor held[2];  // parents, new_tokens
+  int i = 0;
+  for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"parents", get(parents)},
+                                {"new_tokens", get(new_tokens)}}) {
+    at::Tensor& to = held[i++];
+    if (!t) continue;
+    check_inputs({{"key_cache", &k_cache}, {name, t}}, c10::nullopt);
+    expect(name, *t, {table.size(0)}, at::kInt);
+    if (overlap(*t, table) || overlap(*t, lengths))
+      value_error(std::string(name) + " overlaps page_table or lengths");
+    to = contig(*t);
+  }
+  if (c.batch == 0) value_error("expected at least one row of page_table");
+  at::Tensor free = at::empty({}, lengths.options());
+  c10::DeviceGuard guard(k_cache.device());
+  const size_t size = api().pages_bytes(c.batch, c.pages, c.width);
+  const at::Tensor ws = bytes_on(k_cache, size);
+  check_status(api().cache_extend(current_stream(k_cache), k_cache.data_ptr(), v_cache.data_ptr(),
+                                  const_cast<void*>(ptr(c.k_scale)), const_cast<void*>(ptr(c.v_scale)),
+                                  table.data_ptr<int>(), lengths.data_ptr<int>(), (const int*)data_or_null(held[0]),
+                                  (const int*)data_or_null(held[1]), new_each, free.data_ptr<int>(), data_or_null(ws), size,
+                                  c.batch, c.kv_heads, c.head_dim, c.pages, c.page, c.width, c.dtype));
+  for (const at::Tensor* t : {&k_cache, &v_cache, c.k_scale, c.v_scale, &table, &lengths})
+    if (t) written(*t);
+  return free;
+}
+
+void check_key_means(const at::Tensor& means, const char* first_name, const at::Tensor& first, at::IntArrayRef shape) {
+  check_inputs({{first_name, &first}, {"key_means", &means}}, c10::nullopt);
+  expect("key_means", means, shape, at::kFloat);
+  if (!means.is_contiguous()) value_error("key_means must be contiguous");
+}
+
+// (k_cache, v_cache, k_scale, v_scale, key_means, page_table), undefined for what is not given.
+std::tuple<at::Tensor, at::Tensor, MaybeTensor, MaybeTensor, MaybeTensor, at::Tensor> cache_compact_core(
+    const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& lengths,
+    int64_t num_pages, const MaybeTensor& k_scale, const MaybeTensor& v_scale, const MaybeTensor& key_means) {
+  const Cache c("key_cache", k_cache, k_cache, v_cache, table, lengths, c10::nullopt, k_scale, v_scale,
+                k_cache.scalar_type());
+  const at::Tensor* means = get(key_means);
+  if (means) check_key_means(*means, "key_cache", k_cache, {k_cache.size(0), k_cache.size(1), k_cache.size(3)});
+  if (num_pages < 1 || num_pages > INT32_MAX)
+    value_error("num_pages must be >= 1 and below 2 ** 31, got " + std::to_string(num_pages));
+  const at::Tensor* in[5] = {&k_cache, &v_cache, c.k_scale, c.v_scale, means};
+  at::Tensor out[5];
+  for (int i = 0; i < 5; ++i)
+    if (in[i]) {
+      std::vector<int64_t> shape = in[i]->sizes().vec();
+      shape[0] = num_pages;
+      out[i] = at::empty(shape, in[i]->options());
+    }
+  at::Tensor table_out = at::empty(table.sizes(), table.options());
+  c10::DeviceGuard guard(k_cache.device());
+  const size_t size = api().pages_bytes(c.batch, c.pages, c.width);
+  const at::Tensor ws = bytes_on(k_cache, size);
+  check_status(api().cache_compact(
+      current_stream(k_cache), k_cache.data_ptr(), v_cache.data_ptr(), ptr(c.k_scale), ptr(c.v_scale), (const float*)ptr(means),
+      c.table_ptr(), c.lengths_ptr(), out[0].data_ptr(), out[1].data_ptr(), data_or_null(out[2]), data_or_null(out[3]),
+      (float*)data_or_null(out[4]), table_out.data_ptr<int>(), data_or_null(ws), size, c.batch, c.kv_heads, c.head_dim, c.pages,
+      c.page, c.width, (int)num_pages, c.dtype));
+  auto maybe = [](const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };  // None in Python
+  return {out[0], out[1], maybe(out[2]), maybe(out[3]), maybe(out[4]), table_out};
+}
+
+void key_means_core(const at::Tensor& k_cache, const at::Tensor& means, const at::Tensor& table, const at::Tensor& lengths,
+                    const MaybeTensor& offsets, const MaybeTensor& k_scale) {
+  const Cache c("key_cache", k_cache, k_cache, k_cache, table, lengths, offsets, k_scale, k_scale, k_cache.scalar_type());
+  check_key_means(means, "key_cache", k_cache, {k_cache.size(0), k_cache.size(1), k_cache.size(3)});
+  if (overlap(means, k_cache)) value_error("key_means overlaps key_cache");
+  c10::DeviceGuard guard(k_cache.device());
+  check_status(api().key_means(current_stream(k_cache), k_cache.data_ptr(), ptr(c.k_scale), means.data_ptr<float>(),
+                               c.table_ptr(), c.lengths_ptr(), c.offsets_ptr(), c.batch, c.kv_heads, c.head_dim, c.pages,
+                               c.page, c.width, c.dtype));
+  written(means);
+}
+
+at::Tensor block_select_core(const at::Tensor& q_, const at::Tensor& means, const at::Tensor& table,
+                             const at::Tensor& lengths, const MaybeTensor& offsets_, int64_t page_size, int64_t blocks,
+                             int64_t first, int64_t last) {
+  const int total = rows_of("query", q_);
+  if (means.dim() != 3 || means.size(2) != q_.size(2))
+    value_error("expected (pages, kv_heads, head_dim) key_means for query" + shape_str(q_) + ", got " + shape_str(means));
+  check_key_means(means, "query", q_, means.sizes());
+  const at::Tensor* off = get(offsets_);
+  check_inputs({{"query", &q_}, {"page_table", &table}, {"lengths", &lengths}}, c10::nullopt);
+  if (off) check_inputs({{"query", &q_}, {"query_offsets", off}}, c10::nullopt);
+  if (table.dim() != 2) value_error("expected a (batch, pages) page_table, got " + shape_str(table));
+  expect("lengths", lengths, {table.size(0)});
+  if (off) expect("query_offsets", *off, {table.size(0) + 1});
+  for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"page_table", &table},
+                                {"lengths", &lengths}, {"query_offsets", off}})
+    if (t && t->scalar_type() != at::kInt)
+      value_error(std::string(name) + " has dtype " + dtype_str(t->scalar_type()) + ", expected torch.int32");
+  const int dt = dtype_code(q_.scalar_type());
+  for (int64_t s : {means.size(0), means.size(1), table.size(0), table.size(1), page_size})
+    if (s > INT32_MAX) value_error("a size is beyond the C ABI's int range");
+  if (blocks < 1 || blocks > 32768) value_error("blocks must be 1 to 32768, got " + std::to_string(blocks));
+  if (first < 0 || last < 1 || first + last > blocks)
+    value_error("needs first >= 0, last >= 1 and first + last <= blocks, got " + std::to_string(first) + ", " +
+                std::to_string(last) + " and " + std::to_string(blocks));
+  const at::Tensor q = contig(q_), t = contig(table), n = contig(lengths), o = off ? contig(*off) : at::Tensor();
+  const int kv = (int)means.size(1), batch = (int)table.size(0), width = (int)table.size(1);
+  at::Tensor chosen = at::empty({(int64_t)total, (int64_t)kv, blocks}, t.options());
+  c10::DeviceGuard guard(q.device());
+  const size_t size = api().select_bytes(batch, total, !off, kv, width, (int)first, (int)last);
+  const at::Tensor ws = bytes_on(q, size);
+  check_status(api().block_select(current_stream(q), q.data_ptr(), means.data_ptr<float>(), t.data_ptr<int>(),
+                                  n.data_ptr<int>(), (const int*)data_or_null(o), chosen.data_ptr<int>(), data_or_null(ws),
+                                  size, batch, total, (int)q.size(1), kv, (int)q.size(2), (int)means.size(0), (int)page_size,
+                                  width, dt, (int)blocks, (int)first, (int)last));
+  return chosen;
+}
+
+at::Tensor block_attention_core(const at::Tensor& q_, const at::Tensor& chosen_, const at::Tensor& k_cache,
+                                const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& lengths,
+                                const MaybeTensor& offsets, const MaybeTensor& k_scale, const MaybeTensor& v_scale,
+                                double scale, const MaybeTensor& out_) {
+  const int total = rows_of("query", q_);
+  const Cache c("query", q_, k_cache, v_cache, table, lengths, offsets, k_scale, v_scale, q_.scalar_type());
+  if (q_.size(2) != c.head_dim)
+    value_error("query" + shape_str(q_) + " and key_cache" + shape_str(k_cache) + " disagree on head_dim");
+  const int dt = dtype_code(q_.scalar_type());
+  check_inputs({{"query", &q_}, {"blocks", &chosen_}}, c10::nullopt);
+  if (chosen_.dim() != 3 || chosen_.size(0) != total || chosen_.size(1) != c.kv_heads || chosen_.scalar_type() != at::kInt)
+    value_error("blocks must be torch.int32 (" + std::to_string(total) + ", " + std::to_string(c.kv_heads) +
+                ", 'blocks'), got " + shape_str(chosen_) + " of " + dtype_str(chosen_.scalar_type()));
+  if (chosen_.size(2) > INT32_MAX) value_error("blocks has a dimension beyond the C ABI's int range");
+  const at::Tensor* given = get(out_);
+  if (given) {
+    check_inputs({{"query", &q_}, {"out", given}}, q_.scalar_type());
+    expect("out", *given, q_.sizes());
+    if (!given->is_contiguous()) value_error("out must be contiguous");
+  }
+  at::Tensor out = given ? *given : at::empty(q_.sizes(), q_.options());
+  const at::Tensor q = contig(q_), chosen = contig(chosen_);
+  if (given) {
+    check_apart(out, "query", q, false);
+    check_apart(out, "blocks", chosen, false);
+    check_apart(out, "key_cache", k_cache, false);
+    check_apart(out, "value_cache", v_cache, false);
+  }
+  const int heads = (int)q.size(1), blocks = (int)chosen.size(2), single = !c.offsets.defined();
+  c10::DeviceGuard guard(q.device());
+  const size_t size = api().block_bytes(c.batch, total, single, heads, c.kv_heads, c.head_dim, c.page, c.width, blocks);
+  const at::Tensor ws = bytes_on(q, size);
+  check_status(api().block_attention(current_stream(q), q.data_ptr(), chosen.data_ptr<int>(), k_cache.data_ptr(),
+                                     v_cache.data_ptr(), ptr(c.k_scale), ptr(c.v_scale), c.table_ptr(), c.lengths_ptr(),
+                                     c.offsets_ptr(), out.data_ptr(), data_or_null(ws), size, c.batch, total, heads,
+                                     c.kv_heads, c.head_dim, c.pages, c.page, c.width, dt, c.dtype, blocks,
+                                     given == nullptr, (float)scale));
+  if (given) written(out);
+  return out;
+}
+
+// ------------------------------------------------- norms with rotation
+
+// What the three calls share, checked (_hip.py _RotaryCall); q and k of three axes are unbatched. Where the rows are
+// not read (`rows` false), q and k only give their shapes.
+struct RotaryOptions {
+  bool interleaved;
+  c10::optional<double> eps;
+};
+struct RotaryWhere {
+  at::Tensor frequencies, positions, lengths, offsets;  // undefined: none
+};
+struct RotaryCall {
+  at::Tensor q, k, wq, wk;
+  RotaryWhere at;
+  fhog_rotary shape{};
+
+  RotaryCall(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& wq_, const at::Tensor& wk_,
+             const RotaryWhere& where, const RotaryOptions& o, bool rows) {
+    check_inputs({{"query", &q_}, {"key", &k_}}, c10::nullopt);
+    for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"query_weight", &wq_}, {"key_weight", &wk_},
+                                  {"frequencies", &where.frequencies}, {"positions", &where.positions},
+                                  {"lengths", &where.lengths}, {"query_offsets", &where.offsets}})
+      if (t->defined()) check_inputs({{"query", &q_}, {name, t}}, c10::nullopt);
+    check_inputs({{"query", &q_}, {"key", &k_}}, q_.scalar_type());
+    const int dt = dtype_code(q_.scalar_type());
+    const int64_t d = q_.dim();
+    if ((d != 3 && d != 4) || k_.dim() != d || q_.size(0) != k_.size(0) || (d == 4 && q_.size(1) != k_.size(1)) ||
+        q_.size(d - 1) != k_.size(d - 1))
+      value_error("expected query (B, T, N, H) and key (B, T, N_kv, H) of the same tokens and head_dim, got " +
+                  shape_str(q_) + " and " + shape_str(k_));
+    const int64_t B = d == 4 ? q_.size(0) : 1, T = q_.size(d - 3), H = q_.size(d - 1);
+    for (int64_t s : {B, T, q_.size(d - 2), k_.size(d - 2), H})
+      if (s > INT32_MAX) value_error("query" + shape_str(q_) + " has a dimension beyond the C ABI's int range");
+    if (!o.eps && (wq_.defined() || wk_.defined())) value_error("weights need norms (eps is None)");
+    const at::ScalarType wt = wq_.defined() ? wq_.scalar_type() : wk_.defined() ? wk_.scalar_type() : q_.scalar_type();
+    if (wq_.defined()) expect("query_weight", wq_, {H}, wt);
+    if (wk_.defined()) expect("key_weight", wk_, {H}, wt);
+    if (wt != q_.scalar_type() && wt != at::kFloat)
+      value_error("weights must be of " + dtype_str(q_.scalar_type()) + " or torch.float32, got " + dtype_str(wt));
+    const at::Tensor &f = where.frequencies, &p = where.positions, &n = where.lengths, &off = where.offsets;
+    if (f.defined() && (f.dim() != 1 || 2 * f.size(0) > H || f.scalar_type() != at::kFloat))
+      value_error("frequencies must be torch.float32 (R / 2,) with R <= head_dim, got " + shape_str(f) + " of " +
+                  dtype_str(f.scalar_type()) + " for head_dim " + std::to_string(H));
+    if (p.defined()) {
+      if (n.defined()) value_error("positions and lengths exclude each other");
+      if (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong)
+        value_error("positions has dtype " + dtype_str(p.scalar_type()) + ", expected torch.int32 or torch.int64");
+      if (!(p.dim() == 1 && p.size(0) == T) && !(p.dim() == 2 && p.size(0) == B && p.size(1) == T))
+        value_error("positions has shape " + shape_str(p) + ", expected (" + std::to_string(T) + ",) or (" +
+                    std::to_string(B) + ", " + std::to_string(T) + ")");
+    }
+    if (off.defined() && !n.defined()) value_error("query_offsets needs lengths");
+    if (n.defined()) {
+      if (n.dim() != 1) value_error("expected (batch,) lengths, got " + shape_str(n));
+      if (B != 1) value_error("lengths go with packed tokens (T, N, H), got a batch of " + std::to_string(B));
+      if (off.defined())
+        expect("query_offsets", off, {n.size(0) + 1});
+      else
+        expect("lengths", n, {T});
+      for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"lengths", &n}, {"query_offsets", &off}})
+        if (t->defined() && t->scalar_type() != at::kInt)
+          value_error(std::string(name) + " has dtype " + dtype_str(t->scalar_type()) + ", expected torch.int32");
+    }
+    auto lines = [&](const at::Tensor& t) { return !rows || t.stride(d - 1) == 1 || H == 1 ? t : t.contiguous(); };
+    q = lines(q_), k = lines(k_);
+    auto held = [](const at::Tensor& t) { return t.defined() ? contig(t) : t; };
+    wq = held(wq_), wk = held(wk_);
+    at = {held(f), held(p), held(n), held(off)};
+    shape.batch = (int)B, shape.tokens = (int)T, shape.heads = (int)q.size(d - 2), shape.kv_heads = (int)k.size(d - 2);
+    shape.head_dim = (int)H, shape.rotated = f.defined() ? 2 * (int)f.size(0) : 0;
+    shape.dtype = dt, shape.weight_dtype = dtype_code(wt);
+    shape.interleaved = o.interleaved, shape.norm = o.eps.has_value(), shape.eps = o.eps ? (float)*o.eps : 0.f;
+    shape.position_bytes = p.defined() ? (int)p.element_size() : 0;
+    shape.position_rows = !p.defined() ? 0 : p.dim() == 1 ? 1 : (int)B;
+    shape.sequences = n.defined() ? (int)n.size(0) : 0;
+    for (int i = 0; i < 3; ++i) {
+      const int64_t axis = i + d - 4;
+      shape.q_stride[i] = axis < 0 ? 0 : q.stride(axis);
+      shape.k_stride[i] = axis < 0 ? 0 : k.stride(axis);
+    }
+    shape.frequencies = (const float*)data_or_null(at.frequencies);
+    shape.positions = data_or_null(at.positions);
+    shape.lengths = (const int*)data_or_null(at.lengths);
+    shape.query_offsets = (const int*)data_or_null(at.offsets);
+  }
+  at::Tensor like(const at::Tensor& t) const { return at::empty(t.sizes(), t.options()); }
+  at::Tensor like_weight(const at::Tensor& w) const { return w.defined() ? at::empty(w.sizes(), w.options()) : w; }
+  // A tensor of q's (or k's) shape, contiguous.
+  at::Tensor rows(const char* name, const at::Tensor& t, const at::Tensor& x) const {
+    check_inputs({{"query", &q}, {name, &t}}, q.scalar_type());
+    expect(name, t, x.sizes());
+    return contig(t);
+  }
+  at::Tensor workspace() const {
+    return wq.defined() || wk.defined() ? bytes_on(q, api().rotary_bytes(&shape)) : at::Tensor();
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> rotary_fwd_core(const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq,
+                                                   const at::Tensor& wk, const RotaryWhere& where,
+                                                   const RotaryOptions& o) {
+  const RotaryCall c(q, k, wq, wk, where, o, true);
+  at::Tensor q_out = c.like(c.q), k_out = c.like(c.k);
+  c10::DeviceGuard guard(c.q.device());
+  check_status(api().rotary_fwd(current_stream(c.q), &c.shape, c.q.data_ptr(), c.k.data_ptr(), data_or_null(c.wq),
+                                data_or_null(c.wk), q_out.data_ptr(), k_out.data_ptr()));
+  return {q_out, k_out};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rotary_bwd_core(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& gq_,
+    const at::Tensor& gk_, const RotaryWhere& where, const RotaryOptions& o) {
+  const RotaryCall c(q, k, wq, wk, where, o, o.eps.has_value());
+  const at::Tensor gq = c.rows("query's cotangent", gq_, c.q), gk = c.rows("key's cotangent", gk_, c.k);
+  at::Tensor dq = c.like(c.q), dk = c.like(c.k), dwq = c.like_weight(c.wq), dwk = c.like_weight(c.wk);
+  c10::DeviceGuard guard(c.q.device());
+  const at::Tensor ws = c.workspace();
+  check_status(api().rotary_bwd(current_stream(c.q), &c.shape, o.eps ? c.q.data_ptr() : nullptr,
+                                o.eps ? c.k.data_ptr() : nullptr, data_or_null(c.wq), data_or_null(c.wk), gq.data_ptr(),
+                                gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), data_or_null(dwq), data_or_null(dwk),
+                                data_or_null(ws)));
+  return {dq, dk, dwq, dwk};
+}
+
+// dq2, dk2, dwq2, dwk2, dgq, dgk
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> rotary_bwdbwd_core(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& gq_,
+    const at::Tensor& gk_, const at::Tensor& uq_, const at::Tensor& uk_, const at::Tensor& zq_, const at::Tensor& zk_,
+    const RotaryWhere& where, const RotaryOptions& o) {
+  const RotaryCall c(q, k, wq, wk, where, o, true);
+  const at::Tensor gq = c.rows("query's cotangent", gq_, c.q), gk = c.rows("key's cotangent", gk_, c.k);
+  const at::Tensor uq = c.rows("cotangent of query's gradient", uq_, c.q), uk = c.rows("cotangent of key's gradient", uk_, c.k);
+  auto weight = [&](const at::Tensor& w, const at::Tensor& z) {
+    if (!w.defined()) return at::Tensor();
+    check_inputs({{"query", &c.q}, {"cotangent of a weight's gradient", &z}}, c10::nullopt);
+    expect("cotangent of a weight's gradient", z, w.sizes(), w.scalar_type());
+    return contig(z);
+  };
+  const at::Tensor zq = weight(c.wq, zq_), zk = weight(c.wk, zk_);
+  at::Tensor dq2 = c.like(c.q), dk2 = c.like(c.k), dgq = c.like(c.q), dgk = c.like(c.k);
+  at::Tensor dwq2 = c.like_weight(c.wq), dwk2 = c.like_weight(c.wk);
+  c10::DeviceGuard guard(c.q.device());
+  const at::Tensor ws = c.workspace();
+  check_status(api().rotary_bwdbwd(current_stream(c.q), &c.shape, c.q.data_ptr(), c.k.data_ptr(), data_or_null(c.wq),
+                                   data_or_null(c.wk), gq.data_ptr(), gk.data_ptr(), uq.data_ptr(), uk.data_ptr(),
+                                   data_or_null(zq), data_or_null(zk), dq2.data_ptr(), dk2.data_ptr(), data_or_null(dwq2),
+                                   data_or_null(dwk2), dgq.data_ptr(), dgk.data_ptr(), data_or_null(ws)));
+  return {dq2, dk2, dwq2, dwk2, dgq, dgk};
+}
+
 // ------------------------------------------------------------------ autograd
 
 using torch::autograd::AutogradContext;
@@ -578,6 +938,98 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
   }
 };
 
+// qk_norm_rotary's nodes, as flash_hog/torch/rotary.py has them. Absent tensors are undefined, among the nodes'
+// arguments (which take no undefined ones) empty; a result that an absent weight would have is a tensor of no
+// elements.
+at::Tensor given(const MaybeTensor& t) { return t ? *t : at::Tensor(); }
+MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+
+struct RotarySaved {
+  static void save(AutogradContext* ctx, const RotaryWhere& w, const RotaryOptions& o, variable_list more) {
+    variable_list all = {w.frequencies, w.positions, w.lengths, w.offsets};
+    all.insert(all.end(), more.begin(), more.end());
+    ctx->save_for_backward(std::move(all));
+    ctx->saved_data["interleaved"] = o.interleaved;
+    if (o.eps) ctx->saved_data["eps"] = *o.eps;
+  }
+  static RotaryOptions options(AutogradContext* ctx) {
+    const auto eps = ctx->saved_data.find("eps");
+    return {ctx->saved_data["interleaved"].toBool(),
+            eps == ctx->saved_data.end() ? c10::nullopt : c10::optional<double>(eps->second.toDouble())};
+  }
+  static RotaryWhere where(const variable_list& r) { return {r[0], r[1], r[2], r[3]}; }
+};
+
+// Refuses a third derivative (NoThirdOrder).
+struct NoThirdOrderRotary : public torch::autograd::Function<NoThirdOrderRotary> {
+  static variable_list forward(AutogradContext*, const at::Tensor& a, const at::Tensor& b, const at::Tensor& c,
+                               const at::Tensor& d, const at::Tensor& e, const at::Tensor& f) {
+    return {a.clone(), b.clone(), c.clone(), d.clone(), e.clone(), f.clone()};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    throw std::runtime_error("trying to differentiate twice a function that was marked with @once_differentiable");
+  }
+};
+
+struct RotaryBwdFn : public torch::autograd::Function<RotaryBwdFn> {
+  static variable_list forward(AutogradContext* ctx, const RotaryOptions& o, const at::Tensor& q, const at::Tensor& k,
+                               const MaybeTensor& wq_, const MaybeTensor& wk_, const at::Tensor& gq, const at::Tensor& gk,
+                               const MaybeTensor& frequencies, const MaybeTensor& positions, const MaybeTensor& lengths,
+                               const MaybeTensor& offsets) {
+    const at::Tensor wq = given(wq_), wk = given(wk_);
+    const RotaryWhere w{given(frequencies), given(positions), given(lengths), given(offsets)};
+    auto [dq, dk, dwq, dwk] = rotary_bwd_core(q, k, wq, wk, gq, gk, w, o);
+    RotarySaved::save(ctx, w, o, o.eps ? variable_list{q, k, wq, wk, gq, gk} : variable_list{});
+    if (!dwq.defined()) dwq = at::empty({0}, q.options());
+    if (!dwk.defined()) dwk = at::empty({0}, k.options());
+    return {dq, dk, dwq, dwk};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list r = ctx->get_saved_variables();
+    const RotaryOptions o = RotarySaved::options(ctx);
+    const RotaryWhere w = RotarySaved::where(r);
+    at::Tensor none, d[6];  // dq2, dk2, dwq2, dwk2, dgq, dgk
+    if (o.eps)
+      std::tie(d[0], d[1], d[2], d[3], d[4], d[5]) =
+          rotary_bwdbwd_core(r[4], r[5], r[6], r[7], r[8], r[9], grads[0], grads[1], grads[2], grads[3], w, o);
+    else
+      std::tie(d[4], d[5]) = rotary_fwd_core(grads[0], grads[1], none, none, w, o);
+    if (c10::GradMode::is_enabled() &&
+        std::any_of(grads.begin(), grads.end(), [](const at::Tensor& t) { return t.requires_grad(); })) {
+      auto mark = [&](const at::Tensor& t) {
+        return (t.defined() ? t.detach() : at::empty({0}, grads[0].options())).requires_grad_(true);
+      };
+      const variable_list marked = NoThirdOrderRotary::apply(mark(d[0]), mark(d[1]), mark(d[2]), mark(d[3]), mark(d[4]), mark(d[5]));
+      for (int i = 0; i < 6; ++i)
+        if (d[i].defined()) d[i] = marked[i];
+    }
+    return {none, d[0], d[1], d[2], d[3], d[4], d[5], none, none, none, none};
+  }
+};
+
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const RotaryOptions& o, const at::Tensor& q, const at::Tensor& k,
+                               const MaybeTensor& wq_, const MaybeTensor& wk_, const MaybeTensor& frequencies,
+                               const MaybeTensor& positions, const MaybeTensor& lengths, const MaybeTensor& offsets) {
+    const at::Tensor wq = given(wq_), wk = given(wk_);
+    const RotaryWhere w{given(frequencies), given(positions), given(lengths), given(offsets)};
+    auto [q_out, k_out] = rotary_fwd_core(q, k, wq, wk, w, o);
+    RotarySaved::save(ctx, w, o, o.eps ? variable_list{q, k, wq, wk} : variable_list{});
+    return {q_out, k_out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list r = ctx->get_saved_variables();
+    const RotaryOptions o = RotarySaved::options(ctx);
+    at::Tensor none;
+    // (without norms the cotangents stand in for the rows, of which only the shapes matter)
+    const at::Tensor q = o.eps ? r[4] : grads[0].detach(), k = o.eps ? r[5] : grads[1].detach();
+    const at::Tensor wq = o.eps ? r[6] : none, wk = o.eps ? r[7] : none;
+    const variable_list d = RotaryBwdFn::apply(o, q, k, maybe(wq), maybe(wk), grads[0], grads[1], maybe(r[0]), maybe(r[1]),
+                                              maybe(r[2]), maybe(r[3]));
+    return {none, d[0], d[1], wq.defined() ? d[2] : none, wk.defined() ? d[3] : none, none, none, none, none};
+  }
+};
+
 // ----------------------------------------------------------- Python-facing
 
 // Runs f without the GIL and raises its errors as Python exceptions.
@@ -649,6 +1101,65 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   return py_call([&] { return AttentionFn::apply(q, k, v, Mask{(int)causal, scale, {(int)window, (int)sinks}})[0]; });
 }
 
+at::Tensor paged_cache_extend(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table,
+                              const at::Tensor& lengths, const MaybeTensor& new_tokens, int new_each,
+                              const MaybeTensor& parents, const MaybeTensor& k_scale, const MaybeTensor& v_scale) {
+  require_bound((const void*)api().cache_extend);
+  return py_call([&] {
+    return cache_extend_core(k_cache, v_cache, table, lengths, new_tokens, new_each, parents, k_scale, v_scale);
+  });
+}
+
+std::tuple<at::Tensor, at::Tensor, MaybeTensor, MaybeTensor, MaybeTensor, at::Tensor> paged_cache_compact(
+    const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& lengths,
+    int64_t num_pages, const MaybeTensor& k_scale, const MaybeTensor& v_scale, const MaybeTensor& key_means) {
+  require_bound((const void*)api().cache_compact);
+  return py_call([&] { return cache_compact_core(k_cache, v_cache, table, lengths, num_pages, k_scale, v_scale, key_means); });
+}
+
+void paged_key_means(const at::Tensor& k_cache, const at::Tensor& means, const at::Tensor& table,
+                     const at::Tensor& lengths, const MaybeTensor& offsets, const MaybeTensor& k_scale) {
+  require_bound((const void*)api().key_means);
+  py_call([&] { key_means_core(k_cache, means, table, lengths, offsets, k_scale); });
+}
+
+at::Tensor paged_block_select(const at::Tensor& q, const at::Tensor& means, const at::Tensor& table,
+                              const at::Tensor& lengths, const MaybeTensor& offsets, int64_t page_size, int64_t blocks,
+                              int64_t first, int64_t last) {
+  require_bound((const void*)api().block_select);
+  return py_call([&] { return block_select_core(q, means, table, lengths, offsets, page_size, blocks, first, last); });
+}
+
+at::Tensor paged_block_attention(const at::Tensor& q, const at::Tensor& chosen, const at::Tensor& k_cache,
+                                 const at::Tensor& v_cache, const at::Tensor& table, const at::Tensor& lengths,
+                                 const MaybeTensor& offsets, const MaybeTensor& k_scale, const MaybeTensor& v_scale,
+                                 double scale, const MaybeTensor& out) {
+  require_bound((const void*)api().block_attention);
+  return py_call([&] {
+    return block_attention_core(q, chosen, k_cache, v_cache, table, lengths, offsets, k_scale, v_scale, scale, out);
+  });
+}
+
+// qk_norm_rotary(q, k, ...) with the autograd nodes above (when q, k or a weight requires grad and grad mode is on);
+// three axes: unbatched.
+std::tuple<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const MaybeTensor& wq,
+                                                  const MaybeTensor& wk, const MaybeTensor& frequencies,
+                                                  const MaybeTensor& positions, const MaybeTensor& lengths,
+                                                  const MaybeTensor& offsets, bool interleaved,
+                                                  c10::optional<double> eps) {
+  require_bound((const void*)api().rotary_bwdbwd);
+  return py_call([&]() -> std::tuple<at::Tensor, at::Tensor> {
+    const at::Tensor a = given(wq), b = given(wk);
+    const RotaryOptions o{interleaved, eps};
+    if (c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (a.defined() && a.requires_grad()) ||
+                                        (b.defined() && b.requires_grad()))) {
+      const variable_list out = RotaryFn::apply(o, q, k, wq, wk, frequencies, positions, lengths, offsets);
+      return {out[0], out[1]};
+    }
+    return rotary_fwd_core(q, k, a, b, {given(frequencies), given(positions), given(lengths), given(offsets)}, o);
+  });
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -656,6 +1167,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind, "bind(fwd, bwd, bwdbwd, last_error, status_string, error_cls): entry-point addresses");
   m.def("bind_window", &bind_window, "bind_window(workspace_bytes, fwd, bwd, bwdbwd): their addresses");
   m.def("bind_paged", &bind_paged, "bind_paged(workspace_bytes, attention, write, read): their addresses");
+  m.def("bind_pages", &bind_pages, "bind_pages(workspace_bytes, extend, compact): their addresses");
+  m.def("bind_blocks", &bind_blocks,
+        "bind_blocks(key_means, select_workspace_bytes, select, workspace_bytes, attention): their addresses");
+  m.def("bind_rotary", &bind_rotary, "bind_rotary(workspace_bytes, fwd, bwd, bwdbwd): their addresses");
+  m.def("paged_cache_extend", &paged_cache_extend);
+  m.def("paged_cache_compact", &paged_cache_compact);
+  m.def("paged_key_means", &paged_key_means);
+  m.def("paged_block_select", &paged_block_select);
+  m.def("paged_block_attention", &paged_block_attention);
+  m.def("qk_norm_rotary", &qk_norm_rotary);
   m.def("paged_attention", &paged_attention);
   m.def("paged_cache_write", &paged_cache_write);
   m.def("paged_cache_read", &paged_cache_read);

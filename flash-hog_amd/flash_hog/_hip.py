@@ -141,6 +141,13 @@ def torch_ext():
                         addr(L.fhog_window_attention_bwd), addr(L.fhog_window_attention_bwdbwd))
         mod.bind_paged(addr(L.fhog_paged_workspace_bytes), addr(L.fhog_paged_attention),
                        addr(L.fhog_paged_cache_write), addr(L.fhog_paged_cache_read))
+        mod.bind_pages(addr(L.fhog_paged_pages_workspace_bytes), addr(L.fhog_paged_cache_extend),
+                       addr(L.fhog_paged_cache_compact))
+        mod.bind_blocks(addr(L.fhog_paged_key_means), addr(L.fhog_paged_block_select_workspace_bytes),
+                        addr(L.fhog_paged_block_select), addr(L.fhog_paged_block_workspace_bytes),
+                        addr(L.fhog_paged_block_attention))
+        mod.bind_rotary(addr(L.fhog_qk_norm_rotary_workspace_bytes), addr(L.fhog_qk_norm_rotary_fwd),
+                        addr(L.fhog_qk_norm_rotary_bwd), addr(L.fhog_qk_norm_rotary_bwdbwd))
     except (ImportError, OSError, AttributeError) as exc:
         warnings.warn(f"Flash-HOG torch extension {TORCH_EXT_PATH} not loaded ({exc}); "
                       "using the Python wrappers", RuntimeWarning, stacklevel=2)
@@ -543,6 +550,10 @@ def _overlap(a, b) -> bool:
 def paged_cache_extend(k_cache, v_cache, page_table, lengths, new_tokens, new_each: int, parents, k_scale, v_scale):
     """Rows of page_table and lengths go on from their parents and grow by new_tokens (None: new_each) tokens,
     in place (fhog_paged_cache_extend); returns the free pages left, an int32 tensor of no axes."""
+    ext = torch_ext()
+    if ext is not None:
+        return ext.paged_cache_extend(k_cache, v_cache, page_table, lengths, new_tokens, new_each, parents, k_scale,
+                                      v_scale)
     (pages, Nk, page, Hd, B, width), _, _, _ = _check_cache(
         ("key_cache", k_cache), k_cache, v_cache, page_table, lengths, None, k_scale, v_scale, k_cache.dtype)
     if k_cache.dtype not in CACHE_DTYPE_CODES:
@@ -575,6 +586,9 @@ def paged_cache_extend(k_cache, v_cache, page_table, lengths, new_tokens, new_ea
 def paged_cache_compact(k_cache, v_cache, page_table, lengths, num_pages: int, k_scale, v_scale, key_means):
     """(k_cache, v_cache, k_scale, v_scale, key_means, page_table): the used pages as the first of new caches
     of num_pages pages (fhog_paged_cache_compact); None for what is not given."""
+    ext = torch_ext()
+    if ext is not None:
+        return ext.paged_cache_compact(k_cache, v_cache, page_table, lengths, num_pages, k_scale, v_scale, key_means)
     (pages, Nk, page, Hd, B, width), page_table, lengths, _ = _check_cache(
         ("key_cache", k_cache), k_cache, v_cache, page_table, lengths, None, k_scale, v_scale, k_cache.dtype)
     if k_cache.dtype not in CACHE_DTYPE_CODES:
@@ -622,6 +636,10 @@ def _check_index(first, page_table, lengths, query_offsets):
 
 def paged_key_means(k_cache, key_means, page_table, lengths, query_offsets, k_scale) -> None:
     """The means of the pages that the new tokens fill, into key_means (fhog_paged_key_means)."""
+    ext = torch_ext()
+    if ext is not None:
+        ext.paged_key_means(k_cache, key_means, page_table, lengths, query_offsets, k_scale)
+        return
     (pages, Nk, page, Hd, B, width), page_table, lengths, query_offsets = _check_cache(
         ("key_cache", k_cache), k_cache, k_cache, page_table, lengths, query_offsets, k_scale, k_scale, k_cache.dtype)
     if k_cache.dtype not in CACHE_DTYPE_CODES:
@@ -639,6 +657,9 @@ def paged_key_means(k_cache, key_means, page_table, lengths, query_offsets, k_sc
 def paged_block_select(q, key_means, page_table, lengths, query_offsets, page_size: int, blocks: int, first: int,
                        last: int):
     """(T, N_kv, blocks) int32, the columns that each new token attends to (fhog_paged_block_select)."""
+    ext = torch_ext()
+    if ext is not None:
+        return ext.paged_block_select(q, key_means, page_table, lengths, query_offsets, page_size, blocks, first, last)
     if q.ndim != 3:
         raise ValueError(f"expected a (T, N, H) query, got {tuple(q.shape)}")
     if key_means.ndim != 3 or key_means.shape[2] != q.shape[2]:
@@ -669,6 +690,10 @@ def paged_block_attention(q, chosen, k_cache, v_cache, page_table, lengths, quer
                           out=None):
     """out (T, N, H) of the packed new tokens q over the chosen (T, N_kv, blocks) columns of a paged cache
     (fhog_paged_block_attention)."""
+    ext = torch_ext()
+    if ext is not None:
+        return ext.paged_block_attention(q, chosen, k_cache, v_cache, page_table, lengths, query_offsets, k_scale, v_scale,
+                                         float(scale), out)
     if q.ndim != 3:
         raise ValueError(f"expected a (T, N, H) query, got {tuple(q.shape)}")
     (pages, Nk, page, Hd, B, width), page_table, lengths, query_offsets = _check_cache(

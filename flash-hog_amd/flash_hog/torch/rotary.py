@@ -103,7 +103,8 @@ def _fwd(q, k, wq, wk, where, interleaved, eps):
 
 
 # As in flash_hog.torch.attention: Functions in the setup_context form, which torch.func transforms
-# compose with, and in the ctx-first form for eager calls. `where`: frequencies, positions, lengths,
+# compose with, and in the ctx-first form for eager calls without the torch extension, which has the same
+# two in C++ (csrc/fhog_torch.cpp, RotaryFn and RotaryBwdFn). `where`: frequencies, positions, lengths,
 # query_offsets.
 
 class _QKNormRotary(torch.autograd.Function):
@@ -221,6 +222,11 @@ def qk_norm_rotary(query, key, positions=None, *, frequencies=None, query_weight
         raise ValueError(f"lengths go with packed tokens (T, N, H), got {tuple(query.shape)}")
     if eps is not None:
         eps = float(eps)
+    tensors = (query, key, query_weight, key_weight, frequencies, positions, lengths, query_offsets)
+    if _plain(*tensors) and forward_ad._current_level < 0:
+        ext = _hip.torch_ext()
+        if ext is not None:  # the Functions above in C++
+            return ext.qk_norm_rotary(*tensors, bool(interleaved), eps)
     unbatched = query.ndim == 3
     if unbatched:
         query, key = query.unsqueeze(0), key.unsqueeze(0)

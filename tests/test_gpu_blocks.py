@@ -439,9 +439,13 @@ def test_slabs(cuda_device):
     assert got[299, 0].tolist() == sorted(scores.topk(12).indices.tolist())
 
 
-def test_refusals(cuda_device):
+@pytest.mark.parametrize("extension", [True, False])
+def test_refusals(extension, cuda_device, monkeypatch):
     import flash_hog
+    from flash_hog import _hip
 
+    if not extension:
+        monkeypatch.setattr(_hip, "torch_ext", lambda: None)
     case = CASES[1]
     cache, counts, q, moved, where = make(case, cuda_device)
     q = q.to(cuda_device)
@@ -480,9 +484,10 @@ def test_refusals(cuda_device):
             bad()
 
 
-def test_repeats(cuda_device):
-    """The same bits at every call, with and without a table wider than needed."""
+def test_repeats(cuda_device, monkeypatch):
+    """The same bits at every call, with and without a table wider than needed, through the extension and without."""
     import flash_hog
+    from flash_hog import _hip
 
     case = (8, 2, 128, BF16, True, 64, [6000, 2000], [40, 9], 12, 1, 2)
     for width in (None, 3000):
@@ -496,4 +501,5 @@ def test_repeats(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(*runs))
         if width is None:
             narrow = runs[0]
+            monkeypatch.setattr(_hip, "torch_ext", lambda: None)
     assert all(torch.equal(a, b) for a, b in zip(narrow, runs[0]))

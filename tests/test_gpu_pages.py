@@ -197,9 +197,14 @@ def test_graph_and_streams(cuda_device):
         assert moved[5].tolist() == want and torch.equal(raw(moved[0])[:len(used)], raw(x["key_cache"])[used])
 
 
-def test_versions_and_refusals(cuda_device):
+@pytest.mark.parametrize("extension", [True, False])
+def test_versions_and_refusals(extension, cuda_device, monkeypatch):
     """Written tensors get a new autograd version; wrong arguments raise before anything is written."""
     import flash_hog
+    from flash_hog import _hip
+
+    if not extension:
+        monkeypatch.setattr(_hip, "torch_ext", lambda: None)
 
     x = cache(4, 2, 16, 64, BF16, cuda_device)
     t, n = i32([[0, -1]], cuda_device), i32([3], cuda_device)

@@ -387,8 +387,13 @@ def test_compile(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-def test_third_derivative_raises(cuda_device):
+@pytest.mark.parametrize("extension", [True, False])
+def test_third_derivative_raises(extension, cuda_device, monkeypatch):
     import flash_hog
+    from flash_hog import _hip
+
+    if not extension:
+        monkeypatch.setattr(_hip, "torch_ext", lambda: None)
 
     q, k = (torch.randn((1, 5, n, 64), device=cuda_device, requires_grad=True) for n in (2, 1))
     out = flash_hog.qk_norm_rotary(q, k)
@@ -414,6 +419,57 @@ def test_python_wrappers_agree(cuda_device, monkeypatch):
         grads = torch.autograd.grad(out, leaves, [torch.ones_like(o) for o in out], create_graph=True)
         return [*out, *grads, *torch.autograd.grad(grads, leaves, [torch.ones_like(g) for g in grads])]
 
+    assert _hip.torch_ext() is not None
     a = run()
     monkeypatch.setattr(_hip, "torch_ext", lambda: None)
     assert all(torch.equal(x, y) for x, y in zip(a, run()))
+
+
+@pytest.mark.parametrize("extension", [True, False])
+def test_refusals(extension, cuda_device, monkeypatch):
+    """Both front doors say the same."""
+    import flash_hog
+    from flash_hog import _hip
+
+    if not extension:
+        monkeypatch.setattr(_hip, "torch_ext", lambda: None)
+    q, k = (torch.zeros((2, 5, n, 64), dtype=BF16, device=cuda_device) for n in (4, 2))
+    w, freq = torch.ones(64, dtype=BF16, device=cuda_device), frequencies(64, cuda_device)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=cuda_device)
+    call = flash_hog.qk_norm_rotary
+    for bad, match in ((lambda: call(q, k[:1]), "of the same tokens and head_dim"), (lambda: call(q, k[..., :32]), "of the same tokens"),
+                       (lambda: call(q, k.float()), "key has dtype"), (lambda: call(q, k.cpu()), "must be on a GPU device"),
+                       (lambda: call(q.double(), k.double()), "unsupported dtype"),
+                       (lambda: call(q, k, query_weight=w[:32]), "query_weight has shape"),
+                       (lambda: call(q, k, query_weight=w, key_weight=w.float()), "key_weight has dtype"),
+                       (lambda: call(q, k, query_weight=w.half()), "weights must be of"),
+                       (lambda: call(q, k, query_weight=w, eps=None), "weights need norms"),
+                       (lambda: call(q, k, frequencies=freq.double()), "frequencies must be"),
+                       (lambda: call(q, k, frequencies=torch.cat([freq, freq])), "frequencies must be"),
+                       (lambda: call(q, k, i32(5).float()), "positions has dtype"), (lambda: call(q, k, i32(2, 4)), "positions has shape"),
+                       (lambda: call(q, k, i32(1, 5)), "positions has shape"), (lambda: call(q[0], k[0], i32(5), lengths=i32(5)), "exclude each other"),
+                       (lambda: call(q[0], k[0], lengths=i32(4)), "lengths has shape"),
+                       (lambda: call(q[0], k[0], lengths=i32(4), query_offsets=i32(4)), "query_offsets has shape"),
+                       (lambda: call(q[0], k[0], query_offsets=i32(4)), "query_offsets needs lengths"),
+                       (lambda: call(q[0], k[0], lengths=i32(5).long()), "lengths has dtype"),
+                       (lambda: call(q, k, lengths=i32(10)), "packed tokens")):
+        with pytest.raises(ValueError, match=match):
+            bad()
+    for bad, match in ((lambda: call(q, k, eps=-1.0), "eps must be finite"),
+                       (lambda: call(torch.zeros((1, 1, 1, 300), device=cuda_device), torch.zeros((1, 1, 1, 300), device=cuda_device)),
+                        "head_dim must be 1 to 256")):
+        with pytest.raises(_hip.FlashHogError, match=match):
+            bad()
+
+
+def test_in_place_changes_are_noticed(cuda_device):
+    """A row or a position that changed after the forward makes its backward raise."""
+    import flash_hog
+
+    for which in range(3):
+        q, k = (torch.randn((1, 5, n, 64), device=cuda_device) for n in (2, 1))
+        w, positions = torch.ones(64, device=cuda_device, requires_grad=True), torch.arange(5, device=cuda_device)
+        out = flash_hog.qk_norm_rotary(q, k, positions, frequencies=frequencies(64, cuda_device), query_weight=w)
+        (q, k, positions)[which].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out[0].sum().backward()
