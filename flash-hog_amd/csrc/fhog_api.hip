@@ -648,15 +648,16 @@ void rotary_strides(const fhog_rotary& s, fhog::RowStrides out[2]) {
   out[0] = {(long)s.q_stride[0], (long)s.q_stride[1], (long)s.q_stride[2]};
   out[1] = {(long)s.k_stride[0], (long)s.k_stride[1], (long)s.k_stride[2]};
 }
-// Whether rows can be read in 16-byte pieces of which each holds whole pairs: `rows` are the tensors, of which
-// the first `strided` have q's and k's strides.
+// Whether rows can be read in pieces of kRotaryPairs elements, a lane's two pieces whole pairs: `rows` are the tensors;
+// strided: q and k, with their strides, are among them.
 bool rotary_wide(const fhog_rotary& s, bool strided, std::initializer_list<const void*> rows) {
-  const long long each = s.dtype == FHOG_DTYPE_F32 ? 4 : 8;
-  if (s.head_dim % 16 != 0 || s.rotated % 16 != 0) return false;
+  constexpr int pairs = fhog::kRotaryPairs;
+  const int item = s.dtype == FHOG_DTYPE_F32 ? 4 : 2, bytes = pairs * item;
+  if (s.head_dim % (2 * pairs) != 0 || s.rotated % (2 * pairs) != 0) return false;
   for (const void* p : rows)
-    if (p != nullptr && !aligned(p, 16)) return false;
+    if (p != nullptr && !aligned(p, bytes)) return false;
   for (int i = 0; strided && i < 3; ++i)
-    if (s.q_stride[i] % each != 0 || s.k_stride[i] % each != 0) return false;
+    if (s.q_stride[i] * item % bytes != 0 || s.k_stride[i] * item % bytes != 0) return false;
   return true;
 }
 template <typename F> hipError_t dispatch_rows(int dtype, F&& f) {
@@ -702,7 +703,7 @@ extern "C" {
 size_t fhog_qk_norm_rotary_workspace_bytes(const fhog_rotary* shape) {
   if (check_rotary("fhog_qk_norm_rotary_workspace_bytes", shape) || !shape->norm) return 0;
   const long tokens = (long)shape->batch * shape->tokens;
-  return (size_t)2 * fhog::rotary_grid(tokens, compute_units()).groups * shape->head_dim * sizeof(float);
+  return (size_t)2 * fhog::rotary_grid(tokens, shape->heads, shape->head_dim, compute_units()).groups * shape->head_dim * sizeof(float);
 }
 
 int fhog_qk_norm_rotary_fwd(fhog_stream_t stream, const fhog_rotary* shape, const void* q, const void* k,
@@ -717,7 +718,7 @@ int fhog_qk_norm_rotary_fwd(fhog_stream_t stream, const fhog_rotary* shape, cons
   auto run = [&]<typename T>() {
     fhog::RotaryFwdParams<T> p{{(const T*)q, (const T*)k}, {q_weight, k_weight}, {(T*)q_out, (T*)k_out}, {}, rotary_shape(s)};
     rotary_strides(s, p.stride);
-    return fhog::launch_rotary_fwd<T>(p, fhog::rotary_grid(tokens, compute_units()),
+    return fhog::launch_rotary_fwd<T>(p, fhog::rotary_grid(tokens, s.heads, s.head_dim, compute_units()),
                                       rotary_wide(s, true, {q, k, q_out, k_out}), (hipStream_t)stream);
   };
   return launch_status(dispatch_rows(s.dtype, run), who);
@@ -745,7 +746,7 @@ int fhog_qk_norm_rotary_bwd(fhog_stream_t stream, const fhog_rotary* shape, cons
                                rotary_shape(s)};
     rotary_strides(s, p.stride);
     const bool wide = rotary_wide(s, s.norm, {s.norm ? q : nullptr, s.norm ? k : nullptr, dq_out, dk_out, dq, dk});
-    return fhog::launch_rotary_bwd<T>(p, fhog::rotary_grid(tokens, compute_units()), wide, (hipStream_t)stream);
+    return fhog::launch_rotary_bwd<T>(p, fhog::rotary_grid(tokens, s.heads, s.head_dim, compute_units()), wide, (hipStream_t)stream);
   };
   return launch_status(dispatch_rows(s.dtype, run), who);
 }
@@ -776,7 +777,7 @@ int fhog_qk_norm_rotary_bwdbwd(fhog_stream_t stream, const fhog_rotary* shape, c
                                   parts ? (float*)workspace : nullptr, {dq_weight2, dk_weight2}, {}, rotary_shape(s)};
     rotary_strides(s, p.stride);
     const bool wide = rotary_wide(s, true, {q, k, dq_out, dk_out, ddq, ddk, dq2, dk2, ddq_out, ddk_out});
-    return fhog::launch_rotary_bwdbwd<T>(p, fhog::rotary_grid(tokens, compute_units()), wide, (hipStream_t)stream);
+    return fhog::launch_rotary_bwdbwd<T>(p, fhog::rotary_grid(tokens, s.heads, s.head_dim, compute_units()), wide, (hipStream_t)stream);
   };
   return launch_status(dispatch_rows(s.dtype, run), who);
 }

@@ -15,8 +15,8 @@
 // would leave 4 10^-3 of an angle. They belong to a token, not to a head: a workgroup forms those of
 // its tokens once, in LDS.
 //
-// L neighbouring lanes hold a row, eight pairs a lane: both partners of a rotation are in one lane, in
-// two 16-byte loads (of 2-byte types) where the row allows them. Every row is read once and written
+// L neighbouring lanes hold a row, N pairs a lane: both partners of a rotation are in one lane, in
+// two loads of N elements where the row allows them. Every row is read once and written
 // once. The weights' gradients are summed in registers over a workgroup's rows, then over its threads,
 // then by a small kernel over the workgroups, always in the same order.
 #include "fhog_paged.h"
@@ -27,50 +27,61 @@ namespace fhog {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int N = kRotaryPairs;
 constexpr int kMostTile = 16;
 
-// Eight pairs of a row.
+// N pairs of a row, a lane's.
 struct Pairs {
-  float a[8], b[8];
+  float a[N], b[N];
 };
 
-// Where lane c of a row finds its pairs 8 c .. 8 c + 7. Columns behind the rotated ones are paired with
+// Where lane c of a row finds its pairs N c .. N c + N - 1. Columns behind the rotated ones are paired with
 // their neighbours and turned by nothing.
+// WIDE: head_dim and rotated are multiples of 2 N, and N elements of a row are aligned to their size.
 template <bool WIDE> struct Columns {
   int head_dim, half, pair0;
   bool apart;  // partners are half the rotated columns apart
   __device__ __forceinline__ Columns(const RotaryShape& s, int c)
-      : head_dim(s.head_dim), half(s.rotated / 2), pair0(8 * c), apart(!s.interleaved && 8 * c < s.rotated / 2) {}
-  // WIDE: head_dim and rotated are multiples of 16, rows of 16 bytes.
+      : head_dim(s.head_dim), half(s.rotated / 2), pair0(N * c), apart(!s.interleaved && N * c < s.rotated / 2) {}
   __device__ __forceinline__ bool any() const { return 2 * pair0 < head_dim; }
   __device__ __forceinline__ int column(int i, int side, bool interleaved) const {
     const int p = pair0 + i;
     return p < half && !interleaved ? p + side * half : 2 * p + side;
   }
-  template <typename T> __device__ __forceinline__ Pairs load(const T* row, bool interleaved) const {
-    Pairs x;
+  // A lane's part of a row as it lies in memory, and as pairs.
+  template <typename T> struct Raw {
+    typedef T VN __attribute__((ext_vector_type(N)));
+    VN lo, hi;
+  };
+  template <typename T> __device__ __forceinline__ Raw<T> fetch(const T* row, bool interleaved) const {
+    Raw<T> x;
     if constexpr (WIDE) {
-      V8<T> lo = zero8<T>(), hi = zero8<T>();
+#pragma unroll
+      for (int i = 0; i < N; ++i) x.lo[i] = x.hi[i] = (T)0.f;
       if (any()) {
-        lo = *reinterpret_cast<const V8<T>*>(row + (apart ? pair0 : 2 * pair0));
-        hi = *reinterpret_cast<const V8<T>*>(row + (apart ? pair0 + half : 2 * pair0 + 8));
-      }
-      if (apart) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x.a[i] = (float)lo[i], x.b[i] = (float)hi[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x.a[i] = (float)lo[2 * i], x.b[i] = (float)lo[2 * i + 1];
-          x.a[4 + i] = (float)hi[2 * i], x.b[4 + i] = (float)hi[2 * i + 1];
-        }
+        x.lo = *reinterpret_cast<const typename Raw<T>::VN*>(row + (apart ? pair0 : 2 * pair0));
+        x.hi = *reinterpret_cast<const typename Raw<T>::VN*>(row + (apart ? pair0 + half : 2 * pair0 + N));
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         const int ca = column(i, 0, interleaved), cb = column(i, 1, interleaved);
-        x.a[i] = ca < head_dim ? (float)row[ca] : 0.f;
-        x.b[i] = cb < head_dim ? (float)row[cb] : 0.f;
+        x.lo[i] = ca < head_dim ? row[ca] : (T)0.f;
+        x.hi[i] = cb < head_dim ? row[cb] : (T)0.f;
+      }
+    }
+    return x;
+  }
+  template <typename T> __device__ __forceinline__ Pairs take(const Raw<T>& r) const {
+    Pairs x;
+    if (apart || !WIDE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x.a[i] = (float)r.lo[i], x.b[i] = (float)r.hi[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        x.a[i] = (float)r.lo[2 * i], x.b[i] = (float)r.lo[2 * i + 1];
+        x.a[N / 2 + i] = (float)r.hi[2 * i], x.b[N / 2 + i] = (float)r.hi[2 * i + 1];
       }
     }
     return x;
@@ -78,22 +89,24 @@ template <bool WIDE> struct Columns {
   template <typename T> __device__ __forceinline__ void store(T* row, const Pairs& x, bool interleaved) const {
     if constexpr (WIDE) {
       if (!any()) return;
-      f32x8 lo, hi;
+      typedef T VN __attribute__((ext_vector_type(N)));
+      typedef float FN __attribute__((ext_vector_type(N)));
+      FN lo, hi;
       if (apart) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) lo[i] = x.a[i], hi[i] = x.b[i];
+        for (int i = 0; i < N; ++i) lo[i] = x.a[i], hi[i] = x.b[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < N / 2; ++i) {
           lo[2 * i] = x.a[i], lo[2 * i + 1] = x.b[i];
-          hi[2 * i] = x.a[4 + i], hi[2 * i + 1] = x.b[4 + i];
+          hi[2 * i] = x.a[N / 2 + i], hi[2 * i + 1] = x.b[N / 2 + i];
         }
       }
-      *reinterpret_cast<V8<T>*>(row + (apart ? pair0 : 2 * pair0)) = cvt8<T>(lo);
-      *reinterpret_cast<V8<T>*>(row + (apart ? pair0 + half : 2 * pair0 + 8)) = cvt8<T>(hi);
+      *reinterpret_cast<VN*>(row + (apart ? pair0 : 2 * pair0)) = __builtin_convertvector(lo, VN);
+      *reinterpret_cast<VN*>(row + (apart ? pair0 + half : 2 * pair0 + N)) = __builtin_convertvector(hi, VN);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         const int ca = column(i, 0, interleaved), cb = column(i, 1, interleaved);
         if (ca < head_dim) row[ca] = (T)x.a[i];
         if (cb < head_dim) row[cb] = (T)x.b[i];
@@ -108,11 +121,11 @@ __device__ __forceinline__ Pairs load_weight(const Columns<WIDE>& at, const void
   Pairs x;
   if (w == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x.a[i] = x.b[i] = none;
+    for (int i = 0; i < N; ++i) x.a[i] = x.b[i] = none;
     return x;
   }
-  const Columns<false> one(s, at.pair0 / 8);  // (its own alignment is not known)
-  return s.wide_weights ? one.load((const float*)w, s.interleaved) : one.load((const T*)w, s.interleaved);
+  const Columns<false> one(s, at.pair0 / N);  // (its own alignment is not known)
+  return s.wide_weights ? one.take(one.fetch((const float*)w, s.interleaved)) : one.take(one.fetch((const T*)w, s.interleaved));
 }
 
 // Sum over the L lanes of a row, in all of them.
@@ -125,18 +138,18 @@ template <int L> __device__ __forceinline__ float row_sum(float x) {
 __device__ __forceinline__ float dot(const Pairs& x, const Pairs& y) {
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum = fmaf(x.a[i], y.a[i], fmaf(x.b[i], y.b[i], sum));
+  for (int i = 0; i < N; ++i) sum = fmaf(x.a[i], y.a[i], fmaf(x.b[i], y.b[i], sum));
   return sum;
 }
 
-// cos and sin of a token's angles for eight pairs of a row, and the rotations.
+// cos and sin of a token's angles for a lane's pairs, and the rotations.
 struct Turn {
-  alignas(16) float c[8];
-  alignas(16) float s[8];
+  alignas(16) float c[N];
+  alignas(16) float s[N];
   __device__ __forceinline__ Pairs there(const Pairs& x) const {
     Pairs y;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       y.a[i] = x.a[i] * c[i] - x.b[i] * s[i];
       y.b[i] = x.b[i] * c[i] + x.a[i] * s[i];
     }
@@ -145,7 +158,7 @@ struct Turn {
   __device__ __forceinline__ Pairs back(const Pairs& y) const {
     Pairs x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       x.a[i] = y.a[i] * c[i] + y.b[i] * s[i];
       x.b[i] = y.b[i] * c[i] - y.a[i] * s[i];
     }
@@ -167,12 +180,17 @@ __device__ __forceinline__ double position(const RotaryShape& s, long token) {
   return t < begin || t >= end ? 0.0 : (double)s.lengths[b] - (double)(end - t);
 }
 
-// The workgroup's angles: those of tokens [first, first + count), kPairs a token.
-template <int L> struct Angles {
-  static constexpr int kPairs = 8 * L;
+// The workgroup's tokens [first, first + count): their angles, kPairs a token, and where their rows begin.
+template <int L> struct Tokens {
+  static constexpr int kPairs = N * L;
   alignas(16) float c[kMostTile][kPairs];
   alignas(16) float s[kMostTile][kPairs];
-  __device__ __forceinline__ void form(const RotaryShape& shape, long first, int count) {
+  long from[kMostTile];
+  __device__ __forceinline__ void form(const RotaryShape& shape, const RowStrides& stride, long first, int count) {
+    if ((int)threadIdx.x < count) {
+      const long token = first + threadIdx.x, b = shape.batch == 1 ? 0 : token / shape.tokens;
+      from[threadIdx.x] = b * stride.batch + (token - b * shape.tokens) * stride.token;
+    }
     for (int i = threadIdx.x; i < count * kPairs; i += kThreads) {
       const int token = i / kPairs, pair = i % kPairs;
       float cos = 1.f, sin = 0.f;
@@ -184,36 +202,44 @@ template <int L> struct Angles {
       s[token][pair] = sin;
     }
   }
-  __device__ __forceinline__ Turn of(int token, int lane) const {
+  __device__ __forceinline__ Turn turn(int token, int lane) const {
     Turn t;
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      *reinterpret_cast<f32x4*>(t.c + i) = *reinterpret_cast<const f32x4*>(&c[token][8 * lane + i]);
-      *reinterpret_cast<f32x4*>(t.s + i) = *reinterpret_cast<const f32x4*>(&s[token][8 * lane + i]);
+    for (int i = 0; i < N; i += 4) {
+      *reinterpret_cast<f32x4*>(t.c + i) = *reinterpret_cast<const f32x4*>(&c[token][N * lane + i]);
+      *reinterpret_cast<f32x4*>(t.s + i) = *reinterpret_cast<const f32x4*>(&s[token][N * lane + i]);
     }
     return t;
   }
 };
 
-// Calls f(token of the tile, offset of the row in x, offset in contiguous tensors, Turn) for every row
-// that this thread's lane group has, of the workgroup's tiles.
-template <int L, typename F>
+// For every row that this thread's lane group has, of the workgroup's tiles: fetch(offset of the row in x, offset in
+// contiguous tensors), a row ahead, and work(what it gave, offset in contiguous tensors, Turn).
+template <int L, typename Fetch, typename Work>
 __device__ __forceinline__ void for_rows(const RotaryShape& s, const RowStrides& stride, int which, int tile,
-                                         Angles<L>& angles, F&& f) {
+                                         Tokens<L>& held, Fetch&& fetch, Work&& work) {
   constexpr int kRows = kThreads / L;
   const int heads = s.heads[which], lane = threadIdx.x % L, group = threadIdx.x / L;
+  const int step_t = kRows / heads, step_h = kRows - step_t * heads, t_first = group / heads, h_first = group - t_first * heads;
   const long tokens = (long)s.batch * s.tokens;
   for (long t0 = (long)blockIdx.x * tile; t0 < tokens; t0 += (long)gridDim.x * tile) {
     const int count = (int)(tokens - t0 < tile ? tokens - t0 : tile);
     __syncthreads();  // (the tile before is read)
-    angles.form(s, t0, count);
+    held.form(s, stride, t0, count);
     __syncthreads();
+    int t = t_first, h = h_first;
+    if (t >= count) continue;
+    auto place = [&] { return ((t0 + t) * heads + h) * (long)s.head_dim; };
+    auto ahead = fetch(held.from[t] + h * stride.head, place());
     // (every lane of a group takes the same way, so the sums' shuffles find each other)
-    for (int r = group; r < count * heads; r += kRows) {
-      const int t = r / heads, h = r % heads;
-      const long token = t0 + t, b = token / s.tokens;
-      f(b * stride.batch + (token - b * s.tokens) * stride.token + h * stride.head,
-        (token * heads + h) * (long)s.head_dim, angles.of(t, lane));
+    while (t < count) {
+      const auto now = ahead;
+      const int at = t;
+      const long to = place();
+      t += step_t, h += step_h;
+      if (h >= heads) h -= heads, ++t;
+      if (t < count) ahead = fetch(held.from[t] + h * stride.head, place());
+      work(now, to, held.turn(at, lane));
     }
   }
 }
@@ -225,7 +251,7 @@ __device__ __forceinline__ void leave_parts(const Columns<WIDE>& at, const Rotar
   // Lanes with the same columns within a wave, then the waves, through LDS.
   Pairs x = sum;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < N; ++i)
     for (int d = L; d < 64; d <<= 1) {
       x.a[i] += __shfl_xor(x.a[i], d, 64);
       x.b[i] += __shfl_xor(x.b[i], d, 64);
@@ -234,36 +260,37 @@ __device__ __forceinline__ void leave_parts(const Columns<WIDE>& at, const Rotar
   __syncthreads();
   if (lane < L)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      box[(wave * L + lane) * 16 + i] = x.a[i];
-      box[(wave * L + lane) * 16 + 8 + i] = x.b[i];
+    for (int i = 0; i < N; ++i) {
+      box[(wave * L + lane) * 2 * N + i] = x.a[i];
+      box[(wave * L + lane) * 2 * N + N + i] = x.b[i];
     }
   __syncthreads();
   if (threadIdx.x < L)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 2 * N; ++i) {
       float y = 0.f;
-      for (int w = 0; w < kThreads / 64; ++w) y += box[(w * L + threadIdx.x) * 16 + i];
-      const int col = at.column(i & 7, i >> 3, s.interleaved);
+      for (int w = 0; w < kThreads / 64; ++w) y += box[(w * L + threadIdx.x) * 2 * N + i];
+      const int col = at.column(i % N, i / N, s.interleaved);
       if (col < s.head_dim) part[col] = y;
     }
 }
 
 template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(RotaryFwdParams<T> p, int tile) {
-  __shared__ Angles<L> angles;
+  __shared__ Tokens<L> held;
   const int which = blockIdx.y;
   const Columns<WIDE> at(p.s, threadIdx.x % L);
   const Pairs w = load_weight<T>(at, p.weight[which], p.s, 1.f);
   const float inv = 1.f / (float)p.s.head_dim;
   const T* const rows = p.x[which];
   T* const out = p.y[which];
-  for_rows<L>(p.s, p.stride[which], which, tile, angles, [&](long from, long to, const Turn& turn) {
-    Pairs x = at.load(rows + from, p.s.interleaved);
+  auto fetch = [&](long from, long) { return at.fetch(rows + from, p.s.interleaved); };
+  for_rows<L>(p.s, p.stride[which], which, tile, held, fetch, [&](const auto& raw, long to, const Turn& turn) {
+    Pairs x = at.take(raw);
     if (p.s.norm) {
       const float r = rsqrtf(row_sum<L>(dot(x, x)) * inv + p.s.eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         x.a[i] *= r * w.a[i];
         x.b[i] *= r * w.b[i];
       }
@@ -274,8 +301,8 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(RotaryFwdParams<T>
 
 template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(RotaryBwdParams<T> p, int tile) {
-  __shared__ Angles<L> angles;
-  __shared__ float box[kThreads / 64 * L * 16];
+  __shared__ Tokens<L> held;
+  __shared__ float box[kThreads / 64 * L * 2 * N];
   const int which = blockIdx.y;
   const Columns<WIDE> at(p.s, threadIdx.x % L);
   const Pairs w = load_weight<T>(at, p.weight[which], p.s, 1.f);
@@ -284,13 +311,21 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(RotaryBwdParams<T>
   const T* const dy = p.dy[which];
   T* const dx = p.dx[which];
   Pairs sum{};
-  for_rows<L>(p.s, p.stride[which], which, tile, angles, [&](long from, long to, const Turn& turn) {
-    Pairs g = turn.back(at.load(dy + to, p.s.interleaved));
+  struct Rows {
+    typename Columns<WIDE>::template Raw<T> dy, x;
+  };
+  auto fetch = [&](long from, long to) {
+    Rows r{at.fetch(dy + to, p.s.interleaved), {}};
+    if (p.s.norm) r.x = at.fetch(rows + from, p.s.interleaved);
+    return r;
+  };
+  for_rows<L>(p.s, p.stride[which], which, tile, held, fetch, [&](const Rows& raw, long to, const Turn& turn) {
+    Pairs g = turn.back(at.take(raw.dy));
     if (p.s.norm) {
-      Pairs n = at.load(rows + from, p.s.interleaved);
+      Pairs n = at.take(raw.x);
       const float r = rsqrtf(row_sum<L>(dot(n, n)) * inv + p.s.eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         n.a[i] *= r;
         n.b[i] *= r;
         sum.a[i] = fmaf(g.a[i], n.a[i], sum.a[i]);
@@ -300,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(RotaryBwdParams<T>
       }
       const float C = row_sum<L>(dot(g, n)) * inv;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         g.a[i] = r * (g.a[i] - C * n.a[i]);
         g.b[i] = r * (g.b[i] - C * n.b[i]);
       }
@@ -313,8 +348,8 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(RotaryBwdParams<T>
 
 template <typename T, int L, bool WIDE>
 __global__ void __launch_bounds__(kThreads) rotary_bwdbwd_kernel(RotaryBwdBwdParams<T> p, int tile) {
-  __shared__ Angles<L> angles;
-  __shared__ float box[kThreads / 64 * L * 16];
+  __shared__ Tokens<L> held;
+  __shared__ float box[kThreads / 64 * L * 2 * N];
   const int which = blockIdx.y;
   const Columns<WIDE> at(p.s, threadIdx.x % L);
   const Pairs w = load_weight<T>(at, p.weight[which], p.s, 1.f);
@@ -324,14 +359,20 @@ __global__ void __launch_bounds__(kThreads) rotary_bwdbwd_kernel(RotaryBwdBwdPar
   const T* const dy = p.dy[which];
   const T* const cot = p.u[which];
   Pairs sum{};
-  for_rows<L>(p.s, p.stride[which], which, tile, angles, [&](long from, long to, const Turn& turn) {
-    Pairs n = at.load(rows + from, p.s.interleaved);
-    const Pairs g = turn.back(at.load(dy + to, p.s.interleaved));
-    const Pairs u = at.load(cot + to, p.s.interleaved);
+  struct Rows {
+    typename Columns<WIDE>::template Raw<T> x, dy, u;
+  };
+  auto fetch = [&](long from, long to) {
+    return Rows{at.fetch(rows + from, p.s.interleaved), at.fetch(dy + to, p.s.interleaved), at.fetch(cot + to, p.s.interleaved)};
+  };
+  for_rows<L>(p.s, p.stride[which], which, tile, held, fetch, [&](const Rows& raw, long to, const Turn& turn) {
+    Pairs n = at.take(raw.x);
+    const Pairs g = turn.back(at.take(raw.dy));
+    const Pairs u = at.take(raw.u);
     const float r = rsqrtf(row_sum<L>(dot(n, n)) * inv + p.s.eps);
     Pairs gw, zg;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       n.a[i] *= r, n.b[i] *= r;
       gw.a[i] = g.a[i] * w.a[i], gw.b[i] = g.b[i] * w.b[i];
       zg.a[i] = g.a[i] * z.a[i], zg.b[i] = g.b[i] * z.b[i];
@@ -348,7 +389,7 @@ __global__ void __launch_bounds__(kThreads) rotary_bwdbwd_kernel(RotaryBwdBwdPar
       sum1 = fmaf(r * g1, rest, sum1);
     };
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
       one(n.a[i], g.a[i], gw.a[i], zg.a[i], u.a[i], w.a[i], z.a[i], dd.a[i], d2.a[i], sum.a[i]);
       one(n.b[i], g.b[i], gw.b[i], zg.b[i], u.b[i], w.b[i], z.b[i], dd.b[i], d2.b[i], sum.b[i]);
     }
@@ -360,36 +401,42 @@ __global__ void __launch_bounds__(kThreads) rotary_bwdbwd_kernel(RotaryBwdBwdPar
 }
 
 // The workgroups' parts of both weights' gradients to one: a workgroup eight columns, whose
-// threads take every 32nd part and meet in LDS.
+// threads take every 64th part and meet in LDS.
+constexpr int kWeightThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) rotary_weights_kernel(const float* parts, void* out_q, void* out_k, int groups,
-                                                                  int head_dim, int wide_weights) {
-  __shared__ float box[kThreads];
+__global__ void __launch_bounds__(kWeightThreads) rotary_weights_kernel(const float* parts, void* out_q, void* out_k, int groups,
+                                                                        int head_dim, int wide_weights) {
+  __shared__ float box[kWeightThreads];
   void* const out = blockIdx.y ? out_k : out_q;
   if (out == nullptr) return;
+  constexpr int kWays = kWeightThreads / 8;
   const int col = 8 * (int)blockIdx.x + (int)threadIdx.x % 8, way = threadIdx.x / 8;
+  const float* const from = parts + (long)blockIdx.y * groups * head_dim + min(col, head_dim - 1);
   float sum = 0.f;
-  if (col < head_dim)
-    for (int i = way; i < groups; i += kThreads / 8) sum += parts[((long)blockIdx.y * groups + i) * head_dim + col];
+#pragma unroll 8
+  for (int i = way; i < groups; i += kWays) sum += from[(long)i * head_dim];
   box[threadIdx.x] = sum;
-  __syncthreads();
+  for (int half = kWays / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (way < half) box[threadIdx.x] += box[threadIdx.x + 8 * half];
+  }
   if (way > 0 || col >= head_dim) return;
-  for (int w = 1; w < kThreads / 8; ++w) sum += box[8 * w + threadIdx.x];
+  sum = box[threadIdx.x];
   if (wide_weights)
     ((float*)out)[col] = sum;
   else
     ((T*)out)[col] = (T)sum;
 }
 
-// f.template operator()<L, WIDE>() with the lanes that a row takes.
+// f.template operator()<L, WIDE>() with the lanes that a row takes, N pairs each.
 template <typename F> void with_lanes(int head_dim, bool wide, F&& f) {
   auto lanes = [&]<int L>() { wide ? f.template operator()<L, true>() : f.template operator()<L, false>(); };
   if (head_dim <= 64)
-    lanes.template operator()<4>();
+    lanes.template operator()<32 / N>();
   else if (head_dim <= 128)
-    lanes.template operator()<8>();
+    lanes.template operator()<64 / N>();
   else
-    lanes.template operator()<16>();
+    lanes.template operator()<128 / N>();
 }
 
 }  // namespace
@@ -398,7 +445,7 @@ template <typename T>
 hipError_t sum_rotary_weights(const float* parts, void* const out[2], const RotaryShape& s, int groups, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (out[0] == nullptr && out[1] == nullptr)) return e;
-  hipLaunchKernelGGL((rotary_weights_kernel<T>), dim3((s.head_dim + 7) / 8, 2), dim3(kThreads), 0, stream, parts, out[0],
+  hipLaunchKernelGGL((rotary_weights_kernel<T>), dim3((s.head_dim + 7) / 8, 2), dim3(kWeightThreads), 0, stream, parts, out[0],
                      out[1], groups, s.head_dim, s.wide_weights);
   return hipGetLastError();
 }
