@@ -67,7 +67,10 @@ inline BlockPlan block_plan(int total, int heads, int kv_heads, int head_dim, in
   p.slots = total * ((heads / kv_heads + 15) / 16);
   const long tiles = ((long)blocks * page_size + 31) / 32;
   const int waves = head_dim == 64 ? 8 : head_dim == 128 ? 4 : 2;
-  const long work = (long)p.slots * kv_heads, target = 8l * cus;
+  // Few long splits: a workgroup's start, four dependent loads, is as long as its walk over 500 keys. (Eight / four / two /
+  // one a CU, us, without the join, which one split does without: B16 x 64 blocks of 64, H32/8 D128 e4m3 38 / 30 / 26 / 27,
+  // B32 x 32 of 32 bf16 34 / 28 / 25 / 25, B64 x 64 of 16, H16/4 D64 18 / 18 / 15 / 15, B8 x 32 of 64 e4m3 17 / 17 / 13 / 12.)
+  const long work = (long)p.slots * kv_heads, target = cus;
   long splits = work >= target ? 1 : (target + work - 1) / work;
   const long least = work < 2l * cus ? waves : 4l * waves;
   if (splits > tiles / least) splits = tiles / least;
@@ -86,15 +89,16 @@ constexpr int kTileRows = 128;       // rows of a tile
 constexpr int kMostColumns = 8192;   // of the page table (the masks of 64 tokens are in LDS)
 constexpr int kSumBlocks = 256;      // blocks of a list (a join's weights are)
 constexpr int kMostLists = 32768;    // sequences times heads times columns
-// A tile of a list (the tokens that chose one column of a sequence, for one head): its rows from row0 of its first
-// entry's token on.
+// A tile of a list (the tokens that chose one column of a sequence, for one head): whole tokens, whose entries are
+// the tile's own kTileRows.
 struct BlockItem {
-  int first, row0, rows;  // entries from first on
+  int rows;
   int page, hk;
-  int key0;               // the column's first position
-  int shift;              // positions above the tokens' indexes in the slab
-  int pad;
+  int key0;   // the column's first position
+  int shift;  // positions above the tokens' indexes in the slab
+  int pad[3];
 };
+inline __host__ __device__ int tile_tokens(int group) { return kTileRows / group; }
 struct BlockEntryAt {
   int token, slot;  // of the slab; where its list has the column, first of all
 };
@@ -116,10 +120,10 @@ template <typename T, typename C> struct BlockChunkParams {
   unsigned long* masks;     // (kv_heads, groups, pages_per_seq) which of a group's tokens chose each column
   unsigned long* falling;   // (kv_heads, groups) whose lists do not rise
   int* before;              // (kv_heads, groups, pages_per_seq) entries of a list before the group
-  int* base;                // (lists) its first entry
-  BlockEntryAt* entries;
+  int* base;                // (lists) its first tile
+  BlockEntryAt* entries;    // (items, kTileRows)
   BlockItem* items;
-  int* totals;              // items, entries
+  int* total;               // of them; whether the offsets fall somewhere
   float* parts;      // (tokens, kv_heads, blocks, group, head_dim)
   float* parts_ml;   // and their maxima and sums
 };
@@ -138,8 +142,8 @@ inline BlockChunkPlan block_chunk_plan(int batch, int total, int heads, int kv_h
   p.lists = (long)batch * kv_heads * pages_per_seq;
   p.groups = (long)kv_heads * ((p.slab + 63) / 64);
   p.masks = p.groups * pages_per_seq;
-  p.entries = (long)p.slab * blocks * kv_heads;
-  p.items = (long)p.slab * blocks * heads / kTileRows + p.lists;
+  p.items = (long)p.slab * blocks * kv_heads / tile_tokens(heads / kv_heads) + p.lists;
+  p.entries = p.items * kTileRows;
   p.parts = (long)p.slab * heads * blocks;
   p.bytes = (size_t)(p.parts * (head_dim + 2) * 4 + p.items * sizeof(BlockItem) + p.entries * sizeof(BlockEntryAt) +
                      (p.masks + p.groups) * 8 + (p.masks + p.lists + 2) * 4);
@@ -155,11 +159,11 @@ template <typename T, typename C> void block_chunk_workspace(BlockChunkParams<T,
   p.falling = p.masks + plan.masks;
   p.before = (int*)(p.falling + plan.groups);
   p.base = p.before + plan.masks;
-  p.totals = p.base + plan.lists;
+  p.total = p.base + plan.lists;
 }
 // Whether a call goes a block at a time.
 inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int pages_per_seq, int blocks, bool single) {
-  return !single && pages_per_seq <= kMostColumns && blocks <= kSumBlocks &&
+  return !single && pages_per_seq <= kMostColumns && blocks <= kSumBlocks && heads / kv_heads <= kTileRows &&
          (long)batch * kv_heads * pages_per_seq <= kMostLists;
 }
 

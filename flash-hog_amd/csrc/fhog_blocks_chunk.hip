@@ -62,12 +62,20 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   const CacheShape& c = p.at;
   const int group = blockIdx.x, hk = blockIdx.y, width = c.pages_per_seq;
   const int count = min(64, p.tokens - 64 * group);
-  if (group == 0 && hk == 0 && threadIdx.x < 2) p.totals[threadIdx.x] = 0;
+  // Lists and their tokens agree on whose a token is only if the offsets rise. If they do not, nothing is listed,
+  // and the rows become NaN (block_sum_kernel).
+  bool falls = false;
+  for (int i = threadIdx.x; i < c.batch; i += kThreads) falls = falls || packed_begin(c, i + 1) < packed_begin(c, i);
+  falls = __syncthreads_or(falls);
+  if (group == 0 && hk == 0 && threadIdx.x == 0) {
+    p.total[0] = 0;
+    p.total[1] = falls;
+  }
   if (threadIdx.x == 0) s_falling = 0;
   for (int i = threadIdx.x; i < width; i += kThreads) s_mask[i] = 0;
   if ((int)threadIdx.x < count) {
     const PackedToken t(p, p.token0 + 64 * group + threadIdx.x);
-    s_token[threadIdx.x] = {t.there ? t.pos : -1};
+    s_token[threadIdx.x] = {t.there && !falls ? t.pos : -1};
   }
   __syncthreads();
   for (int i = threadIdx.x; i < count * p.blocks; i += kThreads) {
@@ -84,8 +92,8 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   if (threadIdx.x == 0) p.falling[(long)hk * p.groups + group] = s_falling;
 }
 
-// Four threads a list, each a quarter of the groups, and then the first: the list's entries and tiles get places
-// behind others', a wave at a time (in any order: each tile's outputs have places of their own).
+// Four threads a list, each a quarter of the groups, and then the first: the list's tiles get places behind
+// others', a wave at a time (in any order: each tile's outputs have places of their own).
 template <typename T, typename C> __global__ void __launch_bounds__(kThreads) block_items_kernel(BlockChunkParams<T, C> p) {
   __shared__ int s_count[4][64];
   const CacheShape& c = p.at;
@@ -114,28 +122,22 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   }
   if (way > 0) return;
   count = s_count[0][lane] + s_count[1][lane] + s_count[2][lane] + s_count[3][lane];
-  const int tiles = (int)(((long)count * group + kTileRows - 1) / kTileRows);
-  int sums[2], first[2];
-  const int before[2] = {wave_scan(tiles, sums[0]), wave_scan(count, sums[1])};
-  first[0] = 0;
-  if (lane < 2) first[0] = atomicAdd(&p.totals[lane], lane ? sums[1] : sums[0]);
-  first[1] = __shfl(first[0], 1, 64);
-  first[0] = __shfl(first[0], 0, 64);
+  const int each = tile_tokens(group), tiles = (count + each - 1) / each;
+  int sum, first = 0;
+  const int before = wave_scan(tiles, sum);
+  if (lane == 0) first = atomicAdd(p.total, sum);
+  first = __shfl(first, 0, 64) + before;
   if (count == 0) return;
-  p.base[i] = first[1] + before[1];
-  BlockItem item;
+  p.base[i] = first;
+  BlockItem item{};
   item.page = c.table[(long)b * width + col];
   item.hk = hk;
   item.key0 = col << c.page_shift;
   // (a token's position is its index in the packed rows, less its sequence's end, plus the length)
   item.shift = max(0, c.lengths[b]) - (c.offsets ? packed_begin(c, b + 1) : b + 1) + p.token0;
-  item.pad = 0;
   for (int k = 0; k < tiles; ++k) {
-    const long row = (long)k * kTileRows, left = (long)count * group - row;
-    item.first = first[1] + before[1] + (int)(row / group);
-    item.row0 = (int)(row % group);
-    item.rows = (int)(left < kTileRows ? left : kTileRows);
-    p.items[first[0] + before[0] + k] = item;
+    item.rows = min(each, count - k * each) * group;
+    p.items[first + k] = item;
   }
 }
 
@@ -153,6 +155,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
     slab_range(p, t.b, s_begin[threadIdx.x], s_end[threadIdx.x]);
   }
   const unsigned long falling = p.falling[(long)hk * p.groups + group];
+  const int each = tile_tokens(p.heads / c.kv_heads);
   __syncthreads();
   for (int i = threadIdx.x; i < count * p.blocks; i += kThreads) {
     const int t = i / p.blocks, at = i - t * p.blocks;
@@ -166,13 +169,15 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
     }
     const int begin = s_begin[t], end = s_end[t];
     const long place = ((long)hk * p.groups + group) * width + col;
-    const unsigned long bits = p.masks[place] & group_bits(group, begin, end) & ((1ul << t) - 1);
+    const unsigned long mask = p.masks[place], bits = mask & group_bits(group, begin, end) & ((1ul << t) - 1);
+    if (!(mask >> t & 1)) continue;  // (nothing is listed)
     const int before = group > begin / 64 ? p.before[place] : 0;
-    p.entries[p.base[((long)s_b[t] * c.kv_heads + hk) * width + col] + before + __popcll(bits)] = {64 * group + t, at};
+    const int rank = before + (int)__popcll(bits), tile = p.base[((long)s_b[t] * c.kv_heads + hk) * width + col] + rank / each;
+    p.entries[(long)tile * kTileRows + rank % each] = {64 * group + t, at};
   }
 }
 
-// 128 rows of tokens that chose one column, 32 a wave; row r of a list is its token r / group, head r % group.
+// Up to 128 rows of tokens that chose one column, 32 a wave; row r of a tile is its token r / group, head r % group.
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 128 ? 3 : 4)))
@@ -187,23 +192,31 @@ block_tile_kernel(BlockChunkParams<T, C> p) {
   __shared__ BlockEntryAt s_entry[kTileRows];
 
   const CacheShape& c = p.at;
-  const BlockItem item = p.items[blockIdx.x];  // (as many as there can be; read beside their number)
-  if ((int)blockIdx.x >= p.totals[0]) return;
-  const int group = p.heads / c.kv_heads, hk = item.hk, rows = item.rows;
-  const int count = (item.row0 + rows + group - 1) / group;  // tokens
-  if ((int)threadIdx.x < count) s_entry[threadIdx.x] = p.entries[item.first + threadIdx.x];
-  const int page_rows = 1 << c.page_shift;
+  const int group = p.heads / c.kv_heads, page_rows = 1 << c.page_shift;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, g = lane >> 5;
+  const bool negate = p.scale < 0.f;  // applied as |scale| to -q (negation is exact)
+  const float c2 = fabsf(p.scale) * kLog2e;
+  std::conditional_t<D == 64, SwzFrags<T, D>, WideFrags<T, D>> fr;
+  fr.init(lane);
+  const uint32_t lds = lds_base_u32(s_kv);
+
+  // (There is a place for as many tiles as there can be: this one's is read beside their number. A workgroup that
+  // took tile after tile, the next one's description a tile ahead, took 92 us where this takes 93, and 79 for 63 at D = 64.)
+  const BlockItem item = p.items[blockIdx.x];
+  const BlockEntryAt entry = p.entries[(long)blockIdx.x * kTileRows + threadIdx.x % kTileRows];
+  if ((int)blockIdx.x >= p.total[0]) return;
+  const int hk = item.hk, rows = item.rows, count = rows / group;  // tokens
+  if ((int)threadIdx.x < count) s_entry[threadIdx.x] = entry;
   const bool bad = (unsigned)item.page >= (unsigned)c.pages;
   const long line0 = ((long)(bad ? 0 : item.page) * c.kv_heads + hk) << c.page_shift;
   auto seen_by = [&](int token) { return (int)min((long)token + item.shift + 1 - item.key0, (long)page_rows); };
   __syncthreads();
   const int most = __builtin_amdgcn_readfirstlane(seen_by(s_entry[count - 1].token));  // (tokens rise)
 
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 31, g = lane >> 5;
   const bool any = 32 * wave < rows;
-  const int row = item.row0 + min(32 * wave + n, rows - 1);  // from the first token's first head on
+  const int row = min(32 * wave + n, rows - 1);
   const int token = row / group, head = row - token * group;
   const int seen = seen_by(s_entry[token].token);
   // Tiles of 32 keys, two stages: a tile is stored while the one before is worked on.
@@ -217,7 +230,6 @@ block_tile_kernel(BlockChunkParams<T, C> p) {
     tile.fetch(p.cache, at, threadIdx.x);
   };
   fetch(0);
-  const bool negate = p.scale < 0.f;  // applied as |scale| to -q (negation is exact)
   V8<T> qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
@@ -225,11 +237,7 @@ block_tile_kernel(BlockChunkParams<T, C> p) {
         p.q + ((long)(p.token0 + s_entry[token].token) * p.heads + hk * group + head) * D + 16 * ks + 8 * g);
     if (negate) qf[ks] = -qf[ks];
   }
-  const float c2 = fabsf(p.scale) * kLog2e;
 
-  std::conditional_t<D == 64, SwzFrags<T, D>, WideFrags<T, D>> fr;
-  fr.init(lane);
-  const uint32_t lds = lds_base_u32(s_kv);
   float m = -1e30f, lpart = 0.f;
   f32x16 acc[DT];
 #pragma unroll
@@ -290,12 +298,11 @@ block_tile_kernel(BlockChunkParams<T, C> p) {
   if (!any) return;
   if (bad) lpart = NAN;
   const float l = xgroup_sum(lpart);
-
   // Each row to its place, 128 bytes of it at a time: 32 x 32 outputs turned in LDS, in place of the tiles (all
   // waves are behind the last barrier, and each has a part of its own).
   const int mine = min(32, rows - 32 * wave);
   auto place = [&](int r) {  // of row r of this wave: the index of its outputs
-    const int at = item.row0 + 32 * wave + r, tk = at / group;
+    const int at = 32 * wave + r, tk = at / group;
     return ((long)(s_entry[tk].token * c.kv_heads + hk) * p.blocks + s_entry[tk].slot) * group + at - tk * group;
   };
   if (lane < mine) {
@@ -381,8 +388,9 @@ template <typename T, typename C, int D> __global__ void __launch_bounds__(kThre
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     for (int i = lane; i < count; i += 64) s_w[r][i] *= inv;
-    // a row that sees nothing: 0; a length beyond the table: NaN; no sequence's: 0, or left as it is
-    if (lane == 0) s_count[r] = pt.there ? (pt.beyond ? -1 : count) : p.clear_rest ? 0 : -2;
+    // a row that sees nothing: 0; a length beyond the table: NaN; no sequence's: 0, or left as it is; offsets that do
+    // not rise: NaN
+    if (lane == 0) s_count[r] = p.total[1] ? -1 : pt.there ? (pt.beyond ? -1 : count) : p.clear_rest ? 0 : -2;
   }
   __syncthreads();
   const int r = threadIdx.x / kLanes, column = 4 * (int)(threadIdx.x % kLanes);
@@ -407,7 +415,7 @@ hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p_, int slab, hipStr
   for (p.token0 = 0; p.token0 < p.at.total; p.token0 += slab) {
     p.tokens = p.at.total - p.token0 < slab ? p.at.total - p.token0 : slab;
     p.groups = (p.tokens + 63) / 64;
-    const long most = (long)p.tokens * p.blocks * p.heads / kTileRows + p.lists;
+    const long most = (long)p.tokens * p.blocks * p.at.kv_heads / tile_tokens(p.heads / p.at.kv_heads) + p.lists;
     hipLaunchKernelGGL((block_masks_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_items_kernel<T, C>), dim3((p.lists + 63) / 64), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_entries_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);

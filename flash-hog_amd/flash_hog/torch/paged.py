@@ -333,7 +333,8 @@ def paged_block_attention(query, blocks, key_cache, value_cache, page_table, len
     """paged_attention (without a window) in which a new token sees, through each key/value head, only the
     keys of the pages in columns blocks[token, head], up to its own position; blocks (T, N_kv, n) int32 as
     paged_block_select gives them. Columns outside the table or behind the token show nothing, one named
-    twice counts twice, and a token that sees no key gives zeros. out: as in paged_attention, but apart from query."""
+    twice counts twice, and a token that sees no key gives zeros. Offsets that fall somewhere may give NaN in every row.
+    out: as in paged_attention, but apart from query."""
     through = _checked("paged_block_attention", (blocks, page_table, lengths, query_offsets), query, key_cache, value_cache,
                        key_scale, value_scale, out)
     scale = _default_scale(query, scale)

@@ -305,6 +305,16 @@ def test_bad_pages_and_lengths(cuda_device):
         lists = flash_hog.paged_block_select(args[0], means, **more, page_size=16, blocks=3)
         assert ((lists >= -1) & (lists < 8)).all()
         assert flash_hog.paged_block_attention(*args, **more).shape == q.shape
+    # many tokens a sequence: rows of offsets that fall are NaN, all of them; offsets are cut to the rows first
+    many = q[:1].expand(200, -1, -1).contiguous().to(cuda_device)
+    some = torch.zeros((200, 2, 3), dtype=torch.int32, device=cuda_device)
+    for offsets, falls in (([0, 150, 100, 200], True), ([0, 200, 0, 200], True), ([200, 100, 50, 0], True), ([-7, 60, 60, 2 ** 31 - 1], False)):
+        more = {**where, "query_offsets": torch.tensor(offsets, dtype=torch.int32, device=cuda_device)}
+        out = flash_hog.paged_block_attention(many, some, *args[2:], **more)
+        assert torch.isnan(out).all() if falls else torch.isfinite(out).all()
+        lists = flash_hog.paged_block_select(many, means, **more, page_size=16, blocks=3)
+        assert lists.shape == (200, 2, 3)
+        flash_hog.paged_key_means(moved["key_cache"], means, **more)
 
 
 def test_serving_loop(cuda_device):
