@@ -988,7 +988,7 @@ size_t fhog_paged_block_workspace_bytes(int batch, int total, int single, int he
   static const char* who = "fhog_paged_block_workspace_bytes";
   const Paged s{batch, total, heads, kv_heads, head_dim, 1, page_size, pages_per_seq, FHOG_DTYPE_BF16, FHOG_DTYPE_BF16};
   if (check_paged(s, who) || check_blocks(who, s, blocks) || batch < 1 || total < 1) return 0;
-  if (fhog::block_chunk_rule(batch, total, heads, kv_heads, pages_per_seq, blocks, single != 0))
+  if (fhog::block_chunk_rule(batch, total, heads, kv_heads, head_dim, page_size, pages_per_seq, blocks, single != 0))
     return fhog::block_chunk_plan(batch, total, heads, kv_heads, head_dim, pages_per_seq, blocks).bytes;
   const fhog::BlockPlan plan = fhog::block_plan(total, heads, kv_heads, head_dim, page_size, blocks, compute_units());
   return (size_t)plan.parts * (head_dim + 2) * sizeof(float);
@@ -1019,7 +1019,7 @@ int fhog_paged_block_attention(fhog_stream_t stream, const void* q, const int* c
                                                        page_size, pages_per_seq, blocks);
   if (need > 0 && (!aligned(workspace, 16) || workspace_bytes < need))
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null, not 16-byte aligned or below its %zu bytes", who, need);
-  if (fhog::block_chunk_rule(batch, total, heads, kv_heads, pages_per_seq, blocks, query_offsets == nullptr)) {
+  if (fhog::block_chunk_rule(batch, total, heads, kv_heads, head_dim, page_size, pages_per_seq, blocks, query_offsets == nullptr)) {
     const fhog::BlockChunkPlan plan = fhog::block_chunk_plan(batch, total, heads, kv_heads, head_dim, pages_per_seq, blocks);
     auto run = [&]<typename T, typename C, int D>() {
       fhog::BlockChunkParams<T, C> p{(const T*)q, (T*)out,

@@ -161,10 +161,22 @@ template <typename T, typename C> void block_chunk_workspace(BlockChunkParams<T,
   p.base = p.before + plan.masks;
   p.total = p.base + plan.lists;
 }
-// Whether a call goes a block at a time.
-inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int pages_per_seq, int blocks, bool single) {
-  return !single && pages_per_seq <= kMostColumns && blocks <= kSumBlocks && heads / kv_heads <= kTileRows &&
-         (long)batch * kv_heads * pages_per_seq <= kMostLists;
+// Whether a call goes a block at a time: where its estimate is below that of a token at a time. A chosen block of a token
+// and head (an entry) costs a token's kernel its keys and values out of a cache, at 14 TB/s with 16-bit elements; a block at
+// a time costs it fp32 outputs written and read, at 3.8 TB/s both ways, and each listed block its keys and values once. Five
+// more launches are 16 us. (us a block / a token at a time, table of 8192 positions, bf16: H32/8 D128, 16 blocks of 64, one
+// sequence of 8 / 32 / 128 / 512 / 2048 tokens 24 / 12, 30 / 17, 41 / 42, 79 / 140, 330 / 543; 16 sequences of 2 / 8 / 32 tokens
+// 47 / 20, 57 / 43, 95 / 143. One of 2048 tokens: H8/8 83 / 500, H32/4 321 / 306, H8/1 D256 195 / 172, blocks of 32 305 / 353;
+// of 512, 32 blocks of 16 166 / 91. e4m3 takes a token's kernel 8 to 25 % less; the sides change where they are as near.)
+inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int head_dim, int page_size, int pages_per_seq,
+                             int blocks, bool single) {
+  const int group = heads / kv_heads;
+  const long lists = (long)batch * kv_heads * pages_per_seq;
+  if (single || pages_per_seq > kMostColumns || blocks > kSumBlocks || group > kTileRows || lists > kMostLists) return false;
+  const double entries = (double)total * kv_heads * blocks, block = 4.0 * page_size * head_dim;
+  const double token_us = entries * block / 14e6;
+  const double block_us = 16 + entries * 8.0 * group * (head_dim + 2) / 3.8e6 + (entries < lists ? entries : lists) * block / 14e6;
+  return block_us < token_us;
 }
 
 template <typename T, typename C, int D>

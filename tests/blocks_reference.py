@@ -62,3 +62,30 @@ def attention(q, cache, new, chosen, scale):
                     out[row, h] = w @ v[s, n]
             row += 1
     return out
+
+
+def attention_dense(q, cache, new, chosen, scale):
+    """attention() for many tokens: the softmax over all keys, each as often as the token's list shows it."""
+    T, H, D = q.shape
+    N, width, page = cache.cache["k"].shape[1], cache.table.shape[1], cache.page
+    G = H // N
+    out = torch.zeros((T, H, D), dtype=torch.float64)
+    ends = torch.tensor(new).cumsum(0).tolist()
+    for count, end, length, b in zip(new, ends, cache.lengths, range(len(new))):
+        if not count or not length:
+            continue
+        k, v = cache.rows("k", b, length), cache.rows("v", b, length)
+        at = torch.arange(length)
+        seen = at <= torch.arange(length - count, length)[:, None]
+        for n in range(N):
+            lists = chosen[end - count:end, n].long()
+            lists = torch.where((lists >= 0) & (lists < width), lists, width)
+            times = torch.zeros((count, width + 1), dtype=torch.float64).scatter_add_(1, lists, torch.ones(lists.shape, dtype=torch.float64))
+            times = times[:, at // page] * seen
+            s = q[end - count:end, n * G:(n + 1) * G].double() @ k[:, n].T * scale  # (count, G, length)
+            s = torch.where(times[:, None] > 0, s, -torch.inf)
+            top = s.amax(-1, keepdim=True).clamp(min=-1e300)
+            w = times[:, None] * torch.exp(s - top)
+            total = w.sum(-1, keepdim=True)
+            out[end - count:end, n * G:(n + 1) * G] = (w / torch.where(total > 0, total, 1.0)) @ v[:, n]
+    return out

@@ -305,16 +305,127 @@ def test_bad_pages_and_lengths(cuda_device):
         lists = flash_hog.paged_block_select(args[0], means, **more, page_size=16, blocks=3)
         assert ((lists >= -1) & (lists < 8)).all()
         assert flash_hog.paged_block_attention(*args, **more).shape == q.shape
-    # many tokens a sequence: rows of offsets that fall are NaN, all of them; offsets are cut to the rows first
-    many = q[:1].expand(200, -1, -1).contiguous().to(cuda_device)
-    some = torch.zeros((200, 2, 3), dtype=torch.int32, device=cuda_device)
-    for offsets, falls in (([0, 150, 100, 200], True), ([0, 200, 0, 200], True), ([200, 100, 50, 0], True), ([-7, 60, 60, 2 ** 31 - 1], False)):
-        more = {**where, "query_offsets": torch.tensor(offsets, dtype=torch.int32, device=cuda_device)}
-        out = flash_hog.paged_block_attention(many, some, *args[2:], **more)
-        assert torch.isnan(out).all() if falls else torch.isfinite(out).all()
-        lists = flash_hog.paged_block_select(many, means, **more, page_size=16, blocks=3)
-        assert lists.shape == (200, 2, 3)
-        flash_hog.paged_key_means(moved["key_cache"], means, **more)
+
+
+# (heads, kv_heads, head_dim, dtype, quantised, page, lengths, new, blocks): so many entries that blocks are taken
+# one at a time
+MANY = [
+    (4, 4, 64, BF16, False, 64, [2000, 130, 0, 77], [400, 130, 0, 9], 13),
+    (8, 4, 128, BF16, False, 128, [1500, 700], [333, 260], 8),
+    (3, 3, 64, FP16, True, 64, [900, 1030], [260, 900], 15),
+    (4, 2, 256, FP16, True, 128, [1700], [401], 9),
+    (6, 2, 128, BF16, False, 256, [3000, 1, 300], [700, 1, 250], 7),
+    (8, 8, 64, FP16, False, 16, [1300, 40], [1300, 40], 14),
+    (2, 2, 256, BF16, False, 32, [2050], [2050], 17),
+    (8, 2, 128, BF16, True, 64, [1200] * 5, [130, 64, 63, 1, 1200], 16),
+    (32, 1, 64, BF16, False, 1024, [5000], [700], 4),             # 4 tokens a tile
+    (5, 5, 128, BF16, False, 64, [8000], [300], 70),
+]
+
+
+def many_lists(case, cache, counts, kind):
+    """Rising lists as a choice gives them, or any: not rising, with columns twice, behind the token or outside the table."""
+    blocks, T, N, width = case[8], sum(counts), case[1], cache.table.shape[1]
+    gen = torch.Generator().manual_seed(4)
+    if kind == "any":
+        lists = torch.randint(-1, width + 2, (T, N, blocks), generator=gen).to(torch.int32)
+        lists[::3, 0] = -1
+        lists[1::4, :, 3] = 2 ** 31 - 1
+        lists[2::4, :, 2] = -2 ** 31
+        return lists
+    at = torch.cat([torch.arange(n - c, n) for n, c in zip(cache.lengths, counts)])
+    own = (at // cache.page).clamp(min=0)[:, None, None]
+    scores = torch.rand((T, N, width), generator=gen)
+    columns = torch.arange(width)
+    scores = torch.where(columns < own, scores, torch.where(columns == own, 2.0, -1.0))
+    best, lists = scores.topk(min(blocks, width), -1)
+    lists = torch.where(best >= 0, lists, 2 ** 31 - 1).sort(-1).values
+    lists = torch.where(lists == 2 ** 31 - 1, -1, lists).to(torch.int32)
+    return torch.nn.functional.pad(lists, (0, blocks - lists.shape[-1]), value=-1)
+
+
+@pytest.mark.parametrize("kind", ["chosen", "any"])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: case_id((*c, 1, 1)))
+def test_many_tokens(case, kind, cuda_device):
+    import flash_hog
+
+    print("[case] many tokens", case_id((*case, 1, 1)), kind, flush=True)
+    cache, counts, q, moved, where = make(case, cuda_device)
+    lists = many_lists(case, cache, counts, kind)
+    for scale in (None, -0.21):
+        got = flash_hog.paged_block_attention(q.to(cuda_device), lists.to(cuda_device), moved["key_cache"],
+                                              moved["value_cache"], **where, **scales(moved), scale=scale)
+        check(got, ref.attention_dense(q, cache, counts, lists, scale or q.shape[-1] ** -0.5), case_id((*case, 1, 1)))
+    if kind == "any":
+        assert not got[::3, :case[0] // case[1]].any()
+
+
+def test_many_tokens_of_no_sequence(cuda_device):
+    """Rows of no sequence between many that have one; pages outside the cache; lengths beyond the table and shorter
+    than the new tokens; two sequences' tokens in one group of 64; offsets that fall, where all rows are NaN."""
+    import flash_hog
+
+    print("[case] many tokens of no sequence", flush=True)
+    case = MANY[0]
+    cache, counts, q, moved, where = make(case, cuda_device)
+    lists = many_lists(case, cache, counts, "chosen")
+    kv = moved["key_cache"], moved["value_cache"]
+    pad = lambda x, value: torch.cat([torch.full_like(x[:70], value), x, torch.full_like(x[:33], value)])
+    padded, plists = pad(q, 3.0).to(cuda_device), pad(lists, 0).to(cuda_device)
+    more = {**where, "query_offsets": where["query_offsets"] + 70}
+    exact = ref.attention_dense(q, cache, counts, lists, 0.125)
+    out = flash_hog.paged_block_attention(padded, plists, *kv, **more)
+    check(out[70:-33], exact)
+    assert not out[:70].any() and not out[-33:].any()
+    given = torch.full_like(padded, 7.0)
+    assert flash_hog.paged_block_attention(padded, plists, *kv, **more, out=given) is given
+    assert torch.equal(given[70:-33], out[70:-33]) and (given[:70] == 7).all() and (given[-33:] == 7).all()
+    for entry in (-1, cache.cache["k"].shape[0], 2 ** 31 - 1, -2 ** 31):
+        table = moved["page_table"].clone()
+        table[0, 5] = entry
+        hit = (lists == 5).any(-1) & (torch.arange(539) < 400)[:, None]
+        bad = flash_hog.paged_block_attention(padded, plists, *kv, **{**more, "page_table": table})[70:-33]
+        nan = torch.isnan(bad).all(-1).cpu()
+        assert torch.equal(nan, hit) and torch.equal(torch.isnan(bad).any(-1).cpu(), hit)
+        assert torch.equal(bad[~nan.to(cuda_device)], out[70:-33][~nan.to(cuda_device)])
+    lengths = moved["lengths"].clone()
+    lengths[1] = 2 ** 31 - 1
+    bad = flash_hog.paged_block_attention(padded, plists, *kv, **{**more, "lengths": lengths})[70:-33]
+    assert torch.isnan(bad[400:530]).all() and torch.equal(bad[:400], out[70:470]) and torch.equal(bad[530:], out[600:-33])
+    lengths[1] = 100  # its first 30 tokens see nothing
+    bad = flash_hog.paged_block_attention(padded, plists, *kv, **{**more, "lengths": lengths})[70:-33]
+    assert not bad[400:430].any() and torch.equal(bad[:400], out[70:470]) and torch.equal(bad[530:], out[600:-33])
+    rows = padded.shape[0]
+    for offsets in ([0, 400, 300, 500, 600], [0, rows, 0, rows, rows], [rows, 300, 200, 100, 0], [-7, 60, 60, 70, 2 ** 31 - 1]):
+        more["query_offsets"] = torch.tensor(offsets, dtype=torch.int32, device=cuda_device)
+        out = flash_hog.paged_block_attention(padded, plists, *kv, **more)
+        assert torch.isnan(out).all() if offsets[0] != -7 else torch.isfinite(out).all()
+        choice = flash_hog.paged_block_select(padded, all_means(cache).to(cuda_device), **more, page_size=64, blocks=13)
+        assert ((choice >= -1) & (choice < cache.table.shape[1])).all()
+
+
+def test_many_tokens_in_slabs(cuda_device):
+    """More tokens than one slab holds, captured, replayed with other lists, and each like the call of its own."""
+    import flash_hog
+
+    print("[case] many tokens in slabs", flush=True)
+    case = (8, 4, 64, BF16, False, 64, [5000, 3000], [3001, 2900], 24)  # 48 KiB a token and 256 MiB a slab
+    cache, counts, q, moved, where = make(case, cuda_device)
+    kv = moved["key_cache"], moved["value_cache"]
+    q = q.to(cuda_device)
+    runs = [many_lists(case, cache, counts, kind) for kind in ("chosen", "any")]
+    want = [flash_hog.paged_block_attention(q, lists.to(cuda_device), *kv, **where) for lists in runs]
+    check(want[1], ref.attention_dense(q.cpu(), cache, counts, runs[1], 0.125))
+    given = runs[0].to(cuda_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = flash_hog.paged_block_attention(q, given, *kv, **where)
+    for i in (0, 1, 0, 1):
+        given.copy_(runs[i])
+        graph.replay()
+        flash_hog.paged_block_attention(q, runs[1 - i].to(cuda_device), *kv, **where)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
 
 
 def test_serving_loop(cuda_device):
