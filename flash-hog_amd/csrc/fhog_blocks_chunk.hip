@@ -7,6 +7,12 @@
 // list gives it, and a last kernel joins a row's outputs in the order of its list: no atomics on numbers, the
 // same bits at every call.
 //
+// What bounds it: those outputs, written and read once, 8 (head_dim + 2) bytes for each row and block, in slabs that fit
+// the 256 MB behind the L2s. 3900 tokens in 4 sequences, H32/8 D128 bf16, 16 blocks of 64, us for each of two slabs of
+// 250 MB: masks 6, items 6, entries 6, tiles 91 (without their stores 57), sum 50 (5.0 TB/s). 4096 tokens, H12/12 D64 e4m3, 16
+// blocks: 9, 9, 10, 58, 52. (A token at a time 583 and 744 in all; slabs of 64 / 128 / 256 / 1024 MB 422 / 316 / 333 / 346 us
+// for tiles and sums, and half the launches with 256.)
+//
 //   block_masks_kernel   64 tokens and a key/value head: which of them chose each column
 //   block_items_kernel   tokens of each sequence, head and column: how many, in tiles of 128 rows
 //   block_entries_kernel who they are, in order
@@ -27,8 +33,8 @@ struct PackedToken {
   bool there, beyond;
   template <typename P> __device__ __forceinline__ PackedToken(const P& p, int t) {
     const CacheShape& c = p.at;
-    b = c.offsets ? last_at_or_before(c.batch, t, [&](int s) { return packed_begin(c, s); }) : t;
-    const int begin = packed_begin(c, b), end = c.offsets ? packed_begin(c, b + 1) : b + 1;
+    b = last_at_or_before(c.batch, t, [&](int s) { return packed_begin(c, s); });
+    const int begin = packed_begin(c, b), end = packed_begin(c, b + 1);
     there = t >= begin && t < end;
     const int length = max(0, c.lengths[b]);
     beyond = length > (long)c.pages_per_seq << c.page_shift;
@@ -42,8 +48,8 @@ struct PackedToken {
 
 // Tokens of sequence b among the slab's, as indexes from its first on.
 template <typename P> __device__ __forceinline__ void slab_range(const P& p, int b, int& begin, int& end) {
-  begin = (p.at.offsets ? packed_begin(p.at, b) : b) - p.token0;
-  end = (p.at.offsets ? packed_begin(p.at, b + 1) : b + 1) - p.token0;
+  begin = packed_begin(p.at, b) - p.token0;
+  end = packed_begin(p.at, b + 1) - p.token0;
   begin = max(begin, 0);
   end = max(begin, min(end, p.tokens));
 }
@@ -202,11 +208,13 @@ block_tile_kernel(BlockChunkParams<T, C> p) {
   fr.init(lane);
   const uint32_t lds = lds_base_u32(s_kv);
 
-  // (There is a place for as many tiles as there can be: this one's is read beside their number. A workgroup that
-  // took tile after tile, the next one's description a tile ahead, took 92 us where this takes 93, and 79 for 63 at D = 64.)
-  const BlockItem item = p.items[blockIdx.x];
-  const BlockEntryAt entry = p.entries[(long)blockIdx.x * kTileRows + threadIdx.x % kTileRows];
-  if ((int)blockIdx.x >= p.total[0]) return;
+  // An eighth of the tiles, which are ordered by sequence and head, to each XCD: its L2 has their queries, and the keys of
+  // tiles of one list. (94 us before, 62 at D = 64; runs of 16 / 64 / 256 tiles a XCD 92 / 95 / 107. A workgroup that took
+  // tile after tile, the next one's description a tile ahead, took 92 where this took 94, and 79 for 63.)
+  const int all = p.total[0], each = (all + 7) / 8, index = blockIdx.x % 8 * each + blockIdx.x / 8;
+  if ((int)blockIdx.x / 8 >= each || index >= all) return;
+  const BlockItem item = p.items[index];
+  const BlockEntryAt entry = p.entries[(long)index * kTileRows + threadIdx.x % kTileRows];
   const int hk = item.hk, rows = item.rows, count = rows / group;  // tokens
   if ((int)threadIdx.x < count) s_entry[threadIdx.x] = entry;
   const bool bad = (unsigned)item.page >= (unsigned)c.pages;
@@ -419,7 +427,8 @@ hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p_, int slab, hipStr
     hipLaunchKernelGGL((block_masks_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_items_kernel<T, C>), dim3((p.lists + 63) / 64), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_entries_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((block_tile_kernel<T, C, D>), dim3((unsigned)most), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((block_tile_kernel<T, C, D>), dim3((unsigned)((most + 7) / 8 * 8)), dim3(kThreads), 0,
+                       stream, p);
     constexpr long R = kThreads / (D / 4);
     hipLaunchKernelGGL((block_sum_kernel<T, C, D>), dim3((unsigned)(((long)p.tokens * p.heads + R - 1) / R)), dim3(kThreads), 0,
                        stream, p);
