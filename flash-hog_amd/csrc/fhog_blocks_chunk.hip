@@ -8,7 +8,7 @@
 // same bits at every call.
 //
 // What bounds it: those outputs, written and read once, 8 (head_dim + 2) bytes for each row and block, in slabs that fit
-// the 256 MB behind the L2s. 3900 tokens in 4 sequences, H32/8 D128 bf16, 16 blocks of 64, us for each of two slabs of
+// the 256 MB behind the L2s. 2035 tokens in 4 sequences, H32/8 D128 bf16, 16 blocks of 64, us for each slab of
 // 250 MB: masks 6, items 6, entries 6, tiles 91 (without their stores 57), sum 50 (5.0 TB/s). 4096 tokens, H12/12 D64 e4m3, 16
 // blocks: 9, 9, 10, 58, 52. (A token at a time 583 and 744 in all; slabs of 64 / 128 / 256 / 1024 MB 422 / 316 / 333 / 346 us
 // for tiles and sums, and half the launches with 256.)
@@ -140,7 +140,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   item.hk = hk;
   item.key0 = col << c.page_shift;
   // (a token's position is its index in the packed rows, less its sequence's end, plus the length)
-  item.shift = max(0, c.lengths[b]) - (c.offsets ? packed_begin(c, b + 1) : b + 1) + p.token0;
+  item.shift = max(0, c.lengths[b]) - packed_begin(c, b + 1) + p.token0;
   for (int k = 0; k < tiles; ++k) {
     item.rows = min(each, count - k * each) * group;
     p.items[first + k] = item;

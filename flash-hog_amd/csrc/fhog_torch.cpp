@@ -1024,6 +1024,10 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
     // (without norms the cotangents stand in for the rows, of which only the shapes matter)
     const at::Tensor q = o.eps ? r[4] : grads[0].detach(), k = o.eps ? r[5] : grads[1].detach();
     const at::Tensor wq = o.eps ? r[6] : none, wk = o.eps ? r[7] : none;
+    if (!c10::GradMode::is_enabled()) {  // no graph, no node
+      const auto [dq, dk, dwq, dwk] = rotary_bwd_core(q, k, wq, wk, grads[0], grads[1], RotarySaved::where(r), o);
+      return {none, dq, dk, dwq, dwk, none, none, none, none};
+    }
     const variable_list d = RotaryBwdFn::apply(o, q, k, maybe(wq), maybe(wk), grads[0], grads[1], maybe(r[0]), maybe(r[1]),
                                               maybe(r[2]), maybe(r[3]));
     return {none, d[0], d[1], wq.defined() ? d[2] : none, wk.defined() ? d[3] : none, none, none, none, none};
