@@ -333,7 +333,8 @@ int fhog_paged_key_means(fhog_stream_t stream, const void* k_cache, const void* 
  * a page that is not full yet is never chosen by its mean), and of the others those whose mean has the largest
  * product with the sum of the queries q (total, heads, head_dim) of the head's group, formed in 64 bits, ties to
  * the lowest column, NaN (also: a page outside the cache) last; `blocks` (>= first + last) in all, or all there
- * are. Tokens of no sequence, before position 0 or beyond the table: -1 throughout.
+ * are. Tokens of no sequence, before position 0 or beyond the table: -1 throughout. Offsets that fall somewhere may
+ * leave lists of any values.
  */
 size_t fhog_paged_block_select_workspace_bytes(int batch, int total, int single, int kv_heads, int pages_per_seq, int first,
                                                int last);
@@ -345,7 +346,8 @@ int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* ke
 /*
  * fhog_paged_attention (without a window) in which a token sees, through each key/value head, only the keys
  * of the pages in columns chosen[token][head], up to its own position. Columns outside [0, pages_per_seq) and
- * ones behind the token show nothing; one that is named twice counts twice.
+ * ones behind the token show nothing; one that is named twice counts twice. Offsets that fall somewhere may give NaN
+ * in every row.
  */
 size_t fhog_paged_block_workspace_bytes(int batch, int total, int single, int heads, int kv_heads, int head_dim,
                                         int page_size, int pages_per_seq, int blocks);
