@@ -939,10 +939,10 @@ int fhog_paged_key_means(fhog_stream_t stream, const void* k_cache, const void* 
                        who);
 }
 
-size_t fhog_paged_block_select_workspace_bytes(int batch, int total, int single, int kv_heads, int pages_per_seq, int first,
-                                               int last) {
+size_t fhog_paged_block_select_workspace_bytes(int batch, int total, int single, int kv_heads, int head_dim,
+                                               int pages_per_seq, int first, int last) {
   if (batch < 1 || total < 1 || kv_heads < 1 || pages_per_seq < 1 || first < 0 || last < 1) return 0;
-  return (size_t)fhog::select_plan(batch, total, single != 0, kv_heads, pages_per_seq, first, last).slab * kv_heads *
+  return (size_t)fhog::select_plan(batch, total, single != 0, kv_heads, head_dim, pages_per_seq, first, last).slab * kv_heads *
          pages_per_seq * 8;
 }
 
@@ -965,11 +965,11 @@ int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* ke
   if (int st = check_ptrs(who, {{"q", q}, {"key_means", key_means}},
                           {{"page_table", page_table}, {"lengths", lengths}, {"chosen", chosen}}))
     return st;
-  const fhog::SelectPlan plan = fhog::select_plan(batch, total, query_offsets == nullptr, kv_heads, pages_per_seq, first, last);
+  const fhog::SelectPlan plan = fhog::select_plan(batch, total, query_offsets == nullptr, kv_heads, head_dim, pages_per_seq, first, last);
   if ((long long)plan.slots * kv_heads >= (1ll << 23))
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: problem too large", who);
-  const size_t need = fhog_paged_block_select_workspace_bytes(batch, total, query_offsets == nullptr, kv_heads, pages_per_seq,
-                                                              first, last);
+  const size_t need = fhog_paged_block_select_workspace_bytes(batch, total, query_offsets == nullptr, kv_heads, head_dim,
+                                                              pages_per_seq, first, last);
   if (need > 0 && (!aligned(workspace, 8) || workspace_bytes < need))
     return fail(FHOG_ERR_INVALID_ARGUMENT, "%s: workspace is null, not 8-byte aligned or below its %zu bytes", who, need);
   auto run = [&]<typename T>() {

@@ -8,8 +8,8 @@
 // between the ones with the largest scores, ties to the lowest index; NaN is below every number.
 //
 // Scores are kept as their bits in an order that compares as they do. Where sequences have many new tokens, 16 of
-// them share the means' reads, as matrix products of 64 bits, whose scores stay in LDS; a wave then chooses for a
-// token. Else, and where a table is wider than LDS, scores go through memory.
+// them share the means' reads, as matrix products of 64 bits, whose scores stay in LDS, where a wave chooses for a
+// token; few tokens have a workgroup each. Else, and for tables wider than LDS, scores go through memory.
 #include "fhog_blocks.h"
 
 namespace fhog {
@@ -255,6 +255,20 @@ template <int KJ, typename F> __device__ __forceinline__ void choose_in_wave(int
 
 // ------------------------------------------------------------------ scores
 
+// Sum over sixteen neighbouring lanes, in all of them.
+__device__ __forceinline__ double row16_sum(double x) {
+  auto step = [&](auto moved) {
+    const long bits = __builtin_bit_cast(long, x);
+    const uint32_t lo = (uint32_t)moved((int)bits), hi = (uint32_t)moved((int)(bits >> 32));
+    x += __builtin_bit_cast(double, (unsigned long)hi << 32 | lo);
+  };
+  step([](int i) { return __builtin_amdgcn_mov_dpp(i, 0xb1, 0xf, 0xf, true); });   // quad_perm:[1,0,3,2]
+  step([](int i) { return __builtin_amdgcn_mov_dpp(i, 0x4e, 0xf, 0xf, true); });   // quad_perm:[2,3,0,1]
+  step([](int i) { return __builtin_amdgcn_mov_dpp(i, 0x141, 0xf, 0xf, true); });  // row_half_mirror
+  step([](int i) { return __builtin_amdgcn_mov_dpp(i, 0x140, 0xf, 0xf, true); });  // row_mirror
+  return x;
+}
+
 // A token's scores of kColumns columns for a key/value head; sixteen lanes a column.
 constexpr int kColumns = 64;
 template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_score_kernel(BlockSelectParams<T> p) {
@@ -299,8 +313,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_s
     for (int j = 0; j < E / 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum = fma(q[4 * j + e], (double)m[i][j][e], sum);
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    sum = row16_sum(sum);
     const int col = c0 + way + 16 * i;
     if (lane == 0 && col >= tb.lo && col < tb.hi) scores[col] = (unsigned)page[i] < (unsigned)c.pages ? sortable(sum) : 0;
   }
@@ -415,6 +428,78 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads) block_s
   });
 }
 
+// A token and key/value head by itself: scores of up to COLUMNS columns in LDS, sixteen lanes a column, of which a wave
+// chooses. (32 of 500 columns, H16/4 D64 7.3 us, and 64 of up to 1024, 16 tokens of H32/8 D128 16.2: 5.2 and 12.4 of it the
+// scores. Scores in memory and a launch of its own for the choice: 4.3 + 5.2 and 11.5 + 7.0.)
+constexpr int kTokenThreads = 1024;
+template <typename T, int D, int COLUMNS> __global__ void __launch_bounds__(kTokenThreads) block_select_token_kernel(BlockSelectParams<T> p) {
+  constexpr int E = D / 16, kWays = kTokenThreads / 16, kEach = 4;
+  __shared__ unsigned long s_key[COLUMNS];
+  __shared__ __attribute__((aligned(16))) double s_q[D];
+  const CacheShape& c = p.at;
+  const int hk = blockIdx.x % c.kv_heads, t = p.token0 + blockIdx.x / c.kv_heads;
+  const TokenAt token(c, t);
+  const TokenBlocks tb(p, token.pos);
+  int* const out = p.chosen + ((long)t * c.kv_heads + hk) * p.blocks;
+  write_forced(tb, out, p.blocks, threadIdx.x, kTokenThreads);
+  if (!tb.by_score() || tb.room == 0) return;
+  const int lane = threadIdx.x % 16, way = threadIdx.x / 16, group = p.heads / c.kv_heads;
+  // A step's means are loaded a step ahead, their pages another one.
+  const int* const table = c.table + (long)token.b * c.pages_per_seq;
+  int page[kEach], ahead[kEach];
+  f32x4 m[kEach][E / 4];
+  bool bad[kEach];
+  auto pages = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) ahead[i] = table[min(c0 + way + kWays * i, tb.hi - 1)];
+  };
+  auto load = [&] {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      page[i] = ahead[i];
+      bad[i] = (unsigned)page[i] >= (unsigned)c.pages;
+      const float* from = p.means + ((long)(bad[i] ? 0 : page[i]) * c.kv_heads + hk) * D + lane * 4;
+#pragma unroll
+      for (int j = 0; j < E / 4; ++j) m[i][j] = *reinterpret_cast<const f32x4*>(from + 64 * j);
+    }
+  };
+  pages(tb.lo);
+  if ((int)threadIdx.x < D) {
+    const T* row = p.q + ((long)t * p.heads + hk * group) * D + threadIdx.x;
+    double sum = 0.;
+#pragma unroll 4
+    for (int h = 0; h < group; ++h) sum += (double)(float)row[h * D];
+    s_q[threadIdx.x] = sum;
+  }
+  load();
+  __syncthreads();
+  double q[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) q[j] = s_q[64 * (j / 4) + lane * 4 + j % 4];
+  for (int c0 = tb.lo; c0 < tb.hi; c0 += kWays * kEach) {
+    double sum[kEach] = {};
+    bool none[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      none[i] = bad[i];
+#pragma unroll
+      for (int j = 0; j < E; ++j) sum[i] = fma(q[j], (double)m[i][j / 4][j % 4], sum[i]);
+    }
+    if (c0 + kWays * kEach < tb.hi) {
+      pages(c0 + kWays * kEach);
+      load();
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      sum[i] = row16_sum(sum[i]);
+      const int col = c0 + way + kWays * i;
+      if (lane == 0 && col < tb.hi) s_key[col - tb.lo] = none[i] ? 0ul : sortable(sum[i]);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) choose_in_wave<COLUMNS / 64>(tb.hi - tb.lo, tb.lo, tb.room, out + tb.lo, [&](int i) { return s_key[i]; });
+}
+
 // ------------------------------------------------------------------ choice from scores in memory
 
 // A wave a token and key/value head, which chooses from up to COLUMNS columns.
@@ -494,7 +579,7 @@ template <typename C, int D> hipError_t launch_key_means(const KeyMeansParams<C>
 template <typename T, int D> hipError_t launch_block_select(const BlockSelectParams<T>& p_, SelectPlan plan, hipStream_t stream) {
   BlockSelectParams<T> p = p_;
   const int width = p.at.pages_per_seq, most = width - p.first - p.last;  // columns chosen from
-  if (plan.tiles && most <= kFusedColumns) {
+  if (plan.tiles && plan.slab == 0) {
     const dim3 grid((unsigned)((long)plan.slots * p.at.kv_heads));
     if (most <= 256)
       hipLaunchKernelGGL((block_select_tile_kernel<T, D, 256>), grid, dim3(kThreads), 0, stream, p);
@@ -503,6 +588,19 @@ template <typename T, int D> hipError_t launch_block_select(const BlockSelectPar
     else
       hipLaunchKernelGGL((block_select_tile_kernel<T, D, kFusedColumns>), grid, dim3(kThreads), 0, stream, p);
     return hipGetLastError();
+  }
+  if constexpr (D <= 128) {  // (select_plan)
+    if (plan.slab == 0) {
+      const dim3 grid((unsigned)p.at.total * p.at.kv_heads);
+      p.token0 = 0;
+      if (most <= 256)
+        hipLaunchKernelGGL((block_select_token_kernel<T, D, 256>), grid, dim3(kTokenThreads), 0, stream, p);
+      else if (most <= 512)
+        hipLaunchKernelGGL((block_select_token_kernel<T, D, 512>), grid, dim3(kTokenThreads), 0, stream, p);
+      else
+        hipLaunchKernelGGL((block_select_token_kernel<T, D, kFusedColumns>), grid, dim3(kTokenThreads), 0, stream, p);
+      return hipGetLastError();
+    }
   }
   for (p.token0 = 0; p.token0 < p.at.total; p.token0 += plan.slab) {
     p.tokens = p.at.total - p.token0 < plan.slab ? p.at.total - p.token0 : plan.slab;
@@ -514,8 +612,8 @@ template <typename T, int D> hipError_t launch_block_select(const BlockSelectPar
       hipLaunchKernelGGL((block_score_kernel<T, D>), dim3(rows, (width + kColumns - 1) / kColumns), dim3(kThreads), 0, stream, p);
     if (most <= 256)
       hipLaunchKernelGGL((block_choose_wave_kernel<T, 256>), dim3((rows + 3) / 4), dim3(kThreads), 0, stream, p);
-    else if (most <= 1024)
-      hipLaunchKernelGGL((block_choose_wave_kernel<T, 1024>), dim3((rows + 3) / 4), dim3(kThreads), 0, stream, p);
+    else if (most <= kFusedColumns)
+      hipLaunchKernelGGL((block_choose_wave_kernel<T, kFusedColumns>), dim3((rows + 3) / 4), dim3(kThreads), 0, stream, p);
     else
       hipLaunchKernelGGL((block_choose_kernel<T>), dim3(rows), dim3(kThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();

@@ -36,22 +36,45 @@ template <typename T, typename C> struct BlockParams {
   float scale;
 };
 
-// How choices are made: by tiles of 16 tokens of a sequence (slots of them), or token by token; and how many
-// tokens' scores are in memory at a time (none where they stay in LDS).
+// How choices are made: by tiles of 16 tokens of a sequence (slots of them), token by token in a workgroup each, or with
+// scores in memory, of how many tokens at a time (slab; 0: scores stay in LDS).
 struct SelectPlan {
   bool tiles;
   int slots, slab;
 };
 constexpr long kScoreBytes = 256l << 20;
 constexpr int kFusedColumns = 1024;
-inline SelectPlan select_plan(int batch, int total, bool single, int kv_heads, int pages_per_seq, int first, int last) {
+// Up to kFusedColumns columns: a workgroup a token and head, up to 512 of them; a tile's workgroup reads the means once for
+// 16 tokens, but chooses for them four at a time; with scores in memory every token reads the means and another launch
+// chooses. us, tiles / tokens / memory, 250 columns of D128: 1 token of 8 heads 13 / 10 / 12, 64 tokens of one sequence
+// 30 / 14 / 14, 16 sequences of 4 14 / 14 / 14, 64 of 2 24 / 25 / 20, 256 of 1 52 / 47 / 35, 64 of 4 25 / 42 / 35, 64 of 8
+// 27 / 75 / 66; 1000 columns: 41 / 23 / 20, 80 / 35 / 40, 43 / 37 / 43, 86 / 69 / 74; 1000 of D256, 2 heads, where a token's
+// workgroup would wait for 1 MB by itself: 63 / 73 / 19, 102 / 76 / 28, 66 / 81 / 39, 67 / 104 / 59.
+inline SelectPlan select_plan(int batch, int total, bool single, int kv_heads, int head_dim, int pages_per_seq, int first, int last) {
   SelectPlan p;
-  p.tiles = !single && total >= 8l * batch;
   p.slots = total / 16 + batch;
   long fit = kScoreBytes / (8l * kv_heads * pages_per_seq);
   if (fit > (1l << 22) / kv_heads) fit = (1l << 22) / kv_heads;  // (a launch's threads are 32 bits)
   p.slab = (int)(fit < 1 ? 1 : fit < total ? fit : total);
-  if (p.tiles && (long)pages_per_seq - first - last <= kFusedColumns) p.slab = 0;
+  const long columns = (long)pages_per_seq - first - last, rows = (long)total * kv_heads;
+  if (columns > kFusedColumns) {
+    p.tiles = !single && total >= 8l * batch;
+    return p;
+  }
+  p.tiles = false;
+  if (head_dim <= 128 && rows <= 512) {
+    p.slab = 0;
+    return p;
+  }
+  const double n = columns > 0 ? (double)columns : 0.;
+  const int each = total < 16l * batch ? (total + batch - 1) / batch : 16, held = n <= 256 ? 1024 : n <= 512 ? 512 : 256;
+  const double full = (double)p.slots * kv_heads / held;  // of the tiles that 256 CUs hold
+  const double tile_us = (full < 1 ? 1 : full) * (4 + n * head_dim * 1.9e-4 + (each + 3) / 4 * (2.5 + 0.0105 * n));
+  const double memory_us = 10 + rows * n * head_dim * 4 / 5.5e6;
+  if (!single && tile_us < memory_us) {
+    p.tiles = true;
+    p.slab = 0;
+  }
   return p;
 }
 

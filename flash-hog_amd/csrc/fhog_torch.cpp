@@ -646,7 +646,7 @@ at::Tensor block_select_core(const at::Tensor& q_, const at::Tensor& means, cons
   const int kv = (int)means.size(1), batch = (int)table.size(0), width = (int)table.size(1);
   at::Tensor chosen = at::empty({(int64_t)total, (int64_t)kv, blocks}, t.options());
   c10::DeviceGuard guard(q.device());
-  const size_t size = api().select_bytes(batch, total, !off, kv, width, (int)first, (int)last);
+  const size_t size = api().select_bytes(batch, total, !off, kv, (int)q.size(2), width, (int)first, (int)last);
   const at::Tensor ws = bytes_on(q, size);
   check_status(api().block_select(current_stream(q), q.data_ptr(), means.data_ptr<float>(), t.data_ptr<int>(),
                                   n.data_ptr<int>(), (const int*)data_or_null(o), chosen.data_ptr<int>(), data_or_null(ws),

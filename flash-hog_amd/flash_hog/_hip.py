@@ -66,7 +66,7 @@ SIGNATURES = {
     "fhog_paged_cache_extend": (_i, [_p] * 9 + [_i, _p, _p, ctypes.c_size_t] + [_i] * 7),
     "fhog_paged_cache_compact": (_i, [_p] * 15 + [ctypes.c_size_t] + [_i] * 8),
     "fhog_paged_key_means": (_i, [_p] * 7 + [_i] * 7),
-    "fhog_paged_block_select_workspace_bytes": (ctypes.c_size_t, [_i] * 7),
+    "fhog_paged_block_select_workspace_bytes": (ctypes.c_size_t, [_i] * 8),
     "fhog_paged_block_select": (_i, [_p] * 8 + [ctypes.c_size_t] + [_i] * 12),
     "fhog_paged_block_workspace_bytes": (ctypes.c_size_t, [_i] * 9),
     "fhog_paged_block_attention": (_i, [_p] * 12 + [ctypes.c_size_t] + [_i] * 12 + [_f]),
@@ -678,7 +678,7 @@ def paged_block_select(q, key_means, page_table, lengths, query_offsets, page_si
         raise ValueError(f"needs first >= 0, last >= 1 and first + last <= blocks, got {first}, {last} and {blocks}")
     chosen = torch.empty((T, Nk, blocks), device=q.device, dtype=torch.int32)
     with _on_device(q.device):
-        size = lib().fhog_paged_block_select_workspace_bytes(B, T, int(query_offsets is None), Nk, width, first, last)
+        size = lib().fhog_paged_block_select_workspace_bytes(B, T, int(query_offsets is None), Nk, Hd, width, first, last)
         ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
         check(lib().fhog_paged_block_select(
             _stream(q.device), _ptr(q), _ptr(key_means), _ptr(page_table), _ptr(lengths), _ptr(query_offsets), _ptr(chosen),

@@ -336,8 +336,8 @@ int fhog_paged_key_means(fhog_stream_t stream, const void* k_cache, const void* 
  * are. Tokens of no sequence, before position 0 or beyond the table: -1 throughout. Offsets that fall somewhere may
  * leave lists of any values.
  */
-size_t fhog_paged_block_select_workspace_bytes(int batch, int total, int single, int kv_heads, int pages_per_seq, int first,
-                                               int last);
+size_t fhog_paged_block_select_workspace_bytes(int batch, int total, int single, int kv_heads, int head_dim,
+                                               int pages_per_seq, int first, int last);
 int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* key_means, const int* page_table,
                             const int* lengths, const int* query_offsets, int* chosen, void* workspace,
                             size_t workspace_bytes, int batch, int total, int heads, int kv_heads, int head_dim,

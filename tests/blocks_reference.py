@@ -45,6 +45,40 @@ def select(q, means, table, lengths, new, page, blocks, first, last):
     return out
 
 
+def select_dense(q, means, table, lengths, new, page, blocks, first, last):
+    """select() for many tokens: a sequence's scores at once."""
+    T, H, D = q.shape
+    pages, N, _ = means.shape
+    width = table.shape[1]
+    out = torch.full((T, N, blocks), -1, dtype=torch.int32)
+    sums = q.double().view(T, N, H // N, D).sum(2)
+    at = torch.arange(width)
+    row = 0
+    for b, (count, length) in enumerate(zip(new, lengths)):
+        bad = (table[b] < 0) | (table[b] >= pages)
+        m = means[torch.where(bad, 0, table[b]).long()].double()
+        own = torch.div(torch.arange(length - count, length), page, rounding_mode="floor")[:, None]
+        inside = (own >= 0) & (own < width)
+        lo = own.clamp(max=first - 1) + 1
+        hi = torch.maximum(lo, own + 1 - last)
+        room = (blocks - (own + 1 - (hi - lo))).clamp(min=0)
+        for n in range(N):
+            scores = sums[row:row + count, n] @ m[:, n].T
+            none = bad | torch.isnan(scores)
+            scores = torch.where(none, -torch.inf, scores)
+            rank = torch.where((at < lo) | (at >= hi), 2, none.long())
+            scores, order = torch.sort(scores, dim=1, descending=True, stable=True)
+            rank, again = torch.sort(rank.gather(1, order), dim=1, stable=True)
+            order = order.gather(1, again)
+            taken = torch.zeros((count, width), dtype=torch.bool).scatter_(1, order, (rank < 2) & (at < room))
+            taken |= ((at < lo) | (at >= hi)) & (at <= own)
+            columns = torch.where(taken & inside, at, width).sort(1).values[:, :blocks]
+            columns = torch.where(columns == width, -1, columns).to(torch.int32)
+            out[row:row + count, n, :columns.shape[1]] = columns
+        row += count
+    return out
+
+
 def attention(q, cache, new, chosen, scale):
     q = q.double()
     out = torch.zeros_like(q)

@@ -56,8 +56,8 @@ def test_means_refusals(lib, kwargs, status, needle):
 
 @pytest.mark.parametrize("kwargs,status,needle", SIZES + TOKENS + [
     (dict(first=-1), 1, "first >= 0"), (dict(last=0), 1, "last >= 1"), (dict(first=3, last=2), 1, "first + last <= blocks"),
-    (dict(first=(1 << 31) - 1, last=2), 1, "first + last <= blocks"), (dict(ws=None), 1, "workspace is null"),
-    (dict(size=100), 1, "below its"), (dict(ws=4), 1, "8-byte aligned"), (dict(means=8), 1, "not 16-byte aligned"),
+    (dict(first=(1 << 31) - 1, last=2), 1, "first + last <= blocks"), (dict(ws=None, width=2000), 1, "workspace is null"),
+    (dict(size=100, width=2000), 1, "below its"), (dict(ws=4, width=2000), 1, "8-byte aligned"), (dict(means=8), 1, "not 16-byte aligned"),
     (dict(width=(1 << 21) + 1), 1, "problem too large")])
 def test_select_refusals(lib, kwargs, status, needle):
     assert lib.fhog_paged_block_select(*select_args(**kwargs)) == status
@@ -80,15 +80,17 @@ def test_nothing_to_do(lib):
 
 
 def test_workspace_bytes(lib):
-    """Scores of the tokens of a slab: all of them, or as many as 256 MiB hold; at least one. None where
-    tiles of tokens keep them in LDS."""
+    """Scores of the tokens of a slab: all of them, or as many as 256 MiB hold; at least one. None where LDS holds
+    them."""
     scores = lambda *sizes: lib.fhog_paged_block_select_workspace_bytes(*sizes, 1, 1)
-    assert scores(10, 10, 1, 4, 100) == 10 * 4 * 100 * 8
-    assert scores(1, 7, 0, 4, 100) == 7 * 4 * 100 * 8
-    assert scores(1, 8, 0, 4, 1026) == 0 and scores(1, 8, 0, 4, 1027) == 8 * 4 * 1027 * 8
-    assert scores(1, 1 << 20, 0, 8, 2048) == 1 << 28
-    assert scores(5, 5, 1, 64, 1 << 21) == 64 * 8 << 21
-    assert scores(0, 0, 1, 4, 100) == 0
+    assert scores(10, 10, 1, 4, 64, 2000) == 10 * 4 * 2000 * 8
+    assert scores(1, 7, 0, 4, 64, 2000) == 7 * 4 * 2000 * 8
+    assert scores(10, 10, 1, 4, 128, 1026) == 0 and scores(10, 10, 1, 4, 256, 1026) == 10 * 4 * 1026 * 8  # a workgroup a token
+    assert scores(512, 512, 1, 1, 64, 100) == 0 and scores(513, 513, 1, 1, 64, 100) == 513 * 100 * 8
+    assert scores(1, 1000, 0, 4, 256, 1026) == 0 and scores(1, 1000, 0, 4, 256, 1027) == 1000 * 4 * 1027 * 8  # tiles
+    assert scores(1, 1 << 20, 0, 8, 64, 2048) == 1 << 28
+    assert scores(5, 5, 1, 64, 64, 1 << 21) == 64 * 8 << 21
+    assert scores(0, 0, 1, 4, 64, 100) == 0
     assert lib.fhog_paged_block_workspace_bytes(1, 1, 1, 4, 2, 64, 16, 5, 1) == 0
     assert lib.fhog_paged_block_workspace_bytes(1, 1, 1, 4, 2, 64, 15, 5, 1) == 0
     few, many = (lib.fhog_paged_block_workspace_bytes(t, t, 1, 32, 8, 128, 64, 500, 64) for t in (1, 4096))

@@ -157,26 +157,58 @@ def test_many_blocks(blocks, page, length, cuda_device):
 
 
 def choose(means, q, page, blocks, length, device, first=0, last=1, table=None, tiles=False):
-    """The lists of one token; tiles: as the last of sixteen."""
+    """The lists of one token; tiles: as the last of so many that sixteen share a workgroup."""
     import flash_hog
 
     pages = means.shape[0]
     table = torch.arange(pages, dtype=torch.int32)[None] if table is None else table
     if tiles:
-        offsets = torch.tensor([0, 16], dtype=torch.int32, device=device)
-        return flash_hog.paged_block_select(q.expand(16, -1, -1).to(device), means.to(device), table.to(device),
+        offsets = torch.tensor([0, 4096], dtype=torch.int32, device=device)
+        return flash_hog.paged_block_select(q.to(device).expand(4096, -1, -1), means.to(device), table.to(device),
                                             torch.tensor([length], dtype=torch.int32, device=device), offsets,
-                                            page_size=page, blocks=blocks, first=first, last=last).cpu()[15]
+                                            page_size=page, blocks=blocks, first=first, last=last)[-1].cpu()
     return flash_hog.paged_block_select(q.to(device), means.to(device), table.to(device),
                                         torch.tensor([length], dtype=torch.int32, device=device), page_size=page,
                                         blocks=blocks, first=first, last=last).cpu()[0]
 
 
+@pytest.mark.parametrize("head_dim,dtype", [(64, BF16), (128, FP16), (256, BF16)])
+@pytest.mark.parametrize("width", [None, 300, 514, 1027, 1028])
+def test_select_many(width, head_dim, dtype, cuda_device):
+    """So many tokens that sixteen share a workgroup; sequences of one token, so many that scores go through memory."""
+    import flash_hog
+
+    print("[case] select many", head_dim, width, flush=True)
+    gen = torch.Generator().manual_seed(6)
+    for lengths, new in (([3000, 700, 16, 2049], [1000, 400, 16, 700]), (torch.randint(0, 3000, (300,), generator=gen).tolist(), None)):
+        counts = new or [1] * len(lengths)
+        pages, batch, T, cols = 500, len(lengths), sum(counts), width or -(-max(lengths) // 16)
+        means = torch.randn((pages, 4, head_dim), generator=gen)
+        q = torch.randn((T, 8, head_dim), generator=gen).to(dtype)
+        # (random pages: one twice in a row ties)
+        table = torch.randint(-2, pages + 2, (batch, cols), generator=gen).to(torch.int32)
+        offsets = torch.zeros(batch + 1, dtype=torch.int32)
+        offsets[1:] = torch.tensor(counts).cumsum(0)
+        for blocks, first, last in ((20, 2, 1), (3, 1, 2), (260, 0, 3)):
+            got = flash_hog.paged_block_select(
+                q.to(cuda_device), means.to(cuda_device), table.to(cuda_device), torch.tensor(lengths, dtype=torch.int32, device=cuda_device),
+                None if new is None else offsets.to(cuda_device), page_size=16, blocks=blocks, first=first, last=last)
+            assert torch.equal(got.cpu(), ref.select_dense(q, means, table, lengths, counts, 16, blocks, first, last)), (blocks, new is None)
+
+
+@pytest.mark.parametrize("case", [CASES[i] for i in (0, 1, 3, 8, 12, 18)], ids=case_id)
+def test_select_oracles_agree(case, cuda_device):
+    cache, counts, q, *_ = make(case, "cpu")
+    blocks, first, last = case[8:]
+    args = (q, all_means(cache), cache.table, cache.lengths, counts, cache.page, blocks, first, last)
+    assert torch.equal(ref.select(*args), ref.select_dense(*args))
+
+
 @pytest.mark.parametrize("width", [None, 300, 514, 1027, 1028, 3000])
 @pytest.mark.parametrize("new", [[1, 40, 16, 5], [130, 1, 0, 33], [2, 9, 1, 3]], ids=str)
 def test_select_tiles_and_tokens(new, width, cuda_device):
-    """Sequences with many and with few new tokens, and tables as wide as the rules tell apart: tiles of 16 tokens
-    that end anywhere, scores in LDS and in memory."""
+    """Sequences with many and with few new tokens, and tables as wide as the rules tell apart: scores in LDS, and in
+    memory with tiles of 16 tokens that end anywhere."""
     import flash_hog
 
     lengths = [3000, 700, 16, 2049]
