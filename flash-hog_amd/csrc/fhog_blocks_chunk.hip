@@ -7,11 +7,10 @@
 // list gives it, and a last kernel joins a row's outputs in the order of its list: no atomics on numbers, the
 // same bits at every call.
 //
-// What bounds it: those outputs, written and read once, 8 (head_dim + 2) bytes for each row and block, in slabs that fit
-// the 256 MB behind the L2s. 2035 tokens in 4 sequences, H32/8 D128 bf16, 16 blocks of 64, us for each slab of
-// 250 MB: masks 6, items 6, entries 6, tiles 91 (without their stores 57), sum 50 (5.0 TB/s). 4096 tokens, H12/12 D64 e4m3, 16
-// blocks: 9, 9, 10, 58, 52. (A token at a time 583 and 744 in all; slabs of 64 / 128 / 256 / 1024 MB 422 / 316 / 333 / 346 us
-// for tiles and sums, and half the launches with 256.)
+// What bounds it: those outputs, written and read once, 8 (head_dim + 2) bytes for each row and block. 2035 tokens in 4
+// sequences, H32/8 D128 bf16, 16 blocks of 64, 540 MB of outputs, us: masks 6, items 8, entries 8, tiles 192, sum 141 (3.8 TB/s).
+// 4096 tokens, H12/12 D64 e4m3, 16 blocks, 207 MB: 9, 9, 10, 61, 51. (250 MB at D = 128: tiles 91, without their stores 57,
+// and sum 50, 5.0 TB/s. A token at a time 583 and 744 in all.)
 //
 //   block_masks_kernel   64 tokens and a key/value head: which of them chose each column
 //   block_items_kernel   tokens of each sequence, head and column: how many, in tiles of 128 rows

@@ -443,7 +443,7 @@ def test_many_tokens_in_slabs(cuda_device):
     import flash_hog
 
     print("[case] many tokens in slabs", flush=True)
-    case = (8, 4, 64, BF16, False, 64, [5000, 3000], [3001, 2900], 24)  # 48 KiB a token and 256 MiB a slab
+    case = (8, 4, 64, BF16, False, 64, [6000, 5000], [5001, 4900], 64)  # 132 KiB a token and 1 GiB a slab
     cache, counts, q, moved, where = make(case, cuda_device)
     kv = moved["key_cache"], moved["value_cache"]
     q = q.to(cuda_device)
