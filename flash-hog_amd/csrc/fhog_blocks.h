@@ -150,9 +150,10 @@ template <typename T, typename C> struct BlockChunkParams {
   float* parts;      // (tokens, kv_heads, blocks, group, head_dim)
   float* parts_ml;   // and their maxima and sums
 };
-// Tokens are taken in slabs whose outputs stay within this. (540 MB of them in slabs of 256 / 512 / 1024 MB: 415 / 429 / 394 us.
-// Smaller ones stay in the 256 MB cache, but each has five launches, and ends with CUs idle.)
-constexpr long kPartBytes = 1l << 30;
+// Tokens are taken in slabs whose outputs stay within this (540 MB of them in slabs of 256 / 512 / 1024 MB: 415 / 429 /
+// 394 us; each slab has five launches, and ends with CUs idle). Where they would not stay in the cache behind the L2s, they
+// are stored past it: tiles / sum of 540 MB 189 / 105 us in it, 134 / 107 past it; of 207 MB 60 / 51 and 59 / 59.
+constexpr long kPartBytes = 1l << 30, kCacheBytes = 256l << 20;
 struct BlockChunkPlan {
   int slab;
   long lists, masks, groups, entries, items, parts;  // elements

@@ -8,9 +8,9 @@
 // same bits at every call.
 //
 // What bounds it: those outputs, written and read once, 8 (head_dim + 2) bytes for each row and block. 2035 tokens in 4
-// sequences, H32/8 D128 bf16, 16 blocks of 64, 540 MB of outputs, us: masks 6, items 8, entries 8, tiles 192, sum 141 (3.8 TB/s).
-// 4096 tokens, H12/12 D64 e4m3, 16 blocks, 207 MB: 9, 9, 10, 61, 51. (250 MB at D = 128: tiles 91, without their stores 57,
-// and sum 50, 5.0 TB/s. A token at a time 583 and 744 in all.)
+// sequences, H32/8 D128 bf16, 16 blocks of 64, 540 MB of outputs, us: masks 6, items 8, entries 8, tiles 133, sum 108 (5.0 TB/s).
+// 4096 tokens, H12/12 D64 e4m3, 16 blocks, 207 MB: 9, 9, 10, 60, 51. (250 MB at D = 128: tiles 91, without their stores 57.
+// A token at a time 583 and 744 in all.)
 //
 //   block_masks_kernel   64 tokens and a key/value head: which of them chose each column
 //   block_items_kernel   tokens of each sequence, head and column: how many, in tiles of 128 rows
@@ -183,7 +183,8 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
 }
 
 // Up to 128 rows of tokens that chose one column, 32 a wave; row r of a tile is its token r / group, head r % group.
-template <typename T, typename C, int D>
+// kPast: the outputs are stored past the caches (kCacheBytes; in a branch of one kernel the stores would become one).
+template <typename T, typename C, int D, bool kPast>
 __global__ void __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : D == 128 ? 3 : 4)))
 block_tile_kernel(BlockChunkParams<T, C> p) {
@@ -332,9 +333,14 @@ block_tile_kernel(BlockChunkParams<T, C> p) {
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (8 * i + (lane >> 3) < mine)
-        *reinterpret_cast<f32x4*>(p.parts + to[i] + 32 * dt) =
-            *reinterpret_cast<const f32x4*>(turn + (8 * i + (lane >> 3)) * 36 + 4 * (lane & 7));
+      if (8 * i + (lane >> 3) < mine) {
+        f32x4* const at = reinterpret_cast<f32x4*>(p.parts + to[i] + 32 * dt);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(turn + (8 * i + (lane >> 3)) * 36 + 4 * (lane & 7));
+        if constexpr (kPast)
+          __builtin_nontemporal_store(x, at);
+        else
+          *at = x;
+      }
   }
 }
 
@@ -409,7 +415,7 @@ template <typename T, typename C, int D> __global__ void __launch_bounds__(kThre
   const float* const from = p.parts + place(row) * D + column;
   const long apart = (long)group * D;
 #pragma unroll 8
-  for (int i = 0; i < count; ++i) o += s_w[r][i] * *reinterpret_cast<const f32x4*>(from + s_from[r][i] * apart);
+  for (int i = 0; i < count; ++i) o += s_w[r][i] * __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(from + s_from[r][i] * apart));
   if (count == -1) o = f32x4{NAN, NAN, NAN, NAN};
   *reinterpret_cast<V4<T>*>(p.out + ((long)p.token0 * p.heads + row) * D + column) = cvt4<T>(o);
 }
@@ -426,8 +432,11 @@ hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p_, int slab, hipStr
     hipLaunchKernelGGL((block_masks_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_items_kernel<T, C>), dim3((p.lists + 63) / 64), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((block_entries_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((block_tile_kernel<T, C, D>), dim3((unsigned)((most + 7) / 8 * 8)), dim3(kThreads), 0,
-                       stream, p);
+    const dim3 tiles((unsigned)((most + 7) / 8 * 8));
+    if ((long)p.tokens * p.heads * p.blocks * D * 4 > kCacheBytes)
+      hipLaunchKernelGGL((block_tile_kernel<T, C, D, true>), tiles, dim3(kThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((block_tile_kernel<T, C, D, false>), tiles, dim3(kThreads), 0, stream, p);
     constexpr long R = kThreads / (D / 4);
     hipLaunchKernelGGL((block_sum_kernel<T, C, D>), dim3((unsigned)(((long)p.tokens * p.heads + R - 1) / R)), dim3(kThreads), 0,
                        stream, p);

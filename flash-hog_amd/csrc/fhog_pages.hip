@@ -195,10 +195,16 @@ hipError_t bookkeeping(const PagesParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// `bytes` bytes (a multiple of 16, both ends aligned to it) by the workgroup; null source: zeros.
-__device__ __forceinline__ void copy_bytes(char* to, const char* from, int bytes) {
-  for (int i = 16 * (int)threadIdx.x; i < bytes; i += 16 * 256)
-    *reinterpret_cast<u32x4*>(to + i) = from ? *reinterpret_cast<const u32x4*>(from + i) : u32x4{0, 0, 0, 0};
+// `bytes` bytes (a multiple of 16, both ends aligned to it) by the workgroup; null source: zeros. kPast: stored past the
+// caches, for copies larger than these (460 MB 82 us, in them 106).
+template <bool kPast> __device__ __forceinline__ void copy_bytes(char* to, const char* from, int bytes) {
+  for (int i = 16 * (int)threadIdx.x; i < bytes; i += 16 * 256) {
+    const u32x4 x = from ? *reinterpret_cast<const u32x4*>(from + i) : u32x4{0, 0, 0, 0};
+    if constexpr (kPast)
+      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to + i));
+    else
+      *reinterpret_cast<u32x4*>(to + i) = x;
+  }
 }
 
 // A workgroup a row and key/value head, whose rows of a shared page it copies if there are any; the
@@ -233,7 +239,7 @@ __global__ void __launch_bounds__(256) pages_extend_kernel(PagesParams p, PageBy
     char* to = cache.at[i] + ((long)target * p.kv_heads + hk) * cache.row[i];
     const char* from = cache.at[i] + ((long)source * p.kv_heads + hk) * cache.row[i];
     if (i < 2)
-      copy_bytes(to, from, rows * cache.token[i]);
+      copy_bytes<false>(to, from, rows * cache.token[i]);
     else  // a byte a token
       for (int r = threadIdx.x; r < rows; r += 256) to[r] = from[r];
   }
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(256) pages_compact_kernel(PagesParams p, PageB
     const long piece = (size / 16 + pieces - 1) / pieces * 16;
     const long at = piece * blockIdx.y, left = size - at;
     if (left > 0)
-      copy_bytes(out.at[i] + page * size + at, from < 0 ? nullptr : cache.at[i] + from * size + at,
+      copy_bytes<true>(out.at[i] + page * size + at, from < 0 ? nullptr : cache.at[i] + from * size + at,
                  (int)(left < piece ? left : piece));
   }
 }
