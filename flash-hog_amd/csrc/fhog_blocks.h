@@ -190,8 +190,8 @@ template <typename T, typename C> void block_chunk_workspace(BlockChunkParams<T,
 // and head (an entry) costs a token's kernel its keys and values out of a cache, at 14 TB/s with 16-bit elements; a block at
 // a time costs it fp32 outputs written and read, at 3.8 TB/s both ways, and each listed block its keys and values once. Five
 // more launches are 16 us. (us a block / a token at a time, table of 8192 positions, bf16: H32/8 D128, 16 blocks of 64, one
-// sequence of 8 / 32 / 128 / 512 / 2048 tokens 24 / 12, 30 / 17, 41 / 42, 79 / 140, 330 / 543; 16 sequences of 2 / 8 / 32 tokens
-// 47 / 20, 57 / 43, 95 / 143. One of 2048 tokens: H8/8 83 / 500, H32/4 321 / 306, H8/1 D256 195 / 172, blocks of 32 305 / 353;
+// sequence of 8 / 32 / 128 / 512 / 2048 tokens 24 / 12, 30 / 17, 45 / 42, 79 / 145, 250 / 543; 16 sequences of 2 / 8 / 32 tokens
+// 47 / 20, 57 / 43, 92 / 145. One of 2048 tokens: H8/8 83 / 500, H32/4 256 / 306, H8/1 D256 195 / 172, blocks of 32 246 / 353;
 // of 512, 32 blocks of 16 166 / 91. e4m3 takes a token's kernel 8 to 25 % less; the sides change where they are as near.)
 inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int head_dim, int page_size, int pages_per_seq,
                              int blocks, bool single) {
