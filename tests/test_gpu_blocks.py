@@ -352,6 +352,9 @@ MANY = [
     (8, 2, 128, BF16, True, 64, [1200] * 5, [130, 64, 63, 1, 1200], 16),
     (32, 1, 64, BF16, False, 1024, [5000], [700], 4),             # 4 tokens a tile
     (5, 5, 128, BF16, False, 64, [8000], [300], 70),
+    # a token at a time again: more blocks than a join's weights, more heads a group than a tile's rows
+    (4, 2, 64, FP16, False, 16, [9000], [200], 300),
+    (130, 1, 64, BF16, False, 256, [2000, 700], [500, 30], 3),
 ]
 
 
@@ -362,7 +365,7 @@ def many_lists(case, cache, counts, kind):
     if kind == "any":
         lists = torch.randint(-1, width + 2, (T, N, blocks), generator=gen).to(torch.int32)
         lists[::3, 0] = -1
-        lists[1::4, :, 3] = 2 ** 31 - 1
+        lists[1::4, :, min(3, blocks - 1)] = 2 ** 31 - 1
         lists[2::4, :, 2] = -2 ** 31
         return lists
     at = torch.cat([torch.arange(n - c, n) for n, c in zip(cache.lengths, counts)])
@@ -436,6 +439,69 @@ def test_many_tokens_of_no_sequence(cuda_device):
         choice = flash_hog.paged_block_select(padded, all_means(cache).to(cuda_device), **more, page_size=64, blocks=13)
         out = flash_hog.paged_block_attention(padded, choice, *kv, **more)
         assert torch.isnan(out).all() if offsets[0] != -7 else torch.isfinite(out).all()
+
+
+def test_many_tokens_wide_table(cuda_device):
+    """A table wider than a workgroup's masks, and one just as wide."""
+    import flash_hog
+
+    print("[case] many tokens, wide table", flush=True)
+    case = MANY[4]
+    for width in (None, 8192, 8193):
+        cache, counts, q, moved, where = make(case, cuda_device, width=width)
+        lists = many_lists((*case[:8], 7), cache, counts, "chosen")
+        out = flash_hog.paged_block_attention(q.to(cuda_device), lists.to(cuda_device), moved["key_cache"], moved["value_cache"], **where)
+        check(out, ref.attention_dense(q, cache, counts, lists, 128 ** -0.5))
+
+
+def test_strided_inputs(cuda_device):
+    """Views: queries of a joint projection, lists and tables that are parts of wider ones."""
+    import flash_hog
+
+    for case in (CASES[8], CASES[13], (*MANY[0], 1, 1)):
+        print("[case] strided", case_id(case), flush=True)
+        cache, counts, q, moved, where = make(case, cuda_device)
+        lists = many_lists(case, cache, counts, "chosen").to(cuda_device)
+        q, means = q.to(cuda_device), all_means(cache).to(cuda_device)
+        kv = moved["key_cache"], moved["value_cache"]
+        wide = lambda t, axis: torch.cat([t, t.flip(0)], axis).narrow(axis, 0, t.shape[axis])
+        strange = {**where, "page_table": wide(where["page_table"], 1), "lengths": torch.stack([where["lengths"]] * 2, 1)[:, 0]}
+        if where["query_offsets"] is not None:
+            strange["query_offsets"] = torch.stack([where["query_offsets"]] * 3, 1)[:, 1]
+        assert not strange["page_table"].is_contiguous() or cache.table.shape[0] == 1
+        out = flash_hog.paged_block_attention(q, lists, *kv, **where, **scales(moved))
+        got = flash_hog.paged_block_attention(wide(q, 1), wide(lists, 2), *kv, **strange, **scales(moved))
+        assert torch.equal(out, got)
+        choice = [flash_hog.paged_block_select(x, means, **w, page_size=cache.page, blocks=4) for x, w in ((q, where), (wide(q, 2), strange))]
+        assert torch.equal(*choice)
+
+
+def test_two_streams(cuda_device):
+    """Calls of two streams at once, each with workspaces of its own."""
+    import flash_hog
+
+    print("[case] two streams", flush=True)
+    calls = []
+    for case, kind in ((MANY[1], "chosen"), (MANY[7], "any"), (CASES[3], None)):
+        cache, counts, q, moved, where = make(case, cuda_device)
+        lists = many_lists(case, cache, counts, kind) if kind else ref.select(q, all_means(cache), cache.table, cache.lengths, counts, cache.page, *case[8:])
+        q, lists, means = q.to(cuda_device), lists.to(cuda_device), all_means(cache).to(cuda_device)
+
+        def call(q=q, lists=lists, means=means, moved=moved, where=where, page=cache.page):
+            return (flash_hog.paged_block_attention(q, lists, moved["key_cache"], moved["value_cache"], **where, **scales(moved)),
+                    flash_hog.paged_block_select(q, means, **where, page_size=page, blocks=5))
+        calls.append(call)
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    runs = []
+    for _ in range(10):
+        for stream, call in zip(streams, calls):
+            with torch.cuda.stream(stream):
+                runs.append(call())
+    torch.cuda.synchronize()
+    for i, run in enumerate(runs):
+        assert all(torch.equal(a, b) for a, b in zip(run, want[i % len(calls)]))
 
 
 def test_many_tokens_in_slabs(cuda_device):

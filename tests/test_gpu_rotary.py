@@ -337,6 +337,42 @@ def test_through_attention(cuda_device):
         assert float((a.double().cpu() - b).abs().max()) <= 4e-5 * float(b.abs().max())
 
 
+@pytest.mark.parametrize("extension", [True, False])
+@pytest.mark.parametrize("norm", [True, False])
+def test_parts_of_a_graph(norm, extension, cuda_device, monkeypatch):
+    """One result used, one leaf asked for, one gradient differentiated: as with zeros in the other places."""
+    import flash_hog
+    from flash_hog import _hip
+
+    if not extension:
+        monkeypatch.setattr(_hip, "torch_ext", lambda: None)
+    gen = torch.Generator().manual_seed(3)
+    rand = lambda *shape: torch.randn(shape, generator=gen).to(cuda_device)
+    q, k, wq, wk = rand(2, 9, 4, 64), rand(2, 9, 2, 64), rand(64), rand(64)
+    cq, ck, freq = rand(2, 9, 4, 64), rand(2, 9, 2, 64), frequencies(64, cuda_device)
+    leaves = [t.requires_grad_() for t in ((q, k, wq, wk) if norm else (q, k))]
+    weights = dict(query_weight=wq, key_weight=wk) if norm else dict(eps=None)
+    call = lambda q=q, k=k: flash_hog.qk_norm_rotary(q, k, frequencies=freq, **weights)
+    full = torch.autograd.grad(call(), leaves, (cq, torch.zeros_like(ck)))
+    part = torch.autograd.grad(call()[0], leaves, cq, allow_unused=True)
+    for a, b in zip(full, part):
+        assert torch.equal(a, b) if b is not None else not a.any()
+    both = torch.autograd.grad(call(), leaves, (cq, ck))
+    for leaf, want in zip(leaves, both):
+        assert torch.equal(torch.autograd.grad(call(), leaf, (cq, ck))[0], want)
+    # q alone needs a gradient; k is a leaf that needs none
+    assert torch.equal(torch.autograd.grad(call(k=k.detach()), q, (cq, ck))[0], both[0])
+    for i, leaf in enumerate(leaves):
+        c = [cq.clone().requires_grad_(), ck.clone().requires_grad_()]
+        wanted = (*leaves, *c) if norm else c
+        tangent = rand(*leaf.shape)
+        grads = torch.autograd.grad(call(), leaves, c, create_graph=True)
+        one = torch.autograd.grad(grads[i], wanted, tangent, allow_unused=True, retain_graph=True)
+        zeros = [tangent if j == i else torch.zeros_like(g) for j, g in enumerate(grads)]
+        for a, b in zip(torch.autograd.grad(grads, wanted, zeros), one):
+            assert torch.equal(a, b) if b is not None else not a.any()
+
+
 def test_transforms(cuda_device):
     """torch.func.grad, vmap (also of weights), and jvp, which is refused."""
     import flash_hog
