@@ -93,10 +93,12 @@ inline BlockPlan block_plan(int total, int heads, int kv_heads, int head_dim, in
   // Few long splits: a workgroup's start, four dependent loads, is as long as its walk over 500 keys. (Eight / four / two /
   // one a CU, us, without the join, which one split does without: B16 x 64 blocks of 64, H32/8 D128 e4m3 38 / 30 / 26 / 27,
   // B32 x 32 of 32 bf16 34 / 28 / 25 / 25, B64 x 64 of 16, H16/4 D64 18 / 18 / 15 / 15, B8 x 32 of 64 e4m3 17 / 17 / 13 / 12.)
-  const long work = (long)p.slots * kv_heads, target = cus;
-  long splits = work >= target ? 1 : (target + work - 1) / work;
-  const long least = work < 2l * cus ? waves : 4l * waves;
-  if (splits > tiles / least) splits = tiles / least;
+  const long work = (long)p.slots * kv_heads;
+  long splits = work >= cus ? 1 : (cus + work - 1) / work;
+  if (splits > tiles / waves) splits = tiles / waves;
+  // (the join costs 3 us: up to four tiles a wave go without. B1 x 32 of 16, H16/4 D64 7.0, in two splits 9.2; B16 x 32 of 32,
+  // H12/12 D64 12.4, in two 16.5; B1 x 16 of 64, H32/8 D128, eight tiles a wave, 9.8 in eight splits, in two 13.6)
+  if (tiles <= 4l * waves) splits = 1;
   if (splits > kJoinWeights / 16) splits = kJoinWeights / 16;
   const long needed = (tiles * 32 + (long)(kSplitBlocks - 1) * page_size - 1) / ((long)(kSplitBlocks - 1) * page_size);
   if (splits < needed) splits = needed;

@@ -34,9 +34,13 @@ struct PagesParams {
 };
 
 constexpr int kPageChunk = 4096;
-// Up to this many pages and entries one workgroup does the bookkeeping, with the pages' states in LDS: six
-// launches become two. (128 rows of 34 entries, 556 pages.)
-constexpr int kFewPages = 32768, kFewEntries = 1 << 17, kFewRows = 1 << 14;
+// Up to this many pages, entries and rows one workgroup does the bookkeeping, with the pages' states in LDS: six launches
+// become two.
+constexpr int kFewPages = 32768, kFewEntries = 1 << 17, kFewRows = 1024;
+// And one, if the copies are no more than this at most, a wave a row and head. (us, two launches / one, without / with a copy a
+// row: 1 row of 4 heads of 64, pages of 16 5.0 / 3.9, 4 5.6 / 4.3 and 6.0 / 4.9, 8, 128 KB 5.8 / 4.9 and 6.0 / 6.3, 16 6.2 / 6.5
+// and 6.5 / 9.2; 2 of 8 heads of 128, pages of 64, 512 KB 5.8 / 4.0 and 6.3 / 7.0, 4 5.7 / 4.6 and 6.1 / 11.6.)
+constexpr long kFewBytes = 128l << 10, kFewHeads = 32;
 inline bool few_pages(int batch, int width, int pages) {
   return pages <= kFewPages && (long)batch * width <= kFewEntries && batch <= kFewRows;
 }

@@ -10,7 +10,8 @@
 // New pages are the free ones, lowest first, to the rows in their order, each row's columns in theirs:
 // sums over rows and pages give every row its place, whatever order the atomics ran in.
 //
-// The bookkeeping is bound by latency (a few dependent round trips), the copies by memory.
+// The bookkeeping is bound by latency, four dependent round trips: 5.8 us for 128 rows of 34 entries, of which the launch is
+// two. The copies are bound by memory.
 #include "fhog_pages.h"
 
 namespace fhog {
@@ -20,10 +21,11 @@ namespace {
 constexpr int kFree = 0x7fffffff, kRead = -1;  // PageState: else the lowest row that grows in the page
 
 struct PageRow {
-  int from;         // the parent, or -1: an empty row
-  long held, more;  // tokens held and new
-  int used;         // entries in use, of the table's
-  bool grows;       // within its last page
+  int from = -1;             // the parent, or -1: an empty row
+  long held = 0, more = 0;  // tokens held and new
+  int used = 0;             // entries in use, of the table's
+  bool grows = false;       // within its last page
+  __device__ PageRow() = default;
   __device__ __forceinline__ PageRow(const PagesParams& p, int b) {
     from = p.parents ? p.parents[b] : b;
     if ((unsigned)from >= (unsigned)p.batch) from = -1;
@@ -38,31 +40,27 @@ struct PageRow {
   }
 };
 
-// Entry i of all rows: kept for later with parents, and what it says about its page.
-template <typename State> __device__ __forceinline__ void mark_entry(const PagesParams& p, State* state, long i) {
-  const int b = (int)(i / p.width), c = (int)(i - (long)b * p.width);
-  const PageRow row(p, b);
-  if (c >= row.used) return;
+// Entry c of row b, from what is known of it: kept for later with parents, and what it says about its page.
+template <typename State, typename Row>
+__device__ __forceinline__ int mark_entry(const PagesParams& p, State* state, int b, int c, const Row& row) {
   const int page = p.table[(long)row.from * p.width + c];
-  if (p.parents) p.entries[i] = page;
+  if (p.parents) p.entries[(long)b * p.width + c] = page;
   if ((unsigned)page < (unsigned)p.pages) atomicMin(&state[page], row.grows && c == row.used - 1 ? b : kRead);
+  return page;
 }
 
-// What row b asks for: how many pages; notes which column is the first and which page it copies.
-__device__ __forceinline__ int ask(const PagesParams& p, const int* state, int b) {
-  const PageRow row(p, b);
-  int begin = row.used, source = -1;
-  if (row.grows) {
-    const int page = p.table[(long)row.from * p.width + row.used - 1];
-    if ((unsigned)page < (unsigned)p.pages && state[page] != b) {
-      source = page;
-      --begin;
-    }
-  }
+// What row b, whose last page is `last`, asks for: how many pages; notes which column is the first and which page it copies.
+template <typename State> __device__ __forceinline__ int ask(const PagesParams& p, const State* state, int b, const PageRow& row, int last) {
+  const bool copies = row.grows && (unsigned)last < (unsigned)p.pages && state[last] != b;
+  const int begin = row.used - copies;
   p.held[b] = (int)row.held;
   p.begin[b] = begin;
-  p.source[b] = source;
+  p.source[b] = copies ? last : -1;
   return max(0, row.end(p) - begin);
+}
+__device__ __forceinline__ int ask(const PagesParams& p, int b) {
+  const PageRow row(p, b);
+  return ask(p, p.state, b, row, row.grows ? p.table[(long)row.from * p.width + row.used - 1] : -1);
 }
 
 __device__ __forceinline__ bool is_listed(const PagesParams& p, int state) { return (state == kFree) != (p.list_used != 0); }
@@ -91,23 +89,84 @@ __device__ __forceinline__ int count_pages(const PagesParams& p, const State* st
   return sum;
 }
 
-// All of the bookkeeping in one workgroup.
-__global__ void __launch_bounds__(1024) pages_few_kernel(PagesParams p) {
+// `bytes` bytes (a multiple of 16, both ends aligned to it) by kThreads threads; null source: zeros. kPast: stored past the
+// caches, for copies larger than these (230 MB of e4m3 pages 82 us where they went to them in 106; after other work, with the
+// bookkeeping, 116 and 121).
+template <bool kPast, int kThreads> __device__ __forceinline__ void copy_bytes(char* to, const char* from, int bytes, int thread) {
+  for (int i = 16 * thread; i < bytes; i += 16 * kThreads) {
+    const u32x4 x = from ? *reinterpret_cast<const u32x4*>(from + i) : u32x4{0, 0, 0, 0};
+    if constexpr (kPast)
+      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to + i));
+    else
+      *reinterpret_cast<u32x4*>(to + i) = x;
+  }
+}
+
+// After the bookkeeping, by kThreads threads: row b's entries and length, by the first key/value head's, and this head's
+// rows of a shared page, if it copies one.
+template <int kThreads>
+__device__ __forceinline__ void extend_row(const PagesParams& p, const PageBytes& cache, int* free_pages, int b, int hk, int thread) {
+  const int begin = p.begin[b], first = p.first[b], source = p.source[b], listed = p.totals[0];
+  const long held = p.held[b];
+  if (hk == 0) {
+    const long more = max(0, p.new_tokens ? p.new_tokens[b] : p.new_each);
+    const long pages = (held + more + (1l << p.page_shift) - 1) >> p.page_shift;
+    const int end = (int)min(pages, (long)p.width);
+    int* const row = p.table + (long)b * p.width;
+    for (int c = thread; c < p.width; c += kThreads) {
+      if (c < begin) {
+        if (p.parents) row[c] = p.entries[(long)b * p.width + c];
+      } else {
+        const int place = first + c - begin;
+        row[c] = c < end && place < listed ? p.listed[place] : -1;
+      }
+    }
+    if (thread == 0) {
+      p.lengths[b] = (int)min(held + more, 0x7fffffffl);
+      if (b == 0) *free_pages = listed - p.totals[1];
+    }
+  }
+  if (source < 0 || first >= listed) return;
+  const int target = p.listed[first], rows = (int)(held & ((1l << p.page_shift) - 1));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!cache.at[i]) continue;
+    char* to = cache.at[i] + ((long)target * p.kv_heads + hk) * cache.row[i];
+    const char* from = cache.at[i] + ((long)source * p.kv_heads + hk) * cache.row[i];
+    if (i < 2)
+      copy_bytes<false, kThreads>(to, from, rows * cache.token[i], thread);
+    else  // a byte a token
+      for (int r = thread; r < rows; r += kThreads) to[r] = from[r];
+  }
+}
+
+// All of the bookkeeping in one workgroup, a thread a row; kExtend: and what follows it.
+struct FewRow {
+  int from, used, grows, last;
+};
+template <bool kExtend> __global__ void __launch_bounds__(1024) pages_few_kernel(PagesParams p, PageBytes cache, int* free_pages) {
   __shared__ int state[kFewPages];
+  __shared__ FewRow s_row[kFewRows];
   __shared__ int box[16];
+  static_assert(kFewRows == 1024);
+  const int b = threadIdx.x;
+  PageRow row;
+  if (b < p.batch) row = PageRow(p, b);
+  s_row[b] = {row.from, row.used, row.grows, -1};
   for (int i = threadIdx.x; i < p.pages; i += 1024) state[i] = kFree;
   __syncthreads();
-  const long entries = (long)p.batch * p.width;
-  for (long i = threadIdx.x; i < entries; i += 1024) mark_entry(p, state, i);
-  __syncthreads();
-  int asked = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 1024) {
-    const int b = b0 + (int)threadIdx.x;
-    int sum;
-    const int before = group_scan<1024>(b < p.batch ? ask(p, state, b) : 0, sum, box);
-    if (b < p.batch) p.first[b] = asked + before;
-    asked += sum;
+  const int entries = p.batch * p.width;
+  for (int i = threadIdx.x; i < entries; i += 1024) {
+    const int r = i / p.width, c = i - r * p.width;
+    FewRow& of = s_row[r];
+    if (c >= of.used) continue;
+    const int page = mark_entry(p, state, r, c, of);
+    if (c == of.used - 1) of.last = page;
   }
+  __syncthreads();
+  int asked;
+  const int before = group_scan<1024>(b < p.batch ? ask(p, state, b, row, s_row[b].last) : 0, asked, box);
+  if (b < p.batch) p.first[b] = before;
   // Each wave lists a run of pages.
   const int wave = threadIdx.x >> 6, run = ((p.pages + 16 * 64 - 1) / (16 * 64)) * 64;
   const int from = min(p.pages, wave * run), to = min(p.pages, from + run);
@@ -125,6 +184,10 @@ __global__ void __launch_bounds__(1024) pages_few_kernel(PagesParams p) {
     p.totals[0] = total;
     p.totals[1] = asked;
   }
+  if constexpr (kExtend) {
+    __syncthreads();  // (what this workgroup wrote it reads)
+    for (int i = wave; i < p.batch * p.kv_heads; i += 16) extend_row<64>(p, cache, free_pages, i / p.kv_heads, i % p.kv_heads, threadIdx.x & 63);
+  }
 }
 
 // The same in steps, for more.
@@ -134,7 +197,10 @@ __global__ void __launch_bounds__(256) pages_clear_kernel(PagesParams p) {
 }
 __global__ void __launch_bounds__(256) pages_mark_kernel(PagesParams p) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i < (long)p.batch * p.width) mark_entry(p, p.state, i);
+  if (i >= (long)p.batch * p.width) return;
+  const int b = (int)(i / p.width), c = (int)(i - (long)b * p.width);
+  const PageRow row(p, b);
+  if (c < row.used) mark_entry(p, p.state, b, c, row);
 }
 __global__ void __launch_bounds__(256) pages_count_kernel(PagesParams p) {
   __shared__ int box[4];
@@ -151,7 +217,7 @@ __global__ void __launch_bounds__(1024) pages_scan_kernel(PagesParams p) {
   for (int b0 = 0; b0 < p.batch; b0 += 1024) {
     const int b = b0 + (int)threadIdx.x;
     int sum;
-    const int before = group_scan<1024>(b < p.batch ? ask(p, p.state, b) : 0, sum, box);
+    const int before = group_scan<1024>(b < p.batch ? ask(p, b) : 0, sum, box);
     if (b < p.batch) p.first[b] = asked + before;
     asked += sum;
   }
@@ -182,7 +248,7 @@ __global__ void __launch_bounds__(256) pages_list_kernel(PagesParams p) {
 
 hipError_t bookkeeping(const PagesParams& p, hipStream_t stream) {
   if (few_pages(p.batch, p.width, p.pages)) {
-    hipLaunchKernelGGL(pages_few_kernel, dim3(1), dim3(1024), 0, stream, p);
+    hipLaunchKernelGGL((pages_few_kernel<false>), dim3(1), dim3(1024), 0, stream, p, PageBytes{}, nullptr);
     return hipGetLastError();
   }
   const long entries = (long)p.batch * p.width;
@@ -195,55 +261,9 @@ hipError_t bookkeeping(const PagesParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// `bytes` bytes (a multiple of 16, both ends aligned to it) by the workgroup; null source: zeros. kPast: stored past the
-// caches, for copies larger than these (230 MB of e4m3 pages 82 us where they went to them in 106; after other work, with the
-// bookkeeping, 116 and 121).
-template <bool kPast> __device__ __forceinline__ void copy_bytes(char* to, const char* from, int bytes) {
-  for (int i = 16 * (int)threadIdx.x; i < bytes; i += 16 * 256) {
-    const u32x4 x = from ? *reinterpret_cast<const u32x4*>(from + i) : u32x4{0, 0, 0, 0};
-    if constexpr (kPast)
-      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to + i));
-    else
-      *reinterpret_cast<u32x4*>(to + i) = x;
-  }
-}
-
-// A workgroup a row and key/value head, whose rows of a shared page it copies if there are any; the
-// first of a row's writes its entries and length too.
+// A workgroup a row and key/value head.
 __global__ void __launch_bounds__(256) pages_extend_kernel(PagesParams p, PageBytes cache, int* free_pages) {
-  const int b = blockIdx.x, hk = blockIdx.y;
-  const int begin = p.begin[b], first = p.first[b], source = p.source[b], listed = p.totals[0];
-  const long held = p.held[b];
-  if (hk == 0) {
-    const long more = max(0, p.new_tokens ? p.new_tokens[b] : p.new_each);
-    const long pages = (held + more + (1l << p.page_shift) - 1) >> p.page_shift;
-    const int end = (int)min(pages, (long)p.width);
-    int* const row = p.table + (long)b * p.width;
-    for (int c = threadIdx.x; c < p.width; c += 256) {
-      if (c < begin) {
-        if (p.parents) row[c] = p.entries[(long)b * p.width + c];
-      } else {
-        const int place = first + c - begin;
-        row[c] = c < end && place < listed ? p.listed[place] : -1;
-      }
-    }
-    if (threadIdx.x == 0) {
-      p.lengths[b] = (int)min(held + more, 0x7fffffffl);
-      if (b == 0) *free_pages = listed - p.totals[1];
-    }
-  }
-  if (source < 0 || first >= listed) return;
-  const int target = p.listed[first], rows = (int)(held & ((1l << p.page_shift) - 1));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (!cache.at[i]) continue;
-    char* to = cache.at[i] + ((long)target * p.kv_heads + hk) * cache.row[i];
-    const char* from = cache.at[i] + ((long)source * p.kv_heads + hk) * cache.row[i];
-    if (i < 2)
-      copy_bytes<false>(to, from, rows * cache.token[i]);
-    else  // a byte a token
-      for (int r = threadIdx.x; r < rows; r += 256) to[r] = from[r];
-  }
+  extend_row<256>(p, cache, free_pages, blockIdx.x, blockIdx.y, threadIdx.x);
 }
 
 // Workgroups y take the tensors' pieces of a page in turn, the last of y the table.
@@ -272,14 +292,19 @@ __global__ void __launch_bounds__(256) pages_compact_kernel(PagesParams p, PageB
     const long piece = (size / 16 + pieces - 1) / pieces * 16;
     const long at = piece * blockIdx.y, left = size - at;
     if (left > 0)
-      copy_bytes<true>(out.at[i] + page * size + at, from < 0 ? nullptr : cache.at[i] + from * size + at,
-                 (int)(left < piece ? left : piece));
+      copy_bytes<true, 256>(out.at[i] + page * size + at, from < 0 ? nullptr : cache.at[i] + from * size + at,
+                 (int)(left < piece ? left : piece), threadIdx.x);
   }
 }
 
 }  // namespace
 
 hipError_t launch_pages_extend(const PagesParams& p, const PageBytes& cache, int* free_pages, hipStream_t stream) {
+  const long most = (long)p.batch * p.kv_heads * (cache.row[0] + cache.row[1]);  // bytes that the rows copy
+  if (few_pages(p.batch, p.width, p.pages) && most <= kFewBytes && (long)p.batch * p.kv_heads <= kFewHeads) {
+    hipLaunchKernelGGL((pages_few_kernel<true>), dim3(1), dim3(1024), 0, stream, p, cache, free_pages);
+    return hipGetLastError();
+  }
   const hipError_t e = bookkeeping(p, stream);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(pages_extend_kernel, dim3(p.batch, p.kv_heads), dim3(256), 0, stream, p, cache, free_pages);
