@@ -111,7 +111,7 @@ inline BlockPlan block_plan(int total, int heads, int kv_heads, int head_dim, in
 
 // Attention of many tokens, a block at a time (fhog_blocks_chunk.hip).
 constexpr int kTileRows = 128;       // rows of a tile
-constexpr int kMostColumns = 8192;   // of the page table (the masks of 64 tokens are in LDS)
+constexpr int kMostColumns = 8192;   // of the page table (the masks of 64 tokens are in LDS, 64 KB)
 constexpr int kSumBlocks = 256;      // blocks of a list (a join's weights are)
 constexpr int kMostLists = 32768;    // sequences times heads times columns
 // A tile of a list (the tokens that chose one column of a sequence, for one head): whole tokens, whose entries are

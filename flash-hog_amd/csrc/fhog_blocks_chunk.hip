@@ -8,8 +8,8 @@
 // same bits at every call.
 //
 // What bounds it: those outputs, written and read once, 8 (head_dim + 2) bytes for each row and block. 2035 tokens in 4
-// sequences, H32/8 D128 bf16, 16 blocks of 64, 540 MB of outputs, us: masks 6, items 8, entries 8, tiles 133, sum 108 (5.0 TB/s).
-// 4096 tokens, H12/12 D64 e4m3, 16 blocks, 207 MB: 9, 9, 10, 60, 51. (250 MB at D = 128: tiles 91, without their stores 57.
+// sequences, H32/8 D128 bf16, 16 blocks of 64, 540 MB of outputs, us: masks 5, items 6, entries 6, tiles 133, sum 108 (5.0 TB/s).
+// 4096 tokens, H12/12 D64 e4m3, 16 blocks, 207 MB: 5, 7, 9, 60, 51. (250 MB at D = 128: tiles 91, without their stores 57.
 // A token at a time 583 and 744 in all.)
 //
 //   block_masks_kernel   64 tokens and a key/value head: which of them chose each column
@@ -60,8 +60,10 @@ __device__ __forceinline__ unsigned long group_bits(int group, int begin, int en
   return below & ~((1ul << lo) - 1);
 }
 
-template <typename T, typename C> __global__ void __launch_bounds__(kThreads) block_masks_kernel(BlockChunkParams<T, C> p) {
-  __shared__ unsigned long s_mask[kMostColumns];
+// (256 / 512 / 1024 threads, us in all three, 2035 tokens of 8 heads 20 / 17 / 17, 4096 of 12 24 / 21 / 24)
+constexpr int kListThreads = 512;
+template <typename T, typename C> __global__ void __launch_bounds__(kListThreads) block_masks_kernel(BlockChunkParams<T, C> p) {
+  extern __shared__ unsigned long s_mask[];  // (columns)
   __shared__ PackedTokenAt s_token[64];
   __shared__ unsigned long s_falling;
   const CacheShape& c = p.at;
@@ -70,20 +72,20 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   // Lists and their tokens agree on whose a token is only if the offsets rise. If they do not, nothing is listed,
   // and the rows become NaN (block_sum_kernel).
   bool falls = false;
-  for (int i = threadIdx.x; i < c.batch; i += kThreads) falls = falls || packed_begin(c, i + 1) < packed_begin(c, i);
+  for (int i = threadIdx.x; i < c.batch; i += kListThreads) falls = falls || packed_begin(c, i + 1) < packed_begin(c, i);
   falls = __syncthreads_or(falls);
   if (group == 0 && hk == 0 && threadIdx.x == 0) {
     p.total[0] = 0;
     p.total[1] = falls;
   }
   if (threadIdx.x == 0) s_falling = 0;
-  for (int i = threadIdx.x; i < width; i += kThreads) s_mask[i] = 0;
+  for (int i = threadIdx.x; i < width; i += kListThreads) s_mask[i] = 0;
   if ((int)threadIdx.x < count) {
     const PackedToken t(p, p.token0 + 64 * group + threadIdx.x);
     s_token[threadIdx.x] = {t.there && !falls ? t.pos : -1};
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < count * p.blocks; i += kThreads) {
+  for (int i = threadIdx.x; i < count * p.blocks; i += kListThreads) {
     const int t = i / p.blocks, at = i - t * p.blocks;
     const int* const list = p.chosen + ((long)(p.token0 + 64 * group + t) * c.kv_heads + hk) * p.blocks;
     const int col = list[at];
@@ -93,14 +95,15 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   }
   __syncthreads();
   unsigned long* const out = p.masks + ((long)hk * p.groups + group) * width;
-  for (int i = threadIdx.x; i < width; i += kThreads) out[i] = s_mask[i];
+  for (int i = threadIdx.x; i < width; i += kListThreads) out[i] = s_mask[i];
   if (threadIdx.x == 0) p.falling[(long)hk * p.groups + group] = s_falling;
 }
 
-// Four threads a list, each a quarter of the groups, and then the first: the list's tiles get places behind
+// Eight threads a list, each an eighth of the groups, and then the first: the list's tiles get places behind
 // others', a wave at a time (in any order: each tile's outputs have places of their own).
-template <typename T, typename C> __global__ void __launch_bounds__(kThreads) block_items_kernel(BlockChunkParams<T, C> p) {
-  __shared__ int s_count[4][64];
+template <typename T, typename C> __global__ void __launch_bounds__(kListThreads) block_items_kernel(BlockChunkParams<T, C> p) {
+  constexpr int kWays = kListThreads / 64;
+  __shared__ int s_count[kWays][64];
   const CacheShape& c = p.at;
   const int way = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int i = blockIdx.x * 64 + lane, width = c.pages_per_seq, group = p.heads / c.kv_heads;
@@ -110,7 +113,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
     col = i % width, hk = i / width % c.kv_heads, b = i / width / c.kv_heads;
     slab_range(p, b, begin, end);
     at = (long)hk * p.groups * width + col;
-    const int first = begin / 64, last = max(first, (end + 63) / 64), each = (last - first + 3) / 4;
+    const int first = begin / 64, last = max(first, (end + 63) / 64), each = (last - first + kWays - 1) / kWays;
     g0 = min(last, first + way * each), g1 = min(last, g0 + each);
   }
 #pragma unroll 8
@@ -126,7 +129,8 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
     earlier += __popcll(p.masks[at + (long)g * width] & group_bits(g, begin, end));
   }
   if (way > 0) return;
-  count = s_count[0][lane] + s_count[1][lane] + s_count[2][lane] + s_count[3][lane];
+  count = 0;
+  for (int w = 0; w < kWays; ++w) count += s_count[w][lane];
   const int each = tile_tokens(group), tiles = (count + each - 1) / each;
   int sum, first = 0;
   const int before = wave_scan(tiles, sum);
@@ -147,7 +151,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
 }
 
 // A thread an element of the tokens' lists, at its rank among the tokens that chose the same.
-template <typename T, typename C> __global__ void __launch_bounds__(kThreads) block_entries_kernel(BlockChunkParams<T, C> p) {
+template <typename T, typename C> __global__ void __launch_bounds__(kListThreads) block_entries_kernel(BlockChunkParams<T, C> p) {
   __shared__ PackedTokenAt s_token[64];
   __shared__ int s_b[64], s_begin[64], s_end[64];
   const CacheShape& c = p.at;
@@ -162,7 +166,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kThreads) bl
   const unsigned long falling = p.falling[(long)hk * p.groups + group];
   const int each = tile_tokens(p.heads / c.kv_heads);
   __syncthreads();
-  for (int i = threadIdx.x; i < count * p.blocks; i += kThreads) {
+  for (int i = threadIdx.x; i < count * p.blocks; i += kListThreads) {
     const int t = i / p.blocks, at = i - t * p.blocks;
     const int* const list = p.chosen + ((long)(p.token0 + 64 * group + t) * c.kv_heads + hk) * p.blocks;
     const int col = list[at];
@@ -429,9 +433,10 @@ hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p_, int slab, hipStr
     p.tokens = p.at.total - p.token0 < slab ? p.at.total - p.token0 : slab;
     p.groups = (p.tokens + 63) / 64;
     const long most = (long)p.tokens * p.blocks * p.at.kv_heads / tile_tokens(p.heads / p.at.kv_heads) + p.lists;
-    hipLaunchKernelGGL((block_masks_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((block_items_kernel<T, C>), dim3((p.lists + 63) / 64), dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((block_entries_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((block_masks_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kListThreads),
+                       p.at.pages_per_seq * sizeof(unsigned long), stream, p);
+    hipLaunchKernelGGL((block_items_kernel<T, C>), dim3((p.lists + 63) / 64), dim3(kListThreads), 0, stream, p);
+    hipLaunchKernelGGL((block_entries_kernel<T, C>), dim3(p.groups, p.at.kv_heads), dim3(kListThreads), 0, stream, p);
     const dim3 tiles((unsigned)((most + 7) / 8 * 8));
     if ((long)p.tokens * p.heads * p.blocks * D * 4 > kCacheBytes)
       hipLaunchKernelGGL((block_tile_kernel<T, C, D, true>), tiles, dim3(kThreads), 0, stream, p);

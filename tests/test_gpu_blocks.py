@@ -446,12 +446,12 @@ def test_many_tokens_wide_table(cuda_device):
     import flash_hog
 
     print("[case] many tokens, wide table", flush=True)
-    case = MANY[4]
+    case = MANY[6]
     for width in (None, 8192, 8193):
         cache, counts, q, moved, where = make(case, cuda_device, width=width)
-        lists = many_lists((*case[:8], 7), cache, counts, "chosen")
+        lists = many_lists(case, cache, counts, "chosen")
         out = flash_hog.paged_block_attention(q.to(cuda_device), lists.to(cuda_device), moved["key_cache"], moved["value_cache"], **where)
-        check(out, ref.attention_dense(q, cache, counts, lists, 128 ** -0.5))
+        check(out, ref.attention_dense(q, cache, counts, lists, 256 ** -0.5))
 
 
 def test_strided_inputs(cuda_device):
