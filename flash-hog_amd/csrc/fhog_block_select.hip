@@ -581,7 +581,9 @@ template <typename T, int D> hipError_t launch_block_select(const BlockSelectPar
   const int width = p.at.pages_per_seq, most = width - p.first - p.last;  // columns chosen from
   if (plan.tiles && plan.slab == 0) {
     const dim3 grid((unsigned)((long)plan.slots * p.at.kv_heads));
-    if (most <= 256)
+    if (most <= 128)
+      hipLaunchKernelGGL((block_select_tile_kernel<T, D, 128>), grid, dim3(kThreads), 0, stream, p);
+    else if (most <= 256)
       hipLaunchKernelGGL((block_select_tile_kernel<T, D, 256>), grid, dim3(kThreads), 0, stream, p);
     else if (most <= 512)
       hipLaunchKernelGGL((block_select_tile_kernel<T, D, 512>), grid, dim3(kThreads), 0, stream, p);
