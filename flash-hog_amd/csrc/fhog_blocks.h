@@ -156,6 +156,7 @@ template <typename T, typename C> struct BlockChunkParams {
 // 394 us; each slab has five launches, and ends with CUs idle). Where they would not stay in the cache behind the L2s, they
 // are stored past it: tiles / sum of 540 MB 189 / 105 us in it, 134 / 107 past it; of 207 MB 60 / 51 and 59 / 59.
 constexpr long kPartBytes = 1l << 30, kCacheBytes = 256l << 20;
+inline long block_token_bytes(int heads, int head_dim, int blocks) { return (long)heads * blocks * (head_dim + 2) * 4; }
 struct BlockChunkPlan {
   int slab;
   long lists, masks, groups, entries, items, parts;  // elements
@@ -163,9 +164,8 @@ struct BlockChunkPlan {
 };
 inline BlockChunkPlan block_chunk_plan(int batch, int total, int heads, int kv_heads, int head_dim, int pages_per_seq, int blocks) {
   BlockChunkPlan p;
-  const long token = (long)heads * blocks * (head_dim + 2) * 4;
-  const long fit = kPartBytes / token / 64 * 64;
-  p.slab = (int)(fit < 64 ? 64 : fit < total ? fit : total);
+  const long fit = kPartBytes / block_token_bytes(heads, head_dim, blocks) / 64 * 64;  // (64 at least: block_chunk_rule)
+  p.slab = (int)(fit < total ? fit : total);
   p.lists = (long)batch * kv_heads * pages_per_seq;
   p.groups = (long)kv_heads * ((p.slab + 63) / 64);
   p.masks = p.groups * pages_per_seq;
@@ -199,7 +199,9 @@ inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int 
                              int blocks, bool single) {
   const int group = heads / kv_heads;
   const long lists = (long)batch * kv_heads * pages_per_seq;
-  if (single || pages_per_seq > kMostColumns || blocks > kSumBlocks || group > kTileRows || lists > kMostLists) return false;
+  if (single || pages_per_seq > kMostColumns || blocks > kSumBlocks || group > kTileRows || lists > kMostLists ||
+      64 * block_token_bytes(heads, head_dim, blocks) > kPartBytes)
+    return false;
   const double entries = (double)total * kv_heads * blocks, block = 4.0 * page_size * head_dim;
   const double token_us = entries * block / 14e6;
   const double block_us = 16 + entries * 8.0 * group * (head_dim + 2) / 3.8e6 + (entries < lists ? entries : lists) * block / 14e6;

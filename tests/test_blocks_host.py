@@ -95,6 +95,12 @@ def test_workspace_bytes(lib):
     assert lib.fhog_paged_block_workspace_bytes(1, 1, 1, 4, 2, 64, 15, 5, 1) == 0
     few, many = (lib.fhog_paged_block_workspace_bytes(t, t, 1, 32, 8, 128, 64, 500, 64) for t in (1, 4096))
     assert few > 0 and many == 0
+    # many tokens: their blocks' outputs, a slab of 1 GiB at a time; a token at a time where 64 tokens' do not fit
+    outputs = lambda heads, dim, page, blocks, total=1 << 15: lib.fhog_paged_block_workspace_bytes(
+        1, total, 0, heads, 8, dim, page, 512, blocks)
+    assert 32 * 16 * 130 * 4 * 2035 < outputs(32, 128, 64, 16, 2035) < 32 * 16 * 130 * 4 * 2035 + (64 << 20)
+    assert 0.9 * 2 ** 30 < outputs(32, 128, 64, 16) < 1.1 * 2 ** 30
+    assert outputs(64, 256, 1024, 253) > 0 and outputs(64, 256, 1024, 255) == 0
 
 
 def cpu(kind=BF16, device="cpu"):
