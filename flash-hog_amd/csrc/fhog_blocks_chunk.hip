@@ -45,12 +45,9 @@ struct PackedToken {
   }
 };
 
-// Tokens of sequence b among the slab's, as indexes from its first on.
-template <typename P> __device__ __forceinline__ void slab_range(const P& p, int b, int& begin, int& end) {
-  begin = packed_begin(p.at, b) - p.token0;
-  end = packed_begin(p.at, b + 1) - p.token0;
-  begin = max(begin, 0);
-  end = max(begin, min(end, p.tokens));
+// Tokens of sequence b among the slab's.
+template <typename P> __device__ __forceinline__ IndexRange tokens_of(const P& p, int b) {
+  return slab_range(packed_begin(p.at, b), packed_begin(p.at, b + 1), p.token0, p.tokens);
 }
 // The bits of group `group` that are tokens [begin, end).
 __device__ __forceinline__ unsigned long group_bits(int group, int begin, int end) {
@@ -107,26 +104,26 @@ template <typename T, typename C> __global__ void __launch_bounds__(kListThreads
   const CacheShape& c = p.at;
   const int way = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int i = blockIdx.x * 64 + lane, width = c.pages_per_seq, group = p.heads / c.kv_heads;
-  int count = 0, col = 0, hk = 0, b = 0, begin = 0, end = 0, g0 = 0, g1 = 0;
+  int count = 0, col = 0, hk = 0, b = 0;
+  IndexRange of{0, 0}, groups{0, 0};
   long at = 0;
   if (i < p.lists) {
     col = i % width, hk = i / width % c.kv_heads, b = i / width / c.kv_heads;
-    slab_range(p, b, begin, end);
+    of = tokens_of(p, b);
+    groups = list_groups(of, way, kWays);
     at = (long)hk * p.groups * width + col;
-    const int first = begin / 64, last = max(first, (end + 63) / 64), each = (last - first + kWays - 1) / kWays;
-    g0 = min(last, first + way * each), g1 = min(last, g0 + each);
   }
 #pragma unroll 8
-  for (int g = g0; g < g1; ++g) count += __popcll(p.masks[at + (long)g * width] & group_bits(g, begin, end));
+  for (int g = groups.begin; g < groups.end; ++g) count += __popcll(p.masks[at + (long)g * width] & group_bits(g, of.begin, of.end));
   s_count[way][lane] = count;
   __syncthreads();
   int earlier = 0;
   for (int w = 0; w < way; ++w) earlier += s_count[w][lane];
   // (a group that begins with an earlier sequence's tokens is that one's: this one's count there is 0)
 #pragma unroll 8
-  for (int g = g0; g < g1; ++g) {
-    if (g > begin / 64) p.before[at + (long)g * width] = earlier;
-    earlier += __popcll(p.masks[at + (long)g * width] & group_bits(g, begin, end));
+  for (int g = groups.begin; g < groups.end; ++g) {
+    if (g > of.begin / 64) p.before[at + (long)g * width] = earlier;
+    earlier += __popcll(p.masks[at + (long)g * width] & group_bits(g, of.begin, of.end));
   }
   if (way > 0) return;
   count = 0;
@@ -153,7 +150,8 @@ template <typename T, typename C> __global__ void __launch_bounds__(kListThreads
 // A thread an element of the tokens' lists, at its rank among the tokens that chose the same.
 template <typename T, typename C> __global__ void __launch_bounds__(kListThreads) block_entries_kernel(BlockChunkParams<T, C> p) {
   __shared__ PackedTokenAt s_token[64];
-  __shared__ int s_b[64], s_begin[64], s_end[64];
+  __shared__ int s_b[64];
+  __shared__ IndexRange s_of[64];
   const CacheShape& c = p.at;
   const int group = blockIdx.x, hk = blockIdx.y, width = c.pages_per_seq;
   const int count = min(64, p.tokens - 64 * group);
@@ -161,7 +159,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kListThreads
     const PackedToken t(p, p.token0 + 64 * group + threadIdx.x);
     s_token[threadIdx.x] = {t.there ? t.pos : -1};
     s_b[threadIdx.x] = t.b;
-    slab_range(p, t.b, s_begin[threadIdx.x], s_end[threadIdx.x]);
+    s_of[threadIdx.x] = tokens_of(p, t.b);
   }
   const unsigned long falling = p.falling[(long)hk * p.groups + group];
   const int each = tile_tokens(p.heads / c.kv_heads);
@@ -176,7 +174,7 @@ template <typename T, typename C> __global__ void __launch_bounds__(kListThreads
       while (list[first] != col) ++first;
       if (first < at) continue;
     }
-    const int begin = s_begin[t], end = s_end[t];
+    const int begin = s_of[t].begin, end = s_of[t].end;
     const long place = ((long)hk * p.groups + group) * width + col;
     const unsigned long mask = p.masks[place], bits = mask & group_bits(group, begin, end) & ((1ul << t) - 1);
     if (!(mask >> t & 1)) continue;  // (nothing is listed)
