@@ -43,11 +43,14 @@ constexpr IndexRange list_groups(IndexRange of, int way, int ways) {
   return {begin, begin + each < last ? begin + each : last};
 }
 
-// Tokens are taken in slabs whose outputs stay within this (540 MB of them in slabs of 256 / 512 / 1024 MB: 415 / 429 /
+// Tokens are taken in slabs whose outputs and masks stay within this (540 MB of outputs in slabs of 256 / 512 / 1024 MB: 415 / 429 /
 // 394 us; each slab has five launches, and ends with CUs idle). Where they would not stay in the cache behind the L2s, they
 // are stored past it: tiles / sum of 540 MB 189 / 105 us in it, 134 / 107 past it; of 207 MB 60 / 51 and 59 / 59.
 constexpr long kPartBytes = 1l << 30, kCacheBytes = 256l << 20;
-inline long block_token_bytes(int heads, int head_dim, int blocks) { return (long)heads * blocks * (head_dim + 2) * 4; }
+// Outputs, and masks with the counts before them, of 64 tokens.
+inline long block_group_bytes(int heads, int kv_heads, int head_dim, int pages_per_seq, int blocks) {
+  return 64l * heads * blocks * (head_dim + 2) * 4 + kv_heads * (12l * pages_per_seq + 8);
+}
 struct BlockChunkPlan {
   int slab;
   long lists, masks, groups, entries, items, parts;  // elements
@@ -55,7 +58,7 @@ struct BlockChunkPlan {
 };
 inline BlockChunkPlan block_chunk_plan(int batch, int total, int heads, int kv_heads, int head_dim, int pages_per_seq, int blocks) {
   BlockChunkPlan p;
-  const long fit = kPartBytes / block_token_bytes(heads, head_dim, blocks) / 64 * 64;  // (64 at least: block_chunk_rule)
+  const long fit = kPartBytes / block_group_bytes(heads, kv_heads, head_dim, pages_per_seq, blocks) * 64;  // (64 at least: block_chunk_rule)
   p.slab = (int)(fit < total ? fit : total);
   p.lists = (long)batch * kv_heads * pages_per_seq;
   p.groups = (long)kv_heads * ((p.slab + 63) / 64);
@@ -79,7 +82,7 @@ inline bool block_chunk_rule(int batch, int total, int heads, int kv_heads, int 
   const int group = heads / kv_heads;
   const long lists = (long)batch * kv_heads * pages_per_seq;
   if (single || pages_per_seq > kMostColumns || blocks > kSumBlocks || group > kTileRows || lists > kMostLists ||
-      64 * block_token_bytes(heads, head_dim, blocks) > kPartBytes)
+      block_group_bytes(heads, kv_heads, head_dim, pages_per_seq, blocks) > kPartBytes)
     return false;
   const double entries = (double)total * kv_heads * blocks, block = 4.0 * page_size * head_dim;
   const double token_us = entries * block / 14e6;

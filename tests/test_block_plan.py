@@ -111,3 +111,27 @@ def test_any_offsets(rules):
         if rng.random() < 0.7:
             offsets.sort()
         check_walk(rules, offsets, total, slab, kv_heads, width, masks)
+
+
+# (batch, total, heads, kv_heads, head_dim, page, width, blocks): small outputs beside wide masks
+WIDE = [(1, 131072, 8, 8, 64, 128, 4096, 4), (1, 262144, 4, 4, 64, 32, 8192, 8), (1, 1 << 20, 1, 1, 64, 128, 8192, 4)]
+
+
+def test_workspace_bound(rules):
+    """At most 1.1 GiB: the outputs and masks of a slab within 1 GiB; entries and items, of at most 1056 bytes for
+    a tile of at least 65 rows of 264 bytes of outputs, and of 1060 for each of 32768 lists, are 9.5 % more."""
+    rng, taken = random.Random(3), 0
+    cases = list(WIDE)
+    for _ in range(60000):
+        kv_heads, group = rng.choice([1, 2, 4, 8, 12, 32]), rng.choice([1, 2, 3, 4, 8, 16, 43, 64, 65, 128])
+        cases.append((rng.choice([1, 2, 16, 100]), int(2 ** rng.uniform(4, 21)), group * kv_heads, kv_heads, rng.choice([64, 128, 256]),
+                      1 << rng.randint(4, 10), int(2 ** rng.uniform(0, 13)), int(2 ** rng.uniform(0, 8))))
+    for batch, total, heads, kv_heads, head_dim, page, width, blocks in cases:
+        if not rules.rule(batch, total, heads, kv_heads, head_dim, page, width, blocks):
+            continue
+        taken += 1
+        p = plan(rules, batch, total, heads, kv_heads, head_dim, width, blocks)
+        assert p["bytes"] <= 1.1 * 2 ** 30, (batch, total, heads, kv_heads, head_dim, page, width, blocks)
+        assert p["slab"] == total or (p["slab"] >= 64 and p["slab"] % 64 == 0)
+    assert taken > 5000
+    assert all(rules.rule(*c[:6], *c[6:]) for c in WIDE)

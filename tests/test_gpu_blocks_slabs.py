@@ -13,7 +13,7 @@ from test_gpu_paged import check
 pytestmark = pytest.mark.gpu
 
 
-# 132 KiB a token: slabs of 8064 tokens
+# 132 KiB a token: slabs of 7936 tokens
 @pytest.mark.parametrize("lengths,new", [([6000, 5000, 4000], [5001, 4001, 3001]), ([20001, 200], [20001, 3])], ids=str)
 def test_sequences_behind_a_slab(lengths, new, cuda_device):
     """Each sequence like the call of its own: the same bits where its slabs hold the same tokens of it (rows of a tile share
@@ -34,7 +34,7 @@ def test_sequences_behind_a_slab(lengths, new, cuda_device):
         own = dict(page_table=where["page_table"][b:b + 1], lengths=where["lengths"][b:b + 1],
                    query_offsets=torch.tensor([0, n], dtype=torch.int32, device=cuda_device))
         one = flash_hog.paged_block_attention(q[rows].to(cuda_device), lists[rows].to(cuda_device), *kv, **own)
-        if n > 1000 and (rows.start == 0 or rows.start // 8064 == (rows.stop - 1) // 8064):
+        if n > 1000 and (rows.start == 0 or rows.start // 7936 == (rows.stop - 1) // 7936):
             assert torch.equal(got[rows], one)
         if n <= 5001:
             alone = [n if i == b else 0 for i in range(len(new))]
