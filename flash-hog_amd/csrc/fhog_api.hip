@@ -1036,8 +1036,8 @@ int fhog_paged_block_attention(fhog_stream_t stream, const void* q, const int* c
     fhog::BlockParams<T, C> p{(const T*)q, (T*)out,
                               {(const C*)k_cache, (const C*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale},
                               cache_shape(s, page_table, lengths, query_offsets), chosen, (float*)workspace, heads, blocks,
-                              plan.slots, plan.splits, plan.split_tiles, clear_rest, scale};
-    return fhog::launch_block_attention<T, C, D>(p, (hipStream_t)stream);
+                              plan.slots, plan.splits, plan.split_tiles, clear_rest, scale, 0};
+    return fhog::launch_block_attention<T, C, D>(p, plan.slab, (hipStream_t)stream);
   };
   return launch_status(dispatch_paged(s, run), who);
 }

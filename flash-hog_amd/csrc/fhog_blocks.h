@@ -32,9 +32,10 @@ template <typename T, typename C> struct BlockParams {
   const int* chosen;
   float* parts;  // as PagedParams'
   int heads, blocks;
-  int slots, splits, split_tiles;  // slots: tiles of 16 rows of a token's group
+  int slots, splits, split_tiles;  // slots: tiles of 16 rows of a token's group, at a time
   int clear_rest;
   float scale;
+  int slot0;  // the first of these
 };
 
 // How choices are made: by tiles of 16 tokens of a sequence (slots of them), token by token in a workgroup each, or with
@@ -82,7 +83,8 @@ inline SelectPlan select_plan(int batch, int total, bool single, int kv_heads, i
 // Attention of tokens over chosen blocks: tiles of 16 rows, and how the blocks are split.
 struct BlockPlan {
   int slots, splits, split_tiles;
-  long parts;
+  int slab;    // slots at a time: as many as leave no more than kPartBytes of parts
+  long parts;  // rows of them
 };
 constexpr int kSplitBlocks = 512;  // blocks of a split, whose places are in LDS
 inline BlockPlan block_plan(int total, int heads, int kv_heads, int head_dim, int page_size, int blocks, int cus) {
@@ -106,7 +108,10 @@ inline BlockPlan block_plan(int total, int heads, int kv_heads, int head_dim, in
   if (splits < 1) splits = 1;
   p.split_tiles = (int)((tiles + splits - 1) / splits);
   p.splits = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
-  p.parts = p.splits > 1 ? work * p.splits * 16 : 0;
+  // (lists of more than kSplitBlocks have several splits however many tokens there are)
+  const long rows = p.splits > 1 ? (long)kv_heads * p.splits * 16 : 0, fit = rows ? kPartBytes / (rows * (head_dim + 2) * 4) : p.slots;
+  p.slab = (int)(fit < 1 ? 1 : fit < p.slots ? fit : p.slots);
+  p.parts = p.slab * rows;
   return p;
 }
 
@@ -152,6 +157,6 @@ template <typename T, typename C, int D>
 hipError_t launch_block_chunk(const BlockChunkParams<T, C>& p, int slab, hipStream_t s);
 template <typename C, int D> hipError_t launch_key_means(const KeyMeansParams<C>& p, int workgroups, hipStream_t s);
 template <typename T, int D> hipError_t launch_block_select(const BlockSelectParams<T>& p, SelectPlan plan, hipStream_t s);
-template <typename T, typename C, int D> hipError_t launch_block_attention(const BlockParams<T, C>& p, hipStream_t s);
+template <typename T, typename C, int D> hipError_t launch_block_attention(const BlockParams<T, C>& p, int slab, hipStream_t s);
 
 }  // namespace fhog

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(64 * kWaves) block_token_kernel(BlockParams<T,
   const int n = lane & 15, g = lane >> 4;
   const CacheShape& c = p.at;
   const int hk = blockIdx.x % c.kv_heads, slot = blockIdx.x / c.kv_heads, split = blockIdx.y;
-  const TokenRows tr(p, slot);
+  const TokenRows tr(p, p.slot0 + slot);
   if (!tr.there) {
     if (p.clear_rest && split == 0)
       for (int i = threadIdx.x; i < tr.rows * (D / 8); i += 64 * kWaves)
@@ -258,7 +258,7 @@ template <typename T, typename C, int D> __global__ void __launch_bounds__(256) 
   __shared__ float s_w[kJoinWeights];
   const CacheShape& c = p.at;
   const int hk = blockIdx.x % c.kv_heads, slot = blockIdx.x / c.kv_heads;
-  const TokenRows tr(p, slot);
+  const TokenRows tr(p, p.slot0 + slot);
   if (!tr.there) return;
   const long part = ((long)slot * c.kv_heads + hk) * p.splits, parts = (long)p.slots * c.kv_heads * p.splits;
   const float* const part_out = p.parts + part * kRows * D;
@@ -289,17 +289,21 @@ template <typename T, typename C, int D> __global__ void __launch_bounds__(256) 
 }  // namespace
 
 template <typename T, typename C, int D>
-hipError_t launch_block_attention(const BlockParams<T, C>& p, hipStream_t stream) {
+hipError_t launch_block_attention(const BlockParams<T, C>& p_, int slab, hipStream_t stream) {
   constexpr int kWaves = D == 64 ? 8 : D == 128 ? 4 : 2;
-  const dim3 grid(p.slots * p.at.kv_heads, p.splits);
-  hipLaunchKernelGGL((block_token_kernel<T, C, D, kWaves>), grid, dim3(64 * kWaves), 0, stream, p);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  hipLaunchKernelGGL((block_join_kernel<T, C, D>), dim3(grid.x), dim3(256), 0, stream, p);
-  return hipGetLastError();
+  BlockParams<T, C> p = p_;
+  for (p.slot0 = 0; p.slot0 < p_.slots; p.slot0 += slab) {
+    p.slots = p_.slots - p.slot0 < slab ? p_.slots - p.slot0 : slab;
+    const dim3 grid(p.slots * p.at.kv_heads, p.splits);
+    hipLaunchKernelGGL((block_token_kernel<T, C, D, kWaves>), grid, dim3(64 * kWaves), 0, stream, p);
+    if (p.splits > 1) hipLaunchKernelGGL((block_join_kernel<T, C, D>), dim3(grid.x), dim3(256), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
-#define FHOG_INST(T, C, D) template hipError_t launch_block_attention<T, C, D>(const BlockParams<T, C>&, hipStream_t);
+#define FHOG_INST(T, C, D) template hipError_t launch_block_attention<T, C, D>(const BlockParams<T, C>&, int, hipStream_t);
 FHOG_INST(__bf16, __bf16, 64)
 FHOG_INST(__bf16, __bf16, 128)
 FHOG_INST(__bf16, __bf16, 256)

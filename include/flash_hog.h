@@ -348,7 +348,8 @@ int fhog_paged_block_select(fhog_stream_t stream, const void* q, const float* ke
  * of the pages in columns chosen[token][head], up to its own position. Columns outside [0, pages_per_seq) and
  * ones behind the token show nothing; one that is named twice counts twice. Offsets that fall somewhere may give NaN
  * in every row. The workspace of many tokens is as large as an fp32 output for each of their blocks, and 12 bytes for each
- * column of 64 tokens and a key/value head, up to 1.1 GiB (they are then taken in turn).
+ * column of 64 tokens and a key/value head; that of long lists as a few outputs for each token. Up to 1.1 GiB: more tokens
+ * are taken in turn.
  */
 size_t fhog_paged_block_workspace_bytes(int batch, int total, int single, int heads, int kv_heads, int head_dim,
                                         int page_size, int pages_per_seq, int blocks);

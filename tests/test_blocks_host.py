@@ -148,3 +148,12 @@ def test_fake_tensors(device, kind):
         assert out.shape == q.shape and out.dtype == BF16 and out.device == q.device
         with pytest.raises(ValueError, match="out is not supported"):
             flash_hog.paged_block_attention(q, chosen, **x, out=torch.empty_like(q))
+
+
+def test_workspace_of_long_lists(lib):
+    """Lists of more blocks than a split holds have parts for every token, within 1 GiB for however many tokens."""
+    size = lambda total, heads, kv_heads, dim, page, blocks: lib.fhog_paged_block_workspace_bytes(
+        1, total, 0, heads, kv_heads, dim, page, 4096, blocks)
+    for shape in ((4, 4, 64, 16, 600), (8, 8, 128, 16, 2000), (64, 1, 256, 64, 4096), (32, 8, 128, 32, 32768)):
+        one, few, many = (size(total, *shape) for total in (1, 300, 60000))
+        assert 0 < one and few <= many <= 1 << 30 and many > 0.9 * 2 ** 30

@@ -39,3 +39,29 @@ def test_sequences_behind_a_slab(lengths, new, cuda_device):
         if n <= 5001:
             alone = [n if i == b else 0 for i in range(len(new))]
             check(got[rows], ref.attention_dense(q[rows], cache, alone, lists[rows], 0.125))
+
+
+def test_long_lists_of_many_tokens(cuda_device):
+    """Lists of more blocks than a split holds, of more tokens than 1 GiB of parts: a token's bits are those of a call
+    of fewer tokens (a workgroup has one token's rows), and the padded rows behind the last sequence stay."""
+    import flash_hog
+
+    print("[case] long lists of many tokens", flush=True)
+    length, new, rows = 33000, 32500, 33000
+    cache, _, _, moved, where = make((4, 4, 64, BF16, False, 16, [length], [new]), cuda_device)
+    kv = moved["key_cache"], moved["value_cache"]
+    q = torch.randn((rows, 4, 64), generator=torch.Generator().manual_seed(8)).to(BF16).to(cuda_device)
+    lists = (3 * torch.arange(600, dtype=torch.int32) + torch.arange(rows, dtype=torch.int32)[:, None, None] % 3).repeat(1, 4, 1)
+    lists = lists.to(cuda_device)
+    out = torch.full_like(q, 7.0)
+    flash_hog.paged_block_attention(q, lists, *kv, **where, out=out)
+    torch.cuda.synchronize()
+    assert (out[new:] == 7).all()
+    for first, last in ((0, 400), (31000, 32500)):
+        own = {**where, "lengths": where["lengths"] - (new - last), "query_offsets": where["query_offsets"] * 0}
+        own["query_offsets"][1] = last - first
+        assert torch.equal(flash_hog.paged_block_attention(q[first:last], lists[first:last], *kv, **own), out[first:last])
+    for t in (0, 31774, 31775, 32499):  # (31775 tokens a slab)
+        cache.lengths = [length - new + t + 1]
+        want = ref.attention(q[t:t + 1].cpu(), cache, [1], lists[t:t + 1].cpu(), 0.125)
+        check(out[t:t + 1], want)
