@@ -254,7 +254,8 @@ hipError_t bookkeeping(const PagesParams& p, hipStream_t stream) {
   const long entries = (long)p.batch * p.width;
   const int chunks = (p.pages + kPageChunk - 1) / kPageChunk;
   hipLaunchKernelGGL(pages_clear_kernel, dim3((p.pages + 255) / 256), dim3(256), 0, stream, p);
-  hipLaunchKernelGGL(pages_mark_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, stream, p);
+  if (entries > 0)  // (a cache without rows may be compacted)
+    hipLaunchKernelGGL(pages_mark_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, stream, p);
   hipLaunchKernelGGL(pages_count_kernel, dim3(chunks), dim3(256), 0, stream, p);
   hipLaunchKernelGGL(pages_scan_kernel, dim3(1), dim3(1024), 0, stream, p);
   hipLaunchKernelGGL(pages_list_kernel, dim3(chunks), dim3(256), 0, stream, p);

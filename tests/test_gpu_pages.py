@@ -230,3 +230,14 @@ def test_versions_and_refusals(extension, cuda_device, monkeypatch):
         with pytest.raises(ValueError, match=match):
             bad()
     assert n.tolist() == [5]
+
+
+def test_compact_many_pages_without_rows(cuda_device):
+    """More pages than one workgroup keeps books of, and no row: zeros."""
+    import flash_hog
+
+    print("[case] many pages without rows", flush=True)
+    x = [torch.ones((40000, 1, 16, 64), dtype=BF16, device=cuda_device) for _ in range(2)]
+    none = torch.empty((0, 3), dtype=torch.int32, device=cuda_device)
+    got = flash_hog.paged_cache_compact(*x, none, none[:, 0], num_pages=33000)
+    assert got[0].shape[0] == 33000 and not raw(got[0]).any() and not raw(got[1]).any() and got[5].shape == (0, 3)
