@@ -809,10 +809,11 @@ int check_pages_workspace(const char* who, const void* workspace, size_t bytes, 
 fhog::PageBytes page_bytes(const void* k, const void* v, const void* ks, const void* vs, const void* means, int head_dim,
                            int page_size, int cache_dtype) {
   const bool quantised = cache_dtype == FHOG_DTYPE_E4M3;
-  const int row = head_dim * (quantised ? 1 : 2);
+  const int token = head_dim * (quantised ? 1 : 2);
+  const long row = (long)token * page_size;
   return fhog::PageBytes{{(char*)k, (char*)v, quantised ? (char*)ks : nullptr, quantised ? (char*)vs : nullptr,
                           (char*)means},
-                         {row * page_size, row * page_size, page_size, page_size, head_dim * 4}, {row, row, 1, 1, 0}};
+                         {row, row, page_size, page_size, head_dim * 4}, {token, token, 1, 1, 0}};
 }
 
 }  // namespace

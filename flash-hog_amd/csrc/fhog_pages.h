@@ -8,7 +8,7 @@ namespace fhog {
 // A cache as bytes: page p of tensor i is rows [p * kv_heads, (p + 1) * kv_heads) of `row` bytes.
 struct PageBytes {
   char* at[5];    // keys, values, their scales, key means; null: none
-  int row[5];     // bytes of one head in a page
+  long row[5];    // bytes of one head in a page (2^31 and more with large pages)
   int token[5];   // bytes of one token of one head (0: not by token)
 };
 

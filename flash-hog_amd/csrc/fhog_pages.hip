@@ -92,8 +92,8 @@ __device__ __forceinline__ int count_pages(const PagesParams& p, const State* st
 // `bytes` bytes (a multiple of 16, both ends aligned to it) by kThreads threads; null source: zeros. kPast: stored past the
 // caches, for copies larger than these (230 MB of e4m3 pages 82 us where they went to them in 106; after other work, with the
 // bookkeeping, 116 and 121).
-template <bool kPast, int kThreads> __device__ __forceinline__ void copy_bytes(char* to, const char* from, int bytes, int thread) {
-  for (int i = 16 * thread; i < bytes; i += 16 * kThreads) {
+template <bool kPast, int kThreads> __device__ __forceinline__ void copy_bytes(char* to, const char* from, long bytes, int thread) {
+  for (long i = 16 * thread; i < bytes; i += 16 * kThreads) {
     const u32x4 x = from ? *reinterpret_cast<const u32x4*>(from + i) : u32x4{0, 0, 0, 0};
     if constexpr (kPast)
       __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(to + i));
@@ -134,7 +134,7 @@ __device__ __forceinline__ void extend_row(const PagesParams& p, const PageBytes
     char* to = cache.at[i] + ((long)target * p.kv_heads + hk) * cache.row[i];
     const char* from = cache.at[i] + ((long)source * p.kv_heads + hk) * cache.row[i];
     if (i < 2)
-      copy_bytes<false, kThreads>(to, from, rows * cache.token[i], thread);
+      copy_bytes<false, kThreads>(to, from, (long)rows * cache.token[i], thread);
     else  // a byte a token
       for (int r = thread; r < rows; r += kThreads) to[r] = from[r];
   }
@@ -289,12 +289,12 @@ __global__ void __launch_bounds__(256) pages_compact_kernel(PagesParams p, PageB
 #pragma unroll
   for (int i = 0; i < 5; ++i) {
     if (!cache.at[i]) continue;
-    const long size = (long)p.kv_heads * cache.row[i];  // of a page
+    const long size = p.kv_heads * cache.row[i];  // of a page
     const long piece = (size / 16 + pieces - 1) / pieces * 16;
     const long at = piece * blockIdx.y, left = size - at;
     if (left > 0)
       copy_bytes<true, 256>(out.at[i] + page * size + at, from < 0 ? nullptr : cache.at[i] + from * size + at,
-                 (int)(left < piece ? left : piece), threadIdx.x);
+                            left < piece ? left : piece, threadIdx.x);
   }
 }
 
@@ -317,7 +317,7 @@ hipError_t launch_pages_compact(const PagesParams& p, const PageBytes& cache, co
   const hipError_t e = bookkeeping(p, stream);
   if (e != hipSuccess) return e;
   // about 16 KB of a tensor a workgroup
-  const long page = (long)p.kv_heads * cache.row[0];
+  const long page = p.kv_heads * cache.row[0];
   const int pieces = (int)(page >= 16384 * 64l ? 64 : page > 16384 ? page / 16384 : 1);
   hipLaunchKernelGGL(pages_compact_kernel, dim3(out_pages, pieces + 1), dim3(256), 0, stream, p, cache, out, out_pages,
                      table_out, pieces);

@@ -241,3 +241,25 @@ def test_compact_many_pages_without_rows(cuda_device):
     none = torch.empty((0, 3), dtype=torch.int32, device=cuda_device)
     got = flash_hog.paged_cache_compact(*x, none, none[:, 0], num_pages=33000)
     assert got[0].shape[0] == 33000 and not raw(got[0]).any() and not raw(got[1]).any() and got[5].shape == (0, 3)
+
+
+def test_pages_of_two_gib(cuda_device):
+    """A head of a page of 2^31 bytes: a fork's copy, and a compaction."""
+    import flash_hog
+
+    print("[case] pages of 2 GiB", flush=True)
+    page = 1 << 22
+    x = [torch.empty((3, 1, page, 256), dtype=BF16, device=cuda_device) for _ in range(2)]
+    columns = torch.arange(256, device=cuda_device)
+    for i, c in enumerate(x):
+        c[2, 0] = ((torch.arange(page, device=cuda_device)[:, None] * (3 + i) + columns) % 251).to(BF16)
+        c[0], c[1] = -1.0, -2.0
+    t, n = i32([[2], [2]], cuda_device), i32([page - 5, page - 5], cuda_device)
+    assert int(flash_hog.paged_cache_extend(*x, t, n, i32([1, 0], cuda_device))) == 1
+    assert t.tolist() == [[0], [2]] and n.tolist() == [page - 4, page - 5]
+    for c in x:
+        assert torch.equal(c[0, 0, :-5], c[2, 0, :-5]) and (c[0, 0, -5:] == -1).all() and (c[1] == -2).all()
+    k, v, _, _, _, table = flash_hog.paged_cache_compact(*x, t[1:].contiguous(), n[1:].contiguous(), num_pages=2)
+    assert table.tolist() == [[0]]
+    for got, c in ((k, x[0]), (v, x[1])):
+        assert torch.equal(got[0], c[2]) and not got[1].any()
