@@ -368,6 +368,14 @@ typedef c10::optional<at::Tensor> MaybeTensor;
 const at::Tensor* get(const MaybeTensor& t) { return t && t->defined() ? &*t : nullptr; }
 const void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
+// Refuses an out whose memory a contiguous tensor that the kernels read shares; `same`: but for all
+// of it, row by row.
+void check_apart(const char* out_name, const at::Tensor& out, const char* name, const at::Tensor& t, bool same) {
+  const char *a = (const char*)out.data_ptr(), *b = (const char*)t.data_ptr();
+  if (a < b + t.nbytes() && b < a + out.nbytes() && !(same && a == b))
+    value_error(std::string(out_name) + " overlaps " + name);
+}
+
 // A paged cache and what finds tokens in it, checked (_hip.py _check_cache).
 struct Cache {
   const at::Tensor *k, *v, *k_scale = nullptr, *v_scale = nullptr;
@@ -424,6 +432,13 @@ struct Cache {
     batch = (int)table_.size(0), width = (int)table_.size(1);
     dtype = quantised ? FHOG_DTYPE_E4M3 : dtype_code(dt);
   }
+  // Refuses an out that shares memory with any of it.
+  void check_apart_from(const char* out_name, const at::Tensor& out) const {
+    for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"key_cache", k}, {"value_cache", v},
+                                  {"key_scale", k_scale}, {"value_scale", v_scale}, {"page_table", &table},
+                                  {"lengths", &lengths}, {"query_offsets", offsets.defined() ? &offsets : nullptr}})
+      if (t) check_apart(out_name, out, name, *t, false);
+  }
   const int* table_ptr() const { return table.data_ptr<int>(); }
   const int* lengths_ptr() const { return lengths.data_ptr<int>(); }
   const int* offsets_ptr() const { return offsets.defined() ? offsets.data_ptr<int>() : nullptr; }
@@ -433,14 +448,6 @@ struct Cache {
 // backward. (Inference tensors, which no graph can save, have no version.)
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-// Refuses an out whose memory a contiguous tensor that the kernels read shares; `same`: but for all
-// of it, row by row.
-void check_apart(const at::Tensor& out, const char* name, const at::Tensor& t, bool same) {
-  const char *a = (const char*)out.data_ptr(), *b = (const char*)t.data_ptr();
-  if (a < b + t.nbytes() && b < a + out.nbytes() && !(same && a == b))
-    value_error(std::string("out overlaps ") + name);
 }
 
 int rows_of(const char* name, const at::Tensor& t) {
@@ -468,9 +475,8 @@ at::Tensor paged_attention_core(const at::Tensor& q_, const at::Tensor& k_cache,
   at::Tensor out = given ? *given : at::empty(q_.sizes(), q_.options());
   const at::Tensor q = contig(q_);
   if (given) {
-    check_apart(out, "query", q, true);
-    check_apart(out, "key_cache", k_cache, false);
-    check_apart(out, "value_cache", v_cache, false);
+    check_apart("out", out, "query", q, true);
+    c.check_apart_from("out", out);
   }
   const int heads = (int)q.size(1);
   c10::DeviceGuard guard(q.device());
@@ -610,7 +616,7 @@ void key_means_core(const at::Tensor& k_cache, const at::Tensor& means, const at
                     const MaybeTensor& offsets, const MaybeTensor& k_scale) {
   const Cache c("key_cache", k_cache, k_cache, k_cache, table, lengths, offsets, k_scale, k_scale, k_cache.scalar_type());
   check_key_means(means, "key_cache", k_cache, {k_cache.size(0), k_cache.size(1), k_cache.size(3)});
-  if (overlap(means, k_cache)) value_error("key_means overlaps key_cache");
+  c.check_apart_from("key_means", means);
   c10::DeviceGuard guard(k_cache.device());
   check_status(api().key_means(current_stream(k_cache), k_cache.data_ptr(), ptr(c.k_scale), means.data_ptr<float>(),
                                c.table_ptr(), c.lengths_ptr(), c.offsets_ptr(), c.batch, c.kv_heads, c.head_dim, c.pages,
@@ -678,10 +684,9 @@ at::Tensor block_attention_core(const at::Tensor& q_, const at::Tensor& chosen_,
   at::Tensor out = given ? *given : at::empty(q_.sizes(), q_.options());
   const at::Tensor q = contig(q_), chosen = contig(chosen_);
   if (given) {
-    check_apart(out, "query", q, false);
-    check_apart(out, "blocks", chosen, false);
-    check_apart(out, "key_cache", k_cache, false);
-    check_apart(out, "value_cache", v_cache, false);
+    check_apart("out", out, "query", q, false);
+    check_apart("out", out, "blocks", chosen, false);
+    c.check_apart_from("out", out);
   }
   const int heads = (int)q.size(1), blocks = (int)chosen.size(2), single = !c.offsets.defined();
   c10::DeviceGuard guard(q.device());

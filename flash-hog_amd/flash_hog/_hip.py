@@ -441,12 +441,23 @@ def _check_cache(first, k_cache, v_cache, page_table, lengths, query_offsets, k_
     return (*k_cache.shape, batch, page_table.shape[1]), page_table, lengths, query_offsets
 
 
+def _overlap(a, b) -> bool:
+    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
+
+
 def _check_apart(out, name, t, same=False):
     """Refuses an out whose memory a contiguous tensor that the kernels read shares; same: but for all
     of it, row by row."""
-    a, b = out.data_ptr(), t.data_ptr()
-    if a < b + t.nbytes and b < a + out.nbytes and not (same and a == b):
+    if _overlap(out, t) and not (same and out.data_ptr() == t.data_ptr()):
         raise ValueError(f"out overlaps {name}")
+
+
+def _check_apart_from(out_name, out, k_cache, v_cache, k_scale, v_scale, page_table, lengths, query_offsets):
+    """Refuses an out that shares memory with a cache or with what finds tokens in it."""
+    for name, t in (("key_cache", k_cache), ("value_cache", v_cache), ("key_scale", k_scale), ("value_scale", v_scale),
+                    ("page_table", page_table), ("lengths", lengths), ("query_offsets", query_offsets)):
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"{out_name} overlaps {name}")
 
 
 def _written(*tensors):
@@ -483,8 +494,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, query_offsets, k_s
     q = q.contiguous()
     if not clear:
         _check_apart(out, "query", q, same=True)
-        _check_apart(out, "key_cache", k_cache)
-        _check_apart(out, "value_cache", v_cache)
+        _check_apart_from("out", out, k_cache, v_cache, k_scale, v_scale, page_table, lengths, query_offsets)
     with _on_device(q.device):
         size = lib().fhog_paged_workspace_bytes(B, T, int(query_offsets is None), N, Nk, Hd, page, width, window, sinks)
         ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
@@ -541,10 +551,6 @@ def paged_cache_read(k_cache, v_cache, page_table, lengths, max_length: int, dty
             _ptr(lengths), _ptr(k), _ptr(v), B, max_length, Nk, Hd, pages, page, width, DTYPE_CODES[dtype],
             CACHE_DTYPE_CODES[k_cache.dtype]))
     return k, v
-
-
-def _overlap(a, b) -> bool:
-    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
 
 
 def paged_cache_extend(k_cache, v_cache, page_table, lengths, new_tokens, new_each: int, parents, k_scale, v_scale):
@@ -645,8 +651,7 @@ def paged_key_means(k_cache, key_means, page_table, lengths, query_offsets, k_sc
     if k_cache.dtype not in CACHE_DTYPE_CODES:
         raise ValueError(f"unsupported dtype {k_cache.dtype}")
     _check_key_means(key_means, ("key_cache", k_cache), (pages, Nk, Hd))
-    if _overlap(key_means, k_cache):
-        raise ValueError("key_means overlaps key_cache")
+    _check_apart_from("key_means", key_means, k_cache, None, k_scale, None, page_table, lengths, query_offsets)
     with _on_device(k_cache.device):
         check(lib().fhog_paged_key_means(
             _stream(k_cache.device), _ptr(k_cache), _ptr(k_scale), _ptr(key_means), _ptr(page_table), _ptr(lengths),
@@ -718,8 +723,7 @@ def paged_block_attention(q, chosen, k_cache, v_cache, page_table, lengths, quer
     if not clear:
         _check_apart(out, "query", q)
         _check_apart(out, "blocks", chosen)
-        _check_apart(out, "key_cache", k_cache)
-        _check_apart(out, "value_cache", v_cache)
+        _check_apart_from("out", out, k_cache, v_cache, k_scale, v_scale, page_table, lengths, query_offsets)
     with _on_device(q.device):
         size = lib().fhog_paged_block_workspace_bytes(B, T, int(query_offsets is None), N, Nk, Hd, page, width,
                                                       chosen.shape[2])
