@@ -80,8 +80,12 @@ def _one_by_one(op):
     cannot share one)."""
 
     def rule(info, in_dims, *args):
-        each = [op(*(a if d is None else a.select(d, i) for a, d in zip(args, in_dims))) for i in range(info.batch_size)]
-        outs = tuple(torch.stack(x) for x in zip(*each))
+        if info.batch_size == 0:  # (a call on zeros for the results' shapes)
+            one = op(*(a if d is None else a.new_zeros(a.shape[:d] + a.shape[d + 1:]) for a, d in zip(args, in_dims)))
+            outs = tuple(x.new_empty((0, *x.shape)) for x in one)
+        else:
+            each = [op(*(a if d is None else a.select(d, i) for a, d in zip(args, in_dims))) for i in range(info.batch_size)]
+            outs = tuple(torch.stack(x) for x in zip(*each))
         return outs, (0,) * len(outs)
 
     op.register_vmap(rule)

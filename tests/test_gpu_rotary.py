@@ -509,3 +509,22 @@ def test_in_place_changes_are_noticed(cuda_device):
         (q, k, positions)[which].add_(1)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             out[0].sum().backward()
+
+
+@pytest.mark.parametrize("eps", [1e-6, None])
+def test_vmap_of_nothing(eps, cuda_device):
+    """No elements: empty results of the elements' shapes, of the derivatives as well."""
+    import flash_hog
+
+    print("[case] vmap of nothing", flush=True)
+    q, k = (torch.zeros((5, 0, 3, n, 64), device=cuda_device) for n in (4, 2))
+    freq = frequencies(64, cuda_device)
+    call = lambda a, b: flash_hog.qk_norm_rotary(a, b, frequencies=freq, eps=eps)
+    out = torch.func.vmap(call, in_dims=1)(q, k)
+    assert out[0].shape == (0, 5, 3, 4, 64) and out[1].shape == (0, 5, 3, 2, 64)
+    squares = lambda x, y: (x ** 2).sum() + (y ** 2).sum()  # (0 + a batch of no numbers is an error of torch's own)
+    loss = lambda a, b: squares(*call(a, b))
+    second = torch.func.grad(lambda a, b: squares(*torch.func.grad(loss, (0, 1))(a, b)), (0, 1))
+    for run in (torch.func.grad(loss, (0, 1)), second):
+        grads = torch.func.vmap(run, in_dims=(1, 1))(q, k)
+        assert grads[0].shape == (0, 5, 3, 4, 64) and grads[1].shape == (0, 5, 3, 2, 64)
