@@ -9,7 +9,11 @@ namespace fhog {
 constexpr int kTileRows = 128;       // rows of a tile
 constexpr int kMostColumns = 8192;   // of the page table (the masks of 64 tokens are in LDS, 64 KB)
 constexpr int kSumBlocks = 256;      // blocks of a list (a join's weights are)
-constexpr int kMostLists = 32768;    // sequences times heads times columns
+// Sequences times heads times columns: each of their lists adds an item and 128 entries to the workspace, 1 KB. A bound on
+// memory, not where the two ways cross: us a token / a block at a time, bf16 H32/8 D128, 16 blocks of 64, one list too many for it:
+// 4 sequences of 512 tokens, 1025 columns, at 8192 keys 555 / 264, at 65536 857 / 505; 32 of 64, 129 columns 587 / 502; 16 of
+// 128, 1024 columns 571 / 406; 64 of 32, 256 columns 640 / 795; 16 of 512 of H8/8, 1025 columns 2049 / 424.
+constexpr int kMostLists = 32768;
 // A tile of a list (the tokens that chose one column of a sequence, for one head): whole tokens, whose entries are
 // the tile's own kTileRows.
 struct BlockItem {
@@ -43,9 +47,11 @@ constexpr IndexRange list_groups(IndexRange of, int way, int ways) {
   return {begin, begin + each < last ? begin + each : last};
 }
 
-// Tokens are taken in slabs whose outputs and masks stay within this (540 MB of outputs in slabs of 256 / 512 / 1024 MB: 415 / 429 /
-// 394 us; each slab has five launches, and ends with CUs idle). Where they would not stay in the cache behind the L2s, they
-// are stored past it: tiles / sum of 540 MB 189 / 105 us in it, 134 / 107 past it; of 207 MB 60 / 51 and 59 / 59.
+// Tokens are taken in slabs whose outputs and masks stay within this: each slab has five launches, and ends with CUs idle
+// (540 MB of outputs in slabs of 256 / 512 / 1024 MB: 415 / 429 / 394 us; in slabs of 256 / 512 / 1024 / 2048 MB: 4096 tokens of
+// H32/8 D128, 1.1 GB, 600 / 499 / 475 / 458, 16384 tokens, 4.4 GB, 2439 / 1968 / 1893 / 1911). Where the outputs would not stay
+// in the cache behind the L2s, they are stored past it: tiles / sum of 540 MB 189 / 105 us in it, 134 / 107 past it; of
+// 207 MB 60 / 51 and 59 / 59.
 constexpr long kPartBytes = 1l << 30, kCacheBytes = 256l << 20;
 // Outputs, and masks with the counts before them, of 64 tokens.
 inline long block_group_bytes(int heads, int kv_heads, int head_dim, int pages_per_seq, int blocks) {
@@ -58,7 +64,8 @@ struct BlockChunkPlan {
 };
 inline BlockChunkPlan block_chunk_plan(int batch, int total, int heads, int kv_heads, int head_dim, int pages_per_seq, int blocks) {
   BlockChunkPlan p;
-  const long fit = kPartBytes / block_group_bytes(heads, kv_heads, head_dim, pages_per_seq, blocks) * 64;  // (64 at least: block_chunk_rule)
+  // (64 at least: block_chunk_rule)
+  const long fit = kPartBytes / block_group_bytes(heads, kv_heads, head_dim, pages_per_seq, blocks) * 64;
   p.slab = (int)(fit < total ? fit : total);
   p.lists = (long)batch * kv_heads * pages_per_seq;
   p.groups = (long)kv_heads * ((p.slab + 63) / 64);

@@ -1,9 +1,11 @@
 // Which blocks of a paged cache a new token attends to (fhog_blocks.h).
 //
 // A full page has the mean of its keys, m_j = sum over its rows / page_size, summed in 64 bits and rounded to
-// fp32 once: sums of 2-byte values are exact there, so a mean does not depend on any order. For a
-// token and key/value head, s_j = <sum over its group's queries, m_j> in 64 bits, since a choice has no
-// tolerance: fp32 would choose otherwise wherever two scores are within its rounding. A token at
+// fp32 once. The sum is exact for fp16 and wherever the values lie within 2^40 or so of each other; beyond that it is a fixed
+// order of the rows that makes a mean the same at every call. For a token and key/value head,
+// s_j = <sum over its group's queries, m_j> in 64 bits, since a choice has no tolerance: fp32 would choose otherwise
+// wherever two scores are within its rounding. The three kernels below add the products in orders of their own, so scores
+// within a rounding of 64 bits may be ranked differently by another of them; equal means have equal scores in each. A token at
 // position p of pages 0 to p / page_size takes the first `first` and the last `last` of them, and of those
 // between the ones with the largest scores, ties to the lowest index; NaN is below every number.
 //

@@ -52,6 +52,9 @@ constexpr int kFusedColumns = 1024;
 // 30 / 14 / 14, 16 sequences of 4 14 / 14 / 14, 64 of 2 24 / 25 / 20, 256 of 1 52 / 47 / 35, 64 of 4 25 / 42 / 35, 64 of 8
 // 27 / 75 / 66; 1000 columns: 41 / 23 / 20, 80 / 35 / 40, 43 / 37 / 43, 86 / 69 / 74; 1000 of D256, 2 heads, where a token's
 // workgroup would wait for 1 MB by itself: 63 / 73 / 19, 102 / 76 / 28, 66 / 81 / 39, 67 / 104 / 59.
+// Wider tables have no kernel of their own, scores go through memory and, in up to nine passes, back: with 1026 / 1027 / 2048 / 8192
+// columns 2048 tokens of 8 heads of 128 take 175 / 208 / 389 / 1675 us, 16 single tokens 18 / 25 / 37 / 164, one of 4 heads of 64
+// 12 / 13 / 18 / 52.
 inline SelectPlan select_plan(int batch, int total, bool single, int kv_heads, int head_dim, int pages_per_seq, int first, int last) {
   SelectPlan p;
   p.slots = total / 16 + batch;

@@ -5,7 +5,8 @@
 // it (as bits), whose rows then fill whole matrix tiles against that one page, read once for 128 of them. Each
 // row leaves an unnormalised fp32 output with its maximum and sum for each of its blocks, in the place that its
 // list gives it, and a last kernel joins a row's outputs in the order of its list: no atomics on numbers, the
-// same bits at every call.
+// same bits at every call. Scores, statistics and outputs are fp32; a probability enters the second product in T, half a
+// step of rounding a term, as in block_token_kernel.
 //
 // What bounds it: those outputs, written and read once, 8 (head_dim + 2) bytes for each row and block. 2035 tokens in 4
 // sequences, H32/8 D128 bf16, 16 blocks of 64, 540 MB of outputs, us: masks 5, items 6, entries 6, tiles 133, sum 108 (5.0 TB/s).

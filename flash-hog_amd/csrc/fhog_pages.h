@@ -35,7 +35,10 @@ struct PagesParams {
 
 constexpr int kPageChunk = 4096;
 // Up to this many pages, entries and rows one workgroup does the bookkeeping, with the pages' states in LDS: six launches
-// become two.
+// become two. The limits are LDS' (pages), a thread a row (rows), and 128 entries a thread. (us a step of one token a row,
+// page of 16 and one head, one workgroup / launches: 128 rows of 34 columns 10 / 25, 64 of 128 13 / 26, 64 of 256 16 / 26, 16 of
+// 1024 18 / 26, 64 of 512 33 / 27, 256 of 128 32 / 27, 64 of 1024 45 / 27, 256 of 512 76 / 27, 1024 of 128 82 / 28: the two cross at
+// about 25000 entries, and from there to the limit one workgroup is the slower way.)
 constexpr int kFewPages = 32768, kFewEntries = 1 << 17, kFewRows = 1024;
 // And one, if the copies are no more than this at most, a wave a row and head. (us, two launches / one, without / with a copy a
 // row: 1 row of 4 heads of 64, pages of 16 5.0 / 3.9, 4 5.6 / 4.3 and 6.0 / 4.9, 8, 128 KB 5.8 / 4.9 and 6.0 / 6.3, 16 6.2 / 6.5

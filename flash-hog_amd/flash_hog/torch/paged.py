@@ -320,7 +320,8 @@ def paged_block_select(query, key_means, page_table, lengths, query_offsets=None
     are fewer. A token at position p has the pages of columns 0 to p // page_size. It takes the first `first` of
     them and the last `last` (at least its own), and of those between the ones whose mean key has the
     largest product with the sum of the queries of a head's group, `blocks` in all. Products are formed in 64
-    bits; ties go to the lowest column, and NaN (or a page outside the cache) is below every number.
+    bits, in an order that goes with the number of tokens (ones that only a rounding there tells apart may change
+    places); ties go to the lowest column, and NaN (or a page outside the cache) is below every number.
     query (T, N, H) as in paged_attention, key_means as paged_key_means keeps them. Offsets that fall somewhere may
     leave lists of any values."""
     through = _checked("paged_block_select", (page_table, lengths, query_offsets), query, key_means)

@@ -331,10 +331,10 @@ int fhog_paged_key_means(fhog_stream_t stream, const void* k_cache, const void* 
  * chosen (total, kv_heads, blocks) int32: for each new token, at position p, and key/value head the columns to attend
  * to, rising, -1 behind them. Of columns 0 to p / page_size: the first `first` (>= 0), the last `last` (>= 1, so that
  * a page that is not full yet is never chosen by its mean), and of the others those whose mean has the largest
- * product with the sum of the queries q (total, heads, head_dim) of the head's group, formed in 64 bits, ties to
- * the lowest column, NaN (also: a page outside the cache) last; `blocks` (>= first + last) in all, or all there
- * are. Tokens of no sequence, before position 0 or beyond the table: -1 throughout. Offsets that fall somewhere may
- * leave lists of any values.
+ * product with the sum of the queries q (total, heads, head_dim) of the head's group, formed in 64 bits (in an order
+ * that goes with the number of tokens, so products apart by a rounding there may change places), ties to the lowest
+ * column, NaN (also: a page outside the cache) last; `blocks` (>= first + last) in all, or all there are. Tokens of no
+ * sequence, before position 0 or beyond the table: -1 throughout. Offsets that fall somewhere may leave lists of any values.
  */
 size_t fhog_paged_block_select_workspace_bytes(int batch, int total, int single, int kv_heads, int head_dim,
                                                int pages_per_seq, int first, int last);
@@ -389,8 +389,8 @@ typedef struct fhog_rotary {
   const int* query_offsets;
 } fhog_rotary;
 
-/* Bytes of workspace of the two backwards on the current device (0 without weights or norms). Calls
- * that may overlap need one each. */
+/* Bytes of workspace of the two backwards on the current device (0 without norms; without weights it may be
+ * null). Calls that may overlap need one each. */
 size_t fhog_qk_norm_rotary_workspace_bytes(const fhog_rotary* shape);
 
 /* q_out, k_out (contiguous, as all tensors but q and k) from q, k and the weights (head_dim) of their
